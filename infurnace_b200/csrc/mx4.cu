@@ -1,0 +1,524 @@
+// Microscaled 4-bit floating point: matrices whose elements are 4 bits (sign, two bits of exponent, one of mantissa:
+// 0, 0.5, 1, 1.5, 2, 3, 4, 6) with one power of two for each block of 32 elements of a row, and products of two such matrices.
+//
+// The definition.  For a block with the largest magnitude a, the scale is 2^(s - 127), s = max(0, floor(log2 a) + 125), so that
+// a lies in [4, 8) units; an element is x / scale rounded to the nearest level, ties to the even code, what exceeds 6 becoming
+// 6.  A block with an infinity or a NaN has s = 255, which stands for NaN.  Division by a power of two is exact, so every
+// implementation gives the same bits.
+//
+// Layout.  Codes: [rows][k / 2] bytes, element 2 i in the low half.  Scales: in the order in which the tensor core wants them in
+// tensor memory: tiles of 128 rows x 128 of k, 512 bytes each, tile (rt, kt) at (rt * ceil(k / 128) + kt) * 512, the byte of
+// (row, block) at (row % 32) * 16 + (row % 128 / 32) * 4 + block % 4; rows are padded to 256, so that a copy of two tiles of
+// rows stays inside.  A gated matrix (gate rows [0, O), up rows [O, 2 O)) keeps row i of the gate in row 2 i and row i of the
+// up half in row 2 i + 1: the two numbers of an output then lie in neighbouring lanes of the accumulator.
+#include <cuda.h>
+#include "common.cuh"
+
+typedef __nv_bfloat16 bf16;
+constexpr int MX_BLOCK = 32;
+
+// ---------------------------------------------------------------------------------------------
+// Rounding of rows to 4 bits, and the values that the bits stand for
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t mx_scale_byte(float amax_or_bits_max) {
+  const uint32_t f = __float_as_uint(amax_or_bits_max) >> 23;          // the exponent field of a number without its sign
+  return f == 255u ? 255u : (f >= 2u ? f - 2u : 0u);
+}
+__device__ __forceinline__ float mx_inverse_scale(uint32_t s) {        // 2^(127 - s), s = 0 .. 252 (255: any)
+  return __uint_as_float((254u - (s > 253u ? 253u : s)) << 23);
+}
+// Eight scaled numbers to eight codes (the first in the lowest four bits).
+__device__ __forceinline__ uint32_t mx_codes8(const float (&v)[8], float inv) {
+  uint32_t r;
+  asm("{\n .reg .b8 b0, b1, b2, b3;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n"
+      " mov.b32 %0, {b0, b1, b2, b3};\n}\n"
+      : "=r"(r) : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
+        "f"(v[6] * inv), "f"(v[7] * inv));
+  return r;
+}
+__device__ __forceinline__ void mx_load8(const float* p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void mx_load8(const bf16* p, float (&v)[8]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint32_t mx_amax_bits(const float (&v)[8]) {
+  // magnitudes compared as integers: a NaN is larger than infinity, and neither is lost
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+__host__ __device__ __forceinline__ size_t mx_scale_at(int row, int block, int k_tiles) {
+  return ((size_t)(row >> 7) * k_tiles + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+}
+
+// Four neighbouring lanes have a block: eight elements (16 or 32 bytes of input, 4 of output) each.  16 lanes have the four
+// blocks whose scales lie in one 32-bit word.  A grid row walks over rows; the columns of a row are spread over the grid's x.
+template <typename T>
+__global__ void __launch_bounds__(256)
+mx4_quantize_kernel(const T* x, long long row_stride, uint8_t* codes, uint8_t* scales, int rows, int k, int gated_rows) {
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  const int k_tiles = (k + 127) / 128;
+  const int e = (blockIdx.x * 256 + threadIdx.x) * 8;                  // of the row's elements, padded to 128
+  const uint32_t lanes = __ballot_sync(0xffffffffu, e < k_tiles * 128);
+  if (e >= k_tiles * 128) return;                                      // 16 lanes leave together
+  const int row = blockIdx.y;                                          // of the result
+  const int from = gated_rows ? (row & 1) * gated_rows + (row >> 1) : row;
+  const bool in = e < k;
+  float v[8] = {};
+  if (in) mx_load8(x + (size_t)from * row_stride + e, v);
+  uint32_t m = mx_amax_bits(v);
+  m = max(m, __shfl_xor_sync(lanes, m, 1));
+  m = max(m, __shfl_xor_sync(lanes, m, 2));
+  const uint32_t s = mx_scale_byte(__uint_as_float(m));
+  if (in) *reinterpret_cast<uint32_t*>(codes + (size_t)row * (k / 2) + e / 2) = mx_codes8(v, mx_inverse_scale(s));
+  uint32_t word = (in ? s : 0u) << ((threadIdx.x & 12) * 2);
+  word |= __shfl_xor_sync(lanes, word, 4);
+  word |= __shfl_xor_sync(lanes, word, 8);
+  if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(row, e / MX_BLOCK, k_tiles)) = word;
+}
+
+template <typename T> __device__ __forceinline__ void mx_store8(T* p, const float (&v)[8]);
+template <> __device__ __forceinline__ void mx_store8<float>(float* p, const float (&v)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <> __device__ __forceinline__ void mx_store8<bf16>(bf16* p, const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ float mx_value(uint32_t code) {             // of one element, in units of its block's scale
+  const uint32_t e = (code >> 1) & 3u, m = code & 1u;
+  const float mag = e ? __uint_as_float(((126u + e) << 23) | (m << 22)) : 0.5f * (float)m;
+  return code & 8u ? -mag : mag;
+}
+__device__ __forceinline__ float mx_scale(uint32_t s) {                // 2^(s - 127); s = 0 is a subnormal number; 255: NaN
+  return __uint_as_float(s == 255u ? 0x7fffffffu : s ? s << 23 : 0x00400000u);
+}
+template <typename T>
+__global__ void __launch_bounds__(256)
+mx4_values_kernel(const uint8_t* codes, const uint8_t* scales, T* out, int rows, int k, int gated_rows) {
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  const int e = (blockIdx.x * 256 + threadIdx.x) * 8;
+  if (e >= k) return;
+  const int row = blockIdx.y;
+  const int to = gated_rows ? (row & 1) * gated_rows + (row >> 1) : row;
+  const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + (size_t)row * (k / 2) + e / 2);
+  const float f = mx_scale(scales[mx_scale_at(row, e / MX_BLOCK, (k + 127) / 128)]);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = mx_value((c >> (4 * i)) & 15u) * f;
+  mx_store8<T>(out + (size_t)to * k + e, v);
+}
+
+static int mx_sizes(int rows, int k, int gated) {
+  if (rows < 1 || k < MX_BLOCK || k % MX_BLOCK || (gated && (rows & 1))) return IFB_ERR_SIZE;
+  return IFB_OK;
+}
+
+IFB_EXPORT int ifb_mx4_quantize(const void* x, int dtype, long long row_stride, void* codes, void* scales, int rows, int k, int gated,
+                                void* stream) {
+  int bad = mx_sizes(rows, k, gated);
+  if (bad) return bad;
+  const int esize = dtype == IFB_F32 ? 4 : 2;
+  if (dtype != IFB_F32 && dtype != IFB_BF16) return IFB_ERR_DTYPE;
+  if ((((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)scales) | (uintptr_t)(row_stride * esize)) & 15) return IFB_ERR_ALIGN;
+  const int threads = (k + 127) / 128 * 16;
+  for (int r0 = 0; r0 < rows; r0 += 65536 - 256) {      // a grid has at most 65,535 rows; whole tiles of rows, whole pairs
+    const int n = min(rows - r0, 65536 - 256);
+    // (a gated matrix has its rows from two places, so one launch has to hold it)
+    if (gated && n != rows) return IFB_ERR_SIZE;
+    const dim3 grid((threads + 255) / 256, n);
+    uint8_t* c = (uint8_t*)codes + (size_t)r0 * (k / 2);
+    uint8_t* s = (uint8_t*)scales + (size_t)(r0 / 128) * ((k + 127) / 128) * 512;
+    int e;
+    if (dtype == IFB_F32)
+      e = ifb_launch(mx4_quantize_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, (const float*)x + (size_t)r0 * row_stride,
+                     row_stride, c, s, n, k, gated ? rows / 2 : 0);
+    else
+      e = ifb_launch(mx4_quantize_kernel<bf16>, grid, dim3(256), 0, (cudaStream_t)stream, (const bf16*)x + (size_t)r0 * row_stride,
+                     row_stride, c, s, n, k, gated ? rows / 2 : 0);
+    if (e) return e;
+  }
+  return IFB_OK;
+}
+
+IFB_EXPORT int ifb_mx4_values(const void* codes, const void* scales, void* out, int dtype, int rows, int k, int gated, void* stream) {
+  int bad = mx_sizes(rows, k, gated);
+  if (bad) return bad;
+  if (dtype != IFB_F32 && dtype != IFB_BF16) return IFB_ERR_DTYPE;
+  if ((((uintptr_t)out) | ((uintptr_t)codes) | ((uintptr_t)scales)) & 15) return IFB_ERR_ALIGN;
+  for (int r0 = 0; r0 < rows; r0 += 65536 - 256) {
+    const int n = min(rows - r0, 65536 - 256);
+    if (gated && n != rows) return IFB_ERR_SIZE;
+    const dim3 grid((k / 8 + 255) / 256, n);
+    const uint8_t* c = (const uint8_t*)codes + (size_t)r0 * (k / 2);
+    const uint8_t* s = (const uint8_t*)scales + (size_t)(r0 / 128) * ((k + 127) / 128) * 512;
+    int e;
+    if (dtype == IFB_F32)
+      e = ifb_launch(mx4_values_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, c, s, (float*)out + (size_t)r0 * k, n, k,
+                     gated ? rows / 2 : 0);
+    else
+      e = ifb_launch(mx4_values_kernel<bf16>, grid, dim3(256), 0, (cudaStream_t)stream, c, s, (bf16*)out + (size_t)r0 * k, n, k,
+                     gated ? rows / 2 : 0);
+    if (e) return e;
+  }
+  return IFB_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// The product: out[n, o] = sum_k x[n, k] w[o, k] of two microscaled matrices, by tcgen05.mma of kind mxf4, which multiplies
+// 4-bit elements, applies both blocks' scales and adds in float32.
+//
+// The features are the 128 rows of the accumulator (its lanes), the tokens its columns, so that a step of few tokens wastes
+// nothing of the instruction but its width, and one kernel serves one token and a prompt.  A CTA owns 128 rows of w by NT
+// tokens.  Per 256 of k, a stage: 128 bytes of every row (one swizzle row) of both operands by TMA, and their scale tiles (512
+// bytes per 128 x 128) by bulk copies; the issuing thread copies the scales on to tensor memory (tcgen05.cp, 32 lanes x 16
+// bytes, repeated for the four quarters of the lanes) into columns that belong to the stage, then issues four products of k =
+// 64.  Rows and k beyond the matrices are zeros.
+//   warp 0: producer; warp 1: copies scales and issues products; warps 2 ..: epilogue, a quarter of the lanes each (warp % 4).
+// SPLITS: where tiles are few, the k range of a tile is shared by a cluster of CTAs along z, which add their accumulators
+// through distributed shared memory in the order of their ranks.
+// What does not depend on the kernel before this one, the matrix, is requested before the wait for it.
+// Waits are bounded: after a limit a thread records a code in `*err`, raises the CTA's abort flag, and all fall through to the
+// end, where the tensor memory is given back.
+// ---------------------------------------------------------------------------------------------
+constexpr int MX_KSTAGE = 256;
+constexpr int MX_A_BYTES = 128 * 128;
+constexpr uint32_t MX_SPIN_LIMIT = 1u << 22;
+
+__device__ __forceinline__ uint32_t mx_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mx_mbar_init(uint64_t* bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(mx_smem(bar)), "r"(count));
+}
+__device__ __forceinline__ void mx_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(mx_smem(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mx_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  unsigned long long t0 = 0;
+  for (uint32_t i = 0; i < MX_SPIN_LIMIT; ++i) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(mx_smem(bar)), "r"(parity) : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    if (ifb_wait_expired(i, t0)) break;
+  }
+  *abort_flag = 1;
+  atomicExch(err, code);
+  return false;
+}
+__device__ __forceinline__ void mx_tma_2d(uint32_t smem, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
+               ::"r"(smem), "l"(map), "r"(mx_smem(bar)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void mx_bulk(uint32_t smem, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+               ::"r"(smem), "l"(src), "r"(bytes), "r"(mx_smem(bar)) : "memory");
+}
+__device__ __forceinline__ bool mx_elect() {
+  uint32_t pred;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(pred));
+  return pred != 0;
+}
+// K-major rows of 128 bytes in the 128-byte swizzle, groups of 8 rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t mx_desc(uint32_t smem) {
+  return (uint64_t)((smem >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// 32 rows of 16 bytes one after the other: groups of 8 rows 128 bytes apart, no swizzle.
+__device__ __forceinline__ uint64_t mx_scale_desc(uint32_t smem) {
+  return (uint64_t)((smem >> 4) & 0x3FFF) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void mx_copy_scales(uint32_t tmem, uint32_t smem) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(mx_scale_desc(smem)) : "memory");
+}
+__device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mx_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(mx_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void mx_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+
+template <int NT_, int STAGES_> struct MxCfg {
+  static constexpr int NT = NT_, STAGES = STAGES_;
+  static constexpr int RT = NT > 128 ? 2 : 1;                          // scale tiles of 128 tokens
+  static constexpr int B_BYTES = NT * 128;
+  static constexpr int SA = MX_A_BYTES + B_BYTES, SB = SA + 1024, STAGE_BYTES = SB + RT * 1024;      // where the scales lie
+  static constexpr int S_COLS = 8 + 8 * RT;                            // columns of a stage's scales
+  static constexpr int COLS = NT + STAGES * S_COLS;
+  static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static constexpr int EPI_WARPS = NT >= 128 ? 8 : 4, THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;
+  static_assert(COLS <= 512 && STAGE_BYTES % 1024 == 0, "tensor memory and alignment");
+  static_assert(STAGES * STAGE_BYTES >= NT * 128 * 4 || NT > 128, "the float32 tile of a shared k range lies in the stages");
+  // 4-bit elements of both operands (format 1), scales as powers of two, M = 128, N = NT, k = 64, both K-major
+  static constexpr uint32_t IDESC = (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | (1u << 23) | ((uint32_t)(128 >> 4) << 24);
+};
+
+struct MxProduct {
+  const uint8_t* x_scales;
+  const uint8_t* w_scales;
+  void* out;
+  int rows, k, w_rows, out_features, unary, per_split;                 // per_split: stages of a CTA
+};
+
+// y: the activation of a pair's gate times its up; else the unary function.
+__device__ __forceinline__ float mx_gate(float g, float u, int unary) { return ifb_gate_act(g, unary) * u; }
+
+template <typename C, bool GATED, typename TO>
+__global__ void __launch_bounds__(C::THREADS)
+mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, MxProduct p, int* err) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ uint64_t full[C::STAGES], empty[C::STAGES], ready;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const uint32_t base = (mx_smem(raw) + 1023u) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int o0 = blockIdx.x * 128, n0 = blockIdx.y * C::NT;
+  const int k_tiles = (p.k + 127) / 128, stages = (p.k + MX_KSTAGE - 1) / MX_KSTAGE;
+  const int s0 = blockIdx.z * p.per_split, s1 = min(stages, s0 + p.per_split);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) { mx_mbar_init(&full[i], 1); mx_mbar_init(&empty[i], 1); }
+    mx_mbar_init(&ready, 1);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(mx_smem(&tmem_slot)), "r"(C::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const uint32_t tmem = *(volatile uint32_t*)&tmem_slot;
+
+  if (warp == 0) {
+    // the matrix of the first stages before the wait, the tokens after it
+    auto bytes = [&](int s) { return (uint32_t)min(2, k_tiles - 2 * s) * 512u; };      // of one tile of rows' scales
+    auto load_w = [&](int s, int i) {
+      const uint32_t at = base + i * C::STAGE_BYTES;
+      mx_expect_tx(&full[i], MX_A_BYTES + C::B_BYTES + bytes(s) * (1 + C::RT));
+      mx_tma_2d(at, &w_map, &full[i], s * 64, o0);
+      mx_bulk(at + C::SA, p.w_scales + ((size_t)(o0 >> 7) * k_tiles + 2 * s) * 512, bytes(s), &full[i]);
+    };
+    auto load_x = [&](int s, int i) {
+      const uint32_t at = base + i * C::STAGE_BYTES;
+      mx_tma_2d(at + MX_A_BYTES, &x_map, &full[i], s * 64, n0);
+      for (int t = 0; t < C::RT; ++t)
+        mx_bulk(at + C::SB + t * 1024, p.x_scales + ((size_t)((n0 >> 7) + t) * k_tiles + 2 * s) * 512, bytes(s), &full[i]);
+    };
+    const int ahead = min(C::STAGES, s1 - s0);
+    if (mx_elect())
+      for (int i = 0; i < ahead; ++i) load_w(s0 + i, i);
+    __syncwarp();
+    ifb_pdl_wait();
+    ifb_pdl_trigger();
+    if (mx_elect())
+      for (int i = 0; i < ahead; ++i) load_x(s0 + i, i);
+    __syncwarp();
+    for (int s = s0 + ahead; s < s1; ++s) {
+      const int j = s - s0, i = j % C::STAGES;
+      if (!mx_wait(&empty[i], ((j / C::STAGES) & 1) ^ 1, abort_flag, err, 701)) break;
+      if (mx_elect()) { load_w(s, i); load_x(s, i); }
+      __syncwarp();
+    }
+  } else {
+    ifb_pdl_wait();
+    if (warp == 1) {
+      for (int s = s0; s < s1; ++s) {
+        const int j = s - s0, i = j % C::STAGES;
+        if (!mx_wait(&full[i], (j / C::STAGES) & 1, abort_flag, err, 702)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        if (mx_elect()) {
+          const uint32_t at = base + i * C::STAGE_BYTES, sc = tmem + C::NT + i * C::S_COLS;
+          const int tiles = min(2, k_tiles - 2 * s), products = min(4, (p.k - s * MX_KSTAGE + 63) / 64);
+          for (int t = 0; t < tiles; ++t) {
+            mx_copy_scales(sc + t * 4, at + C::SA + t * 512);
+#pragma unroll
+            for (int r = 0; r < C::RT; ++r) mx_copy_scales(sc + 8 + t * 4 * C::RT + r * 4, at + C::SB + r * 1024 + t * 512);
+          }
+          const uint64_t a = mx_desc(at), b = mx_desc(at + MX_A_BYTES);
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            if (m < products) {
+              const uint32_t id = (uint32_t)(m & 1) * 2;               // which two of the four scales of a word
+              mx_mma(tmem, a + m * 2, b + m * 2, C::IDESC | (id << 4) | (id << 29), sc + (m >> 1) * 4, sc + 8 + (m >> 1) * 4 * C::RT,
+                     (j | m) != 0);
+            }
+          mx_commit(&empty[i]);
+        }
+        __syncwarp();
+      }
+      if (mx_elect()) mx_commit(&ready);
+      __syncwarp();
+    }
+  }
+  const bool ok = mx_wait(&ready, 0, abort_flag, err, 703);
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const int splits = gridDim.z;
+  TO* out = (TO*)p.out;
+  if (warp >= 2 && ok && splits == 1) {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    constexpr int PER = C::NT / (C::EPI_WARPS / 4);                    // tokens of a warp
+    const int row = o0 + quarter * 32 + lane;                          // of w
+    for (int c = half * PER; c < (half + 1) * PER; c += 16) {
+      if (n0 + c >= p.rows) break;                                     // warp-uniform
+      uint32_t v[16];
+      mx_tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
+      if (GATED) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[j] : v[j + 1], 1);
+          const int token = n0 + c + j + (lane & 1);
+          const float y = lane & 1 ? mx_gate(__uint_as_float(other), __uint_as_float(v[j + 1]), p.unary)
+                                   : mx_gate(__uint_as_float(v[j]), __uint_as_float(other), p.unary);
+          if (row < p.w_rows && token < p.rows) out[(size_t)token * p.out_features + (row >> 1)] = from_f32<TO>(y);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (row < p.w_rows && n0 + c + j < p.rows)
+            out[(size_t)(n0 + c + j) * p.out_features + row] = from_f32<TO>(ifb_unary(__uint_as_float(v[j]), p.unary));
+      }
+    }
+  }
+  if (splits > 1) {
+    float* mine = reinterpret_cast<float*>(raw + (base - mx_smem(raw)));      // [tokens][128]
+    if (warp >= 2 && ok) {
+      const int quarter = warp & 3, half = (warp - 2) >> 2;
+      constexpr int PER = C::NT / (C::EPI_WARPS / 4);
+      for (int c = half * PER; c < (half + 1) * PER; c += 16) {
+        uint32_t v[16];
+        mx_tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mine[(c + j) * 128 + quarter * 32 + lane] = __uint_as_float(v[j]);
+      }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    const int tokens = min(C::NT, p.rows - n0);
+    // two rows of w (one output, if gated) per thread and turn
+    for (int i = blockIdx.z * C::THREADS + threadIdx.x; i < tokens * 64; i += splits * C::THREADS) {
+      const int token = i >> 6, pair = (i & 63) * 2, row = o0 + pair;
+      float a = 0.f, b = 0.f;
+      for (int r = 0; r < splits; ++r) {
+        uint32_t remote;
+        float2 f;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(mx_smem(mine + token * 128 + pair)), "r"(r));
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(f.x), "=f"(f.y) : "r"(remote) : "memory");
+        a += f.x;
+        b += f.y;
+      }
+      TO* to = out + (size_t)(n0 + token) * p.out_features;
+      if (GATED) {
+        if (row < p.w_rows) to[row >> 1] = from_f32<TO>(mx_gate(a, b, p.unary));
+      } else {
+        if (row < p.w_rows) to[row] = from_f32<TO>(ifb_unary(a, p.unary));
+        if (row + 1 < p.w_rows) to[row + 1] = from_f32<TO>(ifb_unary(b, p.unary));
+      }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  }
+  if (!ok) for (int i = 0; i < 2000; ++i) __nanosleep(1000);           // copies in flight land
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(C::TMEM) : "memory");
+  }
+}
+
+template <typename C, bool GATED, typename TO>
+static int mx_launch(const CUtensorMap& xm, const CUtensorMap& wm, const MxProduct& p, int splits, int* err, cudaStream_t stream) {
+  auto kernel = mx4_linear_kernel<C, GATED, TO>;
+  IFB_ALLOW_SMEM(kernel, C::SMEM);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.w_rows + 127) / 128, (p.rows + C::NT - 1) / C::NT, splits);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = splits;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ifb_pdl_enabled() ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, xm, wm, p, err);
+  if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
+  return IFB_OK;
+}
+template <typename C>
+static int mx_launch_any(const CUtensorMap& xm, const CUtensorMap& wm, const MxProduct& p, bool gated, int dtype, int splits, int* err,
+                         cudaStream_t stream) {
+  if (gated) return dtype == IFB_F32 ? mx_launch<C, true, float>(xm, wm, p, splits, err, stream) : mx_launch<C, true, bf16>(xm, wm, p, splits, err, stream);
+  return dtype == IFB_F32 ? mx_launch<C, false, float>(xm, wm, p, splits, err, stream) : mx_launch<C, false, bf16>(xm, wm, p, splits, err, stream);
+}
+
+// x: [rows][k], w: [w_rows][k] (twice the out features if the epilogue is gated), both microscaled.  epilogue: as in the other products.
+IFB_EXPORT int ifb_mx4_linear(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int out_dtype,
+                              int rows, int k, int w_rows, int epilogue, void* err, void* stream) {
+  const bool gated = epilogue & 1;
+  const int unary = epilogue >> 4;
+  int bad = mx_sizes(rows, k, 0);
+  if (bad) return bad;
+  if (w_rows < 1 || (gated && (w_rows & 1))) return IFB_ERR_SIZE;
+  if ((epilogue & 14) || unary > IFB_UNARY_LAST) return IFB_ERR_ARG;
+  if (out_dtype != IFB_F32 && out_dtype != IFB_BF16) return IFB_ERR_DTYPE;
+  if ((((uintptr_t)x_codes) | ((uintptr_t)x_scales) | ((uintptr_t)w_codes) | ((uintptr_t)w_scales)) & 15) return IFB_ERR_ALIGN;
+  const int nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  const int stages = (k + MX_KSTAGE - 1) / MX_KSTAGE, tiles = (w_rows + 127) / 128;
+  // the k range is shared where tiles leave SMs idle
+  int splits = 1;
+  if (nt <= 128) while (splits < 8 && splits * 2 <= stages && tiles * splits * 2 <= ifb_sm_count() + 8) splits *= 2;
+  MxProduct p = {(const uint8_t*)x_scales, (const uint8_t*)w_scales, out, rows, k, w_rows, gated ? w_rows / 2 : w_rows, unary,
+                 (stages + splits - 1) / splits};
+  splits = (stages + p.per_split - 1) / p.per_split;                   // every CTA has a stage
+  // the maps see pairs of bytes as one number of 16 bits: only widths and strides in bytes count
+  const unsigned long long xd[2] = {(unsigned long long)k / 4, (unsigned long long)rows}, xs[1] = {(unsigned long long)k / 2};
+  const unsigned long long wd[2] = {(unsigned long long)k / 4, (unsigned long long)w_rows}, ws[1] = {(unsigned long long)k / 2};
+  const unsigned xb[2] = {64, (unsigned)nt}, wb[2] = {64, 128};
+  CUtensorMap xm, wm;
+  bad = ifb_tensor_map_bf16(&xm, x_codes, 2, xd, xs, xb);
+  if (!bad) bad = ifb_tensor_map_bf16(&wm, w_codes, 2, wd, ws, wb);
+  if (bad) return bad;
+  cudaStream_t st = (cudaStream_t)stream;
+  int* e = (int*)err;
+  switch (nt) {
+    case 16: return mx_launch_any<MxCfg<16, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
+    case 32: return mx_launch_any<MxCfg<32, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
+    case 64: return mx_launch_any<MxCfg<64, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
+    case 128: return mx_launch_any<MxCfg<128, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
+    default: return mx_launch_any<MxCfg<256, 4>>(xm, wm, p, gated, out_dtype, splits, e, st);
+  }
+}

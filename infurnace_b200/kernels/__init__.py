@@ -3,6 +3,7 @@ it raises :class:`~infurnace_b200.errors.KernelError` when there is no CUDA devi
 from __future__ import annotations
 
 from .build import load_library, register_library  # noqa: F401  (for parts that bring kernels of their own)
+from .low_bits import Kv8Pages, Mx4Matrix  # noqa: F401
 
 _kernels = None
 

@@ -45,6 +45,8 @@ LIBRARIES: Dict[str, tuple] = {
     # decoders with latent attention: norms in groups, the short causal convolution, the average over depth, the
     # preparation of queries and latents, attention over cached latents (plain and on tensor cores), the output gate
     "latent": (["latent.cu", "attention_latent.cu", "attention_latent_mma.cu"], []),
+    # matrices in microscaled 4-bit floating point and their products
+    "mx4": (["mx4.cu"], []),
     # compiled once per head size: defines={"HEAD_DIM": d}
     "attention_mma": (["attention_mma.cu"], []),
 }
@@ -207,7 +209,7 @@ def build_all(progress=None) -> List[str]:
     """Compile every library (used by the build check; needs no GPU)."""
     from concurrent.futures import ThreadPoolExecutor
     jobs = [("core", None), ("linear_tcgen05", None), ("linear_skinny_static", None), ("attention_tc", None),
-            ("mixers", None), ("hybrid", None), ("latent", None)] + DEFAULT_VARIANTS
+            ("mixers", None), ("hybrid", None), ("latent", None), ("mx4", None)] + DEFAULT_VARIANTS
     with ThreadPoolExecutor(max_workers=4) as pool:
         built = list(pool.map(lambda j: compile_library(j[0], j[1], progress), jobs))
     # objects of older sources are never loaded (their names carry another hash); take them out of the folder

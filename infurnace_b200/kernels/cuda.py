@@ -15,6 +15,7 @@ import torch
 
 from ..errors import KernelError
 from .build import load_library
+from .low_bits import LowBitKernels
 
 F32, BF16 = 0, 1
 # the `epilogue` argument of the products: 0 plain, 1 silu_gate (w holds gate rows, then up rows), 16 * u: plain with the
@@ -61,7 +62,7 @@ def _dense(t, name, dtype=None):
     return t
 
 
-class CudaKernels:
+class CudaKernels(LowBitKernels):
     name = "cuda"
     takes_exact_lens = True        # paged_attention's ``exact_lens``
 
