@@ -1,0 +1,200 @@
+// Keys and values held in 8 bits with a scale for each page, kind (keys or values) and head: the store, and the values that
+// the bits stand for.
+//
+// The definition.  A block is what a page holds of one head's keys or values; f is the exponent field of its largest magnitude
+// as a float32 number, step = 2^(f - 133), a code is floor(x / step), which lies in [-128, 127], and stands for (code + 1/2)
+// step.  Floors nest: floor(floor(x / s) / 2^d) = floor(x / (s 2^d)), so when a token with a larger number joins a page, a
+// shift of the older codes to the right makes them what they would be had all been stored at once, and how a prompt was cut
+// leaves no trace in a page's bits.  (With rounding to nearest in place of floor, the second rounding would.)  f = 0 (all
+// numbers zero or subnormal): the values are 0; f = 255 (an infinity or NaN): they are NaN.
+//
+// Layout: codes int8 [pages][2][heads][page_size][dim], exponents uint8 [pages][2][heads].
+#include "common.cuh"
+
+typedef __nv_bfloat16 bf16;
+
+__device__ __forceinline__ float kv8_step(uint32_t f) {                 // 2^(f - 133), 0, NaN
+  if (f == 0u) return 0.f;
+  if (f == 255u) return __uint_as_float(0x7fffffffu);
+  return f > 6u ? __uint_as_float((f - 6u) << 23) : __uint_as_float(1u << (f + 16u));
+}
+// floor(x / step) of a number whose block has the exponent field f.
+__device__ __forceinline__ int kv8_code(float x, uint32_t f) {
+  if (f == 0u) return x < 0.f ? -1 : 0;
+  if (f == 255u) return 0;
+  // rounding downwards keeps a tiny negative number below zero where the quotient leaves the range of floats
+  float t;
+  if (f > 6u) t = __fmul_rd(x, __uint_as_float((260u - f) << 23));      // 2^(133 - f)
+  else t = __fmul_rd(__fmul_rd(x, __uint_as_float((254u - f) << 23)), 64.f);      // a factor that no float holds
+  return (int)floorf(t);
+}
+__device__ __forceinline__ void kv8_load8(const float* p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void kv8_load8(const bf16* p, float (&v)[8]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// A warp per (run of rows, kind, head).  A run is the adjacent rows whose slots follow one another in one page; its first row's
+// warp has the whole run, the other rows' warps leave.  (A page's rows must be one run: the caller's contract.)  The rows are
+// read twice, for the largest and for the codes; the second time they come from the first level of cache.
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv8_store_kernel(const T* k, const T* v, long long k_row, long long v_row, const int* slots, int8_t* codes, uint8_t* exponents, int rows,
+                 int heads, int page_size, int dim) {
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  const int row0 = blockIdx.x, lane = threadIdx.x & 31, block = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (block >= 2 * heads) return;
+  const int slot = slots[row0];
+  if (slot < 0) return;
+  const int page = slot / page_size, first = slot - page * page_size;
+  if (row0 && first && slots[row0 - 1] == slot - 1) return;
+  int n = 1;                                                            // rows of the run
+  for (int at = 1; at < page_size - first; at += 32) {
+    const int i = at + lane;
+    const bool in = i < page_size - first && row0 + i < rows && slots[row0 + i] == slot + i;
+    const uint32_t miss = ~__ballot_sync(0xffffffffu, in);
+    n = at + (miss ? __ffs(miss) - 1 : 32);
+    if (miss) break;
+  }
+  const int kind = block / heads, head = block - kind * heads;
+  const T* src = (kind ? v : k) + (size_t)row0 * (kind ? v_row : k_row) + (size_t)head * dim;
+  const long long pitch = kind ? v_row : k_row;
+  uint8_t* const exponent = exponents + ((size_t)page * 2 + kind) * heads + head;
+  const uint32_t old = first ? *exponent : 0u;
+  const int pieces = dim / 8, total = n * pieces;
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int i = lane; i < total; i += 32) {
+    const int r = i / pieces;
+    float x[8];
+    kv8_load8(src + r * pitch + (i - r * pieces) * 8, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  const uint32_t f = max(old, m >> 23);
+  int8_t* const to = codes + (((size_t)page * 2 + kind) * heads + head) * page_size * dim;
+  if (first && f != old) {
+    if (lane == 0) *exponent = (uint8_t)f;
+    if (f != 255u) {
+      // the page's other rows take the larger step
+      const int shift = min((int)(f - old), 7);
+      const int per = page_size * pieces;
+      for (int i = lane; i < per; i += 32) {
+        const int r = i / pieces;
+        if (r >= first && r < first + n) continue;
+        uint2* p = reinterpret_cast<uint2*>(to + (size_t)i * 8);
+        uint2 c = *p;
+        uint32_t* w = &c.x;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t q = 0;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) q |= ((uint32_t)((int)(int8_t)(w[j] >> (8 * b)) >> shift) & 255u) << (8 * b);
+          w[j] = q;
+        }
+        *p = c;
+      }
+    }
+  }
+  if (!first && lane == 0) *exponent = (uint8_t)f;
+#pragma unroll 4
+  for (int i = lane; i < total; i += 32) {
+    const int r = i / pieces, c = i - r * pieces;
+    float x[8];
+    kv8_load8(src + r * pitch + c * 8, x);
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)kv8_code(x[j], f) & 255u) << (8 * (j & 3));
+    *reinterpret_cast<uint2*>(to + (size_t)(first + r) * dim + c * 8) = make_uint2(w[0], w[1]);
+  }
+}
+
+// What 16 codes stand for, as T (both types hold (code + 1/2) step exactly).
+template <typename T> __device__ __forceinline__ void kv8_write16(T* to, const uint4& c, float step);
+template <> __device__ __forceinline__ void kv8_write16<float>(float* to, const uint4& c, float step) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float4 y;
+    y.x = ((float)(int8_t)(w[i]) + 0.5f) * step;
+    y.y = ((float)(int8_t)(w[i] >> 8) + 0.5f) * step;
+    y.z = ((float)(int8_t)(w[i] >> 16) + 0.5f) * step;
+    y.w = ((float)(int8_t)(w[i] >> 24) + 0.5f) * step;
+    *reinterpret_cast<float4*>(to + 4 * i) = y;
+  }
+}
+template <> __device__ __forceinline__ void kv8_write16<bf16>(bf16* to, const uint4& c, float step) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t y[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(((float)(int8_t)(w[i] >> (16 * h)) + 0.5f) * step,
+                                                     ((float)(int8_t)(w[i] >> (16 * h + 8)) + 0.5f) * step);
+      y[2 * i + h] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+  *reinterpret_cast<uint4*>(to) = make_uint4(y[0], y[1], y[2], y[3]);
+  *reinterpret_cast<uint4*>(to + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+}
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv8_values_kernel(const int8_t* codes, const uint8_t* exponents, T* out, long long pieces, int per_block) {
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (long long)gridDim.x * 256) {
+    const uint4 c = *reinterpret_cast<const uint4*>(codes + i * 16);
+    kv8_write16<T>(out + i * 16, c, kv8_step(exponents[i / per_block]));
+  }
+}
+
+static int kv8_sizes(int heads, int page_size, int dim) {
+  if (heads < 1 || heads > 32767 || page_size < 16 || page_size % 16 || page_size > 4096 || dim < 16 || dim % 16 || dim > 256) return IFB_ERR_SIZE;
+  return IFB_OK;
+}
+
+IFB_EXPORT int ifb_kv8_store(const void* k, const void* v, int dtype, long long k_row, long long v_row, const void* slots, void* codes,
+                             void* exponents, int rows, int heads, int page_size, int dim, void* stream) {
+  const int bad = kv8_sizes(heads, page_size, dim);
+  if (bad) return bad;
+  if (rows < 1) return IFB_ERR_SIZE;
+  if (dtype != IFB_F32 && dtype != IFB_BF16) return IFB_ERR_DTYPE;
+  const int esize = dtype == IFB_F32 ? 4 : 2;
+  if ((((uintptr_t)k) | ((uintptr_t)v) | (uintptr_t)(k_row * esize) | (uintptr_t)(v_row * esize) | ((uintptr_t)codes)) & 15) return IFB_ERR_ALIGN;
+  const int warps = 2 * heads < 8 ? 2 * heads : 8;
+  const dim3 grid(rows, (2 * heads + warps - 1) / warps);
+  if (dtype == IFB_F32)
+    return ifb_launch(kv8_store_kernel<float>, grid, dim3(32 * warps), 0, (cudaStream_t)stream, (const float*)k, (const float*)v, k_row, v_row,
+                      (const int*)slots, (int8_t*)codes, (uint8_t*)exponents, rows, heads, page_size, dim);
+  return ifb_launch(kv8_store_kernel<bf16>, grid, dim3(32 * warps), 0, (cudaStream_t)stream, (const bf16*)k, (const bf16*)v, k_row, v_row,
+                    (const int*)slots, (int8_t*)codes, (uint8_t*)exponents, rows, heads, page_size, dim);
+}
+
+IFB_EXPORT int ifb_kv8_values(const void* codes, const void* exponents, void* out, int dtype, int pages, int heads, int page_size, int dim,
+                              void* stream) {
+  const int bad = kv8_sizes(heads, page_size, dim);
+  if (bad) return bad;
+  if (pages < 1) return IFB_ERR_SIZE;
+  if (dtype != IFB_F32 && dtype != IFB_BF16) return IFB_ERR_DTYPE;
+  if ((((uintptr_t)codes) | ((uintptr_t)out)) & 15) return IFB_ERR_ALIGN;
+  const int per_block = page_size * dim / 16;
+  const long long pieces = (long long)pages * 2 * heads * per_block;
+  const long long blocks = (pieces + 255) / 256, most = (long long)ifb_sm_count() * 64;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most));
+  if (dtype == IFB_F32)
+    return ifb_launch(kv8_values_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, (const int8_t*)codes, (const uint8_t*)exponents,
+                      (float*)out, pieces, per_block);
+  return ifb_launch(kv8_values_kernel<bf16>, grid, dim3(256), 0, (cudaStream_t)stream, (const int8_t*)codes, (const uint8_t*)exponents,
+                    (bf16*)out, pieces, per_block);
+}

@@ -1,0 +1,638 @@
+// Causal attention over pages of keys and values held in 8 bits (kv8.cu has the format), compiled for one head size
+// (-DHEAD_DIM=<multiple of 16, at most 256>) and one number of terms (-DTERMS=1: bfloat16 queries and output; 2: float32).
+//
+// The products run on the tensor cores (mma.sync, float32 accumulation) over the codes as whole numbers, which half precision
+// holds exactly; a page's step enters as a factor of its scores (keys) and of its weights (values), so no number is rounded
+// for having been 8 bits.  With TERMS 2 a query and a softmax weight are each the sum of two half-precision numbers, 22 bits.
+//
+// The products are transposed: S^T = K Q^T and O^T = V^T P^T, so that keys (and head dimensions) fill the 16 rows of an
+// instruction and up to eight score rows (query token x query head of a key head) its 8 columns; decoding with eight query
+// heads per key head wastes nothing.  A warp takes 16 keys of one page at a time: their codes come from global memory to
+// registers in 16-byte pieces, each already where its product wants it (any order of the dimensions serves the sums over
+// them, so the order is the loads'), so there is no shared memory, no barrier and no wait between warps in the loop; the
+// other warps of the SM and the order of the requests (the next keys while the values are multiplied, the next values while
+// the scores are formed) keep the memory busy.
+//
+// From bits to half-precision numbers: u = code + 128 in the low byte of a half is the subnormal number u 2^-24, exactly; two
+// integer instructions make two of them.  Keys of bfloat16 queries stay so (q . (u - 127.5) = q . u - 127.5 sum(q), the second
+// known per row); for values, and for keys of float32 queries, 128 is taken off again: a sum over thousands of keys would lose
+// what the offset swamps, and a float32 score has no bits to spare for it.
+//
+// Softmax: weights are 2^(score - m + 8) with a reference m per row that moves (and then rescales the sums) only when a score
+// exceeds it by 6 in the exponent, so that most tiles need no maximum over lanes; 2^14 is then the largest weight, and
+// half-precision numbers down to 2^-32 of it still count.  A weight enters the product times its page's step over the largest
+// step so far.  Sums are float32.
+//
+// Split form: the work (64 keys of a key head for one tile of score rows is a unit) of all requests is cut into as many equal
+// pieces as CTAs fit on the device, whatever the lengths; a piece that ends inside an item leaves its sums in scratch memory,
+// and the CTA that arrives last at an item adds them in the order of the pieces.  Whole form (prompts): a warp owns its score
+// rows over all their keys.
+// Keys that no row of a tile sees are not read; block-table entries outside are not followed.  A row that sees no key is zero.
+#include "common.cuh"
+#include <cuda_fp16.h>
+#include <math.h>
+
+#ifndef HEAD_DIM
+#error "compile with -DHEAD_DIM=<head size>"
+#endif
+#if HEAD_DIM % 16 != 0 || HEAD_DIM < 16 || HEAD_DIM > 256
+#error "HEAD_DIM must be a multiple of 16 between 16 and 256"
+#endif
+#ifndef TERMS
+#define TERMS 1
+#endif
+
+typedef __nv_bfloat16 bf16;
+#if TERMS == 2
+typedef float qtype;
+#else
+typedef bf16 qtype;
+#endif
+constexpr int D = HEAD_DIM;
+constexpr int KS = D / 16;               // k steps of a score product, m tiles of an output product
+constexpr int WARPS = 4;
+constexpr int K64 = D / 64;              // pieces of 64 dimensions of a key that a quad of lanes takes 16 bytes a lane at a time
+constexpr int UNIT = 16 * WARPS;         // keys of a unit of the split form
+constexpr int NO_ROW = -1000000000;
+constexpr int KV8_MAX_REQUESTS = 1024;   // of the split form (their prefix sums lie in shared memory)
+
+struct Kv8Args {
+  const qtype* q;
+  long long q_row;                       // elements between tokens
+  const int8_t* codes;
+  const uint8_t* exponents;
+  const int* tables;
+  int table_stride;
+  const int* cu_q;
+  const int* seq_lens;
+  qtype* out;                            // [tokens][heads][D]
+  float* parts;                          // split form: [2 per CTA][rows of a tile][D + 2]
+  int* counters;                         // split form: one per item, 0 between launches
+  int requests, heads, kv_heads, page_size, window;
+  float scale;                           // of the scores, times log2(e)
+  int min_rows, max_rows;                // requests with fewer or more score rows than this are another kernel's
+  int tiles;                             // split form: tiles of score rows that any request has at most
+};
+
+__device__ __forceinline__ float kv8_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float kv8_step(uint32_t f) {                 // 2^(f - 133), 0, NaN
+  if (f == 0u) return 0.f;
+  if (f == 255u) return __uint_as_float(0x7fffffffu);
+  return f > 6u ? __uint_as_float((f - 6u) << 23) : __uint_as_float(1u << (f + 16u));
+}
+// d += a b: a 16 x 16 (rows by k), b 16 x 8.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {            // of an 8 x 8 matrix of halves over the warp
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_half_rest(float lo, float hi, uint32_t rounded) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&rounded));
+  return pack_half(lo - f.x, hi - f.y);
+}
+constexpr float KEY_OFFSET = TERMS == 2 ? 0.5f : -127.5f;              // what a key's number has beside its half-precision one
+// Bytes 0 and 2 (and 1 and 3) of a word of codes as half-precision numbers (code + 128) 2^-24.
+__device__ __forceinline__ uint32_t even_bytes(uint32_t w) { return (w & 0x00ff00ffu) ^ 0x00800080u; }
+__device__ __forceinline__ uint32_t odd_bytes(uint32_t w) { return ((w >> 8) & 0x00ff00ffu) ^ 0x00800080u; }
+__device__ __forceinline__ uint32_t centred(uint32_t x) {               // code 2^-24
+  const uint32_t off = 0x80808080u;                                     // -(128 2^-24) twice: sign, subnormal 0x0080
+  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&off));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// ---- pieces of a value row: blocks of 128, 64, 32 and 16 dimensions, an eighth of a block (16, 8, 4, 2 bytes) per lane -------
+template <int W> struct Piece;
+template <> struct Piece<128> { uint4 r; __device__ __forceinline__ void load(const int8_t* p) { r = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; } };
+template <> struct Piece<64> { uint2 r; __device__ __forceinline__ void load(const int8_t* p) { r = *reinterpret_cast<const uint2*>(p); }
+  __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? r.x : r.y; } };
+template <> struct Piece<32> { uint32_t r; __device__ __forceinline__ void load(const int8_t* p) { r = *reinterpret_cast<const uint32_t*>(p); }
+  __device__ __forceinline__ uint32_t word(int) const { return r; } };
+template <> struct Piece<16> { uint32_t r; __device__ __forceinline__ void load(const int8_t* p) { r = *reinterpret_cast<const uint16_t*>(p); }
+  __device__ __forceinline__ uint32_t word(int) const { return r; } };
+
+// The values of 16 keys as a lane holds them: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 (c = lane % 4).  Blocks follow one another.
+template <int LEFT> struct Values {
+  static constexpr int W = LEFT >= 128 ? 128 : LEFT >= 64 ? 64 : LEFT >= 32 ? 32 : 16;
+  Piece<W> v[4];
+  Values<LEFT - W> rest;
+  __device__ __forceinline__ void load(const int8_t* tile, int lane) {       // tile: the first of the 16 keys, at this block
+    const int8_t* p = tile + (lane & 3) * 2 * D + (lane >> 2) * (W / 8);
+    v[0].load(p); v[1].load(p + D); v[2].load(p + 8 * D); v[3].load(p + 9 * D);
+    rest.load(tile + W, lane);
+  }
+  // o^T += v^T p^T; m tile i of a block has dimension chunk + 2 i in its row lane / 4 and chunk + 2 i + 1 in row lane / 4 + 8
+  template <int NT>
+  __device__ __forceinline__ void multiply(float (*o)[NT][4], const uint32_t (&p)[TERMS][NT][2]) const {
+#pragma unroll
+    for (int i = 0; i < W / 16; ++i) {
+      const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;
+      const uint32_t x = __byte_perm(v[0].word(i >> 1), v[1].word(i >> 1), sel), y = __byte_perm(v[2].word(i >> 1), v[3].word(i >> 1), sel);
+      const uint32_t a0 = centred(even_bytes(x)), a1 = centred(odd_bytes(x)), a2 = centred(even_bytes(y)), a3 = centred(odd_bytes(y));
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(o[i][n], a0, a1, a2, a3, p[t][n][0], p[t][n][1]);
+    }
+    rest.template multiply<NT>(o + W / 16, p);
+  }
+  // the dimension of element e (0, 1) of m tile i
+  static __device__ __forceinline__ int dim(int i, int lane, int e) {
+    if (i < W / 16) return (lane >> 2) * (W / 8) + 2 * i + e;
+    return W + Values<LEFT - W>::dim(i - W / 16, lane, e);
+  }
+};
+template <> struct Values<0> {
+  __device__ __forceinline__ void load(const int8_t*, int) {}
+  template <int NT> __device__ __forceinline__ void multiply(float (*)[NT][4], const uint32_t (&)[TERMS][NT][2]) const {}
+  static __device__ __forceinline__ int dim(int, int, int) { return 0; }
+};
+
+// The keys of a tile as a lane holds them: keys lane / 4 and lane / 4 + 8.
+struct Keys {
+  uint4 w[2][K64 ? K64 : 1];
+  uint32_t tail[2][KS - 4 * K64 ? KS - 4 * K64 : 1];
+  __device__ __forceinline__ void load(const int8_t* tile, int lane) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int8_t* p = tile + ((lane >> 2) + 8 * e) * D;
+#pragma unroll
+      for (int h = 0; h < K64; ++h) w[e][h] = *reinterpret_cast<const uint4*>(p + h * 64 + (lane & 3) * 16);
+#pragma unroll
+      for (int s = 0; s < KS - 4 * K64; ++s) tail[e][s] = *reinterpret_cast<const uint32_t*>(p + K64 * 64 + s * 16 + (lane & 3) * 4);
+    }
+  }
+  __device__ __forceinline__ uint32_t word(int e, int ks) const {
+    if (ks >= 4 * K64) return tail[e][ks - 4 * K64];
+    const uint4& x = w[e][ks >> 2];
+    return (ks & 3) == 0 ? x.x : (ks & 3) == 1 ? x.y : (ks & 3) == 2 ? x.z : x.w;
+  }
+};
+// Where the four dimensions of a lane's word of k step ks begin.
+__device__ __forceinline__ int key_dim(int ks, int lane) {
+  return ks < 4 * K64 ? (ks >> 2) * 64 + (lane & 3) * 16 + (ks & 3) * 4 : K64 * 64 + (ks - 4 * K64) * 16 + (lane & 3) * 4;
+}
+
+// One warp over tiles of 16 keys for up to 8 NT score rows of one key head.  In the layout of the results a lane has rows
+// 8 n + 2 (lane % 4) + {0, 1} of row tile n.
+template <int NT>
+struct Stream {
+  uint32_t qf[TERMS][NT][KS][2];
+  float qscale[NT][2], qoff[NT][2];      // what turns a product into a number of real units: times qscale, and qoff
+  int last[NT][2];                       // position of the row's query (NO_ROW: no such row)
+  float m[NT][2], l[NT][2], wsum[NT][2]; // reference of the row's scores; sums of its weights, and of weights times steps, this lane's part
+  float o[KS][NT][4];
+  int v_ref;                             // exponent field that the sums of weighted values are in units of
+
+  __device__ __forceinline__ void reset() {
+    v_ref = 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; wsum[n][e] = 0.f; }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) { o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f; }
+    }
+  }
+  // row0: the first of the rows; rows: how many the request has; pos0: position of its first query; G: query heads per key head.
+  __device__ __forceinline__ void load_queries(const Kv8Args& a, int first_token, int row0, int rows, int pos0, int kv_head, int G, int lane) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = row0 + n * 8 + (lane >> 2);
+      const bool in = row < rows;
+      const qtype* src = a.q + (size_t)(first_token + (in ? row / G : 0)) * a.q_row + (size_t)(kv_head * G + (in ? row % G : 0)) * D;
+      uint32_t raw[KS][4];                                              // float32 bits
+      uint32_t amax = 0;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d = key_dim(ks, lane);
+#if TERMS == 2
+        const uint4 x = in ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+        raw[ks][0] = x.x; raw[ks][1] = x.y; raw[ks][2] = x.z; raw[ks][3] = x.w;
+#else
+        const uint2 x = in ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
+        raw[ks][0] = x.x << 16; raw[ks][1] = x.x & 0xffff0000u; raw[ks][2] = x.y << 16; raw[ks][3] = x.y & 0xffff0000u;
+#endif
+#pragma unroll
+        for (int j = 0; j < 4; ++j) amax = max(amax, raw[ks][j] & 0x7fffffffu);
+      }
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // the row's largest number becomes one of [2^10, 2^11): a power of two that a float holds either way round
+      const int f = min(max((int)(amax >> 23), 11), 250);
+      const float to = __uint_as_float((uint32_t)(127 + 137 - f) << 23);      // 2^(10 - (f - 127))
+      const float back = __uint_as_float((uint32_t)(127 - 137 + f) << 23);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(raw[ks][j]) * to;
+        qf[0][n][ks][0] = pack_half(x[0], x[2]);                        // beside the even and the odd bytes of a word of codes
+        qf[0][n][ks][1] = pack_half(x[1], x[3]);
+#if TERMS == 2
+        qf[1][n][ks][0] = pack_half_rest(x[0], x[2], qf[0][n][ks][0]);
+        qf[1][n][ks][1] = pack_half_rest(x[1], x[3], qf[0][n][ks][1]);
+#endif
+      }
+      // sums of the rounded rows, in the layout of the scores, by a product with ones
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) mma_f16(s, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, qf[t][n][ks][0], qf[t][n][ks][1]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float b = __shfl_sync(0xffffffffu, back, ((lane & 3) * 2 + e) * 4);
+        qscale[n][e] = b * 16777216.f;
+        qoff[n][e] = KEY_OFFSET * s[e] * b;
+        const int r = row0 + n * 8 + (lane & 3) * 2 + e;
+        last[n][e] = r < rows ? pos0 + r / G : NO_ROW;
+      }
+    }
+  }
+
+  // Scores of 16 keys from `key0` on, weights, and o += p v.  step: of the keys, times the softmax's factor; vf: the values' field.
+  template <bool MASK>
+  __device__ __forceinline__ void scores(const Keys& k, float step, int key0, int window, float (&s)[NT][4], int lane) const {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t a0 = even_bytes(k.word(0, ks)), a1 = even_bytes(k.word(1, ks)), a2 = odd_bytes(k.word(0, ks)), a3 = odd_bytes(k.word(1, ks));
+      if (TERMS == 2) { a0 = centred(a0); a1 = centred(a1); a2 = centred(a2); a3 = centred(a3); }
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[t][n][ks][0], qf[t][n][ks][1]);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = fmaf(s[n][j], qscale[n][j & 1], qoff[n][j & 1]) * step;
+        bool seen = true;
+        if (MASK) {
+          const int key = key0 + (lane >> 2) + (j >> 1) * 8, p = last[n][j & 1];
+          seen = key <= p && (window == 0 || key > p - window);
+        }
+        s[n][j] = seen ? x : -INFINITY;
+      }
+  }
+  template <bool MASK>
+  __device__ __forceinline__ void weigh(float (&s)[NT][4], const Values<D>& v, int vf) {
+    bool rise = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) rise |= s[n][j] > m[n][j & 1] + 6.f;
+    const bool larger = vf > v_ref && vf != 255;                        // uniform
+    if (__any_sync(0xffffffffu, rise) || larger) {
+      float fv = 1.f;
+      if (larger) {
+        fv = v_ref ? __uint_as_float((uint32_t)max(0, 127 + v_ref - vf) << 23) : 0.f;
+        v_ref = vf;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(s[n][e], s[n][2 + e]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx = fmaxf(mx, m[n][e]);
+          f[e] = mx == m[n][e] ? 1.f : kv8_exp2(m[n][e] - mx);
+          m[n][e] = mx;
+          l[n][e] *= f[e];
+          f[e] *= fv;
+          wsum[n][e] *= f[e];
+        }
+#pragma unroll
+        for (int i = 0; i < KS; ++i) { o[i][n][0] *= f[0]; o[i][n][1] *= f[1]; o[i][n][2] *= f[0]; o[i][n][3] *= f[1]; }
+      }
+    }
+    // the step of this page's values over the reference; fields in use are 1 .. 254
+    const float fw = vf == 0 ? 0.f : vf == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)max(0, 127 + vf - v_ref) << 23);
+    uint32_t p[TERMS][NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float ref = m[n][j & 1], x = kv8_exp2(s[n][j] - (ref == -INFINITY ? 0.f : ref) + 8.f);
+        l[n][j & 1] += x;
+        w[j] = MASK && s[n][j] == -INFINITY ? 0.f : x * fw;             // (a page of NaN, a key that is not seen)
+        wsum[n][j & 1] += w[j];
+      }
+      const uint32_t lo = pack_half(w[0], w[1]), hi = pack_half(w[2], w[3]);
+      p[0][n][0] = transpose8(lo);
+      p[0][n][1] = transpose8(hi);
+#if TERMS == 2
+      p[1][n][0] = transpose8(pack_half_rest(w[0], w[1], lo));
+      p[1][n][1] = transpose8(pack_half_rest(w[2], w[3], hi));
+#endif
+    }
+    v.template multiply<NT>(o, p);
+  }
+
+  // Tiles first, first + step, ... up to `end` (exclusive) of 16 keys.  full_to: keys up to here are seen by every row that exists
+  // (full_from: from here on).
+  __device__ __forceinline__ void run(const Kv8Args& a, const int* table, int kv_head, int first, int end, int step, int full_from, int full_to,
+                                      int lane) {
+    if (first >= end) return;
+    const size_t head_bytes = (size_t)a.page_size * D, page_bytes = 2 * (size_t)a.kv_heads * head_bytes;
+    const int per_page = a.page_size / 16;
+    auto tile_at = [&](int t, int page) {                               // the keys; the values lie kv_heads heads further
+      return a.codes + (size_t)page * page_bytes + (size_t)kv_head * head_bytes + (size_t)((t % per_page) * 16) * D;
+    };
+    const size_t v_off = (size_t)a.kv_heads * head_bytes;
+    Keys k;
+    Values<D> v;
+    int page = table[first / per_page];
+    const int8_t* at = tile_at(first, page);
+    const uint8_t* fields = a.exponents + (size_t)page * 2 * a.kv_heads + kv_head;
+    int kf = fields[0], vf = fields[a.kv_heads];
+    k.load(at, lane);
+    v.load(at + v_off, lane);
+    int next_page = first + step < end ? table[(first + step) / per_page] : page;
+    for (int t = first; t < end; t += step) {
+      const bool more = t + step < end;
+      float s[NT][4];
+      const bool whole = t * 16 >= full_from && t * 16 + 15 <= full_to;
+      const float ks = kv8_step((uint32_t)kf) * a.scale;
+      if (whole) scores<false>(k, ks, t * 16, a.window, s, lane);
+      else scores<true>(k, ks, t * 16, a.window, s, lane);
+      const int8_t* next = at;
+      const int vf_now = vf;
+      if (more) {                                                       // the next keys while these values are multiplied
+        next = tile_at(t + step, next_page);
+        const uint8_t* nf = a.exponents + (size_t)next_page * 2 * a.kv_heads + kv_head;
+        kf = nf[0];
+        vf = nf[a.kv_heads];
+        k.load(next, lane);
+        if (t + 2 * step < end) next_page = table[(t + 2 * step) / per_page];
+      }
+      if (whole) weigh<false>(s, v, vf_now);
+      else weigh<true>(s, v, vf_now);
+      if (more) v.load(next + v_off, lane);                             // and the next values while the next scores are formed
+      at = next;
+    }
+  }
+  // Sums over the lanes that share a row, and the weighted values in real units (times the weights' common factor).
+  __device__ __forceinline__ void finish() {
+    const float unit = kv8_step((uint32_t)v_ref);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
+          wsum[n][e] += __shfl_xor_sync(0xffffffffu, wsum[n][e], x);
+        }
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][n][j] = fmaf(o[i][n][j], 16777216.f, 0.5f * wsum[n][j & 1]) * unit;
+    }
+  }
+};
+
+__device__ __forceinline__ void kv8_store_pair(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+__device__ __forceinline__ void kv8_store_pair(bf16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
+__device__ __forceinline__ float kv8_ratio(float o, float l) { return l == 0.f ? 0.f : o / l; }
+
+// --------------------------------------------------------------------------------------------
+// Whole form: grid (blocks of 32 NT rows, key heads, requests); a warp has 8 NT rows over all their keys.
+// --------------------------------------------------------------------------------------------
+template <int NT>
+__global__ void __launch_bounds__(32 * WARPS)
+kv8_attention_whole_kernel(Kv8Args a) {
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.z, kv_head = blockIdx.y, G = a.heads / a.kv_heads;
+  const int q0 = a.cu_q[r], q_len = a.cu_q[r + 1] - q0, L = a.seq_lens[r], rows = q_len * G;
+  if (q_len <= 0 || rows < a.min_rows || rows > a.max_rows) return;
+  // the rows with the most keys first
+  const int row0 = ((int)(gridDim.x - 1 - blockIdx.x) * WARPS + warp) * 8 * NT;
+  if (row0 >= rows) return;
+  const int pos0 = L - q_len, p_first = pos0 + row0 / G, p_last = pos0 + min(row0 + 8 * NT - 1, rows - 1) / G;
+  Stream<NT> st;
+  st.reset();
+  st.load_queries(a, q0, row0, rows, pos0, kv_head, G, lane);
+  const int lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
+  if (p_last >= 0)
+    st.run(a, a.tables + (size_t)r * a.table_stride, kv_head, lo / 16, p_last / 16 + 1, 1, a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
+  st.finish();
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = row0 + n * 8 + (lane & 3) * 2 + e;
+      if (row >= rows) continue;
+      qtype* to = a.out + ((size_t)(q0 + row / G) * a.heads + kv_head * G + row % G) * D;
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+        kv8_store_pair(to + Values<D>::dim(i, lane, 0), kv8_ratio(st.o[i][n][e], st.l[n][e]), kv8_ratio(st.o[i][n][2 + e], st.l[n][e]));
+    }
+}
+
+// --------------------------------------------------------------------------------------------
+// Split form.  Items are (request, tile of 8 NT rows, key head), in that order; an item has the units of its request (those of
+// the request's last row: earlier tiles leave a few empty), one at least, so that a row without keys is written.
+// --------------------------------------------------------------------------------------------
+template <int NT>
+__global__ void __launch_bounds__(32 * WARPS)
+kv8_attention_split_kernel(Kv8Args a) {
+  constexpr int ROWS = 8 * NT;
+  extern __shared__ __align__(16) float sums[];                         // [WARPS][ROWS][D], then maxima and sums [WARPS][ROWS] each
+  __shared__ int prefix[KV8_MAX_REQUESTS + 1];                          // units before a request
+  __shared__ int arrived;
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads;
+  float* const sm_m = sums + WARPS * ROWS * D;
+  float* const sm_l = sm_m + WARPS * ROWS;
+  auto shape = [&](int r, int& units, int& tiles) {                     // of a request: units of an item, tiles of rows
+    const int q_len = a.cu_q[r + 1] - a.cu_q[r], L = a.seq_lens[r], rows = q_len * G;
+    units = tiles = 0;
+    if (q_len <= 0 || rows < a.min_rows || rows > a.max_rows) return;
+    tiles = (rows + ROWS - 1) / ROWS;
+    const int lo = a.window > 0 ? max(0, L - q_len - a.window + 1) : 0;
+    units = L > 0 ? max(1, (L - 1) / UNIT - lo / UNIT + 1) : 1;
+  };
+  if (warp == 0) {
+    int before = 0;
+    for (int r0 = 0; r0 < a.requests; r0 += 32) {
+      int units = 0, tiles = 0;
+      if (r0 + lane < a.requests) shape(r0 + lane, units, tiles);
+      int x = units * tiles * a.kv_heads;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      if (r0 + lane < a.requests) prefix[r0 + lane + 1] = before + x;
+      before += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) prefix[0] = 0;
+  }
+  __syncthreads();
+  const int total = prefix[a.requests];
+  const int per = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  int at = (int)blockIdx.x * per;
+  const int end = min(total, at + per);
+  int r = 0;
+  while (at < end) {
+    while (prefix[r + 1] <= at) ++r;
+    int units, tiles;
+    shape(r, units, tiles);
+    const int in_request = at - prefix[r], item = in_request / units, unit0 = in_request - item * units;
+    const int n_units = min(units - unit0, end - at), tile = item / a.kv_heads, kv_head = item - tile * a.kv_heads;
+    const int q0 = a.cu_q[r], q_len = a.cu_q[r + 1] - q0, L = a.seq_lens[r], rows = q_len * G, row0 = tile * ROWS;
+    const int here = min(ROWS, rows - row0);
+    const int pos0 = L - q_len, p_first = pos0 + row0 / G, p_last = pos0 + (row0 + here - 1) / G;
+    const int lo_request = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
+    const int key0 = (lo_request / UNIT + unit0) * UNIT;                // keys of this piece: up to n_units units from here
+    const int key_end = min(p_last + 1, key0 + n_units * UNIT);
+    Stream<NT> st;
+    st.reset();
+    st.load_queries(a, q0, row0, rows, pos0, kv_head, G, lane);
+    const int first = max(key0, lo) / 16;
+    st.run(a, a.tables + (size_t)r * a.table_stride, kv_head, first + warp, key_end > 0 ? (key_end + 15) / 16 : 0, WARPS,
+           a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
+    st.finish();
+    // the warps' sums side by side
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = n * 8 + (lane & 3) * 2 + e;
+        if (row < here) {
+          float* to = sums + ((size_t)warp * ROWS + row) * D;
+#pragma unroll
+          for (int i = 0; i < KS; ++i) kv8_store_pair(to + Values<D>::dim(i, lane, 0), st.o[i][n][e], st.o[i][n][2 + e]);
+          if (lane < 4) { sm_m[warp * ROWS + row] = st.m[n][e]; sm_l[warp * ROWS + row] = st.l[n][e]; }
+        }
+      }
+    __syncthreads();
+    const bool alone = n_units == units;
+    // a piece's place in scratch memory: a CTA has at most two that are not whole items, its first and its last
+    float* const mine = a.parts + ((size_t)blockIdx.x * 2 + (unit0 ? 0 : 1)) * ROWS * (D + 2);
+    for (int i = tid; i < here * D; i += 32 * WARPS) {
+      const int row = i / D, d = i - row * D;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_m[w * ROWS + row]);
+      const float U = M == -INFINITY ? 0.f : M;
+      float o = 0.f, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = exp2f(sm_m[w * ROWS + row] - U);
+        o += sums[((size_t)w * ROWS + row) * D + d] * f;
+        l += sm_l[w * ROWS + row] * f;
+      }
+      if (alone) {
+        const int full = row0 + row;
+        a.out[((size_t)(q0 + full / G) * a.heads + kv_head * G + full % G) * D + d] = from_f32<qtype>(kv8_ratio(o, l));
+      } else {
+        mine[row * (D + 2) + d] = o;
+        if (d == 0) { mine[row * (D + 2) + D] = M; mine[row * (D + 2) + D + 1] = l; }
+      }
+    }
+    if (!alone) {
+      __threadfence();
+      __syncthreads();
+      const int first_unit = prefix[r] + item * units, first_cta = first_unit / per, last_cta = (first_unit + units - 1) / per;
+      int* const counter = a.counters + ((size_t)r * a.tiles + tile) * a.kv_heads + kv_head;
+      if (tid == 0) arrived = atomicAdd(counter, 1);
+      __syncthreads();
+      if (arrived == last_cta - first_cta) {                            // the last of the item's pieces
+        __threadfence();
+        for (int i = tid; i < here * D; i += 32 * WARPS) {
+          const int row = i / D, d = i - row * D;
+          float M = -INFINITY, o = 0.f, l = 0.f;
+          for (int c = first_cta; c <= last_cta; ++c)
+            M = fmaxf(M, __ldcg(a.parts + ((size_t)c * 2 + (c == first_cta ? 1 : 0)) * ROWS * (D + 2) + row * (D + 2) + D));
+          const float U = M == -INFINITY ? 0.f : M;
+          for (int c = first_cta; c <= last_cta; ++c) {
+            const float* part = a.parts + ((size_t)c * 2 + (c == first_cta ? 1 : 0)) * ROWS * (D + 2) + row * (D + 2);
+            const float f = exp2f(__ldcg(part + D) - U);
+            o += __ldcg(part + d) * f;
+            l += __ldcg(part + D + 1) * f;
+          }
+          const int full = row0 + row;
+          a.out[((size_t)(q0 + full / G) * a.heads + kv_head * G + full % G) * D + d] = from_f32<qtype>(kv8_ratio(o, l));
+        }
+        if (tid == 0) *counter = 0;
+      }
+    }
+    __syncthreads();                                                    // the sums are read; the next item writes them
+    at += n_units;
+  }
+}
+
+template <int NT> static size_t kv8_split_smem() { return (size_t)WARPS * 8 * NT * (D + 2) * sizeof(float); }
+template <int NT> static int kv8_split_ctas(int* ctas) {                // that fit on the device at once
+  static int known[IFB_MAX_DEVICES] = {};
+  int dev = 0, per = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= IFB_MAX_DEVICES) return IFB_ERR_ARG;
+  if (!known[dev]) {
+    IFB_ALLOW_SMEM(kv8_attention_split_kernel<NT>, kv8_split_smem<NT>());
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kv8_attention_split_kernel<NT>, 32 * WARPS, kv8_split_smem<NT>());
+    if (e != cudaSuccess) return -(int)e;
+    known[dev] = (per < 1 ? 1 : per) * ifb_sm_count();
+  }
+  *ctas = known[dev];
+  return IFB_OK;
+}
+
+// Floats of scratch memory that the split form of `nt` row tiles wants, or a negative error.
+IFB_EXPORT long long ifb_kv8_attention_scratch(int nt) {
+  int ctas = 0;
+  const int bad = nt == 1 ? kv8_split_ctas<1>(&ctas) : kv8_split_ctas<2>(&ctas);
+  return bad ? (bad > 0 ? -bad : bad) : (long long)ctas * 2 * 8 * nt * (D + 2);
+}
+
+template <int NT>
+static int kv8_launch(const Kv8Args& a, bool whole, int max_q, cudaStream_t stream) {
+  if (whole) {
+    const int rows = max_q * (a.heads / a.kv_heads);
+    const dim3 grid((rows + 8 * NT * WARPS - 1) / (8 * NT * WARPS), a.kv_heads, a.requests);
+    return ifb_launch(kv8_attention_whole_kernel<NT>, grid, dim3(32 * WARPS), 0, stream, a);
+  }
+  int ctas = 0;
+  const int bad = kv8_split_ctas<NT>(&ctas);
+  if (bad) return bad;
+  return ifb_launch(kv8_attention_split_kernel<NT>, dim3(ctas), dim3(32 * WARPS), kv8_split_smem<NT>(), stream, a);
+}
+
+// nt: 1 or 2 tiles of 8 score rows per warp.  whole: the whole form.  Requests of min_rows .. max_rows score rows are worked on.
+IFB_EXPORT int ifb_kv8_attention(const void* q, int dtype, long long q_row, const void* codes, const void* exponents, const void* tables, int table_stride,
+                                 const void* cu_q, const void* seq_lens, void* out, void* parts, void* counters, int requests, int heads, int kv_heads,
+                                 int page_size, int dim, float scale, int window, int max_q, int min_rows, int max_rows, int tiles, int nt, int whole,
+                                 void* stream) {
+  if (dtype != (TERMS == 2 ? IFB_F32 : IFB_BF16)) return IFB_ERR_DTYPE;
+  if (dim != D || heads < 1 || kv_heads < 1 || heads % kv_heads || page_size < 16 || page_size % 16 || requests < 1 || max_q < 1 || window < 0 ||
+      (nt != 1 && nt != 2) || kv_heads > 65535 || requests > 65535)
+    return IFB_ERR_SIZE;
+  if (!whole && (requests > KV8_MAX_REQUESTS || !parts || !counters || tiles < 1)) return IFB_ERR_ARG;
+  if ((((uintptr_t)q) | ((uintptr_t)codes) | ((uintptr_t)out) | (uintptr_t)(q_row * sizeof(qtype))) & 15) return IFB_ERR_ALIGN;
+  const Kv8Args a = {(const qtype*)q, q_row, (const int8_t*)codes, (const uint8_t*)exponents, (const int*)tables, table_stride, (const int*)cu_q,
+                     (const int*)seq_lens, (qtype*)out, (float*)parts, (int*)counters, requests, heads, kv_heads, page_size, window,
+                     scale * 1.4426950408889634f, min_rows, max_rows, tiles};
+  return nt == 1 ? kv8_launch<1>(a, whole, max_q, (cudaStream_t)stream) : kv8_launch<2>(a, whole, max_q, (cudaStream_t)stream);
+}

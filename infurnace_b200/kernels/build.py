@@ -47,6 +47,10 @@ LIBRARIES: Dict[str, tuple] = {
     "latent": (["latent.cu", "attention_latent.cu", "attention_latent_mma.cu"], []),
     # matrices in microscaled 4-bit floating point and their products
     "mx4": (["mx4.cu"], []),
+    # keys and values of 8 bits with a scale for each page and head: store and values; attention over them, compiled once per
+    # head size and type: defines={"HEAD_DIM": d} (bfloat16) and {"HEAD_DIM": d, "TERMS": 2} (float32)
+    "kv8": (["kv8.cu"], []),
+    "kv8_attention": (["kv8_attention.cu"], []),
     # compiled once per head size: defines={"HEAD_DIM": d}
     "attention_mma": (["attention_mma.cu"], []),
 }
@@ -58,6 +62,9 @@ DEFAULT_VARIANTS = [("attention_mma", {"HEAD_DIM": d}) for d in (128, 16, 32, 48
 DEFAULT_VARIANTS += [(name, {"HEAD_DIM": 128, "WEIGHT_TERMS": 2, "SOFTCAP": 1}) for name in ("attention_mma", "attention_tc")]
 # bounded scores of unit queries and keys with two-term weights, heads of 128: prompts, and decoding
 DEFAULT_VARIANTS += [("attention_tc", {"HEAD_DIM": 128, "WEIGHT_TERMS": 2, "SOFTCAP": 2}), ("attention_mma", {"HEAD_DIM": 128, "WEIGHT_TERMS": 2})]
+# attention over 8-bit pages: heads of 128 (bfloat16), the sizes that the tests of the engine run, float32
+DEFAULT_VARIANTS += [("kv8_attention", {"HEAD_DIM": d}) for d in (128, 64, 256, 16)]
+DEFAULT_VARIANTS += [("kv8_attention", {"HEAD_DIM": d, "TERMS": 2}) for d in (128, 64, 256, 16)]
 
 def register_library(name: str, sources: Sequence[str], flags: Sequence[str] = (), *, replace: bool = False) -> None:
     """Make a library of CUDA sources from outside the package known to :func:`load_library`, so that a
@@ -209,7 +216,7 @@ def build_all(progress=None) -> List[str]:
     """Compile every library (used by the build check; needs no GPU)."""
     from concurrent.futures import ThreadPoolExecutor
     jobs = [("core", None), ("linear_tcgen05", None), ("linear_skinny_static", None), ("attention_tc", None),
-            ("mixers", None), ("hybrid", None), ("latent", None), ("mx4", None)] + DEFAULT_VARIANTS
+            ("mixers", None), ("hybrid", None), ("latent", None), ("mx4", None), ("kv8", None)] + DEFAULT_VARIANTS
     with ThreadPoolExecutor(max_workers=4) as pool:
         built = list(pool.map(lambda j: compile_library(j[0], j[1], progress), jobs))
     # objects of older sources are never loaded (their names carry another hash); take them out of the folder

@@ -1,11 +1,12 @@
-"""Serving in few bits: matrices in microscaled 4-bit floating point and the products with them.
+"""Serving in few bits: matrices in microscaled 4-bit floating point and the products with them; pages of keys and values in
+8 bits, the store into them and the attention that reads them.
 
-:class:`Mx4Matrix` is the data, :class:`LowBitKernels` the calls (a part of the kernel set).  Elements, scales and layout are
-defined at the head of ``csrc/mx4.cu``.
+:class:`Mx4Matrix` and :class:`Kv8Pages` are the data, :class:`LowBitKernels` the calls (a part of the kernel set).  Elements,
+scales and layouts are defined at the heads of ``csrc/mx4.cu`` and ``csrc/kv8.cu``.
 """
 from __future__ import annotations
 
-from ctypes import c_int, c_longlong, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -107,6 +108,8 @@ class Kv8Pages:
             raise KernelError("Kv8Pages: exponents are uint8 [pages, 2, kv_heads], contiguous, beside the codes")
         self.codes, self.exponents = codes, exponents
         self.pages, _, self.kv_heads, self.page_size, self.head_dim = codes.shape
+        if self.page_size % 16 or self.head_dim % 16 or not 16 <= self.head_dim <= 256 or not 16 <= self.page_size <= 4096:
+            raise KernelError("Kv8Pages: page_size is a multiple of 16 up to 4,096, head_dim one up to 256")
         self._at = (codes.data_ptr(), exponents.data_ptr())
 
     @classmethod
@@ -197,4 +200,136 @@ class LowBitKernels:
         self._err_armed = True
         self._low_bit_status(lib.ifb_mx4_linear(*x._at, *w._at, out.data_ptr(), code, n, k, w.rows, epi, self._dev_err.data_ptr(),
                                                 stream), "mx4_linear")
+        return out
+
+    # ------------------------------------------------------------------ keys and values of 8 bits
+    _kv8 = None
+
+    def _kv8_lib(self):
+        if self._kv8 is None:
+            lib = load_library("kv8", progress=self._progress)
+            lib.ifb_kv8_store.argtypes = [c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                          c_int, c_int, c_void_p]
+            lib.ifb_kv8_values.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]
+            self._kv8 = lib
+        return self._kv8
+
+    def kv8_store(self, k, v, slot_mapping, pages):
+        """The step's keys and values (bfloat16 or float32 [tokens, kv_heads, head_dim], views with rows of their own pitch) into
+        ``pages`` at ``slot_mapping`` (int32, page * page_size + offset; negative: not stored).  A page's tokens are adjacent
+        rows in ascending order, as the step function lays them out; a token at offset 0 begins its page anew."""
+        code = _CODES.get(k.dtype)
+        n = k.shape[0]
+        heads, dim = pages.kv_heads, pages.head_dim
+        if code is None or v.dtype != k.dtype or k.shape != (n, heads, dim) or v.shape != k.shape:
+            raise KernelError(f"kv8_store: k and v are bfloat16 or float32 [tokens, {heads}, {dim}]; got {k.dtype} {tuple(k.shape)} and "
+                              f"{v.dtype} {tuple(v.shape)}")
+        if k.stride(2) != 1 or v.stride(2) != 1 or (heads > 1 and (k.stride(1) != dim or v.stride(1) != dim)):
+            raise KernelError("kv8_store: the heads of a token lie one after the other")
+        if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (n,) or not slot_mapping.is_contiguous():
+            raise KernelError("kv8_store: slot_mapping is int32, one per token, contiguous")
+        device = pages.codes.device
+        if not k.is_cuda or k.device != device or v.device != device or slot_mapping.device != device:
+            raise KernelError("kv8_store: k, v and slot_mapping are on the pages' device")
+        if n == 0:
+            return
+        self.launches += 1
+        self._low_bit_status(self._kv8_lib().ifb_kv8_store(k.data_ptr(), v.data_ptr(), code, k.stride(0), v.stride(0), slot_mapping.data_ptr(),
+                                                           *pages._at, n, heads, pages.page_size, dim, self._stream()), "kv8_store")
+
+    def kv8_values(self, pages, out):
+        """The numbers that the bits of all pages stand for, as bfloat16 or float32 (both hold them exactly) of the codes' shape."""
+        code = _CODES.get(out.dtype)
+        if code is None or not out.is_cuda or out.shape != pages.codes.shape or not out.is_contiguous() or out.device != pages.codes.device:
+            raise KernelError("kv8_values: out is bfloat16 or float32 of the codes' shape, contiguous, on the pages' device")
+        self.launches += 1
+        self._low_bit_status(self._kv8_lib().ifb_kv8_values(*pages._at, out.data_ptr(), code, pages.pages, pages.kv_heads, pages.page_size,
+                                                            pages.head_dim, self._stream()), "kv8_values")
+        return out
+
+    def _kv8_attention_lib(self, dim, dtype):
+        libs = self.__dict__.setdefault("_kv8_attention", {})
+        lib = libs.get((dim, dtype))
+        if lib is None:
+            defines = {"HEAD_DIM": dim} if dtype == torch.bfloat16 else {"HEAD_DIM": dim, "TERMS": 2}
+            lib = load_library("kv8_attention", defines, progress=self._progress)
+            lib.ifb_kv8_attention.argtypes = [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                              c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int,
+                                              c_int, c_int, c_int, c_void_p]
+            lib.ifb_kv8_attention_scratch.restype = c_longlong
+            lib.ifb_kv8_attention_scratch.argtypes = [c_int]
+            lib.scratch_floats = {nt: int(lib.ifb_kv8_attention_scratch(nt)) for nt in (1, 2)}
+            for floats in lib.scratch_floats.values():
+                if floats < 0:
+                    raise KernelError(f"kv8_attention: the device cannot be asked for its size (error {floats})")
+            libs[(dim, dtype)] = lib
+        return lib
+
+    def _kv8_scratch(self, stream, floats, counters):
+        """(sums, counters) of the split form: of a stream each, and one pair for recorded graphs, whose replays follow one
+        another.  The counters are zero between launches; a recording could not clear new ones, so what it uses is made
+        before, with the first call outside of one."""
+        held = self.__dict__.setdefault("_kv8_held", {})
+        capturing = torch.cuda.is_current_stream_capturing()
+        for key in (("graph",) if capturing else (stream, "graph")):
+            have = held.get(key)
+            if have is None or have[0].numel() < floats or have[1].numel() < counters:
+                if capturing:
+                    raise KernelError("kv8_attention: run the call once before it is recorded into a graph")
+                more = (have[0].numel(), have[1].numel()) if have else (0, 0)
+                held[key] = (torch.empty(max(floats, more[0]), dtype=torch.float32, device="cuda"),
+                             torch.zeros(max(counters, more[1], 4096), dtype=torch.int32, device="cuda"))
+                if key == "graph":
+                    torch.cuda.current_stream().synchronize()            # cleared before a graph on another stream can use them
+                    self.scratch_generation += 1
+        return held["graph" if capturing else stream]
+
+    KV8_SPLIT_REQUESTS = 1024        # the split form keeps their prefix sums in shared memory
+
+    def kv8_attention(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, min_q_len=1):
+        """Causal attention of a step's queries over 8-bit pages: ``q`` and ``out`` bfloat16 or float32 [tokens, heads, head_dim] (the
+        rows of ``q`` may lie apart, those of ``out`` not); the query at position p sees positions max(0, p - window + 1) .. p
+        (``window`` 0: from 0); request r has the rows cu_q[r] .. cu_q[r + 1] - 1 and ``seq_lens[r]`` keys, these queries' own
+        among them.  A row that sees no key becomes zero.  No request has more than ``max_q_len`` queries or ``max_seq_len``
+        keys, none fewer than ``min_q_len`` queries."""
+        code = _CODES.get(q.dtype)
+        n, heads, dim = q.shape
+        kv_heads = pages.kv_heads
+        if code is None or out.dtype != q.dtype or out.shape != q.shape or dim != pages.head_dim or heads % kv_heads:
+            raise KernelError(f"kv8_attention: q and out are bfloat16 or float32 [tokens, a multiple of {kv_heads}, {pages.head_dim}]; got "
+                              f"{q.dtype} {tuple(q.shape)} and {out.dtype} {tuple(out.shape)}")
+        if q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim) or not out.is_contiguous():
+            raise KernelError("kv8_attention: the heads of a query lie one after the other, and out is contiguous")
+        r = seq_lens.numel()
+        if cu_q.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_tables.dtype != torch.int32 or cu_q.numel() != r + 1 \
+                or block_tables.dim() != 2 or block_tables.shape[0] < r or block_tables.stride(1) != 1 or not cu_q.is_contiguous() \
+                or not seq_lens.is_contiguous():
+            raise KernelError("kv8_attention: cu_q, seq_lens and block_tables are int32 for the same requests, dense along their last axis")
+        if block_tables.shape[1] * pages.page_size < max_seq_len:
+            raise KernelError(f"kv8_attention: block tables of {block_tables.shape[1]} pages do not hold {max_seq_len} keys")
+        device = pages.codes.device
+        if any(t.device != device for t in (q, out, cu_q, seq_lens, block_tables)) or not q.is_cuda:
+            raise KernelError("kv8_attention: all tensors are on the pages' device")
+        if n == 0 or r == 0:
+            return out
+        if window < 0 or max_q_len < 1 or not 1 <= min_q_len <= max_q_len:
+            raise KernelError("kv8_attention: window is not negative, and 1 <= min_q_len <= max_q_len")
+        lib, stream, group = self._kv8_attention_lib(dim, q.dtype), self._stream(), heads // kv_heads
+        # score rows beyond which a request's tiles fill the device by themselves and run whole; requests below run split
+        rows, least = max_q_len * group, min_q_len * group
+        limit = 64 if r <= self.KV8_SPLIT_REQUESTS else 0
+        nt = 1 if rows <= 8 or dim > 128 else 2
+        fixed = (q.data_ptr(), code, q.stride(0), *pages._at, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
+                 seq_lens.data_ptr(), out.data_ptr())
+        sizes = (r, heads, kv_heads, pages.page_size, dim, float(scale), int(window))
+        if least <= limit:
+            tiles = -(-min(rows, limit) // (8 * nt))
+            sums, counters = self._kv8_scratch(stream, lib.scratch_floats[nt], r * tiles * kv_heads)
+            self.launches += 1
+            self._low_bit_status(lib.ifb_kv8_attention(*fixed, sums.data_ptr(), counters.data_ptr(), *sizes, max_q_len, 0, limit, tiles, nt, 0,
+                                                       stream), "kv8_attention")
+        if rows > limit:
+            self.launches += 1
+            self._low_bit_status(lib.ifb_kv8_attention(*fixed, 0, 0, *sizes, max_q_len, limit + 1, (1 << 31) - 1, 1, nt, 1, stream),
+                                 "kv8_attention")
         return out

@@ -75,22 +75,33 @@ def store8(codes, fields, k, v, slots):
 
 
 def attention8(q, codes, fields, tables, cu_q, seq_lens, scale, window=0):
-    """Causal attention over the pages' values, request by request; a row that sees no key is zero."""
+    """Causal attention over the pages' values, request by request; a row that sees no key is zero.  Returns the output, for
+    each of its numbers the weighted sum of magnitudes, and for each row the most that rounding could act on in a score:
+    scale * sum |q| * 256 * the largest step."""
     heads, page_size, dim = codes.shape[2:]
     out = torch.zeros(q.shape, dtype=torch.float64)
+    mag, reach = torch.zeros_like(out), torch.zeros(q.shape[:2], dtype=torch.float64)
     group = q.shape[1] // heads
     for r in range(len(seq_lens)):
         a, b, n = int(cu_q[r]), int(cu_q[r + 1]), int(seq_lens[r])
-        for t in range(a, b):
-            p = n - (b - a) + (t - a)
-            lo = max(0, p - window + 1) if window else 0
-            if p < lo or p < 0:
-                continue
-            pos = torch.arange(lo, p + 1)
-            pages = tables[r][pos // page_size].long()
-            for h in range(heads):
-                kv = (codes[pages, :, h, pos % page_size].double() + 0.5) * step_of(fields)[pages, :, h][..., None]
-                for g in range(group):
-                    s = (kv[:, 0] @ q[t, h * group + g].double()) * scale
-                    out[t, h * group + g] = torch.softmax(s, 0) @ kv[:, 1]
-    return out
+        if n == 0 or a == b:
+            continue
+        pos = torch.arange(n)
+        kv = torch.zeros((n, 2, heads, dim), dtype=torch.float64)
+        lowest = max(0, n - (b - a) - window + 1) if window else 0         # entries of pages before it may have been given back
+        pages = tables[r][pos[lowest:] // page_size].long()
+        kv[lowest:] = (codes[pages, :, :, pos[lowest:] % page_size].double() + 0.5) * step_of(fields)[pages][..., None]
+        step = step_of(fields)[pages, 0].nan_to_num(0.0)
+        p = torch.arange(n - (b - a), n)[:, None]
+        seen = (pos <= p) & ((pos > p - window) if window else torch.ones((), dtype=torch.bool))
+        for h in range(heads * group):
+            x = q[a:b, h].double()
+            kvh, vis = kv[:, :, h // group], seen
+            s = torch.where(vis, (x @ kvh[:, 0].T) * scale, -math.inf)
+            w = torch.where(vis.any(1, keepdim=True), torch.softmax(s, 1), 0.0)
+            # a number that is not seen has no part, be it NaN
+            v = torch.where(vis[:, :, None], kvh[None, :, 1], 0.0)
+            out[a:b, h] = torch.einsum("tn,tnd->td", w.nan_to_num(0.0) if not torch.isnan(s[vis]).any() else w, v)
+            mag[a:b, h] = torch.einsum("tn,tnd->td", w, v.abs())
+            reach[a:b, h] = scale * x.abs().sum(1) * 256 * step[:, h // group].max()
+    return out, mag, reach
