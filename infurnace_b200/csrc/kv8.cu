@@ -159,6 +159,44 @@ kv8_values_kernel(const int8_t* codes, const uint8_t* exponents, T* out, long lo
   }
 }
 
+// The pages of the requests with more than `above` score rows as bfloat16 pages, for a kernel that reads those: the pages that a
+// request's keys lie in, one after the other over all such requests, and a table of them.  Exact, but for a block of NaN:
+// either kind's makes the page's keys NaN and its values 0, so that rows that do not see the page keep their numbers (a weight
+// of 0 times NaN would not be 0) and rows that see it are NaN.  Grid (pages of a request, 2 kinds, requests).
+__global__ void __launch_bounds__(256)
+kv8_expand_kernel(const int8_t* codes, const uint8_t* exponents, const int* tables, int table_stride, const int* cu_q, const int* seq_lens, bf16* out,
+                  int* out_tables, int out_pages, int heads, int group, int page_size, int dim, int window, int above) {
+  __shared__ int first_sum;
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  const int r = blockIdx.z, kind = blockIdx.y, p = blockIdx.x;
+  const int q_len = cu_q[r + 1] - cu_q[r], L = seq_lens[r];
+  if (q_len * group <= above || p * page_size >= L) return;
+  if (window > 0 && (p + 1) * page_size <= L - q_len - window + 1) return;
+  if (threadIdx.x < 32) {
+    int sum = 0;
+    for (int i = threadIdx.x; i < r; i += 32)
+      if ((cu_q[i + 1] - cu_q[i]) * group > above) sum += (max(0, seq_lens[i]) + page_size - 1) / page_size;
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (threadIdx.x == 0) first_sum = sum;
+  }
+  __syncthreads();
+  const int to = first_sum + p;
+  if (to >= out_pages) return;                                          // (more keys than the caller said)
+  const int page = tables[(size_t)r * table_stride + p];
+  if (kind == 0 && threadIdx.x == 0) out_tables[(size_t)r * gridDim.x + p] = to;
+  const uint8_t* fields = exponents + (size_t)page * 2 * heads;
+  const int per_head = page_size * dim / 16, total = heads * per_head;
+  const int8_t* src = codes + ((size_t)page * 2 + kind) * heads * page_size * dim;
+  bf16* dst = out + ((size_t)to * 2 + kind) * heads * page_size * dim;
+  for (int i = threadIdx.x; i < total; i += 256) {
+    const int h = i / per_head;
+    const bool nan = fields[h] == 255 || fields[heads + h] == 255;
+    const float step = nan ? (kind ? 0.f : __uint_as_float(0x7fffffffu)) : kv8_step(fields[kind * heads + h]);
+    kv8_write16<bf16>(dst + (size_t)i * 16, *reinterpret_cast<const uint4*>(src + (size_t)i * 16), step);
+  }
+}
+
 static int kv8_sizes(int heads, int page_size, int dim) {
   if (heads < 1 || heads > 32767 || page_size < 16 || page_size % 16 || page_size > 4096 || dim < 16 || dim % 16 || dim > 256) return IFB_ERR_SIZE;
   return IFB_OK;
@@ -197,4 +235,17 @@ IFB_EXPORT int ifb_kv8_values(const void* codes, const void* exponents, void* ou
                       (float*)out, pieces, per_block);
   return ifb_launch(kv8_values_kernel<bf16>, grid, dim3(256), 0, (cudaStream_t)stream, (const int8_t*)codes, (const uint8_t*)exponents,
                     (bf16*)out, pieces, per_block);
+}
+
+// out: bfloat16 [out_pages][2][heads][page_size][dim], out_tables: int32 [requests][max_pages].
+IFB_EXPORT int ifb_kv8_expand(const void* codes, const void* exponents, const void* tables, int table_stride, const void* cu_q, const void* seq_lens,
+                              void* out, void* out_tables, int out_pages, int requests, int max_pages, int heads, int group, int page_size, int dim,
+                              int window, int above, void* stream) {
+  const int bad = kv8_sizes(heads, page_size, dim);
+  if (bad) return bad;
+  if (requests < 1 || requests > 65535 || max_pages < 1 || out_pages < 1 || group < 1) return IFB_ERR_SIZE;
+  if ((((uintptr_t)codes) | ((uintptr_t)out)) & 15) return IFB_ERR_ALIGN;
+  return ifb_launch(kv8_expand_kernel, dim3(max_pages, 2, requests), dim3(256), 0, (cudaStream_t)stream, (const int8_t*)codes, (const uint8_t*)exponents,
+                    (const int*)tables, table_stride, (const int*)cu_q, (const int*)seq_lens, (bf16*)out, (int*)out_tables, out_pages, heads, group,
+                    page_size, dim, window, above);
 }

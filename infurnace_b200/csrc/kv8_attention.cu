@@ -142,9 +142,17 @@ template <int LEFT> struct Values {
       const uint32_t x = __byte_perm(v[0].word(i >> 1), v[1].word(i >> 1), sel), y = __byte_perm(v[2].word(i >> 1), v[3].word(i >> 1), sel);
       const uint32_t a0 = centred(even_bytes(x)), a1 = centred(odd_bytes(x)), a2 = centred(even_bytes(y)), a3 = centred(odd_bytes(y));
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t)
+      for (int n = 0; n < NT; ++n) {
+#if TERMS == 2
+        float x[4] = {0.f, 0.f, 0.f, 0.f};                              // (added up outside of the tensor core, as the scores are)
+        mma_f16(x, a0, a1, a2, a3, p[1][n][0], p[1][n][1]);
+        mma_f16(x, a0, a1, a2, a3, p[0][n][0], p[0][n][1]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16(o[i][n], a0, a1, a2, a3, p[t][n][0], p[t][n][1]);
+        for (int j = 0; j < 4; ++j) o[i][n][j] += x[j];
+#else
+        mma_f16(o[i][n], a0, a1, a2, a3, p[0][n][0], p[0][n][1]);
+#endif
+      }
     }
     rest.template multiply<NT>(o + W / 16, p);
   }
@@ -273,9 +281,18 @@ struct Stream {
       uint32_t a0 = even_bytes(k.word(0, ks)), a1 = even_bytes(k.word(1, ks)), a2 = odd_bytes(k.word(0, ks)), a3 = odd_bytes(k.word(1, ks));
       if (TERMS == 2) { a0 = centred(a0); a1 = centred(a1); a2 = centred(a2); a3 = centred(a3); }
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t)
+      for (int n = 0; n < NT; ++n) {
+#if TERMS == 2
+        // the tensor core's running sum is cut off, not rounded, at each step: a float32 score is added up outside of it
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_f16(x, a0, a1, a2, a3, qf[1][n][ks][0], qf[1][n][ks][1]);
+        mma_f16(x, a0, a1, a2, a3, qf[0][n][ks][0], qf[0][n][ks][1]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[t][n][ks][0], qf[t][n][ks][1]);
+        for (int j = 0; j < 4; ++j) s[n][j] += x[j];
+#else
+        mma_f16(s[n], a0, a1, a2, a3, qf[0][n][ks][0], qf[0][n][ks][1]);
+#endif
+      }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)

@@ -211,6 +211,7 @@ class LowBitKernels:
             lib.ifb_kv8_store.argtypes = [c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                           c_int, c_int, c_void_p]
             lib.ifb_kv8_values.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]
+            lib.ifb_kv8_expand.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p] + [c_int] * 9 + [c_void_p]
             self._kv8 = lib
         return self._kv8
 
@@ -284,6 +285,25 @@ class LowBitKernels:
                     self.scratch_generation += 1
         return held["graph" if capturing else stream]
 
+    kv8_expand_rows = 64             # score rows of the longest request from which prompts' pages are expanded for the tcgen05 kernel
+
+    def _kv8_attention_tc(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, n, r, heads, kv_heads,
+                          group):
+        """The requests with more than 16 score rows: their pages as bfloat16 (exact), and the tcgen05 kernel over those."""
+        most = -(-max_seq_len // pages.page_size)
+        room = most * min(r, n // (16 // group + 1))                      # a long request has so many tokens at least
+        device, ps, dim = q.device, pages.page_size, pages.head_dim
+        wide = torch.empty((room, 2, kv_heads, ps, dim), dtype=torch.bfloat16, device=device)
+        tables = torch.empty((r, most), dtype=torch.int32, device=device)
+        self.launches += 1
+        self._low_bit_status(self._kv8_lib().ifb_kv8_expand(*pages._at, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
+                                                            seq_lens.data_ptr(), wide.data_ptr(), tables.data_ptr(), room, r, most, kv_heads, group,
+                                                            ps, dim, int(window), 16, self._stream()), "kv8_attention")
+        at, stride = wide.data_ptr(), wide.stride(0)
+        self._attention_tc_streams(q.view(n, heads * dim) if q.is_contiguous() else q.as_strided((n, heads * dim), (q.stride(0), 1)),
+                                   heads, kv_heads, 1, dim, dim, (at, stride, ps), (at + 2 * kv_heads * ps * dim, stride, ps), room, tables, cu_q,
+                                   seq_lens, out, scale, int(window), max_q_len, n, r, 2, None, None, kind=0)
+
     KV8_SPLIT_REQUESTS = 1024        # the split form keeps their prefix sums in shared memory
 
     def kv8_attention(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, min_q_len=1):
@@ -318,6 +338,12 @@ class LowBitKernels:
         # score rows beyond which a request's tiles fill the device by themselves and run whole; requests below run split
         rows, least = max_q_len * group, min_q_len * group
         limit = 64 if r <= self.KV8_SPLIT_REQUESTS else 0
+        if self.kv8_expand_rows and rows > self.kv8_expand_rows and q.dtype == torch.bfloat16 and dim == 128 and 128 % group == 0 \
+                and pages.page_size in (16, 32, 64) and self.attention_tc:
+            self._kv8_attention_tc(q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, n, r, heads, kv_heads, group)
+            if least > 16:
+                return out
+            limit = rows = 16
         nt = 1 if rows <= 8 or dim > 128 else 2
         fixed = (q.data_ptr(), code, q.stride(0), *pages._at, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
                  seq_lens.data_ptr(), out.data_ptr())
