@@ -54,7 +54,6 @@ constexpr int WARPS = 4;
 constexpr int K64 = D / 64;              // pieces of 64 dimensions of a key that a quad of lanes takes 16 bytes a lane at a time
 constexpr int UNIT = 16 * WARPS;         // keys of a unit of the split form
 constexpr int NO_ROW = -1000000000;
-constexpr int KV8_MAX_REQUESTS = 1024;   // of the split form (their prefix sums lie in shared memory)
 
 struct Kv8Args {
   const qtype* q;
@@ -371,20 +370,23 @@ struct Stream {
                                       int lane) {
     if (first >= end) return;
     const size_t head_bytes = (size_t)a.page_size * D, page_bytes = 2 * (size_t)a.kv_heads * head_bytes;
-    const int per_page = a.page_size / 16;
+    // t / per_page by a product with the next whole number above 2^32 / per_page: exact for t below 2^32 / per_page
+    const uint32_t per_page = (uint32_t)a.page_size / 16, inverse = per_page > 1 ? 0xffffffffu / per_page + 1 : 0;
+    auto page_of = [&](int t) { return per_page > 1 ? (int)__umulhi((uint32_t)t, inverse) : t; };
+    const int8_t* const base = a.codes + (size_t)kv_head * head_bytes;
     auto tile_at = [&](int t, int page) {                               // the keys; the values lie kv_heads heads further
-      return a.codes + (size_t)page * page_bytes + (size_t)kv_head * head_bytes + (size_t)((t % per_page) * 16) * D;
+      return base + (size_t)page * page_bytes + (uint32_t)(t - page_of(t) * (int)per_page) * (16 * D);
     };
     const size_t v_off = (size_t)a.kv_heads * head_bytes;
     Keys k;
     Values<D> v;
-    int page = table[first / per_page];
+    int page = table[page_of(first)];
     const int8_t* at = tile_at(first, page);
     const uint8_t* fields = a.exponents + (size_t)page * 2 * a.kv_heads + kv_head;
     int kf = fields[0], vf = fields[a.kv_heads];
     k.load(at, lane);
     v.load(at + v_off, lane);
-    int next_page = first + step < end ? table[(first + step) / per_page] : page;
+    int next_page = first + step < end ? table[page_of(first + step)] : page;
     for (int t = first; t < end; t += step) {
       const bool more = t + step < end;
       float s[NT][4];
@@ -400,7 +402,7 @@ struct Stream {
         kf = nf[0];
         vf = nf[a.kv_heads];
         k.load(next, lane);
-        if (t + 2 * step < end) next_page = table[(t + 2 * step) / per_page];
+        if (t + 2 * step < end) next_page = table[page_of(t + 2 * step)];
       }
       if (whole) weigh<false>(s, v, vf_now);
       else weigh<true>(s, v, vf_now);
@@ -469,67 +471,94 @@ kv8_attention_whole_kernel(Kv8Args a) {
 
 // --------------------------------------------------------------------------------------------
 // Split form.  Items are (request, tile of 8 NT rows, key head), in that order; an item has the units of its request (those of
-// the request's last row: earlier tiles leave a few empty), one at least, so that a row without keys is written.
+// the request's last row: earlier tiles leave a few empty), one at least, so that a row without keys is written.  A piece is
+// no shorter than a 32nd of the longest item, so that few sums meet in one place.
 // --------------------------------------------------------------------------------------------
+constexpr int MAX_PARTS = 34;            // pieces of an item
+constexpr int PITCH = D + 8;             // of a row of sums in shared memory (the rows of a quad of lanes fall on two halves of the banks)
+// Where a warp's sums lie in a row: m tile by m tile, the lanes' pairs side by side.
+__device__ __forceinline__ int kv8_place(int i, int lane) { return i * 16 + (lane >> 2) * 2; }
+__device__ __forceinline__ int kv8_place_dim(int place) { return Values<D>::dim(place >> 4, ((place & 15) >> 1) << 2, 0); }
+
+struct Kv8Item { int r, before, units, tiles, q0, q_len, L; };
+
+// The request that has unit `at`, by a look over the requests' lengths (all lanes; every warp for itself).  at < 0: instead the
+// number of all units in `before` and the most units of an item in `units`.
+template <int ROWS>
+__device__ __forceinline__ Kv8Item kv8_find(const Kv8Args& a, int G, int at, int lane) {
+  Kv8Item it = {};
+  int before = 0, most = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += 32) {
+    const int r = r0 + lane;
+    int q0 = 0, q_len = 0, L = 0, units = 0, tiles = 0;
+    if (r < a.requests) {
+      q0 = a.cu_q[r]; q_len = a.cu_q[r + 1] - q0; L = a.seq_lens[r];
+      const int rows = q_len * G;
+      if (q_len > 0 && rows >= a.min_rows && rows <= a.max_rows) {
+        tiles = (rows + ROWS - 1) / ROWS;
+        const int lo = a.window > 0 ? max(0, L - q_len - a.window + 1) : 0;
+        units = L > 0 ? max(1, (L - 1) / UNIT - lo / UNIT + 1) : 1;
+      }
+    }
+    const int mine = units * tiles * a.kv_heads;
+    int x = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (at >= 0) {
+      const uint32_t hit = __ballot_sync(0xffffffffu, at < before + x);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        it.r = r0 + src;
+        it.before = before + __shfl_sync(0xffffffffu, x - mine, src);
+        it.units = __shfl_sync(0xffffffffu, units, src);
+        it.tiles = __shfl_sync(0xffffffffu, tiles, src);
+        it.q0 = __shfl_sync(0xffffffffu, q0, src);
+        it.q_len = __shfl_sync(0xffffffffu, q_len, src);
+        it.L = __shfl_sync(0xffffffffu, L, src);
+        return it;
+      }
+    }
+    most = max(most, units);
+    before += __shfl_sync(0xffffffffu, x, 31);
+  }
+  it.before = before;
+  it.units = __reduce_max_sync(0xffffffffu, most);
+  return it;
+}
+
 template <int NT>
 __global__ void __launch_bounds__(32 * WARPS)
 kv8_attention_split_kernel(Kv8Args a) {
   constexpr int ROWS = 8 * NT;
-  extern __shared__ __align__(16) float sums[];                         // [WARPS][ROWS][D], then maxima and sums [WARPS][ROWS] each
-  __shared__ int prefix[KV8_MAX_REQUESTS + 1];                          // units before a request
+  extern __shared__ __align__(16) float sums[];                         // [WARPS][ROWS][PITCH], then maxima and sums [WARPS][ROWS] each
+  __shared__ float factors[MAX_PARTS][ROWS], denominator[ROWS];
   __shared__ int arrived;
   ifb_pdl_wait();
   ifb_pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads;
-  float* const sm_m = sums + WARPS * ROWS * D;
+  float* const sm_m = sums + WARPS * ROWS * PITCH;
   float* const sm_l = sm_m + WARPS * ROWS;
-  auto shape = [&](int r, int& units, int& tiles) {                     // of a request: units of an item, tiles of rows
-    const int q_len = a.cu_q[r + 1] - a.cu_q[r], L = a.seq_lens[r], rows = q_len * G;
-    units = tiles = 0;
-    if (q_len <= 0 || rows < a.min_rows || rows > a.max_rows) return;
-    tiles = (rows + ROWS - 1) / ROWS;
-    const int lo = a.window > 0 ? max(0, L - q_len - a.window + 1) : 0;
-    units = L > 0 ? max(1, (L - 1) / UNIT - lo / UNIT + 1) : 1;
-  };
-  if (warp == 0) {
-    int before = 0;
-    for (int r0 = 0; r0 < a.requests; r0 += 32) {
-      int units = 0, tiles = 0;
-      if (r0 + lane < a.requests) shape(r0 + lane, units, tiles);
-      int x = units * tiles * a.kv_heads;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, d);
-        if (lane >= d) x += y;
-      }
-      if (r0 + lane < a.requests) prefix[r0 + lane + 1] = before + x;
-      before += __shfl_sync(0xffffffffu, x, 31);
-    }
-    if (lane == 0) prefix[0] = 0;
-  }
-  __syncthreads();
-  const int total = prefix[a.requests];
-  const int per = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  const Kv8Item all = kv8_find<ROWS>(a, G, -1, lane);
+  const int per = max(1, max((all.before + (int)gridDim.x - 1) / (int)gridDim.x, (all.units + 31) / 32));
   int at = (int)blockIdx.x * per;
-  const int end = min(total, at + per);
-  int r = 0;
+  const int end = min(all.before, at + per);
   while (at < end) {
-    while (prefix[r + 1] <= at) ++r;
-    int units, tiles;
-    shape(r, units, tiles);
-    const int in_request = at - prefix[r], item = in_request / units, unit0 = in_request - item * units;
-    const int n_units = min(units - unit0, end - at), tile = item / a.kv_heads, kv_head = item - tile * a.kv_heads;
-    const int q0 = a.cu_q[r], q_len = a.cu_q[r + 1] - q0, L = a.seq_lens[r], rows = q_len * G, row0 = tile * ROWS;
-    const int here = min(ROWS, rows - row0);
-    const int pos0 = L - q_len, p_first = pos0 + row0 / G, p_last = pos0 + (row0 + here - 1) / G;
+    const Kv8Item it = kv8_find<ROWS>(a, G, at, lane);
+    const int in_request = at - it.before, item = in_request / it.units, unit0 = in_request - item * it.units;
+    const int n_units = min(it.units - unit0, end - at), tile = item / a.kv_heads, kv_head = item - tile * a.kv_heads;
+    const int rows = it.q_len * G, row0 = tile * ROWS, here = min(ROWS, rows - row0);
+    const int pos0 = it.L - it.q_len, p_first = pos0 + row0 / G, p_last = pos0 + (row0 + here - 1) / G;
     const int lo_request = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
     const int key0 = (lo_request / UNIT + unit0) * UNIT;                // keys of this piece: up to n_units units from here
     const int key_end = min(p_last + 1, key0 + n_units * UNIT);
     Stream<NT> st;
     st.reset();
-    st.load_queries(a, q0, row0, rows, pos0, kv_head, G, lane);
+    st.load_queries(a, it.q0, row0, rows, pos0, kv_head, G, lane);
     const int first = max(key0, lo) / 16;
-    st.run(a, a.tables + (size_t)r * a.table_stride, kv_head, first + warp, key_end > 0 ? (key_end + 15) / 16 : 0, WARPS,
+    st.run(a, a.tables + (size_t)it.r * a.table_stride, kv_head, first + warp, key_end > 0 ? (key_end + 15) / 16 : 0, WARPS,
            a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
     st.finish();
     // the warps' sums side by side
@@ -539,60 +568,78 @@ kv8_attention_split_kernel(Kv8Args a) {
       for (int e = 0; e < 2; ++e) {
         const int row = n * 8 + (lane & 3) * 2 + e;
         if (row < here) {
-          float* to = sums + ((size_t)warp * ROWS + row) * D;
+          float* to = sums + (warp * ROWS + row) * PITCH;
 #pragma unroll
-          for (int i = 0; i < KS; ++i) kv8_store_pair(to + Values<D>::dim(i, lane, 0), st.o[i][n][e], st.o[i][n][2 + e]);
+          for (int i = 0; i < KS; ++i) *reinterpret_cast<float2*>(to + kv8_place(i, lane)) = make_float2(st.o[i][n][e], st.o[i][n][2 + e]);
           if (lane < 4) { sm_m[warp * ROWS + row] = st.m[n][e]; sm_l[warp * ROWS + row] = st.l[n][e]; }
         }
       }
     __syncthreads();
-    const bool alone = n_units == units;
+    const bool alone = n_units == it.units;
     // a piece's place in scratch memory: a CTA has at most two that are not whole items, its first and its last
     float* const mine = a.parts + ((size_t)blockIdx.x * 2 + (unit0 ? 0 : 1)) * ROWS * (D + 2);
-    for (int i = tid; i < here * D; i += 32 * WARPS) {
-      const int row = i / D, d = i - row * D;
+    for (int i = tid; i < here * (D / 2); i += 32 * WARPS) {
+      const int row = i / (D / 2), place = (i - row * (D / 2)) * 2;
       float M = -INFINITY;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_m[w * ROWS + row]);
       const float U = M == -INFINITY ? 0.f : M;
-      float o = 0.f, l = 0.f;
+      float2 o = make_float2(0.f, 0.f);
+      float l = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float f = exp2f(sm_m[w * ROWS + row] - U);
-        o += sums[((size_t)w * ROWS + row) * D + d] * f;
-        l += sm_l[w * ROWS + row] * f;
+        const float f = kv8_exp2(sm_m[w * ROWS + row] - U);
+        const float2 x = *reinterpret_cast<const float2*>(sums + (w * ROWS + row) * PITCH + place);
+        o.x = fmaf(x.x, f, o.x);
+        o.y = fmaf(x.y, f, o.y);
+        l = fmaf(sm_l[w * ROWS + row], f, l);
       }
       if (alone) {
         const int full = row0 + row;
-        a.out[((size_t)(q0 + full / G) * a.heads + kv_head * G + full % G) * D + d] = from_f32<qtype>(kv8_ratio(o, l));
+        kv8_store_pair(a.out + ((size_t)(it.q0 + full / G) * a.heads + kv_head * G + full % G) * D + kv8_place_dim(place), kv8_ratio(o.x, l), kv8_ratio(o.y, l));
       } else {
-        mine[row * (D + 2) + d] = o;
-        if (d == 0) { mine[row * (D + 2) + D] = M; mine[row * (D + 2) + D + 1] = l; }
+        *reinterpret_cast<float2*>(mine + row * D + place) = o;
+        if (place == 0) { mine[ROWS * D + row] = M; mine[ROWS * (D + 1) + row] = l; }
       }
     }
     if (!alone) {
       __threadfence();
       __syncthreads();
-      const int first_unit = prefix[r] + item * units, first_cta = first_unit / per, last_cta = (first_unit + units - 1) / per;
-      int* const counter = a.counters + ((size_t)r * a.tiles + tile) * a.kv_heads + kv_head;
+      const int first_unit = it.before + item * it.units, first_cta = first_unit / per, parts = (first_unit + it.units - 1) / per - first_cta + 1;
+      int* const counter = a.counters + ((size_t)it.r * a.tiles + tile) * a.kv_heads + kv_head;
       if (tid == 0) arrived = atomicAdd(counter, 1);
       __syncthreads();
-      if (arrived == last_cta - first_cta) {                            // the last of the item's pieces
+      if (arrived == parts - 1) {                                       // the last of the item's pieces
         __threadfence();
-        for (int i = tid; i < here * D; i += 32 * WARPS) {
-          const int row = i / D, d = i - row * D;
-          float M = -INFINITY, o = 0.f, l = 0.f;
-          for (int c = first_cta; c <= last_cta; ++c)
-            M = fmaxf(M, __ldcg(a.parts + ((size_t)c * 2 + (c == first_cta ? 1 : 0)) * ROWS * (D + 2) + row * (D + 2) + D));
+        auto part = [&](int c) { return a.parts + ((size_t)(first_cta + c) * 2 + (c == 0 ? 1 : 0)) * ROWS * (D + 2); };
+        for (int i = tid; i < here * parts; i += 32 * WARPS) factors[i / here][i % here] = __ldcg(part(i / here) + ROWS * D + i % here);
+        __syncthreads();
+        if (tid < here) {
+          float M = -INFINITY, l = 0.f;
+          for (int c = 0; c < parts; ++c) M = fmaxf(M, factors[c][tid]);
           const float U = M == -INFINITY ? 0.f : M;
-          for (int c = first_cta; c <= last_cta; ++c) {
-            const float* part = a.parts + ((size_t)c * 2 + (c == first_cta ? 1 : 0)) * ROWS * (D + 2) + row * (D + 2);
-            const float f = exp2f(__ldcg(part + D) - U);
-            o += __ldcg(part + d) * f;
-            l += __ldcg(part + D + 1) * f;
+#pragma unroll 4
+          for (int c = 0; c < parts; ++c) {
+            const float f = kv8_exp2(factors[c][tid] - U);
+            factors[c][tid] = f;
+            l = fmaf(__ldcg(part(c) + ROWS * (D + 1) + tid), f, l);
+          }
+          denominator[tid] = l;
+        }
+        __syncthreads();
+        for (int i = tid; i < here * (D / 2); i += 32 * WARPS) {
+          const int row = i / (D / 2), place = (i - row * (D / 2)) * 2;
+          float2 o = make_float2(0.f, 0.f);
+#pragma unroll 8
+          for (int c = 0; c < parts; ++c) {
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(part(c) + row * D + place));
+            const float f = factors[c][row];
+            o.x = fmaf(x.x, f, o.x);
+            o.y = fmaf(x.y, f, o.y);
           }
           const int full = row0 + row;
-          a.out[((size_t)(q0 + full / G) * a.heads + kv_head * G + full % G) * D + d] = from_f32<qtype>(kv8_ratio(o, l));
+          const float l = denominator[row];
+          kv8_store_pair(a.out + ((size_t)(it.q0 + full / G) * a.heads + kv_head * G + full % G) * D + kv8_place_dim(place), kv8_ratio(o.x, l), kv8_ratio(o.y, l));
         }
         if (tid == 0) *counter = 0;
       }
@@ -602,7 +649,7 @@ kv8_attention_split_kernel(Kv8Args a) {
   }
 }
 
-template <int NT> static size_t kv8_split_smem() { return (size_t)WARPS * 8 * NT * (D + 2) * sizeof(float); }
+template <int NT> static size_t kv8_split_smem() { return (size_t)WARPS * 8 * NT * (PITCH + 2) * sizeof(float); }
 template <int NT> static int kv8_split_ctas(int* ctas) {                // that fit on the device at once
   static int known[IFB_MAX_DEVICES] = {};
   int dev = 0, per = 0;
@@ -646,7 +693,7 @@ IFB_EXPORT int ifb_kv8_attention(const void* q, int dtype, long long q_row, cons
   if (dim != D || heads < 1 || kv_heads < 1 || heads % kv_heads || page_size < 16 || page_size % 16 || requests < 1 || max_q < 1 || window < 0 ||
       (nt != 1 && nt != 2) || kv_heads > 65535 || requests > 65535)
     return IFB_ERR_SIZE;
-  if (!whole && (requests > KV8_MAX_REQUESTS || !parts || !counters || tiles < 1)) return IFB_ERR_ARG;
+  if (!whole && (!parts || !counters || tiles < 1)) return IFB_ERR_ARG;
   if ((((uintptr_t)q) | ((uintptr_t)codes) | ((uintptr_t)out) | (uintptr_t)(q_row * sizeof(qtype))) & 15) return IFB_ERR_ALIGN;
   const Kv8Args a = {(const qtype*)q, q_row, (const int8_t*)codes, (const uint8_t*)exponents, (const int*)tables, table_stride, (const int*)cu_q,
                      (const int*)seq_lens, (qtype*)out, (float*)parts, (int*)counters, requests, heads, kv_heads, page_size, window,

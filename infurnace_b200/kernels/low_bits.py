@@ -304,8 +304,6 @@ class LowBitKernels:
                                    heads, kv_heads, 1, dim, dim, (at, stride, ps), (at + 2 * kv_heads * ps * dim, stride, ps), room, tables, cu_q,
                                    seq_lens, out, scale, int(window), max_q_len, n, r, 2, None, None, kind=0)
 
-    KV8_SPLIT_REQUESTS = 1024        # the split form keeps their prefix sums in shared memory
-
     def kv8_attention(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, min_q_len=1):
         """Causal attention of a step's queries over 8-bit pages: ``q`` and ``out`` bfloat16 or float32 [tokens, heads, head_dim] (the
         rows of ``q`` may lie apart, those of ``out`` not); the query at position p sees positions max(0, p - window + 1) .. p
@@ -337,7 +335,7 @@ class LowBitKernels:
         lib, stream, group = self._kv8_attention_lib(dim, q.dtype), self._stream(), heads // kv_heads
         # score rows beyond which a request's tiles fill the device by themselves and run whole; requests below run split
         rows, least = max_q_len * group, min_q_len * group
-        limit = 64 if r <= self.KV8_SPLIT_REQUESTS else 0
+        limit = 64
         if self.kv8_expand_rows and rows > self.kv8_expand_rows and q.dtype == torch.bfloat16 and dim == 128 and 128 % group == 0 \
                 and pages.page_size in (16, 32, 64) and self.attention_tc:
             self._kv8_attention_tc(q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, n, r, heads, kv_heads, group)
