@@ -125,9 +125,9 @@ struct IfbMapKey {
   const void* ptr;
   unsigned long long dims[3], strides[2];
   unsigned box[3];
-  int rank;
+  int rank, plain;
   bool operator==(const IfbMapKey& o) const {
-    return ptr == o.ptr && rank == o.rank && dims[0] == o.dims[0] && dims[1] == o.dims[1] && dims[2] == o.dims[2] &&
+    return ptr == o.ptr && rank == o.rank && plain == o.plain && dims[0] == o.dims[0] && dims[1] == o.dims[1] && dims[2] == o.dims[2] &&
            strides[0] == o.strides[0] && strides[1] == o.strides[1] && box[0] == o.box[0] && box[1] == o.box[1] && box[2] == o.box[2];
   }
 };
@@ -135,16 +135,16 @@ typedef CUresult (*IfbEncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32
                                      const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                      CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 // A bfloat16 tensor of rank 2 or 3 (dims and box innermost first, strides in bytes for dims 1..rank-1), 128-byte
-// swizzle, zeros outside.  Returns IFB_OK or IFB_ERR_ARG.
+// swizzle (plain: none), zeros outside.  Returns IFB_OK or IFB_ERR_ARG.
 static inline int ifb_tensor_map_bf16(CUtensorMap* out, const void* ptr, int rank, const unsigned long long* dims,
-                                      const unsigned long long* strides, const unsigned* box) {
+                                      const unsigned long long* strides, const unsigned* box, bool plain = false) {
   constexpr int SLOTS = 4096;
   static IfbMapKey keys[SLOTS];
   static CUtensorMap maps[SLOTS];
   static bool used[SLOTS];
   static IfbEncodeTiledFn enc = nullptr;
   IfbMapKey k = {};
-  k.ptr = ptr; k.rank = rank;
+  k.ptr = ptr; k.rank = rank; k.plain = plain;
   for (int i = 0; i < rank; ++i) { k.dims[i] = dims[i]; k.box[i] = box[i]; }
   for (int i = 0; i + 1 < rank; ++i) k.strides[i] = strides[i];
   unsigned long long h = (unsigned long long)(uintptr_t)ptr * 0x9E3779B97F4A7C15ull;
@@ -167,7 +167,7 @@ static inline int ifb_tensor_map_bf16(CUtensorMap* out, const void* ptr, int ran
   for (int i = 0; i + 1 < rank; ++i) st[i] = strides[i];
   CUtensorMap m;
   if (enc(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(ptr), d, st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+          plain ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return IFB_ERR_ARG;
   if (!used[slot]) { keys[slot] = k; maps[slot] = m; used[slot] = true; }      // a full neighbourhood: encode every time
   *out = m;

@@ -289,12 +289,26 @@ struct MxProduct {
   int rows, k, w_rows, out_features, unary, per_split;                 // per_split: stages of a CTA
 };
 
-// y: the activation of a pair's gate times its up; else the unary function.
-__device__ __forceinline__ float mx_gate(float g, float u, int unary) { return ifb_gate_act(g, unary) * u; }
+// What becomes of a sum.  The function is chosen at compile time, or is one call: copies of every function's code for every
+// element of an unrolled loop are fetched by every SM (33 rows of gated 4,096 x 12,288: 38 us for 16).
+//   MX_PLAIN: nothing; MX_SILU: silu(gate) * up with the hardware's exp2 and reciprocal (relative error about 2^-21; outputs of
+//   16 bits); MX_UNARY, MX_GATED: any function of common.cuh.
+enum { MX_PLAIN, MX_SILU, MX_UNARY, MX_GATED };
+__device__ __noinline__ float mx_unary_call(float y, int kind) { return ifb_unary(y, kind); }
+__device__ __noinline__ float mx_gate_call(float g, int kind) { return ifb_gate_act(g, kind); }
+template <int EPI> __device__ __forceinline__ float mx_gate(float g, float u, int unary) {
+  if (EPI == MX_GATED) return mx_gate_call(g, unary) * u;
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e) : "f"(-1.4426950408889634f * g));
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(1.f + e));
+  return g * r * u;
+}
+template <int EPI> __device__ __forceinline__ float mx_apply(float y, int unary) { return EPI == MX_UNARY ? mx_unary_call(y, unary) : y; }
 
-template <typename C, bool GATED, typename TO>
+template <typename C, int EPI, typename TO>
 __global__ void __launch_bounds__(C::THREADS)
 mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, MxProduct p, int* err) {
+  constexpr bool GATED = EPI == MX_SILU || EPI == MX_GATED;
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ uint64_t full[C::STAGES], empty[C::STAGES], ready;
   __shared__ uint32_t tmem_slot;
@@ -399,15 +413,15 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
         for (int j = 0; j < 16; j += 2) {
           const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[j] : v[j + 1], 1);
           const int token = n0 + c + j + (lane & 1);
-          const float y = lane & 1 ? mx_gate(__uint_as_float(other), __uint_as_float(v[j + 1]), p.unary)
-                                   : mx_gate(__uint_as_float(v[j]), __uint_as_float(other), p.unary);
+          const float y = lane & 1 ? mx_gate<EPI>(__uint_as_float(other), __uint_as_float(v[j + 1]), p.unary)
+                                   : mx_gate<EPI>(__uint_as_float(v[j]), __uint_as_float(other), p.unary);
           if (row < p.w_rows && token < p.rows) out[(size_t)token * p.out_features + (row >> 1)] = from_f32<TO>(y);
         }
       } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (row < p.w_rows && n0 + c + j < p.rows)
-            out[(size_t)(n0 + c + j) * p.out_features + row] = from_f32<TO>(ifb_unary(__uint_as_float(v[j]), p.unary));
+            out[(size_t)(n0 + c + j) * p.out_features + row] = from_f32<TO>(mx_apply<EPI>(__uint_as_float(v[j]), p.unary));
       }
     }
   }
@@ -440,10 +454,10 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
       }
       TO* to = out + (size_t)(n0 + token) * p.out_features;
       if (GATED) {
-        if (row < p.w_rows) to[row >> 1] = from_f32<TO>(mx_gate(a, b, p.unary));
+        if (row < p.w_rows) to[row >> 1] = from_f32<TO>(mx_gate<EPI>(a, b, p.unary));
       } else {
-        if (row < p.w_rows) to[row] = from_f32<TO>(ifb_unary(a, p.unary));
-        if (row + 1 < p.w_rows) to[row + 1] = from_f32<TO>(ifb_unary(b, p.unary));
+        if (row < p.w_rows) to[row] = from_f32<TO>(mx_apply<EPI>(a, p.unary));
+        if (row + 1 < p.w_rows) to[row + 1] = from_f32<TO>(mx_apply<EPI>(b, p.unary));
       }
     }
     asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
@@ -458,9 +472,9 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
   }
 }
 
-template <typename C, bool GATED, typename TO>
+template <typename C, int EPI, typename TO>
 static int mx_launch(const CUtensorMap& xm, const CUtensorMap& wm, const MxProduct& p, int splits, int* err, cudaStream_t stream) {
-  auto kernel = mx4_linear_kernel<C, GATED, TO>;
+  auto kernel = mx4_linear_kernel<C, EPI, TO>;
   IFB_ALLOW_SMEM(kernel, C::SMEM);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.w_rows + 127) / 128, (p.rows + C::NT - 1) / C::NT, splits);
@@ -481,8 +495,240 @@ static int mx_launch(const CUtensorMap& xm, const CUtensorMap& wm, const MxProdu
 template <typename C>
 static int mx_launch_any(const CUtensorMap& xm, const CUtensorMap& wm, const MxProduct& p, bool gated, int dtype, int splits, int* err,
                          cudaStream_t stream) {
-  if (gated) return dtype == IFB_F32 ? mx_launch<C, true, float>(xm, wm, p, splits, err, stream) : mx_launch<C, true, bf16>(xm, wm, p, splits, err, stream);
-  return dtype == IFB_F32 ? mx_launch<C, false, float>(xm, wm, p, splits, err, stream) : mx_launch<C, false, bf16>(xm, wm, p, splits, err, stream);
+  if (dtype == IFB_F32) {
+    if (gated) return mx_launch<C, MX_GATED, float>(xm, wm, p, splits, err, stream);
+    return p.unary ? mx_launch<C, MX_UNARY, float>(xm, wm, p, splits, err, stream) : mx_launch<C, MX_PLAIN, float>(xm, wm, p, splits, err, stream);
+  }
+  if (gated) return p.unary ? mx_launch<C, MX_GATED, bf16>(xm, wm, p, splits, err, stream) : mx_launch<C, MX_SILU, bf16>(xm, wm, p, splits, err, stream);
+  return p.unary ? mx_launch<C, MX_UNARY, bf16>(xm, wm, p, splits, err, stream) : mx_launch<C, MX_PLAIN, bf16>(xm, wm, p, splits, err, stream);
+}
+
+// ---------------------------------------------------------------------------------------------
+// The product of many rows, over pairs of SMs: a cluster of two CTAs owns 256 rows of w by 256 tokens.  Each CTA brings 128 rows
+// of either operand (and the scales of its rows of w and of all 256 tokens), one tcgen05.mma of the pair (M = 256), issued by the
+// first CTA, multiplies out of both shared memories into both tensor memories, where a CTA finds its 128 rows of w.  What bounds
+// these products is the bytes that reach an SM: 8 KB for the 128 cycles of 128 x 256 x 64, where a CTA alone would bring 12.
+// Persistent, one accumulator (the scales leave no room for two): the epilogue's warps take it to registers at once (256
+// columns in some hundred cycles) and let the next tile's products begin, which run while they finish and store.
+// The "full" barriers are the first CTA's and count both CTAs' bytes; "empty" and "accumulator ready" are each CTA's own, by
+// multicast commits; "accumulator read" is the first CTA's and counts all sixteen warps.
+// ---------------------------------------------------------------------------------------------
+constexpr int MXP_STAGES = 5;
+constexpr int MXP_B = MX_A_BYTES, MXP_SA = 2 * MX_A_BYTES, MXP_SB = MXP_SA + 1024, MXP_STAGE = MXP_SB + 2048;      // where things lie in a stage
+constexpr int MXP_SMEM = MXP_STAGES * MXP_STAGE + 1024;
+constexpr int MXP_S_COLS = 24, MXP_TMEM = 512, MXP_THREADS = 320;
+static_assert(256 + MXP_STAGES * MXP_S_COLS <= MXP_TMEM && MXP_STAGE % 1024 == 0 && MXP_SMEM <= 227 * 1024, "pair sizes");
+constexpr uint32_t MXP_IDESC = (1u << 7) | (1u << 10) | ((uint32_t)(256 >> 3) << 17) | (1u << 23) | ((uint32_t)(256 >> 4) << 24);
+
+__device__ __forceinline__ uint32_t mx_peer(const void* p, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(mx_smem(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void mx_tma_pair(uint32_t smem, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
+               ::"r"(smem), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void mx_copy_scales_pair(uint32_t tmem, uint32_t smem) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(mx_scale_desc(smem)) : "memory");
+}
+__device__ __forceinline__ void mx_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+               " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mx_commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+               ::"r"(mx_smem(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void mx_tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr) : "memory");
+}
+
+template <int EPI, typename TO>
+__global__ void __launch_bounds__(MXP_THREADS, 1)
+mx4_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap xs_map,
+                const __grid_constant__ CUtensorMap ws_map, MxProduct p, int token_tiles, int tiles, int* err) {
+  constexpr bool GATED = EPI == MX_SILU || EPI == MX_GATED;
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ uint64_t full[MXP_STAGES], empty[MXP_STAGES], acc_full, acc_empty;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const uint32_t base = (mx_smem(raw) + 1023u) & ~1023u;                // the same offset in both CTAs
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, rank = blockIdx.x & 1;
+  const int stages = (p.k + MX_KSTAGE - 1) / MX_KSTAGE, k_tiles = (p.k + 127) / 128;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < MXP_STAGES; ++i) { mx_mbar_init(&full[i], 1); mx_mbar_init(&empty[i], 1); }
+    mx_mbar_init(&acc_full, 1);
+    mx_mbar_init(&acc_empty, 16);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(mx_smem(&tmem_slot)), "r"(MXP_TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");      // both CTAs' barriers exist
+  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const uint32_t tmem = *(volatile uint32_t*)&tmem_slot;
+
+  if (warp == 0) {
+    // producer, in both CTAs; the matrix of the first tile's first stages before the wait for the kernel that rounds the rows
+    auto load_w = [&](int t, int s, int i) {
+      const uint32_t at = base + i * MXP_STAGE, bar = mx_peer(&full[i], 0);
+      const int o0 = t / token_tiles * 256 + rank * 128;
+      if (rank == 0) mx_expect_tx(&full[i], 2 * MXP_STAGE);
+      mx_tma_pair(at, &w_map, bar, s * 64, o0);
+      mx_tma_pair(at + MXP_SA, &ws_map, bar, 0, (o0 >> 7) * k_tiles + 2 * s);
+    };
+    auto load_x = [&](int t, int s, int i) {
+      const uint32_t at = base + i * MXP_STAGE, bar = mx_peer(&full[i], 0);
+      const int n0 = t % token_tiles * 256;
+      mx_tma_pair(at + MXP_B, &x_map, bar, s * 64, n0 + rank * 128);
+      mx_tma_pair(at + MXP_SB, &xs_map, bar, 0, (n0 >> 7) * k_tiles + 2 * s);
+      mx_tma_pair(at + MXP_SB + 1024, &xs_map, bar, 0, ((n0 >> 7) + 1) * k_tiles + 2 * s);
+    };
+    const int ahead = first < tiles ? min(MXP_STAGES, stages) : 0;
+    if (mx_elect())
+      for (int i = 0; i < ahead; ++i) load_w(first, i, i);
+    __syncwarp();
+    ifb_pdl_wait();
+    ifb_pdl_trigger();
+    if (mx_elect())
+      for (int i = 0; i < ahead; ++i) load_x(first, i, i);
+    __syncwarp();
+    int g = 0;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step)
+      for (int s = 0; s < stages; ++s, ++g) {
+        if (g < ahead) continue;
+        const int i = g % MXP_STAGES;
+        if (g >= MXP_STAGES && !mx_wait(&empty[i], ((g / MXP_STAGES) & 1) ^ 1, abort_flag, err, 711)) { ok = false; break; }
+        if (mx_elect()) { load_w(t, s, i); load_x(t, s, i); }
+        __syncwarp();
+      }
+  } else if (warp == 1) {
+    bool ok = rank == 0;
+    int g = 0, n = 0;
+    for (int t = first; t < tiles && ok; t += step, ++n) {
+      if (n > 0) ok = mx_wait(&acc_empty, (n - 1) & 1, abort_flag, err, 714);
+      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      for (int s = 0; s < stages && ok; ++s, ++g) {
+        const int i = g % MXP_STAGES;
+        ok = mx_wait(&full[i], (g / MXP_STAGES) & 1, abort_flag, err, 712);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        if (mx_elect()) {
+          const uint32_t at = base + i * MXP_STAGE, sc = tmem + 256 + i * MXP_S_COLS;
+          const int products = min(4, (p.k - s * MX_KSTAGE + 63) / 64);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (2 * h < products) {
+              mx_copy_scales_pair(sc + h * 4, at + MXP_SA + h * 512);
+              mx_copy_scales_pair(sc + 8 + h * 8, at + MXP_SB + h * 512);
+              mx_copy_scales_pair(sc + 8 + h * 8 + 4, at + MXP_SB + 1024 + h * 512);
+            }
+          const uint64_t a = mx_desc(at), b = mx_desc(at + MXP_B);
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            if (m < products) {
+              const uint32_t id = (uint32_t)(m & 1) * 2;
+              mx_mma_pair(tmem, a + m * 2, b + m * 2, MXP_IDESC | (id << 4) | (id << 29), sc + (m >> 1) * 4, sc + 8 + (m >> 1) * 8, (s | m) != 0);
+            }
+          mx_commit_pair(&empty[i]);
+          if (s == stages - 1) mx_commit_pair(&acc_full);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    TO* out = (TO*)p.out;
+    int n = 0;
+    ifb_pdl_wait();                                                     // (the kernel before may still read what this one writes)
+    for (int t = first; t < tiles; t += step, ++n) {
+      const int row = t / token_tiles * 256 + rank * 128 + quarter * 32 + lane, n0 = t % token_tiles * 256 + half * 128;
+      const bool ok = __all_sync(0xffffffffu, mx_wait(&acc_full, n & 1, abort_flag, err, 713)) != 0;
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      uint32_t v[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) mx_tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + half * 128 + c * 32, v + c * 32);
+      asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        const uint32_t bar = mx_peer(&acc_empty, 0);
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+      }
+      TO* to = out + (size_t)n0 * p.out_features;
+#pragma unroll
+      for (int j = 0; j < 128; j += 2) {
+        if (GATED) {
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[j] : v[j + 1], 1);
+          const float y = lane & 1 ? mx_gate<EPI>(__uint_as_float(other), __uint_as_float(v[j + 1]), p.unary)
+                                   : mx_gate<EPI>(__uint_as_float(v[j]), __uint_as_float(other), p.unary);
+          if (row < p.w_rows && n0 + j + (lane & 1) < p.rows) to[(size_t)(j + (lane & 1)) * p.out_features + (row >> 1)] = from_f32<TO>(y);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (row < p.w_rows && n0 + j + e < p.rows) to[(size_t)(j + e) * p.out_features + row] = from_f32<TO>(mx_apply<EPI>(__uint_as_float(v[j + e]), p.unary));
+        }
+      }
+    }
+  }
+  if (*abort_flag) for (int i = 0; i < 2000; ++i) __nanosleep(1000);    // copies in flight land
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");      // neither CTA leaves while the other needs its memory
+  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(MXP_TMEM) : "memory");
+  }
+}
+
+template <int EPI, typename TO>
+static int mx_launch_pair(const CUtensorMap (&m)[4], const MxProduct& p, int* err, cudaStream_t stream) {
+  auto kernel = mx4_pair_kernel<EPI, TO>;
+  IFB_ALLOW_SMEM(kernel, MXP_SMEM);
+  const int token_tiles = (p.rows + 255) / 256, tiles = token_tiles * ((p.w_rows + 255) / 256), pairs = ifb_sm_count() / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (tiles < pairs ? tiles : pairs));
+  cfg.blockDim = dim3(MXP_THREADS);
+  cfg.dynamicSmemBytes = MXP_SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ifb_pdl_enabled() ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, m[0], m[1], m[2], m[3], p, token_tiles, tiles, err);
+  if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
+  return IFB_OK;
+}
+static int mx_launch_pair_any(const CUtensorMap (&m)[4], const MxProduct& p, bool gated, int dtype, int* err, cudaStream_t stream) {
+  if (dtype == IFB_F32) {
+    if (gated) return mx_launch_pair<MX_GATED, float>(m, p, err, stream);
+    return p.unary ? mx_launch_pair<MX_UNARY, float>(m, p, err, stream) : mx_launch_pair<MX_PLAIN, float>(m, p, err, stream);
+  }
+  if (gated) return p.unary ? mx_launch_pair<MX_GATED, bf16>(m, p, err, stream) : mx_launch_pair<MX_SILU, bf16>(m, p, err, stream);
+  return p.unary ? mx_launch_pair<MX_UNARY, bf16>(m, p, err, stream) : mx_launch_pair<MX_PLAIN, bf16>(m, p, err, stream);
 }
 
 // x: [rows][k], w: [w_rows][k] (twice the out features if the epilogue is gated), both microscaled.  epilogue: as in the other products.
@@ -496,29 +742,39 @@ IFB_EXPORT int ifb_mx4_linear(const void* x_codes, const void* x_scales, const v
   if ((epilogue & 14) || unary > IFB_UNARY_LAST) return IFB_ERR_ARG;
   if (out_dtype != IFB_F32 && out_dtype != IFB_BF16) return IFB_ERR_DTYPE;
   if ((((uintptr_t)x_codes) | ((uintptr_t)x_scales) | ((uintptr_t)w_codes) | ((uintptr_t)w_scales)) & 15) return IFB_ERR_ALIGN;
-  const int nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-  const int stages = (k + MX_KSTAGE - 1) / MX_KSTAGE, tiles = (w_rows + 127) / 128;
+  const bool pair = rows > 256;
+  const int nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  const int stages = (k + MX_KSTAGE - 1) / MX_KSTAGE, tiles = (w_rows + 127) / 128 * ((rows + nt - 1) / nt);
   // the k range is shared where tiles leave SMs idle
   int splits = 1;
-  if (nt <= 128) while (splits < 8 && splits * 2 <= stages && tiles * splits * 2 <= ifb_sm_count() + 8) splits *= 2;
+  while (splits < 8 && splits * 2 <= stages && tiles * splits * 2 <= ifb_sm_count() + 8) splits *= 2;
   MxProduct p = {(const uint8_t*)x_scales, (const uint8_t*)w_scales, out, rows, k, w_rows, gated ? w_rows / 2 : w_rows, unary,
                  (stages + splits - 1) / splits};
   splits = (stages + p.per_split - 1) / p.per_split;                   // every CTA has a stage
   // the maps see pairs of bytes as one number of 16 bits: only widths and strides in bytes count
   const unsigned long long xd[2] = {(unsigned long long)k / 4, (unsigned long long)rows}, xs[1] = {(unsigned long long)k / 2};
   const unsigned long long wd[2] = {(unsigned long long)k / 4, (unsigned long long)w_rows}, ws[1] = {(unsigned long long)k / 2};
-  const unsigned xb[2] = {64, (unsigned)nt}, wb[2] = {64, 128};
+  const unsigned xb[2] = {64, pair ? 128u : (unsigned)nt}, wb[2] = {64, 128};
   CUtensorMap xm, wm;
   bad = ifb_tensor_map_bf16(&xm, x_codes, 2, xd, xs, xb);
   if (!bad) bad = ifb_tensor_map_bf16(&wm, w_codes, 2, wd, ws, wb);
   if (bad) return bad;
   cudaStream_t st = (cudaStream_t)stream;
   int* e = (int*)err;
+  if (pair) {
+    // scale tiles as rows of 512 bytes
+    const unsigned long long k_tiles = (unsigned long long)(k + 127) / 128, sd[1] = {512};
+    const unsigned long long xsd[2] = {256, k_tiles * 2 * ((rows + 255) / 256)}, wsd[2] = {256, k_tiles * 2 * ((w_rows + 255) / 256)};
+    const unsigned sb[2] = {256, 2};
+    CUtensorMap m[4] = {xm, wm};
+    bad = ifb_tensor_map_bf16(&m[2], x_scales, 2, xsd, sd, sb, true);
+    if (!bad) bad = ifb_tensor_map_bf16(&m[3], w_scales, 2, wsd, sd, sb, true);
+    return bad ? bad : mx_launch_pair_any(m, p, gated, out_dtype, e, st);
+  }
   switch (nt) {
     case 16: return mx_launch_any<MxCfg<16, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
     case 32: return mx_launch_any<MxCfg<32, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
     case 64: return mx_launch_any<MxCfg<64, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
-    case 128: return mx_launch_any<MxCfg<128, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
-    default: return mx_launch_any<MxCfg<256, 4>>(xm, wm, p, gated, out_dtype, splits, e, st);
+    default: return mx_launch_any<MxCfg<128, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
   }
 }
