@@ -12,6 +12,7 @@
 // rows stays inside.  A gated matrix (gate rows [0, O), up rows [O, 2 O)) keeps row i of the gate in row 2 i and row i of the
 // up half in row 2 i + 1: the two numbers of an output then lie in neighbouring lanes of the accumulator.
 #include <cuda.h>
+#include <type_traits>
 #include "common.cuh"
 
 typedef __nv_bfloat16 bf16;
@@ -197,6 +198,9 @@ IFB_EXPORT int ifb_mx4_values(const void* codes, const void* scales, void* out, 
 // SPLITS: where tiles are few, the k range of a tile is shared by a cluster of CTAs along z, which add their accumulators
 // through distributed shared memory in the order of their ranks.
 // What does not depend on the kernel before this one, the matrix, is requested before the wait for it.
+// ROUND: the rows come as numbers, and the epilogue's warps, idle until then, round a stage's 256 of k of them (a thread a block
+// of 32) into the stage, where TMA would have put them: every CTA rounds all rows of its part of k, which for few rows is little
+// beside its part of the matrix, and a launch and a trip through memory are saved.
 // Waits are bounded: after a limit a thread records a code in `*err`, raises the CTA's abort flag, and all fall through to the
 // end, where the tensor memory is given back.
 // ---------------------------------------------------------------------------------------------
@@ -287,7 +291,47 @@ struct MxProduct {
   const uint8_t* w_scales;
   void* out;
   int rows, k, w_rows, out_features, unary, per_split;                 // per_split: stages of a CTA
+  const void* x;                                                       // rows that the kernel rounds itself (ROUND)
+  long long x_row;
 };
+
+// 32 numbers of a row as 16 bytes of codes and the scale's byte.
+__device__ __forceinline__ uint4 mx_round32(const uint32_t (&w)[16], uint32_t& s) {      // pairs of bfloat16
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  m = max(m & 0xffffu, m >> 16);
+  s = mx_scale_byte(__uint_as_float(m << 16));
+  const float inv = mx_inverse_scale(s);
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(w[4 * i + j] << 16);
+      v[2 * j + 1] = __uint_as_float(w[4 * i + j] & 0xffff0000u);
+    }
+    c[i] = mx_codes8(v, inv);
+  }
+  return make_uint4(c[0], c[1], c[2], c[3]);
+}
+__device__ __forceinline__ uint4 mx_round32(const uint32_t (&w)[32], uint32_t& s) {      // float32
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) m = max(m, w[i] & 0x7fffffffu);
+  s = mx_scale_byte(__uint_as_float(m));
+  const float inv = mx_inverse_scale(s);
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[8 * i + j]);
+    c[i] = mx_codes8(v, inv);
+  }
+  return make_uint4(c[0], c[1], c[2], c[3]);
+}
 
 // What becomes of a sum.  The function is chosen at compile time, or is one call: copies of every function's code for every
 // element of an unrolled loop are fetched by every SM (33 rows of gated 4,096 x 12,288: 38 us for 16).
@@ -305,10 +349,11 @@ template <int EPI> __device__ __forceinline__ float mx_gate(float g, float u, in
 }
 template <int EPI> __device__ __forceinline__ float mx_apply(float y, int unary) { return EPI == MX_UNARY ? mx_unary_call(y, unary) : y; }
 
-template <typename C, int EPI, typename TO>
+template <typename C, int EPI, typename TO, typename TX>
 __global__ void __launch_bounds__(C::THREADS)
 mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, MxProduct p, int* err) {
   constexpr bool GATED = EPI == MX_SILU || EPI == MX_GATED;
+  constexpr bool ROUND = !std::is_same<TX, void>::value;
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ uint64_t full[C::STAGES], empty[C::STAGES], ready;
   __shared__ uint32_t tmem_slot;
@@ -320,7 +365,7 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
   const int k_tiles = (p.k + 127) / 128, stages = (p.k + MX_KSTAGE - 1) / MX_KSTAGE;
   const int s0 = blockIdx.z * p.per_split, s1 = min(stages, s0 + p.per_split);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::STAGES; ++i) { mx_mbar_init(&full[i], 1); mx_mbar_init(&empty[i], 1); }
+    for (int i = 0; i < C::STAGES; ++i) { mx_mbar_init(&full[i], ROUND ? 1 + 32 * C::EPI_WARPS : 1); mx_mbar_init(&empty[i], 1); }
     mx_mbar_init(&ready, 1);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -340,7 +385,7 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
     auto bytes = [&](int s) { return (uint32_t)min(2, k_tiles - 2 * s) * 512u; };      // of one tile of rows' scales
     auto load_w = [&](int s, int i) {
       const uint32_t at = base + i * C::STAGE_BYTES;
-      mx_expect_tx(&full[i], MX_A_BYTES + C::B_BYTES + bytes(s) * (1 + C::RT));
+      mx_expect_tx(&full[i], ROUND ? MX_A_BYTES + bytes(s) : MX_A_BYTES + C::B_BYTES + bytes(s) * (1 + C::RT));
       mx_tma_2d(at, &w_map, &full[i], s * 64, o0);
       mx_bulk(at + C::SA, p.w_scales + ((size_t)(o0 >> 7) * k_tiles + 2 * s) * 512, bytes(s), &full[i]);
     };
@@ -356,17 +401,58 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
     __syncwarp();
     ifb_pdl_wait();
     ifb_pdl_trigger();
-    if (mx_elect())
+    if (!ROUND && mx_elect())
       for (int i = 0; i < ahead; ++i) load_x(s0 + i, i);
     __syncwarp();
     for (int s = s0 + ahead; s < s1; ++s) {
       const int j = s - s0, i = j % C::STAGES;
       if (!mx_wait(&empty[i], ((j / C::STAGES) & 1) ^ 1, abort_flag, err, 701)) break;
-      if (mx_elect()) { load_w(s, i); load_x(s, i); }
+      if (mx_elect()) { load_w(s, i); if (!ROUND) load_x(s, i); }
       __syncwarp();
     }
   } else {
     ifb_pdl_wait();
+    if constexpr (ROUND) {
+      if (warp >= 2) {
+        // blocks 32 EPI_WARPS apart; a block's numbers are requested a stage ahead
+        constexpr int THREADS = 32 * C::EPI_WARPS, PER = C::NT * 8 / THREADS, W = sizeof(TX) == 2 ? 16 : 32;
+        const int tid = threadIdx.x - 64;
+        uint32_t w[PER][W];
+        auto request = [&](int s) {
+#pragma unroll
+          for (int b = 0; b < PER; ++b) {
+            const int at = tid + b * THREADS, row = at >> 3, e = (s * 8 + (at & 7)) * MX_BLOCK;
+            const bool in = row < p.rows && e < p.k;
+            const uint4* src = reinterpret_cast<const uint4*>((const TX*)p.x + (size_t)(in ? row : 0) * p.x_row + (in ? e : 0));
+#pragma unroll
+            for (int i = 0; i < W / 4; ++i) {
+              const uint4 v = in ? src[i] : make_uint4(0, 0, 0, 0);
+              w[b][4 * i] = v.x; w[b][4 * i + 1] = v.y; w[b][4 * i + 2] = v.z; w[b][4 * i + 3] = v.w;
+            }
+          }
+        };
+        request(s0);
+        for (int s = s0; s < s1; ++s) {
+          const int j = s - s0, i = j % C::STAGES;
+          uint4 codes[PER];
+          uint32_t scale[PER];
+#pragma unroll
+          for (int b = 0; b < PER; ++b) codes[b] = mx_round32(w[b], scale[b]);
+          if (s + 1 < s1) request(s + 1);
+          if (j >= C::STAGES && !mx_wait(&empty[i], ((j / C::STAGES) & 1) ^ 1, abort_flag, err, 704)) break;
+          unsigned char* const at_b = raw + (base - mx_smem(raw)) + i * C::STAGE_BYTES + MX_A_BYTES;
+          unsigned char* const at_s = raw + (base - mx_smem(raw)) + i * C::STAGE_BYTES + C::SB;
+#pragma unroll
+          for (int b = 0; b < PER; ++b) {
+            const int at = tid + b * THREADS, row = at >> 3, block = at & 7;
+            *reinterpret_cast<uint4*>(at_b + row * 128 + ((block ^ (row & 7)) << 4)) = codes[b];
+            at_s[(block >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (block & 3)] = (unsigned char)scale[b];
+          }
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(mx_smem(&full[i])) : "memory");
+        }
+      }
+    }
     if (warp == 1) {
       for (int s = s0; s < s1; ++s) {
         const int j = s - s0, i = j % C::STAGES;
@@ -472,9 +558,9 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
   }
 }
 
-template <typename C, int EPI, typename TO>
+template <typename C, int EPI, typename TO, typename TX>
 static int mx_launch(const CUtensorMap& xm, const CUtensorMap& wm, const MxProduct& p, int splits, int* err, cudaStream_t stream) {
-  auto kernel = mx4_linear_kernel<C, EPI, TO>;
+  auto kernel = mx4_linear_kernel<C, EPI, TO, TX>;
   IFB_ALLOW_SMEM(kernel, C::SMEM);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.w_rows + 127) / 128, (p.rows + C::NT - 1) / C::NT, splits);
@@ -492,15 +578,15 @@ static int mx_launch(const CUtensorMap& xm, const CUtensorMap& wm, const MxProdu
   if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
   return IFB_OK;
 }
-template <typename C>
+template <typename C, typename TX>
 static int mx_launch_any(const CUtensorMap& xm, const CUtensorMap& wm, const MxProduct& p, bool gated, int dtype, int splits, int* err,
                          cudaStream_t stream) {
   if (dtype == IFB_F32) {
-    if (gated) return mx_launch<C, MX_GATED, float>(xm, wm, p, splits, err, stream);
-    return p.unary ? mx_launch<C, MX_UNARY, float>(xm, wm, p, splits, err, stream) : mx_launch<C, MX_PLAIN, float>(xm, wm, p, splits, err, stream);
+    if (gated) return mx_launch<C, MX_GATED, float, TX>(xm, wm, p, splits, err, stream);
+    return p.unary ? mx_launch<C, MX_UNARY, float, TX>(xm, wm, p, splits, err, stream) : mx_launch<C, MX_PLAIN, float, TX>(xm, wm, p, splits, err, stream);
   }
-  if (gated) return p.unary ? mx_launch<C, MX_GATED, bf16>(xm, wm, p, splits, err, stream) : mx_launch<C, MX_SILU, bf16>(xm, wm, p, splits, err, stream);
-  return p.unary ? mx_launch<C, MX_UNARY, bf16>(xm, wm, p, splits, err, stream) : mx_launch<C, MX_PLAIN, bf16>(xm, wm, p, splits, err, stream);
+  if (gated) return p.unary ? mx_launch<C, MX_GATED, bf16, TX>(xm, wm, p, splits, err, stream) : mx_launch<C, MX_SILU, bf16, TX>(xm, wm, p, splits, err, stream);
+  return p.unary ? mx_launch<C, MX_UNARY, bf16, TX>(xm, wm, p, splits, err, stream) : mx_launch<C, MX_PLAIN, bf16, TX>(xm, wm, p, splits, err, stream);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -731,9 +817,14 @@ static int mx_launch_pair_any(const CUtensorMap (&m)[4], const MxProduct& p, boo
   return p.unary ? mx_launch_pair<MX_UNARY, bf16>(m, p, err, stream) : mx_launch_pair<MX_PLAIN, bf16>(m, p, err, stream);
 }
 
-// x: [rows][k], w: [w_rows][k] (twice the out features if the epilogue is gated), both microscaled.  epilogue: as in the other products.
-IFB_EXPORT int ifb_mx4_linear(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales, void* out, int out_dtype,
-                              int rows, int k, int w_rows, int epilogue, void* err, void* stream) {
+// x: [rows][k], w: [w_rows][k] (twice the out features if the epilogue is gated).  x_dtype IFB_F32 or IFB_BF16: `x` has numbers, rows
+// x_row elements apart; up to MX_ROUND_ROWS rows are rounded within the product, more of them first, into x_codes and x_scales
+// (whose room is the caller's; neither is looked at otherwise).  x_dtype -1: x_codes and x_scales have been rounded.
+// epilogue: as in the other products.  nt, splits: 0, or (for measurements) tokens of a tile and CTAs that share its k range.
+constexpr int MX_ROUND_ROWS = 32;
+IFB_EXPORT int ifb_mx4_round_rows() { return MX_ROUND_ROWS; }
+IFB_EXPORT int ifb_mx4_linear(const void* x, int x_dtype, long long x_row, void* x_codes, void* x_scales, const void* w_codes, const void* w_scales,
+                              void* out, int out_dtype, int rows, int k, int w_rows, int epilogue, int nt, int splits, void* err, void* stream) {
   const bool gated = epilogue & 1;
   const int unary = epilogue >> 4;
   int bad = mx_sizes(rows, k, 0);
@@ -741,26 +832,46 @@ IFB_EXPORT int ifb_mx4_linear(const void* x_codes, const void* x_scales, const v
   if (w_rows < 1 || (gated && (w_rows & 1))) return IFB_ERR_SIZE;
   if ((epilogue & 14) || unary > IFB_UNARY_LAST) return IFB_ERR_ARG;
   if (out_dtype != IFB_F32 && out_dtype != IFB_BF16) return IFB_ERR_DTYPE;
+  if (x_dtype != -1 && x_dtype != IFB_F32 && x_dtype != IFB_BF16) return IFB_ERR_DTYPE;
   if ((((uintptr_t)x_codes) | ((uintptr_t)x_scales) | ((uintptr_t)w_codes) | ((uintptr_t)w_scales)) & 15) return IFB_ERR_ALIGN;
-  const bool pair = rows > 256;
-  const int nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  const bool round = x_dtype != -1 && rows <= MX_ROUND_ROWS;
+  if (round && ((((uintptr_t)x) | (uintptr_t)(x_row * (x_dtype == IFB_F32 ? 4 : 2))) & 15)) return IFB_ERR_ALIGN;
+  if (!round && (!x_codes || !x_scales)) return IFB_ERR_ARG;
+  if (!round && x_dtype != -1) {
+    bad = ifb_mx4_quantize(x, x_dtype, x_row, x_codes, x_scales, rows, k, 0, stream);
+    if (bad) return bad;
+  }
+  const bool pair = nt ? nt == 256 : rows > 256;
+  if (!nt || round) nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  if (nt < rows && nt < 128) return IFB_ERR_ARG;
   const int stages = (k + MX_KSTAGE - 1) / MX_KSTAGE, tiles = (w_rows + 127) / 128 * ((rows + nt - 1) / nt);
   // the k range is shared where tiles leave SMs idle
-  int splits = 1;
-  while (splits < 8 && splits * 2 <= stages && tiles * splits * 2 <= ifb_sm_count() + 8) splits *= 2;
+  if (!splits) {
+    splits = 1;
+    while (splits < 8 && splits * 2 <= stages && tiles * splits * 2 <= ifb_sm_count() + 8) splits *= 2;
+  }
+  if (splits < 1 || splits > 8 || splits > stages) return IFB_ERR_ARG;
   MxProduct p = {(const uint8_t*)x_scales, (const uint8_t*)w_scales, out, rows, k, w_rows, gated ? w_rows / 2 : w_rows, unary,
-                 (stages + splits - 1) / splits};
+                 (stages + splits - 1) / splits, x, x_row};
   splits = (stages + p.per_split - 1) / p.per_split;                   // every CTA has a stage
   // the maps see pairs of bytes as one number of 16 bits: only widths and strides in bytes count
   const unsigned long long xd[2] = {(unsigned long long)k / 4, (unsigned long long)rows}, xs[1] = {(unsigned long long)k / 2};
   const unsigned long long wd[2] = {(unsigned long long)k / 4, (unsigned long long)w_rows}, ws[1] = {(unsigned long long)k / 2};
   const unsigned xb[2] = {64, pair ? 128u : (unsigned)nt}, wb[2] = {64, 128};
   CUtensorMap xm, wm;
-  bad = ifb_tensor_map_bf16(&xm, x_codes, 2, xd, xs, xb);
-  if (!bad) bad = ifb_tensor_map_bf16(&wm, w_codes, 2, wd, ws, wb);
+  bad = ifb_tensor_map_bf16(&wm, w_codes, 2, wd, ws, wb);
   if (bad) return bad;
   cudaStream_t st = (cudaStream_t)stream;
   int* e = (int*)err;
+  if (round) {
+    if (x_dtype == IFB_F32)
+      return nt == 16 ? mx_launch_any<MxCfg<16, 6>, float>(wm, wm, p, gated, out_dtype, splits, e, st)
+                      : mx_launch_any<MxCfg<32, 6>, float>(wm, wm, p, gated, out_dtype, splits, e, st);
+    return nt == 16 ? mx_launch_any<MxCfg<16, 6>, bf16>(wm, wm, p, gated, out_dtype, splits, e, st)
+                    : mx_launch_any<MxCfg<32, 6>, bf16>(wm, wm, p, gated, out_dtype, splits, e, st);
+  }
+  bad = ifb_tensor_map_bf16(&xm, x_codes, 2, xd, xs, xb);
+  if (bad) return bad;
   if (pair) {
     // scale tiles as rows of 512 bytes
     const unsigned long long k_tiles = (unsigned long long)(k + 127) / 128, sd[1] = {512};
@@ -772,9 +883,10 @@ IFB_EXPORT int ifb_mx4_linear(const void* x_codes, const void* x_scales, const v
     return bad ? bad : mx_launch_pair_any(m, p, gated, out_dtype, e, st);
   }
   switch (nt) {
-    case 16: return mx_launch_any<MxCfg<16, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
-    case 32: return mx_launch_any<MxCfg<32, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
-    case 64: return mx_launch_any<MxCfg<64, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
-    default: return mx_launch_any<MxCfg<128, 6>>(xm, wm, p, gated, out_dtype, splits, e, st);
+    case 16: return mx_launch_any<MxCfg<16, 6>, void>(xm, wm, p, gated, out_dtype, splits, e, st);
+    case 32: return mx_launch_any<MxCfg<32, 6>, void>(xm, wm, p, gated, out_dtype, splits, e, st);
+    case 64: return mx_launch_any<MxCfg<64, 4>, void>(xm, wm, p, gated, out_dtype, splits, e, st);
+    case 128: return mx_launch_any<MxCfg<128, 6>, void>(xm, wm, p, gated, out_dtype, splits, e, st);
+    default: return IFB_ERR_ARG;
   }
 }

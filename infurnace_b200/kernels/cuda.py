@@ -143,6 +143,8 @@ class CudaKernels(LowBitKernels):
         self.small_q_tma_calls = 0
         self.tc_shared_k_calls = 0     # tcgen05 products with the k range shared by a cluster; with a folded norm
         self.tc_folded_calls = 0
+        self._dev_err_at = self._dev_err.data_ptr()
+        self._epilogues = EPILOGUES
         self._err_armed = False
         self.tc_min_rows = 65
         if os.environ.get("INFURNACE_GATE_PLAN"):

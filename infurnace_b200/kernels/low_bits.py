@@ -128,9 +128,9 @@ class LowBitKernels:
             lib = load_library("mx4", progress=self._progress)
             lib.ifb_mx4_quantize.argtypes = [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]
             lib.ifb_mx4_values.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]
-            lib.ifb_mx4_linear.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
-                                           c_void_p, c_void_p]
-            self._mx4_scratch = {}
+            lib.ifb_mx4_linear.argtypes = [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                                           c_int, c_int, c_int, c_int, c_void_p, c_void_p]
+            self._mx4_round_rows = int(lib.ifb_mx4_round_rows())
             self._mx4 = lib
         return self._mx4
 
@@ -171,35 +171,42 @@ class LowBitKernels:
             raise KernelError("mx4_matrix: w is [rows, k], a gated one of an even number of rows")
         return self.mx4_quantize(w, Mx4Matrix.empty(w.shape[0], w.shape[1], w.device, gated))
 
-    def mx4_linear(self, x, w, out, epilogue="none"):
+    def mx4_linear(self, x, w, out, epilogue="none", nt=0, splits=0):
         """out = Q(x) w^T with the epilogue (a key of ``EPILOGUES``), ``w`` an :class:`Mx4Matrix` and Q(x) the rows of ``x``
         rounded to 4 bits as ``mx4_quantize`` rounds them; ``x`` bfloat16 or float32 [n, k], or an :class:`Mx4Matrix` that
-        has been rounded already.  ``out`` bfloat16 or float32 [n, features].  The gated epilogues want a gated ``w``."""
-        from .cuda import EPILOGUES
-        epi = EPILOGUES.get(epilogue)
+        has been rounded already.  ``out`` bfloat16 or float32 [n, features].  The gated epilogues want a gated ``w``.  ``nt`` and
+        ``splits`` (for measurements): tokens of a tile and CTAs that share its k range, where the rule's choice is not wanted."""
+        epi = self._epilogues.get(epilogue)
         if epi is None:
-            raise KernelError(f"mx4_linear: unknown epilogue {epilogue!r}; known: {', '.join(EPILOGUES)}")
+            raise KernelError(f"mx4_linear: unknown epilogue {epilogue!r}; known: {', '.join(self._epilogues)}")
         n, k = x.shape
         code = _CODES.get(out.dtype)
-        features = w.rows // 2 if epi & 1 else w.rows
-        if k != w.k or bool(epi & 1) != w.gated or out.shape != (n, features):
+        if k != w.k or (epi & 1 != 0) != w.gated or out.shape != (n, w.rows >> (epi & 1)):
             raise KernelError(f"mx4_linear: x {tuple(x.shape)}, w {w.shape} ({'gated' if w.gated else 'plain'}), out {tuple(out.shape)} "
                               f"and epilogue {epilogue!r} do not match")
-        if code is None or not out.is_cuda or not out.is_contiguous() or out.device != w.codes.device:
-            raise KernelError("mx4_linear: out is bfloat16 or float32, contiguous, on the matrix's device")
-        lib, stream = self._mx4_lib(), self._stream()
-        if not isinstance(x, Mx4Matrix):
-            held = self._mx4_scratch.get((stream, k))
-            if held is None or held.codes.shape[0] < n:
-                held = self._mx4_scratch[(stream, k)] = Mx4Matrix.empty(max(n, 256), k, w.codes.device)
-                self.scratch_generation += 1
-            x = self.mx4_quantize(x, Mx4Matrix(held.codes[:n], held.scales[:Mx4Matrix.scale_bytes(n, k)], n, k))
-        elif x.gated or x.codes.device != w.codes.device:
-            raise KernelError("mx4_linear: x is a plain matrix on w's device")
-        self.launches += 1
+        device = w.codes.device
+        if code is None or out.device != device or not out.is_contiguous() or x.device != device or device.type != "cuda":
+            raise KernelError("mx4_linear: out is bfloat16 or float32, contiguous, and all is on the matrix's device")
+        lib = self._mx4_lib()
+        if isinstance(x, Mx4Matrix):
+            if x.gated:
+                raise KernelError("mx4_linear: x is a plain matrix")
+            rows = (0, -1, 0, *x._at)
+        else:
+            x_code = _CODES.get(x.dtype)
+            if x_code is None or x.stride(1) != 1:
+                raise KernelError("mx4_linear: x is bfloat16 or float32 with unit stride along k, or an Mx4Matrix")
+            if n <= self._mx4_round_rows:
+                rows = (x.data_ptr(), x_code, x.stride(0), 0, 0)
+            else:
+                codes = -(-n * k // 512) * 256                             # half a byte an element, to a multiple of 256
+                room = torch.empty(codes + Mx4Matrix.scale_bytes(n, k), dtype=torch.uint8, device=device)
+                rows = (x.data_ptr(), x_code, x.stride(0), room.data_ptr(), room.data_ptr() + codes)
+        self.launches += 1 if rows[3] == 0 or rows[1] < 0 else 2
         self._err_armed = True
-        self._low_bit_status(lib.ifb_mx4_linear(*x._at, *w._at, out.data_ptr(), code, n, k, w.rows, epi, self._dev_err.data_ptr(),
-                                                stream), "mx4_linear")
+        status = lib.ifb_mx4_linear(*rows, *w._at, out.data_ptr(), code, n, k, w.rows, epi, nt, splits, self._dev_err_at, self._stream())
+        if status:
+            self._low_bit_status(status, "mx4_linear")
         return out
 
     # ------------------------------------------------------------------ keys and values of 8 bits
