@@ -23,10 +23,9 @@
 // half-precision numbers down to 2^-32 of it still count.  A weight enters the product times its page's step over the largest
 // step so far.  Sums are float32.
 //
-// Split form: the work (64 keys of a key head for one tile of score rows is a unit) of all requests is cut into as many equal
-// pieces as CTAs fit on the device, whatever the lengths; a piece that ends inside an item leaves its sums in scratch memory,
-// and the CTA that arrives last at an item adds them in the order of the pieces.  Whole form (prompts): a warp owns its score
-// rows over all their keys.
+// Split form: the keys of a key head for one tile of score rows are cut into pieces of nearly one length for all requests,
+// whatever their lengths, as many as CTAs fit on the device; a piece leaves its sums in scratch memory, and the CTA that arrives
+// last at an item adds them in the order of the pieces.  Whole form (prompts): a warp owns its score rows over all their keys.
 // Keys that no row of a tile sees are not read; block-table entries outside are not followed.  A row that sees no key is zero.
 #include "common.cuh"
 #include <cuda_fp16.h>
@@ -65,12 +64,13 @@ struct Kv8Args {
   const int* cu_q;
   const int* seq_lens;
   qtype* out;                            // [tokens][heads][D]
-  float* parts;                          // split form: [2 per CTA][rows of a tile][D + 2]
+  float* parts;                          // split form: [CTA][rows of a tile][D + 2]
   int* counters;                         // split form: one per item, 0 between launches
   int requests, heads, kv_heads, page_size, window;
   float scale;                           // of the scores, times log2(e)
   int min_rows, max_rows;                // requests with fewer or more score rows than this are another kernel's
   int tiles;                             // split form: tiles of score rows that any request has at most
+  int most;                              // split form: CTAs that run on the device at a time
 };
 
 __device__ __forceinline__ float kv8_exp2(float x) {
@@ -199,7 +199,9 @@ struct Stream {
   uint32_t qf[TERMS][NT][KS][2];
   float qscale[NT][2], qoff[NT][2];      // what turns a product into a number of real units: times qscale, and qoff
   int last[NT][2];                       // position of the row's query (NO_ROW: no such row)
-  float m[NT][2], l[NT][2], wsum[NT][2]; // reference of the row's scores; sums of its weights, and of weights times steps, this lane's part
+  // m: reference of the row's scores; rise: what a score has to exceed to move it; shift: what is added to a score for its weight;
+  // l, wsum: this lane's part of the sums of the weights, and of weights times steps
+  float m[NT][2], rise[NT][2], shift[NT][2], l[NT][2], wsum[NT][2];
   float o[KS][NT][4];
   int v_ref;                             // exponent field that the sums of weighted values are in units of
 
@@ -208,7 +210,7 @@ struct Stream {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; wsum[n][e] = 0.f; }
+      for (int e = 0; e < 2; ++e) { m[n][e] = rise[n][e] = -INFINITY; shift[n][e] = 8.f; l[n][e] = 0.f; wsum[n][e] = 0.f; }
 #pragma unroll
       for (int i = 0; i < KS; ++i) { o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f; }
     }
@@ -306,15 +308,15 @@ struct Stream {
         s[n][j] = seen ? x : -INFINITY;
       }
   }
-  template <bool MASK>
+  // vf: the exponent field of the values; 0 also for a page of NaN, whose scores are NaN where they are seen.
   __device__ __forceinline__ void weigh(float (&s)[NT][4], const Values<D>& v, int vf) {
-    bool rise = false;
+    bool up = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) rise |= s[n][j] > m[n][j & 1] + 6.f;
-    const bool larger = vf > v_ref && vf != 255;                        // uniform
-    if (__any_sync(0xffffffffu, rise) || larger) {
+      for (int e = 0; e < 2; ++e) up |= fmaxf(s[n][e], s[n][2 + e]) > rise[n][e];
+    const bool larger = vf > v_ref;                                     // uniform
+    if (__any_sync(0xffffffffu, up) || larger) {
       float fv = 1.f;
       if (larger) {
         fv = v_ref ? __uint_as_float((uint32_t)max(0, 127 + v_ref - vf) << 23) : 0.f;
@@ -332,6 +334,8 @@ struct Stream {
           mx = fmaxf(mx, m[n][e]);
           f[e] = mx == m[n][e] ? 1.f : kv8_exp2(m[n][e] - mx);
           m[n][e] = mx;
+          rise[n][e] = mx + 6.f;
+          shift[n][e] = mx == -INFINITY ? 8.f : 8.f - mx;
           l[n][e] *= f[e];
           f[e] *= fv;
           wsum[n][e] *= f[e];
@@ -340,19 +344,22 @@ struct Stream {
         for (int i = 0; i < KS; ++i) { o[i][n][0] *= f[0]; o[i][n][1] *= f[1]; o[i][n][2] *= f[0]; o[i][n][3] *= f[1]; }
       }
     }
-    // the step of this page's values over the reference; fields in use are 1 .. 254
-    const float fw = vf == 0 ? 0.f : vf == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)max(0, 127 + vf - v_ref) << 23);
+    // the step of this page's values over the reference
+    const float fw = vf == 0 ? 0.f : __uint_as_float((uint32_t)max(0, 127 + vf - v_ref) << 23);
     uint32_t p[TERMS][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float ref = m[n][j & 1], x = kv8_exp2(s[n][j] - (ref == -INFINITY ? 0.f : ref) + 8.f);
-        l[n][j & 1] += x;
-        w[j] = MASK && s[n][j] == -INFINITY ? 0.f : x * fw;             // (a page of NaN, a key that is not seen)
-        wsum[n][j & 1] += w[j];
+      for (int j = 0; j < 4; ++j) w[j] = kv8_exp2(s[n][j] + shift[n][j & 1]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float both = w[e] + w[2 + e];
+        l[n][e] += both;
+        wsum[n][e] = fmaf(both, fw, wsum[n][e]);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] *= fw;
       const uint32_t lo = pack_half(w[0], w[1]), hi = pack_half(w[2], w[3]);
       p[0][n][0] = transpose8(lo);
       p[0][n][1] = transpose8(hi);
@@ -364,50 +371,65 @@ struct Stream {
     v.template multiply<NT>(o, p);
   }
 
-  // Tiles first, first + step, ... up to `end` (exclusive) of 16 keys.  full_to: keys up to here are seen by every row that exists
-  // (full_from: from here on).
-  __device__ __forceinline__ void run(const Kv8Args& a, const int* table, int kv_head, int first, int end, int step, int full_from, int full_to,
-                                      int lane) {
-    if (first >= end) return;
-    const size_t head_bytes = (size_t)a.page_size * D, page_bytes = 2 * (size_t)a.kv_heads * head_bytes;
-    // t / per_page by a product with the next whole number above 2^32 / per_page: exact for t below 2^32 / per_page
-    const uint32_t per_page = (uint32_t)a.page_size / 16, inverse = per_page > 1 ? 0xffffffffu / per_page + 1 : 0;
-    auto page_of = [&](int t) { return per_page > 1 ? (int)__umulhi((uint32_t)t, inverse) : t; };
-    const int8_t* const base = a.codes + (size_t)kv_head * head_bytes;
-    auto tile_at = [&](int t, int page) {                               // the keys; the values lie kv_heads heads further
-      return base + (size_t)page * page_bytes + (uint32_t)(t - page_of(t) * (int)per_page) * (16 * D);
-    };
-    const size_t v_off = (size_t)a.kv_heads * head_bytes;
+  // Tiles first, first + step, ... up to `end` (exclusive) of 16 keys, in two parts: `begin` requests the first of them, `run` works
+  // through all.  full_from, full_to: keys from and up to here are seen by every row that exists.
+  struct Walk {
+    const int* table;
+    const int8_t* base;
+    const uint8_t* fields;
+    size_t page_bytes, v_off;
+    uint32_t per_page, inverse;
+    int kv_heads, first, end, step, next_page, kf, vf;
     Keys k;
     Values<D> v;
-    int page = table[page_of(first)];
-    const int8_t* at = tile_at(first, page);
-    const uint8_t* fields = a.exponents + (size_t)page * 2 * a.kv_heads + kv_head;
-    int kf = fields[0], vf = fields[a.kv_heads];
-    k.load(at, lane);
-    v.load(at + v_off, lane);
-    int next_page = first + step < end ? table[page_of(first + step)] : page;
-    for (int t = first; t < end; t += step) {
-      const bool more = t + step < end;
+    // (t / per_page by a product with the next whole number above 2^32 / per_page: exact for t below 2^32 / per_page)
+    __device__ __forceinline__ int page_of(int t) const { return per_page > 1 ? (int)__umulhi((uint32_t)t, inverse) : t; }
+    __device__ __forceinline__ const int8_t* tile(int t, int page) const {
+      return base + (size_t)page * page_bytes + (uint32_t)(t - page_of(t) * (int)per_page) * (16 * D);
+    }
+    __device__ __forceinline__ void read_fields(int page) {
+      const uint8_t* f = fields + (size_t)page * 2 * kv_heads;
+      kf = f[0];
+      vf = f[kv_heads];
+    }
+    __device__ __forceinline__ Walk(const Kv8Args& a, const int* table_, int kv_head, int first_, int end_, int step_, int lane) {
+      table = table_;
+      page_bytes = 2 * (size_t)a.kv_heads * a.page_size * D;
+      base = a.codes + (size_t)kv_head * a.page_size * D;
+      v_off = (size_t)a.kv_heads * a.page_size * D;
+      fields = a.exponents + kv_head;
+      kv_heads = a.kv_heads;
+      per_page = (uint32_t)a.page_size / 16;
+      inverse = per_page > 1 ? 0xffffffffu / per_page + 1 : 0;
+      first = first_; end = end_; step = step_; next_page = 0;
+      if (first >= end) return;
+      const int page = table[page_of(first)];
+      if (first + step < end) next_page = table[page_of(first + step)];
+      const int8_t* at = tile(first, page);
+      read_fields(page);
+      k.load(at, lane);
+      v.load(at + v_off, lane);
+    }
+  };
+  __device__ __forceinline__ void run(const Kv8Args& a, Walk& w, int full_from, int full_to, int lane) {
+    for (int t = w.first; t < w.end; t += w.step) {
+      const bool more = t + w.step < w.end;
       float s[NT][4];
       const bool whole = t * 16 >= full_from && t * 16 + 15 <= full_to;
-      const float ks = kv8_step((uint32_t)kf) * a.scale;
-      if (whole) scores<false>(k, ks, t * 16, a.window, s, lane);
-      else scores<true>(k, ks, t * 16, a.window, s, lane);
-      const int8_t* next = at;
-      const int vf_now = vf;
+      // (a page whose values are NaN makes the scores NaN that see it, and with them the row)
+      const float ks = kv8_step(w.vf == 255 ? 255u : (uint32_t)w.kf) * a.scale;
+      const int vf = w.vf == 255 ? 0 : w.vf;
+      if (whole) scores<false>(w.k, ks, t * 16, a.window, s, lane);
+      else scores<true>(w.k, ks, t * 16, a.window, s, lane);
+      const int8_t* next = w.base;
       if (more) {                                                       // the next keys while these values are multiplied
-        next = tile_at(t + step, next_page);
-        const uint8_t* nf = a.exponents + (size_t)next_page * 2 * a.kv_heads + kv_head;
-        kf = nf[0];
-        vf = nf[a.kv_heads];
-        k.load(next, lane);
-        if (t + 2 * step < end) next_page = table[page_of(t + 2 * step)];
+        next = w.tile(t + w.step, w.next_page);
+        w.read_fields(w.next_page);
+        w.k.load(next, lane);
+        if (t + 2 * w.step < w.end) w.next_page = w.table[w.page_of(t + 2 * w.step)];
       }
-      if (whole) weigh<false>(s, v, vf_now);
-      else weigh<true>(s, v, vf_now);
-      if (more) v.load(next + v_off, lane);                             // and the next values while the next scores are formed
-      at = next;
+      weigh(s, w.v, vf);
+      if (more) w.v.load(next + w.v_off, lane);                         // and the next values while the next scores are formed
     }
   }
   // Sums over the lanes that share a row, and the weighted values in real units (times the weights' common factor).
@@ -449,12 +471,12 @@ kv8_attention_whole_kernel(Kv8Args a) {
   const int row0 = ((int)(gridDim.x - 1 - blockIdx.x) * WARPS + warp) * 8 * NT;
   if (row0 >= rows) return;
   const int pos0 = L - q_len, p_first = pos0 + row0 / G, p_last = pos0 + min(row0 + 8 * NT - 1, rows - 1) / G;
+  const int lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
+  typename Stream<NT>::Walk walk(a, a.tables + (size_t)r * a.table_stride, kv_head, lo / 16, p_last >= 0 ? p_last / 16 + 1 : 0, 1, lane);
   Stream<NT> st;
   st.reset();
   st.load_queries(a, q0, row0, rows, pos0, kv_head, G, lane);
-  const int lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
-  if (p_last >= 0)
-    st.run(a, a.tables + (size_t)r * a.table_stride, kv_head, lo / 16, p_last / 16 + 1, 1, a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
+  st.run(a, walk, a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
   st.finish();
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -469,184 +491,178 @@ kv8_attention_whole_kernel(Kv8Args a) {
     }
 }
 
+// CTAs on an SM that the registers are cut for.
+constexpr int split_ctas(int nt) { return nt == 1 && TERMS == 1 ? (D <= 128 ? 4 : 2) : D <= 128 ? 2 : 1; }
+
 // --------------------------------------------------------------------------------------------
 // Split form.  Items are (request, tile of 8 NT rows, key head), in that order; an item has the units of its request (those of
-// the request's last row: earlier tiles leave a few empty), one at least, so that a row without keys is written.  A piece is
-// no shorter than a 32nd of the longest item, so that few sums meet in one place.
+// the request's last row: earlier tiles leave a few empty), one at least, so that a row without keys is written.  A CTA has one
+// piece of one item.  With `most` CTAs on the device at once and fewer items, pieces have total / (most - items) units or a little
+// less, for which the pieces of all items are no more than `most`; else every item is one piece.  (Equal shares of the units, with
+// CTAs that have the end of one item and the beginning of the next, are a tenth shorter and cost a second start and a second join.)
 // --------------------------------------------------------------------------------------------
-constexpr int MAX_PARTS = 34;            // pieces of an item
+constexpr int MAX_PARTS = 32;            // pieces of an item
 constexpr int PITCH = D + 8;             // of a row of sums in shared memory (the rows of a quad of lanes fall on two halves of the banks)
 // Where a warp's sums lie in a row: m tile by m tile, the lanes' pairs side by side.
 __device__ __forceinline__ int kv8_place(int i, int lane) { return i * 16 + (lane >> 2) * 2; }
 __device__ __forceinline__ int kv8_place_dim(int place) { return Values<D>::dim(place >> 4, ((place & 15) >> 1) << 2, 0); }
 
-struct Kv8Item { int r, before, units, tiles, q0, q_len, L; };
-
-// The request that has unit `at`, by a look over the requests' lengths (all lanes; every warp for itself).  at < 0: instead the
-// number of all units in `before` and the most units of an item in `units`.
+// What a lane knows of request r0 + lane: where its queries lie, the units of an item and its items.
+struct Kv8Look { int q0, q_len, L, units, items; };
 template <int ROWS>
-__device__ __forceinline__ Kv8Item kv8_find(const Kv8Args& a, int G, int at, int lane) {
-  Kv8Item it = {};
-  int before = 0, most = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += 32) {
-    const int r = r0 + lane;
-    int q0 = 0, q_len = 0, L = 0, units = 0, tiles = 0;
-    if (r < a.requests) {
-      q0 = a.cu_q[r]; q_len = a.cu_q[r + 1] - q0; L = a.seq_lens[r];
-      const int rows = q_len * G;
-      if (q_len > 0 && rows >= a.min_rows && rows <= a.max_rows) {
-        tiles = (rows + ROWS - 1) / ROWS;
-        const int lo = a.window > 0 ? max(0, L - q_len - a.window + 1) : 0;
-        units = L > 0 ? max(1, (L - 1) / UNIT - lo / UNIT + 1) : 1;
-      }
+__device__ __forceinline__ Kv8Look kv8_look(const Kv8Args& a, int G, int r0, int lane) {
+  Kv8Look k = {};
+  const int r = r0 + lane;
+  if (r < a.requests) {
+    k.q0 = a.cu_q[r]; k.q_len = a.cu_q[r + 1] - k.q0; k.L = a.seq_lens[r];
+    const int rows = k.q_len * G;
+    if (k.q_len > 0 && rows >= a.min_rows && rows <= a.max_rows) {
+      k.items = (rows + ROWS - 1) / ROWS * a.kv_heads;
+      const int lo = a.window > 0 ? max(0, k.L - k.q_len - a.window + 1) : 0;
+      k.units = k.L > 0 ? max(1, (k.L - 1) / UNIT - lo / UNIT + 1) : 1;
     }
-    const int mine = units * tiles * a.kv_heads;
-    int x = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, d);
-      if (lane >= d) x += y;
-    }
-    if (at >= 0) {
-      const uint32_t hit = __ballot_sync(0xffffffffu, at < before + x);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        it.r = r0 + src;
-        it.before = before + __shfl_sync(0xffffffffu, x - mine, src);
-        it.units = __shfl_sync(0xffffffffu, units, src);
-        it.tiles = __shfl_sync(0xffffffffu, tiles, src);
-        it.q0 = __shfl_sync(0xffffffffu, q0, src);
-        it.q_len = __shfl_sync(0xffffffffu, q_len, src);
-        it.L = __shfl_sync(0xffffffffu, L, src);
-        return it;
-      }
-    }
-    most = max(most, units);
-    before += __shfl_sync(0xffffffffu, x, 31);
   }
-  it.before = before;
-  it.units = __reduce_max_sync(0xffffffffu, most);
-  return it;
+  return k;
 }
 
 template <int NT>
-__global__ void __launch_bounds__(32 * WARPS)
+__global__ void __launch_bounds__(32 * WARPS, split_ctas(NT))
 kv8_attention_split_kernel(Kv8Args a) {
   constexpr int ROWS = 8 * NT;
   extern __shared__ __align__(16) float sums[];                         // [WARPS][ROWS][PITCH], then maxima and sums [WARPS][ROWS] each
-  __shared__ float factors[MAX_PARTS][ROWS], denominator[ROWS];
+  __shared__ float part_m[MAX_PARTS][ROWS], part_l[MAX_PARTS][ROWS];
   __shared__ int arrived;
   ifb_pdl_wait();
   ifb_pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads;
   float* const sm_m = sums + WARPS * ROWS * PITCH;
   float* const sm_l = sm_m + WARPS * ROWS;
-  const Kv8Item all = kv8_find<ROWS>(a, G, -1, lane);
-  const int per = max(1, max((all.before + (int)gridDim.x - 1) / (int)gridDim.x, (all.units + 31) / 32));
-  int at = (int)blockIdx.x * per;
-  const int end = min(all.before, at + per);
-  while (at < end) {
-    const Kv8Item it = kv8_find<ROWS>(a, G, at, lane);
-    const int in_request = at - it.before, item = in_request / it.units, unit0 = in_request - item * it.units;
-    const int n_units = min(it.units - unit0, end - at), tile = item / a.kv_heads, kv_head = item - tile * a.kv_heads;
-    const int rows = it.q_len * G, row0 = tile * ROWS, here = min(ROWS, rows - row0);
-    const int pos0 = it.L - it.q_len, p_first = pos0 + row0 / G, p_last = pos0 + (row0 + here - 1) / G;
-    const int lo_request = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
-    const int key0 = (lo_request / UNIT + unit0) * UNIT;                // keys of this piece: up to n_units units from here
-    const int key_end = min(p_last + 1, key0 + n_units * UNIT);
-    Stream<NT> st;
-    st.reset();
-    st.load_queries(a, it.q0, row0, rows, pos0, kv_head, G, lane);
-    const int first = max(key0, lo) / 16;
-    st.run(a, a.tables + (size_t)it.r * a.table_stride, kv_head, first + warp, key_end > 0 ? (key_end + 15) / 16 : 0, WARPS,
-           a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
-    st.finish();
-    // the warps' sums side by side
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = n * 8 + (lane & 3) * 2 + e;
-        if (row < here) {
-          float* to = sums + (warp * ROWS + row) * PITCH;
-#pragma unroll
-          for (int i = 0; i < KS; ++i) *reinterpret_cast<float2*>(to + kv8_place(i, lane)) = make_float2(st.o[i][n][e], st.o[i][n][2 + e]);
-          if (lane < 4) { sm_m[warp * ROWS + row] = st.m[n][e]; sm_l[warp * ROWS + row] = st.l[n][e]; }
-        }
-      }
-    __syncthreads();
-    const bool alone = n_units == it.units;
-    // a piece's place in scratch memory: a CTA has at most two that are not whole items, its first and its last
-    float* const mine = a.parts + ((size_t)blockIdx.x * 2 + (unit0 ? 0 : 1)) * ROWS * (D + 2);
-    for (int i = tid; i < here * (D / 2); i += 32 * WARPS) {
-      const int row = i / (D / 2), place = (i - row * (D / 2)) * 2;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_m[w * ROWS + row]);
-      const float U = M == -INFINITY ? 0.f : M;
-      float2 o = make_float2(0.f, 0.f);
-      float l = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = kv8_exp2(sm_m[w * ROWS + row] - U);
-        const float2 x = *reinterpret_cast<const float2*>(sums + (w * ROWS + row) * PITCH + place);
-        o.x = fmaf(x.x, f, o.x);
-        o.y = fmaf(x.y, f, o.y);
-        l = fmaf(sm_l[w * ROWS + row], f, l);
-      }
-      if (alone) {
-        const int full = row0 + row;
-        kv8_store_pair(a.out + ((size_t)(it.q0 + full / G) * a.heads + kv_head * G + full % G) * D + kv8_place_dim(place), kv8_ratio(o.x, l), kv8_ratio(o.y, l));
-      } else {
-        *reinterpret_cast<float2*>(mine + row * D + place) = o;
-        if (place == 0) { mine[ROWS * D + row] = M; mine[ROWS * (D + 1) + row] = l; }
-      }
-    }
-    if (!alone) {
-      __threadfence();
-      __syncthreads();
-      const int first_unit = it.before + item * it.units, first_cta = first_unit / per, parts = (first_unit + it.units - 1) / per - first_cta + 1;
-      int* const counter = a.counters + ((size_t)it.r * a.tiles + tile) * a.kv_heads + kv_head;
-      if (tid == 0) arrived = atomicAdd(counter, 1);
-      __syncthreads();
-      if (arrived == parts - 1) {                                       // the last of the item's pieces
-        __threadfence();
-        auto part = [&](int c) { return a.parts + ((size_t)(first_cta + c) * 2 + (c == 0 ? 1 : 0)) * ROWS * (D + 2); };
-        for (int i = tid; i < here * parts; i += 32 * WARPS) factors[i / here][i % here] = __ldcg(part(i / here) + ROWS * D + i % here);
-        __syncthreads();
-        if (tid < here) {
-          float M = -INFINITY, l = 0.f;
-          for (int c = 0; c < parts; ++c) M = fmaxf(M, factors[c][tid]);
-          const float U = M == -INFINITY ? 0.f : M;
-#pragma unroll 4
-          for (int c = 0; c < parts; ++c) {
-            const float f = kv8_exp2(factors[c][tid] - U);
-            factors[c][tid] = f;
-            l = fmaf(__ldcg(part(c) + ROWS * (D + 1) + tid), f, l);
-          }
-          denominator[tid] = l;
-        }
-        __syncthreads();
-        for (int i = tid; i < here * (D / 2); i += 32 * WARPS) {
-          const int row = i / (D / 2), place = (i - row * (D / 2)) * 2;
-          float2 o = make_float2(0.f, 0.f);
-#pragma unroll 8
-          for (int c = 0; c < parts; ++c) {
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(part(c) + row * D + place));
-            const float f = factors[c][row];
-            o.x = fmaf(x.x, f, o.x);
-            o.y = fmaf(x.y, f, o.y);
-          }
-          const int full = row0 + row;
-          const float l = denominator[row];
-          kv8_store_pair(a.out + ((size_t)(it.q0 + full / G) * a.heads + kv_head * G + full % G) * D + kv8_place_dim(place), kv8_ratio(o.x, l), kv8_ratio(o.y, l));
-        }
-        if (tid == 0) *counter = 0;
-      }
-    }
-    __syncthreads();                                                    // the sums are read; the next item writes them
-    at += n_units;
+  // every warp for itself: how long pieces are, and whose piece this CTA's is
+  const Kv8Look known = kv8_look<ROWS>(a, G, 0, lane);
+  int total = 0, items = 0, longest = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += 32) {
+    const Kv8Look k = r0 ? kv8_look<ROWS>(a, G, r0, lane) : known;
+    total += __reduce_add_sync(0xffffffffu, k.units * k.items);
+    items += __reduce_add_sync(0xffffffffu, k.items);
+    longest = max(longest, __reduce_max_sync(0xffffffffu, k.units));
   }
+  const int spare = a.most - items;
+  const int per = max(spare > 0 ? (total + spare - 1) / spare : longest, (longest + MAX_PARTS - 1) / MAX_PARTS);
+  int r = -1, q0, q_len, L, units, pieces, at = blockIdx.x;             // at: of the pieces of the request
+  for (int r0 = 0; r0 < a.requests; r0 += 32) {
+    const Kv8Look k = r0 ? kv8_look<ROWS>(a, G, r0, lane) : known;
+    const int mine = k.items ? (k.units + per - 1) / per : 0;
+    int upto = mine * k.items;
+    const int own = upto;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += y;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, at < upto);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      r = r0 + src;
+      at -= __shfl_sync(0xffffffffu, upto - own, src);
+      units = __shfl_sync(0xffffffffu, k.units, src);
+      pieces = __shfl_sync(0xffffffffu, mine, src);
+      q0 = __shfl_sync(0xffffffffu, k.q0, src);
+      q_len = __shfl_sync(0xffffffffu, k.q_len, src);
+      L = __shfl_sync(0xffffffffu, k.L, src);
+      break;
+    }
+    at -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (r < 0) return;                                                    // more CTAs than pieces
+  const int item = at / pieces, piece = at - item * pieces, tile = item / a.kv_heads, kv_head = item - tile * a.kv_heads;
+  const int rows = q_len * G, row0 = tile * ROWS, here = min(ROWS, rows - row0);
+  const int pos0 = L - q_len, p_first = pos0 + row0 / G, p_last = pos0 + (row0 + here - 1) / G;
+  const int lo_request = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
+  const int each = (units + pieces - 1) / pieces;                       // units of a piece
+  const int key0 = (lo_request / UNIT + piece * each) * UNIT, key_end = min(p_last + 1, key0 + each * UNIT);
+  typename Stream<NT>::Walk walk(a, a.tables + (size_t)r * a.table_stride, kv_head, max(key0, lo) / 16 + warp, key_end > 0 ? (key_end + 15) / 16 : 0,
+                                 WARPS, lane);
+  Stream<NT> st;
+  st.reset();
+  st.load_queries(a, q0, row0, rows, pos0, kv_head, G, lane);
+  st.run(a, walk, a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
+  st.finish();
+  // the warps' sums side by side
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = n * 8 + (lane & 3) * 2 + e;
+      if (row < here) {
+        float* to = sums + (warp * ROWS + row) * PITCH;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) *reinterpret_cast<float2*>(to + kv8_place(i, lane)) = make_float2(st.o[i][n][e], st.o[i][n][2 + e]);
+        if (lane < 4) { sm_m[warp * ROWS + row] = st.m[n][e]; sm_l[warp * ROWS + row] = st.l[n][e]; }
+      }
+    }
+  __syncthreads();
+  auto finish_row = [&](int row, int place, float2 o, float l) {
+    const int full = row0 + row;
+    kv8_store_pair(a.out + ((size_t)(q0 + full / G) * a.heads + kv_head * G + full % G) * D + kv8_place_dim(place), kv8_ratio(o.x, l), kv8_ratio(o.y, l));
+  };
+  float* const mine = a.parts + (size_t)blockIdx.x * ROWS * (D + 2);
+  for (int i = tid; i < here * (D / 2); i += 32 * WARPS) {
+    const int row = i / (D / 2), place = (i - row * (D / 2)) * 2;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_m[w * ROWS + row]);
+    const float U = M == -INFINITY ? 0.f : M;
+    float2 o = make_float2(0.f, 0.f);
+    float l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = kv8_exp2(sm_m[w * ROWS + row] - U);
+      const float2 x = *reinterpret_cast<const float2*>(sums + (w * ROWS + row) * PITCH + place);
+      o.x = fmaf(x.x, f, o.x);
+      o.y = fmaf(x.y, f, o.y);
+      l = fmaf(sm_l[w * ROWS + row], f, l);
+    }
+    if (pieces == 1) {
+      finish_row(row, place, o, l);
+    } else {
+      *reinterpret_cast<float2*>(mine + row * D + place) = o;
+      if (place == 0) { mine[ROWS * D + row] = M; mine[ROWS * (D + 1) + row] = l; }
+    }
+  }
+  if (pieces == 1) return;
+  __threadfence();
+  __syncthreads();
+  int* const counter = a.counters + ((size_t)r * a.tiles + tile) * a.kv_heads + kv_head;
+  if (tid == 0) arrived = atomicAdd(counter, 1);
+  __syncthreads();
+  if (arrived != pieces - 1) return;
+  // the last of the item's pieces to arrive adds them all, in their order
+  __threadfence();
+  const float* const first = mine - (size_t)piece * ROWS * (D + 2);
+  auto part = [&](int c) { return first + (size_t)c * ROWS * (D + 2); };
+  for (int i = tid; i < here * pieces; i += 32 * WARPS) {
+    const float* from = part(i / here) + ROWS * D + i % here;
+    part_m[i / here][i % here] = __ldcg(from);
+    part_l[i / here][i % here] = __ldcg(from + ROWS);
+  }
+  __syncthreads();
+  for (int i = tid; i < here * (D / 2); i += 32 * WARPS) {
+    const int row = i / (D / 2), place = (i - row * (D / 2)) * 2;
+    float M = -INFINITY, l = 0.f;
+    for (int c = 0; c < pieces; ++c) M = fmaxf(M, part_m[c][row]);
+    const float U = M == -INFINITY ? 0.f : M;
+    float2 o = make_float2(0.f, 0.f);
+#pragma unroll 8
+    for (int c = 0; c < pieces; ++c) {
+      const float2 x = __ldcg(reinterpret_cast<const float2*>(part(c) + row * D + place));
+      const float f = kv8_exp2(part_m[c][row] - U);
+      o.x = fmaf(x.x, f, o.x);
+      o.y = fmaf(x.y, f, o.y);
+      l = fmaf(part_l[c][row], f, l);
+    }
+    finish_row(row, place, o, l);
+  }
+  if (tid == 0) *counter = 0;
 }
 
 template <int NT> static size_t kv8_split_smem() { return (size_t)WARPS * 8 * NT * (PITCH + 2) * sizeof(float); }
@@ -668,7 +684,7 @@ template <int NT> static int kv8_split_ctas(int* ctas) {                // that 
 IFB_EXPORT long long ifb_kv8_attention_scratch(int nt) {
   int ctas = 0;
   const int bad = nt == 1 ? kv8_split_ctas<1>(&ctas) : kv8_split_ctas<2>(&ctas);
-  return bad ? (bad > 0 ? -bad : bad) : (long long)ctas * 2 * 8 * nt * (D + 2);
+  return bad ? (bad > 0 ? -bad : bad) : (long long)ctas * 8 * nt * (D + 2);
 }
 
 template <int NT>
@@ -681,7 +697,12 @@ static int kv8_launch(const Kv8Args& a, bool whole, int max_q, cudaStream_t stre
   int ctas = 0;
   const int bad = kv8_split_ctas<NT>(&ctas);
   if (bad) return bad;
-  return ifb_launch(kv8_attention_split_kernel<NT>, dim3(ctas), dim3(32 * WARPS), kv8_split_smem<NT>(), stream, a);
+  // (with more items than CTAs at a time each is one piece, and needs no scratch memory)
+  const long long items = (long long)a.requests * a.tiles * a.kv_heads;
+  if (items > 0x7fffffffLL) return IFB_ERR_SIZE;
+  Kv8Args b = a;
+  b.most = ctas;
+  return ifb_launch(kv8_attention_split_kernel<NT>, dim3(items > ctas ? (unsigned)items : (unsigned)ctas), dim3(32 * WARPS), kv8_split_smem<NT>(), stream, b);
 }
 
 // nt: 1 or 2 tiles of 8 score rows per warp.  whole: the whole form.  Requests of min_rows .. max_rows score rows are worked on.
@@ -697,6 +718,6 @@ IFB_EXPORT int ifb_kv8_attention(const void* q, int dtype, long long q_row, cons
   if ((((uintptr_t)q) | ((uintptr_t)codes) | ((uintptr_t)out) | (uintptr_t)(q_row * sizeof(qtype))) & 15) return IFB_ERR_ALIGN;
   const Kv8Args a = {(const qtype*)q, q_row, (const int8_t*)codes, (const uint8_t*)exponents, (const int*)tables, table_stride, (const int*)cu_q,
                      (const int*)seq_lens, (qtype*)out, (float*)parts, (int*)counters, requests, heads, kv_heads, page_size, window,
-                     scale * 1.4426950408889634f, min_rows, max_rows, tiles};
+                     scale * 1.4426950408889634f, min_rows, max_rows, tiles, 0};
   return nt == 1 ? kv8_launch<1>(a, whole, max_q, (cudaStream_t)stream) : kv8_launch<2>(a, whole, max_q, (cudaStream_t)stream);
 }
