@@ -18,7 +18,9 @@ keys of its own chunk of positions only) as soon as the next query stands in a l
 call that stores) of a group has a tensor ``[pages, 2, kv_heads, page_size, head_dim]``
 (keys and values of one shape), or, for a need whose streams differ in shape (values narrower
 than keys, a latent beside a small rotated key), one tensor ``[pages, heads, page_size, width]``
-per stream; the entries of one group share page ids, so one block table serves them all.
+per stream; the entries of one group share page ids, so one block table serves them all.  With ``cache_format`` "int8" an
+entry of keys and values of one shape is a ``Kv8Pages`` (codes of that shape in 8 bits, an exponent for each page, kind and
+head) in the tensor's place.
 
 State slots.  A request gets a slot id when it is added and returns it when it ends.
 The id is the row of the request in every fixed-size state tensor ``[slots, *shape]``
@@ -112,7 +114,7 @@ class CacheLayout:
 
 class CacheManager:
     def __init__(self, plan: ModelPlan, page_size: int, num_pages, max_requests: int,
-                 dtype=None, device=None, allocate_tensors: bool = True):
+                 dtype=None, device=None, allocate_tensors: bool = True, cache_format: str = "dtype"):
         """``num_pages``: pages of every key/value group (an int), or a dict from group key
         to its count.  ``allocate_tensors`` False gives a manager that only does the
         accounting (tests without a device)."""
@@ -147,7 +149,14 @@ class CacheManager:
             for g in self.kv_groups:
                 st = g.need.streams
                 for cid in g.cache_ids:
-                    if g.uniform:
+                    if cache_format == "int8":
+                        from ..kernels.low_bits import Kv8Pages
+                        if not g.uniform or len(st) != 2:
+                            raise CacheError(f"cache entry {cid}: pages of 8 bits hold keys and values of one shape")
+                        t = Kv8Pages.empty(g.pool.num_pages, st[0].heads, page_size, st[0].width, device)
+                        g.tensors[cid] = t
+                        g.streams[cid] = {x.name: t.codes[:, i] for i, x in enumerate(st)}
+                    elif g.uniform:
                         t = torch.zeros((g.pool.num_pages, len(st), st[0].heads, page_size, st[0].width),
                                         dtype=dtype, device=device)
                         g.tensors[cid] = t

@@ -43,6 +43,10 @@ def build_parser() -> argparse.ArgumentParser:
     eng.add_argument("--page-size", type=int, default=16)
     eng.add_argument("--num-pages", type=int, default=None, help="pages of the key/value pool (default: enough for all slots)")
     eng.add_argument("--max-num-batched-tokens", type=int, default=2048, help="token budget of one step")
+    eng.add_argument("--weight-format", default="stored", choices=("stored", "mx4"),
+                     help="mx4: attention and dense feed-forward matrices (and the rows they multiply) in microscaled 4-bit floating point")
+    eng.add_argument("--cache-format", default="dtype", choices=("dtype", "int8"),
+                     help="int8: keys and values in 8 bits with a scale for each page and head")
     ap.add_argument("--json", action="store_true", help="print a JSON report (prompt ids, generated ids, timings)")
     return ap
 
@@ -94,7 +98,8 @@ def main(argv=None) -> int:
                 return 1
         options = EngineOptions(dtype=args.dtype, device=args.device, page_size=args.page_size, num_pages=args.num_pages,
                                 max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens,
-                                max_model_len=args.max_model_len)
+                                max_model_len=args.max_model_len, weight_format=args.weight_format,
+                                cache_format=args.cache_format)
         t0 = time.perf_counter()
         engine = Engine.from_model_dir(model_dir, options, tokenizer=tokenizer)
         load_ms = (time.perf_counter() - t0) * 1000
@@ -135,7 +140,8 @@ def main(argv=None) -> int:
             report = {
                 "model": {"dir": args.model, "random_weights": args.random_weights, "architecture": config.architecture},
                 "execution": {"device": args.device, "dtype": args.dtype, "max_context": args.max_model_len,
-                              "cache_slots": args.max_num_seqs, "page_size": args.page_size, "load_ms": load_ms,
+                              "cache_slots": args.max_num_seqs, "page_size": args.page_size, "weight_format": args.weight_format,
+                              "cache_format": args.cache_format, "load_ms": load_ms,
                               "timings_ms": {"prefill_ms": step_ms[0] if step_ms else None,
                                              "first_decode_ms": decode[0] if decode else None,
                                              "avg_decode_ms": sum(decode) / len(decode) if decode else None,

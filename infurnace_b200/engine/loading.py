@@ -8,6 +8,7 @@ import torch
 
 from ..cache import CacheManager
 from ..errors import ModelConfigError
+from ..config.specs import AttentionSpec, DenseMLPSpec, GatedMLPSpec, KVCacheNeed, PagedCacheNeed
 from ..models import plan_for, read_config
 from ..parts import DecoderModel, Runtime
 from ..weights.loader import load_weights
@@ -27,6 +28,16 @@ class EngineOptions:
     max_num_batched_tokens: int = 2048         # tokens of one step
     max_model_len: Optional[int] = None        # longest sequence; default: the model's limit
     memory_fraction: float = 0.8               # of free device memory, when num_pages is None
+    weight_format: str = "stored"              # "mx4": attention and dense feed-forward matrices in microscaled 4-bit floating point
+    cache_format: str = "dtype"                # "int8": keys and values in 8 bits with a scale for each page and head
+
+    def check_formats(self):
+        if self.weight_format not in ("stored", "mx4"):
+            raise ModelConfigError(f"weight_format {self.weight_format!r}: choose stored or mx4")
+        if self.cache_format not in ("dtype", "int8"):
+            raise ModelConfigError(f"cache_format {self.cache_format!r}: choose dtype or int8")
+        if self.cache_format == "int8" and (self.page_size % 16 or self.page_size < 16):
+            raise ModelConfigError(f"cache_format int8 wants pages of a multiple of 16 tokens, not {self.page_size}")
 
 
 def parse_dtype(name):
@@ -46,12 +57,15 @@ def build_runner(model_dir: Optional[str], options: EngineOptions, kernels=None,
     device as the parts ask for them (weights/random_init.py), which is how models too large to pass
     through a file get their random weights."""
     dtype = parse_dtype(options.dtype)
+    options.check_formats()
     config = read_config(model_dir) if random is None else random[0]
     plan = plan_for(config)
+    check_plan(plan, options)
     if kernels is None:
         from ..kernels import load_cuda_kernels
         kernels = load_cuda_kernels(progress=progress)
-    runtime = Runtime(device=torch.device(options.device), act_dtype=dtype, kernels=kernels)
+    runtime = Runtime(device=torch.device(options.device), act_dtype=dtype, kernels=kernels,
+                      weight_format=options.weight_format)
     if random is None:
         weights = load_weights(model_dir, plan, dtype, runtime.device, progress=progress)
     else:
@@ -63,9 +77,40 @@ def build_runner(model_dir: Optional[str], options: EngineOptions, kernels=None,
     num_pages = options.num_pages
     if num_pages is None:
         num_pages = default_num_pages(plan, options, dtype, runtime.device, max_len)
-    cache = CacheManager(plan, options.page_size, num_pages, options.max_num_seqs, dtype=dtype, device=runtime.device)
+    cache = CacheManager(plan, options.page_size, num_pages, options.max_num_seqs, dtype=dtype, device=runtime.device,
+                         cache_format=options.cache_format)
     runner = ModelRunner(model, cache, runtime, options.max_num_batched_tokens, max_len)
     return config, plan, runner
+
+
+def check_plan(plan, options) -> None:
+    """Refuse formats that a model's parts do not have, before anything is loaded.  4 bits: attention and dense feed-forwards,
+    whose every width is a multiple of 32 (other parts' matrices stay as stored, but a model without any such part is refused).
+    8-bit pages: every mixer that keeps keys and values is plain grouped-query attention with heads of a multiple of 16."""
+    def parts(layer):
+        return [x for x in (getattr(layer, "mixer", None), getattr(layer, "ffn", None)) if x is not None]
+    if options.weight_format == "mx4":
+        widths = []
+        for part in (p for layer in plan.layers for p in parts(layer)):
+            if isinstance(part, AttentionSpec):
+                widths += [part.hidden_size, part.num_heads * part.head_dim]
+            elif isinstance(part, (GatedMLPSpec, DenseMLPSpec)):
+                widths += [part.hidden_size, part.intermediate_size]
+        if not widths:
+            raise ModelConfigError("weight_format mx4: the model has neither grouped-query attention nor a dense feed-forward")
+        if any(w % 32 for w in widths):
+            raise ModelConfigError(f"weight_format mx4: widths are multiples of 32, not {sorted({w for w in widths if w % 32})}")
+    if options.cache_format == "int8":
+        for call in plan.resolved_schedule():
+            layer = plan.layers[call.layer]
+            need = layer.cache_need()
+            for sub in need if isinstance(need, tuple) else (need,):
+                if isinstance(sub, (KVCacheNeed, PagedCacheNeed)):
+                    mixer = getattr(layer, "mixer", None)
+                    if not isinstance(mixer, AttentionSpec):
+                        raise ModelConfigError(f"cache_format int8: {type(mixer or layer).__name__} reads its pages in the engine's dtype")
+                    if mixer.head_dim % 16 or not 16 <= mixer.head_dim <= 256:
+                        raise ModelConfigError(f"cache_format int8: head_dim is a multiple of 16 up to 256, not {mixer.head_dim}")
 
 
 def default_num_pages(plan, options, dtype, device, max_len) -> int:
@@ -74,7 +119,7 @@ def default_num_pages(plan, options, dtype, device, max_len) -> int:
     from ..cache import CacheLayout
     layout = CacheLayout(plan)
     per_page = 0
-    esize = torch.empty((), dtype=dtype).element_size()
+    esize = 1 if options.cache_format == "int8" else torch.empty((), dtype=dtype).element_size()
     for need, ids in layout.kv.values():
         per_page += len(ids) * sum(x.heads * x.width for x in need.streams) * options.page_size * esize
     want = options.max_num_seqs * (-(-max_len // options.page_size)) + 1

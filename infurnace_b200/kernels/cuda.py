@@ -15,7 +15,7 @@ import torch
 
 from ..errors import KernelError
 from .build import load_library
-from .low_bits import LowBitKernels
+from .low_bits import LowBitKernels, Mx4Matrix
 
 F32, BF16 = 0, 1
 # the `epilogue` argument of the products: 0 plain, 1 silu_gate (w holds gate rows, then up rows), 16 * u: plain with the
@@ -224,10 +224,15 @@ class CudaKernels(LowBitKernels):
 
     # ------------------------------------------------------------------ matrix products
     def linear(self, x, w, out, epilogue="none", row_scale=None, bias=None):
-        """out = x w^T with the epilogue (a key of ``EPILOGUES``).  ``row_scale`` (partials, parts, eps, width), from
+        """out = x w^T with the epilogue (a key of ``EPILOGUES``).  ``w`` in 4 bits (an ``Mx4Matrix``): :meth:`mx4_linear`, without
+        row scale and bias.  ``row_scale`` (partials, parts, eps, width), from
         :meth:`linear_residual_norm`, multiplies row n by rsqrt(sum_p partials[p, n] / width + eps)
         before the epilogue; only where :meth:`can_fold_norm` says so.  ``bias`` float32 [out features] is added after that
         and before a unary function (not with "silu_gate")."""
+        if isinstance(w, Mx4Matrix):
+            if row_scale is not None or bias is not None:
+                raise KernelError("linear: a 4-bit matrix takes neither a row scale nor a bias")
+            return self.mx4_linear(x, w, out, epilogue)
         _dense(x, "x"), _dense(w, "w"), _dense(out, "out")
         n, k = x.shape
         o = out.shape[1]

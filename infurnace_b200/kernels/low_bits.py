@@ -293,12 +293,10 @@ class LowBitKernels:
         return held["graph" if capturing else stream]
 
     kv8_expand_rows = 64             # score rows of the longest request from which prompts' pages are expanded for the tcgen05 kernel
+    kv8_expand_bytes = 4 << 30       # room for expanded pages that a call may take
 
-    def _kv8_attention_tc(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, n, r, heads, kv_heads,
-                          group):
+    def _kv8_attention_tc(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r, heads, kv_heads, group, most, room):
         """The requests with more than 16 score rows: their pages as bfloat16 (exact), and the tcgen05 kernel over those."""
-        most = -(-max_seq_len // pages.page_size)
-        room = most * min(r, n // (16 // group + 1))                      # a long request has so many tokens at least
         device, ps, dim = q.device, pages.page_size, pages.head_dim
         wide = torch.empty((room, 2, kv_heads, ps, dim), dtype=torch.bfloat16, device=device)
         tables = torch.empty((r, most), dtype=torch.int32, device=device)
@@ -311,12 +309,14 @@ class LowBitKernels:
                                    heads, kv_heads, 1, dim, dim, (at, stride, ps), (at + 2 * kv_heads * ps * dim, stride, ps), room, tables, cu_q,
                                    seq_lens, out, scale, int(window), max_q_len, n, r, 2, None, None, kind=0)
 
-    def kv8_attention(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, min_q_len=1):
+    def kv8_attention(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, min_q_len=1,
+                      exact_lens=False):
         """Causal attention of a step's queries over 8-bit pages: ``q`` and ``out`` bfloat16 or float32 [tokens, heads, head_dim] (the
         rows of ``q`` may lie apart, those of ``out`` not); the query at position p sees positions max(0, p - window + 1) .. p
         (``window`` 0: from 0); request r has the rows cu_q[r] .. cu_q[r + 1] - 1 and ``seq_lens[r]`` keys, these queries' own
         among them.  A row that sees no key becomes zero.  No request has more than ``max_q_len`` queries or ``max_seq_len``
-        keys, none fewer than ``min_q_len`` queries."""
+        keys, none fewer than ``min_q_len`` queries; ``exact_lens``: some request has ``max_q_len``, and ``q`` no other rows than
+        theirs, which bounds how many are long."""
         code = _CODES.get(q.dtype)
         n, heads, dim = q.shape
         kv_heads = pages.kv_heads
@@ -343,13 +343,17 @@ class LowBitKernels:
         # score rows beyond which a request's tiles fill the device by themselves and run whole; requests below run split
         rows, least = max_q_len * group, min_q_len * group
         limit = 64
-        if self.kv8_expand_rows and rows > self.kv8_expand_rows and q.dtype == torch.bfloat16 and dim == 128 and 128 % group == 0 \
-                and pages.page_size in (16, 32, 64) and self.attention_tc:
-            self._kv8_attention_tc(q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, n, r, heads, kv_heads, group)
-            if least > 16:
-                return out
-            limit = rows = 16
-        nt = 1 if rows <= 8 or dim > 128 else 2
+        if rows > self.kv8_expand_rows and q.dtype == torch.bfloat16 and dim == 128 and 128 % group == 0 and pages.page_size in (16, 32, 64) \
+                and self.attention_tc:
+            # (a long request has more than 16 score rows)
+            most = -(-max_seq_len // pages.page_size)
+            room = most * (self.long_requests(n, r, group, max_q_len, min_q_len) if exact_lens else min(r, n // (16 // group + 1)))
+            if room * pages.page_size * kv_heads * dim * 4 <= self.kv8_expand_bytes:
+                self._kv8_attention_tc(q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r, heads, kv_heads, group, most, room)
+                if least > 16:
+                    return out
+                limit = rows = 16
+        nt = 1 if rows <= 8 or dim > 128 or limit == 16 and group <= 8 else 2      # (beside prompts the short requests decode)
         fixed = (q.data_ptr(), code, q.stride(0), *pages._at, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
                  seq_lens.data_ptr(), out.data_ptr())
         sizes = (r, heads, kv_heads, pages.page_size, dim, float(scale), int(window))

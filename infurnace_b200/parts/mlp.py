@@ -23,8 +23,8 @@ class GatedMLP:
         self.spec = spec
         self.rt = runtime
         self.k = runtime.kernels
-        self.w_gate_up = torch.cat((weights[spec.gate_proj], weights[spec.up_proj]), dim=0).contiguous()
-        self.w_down = weights[spec.down_proj]
+        self.w_gate_up = runtime.matrix(torch.cat((weights[spec.gate_proj], weights[spec.up_proj]), dim=0).contiguous(), gated=True)
+        self.w_down = runtime.matrix(weights[spec.down_proj])
 
     can_fold_output = True
 
@@ -64,8 +64,8 @@ class DenseMLP:
         self.spec = spec
         self.rt = runtime
         self.k = runtime.kernels
-        self.w_up = weights[spec.up_proj]
-        self.w_down = weights[spec.down_proj]
+        self.w_up = runtime.matrix(weights[spec.up_proj])
+        self.w_down = runtime.matrix(weights[spec.down_proj])
 
     def forward(self, h, ctx, fold=None, out=None):
         n = h.shape[0]

@@ -102,3 +102,8 @@ class Runtime:
     device: Any
     act_dtype: Any
     kernels: Any
+    weight_format: str = "stored"      # "mx4": the matrices that parts pass through ``matrix`` are kept in 4 bits
+
+    def matrix(self, w, gated=False):
+        """A matrix as the products take it: the tensor, or its 4-bit form (``gated``: gate rows, then up rows)."""
+        return self.kernels.mx4_matrix(w, gated=gated) if self.weight_format == "mx4" else w

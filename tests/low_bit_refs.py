@@ -4,6 +4,8 @@ import math
 
 import torch
 
+from kernel_refs import ReferenceKernels
+
 LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
@@ -105,3 +107,36 @@ def attention8(q, codes, fields, tables, cu_q, seq_lens, scale, window=0):
             mag[a:b, h] = torch.einsum("tn,tnd->td", w, v.abs())
             reach[a:b, h] = scale * x.abs().sum(1) * 256 * step[:, h // group].max()
     return out, mag, reach
+
+
+class LowBitReference(ReferenceKernels):
+    """The stand-in kernel set with the operators over few bits: a 4-bit matrix is its values, pages are the package's."""
+
+    def mx4_matrix(self, w, gated=False):
+        return FourBits(round4(w.float())[2])
+
+    def linear(self, x, w, out, epilogue="none", row_scale=None, bias=None):
+        if isinstance(w, FourBits):
+            assert row_scale is None and bias is None
+            x, w = round4(x.float())[2], w.values
+        super().linear(x, w, out, epilogue, row_scale, bias)
+
+    def can_fold_norm(self, n, dtype, w, epilogue="none"):
+        return not isinstance(w, FourBits) and super().can_fold_norm(n, dtype, w, epilogue)
+
+    def kv8_store(self, k, v, slot_mapping, pages):
+        codes, fields = store8(pages.codes, pages.exponents, k, v, slot_mapping)
+        pages.codes.copy_(codes.to(torch.int8))
+        pages.exponents.copy_(fields.to(torch.uint8))
+
+    def kv8_attention(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, min_q_len=1, exact_lens=False):
+        assert max_seq_len <= block_tables.shape[1] * pages.page_size
+        out.copy_(attention8(q, pages.codes, pages.exponents, block_tables, cu_q, seq_lens, scale, window)[0].to(out.dtype))
+
+
+class FourBits:
+    """A matrix rounded to 4 bits, as its values."""
+    dtype = torch.uint8
+
+    def __init__(self, values):
+        self.values, self.shape = values, values.shape
