@@ -28,23 +28,32 @@ __device__ __forceinline__ int kv8_code(float x, uint32_t f) {
   else t = __fmul_rd(__fmul_rd(x, __uint_as_float((254u - f) << 23)), 64.f);      // a factor that no float holds
   return (int)floorf(t);
 }
-__device__ __forceinline__ void kv8_load8(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void kv8_load8(const bf16* p, float (&v)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-
 // A warp per (run of rows, kind, head).  A run is the adjacent rows whose slots follow one another in one page; its first row's
-// warp has the whole run, the other rows' warps leave.  (A page's rows must be one run: the caller's contract.)  The rows are
-// read twice, for the largest and for the codes; the second time they come from the first level of cache.
+// warp has the whole run, the other rows' warps leave.  (A page's rows must be one run: the caller's contract.)  A lane keeps HELD
+// pieces of eight numbers in registers between the search for the largest and the rounding (a page of 16 tokens of heads of 128
+// in bfloat16 whole); of longer runs the rest is read again, from the first level of cache.
+template <typename T> struct Piece8;
+template <> struct Piece8<bf16> {
+  uint4 w;
+  __device__ __forceinline__ void load(const bf16* p) { w = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void clear() { w = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void numbers(float (&v)[8]) const {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(x[i] << 16);
+      v[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+    }
+  }
+};
+template <> struct Piece8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
+  __device__ __forceinline__ void clear() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void numbers(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+};
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv8_store_kernel(const T* k, const T* v, long long k_row, long long v_row, const int* slots, int8_t* codes, uint8_t* exponents, int rows,
@@ -71,14 +80,28 @@ kv8_store_kernel(const T* k, const T* v, long long k_row, long long v_row, const
   uint8_t* const exponent = exponents + ((size_t)page * 2 + kind) * heads + head;
   const uint32_t old = first ? *exponent : 0u;
   const int pieces = dim / 8, total = n * pieces;
+  constexpr int HELD = sizeof(T) == 2 ? 8 : 4;
+  auto at = [&](int i) { const int r = i / pieces; return src + r * pitch + (i - r * pieces) * 8; };
+  Piece8<T> held[HELD];
+#pragma unroll
+  for (int j = 0; j < HELD; ++j) {
+    if (lane + 32 * j < total) held[j].load(at(lane + 32 * j));
+    else held[j].clear();
+  }
   uint32_t m = 0;
-#pragma unroll 4
-  for (int i = lane; i < total; i += 32) {
-    const int r = i / pieces;
+  auto largest = [&](const Piece8<T>& p) {
     float x[8];
-    kv8_load8(src + r * pitch + (i - r * pieces) * 8, x);
+    p.numbers(x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+  };
+#pragma unroll
+  for (int j = 0; j < HELD; ++j) largest(held[j]);
+#pragma unroll 4
+  for (int i = lane + 32 * HELD; i < total; i += 32) {
+    Piece8<T> p;
+    p.load(at(i));
+    largest(p);
   }
   m = __reduce_max_sync(0xffffffffu, m);
   const uint32_t f = max(old, m >> 23);
@@ -107,15 +130,23 @@ kv8_store_kernel(const T* k, const T* v, long long k_row, long long v_row, const
     }
   }
   if (!first && lane == 0) *exponent = (uint8_t)f;
-#pragma unroll 4
-  for (int i = lane; i < total; i += 32) {
+  auto round = [&](int i, const Piece8<T>& p) {
     const int r = i / pieces, c = i - r * pieces;
     float x[8];
-    kv8_load8(src + r * pitch + c * 8, x);
+    p.numbers(x);
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)kv8_code(x[j], f) & 255u) << (8 * (j & 3));
     *reinterpret_cast<uint2*>(to + (size_t)(first + r) * dim + c * 8) = make_uint2(w[0], w[1]);
+  };
+#pragma unroll
+  for (int j = 0; j < HELD; ++j)
+    if (lane + 32 * j < total) round(lane + 32 * j, held[j]);
+#pragma unroll 4
+  for (int i = lane + 32 * HELD; i < total; i += 32) {
+    Piece8<T> p;
+    p.load(at(i));
+    round(i, p);
   }
 }
 

@@ -39,94 +39,132 @@ __device__ __forceinline__ uint32_t mx_codes8(const float (&v)[8], float inv) {
         "f"(v[6] * inv), "f"(v[7] * inv));
   return r;
 }
-__device__ __forceinline__ void mx_load8(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void mx_load8(const bf16* p, float (&v)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-__device__ __forceinline__ uint32_t mx_amax_bits(const float (&v)[8]) {
-  // magnitudes compared as integers: a NaN is larger than infinity, and neither is lost
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  return m;
-}
 __host__ __device__ __forceinline__ size_t mx_scale_at(int row, int block, int k_tiles) {
   return ((size_t)(row >> 7) * k_tiles + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 
-// Four neighbouring lanes have a block: eight elements (16 or 32 bytes of input, 4 of output) each.  16 lanes have the four
-// blocks whose scales lie in one 32-bit word.  A grid row walks over rows; the columns of a row are spread over the grid's x.
-template <typename T>
+// 16 numbers as the words they come in, and their largest magnitude as float32 bits.
+template <typename T> struct MxSixteen;
+template <> struct MxSixteen<bf16> {
+  uint4 w[2];
+  __device__ __forceinline__ void load(const bf16* p) {
+    w[0] = reinterpret_cast<const uint4*>(p)[0];
+    w[1] = reinterpret_cast<const uint4*>(p)[1];
+  }
+  __device__ __forceinline__ uint32_t word(int i) const { const uint4& x = w[i >> 2]; return (i & 3) == 0 ? x.x : (i & 3) == 1 ? x.y : (i & 3) == 2 ? x.z : x.w; }
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, word(i) & 0x7fff7fffu);
+    return max(m << 16, m & 0xffff0000u);
+  }
+  __device__ __forceinline__ float at(int i) const { return __uint_as_float(i & 1 ? word(i >> 1) & 0xffff0000u : word(i >> 1) << 16); }
+};
+template <> struct MxSixteen<float> {
+  float4 w[4];
+  __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const float4*>(p)[i];
+  }
+  __device__ __forceinline__ float at(int i) const { const float4& x = w[i >> 2]; return (i & 3) == 0 ? x.x : (i & 3) == 1 ? x.y : (i & 3) == 2 ? x.z : x.w; }
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    // magnitudes compared as integers: a NaN is larger than infinity, and neither is lost
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(at(i)) & 0x7fffffffu);
+    return m;
+  }
+};
+
+// Two neighbouring lanes have a block: 16 elements (32 or 64 bytes of input, 8 of output) each.  8 lanes have the four blocks whose
+// scales lie in one 32-bit word.  The columns of a row are spread over the grid's x; a thread has PER rows, all of them requested
+// at once (a large matrix: one row per thread is a load's latency per CTA of little work).
+template <typename T, int PER>
 __global__ void __launch_bounds__(256)
 mx4_quantize_kernel(const T* x, long long row_stride, uint8_t* codes, uint8_t* scales, int rows, int k, int gated_rows) {
   ifb_pdl_wait();
   ifb_pdl_trigger();
   const int k_tiles = (k + 127) / 128;
-  const int e = (blockIdx.x * 256 + threadIdx.x) * 8;                  // of the row's elements, padded to 128
+  const int e = (blockIdx.x * 256 + threadIdx.x) * 16;                 // of the row's elements, padded to 128
   const uint32_t lanes = __ballot_sync(0xffffffffu, e < k_tiles * 128);
-  if (e >= k_tiles * 128) return;                                      // 16 lanes leave together
-  const int row = blockIdx.y;                                          // of the result
-  const int from = gated_rows ? (row & 1) * gated_rows + (row >> 1) : row;
+  if (e >= k_tiles * 128) return;                                      // 8 lanes leave together
+  const int row0 = blockIdx.y * PER;                                   // of the result
   const bool in = e < k;
-  float v[8] = {};
-  if (in) mx_load8(x + (size_t)from * row_stride + e, v);
-  uint32_t m = mx_amax_bits(v);
-  m = max(m, __shfl_xor_sync(lanes, m, 1));
-  m = max(m, __shfl_xor_sync(lanes, m, 2));
-  const uint32_t s = mx_scale_byte(__uint_as_float(m));
-  if (in) *reinterpret_cast<uint32_t*>(codes + (size_t)row * (k / 2) + e / 2) = mx_codes8(v, mx_inverse_scale(s));
-  uint32_t word = (in ? s : 0u) << ((threadIdx.x & 12) * 2);
-  word |= __shfl_xor_sync(lanes, word, 4);
-  word |= __shfl_xor_sync(lanes, word, 8);
-  if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(row, e / MX_BLOCK, k_tiles)) = word;
+  MxSixteen<T> v[PER];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int row = min(row0 + p, rows - 1), from = gated_rows ? (row & 1) * gated_rows + (row >> 1) : row;
+    v[p].load(x + (size_t)from * row_stride + (in ? e : 0));
+  }
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int row = row0 + p;
+    uint32_t m = v[p].amax_bits();
+    m = max(m, __shfl_xor_sync(lanes, m, 1));
+    const uint32_t s = mx_scale_byte(__uint_as_float(m));
+    uint32_t word = (in ? s : 0u) << ((threadIdx.x & 6) * 4);
+    word |= __shfl_xor_sync(lanes, word, 2);
+    word |= __shfl_xor_sync(lanes, word, 4);
+    if (row >= rows) continue;
+    if (in) {
+      const float inv = mx_inverse_scale(s);
+      float a[8], b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { a[i] = v[p].at(i); b[i] = v[p].at(8 + i); }
+      *reinterpret_cast<uint2*>(codes + (size_t)row * (k / 2) + e / 2) = make_uint2(mx_codes8(a, inv), mx_codes8(b, inv));
+    }
+    if ((threadIdx.x & 7) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(row, e / MX_BLOCK, k_tiles)) = word;
+  }
 }
 
-template <typename T> __device__ __forceinline__ void mx_store8(T* p, const float (&v)[8]);
-template <> __device__ __forceinline__ void mx_store8<float>(float* p, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+// The values of eight codes in pairs of bfloat16, which holds them exactly.  The bits "ee m" of a code at the lowest end of a bfloat16's
+// exponent and the top of its fraction are the code's magnitude times 2^-126, subnormal numbers included, so two products with
+// powers of two (2^126, and the scale) are the value.
+__device__ __forceinline__ uint32_t mx_times(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("mul.rn.bf16x2 %0, %1, %2;\n" : "=r"(y) : "r"(a), "r"(b));
+  return y;
 }
-template <> __device__ __forceinline__ void mx_store8<bf16>(bf16* p, const float (&v)[8]) {
-  uint32_t w[4];
+__device__ __forceinline__ void mx_values8(uint32_t c, uint32_t s, uint32_t (&v)[4]) {
+  const uint32_t one = s == 255u ? 0x7fffu : s ? s << 7 : 0x0040u, scale = one * 0x00010001u;      // 2^(s - 127); 255: NaN
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    const uint32_t n = c >> (8 * i), x = (n & 15u) | (n & 0xf0u) << 12;
+    v[i] = mx_times(mx_times((x & 0x00070007u) << 6 | (x & 0x00080008u) << 12, 0x7e807e80u), scale);
   }
-  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ float mx_value(uint32_t code) {             // of one element, in units of its block's scale
-  const uint32_t e = (code >> 1) & 3u, m = code & 1u;
-  const float mag = e ? __uint_as_float(((126u + e) << 23) | (m << 22)) : 0.5f * (float)m;
-  return code & 8u ? -mag : mag;
+template <typename T> __device__ __forceinline__ void mx_store8(T* p, const uint32_t (&v)[4]);
+template <> __device__ __forceinline__ void mx_store8<bf16>(bf16* p, const uint32_t (&v)[4]) { *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]); }
+template <> __device__ __forceinline__ void mx_store8<float>(float* p, const uint32_t (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    reinterpret_cast<uint4*>(p)[i] = make_uint4(v[2 * i] << 16, v[2 * i] & 0xffff0000u, v[2 * i + 1] << 16, v[2 * i + 1] & 0xffff0000u);
 }
-__device__ __forceinline__ float mx_scale(uint32_t s) {                // 2^(s - 127); s = 0 is a subnormal number; 255: NaN
-  return __uint_as_float(s == 255u ? 0x7fffffffu : s ? s << 23 : 0x00400000u);
-}
-template <typename T>
+template <typename T, int PER>
 __global__ void __launch_bounds__(256)
 mx4_values_kernel(const uint8_t* codes, const uint8_t* scales, T* out, int rows, int k, int gated_rows) {
   ifb_pdl_wait();
   ifb_pdl_trigger();
   const int e = (blockIdx.x * 256 + threadIdx.x) * 8;
   if (e >= k) return;
-  const int row = blockIdx.y;
-  const int to = gated_rows ? (row & 1) * gated_rows + (row >> 1) : row;
-  const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + (size_t)row * (k / 2) + e / 2);
-  const float f = mx_scale(scales[mx_scale_at(row, e / MX_BLOCK, (k + 127) / 128)]);
-  float v[8];
+  const int row0 = blockIdx.y * PER, k_tiles = (k + 127) / 128;
+  uint32_t c[PER];
+  uint32_t s[PER];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = mx_value((c >> (4 * i)) & 15u) * f;
-  mx_store8<T>(out + (size_t)to * k + e, v);
+  for (int p = 0; p < PER; ++p) {
+    const int row = min(row0 + p, rows - 1);
+    c[p] = *reinterpret_cast<const uint32_t*>(codes + (size_t)row * (k / 2) + e / 2);
+    s[p] = scales[mx_scale_at(row, e / MX_BLOCK, k_tiles)];
+  }
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int row = row0 + p;
+    if (row >= rows) break;
+    const int to = gated_rows ? (row & 1) * gated_rows + (row >> 1) : row;
+    uint32_t v[4];
+    mx_values8(c[p], s[p], v);
+    mx_store8<T>(out + (size_t)to * k + e, v);
+  }
 }
 
 static int mx_sizes(int rows, int k, int gated) {
@@ -134,54 +172,60 @@ static int mx_sizes(int rows, int k, int gated) {
   return IFB_OK;
 }
 
-IFB_EXPORT int ifb_mx4_quantize(const void* x, int dtype, long long row_stride, void* codes, void* scales, int rows, int k, int gated,
-                                void* stream) {
-  int bad = mx_sizes(rows, k, gated);
-  if (bad) return bad;
-  const int esize = dtype == IFB_F32 ? 4 : 2;
-  if (dtype != IFB_F32 && dtype != IFB_BF16) return IFB_ERR_DTYPE;
-  if ((((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)scales) | (uintptr_t)(row_stride * esize)) & 15) return IFB_ERR_ALIGN;
-  const int threads = (k + 127) / 128 * 16;
-  for (int r0 = 0; r0 < rows; r0 += 65536 - 256) {      // a grid has at most 65,535 rows; whole tiles of rows, whole pairs
-    const int n = min(rows - r0, 65536 - 256);
-    // (a gated matrix has its rows from two places, so one launch has to hold it)
-    if (gated && n != rows) return IFB_ERR_SIZE;
-    const dim3 grid((threads + 255) / 256, n);
-    uint8_t* c = (uint8_t*)codes + (size_t)r0 * (k / 2);
-    uint8_t* s = (uint8_t*)scales + (size_t)(r0 / 128) * ((k + 127) / 128) * 512;
-    int e;
-    if (dtype == IFB_F32)
-      e = ifb_launch(mx4_quantize_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, (const float*)x + (size_t)r0 * row_stride,
-                     row_stride, c, s, n, k, gated ? rows / 2 : 0);
-    else
-      e = ifb_launch(mx4_quantize_kernel<bf16>, grid, dim3(256), 0, (cudaStream_t)stream, (const bf16*)x + (size_t)r0 * row_stride,
-                     row_stride, c, s, n, k, gated ? rows / 2 : 0);
+// Rows per thread: four where that still gives every SM several CTAs.
+static int mx_rows_per_thread(int rows, int k) { return (long long)rows * k >= (long long)ifb_sm_count() * 65536 ? 4 : 1; }
+constexpr int MX_GRID_ROWS = 65535 / 256 * 256;      // a grid has at most 65,535 rows; whole tiles of rows, whole pairs
+
+template <typename T, int PER>
+static int mx_quantize_launch(const void* x, long long row_stride, void* codes, void* scales, int rows, int k, int gated, cudaStream_t stream) {
+  // (a gated matrix has its rows from two places, so one launch has to hold it)
+  if (gated && (rows + PER - 1) / PER > MX_GRID_ROWS) return IFB_ERR_SIZE;
+  for (long long r0 = 0; r0 < rows; r0 += (long long)MX_GRID_ROWS * PER) {
+    const int n = (int)(rows - r0 < (long long)MX_GRID_ROWS * PER ? rows - r0 : (long long)MX_GRID_ROWS * PER);
+    const dim3 grid(((k + 127) / 128 * 8 + 255) / 256, (n + PER - 1) / PER);
+    const int e = ifb_launch(mx4_quantize_kernel<T, PER>, grid, dim3(256), 0, stream, (const T*)x + (size_t)r0 * row_stride, row_stride,
+                             (uint8_t*)codes + (size_t)r0 * (k / 2), (uint8_t*)scales + (size_t)(r0 / 128) * ((k + 127) / 128) * 512, n, k,
+                             gated ? rows / 2 : 0);
     if (e) return e;
   }
   return IFB_OK;
 }
-
-IFB_EXPORT int ifb_mx4_values(const void* codes, const void* scales, void* out, int dtype, int rows, int k, int gated, void* stream) {
-  int bad = mx_sizes(rows, k, gated);
+IFB_EXPORT int ifb_mx4_quantize(const void* x, int dtype, long long row_stride, void* codes, void* scales, int rows, int k, int gated,
+                                void* stream) {
+  const int bad = mx_sizes(rows, k, gated);
   if (bad) return bad;
+  const int esize = dtype == IFB_F32 ? 4 : 2;
   if (dtype != IFB_F32 && dtype != IFB_BF16) return IFB_ERR_DTYPE;
-  if ((((uintptr_t)out) | ((uintptr_t)codes) | ((uintptr_t)scales)) & 15) return IFB_ERR_ALIGN;
-  for (int r0 = 0; r0 < rows; r0 += 65536 - 256) {
-    const int n = min(rows - r0, 65536 - 256);
-    if (gated && n != rows) return IFB_ERR_SIZE;
-    const dim3 grid((k / 8 + 255) / 256, n);
-    const uint8_t* c = (const uint8_t*)codes + (size_t)r0 * (k / 2);
-    const uint8_t* s = (const uint8_t*)scales + (size_t)(r0 / 128) * ((k + 127) / 128) * 512;
-    int e;
-    if (dtype == IFB_F32)
-      e = ifb_launch(mx4_values_kernel<float>, grid, dim3(256), 0, (cudaStream_t)stream, c, s, (float*)out + (size_t)r0 * k, n, k,
-                     gated ? rows / 2 : 0);
-    else
-      e = ifb_launch(mx4_values_kernel<bf16>, grid, dim3(256), 0, (cudaStream_t)stream, c, s, (bf16*)out + (size_t)r0 * k, n, k,
-                     gated ? rows / 2 : 0);
+  if ((((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)scales) | (uintptr_t)(row_stride * esize)) & 15) return IFB_ERR_ALIGN;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (mx_rows_per_thread(rows, k) == 4)
+    return dtype == IFB_F32 ? mx_quantize_launch<float, 4>(x, row_stride, codes, scales, rows, k, gated, st)
+                            : mx_quantize_launch<bf16, 4>(x, row_stride, codes, scales, rows, k, gated, st);
+  return dtype == IFB_F32 ? mx_quantize_launch<float, 1>(x, row_stride, codes, scales, rows, k, gated, st)
+                          : mx_quantize_launch<bf16, 1>(x, row_stride, codes, scales, rows, k, gated, st);
+}
+
+template <typename T, int PER>
+static int mx_values_launch(const void* codes, const void* scales, void* out, int rows, int k, int gated, cudaStream_t stream) {
+  if (gated && (rows + PER - 1) / PER > MX_GRID_ROWS) return IFB_ERR_SIZE;
+  for (long long r0 = 0; r0 < rows; r0 += (long long)MX_GRID_ROWS * PER) {
+    const int n = (int)(rows - r0 < (long long)MX_GRID_ROWS * PER ? rows - r0 : (long long)MX_GRID_ROWS * PER);
+    const dim3 grid((k / 8 + 255) / 256, (n + PER - 1) / PER);
+    const int e = ifb_launch(mx4_values_kernel<T, PER>, grid, dim3(256), 0, stream, (const uint8_t*)codes + (size_t)r0 * (k / 2),
+                             (const uint8_t*)scales + (size_t)(r0 / 128) * ((k + 127) / 128) * 512, (T*)out + (size_t)r0 * k, n, k, gated ? rows / 2 : 0);
     if (e) return e;
   }
   return IFB_OK;
+}
+IFB_EXPORT int ifb_mx4_values(const void* codes, const void* scales, void* out, int dtype, int rows, int k, int gated, void* stream) {
+  const int bad = mx_sizes(rows, k, gated);
+  if (bad) return bad;
+  if (dtype != IFB_F32 && dtype != IFB_BF16) return IFB_ERR_DTYPE;
+  if ((((uintptr_t)out) | ((uintptr_t)codes) | ((uintptr_t)scales)) & 15) return IFB_ERR_ALIGN;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (mx_rows_per_thread(rows, k) == 4)
+    return dtype == IFB_F32 ? mx_values_launch<float, 4>(codes, scales, out, rows, k, gated, st) : mx_values_launch<bf16, 4>(codes, scales, out, rows, k, gated, st);
+  return dtype == IFB_F32 ? mx_values_launch<float, 1>(codes, scales, out, rows, k, gated, st) : mx_values_launch<bf16, 1>(codes, scales, out, rows, k, gated, st);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -200,7 +244,9 @@ IFB_EXPORT int ifb_mx4_values(const void* codes, const void* scales, void* out, 
 // What does not depend on the kernel before this one, the matrix, is requested before the wait for it.
 // ROUND: the rows come as numbers, and the epilogue's warps, idle until then, round a stage's 256 of k of them (a thread a block
 // of 32) into the stage, where TMA would have put them: every CTA rounds all rows of its part of k, which for few rows is little
-// beside its part of the matrix, and a launch and a trip through memory are saved.
+// beside its part of the matrix, and a launch and a trip through memory are saved.  The numbers are requested some stages ahead
+// (one ahead: 8 rows of 12,288 by 4,096 11.1 us, four 8.3; with a kernel of its own for the rounding 8.9).  From 33 rows on the
+// rounding takes longer than the matrix (24,576 x 4,096: 25 us, 15.5 with the kernel of its own).
 // Waits are bounded: after a limit a thread records a code in `*err`, raises the CTA's abort flag, and all fall through to the
 // end, where the tensor memory is given back.
 // ---------------------------------------------------------------------------------------------
@@ -414,11 +460,12 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
     ifb_pdl_wait();
     if constexpr (ROUND) {
       if (warp >= 2) {
-        // blocks 32 EPI_WARPS apart; a block's numbers are requested a stage ahead
+        // a thread's blocks lie THREADS apart; AHEAD stages' numbers are under way
         constexpr int THREADS = 32 * C::EPI_WARPS, PER = C::NT * 8 / THREADS, W = sizeof(TX) == 2 ? 16 : 32;
+        constexpr int AHEAD = PER * W <= 16 ? 4 : PER * W <= 32 ? 2 : 1;
         const int tid = threadIdx.x - 64;
-        uint32_t w[PER][W];
-        auto request = [&](int s) {
+        uint32_t ring[AHEAD][PER][W];
+        auto request = [&](int s, uint32_t (&w)[PER][W]) {
 #pragma unroll
           for (int b = 0; b < PER; ++b) {
             const int at = tid + b * THREADS, row = at >> 3, e = (s * 8 + (at & 7)) * MX_BLOCK;
@@ -431,15 +478,21 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
             }
           }
         };
-        request(s0);
-        for (int s = s0; s < s1; ++s) {
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) request(s0 + q, ring[q]);      // (beyond the part of k: read and not used, or zeros)
+        bool go = true;
+        for (int s8 = s0; s8 < s1 && go; s8 += AHEAD)
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+          const int s = s8 + q;
+          if (s >= s1) break;
           const int j = s - s0, i = j % C::STAGES;
           uint4 codes[PER];
           uint32_t scale[PER];
 #pragma unroll
-          for (int b = 0; b < PER; ++b) codes[b] = mx_round32(w[b], scale[b]);
-          if (s + 1 < s1) request(s + 1);
-          if (j >= C::STAGES && !mx_wait(&empty[i], ((j / C::STAGES) & 1) ^ 1, abort_flag, err, 704)) break;
+          for (int b = 0; b < PER; ++b) codes[b] = mx_round32(ring[q][b], scale[b]);
+          if (s + AHEAD < s1) request(s + AHEAD, ring[q]);
+          if (j >= C::STAGES && !mx_wait(&empty[i], ((j / C::STAGES) & 1) ^ 1, abort_flag, err, 704)) { go = false; break; }
           unsigned char* const at_b = raw + (base - mx_smem(raw)) + i * C::STAGE_BYTES + MX_A_BYTES;
           unsigned char* const at_s = raw + (base - mx_smem(raw)) + i * C::STAGE_BYTES + C::SB;
 #pragma unroll
@@ -818,11 +871,11 @@ static int mx_launch_pair_any(const CUtensorMap (&m)[4], const MxProduct& p, boo
 }
 
 // x: [rows][k], w: [w_rows][k] (twice the out features if the epilogue is gated).  x_dtype IFB_F32 or IFB_BF16: `x` has numbers, rows
-// x_row elements apart; up to MX_ROUND_ROWS rows are rounded within the product, more of them first, into x_codes and x_scales
-// (whose room is the caller's; neither is looked at otherwise).  x_dtype -1: x_codes and x_scales have been rounded.
+// x_row elements apart; up to ifb_mx4_round_rows rows are rounded within the product, more of them first, into x_codes and
+// x_scales (whose room is the caller's; neither is looked at otherwise).  x_dtype -1: x_codes and x_scales have been rounded.
 // epilogue: as in the other products.  nt, splits: 0, or (for measurements) tokens of a tile and CTAs that share its k range.
 constexpr int MX_ROUND_ROWS = 32;
-IFB_EXPORT int ifb_mx4_round_rows() { return MX_ROUND_ROWS; }
+IFB_EXPORT int ifb_mx4_round_rows(int dtype) { return dtype == IFB_F32 ? MX_ROUND_ROWS / 2 : MX_ROUND_ROWS; }
 IFB_EXPORT int ifb_mx4_linear(const void* x, int x_dtype, long long x_row, void* x_codes, void* x_scales, const void* w_codes, const void* w_scales,
                               void* out, int out_dtype, int rows, int k, int w_rows, int epilogue, int nt, int splits, void* err, void* stream) {
   const bool gated = epilogue & 1;
@@ -834,21 +887,29 @@ IFB_EXPORT int ifb_mx4_linear(const void* x, int x_dtype, long long x_row, void*
   if (out_dtype != IFB_F32 && out_dtype != IFB_BF16) return IFB_ERR_DTYPE;
   if (x_dtype != -1 && x_dtype != IFB_F32 && x_dtype != IFB_BF16) return IFB_ERR_DTYPE;
   if ((((uintptr_t)x_codes) | ((uintptr_t)x_scales) | ((uintptr_t)w_codes) | ((uintptr_t)w_scales)) & 15) return IFB_ERR_ALIGN;
-  const bool round = x_dtype != -1 && rows <= MX_ROUND_ROWS;
+  const bool round = x_dtype != -1 && rows <= (x_dtype == IFB_F32 ? MX_ROUND_ROWS / 2 : MX_ROUND_ROWS);
   if (round && ((((uintptr_t)x) | (uintptr_t)(x_row * (x_dtype == IFB_F32 ? 4 : 2))) & 15)) return IFB_ERR_ALIGN;
   if (!round && (!x_codes || !x_scales)) return IFB_ERR_ARG;
   if (!round && x_dtype != -1) {
     bad = ifb_mx4_quantize(x, x_dtype, x_row, x_codes, x_scales, rows, k, 0, stream);
     if (bad) return bad;
   }
-  const bool pair = nt ? nt == 256 : rows > 256;
+  // Pairs of SMs (tiles of 256 x 256) from the second round of tiles of 128 x 128 on, where their rounds are fewer; theirs is 1.3 times as long.
+  // (24,576 x 4,096: 64 rows 19.5 us and 20.0 over pairs, 256 rows 30.3 and 23.7; 4,096 x 4,096, 193 rows: 8.7 and 13.4.)
+  const long long tiles1 = (long long)((w_rows + 127) / 128) * ((rows + 127) / 128), tiles2 = (long long)((w_rows + 255) / 256) * ((rows + 255) / 256);
+  const int sms = ifb_sm_count(), pairs = sms / 2;
+  const bool many = rows > 128 && tiles1 > sms && 4 * ((tiles2 + pairs - 1) / pairs) <= 3 * ((tiles1 + sms - 1) / sms);
+  const bool pair = nt ? nt == 256 : many;
   if (!nt || round) nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   if (nt < rows && nt < 128) return IFB_ERR_ARG;
   const int stages = (k + MX_KSTAGE - 1) / MX_KSTAGE, tiles = (w_rows + 127) / 128 * ((rows + nt - 1) / nt);
-  // the k range is shared where tiles leave SMs idle
+  // The k range of a tile is shared by the most CTAs, up to 8, that have two stages each and find an SM each; clusters of more
+  // than 4 leave SMs without one (16 tiles of 128 x 128, k = 2,048: 1, 4 and 8 CTAs per tile 5.9, 5.3 and 8.8 us; 32 tiles, k = 4,096: 1, 4, 6:
+  // 7.4, 4.9 to 5.3, 9.8; k = 1,024, four stages: 1, 2, 4: 2.9, 2.9, 3.4).
   if (!splits) {
     splits = 1;
-    while (splits < 8 && splits * 2 <= stages && tiles * splits * 2 <= ifb_sm_count() + 8) splits *= 2;
+    for (int s = 4; s > 1; --s)
+      if (2 * s <= stages && tiles * s <= ifb_sm_count()) { splits = s; break; }
   }
   if (splits < 1 || splits > 8 || splits > stages) return IFB_ERR_ARG;
   MxProduct p = {(const uint8_t*)x_scales, (const uint8_t*)w_scales, out, rows, k, w_rows, gated ? w_rows / 2 : w_rows, unary,

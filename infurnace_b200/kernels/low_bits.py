@@ -130,7 +130,7 @@ class LowBitKernels:
             lib.ifb_mx4_values.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]
             lib.ifb_mx4_linear.argtypes = [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                                            c_int, c_int, c_int, c_int, c_void_p, c_void_p]
-            self._mx4_round_rows = int(lib.ifb_mx4_round_rows())
+            self._mx4_round_rows = {code: int(lib.ifb_mx4_round_rows(code)) for code in _CODES.values()}
             self._mx4 = lib
         return self._mx4
 
@@ -196,7 +196,7 @@ class LowBitKernels:
             x_code = _CODES.get(x.dtype)
             if x_code is None or x.stride(1) != 1:
                 raise KernelError("mx4_linear: x is bfloat16 or float32 with unit stride along k, or an Mx4Matrix")
-            if n <= self._mx4_round_rows:
+            if n <= self._mx4_round_rows[x_code]:
                 rows = (x.data_ptr(), x_code, x.stride(0), 0, 0)
             else:
                 codes = -(-n * k // 512) * 256                             # half a byte an element, to a multiple of 256
