@@ -18,16 +18,21 @@ __device__ __forceinline__ float kv8_step(uint32_t f) {                 // 2^(f 
   if (f == 255u) return __uint_as_float(0x7fffffffu);
   return f > 6u ? __uint_as_float((f - 6u) << 23) : __uint_as_float(1u << (f + 16u));
 }
-// floor(x / step) of a number whose block has the exponent field f.
-__device__ __forceinline__ int kv8_code(float x, uint32_t f) {
-  if (f == 0u) return x < 0.f ? -1 : 0;
-  if (f == 255u) return 0;
-  // rounding downwards keeps a tiny negative number below zero where the quotient leaves the range of floats
-  float t;
-  if (f > 6u) t = __fmul_rd(x, __uint_as_float((260u - f) << 23));      // 2^(133 - f)
-  else t = __fmul_rd(__fmul_rd(x, __uint_as_float((254u - f) << 23)), 64.f);      // a factor that no float holds
-  return (int)floorf(t);
+// Codes of numbers whose block has the exponent field f: floor(x / step) is the lowest byte of x / step + 1.5 2^23, rounded downwards
+// once (a tiny negative number thus stays below zero).  1 / step = 2^(133 - f) is no float for the smallest f, whose numbers are
+// multiplied by 2^64 first; f = 0: any negative number is -1.
+struct Kv8Rounding { float before, factor; };
+__device__ __forceinline__ Kv8Rounding kv8_rounding(uint32_t f) {
+  if (f > 6u) return {1.f, __uint_as_float((260u - min(f, 254u)) << 23)};
+  return {__uint_as_float(191u << 23), f ? __uint_as_float((196u - f) << 23) : 1.f};
 }
+__device__ __forceinline__ uint32_t kv8_codes4(const float* x, const Kv8Rounding& r) {
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(__fmaf_rd(x[i] * r.before, r.factor, 12582912.f));
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+
 // A warp per (run of rows, kind, head).  A run is the adjacent rows whose slots follow one another in one page; its first row's
 // warp has the whole run, the other rows' warps leave.  (A page's rows must be one run: the caller's contract.)  A lane keeps HELD
 // pieces of eight numbers in registers between the search for the largest and the rounding (a page of 16 tokens of heads of 128
@@ -37,6 +42,10 @@ template <> struct Piece8<bf16> {
   uint4 w;
   __device__ __forceinline__ void load(const bf16* p) { w = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void clear() { w = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+    return max(m << 16, m & 0xffff0000u);
+  }
   __device__ __forceinline__ void numbers(float (&v)[8]) const {
     const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -50,6 +59,14 @@ template <> struct Piece8<float> {
   float4 a, b;
   __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
   __device__ __forceinline__ void clear() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    float x[8];
+    numbers(x);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    return m;
+  }
   __device__ __forceinline__ void numbers(float (&v)[8]) const {
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
@@ -89,19 +106,13 @@ kv8_store_kernel(const T* k, const T* v, long long k_row, long long v_row, const
     else held[j].clear();
   }
   uint32_t m = 0;
-  auto largest = [&](const Piece8<T>& p) {
-    float x[8];
-    p.numbers(x);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
-  };
-#pragma unroll
-  for (int j = 0; j < HELD; ++j) largest(held[j]);
+  for (int j = 0; j < HELD; ++j) m = max(m, held[j].amax_bits());
 #pragma unroll 4
   for (int i = lane + 32 * HELD; i < total; i += 32) {
     Piece8<T> p;
     p.load(at(i));
-    largest(p);
+    m = max(m, p.amax_bits());
   }
   m = __reduce_max_sync(0xffffffffu, m);
   const uint32_t f = max(old, m >> 23);
@@ -130,14 +141,11 @@ kv8_store_kernel(const T* k, const T* v, long long k_row, long long v_row, const
     }
   }
   if (!first && lane == 0) *exponent = (uint8_t)f;
+  const Kv8Rounding rounding = kv8_rounding(f);
   auto round = [&](int i, const Piece8<T>& p) {
-    const int r = i / pieces, c = i - r * pieces;
     float x[8];
     p.numbers(x);
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)kv8_code(x[j], f) & 255u) << (8 * (j & 3));
-    *reinterpret_cast<uint2*>(to + (size_t)(first + r) * dim + c * 8) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(to + (size_t)first * dim + (size_t)i * 8) = make_uint2(kv8_codes4(x, rounding), kv8_codes4(x + 4, rounding));
   };
 #pragma unroll
   for (int j = 0; j < HELD; ++j)
