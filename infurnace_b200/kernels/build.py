@@ -62,8 +62,8 @@ DEFAULT_VARIANTS = [("attention_mma", {"HEAD_DIM": d}) for d in (128, 16, 32, 48
 DEFAULT_VARIANTS += [(name, {"HEAD_DIM": 128, "WEIGHT_TERMS": 2, "SOFTCAP": 1}) for name in ("attention_mma", "attention_tc")]
 # bounded scores of unit queries and keys with two-term weights, heads of 128: prompts, and decoding
 DEFAULT_VARIANTS += [("attention_tc", {"HEAD_DIM": 128, "WEIGHT_TERMS": 2, "SOFTCAP": 2}), ("attention_mma", {"HEAD_DIM": 128, "WEIGHT_TERMS": 2})]
-# plain scores with two-term weights, heads of 128: prompts over 8-bit pages
-DEFAULT_VARIANTS += [("attention_tc", {"HEAD_DIM": 128, "WEIGHT_TERMS": 2})]
+# plain scores with two-term weights: prompts over 8-bit pages
+DEFAULT_VARIANTS += [("attention_tc", {"HEAD_DIM": d, "WEIGHT_TERMS": 2}) for d in (128, 64, 32)]
 # attention over 8-bit pages: heads of 128 (bfloat16), the sizes that the tests of the engine run, float32
 DEFAULT_VARIANTS += [("kv8_attention", {"HEAD_DIM": d}) for d in (128, 64, 256, 16)]
 DEFAULT_VARIANTS += [("kv8_attention", {"HEAD_DIM": d, "TERMS": 2}) for d in (128, 64, 256, 16)]

@@ -343,7 +343,7 @@ class LowBitKernels:
         # score rows beyond which a request's tiles fill the device by themselves and run whole; requests below run split
         rows, least = max_q_len * group, min_q_len * group
         limit = 64
-        if rows > self.kv8_expand_rows and q.dtype == torch.bfloat16 and dim == 128 and 128 % group == 0 and pages.page_size in (16, 32, 64) \
+        if rows > self.kv8_expand_rows and q.dtype == torch.bfloat16 and dim <= 128 and group <= 128 and pages.page_size in (16, 32, 64) \
                 and self.attention_tc:
             # (a long request has more than 16 score rows)
             most = -(-max_seq_len // pages.page_size)
