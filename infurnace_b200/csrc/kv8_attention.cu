@@ -706,18 +706,31 @@ static int kv8_launch(const Kv8Args& a, bool whole, int max_q, cudaStream_t stre
 }
 
 // nt: 1 or 2 tiles of 8 score rows per warp.  whole: the whole form.  Requests of min_rows .. max_rows score rows are worked on.
-IFB_EXPORT int ifb_kv8_attention(const void* q, int dtype, long long q_row, const void* codes, const void* exponents, const void* tables, int table_stride,
-                                 const void* cu_q, const void* seq_lens, void* out, void* parts, void* counters, int requests, int heads, int kv_heads,
-                                 int page_size, int dim, float scale, int window, int max_q, int min_rows, int max_rows, int tiles, int nt, int whole,
-                                 void* stream) {
-  if (dtype != (TERMS == 2 ? IFB_F32 : IFB_BF16)) return IFB_ERR_DTYPE;
-  if (dim != D || heads < 1 || kv_heads < 1 || heads % kv_heads || page_size < 16 || page_size % 16 || requests < 1 || max_q < 1 || window < 0 ||
-      (nt != 1 && nt != 2) || kv_heads > 65535 || requests > 65535)
+// One argument, since a call's price on the host is that of its arguments.
+struct Kv8Call {
+  const void* q;
+  long long dtype, q_row;
+  const void *codes, *exponents, *tables;
+  long long table_stride;
+  const void *cu_q, *seq_lens;
+  void *out, *parts, *counters;
+  long long requests, heads, kv_heads, page_size, dim, window, max_q, min_rows, max_rows, tiles, nt, whole;
+  void* stream;
+  double scale;
+};
+IFB_EXPORT int ifb_kv8_attention(const Kv8Call* c) {
+  const bool whole = c->whole != 0;
+  if (c->dtype != (TERMS == 2 ? IFB_F32 : IFB_BF16)) return IFB_ERR_DTYPE;
+  if (c->dim != D || c->heads < 1 || c->kv_heads < 1 || c->heads % c->kv_heads || c->page_size < 16 || c->page_size % 16 || c->requests < 1 ||
+      c->max_q < 1 || c->window < 0 || (c->nt != 1 && c->nt != 2) || c->kv_heads > 65535 || c->requests > 65535 || c->max_q > 0x7fffffff ||
+      c->window > 0x7fffffff || c->heads > 0x7fffffff)
     return IFB_ERR_SIZE;
-  if (!whole && (!parts || !counters || tiles < 1)) return IFB_ERR_ARG;
-  if ((((uintptr_t)q) | ((uintptr_t)codes) | ((uintptr_t)out) | (uintptr_t)(q_row * sizeof(qtype))) & 15) return IFB_ERR_ALIGN;
-  const Kv8Args a = {(const qtype*)q, q_row, (const int8_t*)codes, (const uint8_t*)exponents, (const int*)tables, table_stride, (const int*)cu_q,
-                     (const int*)seq_lens, (qtype*)out, (float*)parts, (int*)counters, requests, heads, kv_heads, page_size, window,
-                     scale * 1.4426950408889634f, min_rows, max_rows, tiles, 0};
-  return nt == 1 ? kv8_launch<1>(a, whole, max_q, (cudaStream_t)stream) : kv8_launch<2>(a, whole, max_q, (cudaStream_t)stream);
+  if (!whole && (!c->parts || !c->counters || c->tiles < 1)) return IFB_ERR_ARG;
+  if ((((uintptr_t)c->q) | ((uintptr_t)c->codes) | ((uintptr_t)c->out) | (uintptr_t)(c->q_row * sizeof(qtype))) & 15) return IFB_ERR_ALIGN;
+  const Kv8Args a = {(const qtype*)c->q, c->q_row, (const int8_t*)c->codes, (const uint8_t*)c->exponents, (const int*)c->tables, (int)c->table_stride,
+                     (const int*)c->cu_q, (const int*)c->seq_lens, (qtype*)c->out, (float*)c->parts, (int*)c->counters, (int)c->requests, (int)c->heads,
+                     (int)c->kv_heads, (int)c->page_size, (int)c->window, (float)c->scale * 1.4426950408889634f, (int)c->min_rows, (int)c->max_rows,
+                     (int)c->tiles, 0};
+  cudaStream_t stream = (cudaStream_t)c->stream;
+  return c->nt == 1 ? kv8_launch<1>(a, whole, (int)c->max_q, stream) : kv8_launch<2>(a, whole, (int)c->max_q, stream);
 }

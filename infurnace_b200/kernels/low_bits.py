@@ -6,12 +6,21 @@ scales and layouts are defined at the heads of ``csrc/mx4.cu`` and ``csrc/kv8.cu
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_char_p, c_int, c_longlong, c_void_p
+
+import struct
 
 import torch
 
 from ..errors import KernelError
 from .build import load_library
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+if _raw_stream is None:                       # an older torch: the public, slower way
+    def _raw_stream(device_index):
+        return torch.cuda.current_stream(device_index).cuda_stream
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+_KV8_CALL = struct.Struct("=25qd").pack       # csrc/kv8_attention.cu: Kv8Call
 
 MX4_BLOCK = 32         # elements of a row that share a scale
 _CODES = {torch.float32: 0, torch.bfloat16: 1}
@@ -32,6 +41,7 @@ class Mx4Matrix:
             raise KernelError("Mx4Matrix: scales are uint8, scale_bytes(rows, k) of them, contiguous, on 16 bytes, beside the codes")
         self.codes, self.scales, self.rows, self.k, self.gated = codes, scales, rows, k, bool(gated)
         self._at = (codes.data_ptr(), scales.data_ptr())
+        self._index = codes.get_device()          # -1: not on a CUDA device
 
     @staticmethod
     def scale_bytes(rows, k):
@@ -107,10 +117,12 @@ class Kv8Pages:
                 or exponents.device != codes.device:
             raise KernelError("Kv8Pages: exponents are uint8 [pages, 2, kv_heads], contiguous, beside the codes")
         self.codes, self.exponents = codes, exponents
+        self._shape = codes.shape
         self.pages, _, self.kv_heads, self.page_size, self.head_dim = codes.shape
         if self.page_size % 16 or self.head_dim % 16 or not 16 <= self.head_dim <= 256 or not 16 <= self.page_size <= 4096:
             raise KernelError("Kv8Pages: page_size is a multiple of 16 up to 4,096, head_dim one up to 256")
         self._at = (codes.data_ptr(), exponents.data_ptr())
+        self._index = codes.get_device()          # -1: not on a CUDA device
 
     @classmethod
     def empty(cls, pages, kv_heads, page_size, head_dim, device="cuda"):
@@ -144,25 +156,28 @@ class LowBitKernels:
         """Rows of ``x`` (bfloat16 or float32 [rows, k], rows may lie apart) rounded to 4 bits into ``matrix``; for a gated
         matrix ``x`` has its gate rows, then its up rows.  Returns ``matrix``."""
         code = _CODES.get(x.dtype)
-        if code is None or not x.is_cuda or x.dim() != 2 or x.shape != (matrix.rows, matrix.k) or x.stride(1) != 1 \
-                or x.device != matrix.codes.device:
+        index = matrix._index
+        if code is None or x.shape != (matrix.rows, matrix.k) or x.stride(1) != 1 or x.get_device() != index or index < 0:
             raise KernelError(f"mx4_quantize: x is bfloat16 or float32 [{matrix.rows}, {matrix.k}] with unit stride along k, on the "
                               f"matrix's device; got {x.dtype} {tuple(x.shape)} on {x.device}")
         self.launches += 1
-        self._low_bit_status(self._mx4_lib().ifb_mx4_quantize(x.data_ptr(), code, x.stride(0), *matrix._at, matrix.rows, matrix.k,
-                                                              matrix.gated, self._stream()), "mx4_quantize")
+        status = self._mx4_lib().ifb_mx4_quantize(x.data_ptr(), code, x.stride(0), *matrix._at, matrix.rows, matrix.k, matrix.gated,
+                                                  _raw_stream(index))
+        if status:
+            self._low_bit_status(status, "mx4_quantize")
         return matrix
 
     def mx4_values(self, matrix, out):
         """The numbers that ``matrix`` stands for, as bfloat16 (which holds them exactly) or float32 [rows, k]; a gated
         matrix's gate rows come before its up rows."""
         code = _CODES.get(out.dtype)
-        if code is None or not out.is_cuda or out.shape != (matrix.rows, matrix.k) or not out.is_contiguous() \
-                or out.device != matrix.codes.device:
+        index = matrix._index
+        if code is None or out.shape != (matrix.rows, matrix.k) or not out.is_contiguous() or out.get_device() != index or index < 0:
             raise KernelError(f"mx4_values: out is bfloat16 or float32 [{matrix.rows}, {matrix.k}], contiguous, on the matrix's device")
         self.launches += 1
-        self._low_bit_status(self._mx4_lib().ifb_mx4_values(*matrix._at, out.data_ptr(), code, matrix.rows, matrix.k, matrix.gated,
-                                                            self._stream()), "mx4_values")
+        status = self._mx4_lib().ifb_mx4_values(*matrix._at, out.data_ptr(), code, matrix.rows, matrix.k, matrix.gated, _raw_stream(index))
+        if status:
+            self._low_bit_status(status, "mx4_values")
         return out
 
     def mx4_matrix(self, w, gated=False):
@@ -184,27 +199,28 @@ class LowBitKernels:
         if k != w.k or (epi & 1 != 0) != w.gated or out.shape != (n, w.rows >> (epi & 1)):
             raise KernelError(f"mx4_linear: x {tuple(x.shape)}, w {w.shape} ({'gated' if w.gated else 'plain'}), out {tuple(out.shape)} "
                               f"and epilogue {epilogue!r} do not match")
-        device = w.codes.device
-        if code is None or out.device != device or not out.is_contiguous() or x.device != device or device.type != "cuda":
+        index = w._index
+        if code is None or out.get_device() != index or not out.is_contiguous() or index < 0:
             raise KernelError("mx4_linear: out is bfloat16 or float32, contiguous, and all is on the matrix's device")
         lib = self._mx4_lib()
         if isinstance(x, Mx4Matrix):
-            if x.gated:
-                raise KernelError("mx4_linear: x is a plain matrix")
+            if x.gated or x._index != index:
+                raise KernelError("mx4_linear: x is a plain matrix on w's device")
             rows = (0, -1, 0, *x._at)
         else:
             x_code = _CODES.get(x.dtype)
-            if x_code is None or x.stride(1) != 1:
-                raise KernelError("mx4_linear: x is bfloat16 or float32 with unit stride along k, or an Mx4Matrix")
+            pitch, unit = x.stride()
+            if x_code is None or unit != 1 or x.get_device() != index:
+                raise KernelError("mx4_linear: x is bfloat16 or float32 with unit stride along k on w's device, or an Mx4Matrix")
             if n <= self._mx4_round_rows[x_code]:
-                rows = (x.data_ptr(), x_code, x.stride(0), 0, 0)
+                rows = (x.data_ptr(), x_code, pitch, 0, 0)
             else:
                 codes = -(-n * k // 512) * 256                             # half a byte an element, to a multiple of 256
-                room = torch.empty(codes + Mx4Matrix.scale_bytes(n, k), dtype=torch.uint8, device=device)
-                rows = (x.data_ptr(), x_code, x.stride(0), room.data_ptr(), room.data_ptr() + codes)
+                room = torch.empty(codes + Mx4Matrix.scale_bytes(n, k), dtype=torch.uint8, device=w.codes.device)
+                rows = (x.data_ptr(), x_code, pitch, room.data_ptr(), room.data_ptr() + codes)
         self.launches += 1 if rows[3] == 0 or rows[1] < 0 else 2
         self._err_armed = True
-        status = lib.ifb_mx4_linear(*rows, *w._at, out.data_ptr(), code, n, k, w.rows, epi, nt, splits, self._dev_err_at, self._stream())
+        status = lib.ifb_mx4_linear(*rows, *w._at, out.data_ptr(), code, n, k, w.rows, epi, nt, splits, self._dev_err_at, _raw_stream(index))
         if status:
             self._low_bit_status(status, "mx4_linear")
         return out
@@ -227,32 +243,37 @@ class LowBitKernels:
         ``pages`` at ``slot_mapping`` (int32, page * page_size + offset; negative: not stored).  A page's tokens are adjacent
         rows in ascending order, as the step function lays them out; a token at offset 0 begins its page anew."""
         code = _CODES.get(k.dtype)
-        n = k.shape[0]
-        heads, dim = pages.kv_heads, pages.head_dim
-        if code is None or v.dtype != k.dtype or k.shape != (n, heads, dim) or v.shape != k.shape:
+        heads, dim, index = pages.kv_heads, pages.head_dim, pages._index
+        shape, pitch, v_pitch = k.shape, k.stride(), v.stride()
+        n = shape[0]
+        if code is None or v.dtype != k.dtype or shape != (n, heads, dim) or v.shape != shape:
             raise KernelError(f"kv8_store: k and v are bfloat16 or float32 [tokens, {heads}, {dim}]; got {k.dtype} {tuple(k.shape)} and "
                               f"{v.dtype} {tuple(v.shape)}")
-        if k.stride(2) != 1 or v.stride(2) != 1 or (heads > 1 and (k.stride(1) != dim or v.stride(1) != dim)):
+        if pitch[2] != 1 or v_pitch[2] != 1 or (heads > 1 and (pitch[1] != dim or v_pitch[1] != dim)):
             raise KernelError("kv8_store: the heads of a token lie one after the other")
         if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (n,) or not slot_mapping.is_contiguous():
             raise KernelError("kv8_store: slot_mapping is int32, one per token, contiguous")
-        device = pages.codes.device
-        if not k.is_cuda or k.device != device or v.device != device or slot_mapping.device != device:
+        if index < 0 or k.get_device() != index or v.get_device() != index or slot_mapping.get_device() != index:
             raise KernelError("kv8_store: k, v and slot_mapping are on the pages' device")
         if n == 0:
             return
         self.launches += 1
-        self._low_bit_status(self._kv8_lib().ifb_kv8_store(k.data_ptr(), v.data_ptr(), code, k.stride(0), v.stride(0), slot_mapping.data_ptr(),
-                                                           *pages._at, n, heads, pages.page_size, dim, self._stream()), "kv8_store")
+        status = self._kv8_lib().ifb_kv8_store(k.data_ptr(), v.data_ptr(), code, pitch[0], v_pitch[0], slot_mapping.data_ptr(), *pages._at, n, heads,
+                                               pages.page_size, dim, _raw_stream(index))
+        if status:
+            self._low_bit_status(status, "kv8_store")
 
     def kv8_values(self, pages, out):
         """The numbers that the bits of all pages stand for, as bfloat16 or float32 (both hold them exactly) of the codes' shape."""
         code = _CODES.get(out.dtype)
-        if code is None or not out.is_cuda or out.shape != pages.codes.shape or not out.is_contiguous() or out.device != pages.codes.device:
+        index = pages._index
+        if code is None or out.shape != pages._shape or not out.is_contiguous() or out.get_device() != index or index < 0:
             raise KernelError("kv8_values: out is bfloat16 or float32 of the codes' shape, contiguous, on the pages' device")
         self.launches += 1
-        self._low_bit_status(self._kv8_lib().ifb_kv8_values(*pages._at, out.data_ptr(), code, pages.pages, pages.kv_heads, pages.page_size,
-                                                            pages.head_dim, self._stream()), "kv8_values")
+        status = self._kv8_lib().ifb_kv8_values(*pages._at, out.data_ptr(), code, pages.pages, pages.kv_heads, pages.page_size, pages.head_dim,
+                                                _raw_stream(index))
+        if status:
+            self._low_bit_status(status, "kv8_values")
         return out
 
     def _kv8_attention_lib(self, dim, dtype):
@@ -261,9 +282,7 @@ class LowBitKernels:
         if lib is None:
             defines = {"HEAD_DIM": dim} if dtype == torch.bfloat16 else {"HEAD_DIM": dim, "TERMS": 2}
             lib = load_library("kv8_attention", defines, progress=self._progress)
-            lib.ifb_kv8_attention.argtypes = [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
-                                              c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int,
-                                              c_int, c_int, c_int, c_void_p]
+            lib.ifb_kv8_attention.argtypes = [c_char_p]
             lib.ifb_kv8_attention_scratch.restype = c_longlong
             lib.ifb_kv8_attention_scratch.argtypes = [c_int]
             lib.scratch_floats = {nt: int(lib.ifb_kv8_attention_scratch(nt)) for nt in (1, 2)}
@@ -274,23 +293,24 @@ class LowBitKernels:
         return lib
 
     def _kv8_scratch(self, stream, floats, counters):
-        """(sums, counters) of the split form: of a stream each, and one pair for recorded graphs, whose replays follow one
-        another.  The counters are zero between launches; a recording could not clear new ones, so what it uses is made
+        """Addresses of (sums, counters) of the split form: of a stream each, and one pair for recorded graphs, whose replays follow
+        one another.  The counters are zero between launches; a recording could not clear new ones, so what it uses is made
         before, with the first call outside of one."""
         held = self.__dict__.setdefault("_kv8_held", {})
-        capturing = torch.cuda.is_current_stream_capturing()
+        capturing = _capturing()
         for key in (("graph",) if capturing else (stream, "graph")):
             have = held.get(key)
-            if have is None or have[0].numel() < floats or have[1].numel() < counters:
+            if have is None or have[0] < floats or have[1] < counters:
                 if capturing:
                     raise KernelError("kv8_attention: run the call once before it is recorded into a graph")
-                more = (have[0].numel(), have[1].numel()) if have else (0, 0)
-                held[key] = (torch.empty(max(floats, more[0]), dtype=torch.float32, device="cuda"),
-                             torch.zeros(max(counters, more[1], 4096), dtype=torch.int32, device="cuda"))
+                floats_, counters_ = max(floats, have[0] if have else 0), max(counters, have[1] if have else 4096)
+                sums = torch.empty(floats_, dtype=torch.float32, device="cuda")
+                zeros = torch.zeros(counters_, dtype=torch.int32, device="cuda")
+                held[key] = (floats_, counters_, sums.data_ptr(), zeros.data_ptr(), sums, zeros)
                 if key == "graph":
                     torch.cuda.current_stream().synchronize()            # cleared before a graph on another stream can use them
                     self.scratch_generation += 1
-        return held["graph" if capturing else stream]
+        return held["graph" if capturing else stream][2:4]
 
     kv8_expand_rows = 64             # score rows of the longest request from which prompts' pages are expanded for the tcgen05 kernel
     kv8_expand_bytes = 4 << 30       # room for expanded pages that a call may take
@@ -318,28 +338,29 @@ class LowBitKernels:
         keys, none fewer than ``min_q_len`` queries; ``exact_lens``: some request has ``max_q_len``, and ``q`` no other rows than
         theirs, which bounds how many are long."""
         code = _CODES.get(q.dtype)
-        n, heads, dim = q.shape
+        shape, pitch, index = q.shape, q.stride(), pages._index
+        n, heads, dim = shape
         kv_heads = pages.kv_heads
-        if code is None or out.dtype != q.dtype or out.shape != q.shape or dim != pages.head_dim or heads % kv_heads:
+        if code is None or out.dtype != q.dtype or out.shape != shape or dim != pages.head_dim or heads % kv_heads:
             raise KernelError(f"kv8_attention: q and out are bfloat16 or float32 [tokens, a multiple of {kv_heads}, {pages.head_dim}]; got "
                               f"{q.dtype} {tuple(q.shape)} and {out.dtype} {tuple(out.shape)}")
-        if q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim) or not out.is_contiguous():
+        if pitch[2] != 1 or (heads > 1 and pitch[1] != dim) or not out.is_contiguous():
             raise KernelError("kv8_attention: the heads of a query lie one after the other, and out is contiguous")
         r = seq_lens.numel()
+        table_shape, table_pitch = block_tables.shape, block_tables.stride()
         if cu_q.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_tables.dtype != torch.int32 or cu_q.numel() != r + 1 \
-                or block_tables.dim() != 2 or block_tables.shape[0] < r or block_tables.stride(1) != 1 or not cu_q.is_contiguous() \
-                or not seq_lens.is_contiguous():
+                or len(table_shape) != 2 or table_shape[0] < r or table_pitch[1] != 1 or not cu_q.is_contiguous() or not seq_lens.is_contiguous():
             raise KernelError("kv8_attention: cu_q, seq_lens and block_tables are int32 for the same requests, dense along their last axis")
-        if block_tables.shape[1] * pages.page_size < max_seq_len:
-            raise KernelError(f"kv8_attention: block tables of {block_tables.shape[1]} pages do not hold {max_seq_len} keys")
-        device = pages.codes.device
-        if any(t.device != device for t in (q, out, cu_q, seq_lens, block_tables)) or not q.is_cuda:
+        if table_shape[1] * pages.page_size < max_seq_len:
+            raise KernelError(f"kv8_attention: block tables of {table_shape[1]} pages do not hold {max_seq_len} keys")
+        if index < 0 or q.get_device() != index or out.get_device() != index or cu_q.get_device() != index or seq_lens.get_device() != index \
+                or block_tables.get_device() != index:
             raise KernelError("kv8_attention: all tensors are on the pages' device")
         if n == 0 or r == 0:
             return out
         if window < 0 or max_q_len < 1 or not 1 <= min_q_len <= max_q_len:
             raise KernelError("kv8_attention: window is not negative, and 1 <= min_q_len <= max_q_len")
-        lib, stream, group = self._kv8_attention_lib(dim, q.dtype), self._stream(), heads // kv_heads
+        lib, stream, group = self._kv8_attention_lib(dim, q.dtype), _raw_stream(index), heads // kv_heads
         # score rows beyond which a request's tiles fill the device by themselves and run whole; requests below run split
         rows, least = max_q_len * group, min_q_len * group
         limit = 64
@@ -354,17 +375,18 @@ class LowBitKernels:
                     return out
                 limit = rows = 16
         nt = 1 if rows <= 8 or dim > 128 or limit == 16 and group <= 8 else 2      # (beside prompts the short requests decode)
-        fixed = (q.data_ptr(), code, q.stride(0), *pages._at, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
-                 seq_lens.data_ptr(), out.data_ptr())
-        sizes = (r, heads, kv_heads, pages.page_size, dim, float(scale), int(window))
+        fixed = (q.data_ptr(), code, pitch[0], *pages._at, block_tables.data_ptr(), table_pitch[0], cu_q.data_ptr(), seq_lens.data_ptr(),
+                 out.data_ptr())
+        sizes = (r, heads, kv_heads, pages.page_size, dim, window, max_q_len)
+        status = 0
         if least <= limit:
             tiles = -(-min(rows, limit) // (8 * nt))
-            sums, counters = self._kv8_scratch(stream, lib.scratch_floats[nt], r * tiles * kv_heads)
             self.launches += 1
-            self._low_bit_status(lib.ifb_kv8_attention(*fixed, sums.data_ptr(), counters.data_ptr(), *sizes, max_q_len, 0, limit, tiles, nt, 0,
-                                                       stream), "kv8_attention")
-        if rows > limit:
+            status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, *self._kv8_scratch(stream, lib.scratch_floats[nt], r * tiles * kv_heads), *sizes, 0, limit,
+                                                     tiles, nt, 0, stream, scale))
+        if rows > limit and not status:
             self.launches += 1
-            self._low_bit_status(lib.ifb_kv8_attention(*fixed, 0, 0, *sizes, max_q_len, limit + 1, (1 << 31) - 1, 1, nt, 1, stream),
-                                 "kv8_attention")
+            status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, 0, 0, *sizes, limit + 1, (1 << 31) - 1, 1, nt, 1, stream, scale))
+        if status:
+            self._low_bit_status(status, "kv8_attention")
         return out
