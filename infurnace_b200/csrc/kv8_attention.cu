@@ -215,28 +215,43 @@ struct Stream {
       for (int i = 0; i < KS; ++i) { o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f; }
     }
   }
-  // row0: the first of the rows; rows: how many the request has; pos0: position of its first query; G: query heads per key head.
-  __device__ __forceinline__ void load_queries(const Kv8Args& a, int first_token, int row0, int rows, int pos0, int kv_head, int G, int lane) {
+  // The queries come in two parts as well, so that their trip and that of the first keys overlap.
+  struct Queries { uint32_t w[NT][KS][sizeof(qtype) == 2 ? 2 : 4]; };
+  // row0: the first of the rows; rows: how many the request has; G: query heads per key head.
+  static __device__ __forceinline__ void request(Queries& raw, const Kv8Args& a, int first_token, int row0, int rows, int kv_head, int G, int lane) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + n * 8 + (lane >> 2);
       const bool in = row < rows;
-      const qtype* src = a.q + (size_t)(first_token + (in ? row / G : 0)) * a.q_row + (size_t)(kv_head * G + (in ? row % G : 0)) * D;
-      uint32_t raw[KS][4];                                              // float32 bits
-      uint32_t amax = 0;
+      const int token = in ? row / G : 0, head = in ? row - token * G : 0;
+      const qtype* src = a.q + (size_t)(first_token + token) * a.q_row + (size_t)(kv_head * G + head) * D;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d = key_dim(ks, lane);
 #if TERMS == 2
         const uint4 x = in ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
-        raw[ks][0] = x.x; raw[ks][1] = x.y; raw[ks][2] = x.z; raw[ks][3] = x.w;
+        raw.w[n][ks][0] = x.x; raw.w[n][ks][1] = x.y; raw.w[n][ks][2] = x.z; raw.w[n][ks][3] = x.w;
 #else
         const uint2 x = in ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
-        raw[ks][0] = x.x << 16; raw[ks][1] = x.x & 0xffff0000u; raw[ks][2] = x.y << 16; raw[ks][3] = x.y & 0xffff0000u;
+        raw.w[n][ks][0] = x.x; raw.w[n][ks][1] = x.y;
+#endif
+      }
+    }
+  }
+  // pos0: position of the request's first query.
+  __device__ __forceinline__ void queries(const Queries& raw, int row0, int rows, int pos0, int G, int lane) {
+#if TERMS == 2
+    auto number = [&](int n, int ks, int j) { return __uint_as_float(raw.w[n][ks][j]); };
+#else
+    auto number = [&](int n, int ks, int j) { const uint32_t w = raw.w[n][ks][j >> 1]; return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16); };
 #endif
 #pragma unroll
-        for (int j = 0; j < 4; ++j) amax = max(amax, raw[ks][j] & 0x7fffffffu);
-      }
+    for (int n = 0; n < NT; ++n) {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) amax = max(amax, __float_as_uint(number(n, ks, j)) & 0x7fffffffu);
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       // the row's largest number becomes one of [2^10, 2^11): a power of two that a float holds either way round
@@ -247,7 +262,7 @@ struct Stream {
       for (int ks = 0; ks < KS; ++ks) {
         float x[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(raw[ks][j]) * to;
+        for (int j = 0; j < 4; ++j) x[j] = number(n, ks, j) * to;
         qf[0][n][ks][0] = pack_half(x[0], x[2]);                        // beside the even and the odd bytes of a word of codes
         qf[0][n][ks][1] = pack_half(x[1], x[3]);
 #if TERMS == 2
@@ -472,10 +487,12 @@ kv8_attention_whole_kernel(Kv8Args a) {
   if (row0 >= rows) return;
   const int pos0 = L - q_len, p_first = pos0 + row0 / G, p_last = pos0 + min(row0 + 8 * NT - 1, rows - 1) / G;
   const int lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
+  typename Stream<NT>::Queries raw;
+  Stream<NT>::request(raw, a, q0, row0, rows, kv_head, G, lane);
   typename Stream<NT>::Walk walk(a, a.tables + (size_t)r * a.table_stride, kv_head, lo / 16, p_last >= 0 ? p_last / 16 + 1 : 0, 1, lane);
   Stream<NT> st;
   st.reset();
-  st.load_queries(a, q0, row0, rows, pos0, kv_head, G, lane);
+  st.queries(raw, row0, rows, pos0, G, lane);
   st.run(a, walk, a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
   st.finish();
 #pragma unroll
@@ -538,19 +555,31 @@ kv8_attention_split_kernel(Kv8Args a) {
   float* const sm_m = sums + WARPS * ROWS * PITCH;
   float* const sm_l = sm_m + WARPS * ROWS;
   // every warp for itself: how long pieces are, and whose piece this CTA's is
-  const Kv8Look known = kv8_look<ROWS>(a, G, 0, lane);
+  const Kv8Look known = kv8_look<ROWS>(a, G, 0, lane), known2 = kv8_look<ROWS>(a, G, 32, lane);
+  auto look = [&](int r0) { return r0 == 0 ? known : r0 == 32 ? known2 : kv8_look<ROWS>(a, G, r0, lane); };
   int total = 0, items = 0, longest = 0;
   for (int r0 = 0; r0 < a.requests; r0 += 32) {
-    const Kv8Look k = r0 ? kv8_look<ROWS>(a, G, r0, lane) : known;
-    total += __reduce_add_sync(0xffffffffu, k.units * k.items);
-    items += __reduce_add_sync(0xffffffffu, k.items);
-    longest = max(longest, __reduce_max_sync(0xffffffffu, k.units));
+    const Kv8Look k = look(r0);
+    total += k.units * k.items;
+    items += k.items;
+    longest = max(longest, k.units);
   }
-  const int spare = a.most - items;
-  const int per = max(spare > 0 ? (total + spare - 1) / spare : longest, (longest + MAX_PARTS - 1) / MAX_PARTS);
+  total = __reduce_add_sync(0xffffffffu, total);
+  items = __reduce_add_sync(0xffffffffu, items);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  const int spare = a.most - items, least = (longest + MAX_PARTS - 1) / MAX_PARTS;
+  int per = max(spare > 0 ? (total + spare - 1) / spare : longest, least);
+  if (spare > 0 && a.requests <= 64) {
+    // pieces a unit shorter, as long as there are CTAs for them (the bound above counts an unfinished piece for every item)
+    for (int tries = 0; tries < 4 && per > max(least, 1); ++tries) {
+      const int one = (known.units + per - 2) / (per - 1) * known.items + (known2.units + per - 2) / (per - 1) * known2.items;
+      if (__reduce_add_sync(0xffffffffu, one) > a.most) break;
+      --per;
+    }
+  }
   int r = -1, q0, q_len, L, units, pieces, at = blockIdx.x;             // at: of the pieces of the request
   for (int r0 = 0; r0 < a.requests; r0 += 32) {
-    const Kv8Look k = r0 ? kv8_look<ROWS>(a, G, r0, lane) : known;
+    const Kv8Look k = look(r0);
     const int mine = k.items ? (k.units + per - 1) / per : 0;
     int upto = mine * k.items;
     const int own = upto;
@@ -580,11 +609,13 @@ kv8_attention_split_kernel(Kv8Args a) {
   const int lo_request = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
   const int each = (units + pieces - 1) / pieces;                       // units of a piece
   const int key0 = (lo_request / UNIT + piece * each) * UNIT, key_end = min(p_last + 1, key0 + each * UNIT);
+  typename Stream<NT>::Queries raw;
+  Stream<NT>::request(raw, a, q0, row0, rows, kv_head, G, lane);
   typename Stream<NT>::Walk walk(a, a.tables + (size_t)r * a.table_stride, kv_head, max(key0, lo) / 16 + warp, key_end > 0 ? (key_end + 15) / 16 : 0,
                                  WARPS, lane);
   Stream<NT> st;
   st.reset();
-  st.load_queries(a, q0, row0, rows, pos0, kv_head, G, lane);
+  st.queries(raw, row0, rows, pos0, G, lane);
   st.run(a, walk, a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
   st.finish();
   // the warps' sums side by side
@@ -601,43 +632,46 @@ kv8_attention_split_kernel(Kv8Args a) {
       }
     }
   __syncthreads();
-  auto finish_row = [&](int row, int place, float2 o, float l) {
+  auto finish_row = [&](int row, int place, float4 o, float l) {       // four numbers side by side are two neighbouring lanes' pairs
     const int full = row0 + row;
-    kv8_store_pair(a.out + ((size_t)(q0 + full / G) * a.heads + kv_head * G + full % G) * D + kv8_place_dim(place), kv8_ratio(o.x, l), kv8_ratio(o.y, l));
+    qtype* to = a.out + ((size_t)(q0 + full / G) * a.heads + kv_head * G + full % G) * D;
+    kv8_store_pair(to + kv8_place_dim(place), kv8_ratio(o.x, l), kv8_ratio(o.y, l));
+    kv8_store_pair(to + kv8_place_dim(place + 2), kv8_ratio(o.z, l), kv8_ratio(o.w, l));
   };
+  auto add = [](float4& o, const float4& x, float f) { o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w); };
   float* const mine = a.parts + (size_t)blockIdx.x * ROWS * (D + 2);
-  for (int i = tid; i < here * (D / 2); i += 32 * WARPS) {
-    const int row = i / (D / 2), place = (i - row * (D / 2)) * 2;
+  for (int i = tid; i < here * (D / 4); i += 32 * WARPS) {
+    const int row = i / (D / 4), place = (i - row * (D / 4)) * 4;
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_m[w * ROWS + row]);
     const float U = M == -INFINITY ? 0.f : M;
-    float2 o = make_float2(0.f, 0.f);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const float f = kv8_exp2(sm_m[w * ROWS + row] - U);
-      const float2 x = *reinterpret_cast<const float2*>(sums + (w * ROWS + row) * PITCH + place);
-      o.x = fmaf(x.x, f, o.x);
-      o.y = fmaf(x.y, f, o.y);
+      add(o, *reinterpret_cast<const float4*>(sums + (w * ROWS + row) * PITCH + place), f);
       l = fmaf(sm_l[w * ROWS + row], f, l);
     }
     if (pieces == 1) {
       finish_row(row, place, o, l);
     } else {
-      *reinterpret_cast<float2*>(mine + row * D + place) = o;
+      *reinterpret_cast<float4*>(mine + row * D + place) = o;
       if (place == 0) { mine[ROWS * D + row] = M; mine[ROWS * (D + 1) + row] = l; }
     }
   }
   if (pieces == 1) return;
-  __threadfence();
   __syncthreads();
   int* const counter = a.counters + ((size_t)r * a.tiles + tile) * a.kv_heads + kv_head;
-  if (tid == 0) arrived = atomicAdd(counter, 1);
+  if (tid == 0) {                                                       // its fence covers what the barrier ordered before it
+    __threadfence();
+    arrived = atomicAdd(counter, 1);
+    __threadfence();
+  }
   __syncthreads();
   if (arrived != pieces - 1) return;
   // the last of the item's pieces to arrive adds them all, in their order
-  __threadfence();
   const float* const first = mine - (size_t)piece * ROWS * (D + 2);
   auto part = [&](int c) { return first + (size_t)c * ROWS * (D + 2); };
   for (int i = tid; i < here * pieces; i += 32 * WARPS) {
@@ -646,19 +680,24 @@ kv8_attention_split_kernel(Kv8Args a) {
     part_l[i / here][i % here] = __ldcg(from + ROWS);
   }
   __syncthreads();
-  for (int i = tid; i < here * (D / 2); i += 32 * WARPS) {
-    const int row = i / (D / 2), place = (i - row * (D / 2)) * 2;
+  for (int i = tid; i < here * (D / 4); i += 32 * WARPS) {
+    const int row = i / (D / 4), place = (i - row * (D / 4)) * 4;
     float M = -INFINITY, l = 0.f;
     for (int c = 0; c < pieces; ++c) M = fmaxf(M, part_m[c][row]);
     const float U = M == -INFINITY ? 0.f : M;
-    float2 o = make_float2(0.f, 0.f);
-#pragma unroll 8
-    for (int c = 0; c < pieces; ++c) {
-      const float2 x = __ldcg(reinterpret_cast<const float2*>(part(c) + row * D + place));
-      const float f = kv8_exp2(part_m[c][row] - U);
-      o.x = fmaf(x.x, f, o.x);
-      o.y = fmaf(x.y, f, o.y);
-      l = fmaf(part_l[c][row], f, l);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = 0; c0 < pieces; c0 += 8) {
+      float4 x[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c0 + c < pieces) x[c] = __ldcg(reinterpret_cast<const float4*>(part(c0 + c) + row * D + place));
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c0 + c < pieces) {
+          const float f = kv8_exp2(part_m[c0 + c][row] - U);
+          add(o, x[c], f);
+          l = fmaf(part_l[c0 + c][row], f, l);
+        }
     }
     finish_row(row, place, o, l);
   }
