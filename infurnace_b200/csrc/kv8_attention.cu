@@ -542,6 +542,10 @@ __device__ __forceinline__ Kv8Look kv8_look(const Kv8Args& a, int G, int r0, int
   return k;
 }
 
+// ceil(x / y) of whole numbers from 1 on, x below 2^20 (units of a request: 2^26 keys): the quotient's error is below the half that
+// is taken off.
+__device__ __forceinline__ int kv8_parts(int x, float inverse) { return (int)(((float)x - 0.5f) * inverse) + 1; }
+
 template <int NT>
 __global__ void __launch_bounds__(32 * WARPS, split_ctas(NT))
 kv8_attention_split_kernel(Kv8Args a) {
@@ -555,7 +559,7 @@ kv8_attention_split_kernel(Kv8Args a) {
   float* const sm_m = sums + WARPS * ROWS * PITCH;
   float* const sm_l = sm_m + WARPS * ROWS;
   // every warp for itself: how long pieces are, and whose piece this CTA's is
-  const Kv8Look known = kv8_look<ROWS>(a, G, 0, lane), known2 = kv8_look<ROWS>(a, G, 32, lane);
+  const Kv8Look known = kv8_look<ROWS>(a, G, 0, lane), known2 = a.requests > 32 ? kv8_look<ROWS>(a, G, 32, lane) : Kv8Look{};
   auto look = [&](int r0) { return r0 == 0 ? known : r0 == 32 ? known2 : kv8_look<ROWS>(a, G, r0, lane); };
   int total = 0, items = 0, longest = 0;
   for (int r0 = 0; r0 < a.requests; r0 += 32) {
@@ -572,15 +576,17 @@ kv8_attention_split_kernel(Kv8Args a) {
   if (spare > 0 && a.requests <= 64) {
     // pieces a unit shorter, as long as there are CTAs for them (the bound above counts an unfinished piece for every item)
     for (int tries = 0; tries < 4 && per > max(least, 1); ++tries) {
-      const int one = (known.units + per - 2) / (per - 1) * known.items + (known2.units + per - 2) / (per - 1) * known2.items;
+      const float inverse = 1.f / (float)(per - 1);
+      const int one = (known.items ? kv8_parts(known.units, inverse) : 0) * known.items + (known2.items ? kv8_parts(known2.units, inverse) : 0) * known2.items;
       if (__reduce_add_sync(0xffffffffu, one) > a.most) break;
       --per;
     }
   }
+  const float per_inverse = 1.f / (float)per;
   int r = -1, q0, q_len, L, units, pieces, at = blockIdx.x;             // at: of the pieces of the request
   for (int r0 = 0; r0 < a.requests; r0 += 32) {
     const Kv8Look k = look(r0);
-    const int mine = k.items ? (k.units + per - 1) / per : 0;
+    const int mine = k.items ? kv8_parts(k.units, per_inverse) : 0;
     int upto = mine * k.items;
     const int own = upto;
 #pragma unroll

@@ -186,6 +186,19 @@ class LowBitKernels:
             raise KernelError("mx4_matrix: w is [rows, k], a gated one of an even number of rows")
         return self.mx4_quantize(w, Mx4Matrix.empty(w.shape[0], w.shape[1], w.device, gated))
 
+    def _mx4_room(self, stream, size, device):
+        """Address of room for rounded rows: of a stream each, whose launches follow one another; memory of its own in a recording."""
+        if _capturing():
+            held = self._mx4_recorded = torch.empty(size, dtype=torch.uint8, device=device)      # the graph's own pool keeps it for its replays
+            return held.data_ptr()
+        rooms = self.__dict__.setdefault("_mx4_rooms", {})
+        held = rooms.get(stream)
+        if held is None or held[0] < size:
+            size = max(size, 1 << 20)
+            room = torch.empty(size, dtype=torch.uint8, device=device)
+            held = rooms[stream] = (size, room.data_ptr(), room)
+        return held[1]
+
     def mx4_linear(self, x, w, out, epilogue="none", nt=0, splits=0):
         """out = Q(x) w^T with the epilogue (a key of ``EPILOGUES``), ``w`` an :class:`Mx4Matrix` and Q(x) the rows of ``x``
         rounded to 4 bits as ``mx4_quantize`` rounds them; ``x`` bfloat16 or float32 [n, k], or an :class:`Mx4Matrix` that
@@ -216,9 +229,9 @@ class LowBitKernels:
                 rows = (x.data_ptr(), x_code, pitch, 0, 0)
             else:
                 codes = -(-n * k // 512) * 256                             # half a byte an element, to a multiple of 256
-                room = torch.empty(codes + Mx4Matrix.scale_bytes(n, k), dtype=torch.uint8, device=w.codes.device)
-                rows = (x.data_ptr(), x_code, pitch, room.data_ptr(), room.data_ptr() + codes)
-        self.launches += 1 if rows[3] == 0 or rows[1] < 0 else 2
+                room = self._mx4_room(_raw_stream(index), codes + Mx4Matrix.scale_bytes(n, k), w.codes.device)
+                rows = (x.data_ptr(), x_code, pitch, room, room + codes)
+        self.launches += 1 if rows[1] < 0 or n <= self._mx4_round_rows[rows[1]] else 2
         self._err_armed = True
         status = lib.ifb_mx4_linear(*rows, *w._at, out.data_ptr(), code, n, k, w.rows, epi, nt, splits, self._dev_err_at, _raw_stream(index))
         if status:

@@ -118,6 +118,47 @@ def test_product(K, dtype, rows, k, features, epilogue):
     check(out, ref, mag, k, dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,features", [(129, 32, 8), (256, 256, 256), (300, 1120, 258), (257, 4096, 385), (513, 160, 130), (700, 96, 1001),
+                                             (1030, 544, 1000), (2048, 512, 304)])
+@pytest.mark.parametrize("epilogue", ["none", "silu_gate"])
+def test_product_over_pairs_of_sms(K, dtype, rows, k, features, epilogue):
+    """The kernel for many rows at sizes that the rule gives to others: rows of the output on 16 bytes (stored by TMA) and not."""
+    gated = epilogue == "silu_gate"
+    x, w = rows_of(rows, k, 11, dtype), rows_of(features * (2 if gated else 1), k, 12, torch.bfloat16) * 0.1
+    ref, mag = product(round4(x)[2], round4(w)[2], epilogue)
+    room = torch.full((rows + 2, features), 7.0, dtype=dtype, device="cuda")
+    out = room[:rows]
+    K.mx4_linear(x.cuda(), K.mx4_matrix(w.cuda(), gated=gated), out, epilogue=epilogue, nt=256)
+    K.check_device_errors()
+    check(out, ref, mag, k, dtype)
+    assert (room[rows:] == 7.0).all()                                  # nothing is written behind the last row
+
+
+@pytest.mark.parametrize("epilogue,dtype", [("none", torch.bfloat16), ("silu_gate", torch.bfloat16), ("none", torch.float32), ("relu2", torch.bfloat16)])
+def test_product_that_the_rule_gives_to_pairs(K, epilogue, dtype):
+    """Several rounds of tiles per pair."""
+    gated = epilogue == "silu_gate"
+    rows, k, features = 1100, 288, 6500 if not gated else 3300
+    x, w = rows_of(rows, k, 13, dtype), rows_of(features * (2 if gated else 1), k, 14, torch.bfloat16) * 0.1
+    ref, mag = product(round4(x)[2], round4(w)[2], epilogue)
+    out = torch.full((rows, features), math.nan, dtype=dtype, device="cuda")
+    K.mx4_linear(x.cuda(), K.mx4_matrix(w.cuda(), gated=gated), out, epilogue=epilogue)
+    K.check_device_errors()
+    check(out, ref, mag, k, dtype)
+
+
+@pytest.mark.parametrize("rows,nt,splits", [(5, 16, 1), (5, 32, 3), (40, 64, 8), (40, 128, 5), (200, 128, 7), (16, 64, 2)])
+def test_tiles_and_shares_that_the_rule_does_not_choose(K, rows, nt, splits):
+    from infurnace_b200.kernels import Mx4Matrix
+    x, w = rows_of(rows, 2208, 15, torch.bfloat16), rows_of(300, 2208, 16, torch.bfloat16) * 0.1
+    q = K.mx4_quantize(x.cuda(), Mx4Matrix.empty(rows, 2208))
+    out = torch.full((rows, 300), math.nan, device="cuda")
+    K.mx4_linear(q, K.mx4_matrix(w.cuda()), out, nt=nt, splits=splits)
+    K.check_device_errors()
+    check(out, *product(round4(x)[2], round4(w)[2], "none"), 2208, torch.float32)
+
+
 @pytest.mark.parametrize("rows", [3, 40, 300])
 def test_rounded_rows_unary_epilogues_and_mixed_types(K, rows):
     """Rows that are rounded once serve several products; the output's type is free of the input's; a unary epilogue."""
