@@ -33,8 +33,9 @@ __device__ __forceinline__ uint32_t kv8_codes4(const float* x, const Kv8Rounding
   return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
-// A warp per (run of rows, kind, head).  A run is the adjacent rows whose slots follow one another in one page; its first row's
-// warp has the whole run, the other rows' warps leave.  (A page's rows must be one run: the caller's contract.)  A lane keeps HELD
+// A warp per (window of rows, kind, head).  A run is the adjacent rows whose slots follow one another in one page; the warp has the
+// runs that begin in its window, a row of a decode step, 16 rows of a prompt (a warp for every row of 2,043, fifteen of sixteen
+// of which leave at once, took 9.9 us).  (A page's rows must be one run: the caller's contract.)  A lane keeps HELD
 // pieces of eight numbers in registers between the search for the largest and the rounding (a page of 16 tokens of heads of 128
 // in bfloat16 whole); of longer runs the rest is read again, from the first level of cache.
 template <typename T> struct Piece8;
@@ -72,17 +73,9 @@ template <> struct Piece8<float> {
   }
 };
 template <typename T>
-__global__ void __launch_bounds__(256)
-kv8_store_kernel(const T* k, const T* v, long long k_row, long long v_row, const int* slots, int8_t* codes, uint8_t* exponents, int rows,
-                 int heads, int page_size, int dim) {
-  ifb_pdl_wait();
-  ifb_pdl_trigger();
-  const int row0 = blockIdx.x, lane = threadIdx.x & 31, block = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (block >= 2 * heads) return;
-  const int slot = slots[row0];
-  if (slot < 0) return;
+__device__ __forceinline__ void kv8_store_run(const T* k, const T* v, long long k_row, long long v_row, const int* slots, int8_t* codes,
+                                              uint8_t* exponents, int rows, int heads, int page_size, int dim, int row0, int slot, int block, int lane) {
   const int page = slot / page_size, first = slot - page * page_size;
-  if (row0 && first && slots[row0 - 1] == slot - 1) return;
   int n = 1;                                                            // rows of the run
   for (int at = 1; at < page_size - first; at += 32) {
     const int i = at + lane;
@@ -155,6 +148,30 @@ kv8_store_kernel(const T* k, const T* v, long long k_row, long long v_row, const
     Piece8<T> p;
     p.load(at(i));
     round(i, p);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv8_store_kernel(const T* k, const T* v, long long k_row, long long v_row, const int* slots, int8_t* codes, uint8_t* exponents, int rows,
+                 int heads, int page_size, int dim, int window) {
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  const int lane = threadIdx.x & 31, block = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (block >= 2 * heads) return;
+  const int row = blockIdx.x * window + lane;
+  int slot = -1, before = -1;
+  if (lane < window && row < rows) {
+    slot = slots[row];
+    if (row) before = slots[row - 1];
+  }
+  // a row begins a run if it is stored and does not follow the row before it in one page
+  uint32_t begins = __ballot_sync(0xffffffffu, slot >= 0 && !(slot % page_size && before == slot - 1));
+  while (begins) {
+    const int src = __ffs(begins) - 1;
+    begins &= begins - 1;
+    kv8_store_run<T>(k, v, k_row, v_row, slots, codes, exponents, rows, heads, page_size, dim, blockIdx.x * window + src,
+                     __shfl_sync(0xffffffffu, slot, src), block, lane);
   }
 }
 
@@ -250,12 +267,13 @@ IFB_EXPORT int ifb_kv8_store(const void* k, const void* v, int dtype, long long 
   const int esize = dtype == IFB_F32 ? 4 : 2;
   if ((((uintptr_t)k) | ((uintptr_t)v) | (uintptr_t)(k_row * esize) | (uintptr_t)(v_row * esize) | ((uintptr_t)codes)) & 15) return IFB_ERR_ALIGN;
   const int warps = 2 * heads < 8 ? 2 * heads : 8;
-  const dim3 grid(rows, (2 * heads + warps - 1) / warps);
+  const int window = rows > 256 ? 16 : 1;
+  const dim3 grid((rows + window - 1) / window, (2 * heads + warps - 1) / warps);
   if (dtype == IFB_F32)
     return ifb_launch(kv8_store_kernel<float>, grid, dim3(32 * warps), 0, (cudaStream_t)stream, (const float*)k, (const float*)v, k_row, v_row,
-                      (const int*)slots, (int8_t*)codes, (uint8_t*)exponents, rows, heads, page_size, dim);
+                      (const int*)slots, (int8_t*)codes, (uint8_t*)exponents, rows, heads, page_size, dim, window);
   return ifb_launch(kv8_store_kernel<bf16>, grid, dim3(32 * warps), 0, (cudaStream_t)stream, (const bf16*)k, (const bf16*)v, k_row, v_row,
-                    (const int*)slots, (int8_t*)codes, (uint8_t*)exponents, rows, heads, page_size, dim);
+                    (const int*)slots, (int8_t*)codes, (uint8_t*)exponents, rows, heads, page_size, dim, window);
 }
 
 IFB_EXPORT int ifb_kv8_values(const void* codes, const void* exponents, void* out, int dtype, int pages, int heads, int page_size, int dim,
