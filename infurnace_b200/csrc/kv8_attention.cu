@@ -1,107 +1,36 @@
-// Causal attention over pages of keys and values held in 8 bits (kv8.cu has the format), compiled for one head size
-// (-DHEAD_DIM=<multiple of 16, at most 256>) and one number of terms (-DTERMS=1: bfloat16 queries and output; 2: float32).
+// Causal attention over pages of keys and values held in 8 bits (kv8.cu has the format), bfloat16 queries and output, compiled for
+// one head size (-DHEAD_DIM=<multiple of 16, at most 256>).
 //
 // The products run on the tensor cores (mma.sync, float32 accumulation) over the codes as whole numbers, which half precision
 // holds exactly; a page's step enters as a factor of its scores (keys) and of its weights (values), so no number is rounded
-// for having been 8 bits.  With TERMS 2 a query and a softmax weight are each the sum of two half-precision numbers, 22 bits.
-//
-// The products are transposed: S^T = K Q^T and O^T = V^T P^T, so that keys (and head dimensions) fill the 16 rows of an
-// instruction and up to eight score rows (query token x query head of a key head) its 8 columns; decoding with eight query
-// heads per key head wastes nothing.  A warp takes 16 keys of one page at a time: their codes come from global memory to
-// registers in 16-byte pieces, each already where its product wants it (any order of the dimensions serves the sums over
-// them, so the order is the loads'), so there is no shared memory, no barrier and no wait between warps in the loop; the
-// other warps of the SM and the order of the requests (the next keys while the values are multiplied, the next values while
-// the scores are formed) keep the memory busy.
+// for having been 8 bits.  A query row times a power of two is half precision too (exact down to 2^-24 of its largest), and so
+// is a softmax weight, the one thing that is rounded (11 bits).
 //
 // From bits to half-precision numbers: u = code + 128 in the low byte of a half is the subnormal number u 2^-24, exactly; two
-// integer instructions make two of them.  Keys of bfloat16 queries stay so (q . (u - 127.5) = q . u - 127.5 sum(q), the second
-// known per row); for values, and for keys of float32 queries, 128 is taken off again: a sum over thousands of keys would lose
-// what the offset swamps, and a float32 score has no bits to spare for it.
+// integer instructions make two of them.  Keys stay so (q . (u - 127.5) = q . u - 127.5 sum(q), the second known per row);
+// for values 128 is taken off again: a sum over thousands of keys would lose what the offset swamps.
 //
 // Softmax: weights are 2^(score - m + 8) with a reference m per row that moves (and then rescales the sums) only when a score
 // exceeds it by 6 in the exponent, so that most tiles need no maximum over lanes; 2^14 is then the largest weight, and
 // half-precision numbers down to 2^-32 of it still count.  A weight enters the product times its page's step over the largest
 // step so far.  Sums are float32.
 //
-// Split form: the keys of a key head for one tile of score rows are cut into pieces of nearly one length for all requests,
-// whatever their lengths, as many as CTAs fit on the device; a piece leaves its sums in scratch memory, and the CTA that arrives
-// last at an item adds them in the order of the pieces.  Whole form (prompts): a warp owns its score rows over all their keys.
-// Keys that no row of a tile sees are not read; block-table entries outside are not followed.  A row that sees no key is zero.
-#include "common.cuh"
+// What bounds it: a warp takes some 380 instructions for 16 keys of 128, 260 of them on the integer pipe, most for the bytes of keys
+// and values; the loop brings 4.8 to 5.8 TB/s, and a call has some 9 us beside it (the look at the lengths, the first trip, the joins).
+// Eight requests of 3,967 to 8,095 keys (32 heads on 8) 28 us, 3.5 TB/s; 64 of 129 to 383 (16 on 8) 16 us.
+#define KV8_F32 0
+#include "kv8_attention.cuh"
 #include <cuda_fp16.h>
-#include <math.h>
 
-#ifndef HEAD_DIM
-#error "compile with -DHEAD_DIM=<head size>"
-#endif
-#if HEAD_DIM % 16 != 0 || HEAD_DIM < 16 || HEAD_DIM > 256
-#error "HEAD_DIM must be a multiple of 16 between 16 and 256"
-#endif
-#ifndef TERMS
-#define TERMS 1
-#endif
-
-typedef __nv_bfloat16 bf16;
-#if TERMS == 2
-typedef float qtype;
-#else
-typedef bf16 qtype;
-#endif
-constexpr int D = HEAD_DIM;
-constexpr int KS = D / 16;               // k steps of a score product, m tiles of an output product
-constexpr int WARPS = 4;
-constexpr int K64 = D / 64;              // pieces of 64 dimensions of a key that a quad of lanes takes 16 bytes a lane at a time
-constexpr int UNIT = 16 * WARPS;         // keys of a unit of the split form
-constexpr int NO_ROW = -1000000000;
-
-struct Kv8Args {
-  const qtype* q;
-  long long q_row;                       // elements between tokens
-  const int8_t* codes;
-  const uint8_t* exponents;
-  const int* tables;
-  int table_stride;
-  const int* cu_q;
-  const int* seq_lens;
-  qtype* out;                            // [tokens][heads][D]
-  float* parts;                          // split form: [CTA][rows of a tile][D + 2]
-  int* counters;                         // split form: one per item, 0 between launches
-  int requests, heads, kv_heads, page_size, window;
-  float scale;                           // of the scores, times log2(e)
-  int min_rows, max_rows;                // requests with fewer or more score rows than this are another kernel's
-  int tiles;                             // split form: tiles of score rows that any request has at most
-  int most;                              // split form: CTAs that run on the device at a time
-};
-
-__device__ __forceinline__ float kv8_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float kv8_step(uint32_t f) {                 // 2^(f - 133), 0, NaN
-  if (f == 0u) return 0.f;
-  if (f == 255u) return __uint_as_float(0x7fffffffu);
-  return f > 6u ? __uint_as_float((f - 6u) << 23) : __uint_as_float(1u << (f + 16u));
-}
 // d += a b: a 16 x 16 (rows by k), b 16 x 8.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t transpose8(uint32_t x) {            // of an 8 x 8 matrix of halves over the warp
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
-  return y;
-}
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t pack_half_rest(float lo, float hi, uint32_t rounded) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&rounded));
-  return pack_half(lo - f.x, hi - f.y);
-}
-constexpr float KEY_OFFSET = TERMS == 2 ? 0.5f : -127.5f;              // what a key's number has beside its half-precision one
 // Bytes 0 and 2 (and 1 and 3) of a word of codes as half-precision numbers (code + 128) 2^-24.
 __device__ __forceinline__ uint32_t even_bytes(uint32_t w) { return (w & 0x00ff00ffu) ^ 0x00800080u; }
 __device__ __forceinline__ uint32_t odd_bytes(uint32_t w) { return ((w >> 8) & 0x00ff00ffu) ^ 0x00800080u; }
@@ -110,17 +39,6 @@ __device__ __forceinline__ uint32_t centred(uint32_t x) {               // code 
   const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&off));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
-
-// ---- pieces of a value row: blocks of 128, 64, 32 and 16 dimensions, an eighth of a block (16, 8, 4, 2 bytes) per lane -------
-template <int W> struct Piece;
-template <> struct Piece<128> { uint4 r; __device__ __forceinline__ void load(const int8_t* p) { r = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; } };
-template <> struct Piece<64> { uint2 r; __device__ __forceinline__ void load(const int8_t* p) { r = *reinterpret_cast<const uint2*>(p); }
-  __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? r.x : r.y; } };
-template <> struct Piece<32> { uint32_t r; __device__ __forceinline__ void load(const int8_t* p) { r = *reinterpret_cast<const uint32_t*>(p); }
-  __device__ __forceinline__ uint32_t word(int) const { return r; } };
-template <> struct Piece<16> { uint32_t r; __device__ __forceinline__ void load(const int8_t* p) { r = *reinterpret_cast<const uint16_t*>(p); }
-  __device__ __forceinline__ uint32_t word(int) const { return r; } };
 
 // The values of 16 keys as a lane holds them: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 (c = lane % 4).  Blocks follow one another.
 template <int LEFT> struct Values {
@@ -134,69 +52,30 @@ template <int LEFT> struct Values {
   }
   // o^T += v^T p^T; m tile i of a block has dimension chunk + 2 i in its row lane / 4 and chunk + 2 i + 1 in row lane / 4 + 8
   template <int NT>
-  __device__ __forceinline__ void multiply(float (*o)[NT][4], const uint32_t (&p)[TERMS][NT][2]) const {
+  __device__ __forceinline__ void multiply(float (*o)[NT][4], const uint32_t (&p)[NT][2]) const {
 #pragma unroll
     for (int i = 0; i < W / 16; ++i) {
       const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;
       const uint32_t x = __byte_perm(v[0].word(i >> 1), v[1].word(i >> 1), sel), y = __byte_perm(v[2].word(i >> 1), v[3].word(i >> 1), sel);
       const uint32_t a0 = centred(even_bytes(x)), a1 = centred(odd_bytes(x)), a2 = centred(even_bytes(y)), a3 = centred(odd_bytes(y));
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#if TERMS == 2
-        float x[4] = {0.f, 0.f, 0.f, 0.f};                              // (added up outside of the tensor core, as the scores are)
-        mma_f16(x, a0, a1, a2, a3, p[1][n][0], p[1][n][1]);
-        mma_f16(x, a0, a1, a2, a3, p[0][n][0], p[0][n][1]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][n][j] += x[j];
-#else
-        mma_f16(o[i][n], a0, a1, a2, a3, p[0][n][0], p[0][n][1]);
-#endif
-      }
+      for (int n = 0; n < NT; ++n) mma_f16(o[i][n], a0, a1, a2, a3, p[n][0], p[n][1]);
     }
     rest.template multiply<NT>(o + W / 16, p);
-  }
-  // the dimension of element e (0, 1) of m tile i
-  static __device__ __forceinline__ int dim(int i, int lane, int e) {
-    if (i < W / 16) return (lane >> 2) * (W / 8) + 2 * i + e;
-    return W + Values<LEFT - W>::dim(i - W / 16, lane, e);
   }
 };
 template <> struct Values<0> {
   __device__ __forceinline__ void load(const int8_t*, int) {}
-  template <int NT> __device__ __forceinline__ void multiply(float (*)[NT][4], const uint32_t (&)[TERMS][NT][2]) const {}
-  static __device__ __forceinline__ int dim(int, int, int) { return 0; }
+  template <int NT> __device__ __forceinline__ void multiply(float (*)[NT][4], const uint32_t (&)[NT][2]) const {}
 };
-
-// The keys of a tile as a lane holds them: keys lane / 4 and lane / 4 + 8.
-struct Keys {
-  uint4 w[2][K64 ? K64 : 1];
-  uint32_t tail[2][KS - 4 * K64 ? KS - 4 * K64 : 1];
-  __device__ __forceinline__ void load(const int8_t* tile, int lane) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int8_t* p = tile + ((lane >> 2) + 8 * e) * D;
-#pragma unroll
-      for (int h = 0; h < K64; ++h) w[e][h] = *reinterpret_cast<const uint4*>(p + h * 64 + (lane & 3) * 16);
-#pragma unroll
-      for (int s = 0; s < KS - 4 * K64; ++s) tail[e][s] = *reinterpret_cast<const uint32_t*>(p + K64 * 64 + s * 16 + (lane & 3) * 4);
-    }
-  }
-  __device__ __forceinline__ uint32_t word(int e, int ks) const {
-    if (ks >= 4 * K64) return tail[e][ks - 4 * K64];
-    const uint4& x = w[e][ks >> 2];
-    return (ks & 3) == 0 ? x.x : (ks & 3) == 1 ? x.y : (ks & 3) == 2 ? x.z : x.w;
-  }
-};
-// Where the four dimensions of a lane's word of k step ks begin.
-__device__ __forceinline__ int key_dim(int ks, int lane) {
-  return ks < 4 * K64 ? (ks >> 2) * 64 + (lane & 3) * 16 + (ks & 3) * 4 : K64 * 64 + (ks - 4 * K64) * 16 + (lane & 3) * 4;
-}
 
 // One warp over tiles of 16 keys for up to 8 NT score rows of one key head.  In the layout of the results a lane has rows
 // 8 n + 2 (lane % 4) + {0, 1} of row tile n.
 template <int NT>
 struct Stream {
-  uint32_t qf[TERMS][NT][KS][2];
+  static constexpr int ROW_TILES = NT, TILE = 16;                        // keys of a step
+  static constexpr int CTAS = NT == 1 ? (D <= 128 ? 4 : 2) : D <= 128 ? 2 : 1;      // on an SM, that the registers are cut for
+  uint32_t qf[NT][KS][2];
   float qscale[NT][2], qoff[NT][2];      // what turns a product into a number of real units: times qscale, and qoff
   int last[NT][2];                       // position of the row's query (NO_ROW: no such row)
   // m: reference of the row's scores; rise: what a score has to exceed to move it; shift: what is added to a score for its weight;
@@ -215,36 +94,9 @@ struct Stream {
       for (int i = 0; i < KS; ++i) { o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f; }
     }
   }
-  // The queries come in two parts as well, so that their trip and that of the first keys overlap.
-  struct Queries { uint32_t w[NT][KS][sizeof(qtype) == 2 ? 2 : 4]; };
-  // row0: the first of the rows; rows: how many the request has; G: query heads per key head.
-  static __device__ __forceinline__ void request(Queries& raw, const Kv8Args& a, int first_token, int row0, int rows, int kv_head, int G, int lane) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int row = row0 + n * 8 + (lane >> 2);
-      const bool in = row < rows;
-      const int token = in ? row / G : 0, head = in ? row - token * G : 0;
-      const qtype* src = a.q + (size_t)(first_token + token) * a.q_row + (size_t)(kv_head * G + head) * D;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const int d = key_dim(ks, lane);
-#if TERMS == 2
-        const uint4 x = in ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
-        raw.w[n][ks][0] = x.x; raw.w[n][ks][1] = x.y; raw.w[n][ks][2] = x.z; raw.w[n][ks][3] = x.w;
-#else
-        const uint2 x = in ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
-        raw.w[n][ks][0] = x.x; raw.w[n][ks][1] = x.y;
-#endif
-      }
-    }
-  }
   // pos0: position of the request's first query.
-  __device__ __forceinline__ void queries(const Queries& raw, int row0, int rows, int pos0, int G, int lane) {
-#if TERMS == 2
-    auto number = [&](int n, int ks, int j) { return __uint_as_float(raw.w[n][ks][j]); };
-#else
+  __device__ __forceinline__ void queries(const Queries<NT>& raw, int row0, int rows, int pos0, int G, int lane) {
     auto number = [&](int n, int ks, int j) { const uint32_t w = raw.w[n][ks][j >> 1]; return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16); };
-#endif
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       uint32_t amax = 0;
@@ -263,24 +115,18 @@ struct Stream {
         float x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = number(n, ks, j) * to;
-        qf[0][n][ks][0] = pack_half(x[0], x[2]);                        // beside the even and the odd bytes of a word of codes
-        qf[0][n][ks][1] = pack_half(x[1], x[3]);
-#if TERMS == 2
-        qf[1][n][ks][0] = pack_half_rest(x[0], x[2], qf[0][n][ks][0]);
-        qf[1][n][ks][1] = pack_half_rest(x[1], x[3], qf[0][n][ks][1]);
-#endif
+        qf[n][ks][0] = pack_half(x[0], x[2]);                        // beside the even and the odd bytes of a word of codes
+        qf[n][ks][1] = pack_half(x[1], x[3]);
       }
       // sums of the rounded rows, in the layout of the scores, by a product with ones
       float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) mma_f16(s, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, qf[t][n][ks][0], qf[t][n][ks][1]);
+      for (int ks = 0; ks < KS; ++ks) mma_f16(s, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, qf[n][ks][0], qf[n][ks][1]);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float b = __shfl_sync(0xffffffffu, back, ((lane & 3) * 2 + e) * 4);
         qscale[n][e] = b * 16777216.f;
-        qoff[n][e] = KEY_OFFSET * s[e] * b;
+        qoff[n][e] = -127.5f * s[e] * b;
         const int r = row0 + n * 8 + (lane & 3) * 2 + e;
         last[n][e] = r < rows ? pos0 + r / G : NO_ROW;
       }
@@ -294,21 +140,9 @@ struct Stream {
     for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      uint32_t a0 = even_bytes(k.word(0, ks)), a1 = even_bytes(k.word(1, ks)), a2 = odd_bytes(k.word(0, ks)), a3 = odd_bytes(k.word(1, ks));
-      if (TERMS == 2) { a0 = centred(a0); a1 = centred(a1); a2 = centred(a2); a3 = centred(a3); }
+      const uint32_t a0 = even_bytes(k.word(0, ks)), a1 = even_bytes(k.word(1, ks)), a2 = odd_bytes(k.word(0, ks)), a3 = odd_bytes(k.word(1, ks));
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#if TERMS == 2
-        // the tensor core's running sum is cut off, not rounded, at each step: a float32 score is added up outside of it
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_f16(x, a0, a1, a2, a3, qf[1][n][ks][0], qf[1][n][ks][1]);
-        mma_f16(x, a0, a1, a2, a3, qf[0][n][ks][0], qf[0][n][ks][1]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] += x[j];
-#else
-        mma_f16(s[n], a0, a1, a2, a3, qf[0][n][ks][0], qf[0][n][ks][1]);
-#endif
-      }
+      for (int n = 0; n < NT; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][ks][0], qf[n][ks][1]);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -361,7 +195,7 @@ struct Stream {
     }
     // the step of this page's values over the reference
     const float fw = vf == 0 ? 0.f : __uint_as_float((uint32_t)max(0, 127 + vf - v_ref) << 23);
-    uint32_t p[TERMS][NT][2];
+    uint32_t p[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float w[4];
@@ -375,53 +209,26 @@ struct Stream {
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] *= fw;
-      const uint32_t lo = pack_half(w[0], w[1]), hi = pack_half(w[2], w[3]);
-      p[0][n][0] = transpose8(lo);
-      p[0][n][1] = transpose8(hi);
-#if TERMS == 2
-      p[1][n][0] = transpose8(pack_half_rest(w[0], w[1], lo));
-      p[1][n][1] = transpose8(pack_half_rest(w[2], w[3], hi));
-#endif
+      p[n][0] = transpose8(pack_half(w[0], w[1]));
+      p[n][1] = transpose8(pack_half(w[2], w[3]));
     }
     v.template multiply<NT>(o, p);
   }
 
   // Tiles first, first + step, ... up to `end` (exclusive) of 16 keys, in two parts: `begin` requests the first of them, `run` works
   // through all.  full_from, full_to: keys from and up to here are seen by every row that exists.
-  struct Walk {
-    const int* table;
-    const int8_t* base;
-    const uint8_t* fields;
-    size_t page_bytes, v_off;
-    uint32_t per_page, inverse;
-    int kv_heads, first, end, step, next_page, kf, vf;
+  struct Walk : Kv8Pages {
+    int first, end, step, next_page, kf, vf;
     Keys k;
     Values<D> v;
-    // (t / per_page by a product with the next whole number above 2^32 / per_page: exact for t below 2^32 / per_page)
-    __device__ __forceinline__ int page_of(int t) const { return per_page > 1 ? (int)__umulhi((uint32_t)t, inverse) : t; }
-    __device__ __forceinline__ const int8_t* tile(int t, int page) const {
-      return base + (size_t)page * page_bytes + (uint32_t)(t - page_of(t) * (int)per_page) * (16 * D);
-    }
-    __device__ __forceinline__ void read_fields(int page) {
-      const uint8_t* f = fields + (size_t)page * 2 * kv_heads;
-      kf = f[0];
-      vf = f[kv_heads];
-    }
-    __device__ __forceinline__ Walk(const Kv8Args& a, const int* table_, int kv_head, int first_, int end_, int step_, int lane) {
-      table = table_;
-      page_bytes = 2 * (size_t)a.kv_heads * a.page_size * D;
-      base = a.codes + (size_t)kv_head * a.page_size * D;
-      v_off = (size_t)a.kv_heads * a.page_size * D;
-      fields = a.exponents + kv_head;
-      kv_heads = a.kv_heads;
-      per_page = (uint32_t)a.page_size / 16;
-      inverse = per_page > 1 ? 0xffffffffu / per_page + 1 : 0;
+    __device__ __forceinline__ Walk(const Kv8Args& a, const int* table_, int kv_head, int, int, int first_, int end_, int step_, int lane)
+        : Kv8Pages(a, table_, kv_head) {
       first = first_; end = end_; step = step_; next_page = 0;
       if (first >= end) return;
-      const int page = table[page_of(first)];
-      if (first + step < end) next_page = table[page_of(first + step)];
-      const int8_t* at = tile(first, page);
-      read_fields(page);
+      const int page = page_of(first);
+      if (first + step < end) next_page = page_of(first + step);
+      const int8_t* at = keys(first, page);
+      read_fields(page, kf, vf);
       k.load(at, lane);
       v.load(at + v_off, lane);
     }
@@ -438,10 +245,10 @@ struct Stream {
       else scores<true>(w.k, ks, t * 16, a.window, s, lane);
       const int8_t* next = w.base;
       if (more) {                                                       // the next keys while these values are multiplied
-        next = w.tile(t + w.step, w.next_page);
-        w.read_fields(w.next_page);
+        next = w.keys(t + w.step, w.next_page);
+        w.read_fields(w.next_page, w.kf, w.vf);
         w.k.load(next, lane);
-        if (t + 2 * w.step < w.end) w.next_page = w.table[w.page_of(t + 2 * w.step)];
+        if (t + 2 * w.step < w.end) w.next_page = w.page_of(t + 2 * w.step);
       }
       weigh(s, w.v, vf);
       if (more) w.v.load(next + w.v_off, lane);                         // and the next values while the next scores are formed
@@ -467,315 +274,5 @@ struct Stream {
   }
 };
 
-__device__ __forceinline__ void kv8_store_pair(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
-__device__ __forceinline__ void kv8_store_pair(bf16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
-__device__ __forceinline__ float kv8_ratio(float o, float l) { return l == 0.f ? 0.f : o / l; }
 
-// --------------------------------------------------------------------------------------------
-// Whole form: grid (blocks of 32 NT rows, key heads, requests); a warp has 8 NT rows over all their keys.
-// --------------------------------------------------------------------------------------------
-template <int NT>
-__global__ void __launch_bounds__(32 * WARPS)
-kv8_attention_whole_kernel(Kv8Args a) {
-  ifb_pdl_wait();
-  ifb_pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.z, kv_head = blockIdx.y, G = a.heads / a.kv_heads;
-  const int q0 = a.cu_q[r], q_len = a.cu_q[r + 1] - q0, L = a.seq_lens[r], rows = q_len * G;
-  if (q_len <= 0 || rows < a.min_rows || rows > a.max_rows) return;
-  // the rows with the most keys first
-  const int row0 = ((int)(gridDim.x - 1 - blockIdx.x) * WARPS + warp) * 8 * NT;
-  if (row0 >= rows) return;
-  const int pos0 = L - q_len, p_first = pos0 + row0 / G, p_last = pos0 + min(row0 + 8 * NT - 1, rows - 1) / G;
-  const int lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
-  typename Stream<NT>::Queries raw;
-  Stream<NT>::request(raw, a, q0, row0, rows, kv_head, G, lane);
-  typename Stream<NT>::Walk walk(a, a.tables + (size_t)r * a.table_stride, kv_head, lo / 16, p_last >= 0 ? p_last / 16 + 1 : 0, 1, lane);
-  Stream<NT> st;
-  st.reset();
-  st.queries(raw, row0, rows, pos0, G, lane);
-  st.run(a, walk, a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
-  st.finish();
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int row = row0 + n * 8 + (lane & 3) * 2 + e;
-      if (row >= rows) continue;
-      qtype* to = a.out + ((size_t)(q0 + row / G) * a.heads + kv_head * G + row % G) * D;
-#pragma unroll
-      for (int i = 0; i < KS; ++i)
-        kv8_store_pair(to + Values<D>::dim(i, lane, 0), kv8_ratio(st.o[i][n][e], st.l[n][e]), kv8_ratio(st.o[i][n][2 + e], st.l[n][e]));
-    }
-}
-
-// CTAs on an SM that the registers are cut for.
-constexpr int split_ctas(int nt) { return nt == 1 && TERMS == 1 ? (D <= 128 ? 4 : 2) : D <= 128 ? 2 : 1; }
-
-// --------------------------------------------------------------------------------------------
-// Split form.  Items are (request, tile of 8 NT rows, key head), in that order; an item has the units of its request (those of
-// the request's last row: earlier tiles leave a few empty), one at least, so that a row without keys is written.  A CTA has one
-// piece of one item.  With `most` CTAs on the device at once and fewer items, pieces have total / (most - items) units or a little
-// less, for which the pieces of all items are no more than `most`; else every item is one piece.  (Equal shares of the units, with
-// CTAs that have the end of one item and the beginning of the next, are a tenth shorter and cost a second start and a second join.)
-// --------------------------------------------------------------------------------------------
-constexpr int MAX_PARTS = 32;            // pieces of an item
-constexpr int PITCH = D + 8;             // of a row of sums in shared memory (the rows of a quad of lanes fall on two halves of the banks)
-// Where a warp's sums lie in a row: m tile by m tile, the lanes' pairs side by side.
-__device__ __forceinline__ int kv8_place(int i, int lane) { return i * 16 + (lane >> 2) * 2; }
-__device__ __forceinline__ int kv8_place_dim(int place) { return Values<D>::dim(place >> 4, ((place & 15) >> 1) << 2, 0); }
-
-// What a lane knows of request r0 + lane: where its queries lie, the units of an item and its items.
-struct Kv8Look { int q0, q_len, L, units, items; };
-template <int ROWS>
-__device__ __forceinline__ Kv8Look kv8_look(const Kv8Args& a, int G, int r0, int lane) {
-  Kv8Look k = {};
-  const int r = r0 + lane;
-  if (r < a.requests) {
-    k.q0 = a.cu_q[r]; k.q_len = a.cu_q[r + 1] - k.q0; k.L = a.seq_lens[r];
-    const int rows = k.q_len * G;
-    if (k.q_len > 0 && rows >= a.min_rows && rows <= a.max_rows) {
-      k.items = (rows + ROWS - 1) / ROWS * a.kv_heads;
-      const int lo = a.window > 0 ? max(0, k.L - k.q_len - a.window + 1) : 0;
-      k.units = k.L > 0 ? max(1, (k.L - 1) / UNIT - lo / UNIT + 1) : 1;
-    }
-  }
-  return k;
-}
-
-// ceil(x / y) of whole numbers from 1 on, x below 2^20 (units of a request: 2^26 keys): the quotient's error is below the half that
-// is taken off.
-__device__ __forceinline__ int kv8_parts(int x, float inverse) { return (int)(((float)x - 0.5f) * inverse) + 1; }
-
-template <int NT>
-__global__ void __launch_bounds__(32 * WARPS, split_ctas(NT))
-kv8_attention_split_kernel(Kv8Args a) {
-  constexpr int ROWS = 8 * NT;
-  extern __shared__ __align__(16) float sums[];                         // [WARPS][ROWS][PITCH], then maxima and sums [WARPS][ROWS] each
-  __shared__ float part_m[MAX_PARTS][ROWS], part_l[MAX_PARTS][ROWS];
-  __shared__ int arrived;
-  ifb_pdl_wait();
-  ifb_pdl_trigger();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads;
-  float* const sm_m = sums + WARPS * ROWS * PITCH;
-  float* const sm_l = sm_m + WARPS * ROWS;
-  // every warp for itself: how long pieces are, and whose piece this CTA's is
-  const Kv8Look known = kv8_look<ROWS>(a, G, 0, lane), known2 = a.requests > 32 ? kv8_look<ROWS>(a, G, 32, lane) : Kv8Look{};
-  auto look = [&](int r0) { return r0 == 0 ? known : r0 == 32 ? known2 : kv8_look<ROWS>(a, G, r0, lane); };
-  int total = 0, items = 0, longest = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += 32) {
-    const Kv8Look k = look(r0);
-    total += k.units * k.items;
-    items += k.items;
-    longest = max(longest, k.units);
-  }
-  total = __reduce_add_sync(0xffffffffu, total);
-  items = __reduce_add_sync(0xffffffffu, items);
-  longest = __reduce_max_sync(0xffffffffu, longest);
-  const int spare = a.most - items, least = (longest + MAX_PARTS - 1) / MAX_PARTS;
-  int per = max(spare > 0 ? (total + spare - 1) / spare : longest, least);
-  if (spare > 0 && a.requests <= 64) {
-    // pieces a unit shorter, as long as there are CTAs for them (the bound above counts an unfinished piece for every item)
-    for (int tries = 0; tries < 4 && per > max(least, 1); ++tries) {
-      const float inverse = 1.f / (float)(per - 1);
-      const int one = (known.items ? kv8_parts(known.units, inverse) : 0) * known.items + (known2.items ? kv8_parts(known2.units, inverse) : 0) * known2.items;
-      if (__reduce_add_sync(0xffffffffu, one) > a.most) break;
-      --per;
-    }
-  }
-  const float per_inverse = 1.f / (float)per;
-  int r = -1, q0, q_len, L, units, pieces, at = blockIdx.x;             // at: of the pieces of the request
-  for (int r0 = 0; r0 < a.requests; r0 += 32) {
-    const Kv8Look k = look(r0);
-    const int mine = k.items ? kv8_parts(k.units, per_inverse) : 0;
-    int upto = mine * k.items;
-    const int own = upto;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += y;
-    }
-    const uint32_t hit = __ballot_sync(0xffffffffu, at < upto);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      r = r0 + src;
-      at -= __shfl_sync(0xffffffffu, upto - own, src);
-      units = __shfl_sync(0xffffffffu, k.units, src);
-      pieces = __shfl_sync(0xffffffffu, mine, src);
-      q0 = __shfl_sync(0xffffffffu, k.q0, src);
-      q_len = __shfl_sync(0xffffffffu, k.q_len, src);
-      L = __shfl_sync(0xffffffffu, k.L, src);
-      break;
-    }
-    at -= __shfl_sync(0xffffffffu, upto, 31);
-  }
-  if (r < 0) return;                                                    // more CTAs than pieces
-  const int item = at / pieces, piece = at - item * pieces, tile = item / a.kv_heads, kv_head = item - tile * a.kv_heads;
-  const int rows = q_len * G, row0 = tile * ROWS, here = min(ROWS, rows - row0);
-  const int pos0 = L - q_len, p_first = pos0 + row0 / G, p_last = pos0 + (row0 + here - 1) / G;
-  const int lo_request = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
-  const int each = (units + pieces - 1) / pieces;                       // units of a piece
-  const int key0 = (lo_request / UNIT + piece * each) * UNIT, key_end = min(p_last + 1, key0 + each * UNIT);
-  typename Stream<NT>::Queries raw;
-  Stream<NT>::request(raw, a, q0, row0, rows, kv_head, G, lane);
-  typename Stream<NT>::Walk walk(a, a.tables + (size_t)r * a.table_stride, kv_head, max(key0, lo) / 16 + warp, key_end > 0 ? (key_end + 15) / 16 : 0,
-                                 WARPS, lane);
-  Stream<NT> st;
-  st.reset();
-  st.queries(raw, row0, rows, pos0, G, lane);
-  st.run(a, walk, a.window > 0 ? p_last - a.window + 1 : 0, p_first, lane);
-  st.finish();
-  // the warps' sums side by side
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int row = n * 8 + (lane & 3) * 2 + e;
-      if (row < here) {
-        float* to = sums + (warp * ROWS + row) * PITCH;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) *reinterpret_cast<float2*>(to + kv8_place(i, lane)) = make_float2(st.o[i][n][e], st.o[i][n][2 + e]);
-        if (lane < 4) { sm_m[warp * ROWS + row] = st.m[n][e]; sm_l[warp * ROWS + row] = st.l[n][e]; }
-      }
-    }
-  __syncthreads();
-  auto finish_row = [&](int row, int place, float4 o, float l) {       // four numbers side by side are two neighbouring lanes' pairs
-    const int full = row0 + row;
-    qtype* to = a.out + ((size_t)(q0 + full / G) * a.heads + kv_head * G + full % G) * D;
-    kv8_store_pair(to + kv8_place_dim(place), kv8_ratio(o.x, l), kv8_ratio(o.y, l));
-    kv8_store_pair(to + kv8_place_dim(place + 2), kv8_ratio(o.z, l), kv8_ratio(o.w, l));
-  };
-  auto add = [](float4& o, const float4& x, float f) { o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w); };
-  float* const mine = a.parts + (size_t)blockIdx.x * ROWS * (D + 2);
-  for (int i = tid; i < here * (D / 4); i += 32 * WARPS) {
-    const int row = i / (D / 4), place = (i - row * (D / 4)) * 4;
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_m[w * ROWS + row]);
-    const float U = M == -INFINITY ? 0.f : M;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float f = kv8_exp2(sm_m[w * ROWS + row] - U);
-      add(o, *reinterpret_cast<const float4*>(sums + (w * ROWS + row) * PITCH + place), f);
-      l = fmaf(sm_l[w * ROWS + row], f, l);
-    }
-    if (pieces == 1) {
-      finish_row(row, place, o, l);
-    } else {
-      *reinterpret_cast<float4*>(mine + row * D + place) = o;
-      if (place == 0) { mine[ROWS * D + row] = M; mine[ROWS * (D + 1) + row] = l; }
-    }
-  }
-  if (pieces == 1) return;
-  __syncthreads();
-  int* const counter = a.counters + ((size_t)r * a.tiles + tile) * a.kv_heads + kv_head;
-  if (tid == 0) {                                                       // its fence covers what the barrier ordered before it
-    __threadfence();
-    arrived = atomicAdd(counter, 1);
-    __threadfence();
-  }
-  __syncthreads();
-  if (arrived != pieces - 1) return;
-  // the last of the item's pieces to arrive adds them all, in their order
-  const float* const first = mine - (size_t)piece * ROWS * (D + 2);
-  auto part = [&](int c) { return first + (size_t)c * ROWS * (D + 2); };
-  for (int i = tid; i < here * pieces; i += 32 * WARPS) {
-    const float* from = part(i / here) + ROWS * D + i % here;
-    part_m[i / here][i % here] = __ldcg(from);
-    part_l[i / here][i % here] = __ldcg(from + ROWS);
-  }
-  __syncthreads();
-  for (int i = tid; i < here * (D / 4); i += 32 * WARPS) {
-    const int row = i / (D / 4), place = (i - row * (D / 4)) * 4;
-    float M = -INFINITY, l = 0.f;
-    for (int c = 0; c < pieces; ++c) M = fmaxf(M, part_m[c][row]);
-    const float U = M == -INFINITY ? 0.f : M;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c0 = 0; c0 < pieces; c0 += 8) {
-      float4 x[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (c0 + c < pieces) x[c] = __ldcg(reinterpret_cast<const float4*>(part(c0 + c) + row * D + place));
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (c0 + c < pieces) {
-          const float f = kv8_exp2(part_m[c0 + c][row] - U);
-          add(o, x[c], f);
-          l = fmaf(part_l[c0 + c][row], f, l);
-        }
-    }
-    finish_row(row, place, o, l);
-  }
-  if (tid == 0) *counter = 0;
-}
-
-template <int NT> static size_t kv8_split_smem() { return (size_t)WARPS * 8 * NT * (PITCH + 2) * sizeof(float); }
-template <int NT> static int kv8_split_ctas(int* ctas) {                // that fit on the device at once
-  static int known[IFB_MAX_DEVICES] = {};
-  int dev = 0, per = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= IFB_MAX_DEVICES) return IFB_ERR_ARG;
-  if (!known[dev]) {
-    IFB_ALLOW_SMEM(kv8_attention_split_kernel<NT>, kv8_split_smem<NT>());
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kv8_attention_split_kernel<NT>, 32 * WARPS, kv8_split_smem<NT>());
-    if (e != cudaSuccess) return -(int)e;
-    known[dev] = (per < 1 ? 1 : per) * ifb_sm_count();
-  }
-  *ctas = known[dev];
-  return IFB_OK;
-}
-
-// Floats of scratch memory that the split form of `nt` row tiles wants, or a negative error.
-IFB_EXPORT long long ifb_kv8_attention_scratch(int nt) {
-  int ctas = 0;
-  const int bad = nt == 1 ? kv8_split_ctas<1>(&ctas) : kv8_split_ctas<2>(&ctas);
-  return bad ? (bad > 0 ? -bad : bad) : (long long)ctas * 8 * nt * (D + 2);
-}
-
-template <int NT>
-static int kv8_launch(const Kv8Args& a, bool whole, int max_q, cudaStream_t stream) {
-  if (whole) {
-    const int rows = max_q * (a.heads / a.kv_heads);
-    const dim3 grid((rows + 8 * NT * WARPS - 1) / (8 * NT * WARPS), a.kv_heads, a.requests);
-    return ifb_launch(kv8_attention_whole_kernel<NT>, grid, dim3(32 * WARPS), 0, stream, a);
-  }
-  int ctas = 0;
-  const int bad = kv8_split_ctas<NT>(&ctas);
-  if (bad) return bad;
-  // (with more items than CTAs at a time each is one piece, and needs no scratch memory)
-  const long long items = (long long)a.requests * a.tiles * a.kv_heads;
-  if (items > 0x7fffffffLL) return IFB_ERR_SIZE;
-  Kv8Args b = a;
-  b.most = ctas;
-  return ifb_launch(kv8_attention_split_kernel<NT>, dim3(items > ctas ? (unsigned)items : (unsigned)ctas), dim3(32 * WARPS), kv8_split_smem<NT>(), stream, b);
-}
-
-// nt: 1 or 2 tiles of 8 score rows per warp.  whole: the whole form.  Requests of min_rows .. max_rows score rows are worked on.
-// One argument, since a call's price on the host is that of its arguments.
-struct Kv8Call {
-  const void* q;
-  long long dtype, q_row;
-  const void *codes, *exponents, *tables;
-  long long table_stride;
-  const void *cu_q, *seq_lens;
-  void *out, *parts, *counters;
-  long long requests, heads, kv_heads, page_size, dim, window, max_q, min_rows, max_rows, tiles, nt, whole;
-  void* stream;
-  double scale;
-};
-IFB_EXPORT int ifb_kv8_attention(const Kv8Call* c) {
-  const bool whole = c->whole != 0;
-  if (c->dtype != (TERMS == 2 ? IFB_F32 : IFB_BF16)) return IFB_ERR_DTYPE;
-  if (c->dim != D || c->heads < 1 || c->kv_heads < 1 || c->heads % c->kv_heads || c->page_size < 16 || c->page_size % 16 || c->requests < 1 ||
-      c->max_q < 1 || c->window < 0 || (c->nt != 1 && c->nt != 2) || c->kv_heads > 65535 || c->requests > 65535 || c->max_q > 0x7fffffff ||
-      c->window > 0x7fffffff || c->heads > 0x7fffffff)
-    return IFB_ERR_SIZE;
-  if (!whole && (!c->parts || !c->counters || c->tiles < 1)) return IFB_ERR_ARG;
-  if ((((uintptr_t)c->q) | ((uintptr_t)c->codes) | ((uintptr_t)c->out) | (uintptr_t)(c->q_row * sizeof(qtype))) & 15) return IFB_ERR_ALIGN;
-  const Kv8Args a = {(const qtype*)c->q, c->q_row, (const int8_t*)c->codes, (const uint8_t*)c->exponents, (const int*)c->tables, (int)c->table_stride,
-                     (const int*)c->cu_q, (const int*)c->seq_lens, (qtype*)c->out, (float*)c->parts, (int*)c->counters, (int)c->requests, (int)c->heads,
-                     (int)c->kv_heads, (int)c->page_size, (int)c->window, (float)c->scale * 1.4426950408889634f, (int)c->min_rows, (int)c->max_rows,
-                     (int)c->tiles, 0};
-  cudaStream_t stream = (cudaStream_t)c->stream;
-  return c->nt == 1 ? kv8_launch<1>(a, whole, (int)c->max_q, stream) : kv8_launch<2>(a, whole, (int)c->max_q, stream);
-}
+KV8_ENTRIES(Stream<1>, Stream<TILES>)

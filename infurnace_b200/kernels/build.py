@@ -47,10 +47,11 @@ LIBRARIES: Dict[str, tuple] = {
     "latent": (["latent.cu", "attention_latent.cu", "attention_latent_mma.cu"], []),
     # matrices in microscaled 4-bit floating point and their products
     "mx4": (["mx4.cu"], []),
-    # keys and values of 8 bits with a scale for each page and head: store and values; attention over them, compiled once per
-    # head size and type: defines={"HEAD_DIM": d} (bfloat16) and {"HEAD_DIM": d, "TERMS": 2} (float32)
+    # keys and values of 8 bits with a scale for each page and head: store and values; attention over them (bfloat16, float32),
+    # compiled once per head size: defines={"HEAD_DIM": d}
     "kv8": (["kv8.cu"], []),
     "kv8_attention": (["kv8_attention.cu"], []),
+    "kv8_attention_f32": (["kv8_attention_f32.cu"], []),
     # compiled once per head size: defines={"HEAD_DIM": d}
     "attention_mma": (["attention_mma.cu"], []),
 }
@@ -65,8 +66,7 @@ DEFAULT_VARIANTS += [("attention_tc", {"HEAD_DIM": 128, "WEIGHT_TERMS": 2, "SOFT
 # plain scores with two-term weights: prompts over 8-bit pages
 DEFAULT_VARIANTS += [("attention_tc", {"HEAD_DIM": d, "WEIGHT_TERMS": 2}) for d in (128, 64, 32)]
 # attention over 8-bit pages: heads of 128 (bfloat16), the sizes that the tests of the engine run, float32
-DEFAULT_VARIANTS += [("kv8_attention", {"HEAD_DIM": d}) for d in (128, 64, 256, 16)]
-DEFAULT_VARIANTS += [("kv8_attention", {"HEAD_DIM": d, "TERMS": 2}) for d in (128, 64, 256, 16)]
+DEFAULT_VARIANTS += [(name, {"HEAD_DIM": d}) for name in ("kv8_attention", "kv8_attention_f32") for d in (128, 64, 256, 16)]
 
 def register_library(name: str, sources: Sequence[str], flags: Sequence[str] = (), *, replace: bool = False) -> None:
     """Make a library of CUDA sources from outside the package known to :func:`load_library`, so that a

@@ -293,12 +293,11 @@ class LowBitKernels:
         libs = self.__dict__.setdefault("_kv8_attention", {})
         lib = libs.get((dim, dtype))
         if lib is None:
-            defines = {"HEAD_DIM": dim} if dtype == torch.bfloat16 else {"HEAD_DIM": dim, "TERMS": 2}
-            lib = load_library("kv8_attention", defines, progress=self._progress)
+            lib = load_library("kv8_attention" if dtype == torch.bfloat16 else "kv8_attention_f32", {"HEAD_DIM": dim}, progress=self._progress)
             lib.ifb_kv8_attention.argtypes = [c_char_p]
             lib.ifb_kv8_attention_scratch.restype = c_longlong
             lib.ifb_kv8_attention_scratch.argtypes = [c_int]
-            lib.scratch_floats = {nt: int(lib.ifb_kv8_attention_scratch(nt)) for nt in (1, 2)}
+            lib.scratch_floats = {nt: int(lib.ifb_kv8_attention_scratch(nt)) for nt in range(1, lib.ifb_kv8_attention_tiles() + 1)}
             for floats in lib.scratch_floats.values():
                 if floats < 0:
                     raise KernelError(f"kv8_attention: the device cannot be asked for its size (error {floats})")
