@@ -215,6 +215,8 @@ class LowBitKernels:
         index = w._index
         if code is None or out.get_device() != index or not out.is_contiguous() or index < 0:
             raise KernelError("mx4_linear: out is bfloat16 or float32, contiguous, and all is on the matrix's device")
+        if n == 0:
+            return out
         lib = self._mx4_lib()
         if isinstance(x, Mx4Matrix):
             if x.gated or x._index != index:

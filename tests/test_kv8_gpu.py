@@ -189,6 +189,43 @@ def test_requests_without_keys_or_queries_and_long_bounds(K, dtype):
     assert (out.double() - ref).abs().le(bound(ref, mag, reach, 128, 70, dtype)).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("requests", [40, 70, 150, 400])
+def test_many_requests(K, dtype, requests):
+    """More requests than a warp looks at once, than it keeps, and more items than CTAs run at a time; none, one and several pieces."""
+    g = torch.Generator().manual_seed(requests)
+    lens = torch.randint(0, 60, (requests,), generator=g).tolist()
+    lens[requests // 2] = 700
+    s = scene([1] * requests, lens, 2, 2, 64, 16, dtype, seed=requests)
+    ref, mag, reach = attention8(*s, 64 ** -0.5)
+    out = attend(K, *s, 0, min_q=1)
+    assert (out.double() - ref).abs().le(bound(ref, mag, reach, 64, 700, dtype)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_len", [1, 100])
+def test_pages_far_into_a_large_pool(K, dtype, q_len):
+    """Codes that begin beyond 2^31 and 2^32 bytes: the store, the values that are read back by attention, prompts and single tokens."""
+    from infurnace_b200.kernels import Kv8Pages
+    ps, heads, dim = 64, 8, 128                                        # 128 KB a page
+    n = (1 << 32) // (2 * heads * ps * dim) + 8
+    pages = Kv8Pages(torch.zeros((n, 2, heads, ps, dim), dtype=torch.int8, device="cuda"), torch.zeros((n, 2, heads), dtype=torch.uint8, device="cuda"))
+    ids = torch.tensor([n - 1, n // 2 + 3, n - 5])                      # of the keys 0 .. 149
+    k, v = tokens_of(150, heads, dim, 21, dtype)
+    pos = torch.arange(150)
+    slots = ids[pos // ps] * ps + pos % ps
+    K.kv8_store(k.cuda(), v.cuda(), slots.to(torch.int32).cuda(), pages)
+    small, fields = pages.codes[ids.cuda()].cpu(), pages.exponents[ids.cuda()].cpu()
+    ref_codes, ref_fields = store8(torch.zeros_like(small), torch.zeros_like(fields), k, v, pos)
+    assert torch.equal(fields.long(), ref_fields) and torch.equal(small.double(), ref_codes)
+    q = (torch.randn((q_len, heads * 2, dim), generator=torch.Generator().manual_seed(1)) * 0.6).to(dtype)
+    cu, lens = torch.tensor([0, q_len], dtype=torch.int32), torch.tensor([150], dtype=torch.int32)
+    out = torch.empty(q.shape, dtype=dtype, device="cuda")
+    K.kv8_attention(q.cuda(), pages, ids[None].to(torch.int32).cuda(), cu.cuda(), lens.cuda(), out, dim ** -0.5, 0, q_len, 150, min_q_len=q_len)
+    ref, mag, reach = attention8(q, small, fields, torch.tensor([[0, 1, 2]]), cu, lens, dim ** -0.5)
+    assert (out.cpu().double() - ref).abs().le(bound(ref, mag, reach, dim, 150, dtype)).all()
+
+
 def test_pages_that_a_window_has_passed_are_not_followed(K):
     q, codes, fields, tables, cu, lens = scene([1, 5], [800, 600], 2, 4, 128, 16, torch.bfloat16, seed=6)
     ref, mag, reach = attention8(q, codes, fields, tables, cu, lens, 128 ** -0.5, 50)

@@ -65,6 +65,25 @@ def test_infinities_nan_and_the_ends_of_the_range(K, dtype):
     assert same(K.mx4_values(m, out).cpu().double(), value)
 
 
+@pytest.mark.parametrize("rows,k", [(70001, 64), (262147, 32), (20001, 2080)])
+def test_more_rows_than_a_grid_has(K, rows, k):
+    """Rows in several launches, and rows four to a thread."""
+    from infurnace_b200.kernels import Mx4Matrix
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn((rows, k), generator=g, device="cuda").to(torch.bfloat16)
+    m = K.mx4_quantize(x, Mx4Matrix.empty(rows, k))
+    out = torch.empty_like(x)
+    K.mx4_values(m, out)
+    for at in (0, 65270, 130540, rows - 300):
+        if at < rows:
+            part = x[at:at + 300]
+            assert torch.equal(out[at:at + 300].double().cpu(), round4(part.cpu())[2])
+
+
+def test_no_rows(K):
+    assert K.mx4_linear(torch.empty((0, 64), device="cuda"), K.mx4_matrix(torch.ones((5, 64), device="cuda")), torch.empty((0, 5), device="cuda")).shape == (0, 5)
+
+
 def test_rows_that_lie_apart_and_gated_rows(K):
     from infurnace_b200.kernels import Mx4Matrix
     wide = rows_of(10, 256, 1, torch.bfloat16).cuda()
