@@ -79,11 +79,13 @@ template <> struct MxSixteen<float> {
 // Two neighbouring lanes have a block: 16 elements (32 or 64 bytes of input, 8 of output) each.  8 lanes have the four blocks whose
 // scales lie in one 32-bit word.  The columns of a row are spread over the grid's x; a thread has PER rows, all of them requested
 // at once (a large matrix: one row per thread is a load's latency per CTA of little work).
+// early: the result is the rows of the product that follows, which reads them behind its wait.  What may become a product's matrix is read
+// before that wait, so then the next kernel may not begin while this one writes: no trigger, and the writes are performed first.
 template <typename T, int PER>
 __global__ void __launch_bounds__(256)
-mx4_quantize_kernel(const T* x, long long row_stride, uint8_t* codes, uint8_t* scales, int rows, int k, int gated_rows) {
+mx4_quantize_kernel(const T* x, long long row_stride, uint8_t* codes, uint8_t* scales, int rows, int k, int gated_rows, int early) {
   ifb_pdl_wait();
-  ifb_pdl_trigger();
+  if (early) ifb_pdl_trigger();
   const int k_tiles = (k + 127) / 128;
   const int e = (blockIdx.x * 256 + threadIdx.x) * 16;                 // of the row's elements, padded to 128
   const uint32_t lanes = __ballot_sync(0xffffffffu, e < k_tiles * 128);
@@ -115,6 +117,7 @@ mx4_quantize_kernel(const T* x, long long row_stride, uint8_t* codes, uint8_t* s
     }
     if ((threadIdx.x & 7) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(row, e / MX_BLOCK, k_tiles)) = word;
   }
+  if (!early) __threadfence();
 }
 
 // The values of eight codes in pairs of bfloat16, which holds them exactly.  The bits "ee m" of a code at the lowest end of a bfloat16's
@@ -140,11 +143,11 @@ template <> __device__ __forceinline__ void mx_store8<float>(float* p, const uin
   for (int i = 0; i < 2; ++i)
     reinterpret_cast<uint4*>(p)[i] = make_uint4(v[2 * i] << 16, v[2 * i] & 0xffff0000u, v[2 * i + 1] << 16, v[2 * i + 1] & 0xffff0000u);
 }
+// (No trigger, and a fence at the end, for the same reason: the numbers may be the matrix of another product.)
 template <typename T, int PER>
 __global__ void __launch_bounds__(256)
 mx4_values_kernel(const uint8_t* codes, const uint8_t* scales, T* out, int rows, int k, int gated_rows) {
   ifb_pdl_wait();
-  ifb_pdl_trigger();
   const int e = (blockIdx.x * 256 + threadIdx.x) * 8;
   if (e >= k) return;
   const int row0 = blockIdx.y * PER, k_tiles = (k + 127) / 128;
@@ -165,6 +168,7 @@ mx4_values_kernel(const uint8_t* codes, const uint8_t* scales, T* out, int rows,
     mx_values8(c[p], s[p], v);
     mx_store8<T>(out + (size_t)to * k + e, v);
   }
+  __threadfence();
 }
 
 static int mx_sizes(int rows, int k, int gated) {
@@ -172,12 +176,12 @@ static int mx_sizes(int rows, int k, int gated) {
   return IFB_OK;
 }
 
-// Rows per thread: four where that still gives every SM several CTAs.
-static int mx_rows_per_thread(int rows, int k) { return (long long)rows * k >= (long long)ifb_sm_count() * 65536 ? 4 : 1; }
 constexpr int MX_GRID_ROWS = 65535 / 256 * 256;      // a grid has at most 65,535 rows; whole tiles of rows, whole pairs
+// Rows per thread: four where that still gives every SM several CTAs, or where a grid would not have the rows.
+static int mx_rows_per_thread(int rows, int k) { return (long long)rows * k >= (long long)ifb_sm_count() * 65536 || rows > MX_GRID_ROWS ? 4 : 1; }
 
 template <typename T, int PER>
-static int mx_quantize_launch(const void* x, long long row_stride, void* codes, void* scales, int rows, int k, int gated, cudaStream_t stream) {
+static int mx_quantize_launch(const void* x, long long row_stride, void* codes, void* scales, int rows, int k, int gated, int early, cudaStream_t stream) {
   // (a gated matrix has its rows from two places, so one launch has to hold it)
   if (gated && (rows + PER - 1) / PER > MX_GRID_ROWS) return IFB_ERR_SIZE;
   for (long long r0 = 0; r0 < rows; r0 += (long long)MX_GRID_ROWS * PER) {
@@ -185,13 +189,12 @@ static int mx_quantize_launch(const void* x, long long row_stride, void* codes, 
     const dim3 grid(((k + 127) / 128 * 8 + 255) / 256, (n + PER - 1) / PER);
     const int e = ifb_launch(mx4_quantize_kernel<T, PER>, grid, dim3(256), 0, stream, (const T*)x + (size_t)r0 * row_stride, row_stride,
                              (uint8_t*)codes + (size_t)r0 * (k / 2), (uint8_t*)scales + (size_t)(r0 / 128) * ((k + 127) / 128) * 512, n, k,
-                             gated ? rows / 2 : 0);
+                             gated ? rows / 2 : 0, early);
     if (e) return e;
   }
   return IFB_OK;
 }
-IFB_EXPORT int ifb_mx4_quantize(const void* x, int dtype, long long row_stride, void* codes, void* scales, int rows, int k, int gated,
-                                void* stream) {
+static int mx_quantize(const void* x, int dtype, long long row_stride, void* codes, void* scales, int rows, int k, int gated, int early, void* stream) {
   const int bad = mx_sizes(rows, k, gated);
   if (bad) return bad;
   const int esize = dtype == IFB_F32 ? 4 : 2;
@@ -199,10 +202,14 @@ IFB_EXPORT int ifb_mx4_quantize(const void* x, int dtype, long long row_stride, 
   if ((((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)scales) | (uintptr_t)(row_stride * esize)) & 15) return IFB_ERR_ALIGN;
   cudaStream_t st = (cudaStream_t)stream;
   if (mx_rows_per_thread(rows, k) == 4)
-    return dtype == IFB_F32 ? mx_quantize_launch<float, 4>(x, row_stride, codes, scales, rows, k, gated, st)
-                            : mx_quantize_launch<bf16, 4>(x, row_stride, codes, scales, rows, k, gated, st);
-  return dtype == IFB_F32 ? mx_quantize_launch<float, 1>(x, row_stride, codes, scales, rows, k, gated, st)
-                          : mx_quantize_launch<bf16, 1>(x, row_stride, codes, scales, rows, k, gated, st);
+    return dtype == IFB_F32 ? mx_quantize_launch<float, 4>(x, row_stride, codes, scales, rows, k, gated, early, st)
+                            : mx_quantize_launch<bf16, 4>(x, row_stride, codes, scales, rows, k, gated, early, st);
+  return dtype == IFB_F32 ? mx_quantize_launch<float, 1>(x, row_stride, codes, scales, rows, k, gated, early, st)
+                          : mx_quantize_launch<bf16, 1>(x, row_stride, codes, scales, rows, k, gated, early, st);
+}
+IFB_EXPORT int ifb_mx4_quantize(const void* x, int dtype, long long row_stride, void* codes, void* scales, int rows, int k, int gated,
+                                void* stream) {
+  return mx_quantize(x, dtype, row_stride, codes, scales, rows, k, gated, 0, stream);
 }
 
 template <typename T, int PER>
@@ -957,7 +964,7 @@ IFB_EXPORT int ifb_mx4_linear(const void* x, int x_dtype, long long x_row, void*
   if (round && ((((uintptr_t)x) | (uintptr_t)(x_row * (x_dtype == IFB_F32 ? 4 : 2))) & 15)) return IFB_ERR_ALIGN;
   if (!round && (!x_codes || !x_scales)) return IFB_ERR_ARG;
   if (!round && x_dtype != -1) {
-    bad = ifb_mx4_quantize(x, x_dtype, x_row, x_codes, x_scales, rows, k, 0, stream);
+    bad = mx_quantize(x, x_dtype, x_row, x_codes, x_scales, rows, k, 0, 1, stream);
     if (bad) return bad;
   }
   // Pairs of SMs (tiles of 256 x 256) from the second round of tiles of 128 x 128 on, where their rounds are fewer; theirs is 1.3 times as long.

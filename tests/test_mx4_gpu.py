@@ -84,6 +84,31 @@ def test_no_rows(K):
     assert K.mx4_linear(torch.empty((0, 64), device="cuda"), K.mx4_matrix(torch.ones((5, 64), device="cuda")), torch.empty((0, 5), device="cuda")).shape == (0, 5)
 
 
+def test_a_matrix_is_written_before_the_next_call_reads_it(K):
+    """A product may ask for its matrix before the kernel ahead of it ends: not one that writes the matrix, be it with bits or as numbers."""
+    from infurnace_b200.kernels import Mx4Matrix
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn((4, 2048), generator=g, device="cuda").to(torch.bfloat16)
+    ws = [torch.randn((20000, 2048), generator=g, device="cuda").to(torch.bfloat16) * 2 ** i for i in range(3)]
+    shared, numbers = Mx4Matrix.empty(20000, 2048), torch.empty((20000, 2048), dtype=torch.bfloat16, device="cuda")
+    want = []
+    for w in ws:
+        m = K.mx4_matrix(w)
+        K.mx4_values(m, numbers)
+        torch.cuda.synchronize()
+        want.append((torch.empty((4, 20000), device="cuda"), torch.empty((4, 20000), dtype=torch.bfloat16, device="cuda")))
+        K.mx4_linear(x, m, want[-1][0])
+        K.linear(x, numbers, want[-1][1])
+    torch.cuda.synchronize()
+    for i in range(12):
+        K.mx4_quantize(ws[i % 3], shared)
+        a, b = torch.empty((4, 20000), device="cuda"), torch.empty((4, 20000), dtype=torch.bfloat16, device="cuda")
+        K.mx4_linear(x, shared, a)
+        K.mx4_values(shared, numbers)
+        K.linear(x, numbers, b)
+        assert torch.equal(a, want[i % 3][0]) and torch.equal(b, want[i % 3][1])
+
+
 def test_rows_that_lie_apart_and_gated_rows(K):
     from infurnace_b200.kernels import Mx4Matrix
     wide = rows_of(10, 256, 1, torch.bfloat16).cuda()
