@@ -443,7 +443,7 @@ template <typename S1, typename S2> static long long kv8_scratch(int nt) {
 }
 
 template <typename S>
-static int kv8_launch(const Kv8Args& a, bool whole, int max_q, cudaStream_t stream) {
+static int kv8_launch(const Kv8Args& a, bool whole, int max_q, long long items, cudaStream_t stream) {
   if (whole) {
     const int rows = max_q * (a.heads / a.kv_heads);
     const dim3 grid((rows + 8 * S::ROW_TILES * WARPS - 1) / (8 * S::ROW_TILES * WARPS), a.kv_heads, a.requests);
@@ -453,14 +453,14 @@ static int kv8_launch(const Kv8Args& a, bool whole, int max_q, cudaStream_t stre
   const int bad = kv8_split_ctas<S>(&ctas);
   if (bad) return bad;
   // (with more items than CTAs at a time each is one piece, and needs no scratch memory)
-  const long long items = (long long)a.requests * a.tiles * a.kv_heads;
   if (items > 0x7fffffffLL) return IFB_ERR_SIZE;
   Kv8Args b = a;
   b.most = ctas;
   return ifb_launch(kv8_attention_split_kernel<S>, dim3(items > ctas ? (unsigned)items : (unsigned)ctas), dim3(32 * WARPS), kv8_split_smem<S>(), stream, b);
 }
 
-// nt: tiles of 8 score rows per warp.  whole: the whole form.  Requests of min_rows .. max_rows score rows are worked on.
+// nt: tiles of 8 score rows per warp.  whole: the whole form.  Requests of min_rows .. max_rows score rows are worked on.  Split form:
+// `tiles` tiles of a request at most, `items` (tiles x key heads) of all requests.
 // One argument, since a call's price on the host is that of its arguments.
 struct Kv8Call {
   const void* q;
@@ -469,7 +469,7 @@ struct Kv8Call {
   long long table_stride;
   const void *cu_q, *seq_lens;
   void *out, *parts, *counters;
-  long long requests, heads, kv_heads, page_size, dim, window, max_q, min_rows, max_rows, tiles, nt, whole;
+  long long requests, heads, kv_heads, page_size, dim, window, max_q, min_rows, max_rows, tiles, nt, whole, items;
   void* stream;
   double scale;
 };
@@ -487,7 +487,7 @@ template <typename S1, typename S2> static int kv8_call(const Kv8Call* c) {
                      (int)c->kv_heads, (int)c->page_size, (int)c->window, (float)c->scale * 1.4426950408889634f, (int)c->min_rows, (int)c->max_rows,
                      (int)c->tiles, 0};
   cudaStream_t stream = (cudaStream_t)c->stream;
-  return c->nt == 1 ? kv8_launch<S1>(a, whole, (int)c->max_q, stream) : kv8_launch<S2>(a, whole, (int)c->max_q, stream);
+  return c->nt == 1 ? kv8_launch<S1>(a, whole, (int)c->max_q, c->items, stream) : kv8_launch<S2>(a, whole, (int)c->max_q, c->items, stream);
 }
 
 // The library's calls over the file's streams of one and of TILES row tiles.

@@ -20,7 +20,7 @@ if _raw_stream is None:                       # an older torch: the public, slow
     def _raw_stream(device_index):
         return torch.cuda.current_stream(device_index).cuda_stream
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
-_KV8_CALL = struct.Struct("=25qd").pack       # csrc/kv8_attention.cu: Kv8Call
+_KV8_CALL = struct.Struct("=26qd").pack       # csrc/kv8_attention.cuh: Kv8Call
 
 MX4_BLOCK = 32         # elements of a row that share a scale
 _CODES = {torch.float32: 0, torch.bfloat16: 1}
@@ -207,6 +207,8 @@ class LowBitKernels:
         epi = self._epilogues.get(epilogue)
         if epi is None:
             raise KernelError(f"mx4_linear: unknown epilogue {epilogue!r}; known: {', '.join(self._epilogues)}")
+        if len(x.shape) != 2:
+            raise KernelError(f"mx4_linear: x is [n, k]; got {tuple(x.shape)}")
         n, k = x.shape
         code = _CODES.get(out.dtype)
         if k != w.k or (epi & 1 != 0) != w.gated or out.shape != (n, w.rows >> (epi & 1)):
@@ -260,7 +262,7 @@ class LowBitKernels:
         code = _CODES.get(k.dtype)
         heads, dim, index = pages.kv_heads, pages.head_dim, pages._index
         shape, pitch, v_pitch = k.shape, k.stride(), v.stride()
-        n = shape[0]
+        n = shape[0] if len(shape) == 3 else -1
         if code is None or v.dtype != k.dtype or shape != (n, heads, dim) or v.shape != shape:
             raise KernelError(f"kv8_store: k and v are bfloat16 or float32 [tokens, {heads}, {dim}]; got {k.dtype} {tuple(k.shape)} and "
                               f"{v.dtype} {tuple(v.shape)}")
@@ -309,7 +311,7 @@ class LowBitKernels:
     def _kv8_scratch(self, stream, floats, counters):
         """Addresses of (sums, counters) of the split form: of a stream each, and one pair for recorded graphs, whose replays follow
         one another.  The counters are zero between launches; a recording could not clear new ones, so what it uses is made
-        before, with the first call outside of one."""
+        before, with the first call outside of one; what an older recording uses is kept when room grows."""
         held = self.__dict__.setdefault("_kv8_held", {})
         capturing = _capturing()
         for key in (("graph",) if capturing else (stream, "graph")):
@@ -322,12 +324,24 @@ class LowBitKernels:
                 zeros = torch.zeros(counters_, dtype=torch.int32, device="cuda")
                 held[key] = (floats_, counters_, sums.data_ptr(), zeros.data_ptr(), sums, zeros)
                 if key == "graph":
+                    self.__dict__.setdefault("_kv8_recorded", []).append(have)
                     torch.cuda.current_stream().synchronize()            # cleared before a graph on another stream can use them
                     self.scratch_generation += 1
         return held["graph" if capturing else stream][2:4]
 
-    kv8_expand_rows = 64             # score rows of the longest request from which prompts' pages are expanded for the tcgen05 kernel
     kv8_expand_bytes = 4 << 30       # room for expanded pages that a call may take
+    # Which form attends to requests of more than 16 score rows (queries x query heads of a key head) in bfloat16.  The split form's time
+    # grows with the rows, 3.7 ns for 1,000 keys and row in all (heads of 128).  The tcgen05 kernel has a tile of 128 rows per SM: 10.7 ns
+    # for a key and round of tiles, and the pages' expansion, 0.12 ns for a key and key head.  So up to 24 rows of an SM in
+    # every round of tiles, and 32 of every request's key head, the split form is the shorter.  Measured, split and tcgen05, 32 query and
+    # 8 key heads of 128: a request of 16 queries over 5,000 and 16,000 keys 22 and 60, 38 and 172 us; of 64 queries 45 and 61, 114 and 174; of
+    # 128 queries 72 and 62, 211 and 175; 16 requests of 8 and of 32 queries over 1,200 keys 24 and 43, 76 and 44 us.
+    kv8_split_rows = (24, 32)
+    # Where that kernel does not fit (float32, heads wider than 128, other pages) all requests run split, but those of more than 64 rows
+    # whole where the device has plenty of rows and the keys are few, so that an item's beginning and end count.  Measured, split and whole,
+    # float32, 8 key heads of 128: 8 requests of 64 queries over 300 keys 53 and 38 us, of 1,024 over 1,200 keys 1,210 and 1,032, of 256 over
+    # 5,000 keys 1,512 and 1,826; one of 64 over 300 keys 16 and 30.
+    kv8_whole_rows, kv8_whole_keys = 64, 2048      # rows of an SM from which, keys up to which
 
     def _kv8_attention_tc(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r, heads, kv_heads, group, most, room):
         """The requests with more than 16 score rows: their pages as bfloat16 (exact), and the tcgen05 kernel over those."""
@@ -353,7 +367,7 @@ class LowBitKernels:
         theirs, which bounds how many are long."""
         code = _CODES.get(q.dtype)
         shape, pitch, index = q.shape, q.stride(), pages._index
-        n, heads, dim = shape
+        n, heads, dim = shape if len(shape) == 3 else (0, 0, 0)
         kv_heads = pages.kv_heads
         if code is None or out.dtype != q.dtype or out.shape != shape or dim != pages.head_dim or heads % kv_heads:
             raise KernelError(f"kv8_attention: q and out are bfloat16 or float32 [tokens, a multiple of {kv_heads}, {pages.head_dim}]; got "
@@ -375,32 +389,38 @@ class LowBitKernels:
         if window < 0 or max_q_len < 1 or not 1 <= min_q_len <= max_q_len:
             raise KernelError("kv8_attention: window is not negative, and 1 <= min_q_len <= max_q_len")
         lib, stream, group = self._kv8_attention_lib(dim, q.dtype), _raw_stream(index), heads // kv_heads
-        # score rows beyond which a request's tiles fill the device by themselves and run whole; requests below run split
         rows, least = max_q_len * group, min_q_len * group
-        limit = 64
-        if rows > self.kv8_expand_rows and q.dtype == torch.bfloat16 and dim <= 128 and group <= 128 and pages.page_size in (16, 32, 64) \
-                and self.attention_tc:
-            # (a long request has more than 16 score rows)
-            most = -(-max_seq_len // pages.page_size)
-            room = most * (self.long_requests(n, r, group, max_q_len, min_q_len) if exact_lens else min(r, n // (16 // group + 1)))
-            if room * pages.page_size * kv_heads * dim * 4 <= self.kv8_expand_bytes:
-                self._kv8_attention_tc(q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r, heads, kv_heads, group, most, room)
-                if least > 16:
-                    return out
-                limit = rows = 16
-        nt = 1 if rows <= 8 or dim > 128 or limit == 16 and group <= 8 else 2      # (beside prompts the short requests decode)
+        tc = False
+        if rows > 16 and q.dtype == torch.bfloat16 and dim <= 128 and group <= 128 and pages.page_size in (16, 32, 64) and self.attention_tc:
+            per_round, per_head = self.kv8_split_rows
+            long = min(r, -(-n // max_q_len)) * kv_heads
+            rounds = -(-long * -(-max_q_len // (128 // group)) // self.sm_count)
+            if n * heads > per_round * self.sm_count * rounds + per_head * long:
+                # (a long request has more than 16 score rows)
+                most = -(-max_seq_len // pages.page_size)
+                room = most * (self.long_requests(n, r, group, max_q_len, min_q_len) if exact_lens else min(r, n // (16 // group + 1)))
+                tc = room * pages.page_size * kv_heads * dim * 4 <= self.kv8_expand_bytes
+        if tc:
+            self._kv8_attention_tc(q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r, heads, kv_heads, group, most, room)
+            if least > 16:
+                return out
+            rows = 16
+        # score rows up to which a request runs split
+        limit = min(rows, 64) if n * heads > self.kv8_whole_rows * self.sm_count and max_seq_len <= self.kv8_whole_keys else rows
+        nt = 1 if rows <= 8 or dim > 128 or tc and group <= 8 else 2      # (beside prompts the short requests decode)
         fixed = (q.data_ptr(), code, pitch[0], *pages._at, block_tables.data_ptr(), table_pitch[0], cu_q.data_ptr(), seq_lens.data_ptr(),
                  out.data_ptr())
         sizes = (r, heads, kv_heads, pages.page_size, dim, window, max_q_len)
         status = 0
         if least <= limit:
-            tiles = -(-min(rows, limit) // (8 * nt))
+            tiles = -(-limit // (8 * nt))
+            items = min(r * tiles, r + n * group // (8 * nt)) * kv_heads
             self.launches += 1
             status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, *self._kv8_scratch(stream, lib.scratch_floats[nt], r * tiles * kv_heads), *sizes, 0, limit,
-                                                     tiles, nt, 0, stream, scale))
+                                                     tiles, nt, 0, items, stream, scale))
         if rows > limit and not status:
             self.launches += 1
-            status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, 0, 0, *sizes, limit + 1, (1 << 31) - 1, 1, nt, 1, stream, scale))
+            status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, 0, 0, *sizes, limit + 1, (1 << 31) - 1, 1, nt, 1, 0, stream, scale))
         if status:
             self._low_bit_status(status, "kv8_attention")
         return out

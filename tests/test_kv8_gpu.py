@@ -179,6 +179,25 @@ def test_attention(K, dtype, q_lens, seq_lens, heads, group, dim, ps, window):
     assert torch.equal(out, attend(K, *s, window))                      # the same bits every time
 
 
+@pytest.mark.parametrize("form,dtype", [("tiles", torch.bfloat16), ("whole", torch.bfloat16), ("whole", torch.float32), ("split", torch.bfloat16), ("split", torch.float32)])
+@pytest.mark.parametrize("q_lens,seq_lens,heads,group,dim,ps,window", [s for s in SCENES if max(s[0]) * s[3] > 16] + [([700, 3], [700, 1100], 2, 4, 64, 64, 0)])
+def test_every_form_of_attention(K, monkeypatch, form, dtype, q_lens, seq_lens, heads, group, dim, ps, window):
+    """The three forms give way to one another by how much work there is; each is right for all of it, blocks of NaN included."""
+    monkeypatch.setattr(K, "kv8_split_rows", (0, 0) if form == "tiles" else (1 << 20, 0))
+    monkeypatch.setattr(K, "kv8_whole_rows", 0 if form == "whole" else 1 << 20)
+    s = scene(q_lens, seq_lens, heads, group, dim, ps, dtype, seed=len(q_lens) + dim + window)
+    ref, mag, reach = attention8(*s, dim ** -0.5, window)
+    out = attend(K, *s, window)
+    assert (out.double() - ref).abs().le(bound(ref, mag, reach, dim, max(seq_lens), dtype)).all()
+    q, codes, fields, tables, cu, lens = s
+    fields[tables[0, (seq_lens[0] - 1) // ps], 1, 0] = 255               # the last page of the first request, its first key head
+    bad = attend(K, *s, window)
+    for t in range(q.shape[0]):
+        sees = t < q_lens[0] and seq_lens[0] - q_lens[0] + t >= (seq_lens[0] - 1) // ps * ps
+        assert bad[t, :group].isnan().all() if sees else torch.equal(bad[t, :group], out[t, :group])
+        assert torch.equal(bad[t, group:], out[t, group:])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_requests_without_keys_or_queries_and_long_bounds(K, dtype):
     """A padded row (length 0) is zero, a request that brings nothing is passed over, the caller's bounds may exceed the lengths."""
@@ -301,6 +320,24 @@ def test_strided_queries_another_stream_and_a_graph(K):
     assert all(torch.equal(o.cpu(), plain) for o in outs)
 
 
+def test_a_recording_outlives_larger_calls(K):
+    """A graph recorded before a call that needs more room gives its bits afterwards."""
+    s = scene([1, 1], [700, 300], 2, 4, 128, 16, torch.bfloat16, seed=12)
+    q, codes, fields, tables, cu, lens = s
+    plain = attend(K, *s, 0)
+    pages, out, held = on_device(codes, fields), torch.zeros(q.shape, dtype=q.dtype, device="cuda"), [t.cuda() for t in (q, tables, cu, lens)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        K.kv8_attention(held[0], pages, *held[1:], out, 128 ** -0.5, 0, 1, 700)
+    many = 3000
+    big = scene([1] * many, [33] * many, 2, 4, 128, 16, torch.bfloat16, seed=13)
+    attend(K, *big, 0)
+    junk = [torch.full((1 << 18,), 7, dtype=torch.int32, device="cuda") for _ in range(64)]      # over whatever was freed
+    g.replay()
+    torch.cuda.synchronize()
+    assert len(junk) == 64 and torch.equal(out.cpu(), plain)
+
+
 def test_refusals(K):
     from infurnace_b200.errors import KernelError
     from infurnace_b200.kernels import Kv8Pages
@@ -318,6 +355,7 @@ def test_refusals(K):
                  lambda: K.kv8_values(pages, torch.empty((1, 2), device="cuda")), lambda: K.kv8_values(pages, codes),
                  lambda: go(q=q.half()), lambda: go(q=q.float()), lambda: go(q=q[:, :3], out=out[:, :3].contiguous()), lambda: go(out=out[:1]),
                  lambda: go(t=tables.long()), lambda: go(cu=cu[:1]), lambda: go(ml=200), lambda: go(w=-1), lambda: go(nq=3), lambda: go(mq=0),
-                 lambda: go(sl=lens.cpu()), lambda: go(t=tables[:0])):
+                 lambda: go(sl=lens.cpu()), lambda: go(t=tables[:0]), lambda: go(q=q[0], out=out[0]), lambda: go(q=q[:, 0], out=out[:, 0].contiguous()),
+                 lambda: K.kv8_store(k[0], k[0], slots[:1], pages), lambda: K.kv8_store(k[:, :, :, None], k[:, :, :, None], slots, pages)):
         with pytest.raises(KernelError):
             call()

@@ -266,6 +266,7 @@ def test_refusals(K):
                  lambda: K.mx4_values(m, out), lambda: K.mx4_matrix(w[:5], gated=True), lambda: K.mx4_matrix(w[:, :40]),
                  lambda: K.mx4_linear(x, m, out, epilogue="swish"), lambda: K.mx4_linear(x, m, out, epilogue="silu_gate"),
                  lambda: K.mx4_linear(x, g, out), lambda: K.mx4_linear(x[:, :32], m, out), lambda: K.mx4_linear(x, m, out[:3]),
-                 lambda: K.mx4_linear(x, m, out.half()), lambda: K.mx4_linear(x, m, out.cpu()), lambda: K.mx4_linear(g, m, out)):
+                 lambda: K.mx4_linear(x, m, out.half()), lambda: K.mx4_linear(x, m, out.cpu()), lambda: K.mx4_linear(g, m, out),
+                 lambda: K.mx4_linear(x[0], m, out), lambda: K.mx4_quantize(x[0], m)):
         with pytest.raises(KernelError):
             call()
