@@ -343,19 +343,17 @@ class LowBitKernels:
     # 5,000 keys 1,512 and 1,826; one of 64 over 300 keys 16 and 30.
     kv8_whole_rows, kv8_whole_keys = 64, 2048      # rows of an SM from which, keys up to which
 
-    def _kv8_attention_tc(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r, heads, kv_heads, group, most, room):
-        """The requests with more than 16 score rows: their pages as bfloat16 (exact), and the tcgen05 kernel over those."""
-        device, ps, dim = q.device, pages.page_size, pages.head_dim
-        wide = torch.empty((room, 2, kv_heads, ps, dim), dtype=torch.bfloat16, device=device)
-        tables = torch.empty((r, most), dtype=torch.int32, device=device)
+    def _kv8_expand(self, pages, block_tables, cu_q, seq_lens, window, r, group, most, room, stream):
+        """The pages of the requests with more than 16 score rows as bfloat16 (exact), and tables of them."""
+        kv_heads, ps, dim = pages.kv_heads, pages.page_size, pages.head_dim
+        wide = torch.empty((room, 2, kv_heads, ps, dim), dtype=torch.bfloat16, device=pages.codes.device)
+        tables = torch.empty((r, most), dtype=torch.int32, device=pages.codes.device)
         self.launches += 1
-        self._low_bit_status(self._kv8_lib().ifb_kv8_expand(*pages._at, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
-                                                            seq_lens.data_ptr(), wide.data_ptr(), tables.data_ptr(), room, r, most, kv_heads, group,
-                                                            ps, dim, int(window), 16, self._stream()), "kv8_attention")
-        at, stride = wide.data_ptr(), wide.stride(0)
-        self._attention_tc_streams(q.view(n, heads * dim) if q.is_contiguous() else q.as_strided((n, heads * dim), (q.stride(0), 1)),
-                                   heads, kv_heads, 1, dim, dim, (at, stride, ps), (at + 2 * kv_heads * ps * dim, stride, ps), room, tables, cu_q,
-                                   seq_lens, out, scale, int(window), max_q_len, n, r, 2, None, None, kind=0)
+        status = self._kv8_lib().ifb_kv8_expand(*pages._at, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(), seq_lens.data_ptr(),
+                                                wide.data_ptr(), tables.data_ptr(), room, r, most, kv_heads, group, ps, dim, window, 16, stream)
+        if status:
+            self._low_bit_status(status, "kv8_attention")
+        return wide, tables
 
     def kv8_attention(self, q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, max_seq_len, min_q_len=1,
                       exact_lens=False):
@@ -401,9 +399,7 @@ class LowBitKernels:
                 room = most * (self.long_requests(n, r, group, max_q_len, min_q_len) if exact_lens else min(r, n // (16 // group + 1)))
                 tc = room * pages.page_size * kv_heads * dim * 4 <= self.kv8_expand_bytes
         if tc:
-            self._kv8_attention_tc(q, pages, block_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r, heads, kv_heads, group, most, room)
-            if least > 16:
-                return out
+            wide, wide_tables = self._kv8_expand(pages, block_tables, cu_q, seq_lens, window, r, group, most, room, stream)
             rows = 16
         # score rows up to which a request runs split
         limit = min(rows, 64) if n * heads > self.kv8_whole_rows * self.sm_count and max_seq_len <= self.kv8_whole_keys else rows
@@ -423,4 +419,9 @@ class LowBitKernels:
             status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, 0, 0, *sizes, limit + 1, (1 << 31) - 1, 1, nt, 1, 0, stream, scale))
         if status:
             self._low_bit_status(status, "kv8_attention")
+        if tc:
+            at, step, block = wide.data_ptr(), wide.stride(0), 2 * kv_heads * pages.page_size * dim
+            self._attention_tc_streams(q.as_strided((n, heads * dim), (pitch[0], 1)), heads, kv_heads, 1, dim, dim, (at, step, pages.page_size),
+                                       (at + block, step, pages.page_size), room, wide_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r,
+                                       2, None, None, kind=0)
         return out
