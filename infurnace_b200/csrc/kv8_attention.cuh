@@ -228,26 +228,27 @@ kv8_attention_whole_kernel(Kv8Args a) {
 // less, for which the pieces of all items are no more than `most`; else every item is one piece.  (Equal shares of the units, with
 // CTAs that have the end of one item and the beginning of the next, are a tenth shorter and cost a second start and a second join.)
 // --------------------------------------------------------------------------------------------
-constexpr int MAX_PARTS = 32;            // pieces of an item
+constexpr int MAX_PARTS = 64;            // pieces of an item
 constexpr int PITCH = D + 8;             // of a row of sums in shared memory (the rows of a quad of lanes fall on two halves of the banks)
 // Where a warp's sums lie in a row: m tile by m tile, the lanes' pairs side by side.
 __device__ __forceinline__ int kv8_place(int i, int lane) { return i * 16 + (lane >> 2) * 2; }
 __device__ __forceinline__ int kv8_place_dim(int place) { return value_dim<D>(place >> 4, ((place & 15) >> 1) << 2, 0); }
 
-// What a lane knows of request r0 + lane: where its queries lie, the units of an item and its items.
+// What a lane knows of a request: where its queries lie, the units of an item and its items (0: not this kernel's).
 struct Kv8Look { int q0, q_len, L, units, items; };
+__device__ __forceinline__ Kv8Look kv8_ask(const Kv8Args& a, int r) {       // (the last request's numbers beyond it)
+  const int at = min(r, a.requests - 1);
+  Kv8Look k = {a.cu_q[at], a.cu_q[at + 1], a.seq_lens[at], 0, 0};
+  return k;
+}
 template <int ROWS, int UNIT>
-__device__ __forceinline__ Kv8Look kv8_look(const Kv8Args& a, int G, int r0, int lane) {
-  Kv8Look k = {};
-  const int r = r0 + lane;
-  if (r < a.requests) {
-    k.q0 = a.cu_q[r]; k.q_len = a.cu_q[r + 1] - k.q0; k.L = a.seq_lens[r];
-    const int rows = k.q_len * G;
-    if (k.q_len > 0 && rows >= a.min_rows && rows <= a.max_rows) {
-      k.items = (rows + ROWS - 1) / ROWS * a.kv_heads;
-      const int lo = a.window > 0 ? max(0, k.L - k.q_len - a.window + 1) : 0;
-      k.units = k.L > 0 ? max(1, (k.L - 1) / UNIT - lo / UNIT + 1) : 1;
-    }
+__device__ __forceinline__ Kv8Look kv8_look(const Kv8Args& a, int G, int r, Kv8Look k) {
+  k.q_len -= k.q0;
+  const int rows = k.q_len * G;
+  if (r < a.requests && k.q_len > 0 && rows >= a.min_rows && rows <= a.max_rows) {
+    k.items = (rows + ROWS - 1) / ROWS * a.kv_heads;
+    const int lo = a.window > 0 ? max(0, k.L - k.q_len - a.window + 1) : 0;
+    k.units = k.L > 0 ? max(1, (k.L - 1) / UNIT - lo / UNIT + 1) : 1;
   }
   return k;
 }
@@ -256,24 +257,15 @@ __device__ __forceinline__ Kv8Look kv8_look(const Kv8Args& a, int G, int r0, int
 // is taken off.
 __device__ __forceinline__ int kv8_parts(int x, float inverse) { return (int)(((float)x - 0.5f) * inverse) + 1; }
 
-template <typename S>
-__global__ void __launch_bounds__(32 * WARPS, S::CTAS)
-kv8_attention_split_kernel(Kv8Args a) {
-  constexpr int NT = S::ROW_TILES, ROWS = 8 * NT, TILE = S::TILE, UNIT = TILE * WARPS;
-  extern __shared__ __align__(16) float sums[];                         // [WARPS][ROWS][PITCH], then maxima and sums [WARPS][ROWS] each
-  __shared__ float part_m[MAX_PARTS][ROWS], part_l[MAX_PARTS][ROWS];
-  __shared__ int arrived;
-  ifb_pdl_wait();
-  ifb_pdl_trigger();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads;
-  float* const sm_m = sums + WARPS * ROWS * PITCH;
-  float* const sm_l = sm_m + WARPS * ROWS;
-  // every warp for itself: how long pieces are, and whose piece this CTA's is
-  const Kv8Look known = kv8_look<ROWS, UNIT>(a, G, 0, lane), known2 = a.requests > 32 ? kv8_look<ROWS, UNIT>(a, G, 32, lane) : Kv8Look{};
-  auto look = [&](int r0) { return r0 == 0 ? known : r0 == 32 ? known2 : kv8_look<ROWS, UNIT>(a, G, r0, lane); };
-  int total = 0, items = 0, longest = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += 32) {
-    const Kv8Look k = look(r0);
+// How long pieces are, and whose piece this CTA's is: request r (-1: there are more CTAs than pieces), number `at` of its items' pieces.
+struct Kv8Plan { int r, at, units, pieces, q0, q_len, L; };
+template <int ROWS, int UNIT>
+__device__ __forceinline__ Kv8Plan kv8_plan(const Kv8Args& a, int G, int lane) {
+  const Kv8Look asked = kv8_ask(a, lane), asked2 = kv8_ask(a, lane + 32);
+  const Kv8Look known = kv8_look<ROWS, UNIT>(a, G, lane, asked), known2 = kv8_look<ROWS, UNIT>(a, G, lane + 32, asked2);
+  int total = known.units * known.items + known2.units * known2.items, items = known.items + known2.items, longest = max(known.units, known2.units);
+  for (int r = 64 + lane; r < a.requests; r += 32) {
+    const Kv8Look k = kv8_look<ROWS, UNIT>(a, G, r, kv8_ask(a, r));
     total += k.units * k.items;
     items += k.items;
     longest = max(longest, k.units);
@@ -281,45 +273,124 @@ kv8_attention_split_kernel(Kv8Args a) {
   total = __reduce_add_sync(0xffffffffu, total);
   items = __reduce_add_sync(0xffffffffu, items);
   longest = __reduce_max_sync(0xffffffffu, longest);
-  const int spare = a.most - items, least = (longest + MAX_PARTS - 1) / MAX_PARTS;
-  int per = max(spare > 0 ? (total + spare - 1) / spare : longest, least);
+  // A unit takes some sixteen times what a piece adds to the join: no more than 4 sqrt(units) pieces.  (A request of 4,000 keys, 63 and 32 pieces:
+  // on 8 key heads 13.5 and 12.3 us, on 2 18.1 and 13.9.  64 and not 32 pieces at the most: 32,000 keys 31.9 and 24.8.)
+  const int spare = a.most - items, least = max((longest + MAX_PARTS - 1) / MAX_PARTS, (int)ceilf(sqrtf((float)longest) * 0.25f));
+  int per = max(spare > 0 ? (int)((uint32_t)(total + spare - 1) / (uint32_t)spare) : longest, least);
   if (spare > 0 && a.requests <= 64) {
-    // pieces a unit shorter, as long as there are CTAs for them (the bound above counts an unfinished piece for every item)
-    for (int tries = 0; tries < 4 && per > max(least, 1); ++tries) {
-      const float inverse = 1.f / (float)(per - 1);
-      const int one = (known.items ? kv8_parts(known.units, inverse) : 0) * known.items + (known2.items ? kv8_parts(known2.units, inverse) : 0) * known2.items;
-      if (__reduce_add_sync(0xffffffffu, one) > a.most) break;
-      --per;
+    // pieces up to four units shorter, as long as there are CTAs for them (the bound above counts an unfinished piece for every item)
+    int shorter = 0;
+#pragma unroll
+    for (int i = 1; i <= 4; ++i) {
+      const float inverse = 1.f / (float)max(per - i, 1);
+      const int all = __reduce_add_sync(0xffffffffu, (known.items ? kv8_parts(known.units, inverse) : 0) * known.items +
+                                                     (known2.items ? kv8_parts(known2.units, inverse) : 0) * known2.items);
+      if (per - i >= least && all <= a.most) shorter = i;
     }
+    per -= shorter;
   }
   const float per_inverse = 1.f / (float)per;
-  int r = -1, q0, q_len, L, units, pieces, at = blockIdx.x;             // at: of the pieces of the request
-  for (int r0 = 0; r0 < a.requests; r0 += 32) {
-    const Kv8Look k = look(r0);
-    const int mine = k.items ? kv8_parts(k.units, per_inverse) : 0;
-    int upto = mine * k.items;
-    const int own = upto;
+  // the first request whose pieces, with all before it, exceed this CTA's number: 64 of them at a time
+  int r = -1, q0 = 0, q_len = 0, L = 0, units = 0, pieces = 0, at = blockIdx.x;
+  for (int r0 = 0; r0 < a.requests; r0 += 64) {
+    const Kv8Look k = r0 == 0 ? known : kv8_look<ROWS, UNIT>(a, G, r0 + lane, kv8_ask(a, r0 + lane));
+    const Kv8Look k2 = r0 == 0 ? known2 : kv8_look<ROWS, UNIT>(a, G, r0 + lane + 32, kv8_ask(a, r0 + lane + 32));
+    const int mine = k.items ? kv8_parts(k.units, per_inverse) : 0, mine2 = k2.items ? kv8_parts(k2.units, per_inverse) : 0;
+    const int own = mine * k.items, own2 = mine2 * k2.items;
+    int upto = own, upto2 = own2;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += y;
+      const int y = __shfl_up_sync(0xffffffffu, upto, d), y2 = __shfl_up_sync(0xffffffffu, upto2, d);
+      if (lane >= d) { upto += y; upto2 += y2; }
     }
-    const uint32_t hit = __ballot_sync(0xffffffffu, at < upto);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      r = r0 + src;
-      at -= __shfl_sync(0xffffffffu, upto - own, src);
-      units = __shfl_sync(0xffffffffu, k.units, src);
-      pieces = __shfl_sync(0xffffffffu, mine, src);
-      q0 = __shfl_sync(0xffffffffu, k.q0, src);
-      q_len = __shfl_sync(0xffffffffu, k.q_len, src);
-      L = __shfl_sync(0xffffffffu, k.L, src);
+    upto2 += __shfl_sync(0xffffffffu, upto, 31);
+    const uint32_t hit = __ballot_sync(0xffffffffu, at < upto), hit2 = __ballot_sync(0xffffffffu, at < upto2);
+    if (hit | hit2) {
+      const bool second = hit == 0;
+      const int src = __ffs(second ? hit2 : hit) - 1;
+      r = r0 + src + (second ? 32 : 0);
+      at -= __shfl_sync(0xffffffffu, second ? upto2 - own2 : upto - own, src);
+      units = __shfl_sync(0xffffffffu, second ? k2.units : k.units, src);
+      pieces = __shfl_sync(0xffffffffu, second ? mine2 : mine, src);
+      q0 = __shfl_sync(0xffffffffu, second ? k2.q0 : k.q0, src);
+      q_len = __shfl_sync(0xffffffffu, second ? k2.q_len : k.q_len, src);
+      L = __shfl_sync(0xffffffffu, second ? k2.L : k.L, src);
       break;
     }
-    at -= __shfl_sync(0xffffffffu, upto, 31);
+    at -= __shfl_sync(0xffffffffu, upto2, 31);
   }
+  return {r, at, units, pieces, q0, q_len, L};
+}
+
+__device__ __forceinline__ void kv8_add(float4& o, const float4& x, float f) {
+  o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+}
+// Four numbers side by side (two neighbouring lanes' pairs) of score row `row`; out: the request's first token at the key head's first query head.
+__device__ __forceinline__ void kv8_finish(qtype* out, int row, int G, int heads, int place, const float4& o, float l) {
+  qtype* to = out + ((size_t)(row / G) * heads + row % G) * D;
+  kv8_store_pair(to + kv8_place_dim(place), kv8_ratio(o.x, l), kv8_ratio(o.y, l));
+  kv8_store_pair(to + kv8_place_dim(place + 2), kv8_ratio(o.z, l), kv8_ratio(o.w, l));
+}
+// The sums of an item's pieces, in their order, by the CTA that arrived last (`first`: of piece 0).  A group's sums are on their way while it looks
+// at the maxima of all, and while the group before is added.  A call, so that the loop over the keys does not share its registers.
+template <int ROWS>
+__device__ __noinline__ void kv8_join(const float* first, float* room, int pieces, int here, int row0, int G, int heads, qtype* out) {
+  float (*const part_m)[ROWS] = reinterpret_cast<float (*)[ROWS]>(room), (*const part_l)[ROWS] = part_m + MAX_PARTS;      // in shared memory
+  constexpr int GROUP = 8;
+  struct Group { float4 x[GROUP]; };
+  const int tid = threadIdx.x;
+  auto request = [&](Group& g, int i, int c0) {                         // number i of a piece's sums, of the pieces from c0 on
+    const float* from = first + (size_t)c0 * ROWS * (D + 2) + i * 4;
+#pragma unroll
+    for (int c = 0; c < GROUP; ++c)
+      if (c0 + c < pieces) g.x[c] = __ldcg(reinterpret_cast<const float4*>(from + (size_t)c * ROWS * (D + 2)));
+  };
+  Group now, next;
+  if (tid < here * (D / 4)) request(now, tid, 0);
+  for (int i = tid; i < here * pieces; i += 32 * WARPS) {
+    const int c = i / here, row = i - c * here;
+    const float* from = first + (size_t)c * ROWS * (D + 2) + ROWS * D + row;
+    part_m[c][row] = __ldcg(from);
+    part_l[c][row] = __ldcg(from + ROWS);
+  }
+  __syncthreads();
+  for (int i = tid; i < here * (D / 4); i += 32 * WARPS) {
+    const int row = i / (D / 4);
+    float M = -INFINITY, l = 0.f;
+    if (i != tid) request(now, i, 0);
+    for (int c = 0; c < pieces; ++c) M = fmaxf(M, part_m[c][row]);
+    const float U = M == -INFINITY ? 0.f : M;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = 0; c0 < pieces; c0 += GROUP) {
+      if (c0 + GROUP < pieces) request(next, i, c0 + GROUP);
+#pragma unroll
+      for (int c = 0; c < GROUP; ++c)
+        if (c0 + c < pieces) {
+          const float f = kv8_exp2(part_m[c0 + c][row] - U);
+          kv8_add(o, now.x[c], f);
+          l = fmaf(part_l[c0 + c][row], f, l);
+        }
+      now = next;
+    }
+    kv8_finish(out, row0 + row, G, heads, (i - row * (D / 4)) * 4, o, l);
+  }
+}
+
+template <typename S>
+__global__ void __launch_bounds__(32 * WARPS, S::CTAS)
+kv8_attention_split_kernel(Kv8Args a) {
+  constexpr int NT = S::ROW_TILES, ROWS = 8 * NT, TILE = S::TILE, UNIT = TILE * WARPS;
+  extern __shared__ __align__(16) float sums[];        // [WARPS][ROWS][PITCH], then maxima and sums [WARPS][ROWS] each; in the join the pieces'
+  __shared__ int arrived;
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.heads / a.kv_heads;
+  float* const sm_m = sums + WARPS * ROWS * PITCH;
+  float* const sm_l = sm_m + WARPS * ROWS;
+  const Kv8Plan plan = kv8_plan<ROWS, UNIT>(a, G, lane);                // every warp for itself
+  const int r = plan.r, q0 = plan.q0, q_len = plan.q_len, L = plan.L, units = plan.units, pieces = plan.pieces, at = plan.at;
   if (r < 0) return;                                                    // more CTAs than pieces
-  const int item = at / pieces, piece = at - item * pieces, tile = item / a.kv_heads, kv_head = item - tile * a.kv_heads;
+  const int item = (uint32_t)at / (uint32_t)pieces, piece = at - item * pieces, tile = (uint32_t)item / (uint32_t)a.kv_heads, kv_head = item - tile * a.kv_heads;
   const int rows = q_len * G, row0 = tile * ROWS, here = min(ROWS, rows - row0);
   const int pos0 = L - q_len, p_first = pos0 + row0 / G, p_last = pos0 + (row0 + here - 1) / G;
   const int lo_request = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
@@ -348,13 +419,6 @@ kv8_attention_split_kernel(Kv8Args a) {
       }
     }
   __syncthreads();
-  auto finish_row = [&](int row, int place, float4 o, float l) {       // four numbers side by side are two neighbouring lanes' pairs
-    const int full = row0 + row;
-    qtype* to = a.out + ((size_t)(q0 + full / G) * a.heads + kv_head * G + full % G) * D;
-    kv8_store_pair(to + kv8_place_dim(place), kv8_ratio(o.x, l), kv8_ratio(o.y, l));
-    kv8_store_pair(to + kv8_place_dim(place + 2), kv8_ratio(o.z, l), kv8_ratio(o.w, l));
-  };
-  auto add = [](float4& o, const float4& x, float f) { o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w); };
   float* const mine = a.parts + (size_t)blockIdx.x * ROWS * (D + 2);
   for (int i = tid; i < here * (D / 4); i += 32 * WARPS) {
     const int row = i / (D / 4), place = (i - row * (D / 4)) * 4;
@@ -367,11 +431,11 @@ kv8_attention_split_kernel(Kv8Args a) {
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const float f = kv8_exp2(sm_m[w * ROWS + row] - U);
-      add(o, *reinterpret_cast<const float4*>(sums + (w * ROWS + row) * PITCH + place), f);
+      kv8_add(o, *reinterpret_cast<const float4*>(sums + (w * ROWS + row) * PITCH + place), f);
       l = fmaf(sm_l[w * ROWS + row], f, l);
     }
     if (pieces == 1) {
-      finish_row(row, place, o, l);
+      kv8_finish(a.out + ((size_t)q0 * a.heads + kv_head * G) * D, row0 + row, G, a.heads, place, o, l);
     } else {
       *reinterpret_cast<float4*>(mine + row * D + place) = o;
       if (place == 0) { mine[ROWS * D + row] = M; mine[ROWS * (D + 1) + row] = l; }
@@ -387,40 +451,14 @@ kv8_attention_split_kernel(Kv8Args a) {
   }
   __syncthreads();
   if (arrived != pieces - 1) return;
-  // the last of the item's pieces to arrive adds them all, in their order
-  const float* const first = mine - (size_t)piece * ROWS * (D + 2);
-  auto part = [&](int c) { return first + (size_t)c * ROWS * (D + 2); };
-  for (int i = tid; i < here * pieces; i += 32 * WARPS) {
-    const float* from = part(i / here) + ROWS * D + i % here;
-    part_m[i / here][i % here] = __ldcg(from);
-    part_l[i / here][i % here] = __ldcg(from + ROWS);
-  }
-  __syncthreads();
-  for (int i = tid; i < here * (D / 4); i += 32 * WARPS) {
-    const int row = i / (D / 4), place = (i - row * (D / 4)) * 4;
-    float M = -INFINITY, l = 0.f;
-    for (int c = 0; c < pieces; ++c) M = fmaxf(M, part_m[c][row]);
-    const float U = M == -INFINITY ? 0.f : M;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c0 = 0; c0 < pieces; c0 += 8) {
-      float4 x[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (c0 + c < pieces) x[c] = __ldcg(reinterpret_cast<const float4*>(part(c0 + c) + row * D + place));
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (c0 + c < pieces) {
-          const float f = kv8_exp2(part_m[c0 + c][row] - U);
-          add(o, x[c], f);
-          l = fmaf(part_l[c0 + c][row], f, l);
-        }
-    }
-    finish_row(row, place, o, l);
-  }
+  kv8_join<ROWS>(mine - (size_t)piece * ROWS * (D + 2), sums, pieces, here, row0, G, a.heads, a.out + ((size_t)q0 * a.heads + kv_head * G) * D);
   if (tid == 0) *counter = 0;
 }
 
-template <typename S> static size_t kv8_split_smem() { return (size_t)WARPS * 8 * S::ROW_TILES * (PITCH + 2) * sizeof(float); }
+template <typename S> static size_t kv8_split_smem() {
+  constexpr int per_row = WARPS * (PITCH + 2) > 2 * MAX_PARTS ? WARPS * (PITCH + 2) : 2 * MAX_PARTS;
+  return (size_t)8 * S::ROW_TILES * per_row * sizeof(float);
+}
 template <typename S> static int kv8_split_ctas(int* ctas) {                // that fit on the device at once
   static int known[IFB_MAX_DEVICES] = {};
   int dev = 0, per = 0;
