@@ -79,8 +79,8 @@ template <> struct MxSixteen<float> {
 // Two neighbouring lanes have a block: 16 elements (32 or 64 bytes of input, 8 of output) each.  8 lanes have the four blocks whose
 // scales lie in one 32-bit word.  The columns of a row are spread over the grid's x; a thread has PER rows, all of them requested
 // at once (a large matrix: one row per thread is a load's latency per CTA of little work).
-// early: the result is the rows of the product that follows, which reads them behind its wait.  What may become a product's matrix is read
-// before that wait, so then the next kernel may not begin while this one writes: no trigger, and the writes are performed first.
+// early: the next kernel may begin at once.  The product that rounds its rows with this kernel reads them behind its wait; but what may become a
+// product's matrix is read before that wait, so nothing may begin ahead of these writes but mx4_written_kernel.
 template <typename T, int PER>
 __global__ void __launch_bounds__(256)
 mx4_quantize_kernel(const T* x, long long row_stride, uint8_t* codes, uint8_t* scales, int rows, int k, int gated_rows, int early) {
@@ -117,7 +117,7 @@ mx4_quantize_kernel(const T* x, long long row_stride, uint8_t* codes, uint8_t* s
     }
     if ((threadIdx.x & 7) == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_at(row, e / MX_BLOCK, k_tiles)) = word;
   }
-  if (!early) __threadfence();
+  if (PER == 1 && !early) __threadfence();
 }
 
 // The values of eight codes in pairs of bfloat16, which holds them exactly.  The bits "ee m" of a code at the lowest end of a bfloat16's
@@ -143,11 +143,11 @@ template <> __device__ __forceinline__ void mx_store8<float>(float* p, const uin
   for (int i = 0; i < 2; ++i)
     reinterpret_cast<uint4*>(p)[i] = make_uint4(v[2 * i] << 16, v[2 * i] & 0xffff0000u, v[2 * i + 1] << 16, v[2 * i + 1] & 0xffff0000u);
 }
-// (No trigger, and a fence at the end, for the same reason: the numbers may be the matrix of another product.)
-template <typename T, int PER>
+template <typename T, int PER>                                          // (the numbers, too, may be the matrix of a product)
 __global__ void __launch_bounds__(256)
-mx4_values_kernel(const uint8_t* codes, const uint8_t* scales, T* out, int rows, int k, int gated_rows) {
+mx4_values_kernel(const uint8_t* codes, const uint8_t* scales, T* out, int rows, int k, int gated_rows, int early) {
   ifb_pdl_wait();
+  if (early) ifb_pdl_trigger();
   const int e = (blockIdx.x * 256 + threadIdx.x) * 8;
   if (e >= k) return;
   const int row0 = blockIdx.y * PER, k_tiles = (k + 127) / 128;
@@ -168,8 +168,16 @@ mx4_values_kernel(const uint8_t* codes, const uint8_t* scales, T* out, int rows,
     mx_values8(c[p], s[p], v);
     mx_store8<T>(out + (size_t)to * k + e, v);
   }
-  __threadfence();
+  if (PER == 1) __threadfence();
 }
+// What a matrix's kernel ends with: the kernel after this one begins when all that went before is complete and visible.  Small matrices have no
+// trigger and a fence per thread in its place (8 rows of 4,096: 3.5 us, 2.5 without; a launch is 2 us of the host's); for large ones that
+// would keep their CTAs waiting (24,576 x 4,096 there and back: 89 us, 82 with this kernel, 81 with neither).
+__global__ void mx4_written_kernel() {
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+}
+static int mx_written(cudaStream_t stream) { return ifb_launch(mx4_written_kernel, dim3(1), dim3(32), 0, stream); }
 
 static int mx_sizes(int rows, int k, int gated) {
   if (rows < 1 || k < MX_BLOCK || k % MX_BLOCK || (gated && (rows & 1))) return IFB_ERR_SIZE;
@@ -189,10 +197,10 @@ static int mx_quantize_launch(const void* x, long long row_stride, void* codes, 
     const dim3 grid(((k + 127) / 128 * 8 + 255) / 256, (n + PER - 1) / PER);
     const int e = ifb_launch(mx4_quantize_kernel<T, PER>, grid, dim3(256), 0, stream, (const T*)x + (size_t)r0 * row_stride, row_stride,
                              (uint8_t*)codes + (size_t)r0 * (k / 2), (uint8_t*)scales + (size_t)(r0 / 128) * ((k + 127) / 128) * 512, n, k,
-                             gated ? rows / 2 : 0, early);
+                             gated ? rows / 2 : 0, early || PER > 1);
     if (e) return e;
   }
-  return IFB_OK;
+  return PER > 1 && !early ? mx_written(stream) : IFB_OK;
 }
 static int mx_quantize(const void* x, int dtype, long long row_stride, void* codes, void* scales, int rows, int k, int gated, int early, void* stream) {
   const int bad = mx_sizes(rows, k, gated);
@@ -219,10 +227,11 @@ static int mx_values_launch(const void* codes, const void* scales, void* out, in
     const int n = (int)(rows - r0 < (long long)MX_GRID_ROWS * PER ? rows - r0 : (long long)MX_GRID_ROWS * PER);
     const dim3 grid((k / 8 + 255) / 256, (n + PER - 1) / PER);
     const int e = ifb_launch(mx4_values_kernel<T, PER>, grid, dim3(256), 0, stream, (const uint8_t*)codes + (size_t)r0 * (k / 2),
-                             (const uint8_t*)scales + (size_t)(r0 / 128) * ((k + 127) / 128) * 512, (T*)out + (size_t)r0 * k, n, k, gated ? rows / 2 : 0);
+                             (const uint8_t*)scales + (size_t)(r0 / 128) * ((k + 127) / 128) * 512, (T*)out + (size_t)r0 * k, n, k, gated ? rows / 2 : 0,
+                             (int)(PER > 1));
     if (e) return e;
   }
-  return IFB_OK;
+  return PER > 1 ? mx_written(stream) : IFB_OK;
 }
 IFB_EXPORT int ifb_mx4_values(const void* codes, const void* scales, void* out, int dtype, int rows, int k, int gated, void* stream) {
   const int bad = mx_sizes(rows, k, gated);
