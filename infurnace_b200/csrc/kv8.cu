@@ -33,11 +33,13 @@ __device__ __forceinline__ uint32_t kv8_codes4(const float* x, const Kv8Rounding
   return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
-// A warp per (window of rows, kind, head).  A run is the adjacent rows whose slots follow one another in one page; the warp has the
-// runs that begin in its window, a row of a decode step, 16 rows of a prompt (a warp for every row of 2,043, fifteen of sixteen
-// of which leave at once, took 9.9 us).  (A page's rows must be one run: the caller's contract.)  A lane keeps HELD
-// pieces of eight numbers in registers between the search for the largest and the rounding (a page of 16 tokens of heads of 128
-// in bfloat16 whole); of longer runs the rest is read again, from the first level of cache.
+// A warp per (place, kind, head).  A run is the adjacent rows whose slots follow one another in one page; the warp of place p has the runs that
+// begin in rows p, p + 257, p + 514 ..: up to 257 decoding rows have a place each, and since 257 is 1 more than a multiple of a usual
+// page, the runs of a prompt fall on all places alike.  (A page's rows must be one run: the caller's contract.)  A warp's time is a
+// run's way through memory and back: places and not windows of 16 rows, 2,048 rows of 8 heads of 128: a prompt 6.1 us and 5.7 (bytes alone
+// 1.9), beside 48 single tokens 6.8 and 21.5, all single tokens 25.8 and 32.1; a place for every row 11.0, 11.4 and 23.2.
+// A lane keeps HELD pieces of eight numbers in registers between the search for the largest and the rounding (a page of 16 tokens of heads
+// of 128 in bfloat16 whole); of longer runs the rest is read again, from the first level of cache.
 template <typename T> struct Piece8;
 template <> struct Piece8<bf16> {
   uint4 w;
@@ -151,74 +153,80 @@ __device__ __forceinline__ void kv8_store_run(const T* k, const T* v, long long 
   }
 }
 
+constexpr int KV8_PLACES = 257;
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv8_store_kernel(const T* k, const T* v, long long k_row, long long v_row, const int* slots, int8_t* codes, uint8_t* exponents, int rows,
-                 int heads, int page_size, int dim, int window) {
+                 int heads, int page_size, int dim) {
   ifb_pdl_wait();
   ifb_pdl_trigger();
   const int lane = threadIdx.x & 31, block = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (block >= 2 * heads) return;
-  const int row = blockIdx.x * window + lane;
-  int slot = -1, before = -1;
-  if (lane < window && row < rows) {
-    slot = slots[row];
-    if (row) before = slots[row - 1];
-  }
-  // a row begins a run if it is stored and does not follow the row before it in one page
-  uint32_t begins = __ballot_sync(0xffffffffu, slot >= 0 && !(slot % page_size && before == slot - 1));
-  while (begins) {
-    const int src = __ffs(begins) - 1;
-    begins &= begins - 1;
-    kv8_store_run<T>(k, v, k_row, v_row, slots, codes, exponents, rows, heads, page_size, dim, blockIdx.x * window + src,
-                     __shfl_sync(0xffffffffu, slot, src), block, lane);
+  for (long long base = blockIdx.x; base < rows; base += 32LL * gridDim.x) {
+    const long long row = base + (long long)lane * gridDim.x;
+    int slot = -1, before = -1;
+    if (row < rows) {
+      slot = slots[row];
+      if (row) before = slots[row - 1];
+    }
+    // a row begins a run if it is stored and does not follow the row before it in one page
+    uint32_t begins = __ballot_sync(0xffffffffu, slot >= 0 && !(slot % page_size && before == slot - 1));
+    while (begins) {
+      const int src = __ffs(begins) - 1;
+      begins &= begins - 1;
+      kv8_store_run<T>(k, v, k_row, v_row, slots, codes, exponents, rows, heads, page_size, dim, (int)(base + (long long)src * gridDim.x),
+                       __shfl_sync(0xffffffffu, slot, src), block, lane);
+    }
   }
 }
 
-// What 16 codes stand for, as T (both types hold (code + 1/2) step exactly).
-template <typename T> __device__ __forceinline__ void kv8_write16(T* to, const uint4& c, float step);
-template <> __device__ __forceinline__ void kv8_write16<float>(float* to, const uint4& c, float step) {
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float4 y;
-    y.x = ((float)(int8_t)(w[i]) + 0.5f) * step;
-    y.y = ((float)(int8_t)(w[i] >> 8) + 0.5f) * step;
-    y.z = ((float)(int8_t)(w[i] >> 16) + 0.5f) * step;
-    y.w = ((float)(int8_t)(w[i] >> 24) + 0.5f) * step;
-    *reinterpret_cast<float4*>(to + 4 * i) = y;
-  }
+__device__ __forceinline__ float4 kv8_numbers4(uint32_t w, float step) {
+  return make_float4(((float)(int8_t)(w) + 0.5f) * step, ((float)(int8_t)(w >> 8) + 0.5f) * step, ((float)(int8_t)(w >> 16) + 0.5f) * step,
+                     ((float)(int8_t)(w >> 24) + 0.5f) * step);
 }
-template <> __device__ __forceinline__ void kv8_write16<bf16>(bf16* to, const uint4& c, float step) {
+// What 16 codes stand for, as bfloat16 (which, as float32, holds (code + 1/2) step exactly).
+__device__ __forceinline__ void kv8_write16(bf16* to, const uint4& c, float step) {
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
   uint32_t y[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const __nv_bfloat162 b = __floats2bfloat162_rn(((float)(int8_t)(w[i] >> (16 * h)) + 0.5f) * step,
-                                                     ((float)(int8_t)(w[i] >> (16 * h + 8)) + 0.5f) * step);
-      y[2 * i + h] = *reinterpret_cast<const uint32_t*>(&b);
-    }
+    const float4 v = kv8_numbers4(w[i], step);
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+    y[2 * i] = *reinterpret_cast<const uint32_t*>(&lo);
+    y[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hi);
   }
   *reinterpret_cast<uint4*>(to) = make_uint4(y[0], y[1], y[2], y[3]);
   *reinterpret_cast<uint4*>(to + 8) = make_uint4(y[4], y[5], y[6], y[7]);
 }
+// Bound by the bytes written.  A lane takes 16 codes; as float32 four of each of its warp's four rows of 128, so that a store fills whole
+// lines.  8,000 pages of 16 tokens of 8 heads of 128: 121 us
+// (6.5 TB/s), as float32 205 (6.4; 291 with a lane's 16 side by side).
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv8_values_kernel(const int8_t* codes, const uint8_t* exponents, T* out, long long pieces, int per_block) {
   ifb_pdl_wait();
   ifb_pdl_trigger();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (long long)gridDim.x * 256) {
-    const uint4 c = *reinterpret_cast<const uint4*>(codes + i * 16);
-    kv8_write16<T>(out + i * 16, c, kv8_step(exponents[i / per_block]));
+    if constexpr (sizeof(T) == 2) {
+      kv8_write16(out + i * 16, *reinterpret_cast<const uint4*>(codes + i * 16), kv8_step(exponents[i / per_block]));
+    } else {
+      const int lane = threadIdx.x & 31;                                // (pieces are a multiple of 32: whole warps have one)
+      const long long first = (i - lane) * 4 + lane;                    // in words of four codes
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = reinterpret_cast<const uint32_t*>(codes)[first + j * 32];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        reinterpret_cast<float4*>(out)[first + j * 32] = kv8_numbers4(w[j], kv8_step(exponents[(first + j * 32) / (4 * per_block)]));
+    }
   }
 }
 
 // The pages of the requests with more than `above` score rows as bfloat16 pages, for a kernel that reads those: the pages that a
 // request's keys lie in, one after the other over all such requests, and a table of them.  Exact, but for a block of NaN:
 // either kind's makes the page's keys NaN and its values 0, so that rows that do not see the page keep their numbers (a weight
-// of 0 times NaN would not be 0) and rows that see it are NaN.  Grid (pages of a request, 2 kinds, requests).
+// of 0 times NaN would not be 0) and rows that see it are NaN.  Grid (pages of a request, 2 kinds, requests).  Bound by memory: a byte read and
+// two written for each number: 2,000 pages of 16 tokens of 8 heads of 128 35 us, 5.6 TB/s.
 __global__ void __launch_bounds__(256)
 kv8_expand_kernel(const int8_t* codes, const uint8_t* exponents, const int* tables, int table_stride, const int* cu_q, const int* seq_lens, bf16* out,
                   int* out_tables, int out_pages, int heads, int group, int page_size, int dim, int window, int above) {
@@ -249,7 +257,7 @@ kv8_expand_kernel(const int8_t* codes, const uint8_t* exponents, const int* tabl
     const int h = i / per_head;
     const bool nan = fields[h] == 255 || fields[heads + h] == 255;
     const float step = nan ? (kind ? 0.f : __uint_as_float(0x7fffffffu)) : kv8_step(fields[kind * heads + h]);
-    kv8_write16<bf16>(dst + (size_t)i * 16, *reinterpret_cast<const uint4*>(src + (size_t)i * 16), step);
+    kv8_write16(dst + (size_t)i * 16, *reinterpret_cast<const uint4*>(src + (size_t)i * 16), step);
   }
 }
 
@@ -267,13 +275,12 @@ IFB_EXPORT int ifb_kv8_store(const void* k, const void* v, int dtype, long long 
   const int esize = dtype == IFB_F32 ? 4 : 2;
   if ((((uintptr_t)k) | ((uintptr_t)v) | (uintptr_t)(k_row * esize) | (uintptr_t)(v_row * esize) | ((uintptr_t)codes)) & 15) return IFB_ERR_ALIGN;
   const int warps = 2 * heads < 8 ? 2 * heads : 8;
-  const int window = rows > 256 ? 16 : 1;
-  const dim3 grid((rows + window - 1) / window, (2 * heads + warps - 1) / warps);
+  const dim3 grid(rows < KV8_PLACES ? rows : KV8_PLACES, (2 * heads + warps - 1) / warps);
   if (dtype == IFB_F32)
     return ifb_launch(kv8_store_kernel<float>, grid, dim3(32 * warps), 0, (cudaStream_t)stream, (const float*)k, (const float*)v, k_row, v_row,
-                      (const int*)slots, (int8_t*)codes, (uint8_t*)exponents, rows, heads, page_size, dim, window);
+                      (const int*)slots, (int8_t*)codes, (uint8_t*)exponents, rows, heads, page_size, dim);
   return ifb_launch(kv8_store_kernel<bf16>, grid, dim3(32 * warps), 0, (cudaStream_t)stream, (const bf16*)k, (const bf16*)v, k_row, v_row,
-                    (const int*)slots, (int8_t*)codes, (uint8_t*)exponents, rows, heads, page_size, dim, window);
+                    (const int*)slots, (int8_t*)codes, (uint8_t*)exponents, rows, heads, page_size, dim);
 }
 
 IFB_EXPORT int ifb_kv8_values(const void* codes, const void* exponents, void* out, int dtype, int pages, int heads, int page_size, int dim,

@@ -78,7 +78,8 @@ template <> struct MxSixteen<float> {
 
 // Two neighbouring lanes have a block: 16 elements (32 or 64 bytes of input, 8 of output) each.  8 lanes have the four blocks whose
 // scales lie in one 32-bit word.  The columns of a row are spread over the grid's x; a thread has PER rows, all of them requested
-// at once (a large matrix: one row per thread is a load's latency per CTA of little work).
+// at once (a large matrix: one row per thread is a load's latency per CTA of little work).  Bound by memory: 24,576 x 4,096 of bfloat16 38 us,
+// 6.7 TB/s, and the way back 40 us, 6.4 TB/s.
 // early: the next kernel may begin at once.  The product that rounds its rows with this kernel reads them behind its wait; but what may become a
 // product's matrix is read before that wait, so nothing may begin ahead of these writes but mx4_written_kernel.
 template <typename T, int PER>
@@ -185,8 +186,12 @@ static int mx_sizes(int rows, int k, int gated) {
 }
 
 constexpr int MX_GRID_ROWS = 65535 / 256 * 256;      // a grid has at most 65,535 rows; whole tiles of rows, whole pairs
-// Rows per thread: four where that still gives every SM several CTAs, or where a grid would not have the rows.
-static int mx_rows_per_thread(int rows, int k) { return (long long)rows * k >= (long long)ifb_sm_count() * 65536 || rows > MX_GRID_ROWS ? 4 : 1; }
+// Rows per thread: four where that still gives every SM several CTAs, or where a grid would not have the rows; the one row of a float32 matrix is as
+// many bytes in flight as two of bfloat16.  One and four, bfloat16: 8 rows of 4,096 1.9 and 2.5 us, 512 rows 2.8 both, 2,048 rows 5.4 and 4.9,
+// 24,576 rows 50.3 and 39.0 (there and back 126 and 80); float32: 2,048 rows 7.2 and 7.8, 8,192 rows 27.1 and 26.4.
+static int mx_rows_per_thread(int rows, int k, int dtype) {
+  return (long long)rows * k >= (long long)ifb_sm_count() * (dtype == IFB_F32 ? 131072 : 32768) || rows > MX_GRID_ROWS ? 4 : 1;
+}
 
 template <typename T, int PER>
 static int mx_quantize_launch(const void* x, long long row_stride, void* codes, void* scales, int rows, int k, int gated, int early, cudaStream_t stream) {
@@ -209,7 +214,7 @@ static int mx_quantize(const void* x, int dtype, long long row_stride, void* cod
   if (dtype != IFB_F32 && dtype != IFB_BF16) return IFB_ERR_DTYPE;
   if ((((uintptr_t)x) | ((uintptr_t)codes) | ((uintptr_t)scales) | (uintptr_t)(row_stride * esize)) & 15) return IFB_ERR_ALIGN;
   cudaStream_t st = (cudaStream_t)stream;
-  if (mx_rows_per_thread(rows, k) == 4)
+  if (mx_rows_per_thread(rows, k, dtype) == 4)
     return dtype == IFB_F32 ? mx_quantize_launch<float, 4>(x, row_stride, codes, scales, rows, k, gated, early, st)
                             : mx_quantize_launch<bf16, 4>(x, row_stride, codes, scales, rows, k, gated, early, st);
   return dtype == IFB_F32 ? mx_quantize_launch<float, 1>(x, row_stride, codes, scales, rows, k, gated, early, st)
@@ -239,7 +244,7 @@ IFB_EXPORT int ifb_mx4_values(const void* codes, const void* scales, void* out, 
   if (dtype != IFB_F32 && dtype != IFB_BF16) return IFB_ERR_DTYPE;
   if ((((uintptr_t)out) | ((uintptr_t)codes) | ((uintptr_t)scales)) & 15) return IFB_ERR_ALIGN;
   cudaStream_t st = (cudaStream_t)stream;
-  if (mx_rows_per_thread(rows, k) == 4)
+  if (mx_rows_per_thread(rows, k, dtype) == 4)
     return dtype == IFB_F32 ? mx_values_launch<float, 4>(codes, scales, out, rows, k, gated, st) : mx_values_launch<bf16, 4>(codes, scales, out, rows, k, gated, st);
   return dtype == IFB_F32 ? mx_values_launch<float, 1>(codes, scales, out, rows, k, gated, st) : mx_values_launch<bf16, 1>(codes, scales, out, rows, k, gated, st);
 }
