@@ -45,10 +45,9 @@ template <int LEFT> struct Values {
   static constexpr int W = LEFT >= 128 ? 128 : LEFT >= 64 ? 64 : LEFT >= 32 ? 32 : 16;
   Piece<W> v[4];
   Values<LEFT - W> rest;
-  __device__ __forceinline__ void load(const int8_t* tile, int lane) {       // tile: the first of the 16 keys, at this block
-    const int8_t* p = tile + (lane & 3) * 2 * D + (lane >> 2) * (W / 8);
+  __device__ __forceinline__ void load(const int8_t* p, int lane) {       // p: the first of the 16 keys at this block, and the lane's offset
     v[0].load(p); v[1].load(p + D); v[2].load(p + 8 * D); v[3].load(p + 9 * D);
-    rest.load(tile + W, lane);
+    rest.load(p + next_block<LEFT>(lane), lane);
   }
   // o^T += v^T p^T; m tile i of a block has dimension chunk + 2 i in its row lane / 4 and chunk + 2 i + 1 in row lane / 4 + 8
   template <int NT>
@@ -222,36 +221,36 @@ struct Stream {
     Keys k;
     Values<D> v;
     __device__ __forceinline__ Walk(const Kv8Args& a, const int* table_, int kv_head, int, int, int first_, int end_, int step_, int lane)
-        : Kv8Pages(a, table_, kv_head) {
+        : Kv8Pages(a, table_, kv_head, lane) {
       first = first_; end = end_; step = step_; next_page = 0;
       if (first >= end) return;
       const int page = page_of(first);
       if (first + step < end) next_page = page_of(first + step);
-      const int8_t* at = keys(first, page);
+      const size_t from = at(first, page);
       read_fields(page, kf, vf);
-      k.load(at, lane);
-      v.load(at + v_off, lane);
+      k.load(k_base + from, lane);
+      v.load(v_base + from, lane);
     }
   };
   __device__ __forceinline__ void run(const Kv8Args& a, Walk& w, int full_from, int full_to, int lane) {
+    const float scale64 = a.scale * 0.015625f;
     for (int t = w.first; t < w.end; t += w.step) {
       const bool more = t + w.step < w.end;
       float s[NT][4];
       const bool whole = t * 16 >= full_from && t * 16 + 15 <= full_to;
-      // (a page whose values are NaN makes the scores NaN that see it, and with them the row)
-      const float ks = kv8_step(w.vf == 255 ? 255u : (uint32_t)w.kf) * a.scale;
-      const int vf = w.vf == 255 ? 0 : w.vf;
+      const float ks = kv8_score_step(w.kf, w.vf, scale64);
+      const int vf = kv8_value_field(w.vf);
       if (whole) scores<false>(w.k, ks, t * 16, a.window, s, lane);
       else scores<true>(w.k, ks, t * 16, a.window, s, lane);
-      const int8_t* next = w.base;
+      size_t next = 0;
       if (more) {                                                       // the next keys while these values are multiplied
-        next = w.keys(t + w.step, w.next_page);
+        next = w.at(t + w.step, w.next_page);
         w.read_fields(w.next_page, w.kf, w.vf);
-        w.k.load(next, lane);
+        w.k.load(w.k_base + next, lane);
         if (t + 2 * w.step < w.end) w.next_page = w.page_of(t + 2 * w.step);
       }
       weigh(s, w.v, vf);
-      if (more) w.v.load(next + w.v_off, lane);                         // and the next values while the next scores are formed
+      if (more) w.v.load(w.v_base + next, lane);                         // and the next values while the next scores are formed
     }
   }
   // Sums over the lanes that share a row, and the weighted values in real units (times the weights' common factor).

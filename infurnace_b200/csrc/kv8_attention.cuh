@@ -85,6 +85,15 @@ template <> struct Piece<32> { uint32_t r; __device__ __forceinline__ void load(
 template <> struct Piece<16> { uint32_t r; __device__ __forceinline__ void load(const int8_t* p) { r = *reinterpret_cast<const uint16_t*>(p); }
   __device__ __forceinline__ uint32_t word(int) const { return r; } };
 
+// Where a lane's piece of a block of W dimensions of values begins: key 2 (lane % 4).
+template <int LEFT> struct ValueBlock { static constexpr int W = LEFT >= 128 ? 128 : LEFT >= 64 ? 64 : LEFT >= 32 ? 32 : LEFT >= 16 ? 16 : 0; };
+__device__ __forceinline__ int value_offset(int lane) { return (lane & 3) * 2 * D + (lane >> 2) * (ValueBlock<D>::W / 8); }
+// From a block's piece to the next block's.
+template <int LEFT> __device__ __forceinline__ int next_block(int lane) {
+  constexpr int W = ValueBlock<LEFT>::W, NEXT = ValueBlock<LEFT - W>::W;
+  return W + (lane >> 2) * ((NEXT - W) / 8);
+}
+
 // The dimension of element e (0, 1) of m tile i of an output product over values of LEFT dimensions, in blocks that follow one another.
 template <int LEFT> __device__ __forceinline__ int value_dim(int i, int lane, int e) {
   if constexpr (LEFT == 0) {
@@ -100,14 +109,15 @@ template <int LEFT> __device__ __forceinline__ int value_dim(int i, int lane, in
 struct Keys {
   uint4 w[2][K64 ? K64 : 1];
   uint32_t tail[2][KS - 4 * K64 ? KS - 4 * K64 : 1];
-  __device__ __forceinline__ void load(const int8_t* keys, int lane) {
+  static __device__ __forceinline__ int offset(int lane) { return (lane >> 2) * D + (lane & 3) * (K64 ? 16 : 4); }
+  __device__ __forceinline__ void load(const int8_t* keys, int lane) {       // keys: the first of the group's, and the lane's offset
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int8_t* p = keys + ((lane >> 2) + 8 * e) * D;
 #pragma unroll
-      for (int h = 0; h < K64; ++h) w[e][h] = *reinterpret_cast<const uint4*>(p + h * 64 + (lane & 3) * 16);
+      for (int h = 0; h < K64; ++h) w[e][h] = *reinterpret_cast<const uint4*>(keys + e * 8 * D + h * 64);
 #pragma unroll
-      for (int s = 0; s < KS - 4 * K64; ++s) tail[e][s] = *reinterpret_cast<const uint32_t*>(p + K64 * 64 + s * 16 + (lane & 3) * 4);
+      for (int s = 0; s < KS - 4 * K64; ++s)
+        tail[e][s] = *reinterpret_cast<const uint32_t*>(keys + e * 8 * D + K64 * 64 + s * 16 - (K64 ? (lane & 3) * 12 : 0));
     }
   }
   __device__ __forceinline__ uint32_t word(int e, int ks) const {
@@ -147,37 +157,41 @@ __device__ __forceinline__ void request_queries(Queries<NT>& raw, const Kv8Args&
   }
 }
 
-// The pages of a request as a stream's walk reads them.
+// The pages of a request as a lane of a stream's walk reads them: few instructions a group, the lane's offsets are in the bases.
 struct Kv8Pages {
   const int* table;
-  const int8_t* base;
-  const uint8_t* fields;
-  size_t page_bytes, v_off;
-  uint32_t per_page, inverse;
-  int kv_heads;
-  __device__ __forceinline__ Kv8Pages(const Kv8Args& a, const int* table_, int kv_head) {
+  const int8_t *k_base, *v_base;
+  const uint8_t *k_fields, *v_fields;
+  uint32_t page_bytes, page_fields, per_page, inverse;
+  __device__ __forceinline__ Kv8Pages(const Kv8Args& a, const int* table_, int kv_head, int lane) {
     table = table_;
-    page_bytes = 2 * (size_t)a.kv_heads * a.page_size * D;
-    base = a.codes + (size_t)kv_head * a.page_size * D;
-    v_off = (size_t)a.kv_heads * a.page_size * D;
-    fields = a.exponents + kv_head;
-    kv_heads = a.kv_heads;
+    page_bytes = 2u * (uint32_t)a.kv_heads * (uint32_t)a.page_size * D;
+    k_base = a.codes + (size_t)kv_head * a.page_size * D + Keys::offset(lane);
+    v_base = a.codes + (size_t)(a.kv_heads + kv_head) * a.page_size * D + value_offset(lane);
+    k_fields = a.exponents + kv_head;
+    v_fields = k_fields + a.kv_heads;
+    page_fields = 2u * (uint32_t)a.kv_heads;
     per_page = (uint32_t)a.page_size / 16;
     inverse = per_page > 1 ? 0xffffffffu / per_page + 1 : 0;
   }
   // The page of a group of 16 keys (its number over groups per page, by a product with the next whole number above 2^32 / per_page:
-  // exact for groups below 2^32 / per_page), where its keys begin (its values v_off further), and its exponent fields.
+  // exact for groups below 2^32 / per_page), where its keys begin from a base (and its values from theirs), and its exponent fields.
   __device__ __forceinline__ int place(int group) const { return per_page > 1 ? (int)__umulhi((uint32_t)group, inverse) : group; }
   __device__ __forceinline__ int page_of(int group) const { return table[place(group)]; }
-  __device__ __forceinline__ const int8_t* keys(int group, int page) const {
-    return base + (size_t)page * page_bytes + (uint32_t)(group - place(group) * (int)per_page) * (16 * D);
+  __device__ __forceinline__ size_t at(int group, int page) const {
+    return (size_t)(uint32_t)page * page_bytes + (uint32_t)(group - place(group) * (int)per_page) * (16 * D);
   }
   __device__ __forceinline__ void read_fields(int page, int& kf, int& vf) const {
-    const uint8_t* f = fields + (size_t)page * 2 * kv_heads;
-    kf = f[0];
-    vf = f[kv_heads];
+    kf = k_fields[(size_t)(uint32_t)page * page_fields];
+    vf = v_fields[(size_t)(uint32_t)page * page_fields];
   }
 };
+// The factor of a page's scores: its keys' step times `scale64`, the scores' scale over 64 (a step is 2^-6 of what its field says as a float's).  A page
+// whose values are NaN makes the scores NaN that see it, and with them the row; as values its block is then one of zeros.
+__device__ __forceinline__ float kv8_score_step(int kf, int vf, float scale64) {
+  return max(kf, vf) == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)kf << 23) * scale64;
+}
+__device__ __forceinline__ int kv8_value_field(int vf) { return vf == 255 ? 0 : vf; }
 
 __device__ __forceinline__ void kv8_store_pair(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
 __device__ __forceinline__ void kv8_store_pair(bf16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
@@ -516,7 +530,7 @@ template <typename S1, typename S2> static int kv8_call(const Kv8Call* c) {
   if (c->dtype != (KV8_F32 ? IFB_F32 : IFB_BF16)) return IFB_ERR_DTYPE;
   if (c->dim != D || c->heads < 1 || c->kv_heads < 1 || c->heads % c->kv_heads || c->page_size < 16 || c->page_size % 16 || c->requests < 1 ||
       c->max_q < 1 || c->window < 0 || c->nt < 1 || c->nt > TILES || c->kv_heads > 65535 || c->requests > 65535 || c->max_q > 0x7fffffff ||
-      c->window > 0x7fffffff || c->heads > 0x7fffffff)
+      c->window > 0x7fffffff || c->heads > 0x7fffffff || 2 * c->kv_heads * c->page_size * D > 0xffffffffLL)
     return IFB_ERR_SIZE;
   if (!whole && (!c->parts || !c->counters || c->tiles < 1)) return IFB_ERR_ARG;
   if ((((uintptr_t)c->q) | ((uintptr_t)c->codes) | ((uintptr_t)c->out) | (uintptr_t)(c->q_row * sizeof(qtype))) & 15) return IFB_ERR_ALIGN;

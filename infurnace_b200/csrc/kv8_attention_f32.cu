@@ -44,10 +44,9 @@ template <int LEFT> struct Values {
   static constexpr int W = LEFT >= 128 ? 128 : LEFT >= 64 ? 64 : LEFT >= 32 ? 32 : 16;
   Piece<W> v[2][4];
   Values<LEFT - W> rest;
-  __device__ __forceinline__ void load(int group, const int8_t* keys, int lane) {       // keys: the first of the group's, at this block
-    const int8_t* p = keys + (lane & 3) * 2 * D + (lane >> 2) * (W / 8);
+  __device__ __forceinline__ void load(int group, const int8_t* p, int lane) {       // p: the first of the group's keys at this block, and the lane's offset
     v[group][0].load(p); v[group][1].load(p + D); v[group][2].load(p + 8 * D); v[group][3].load(p + 9 * D);
-    rest.load(group, keys + W, lane);
+    rest.load(group, p + next_block<LEFT>(lane), lane);
   }
   // o += v^T p^T times the rows' factors.  The k index of a product: 4 c + j is key 2 c + 8 j, 16 + 4 c + j key 2 c + 1 + 8 j, so that a
   // word of an operand has the same byte of four keys that the lane holds.  M tile i of a block has dimension chunk + 2 i in its row
@@ -299,7 +298,7 @@ struct Stream {
     Values<D> v;
     __device__ __forceinline__ int group(int t, int g) const { return min(max(2 * t + g, low), high - 1); }
     __device__ __forceinline__ Walk(const Kv8Args& a, const int* table_, int kv_head, int low_, int high_, int first_, int end_, int step_, int lane)
-        : Kv8Pages(a, table_, kv_head) {
+        : Kv8Pages(a, table_, kv_head, lane) {
       low = low_; high = high_; first = first_; end = end_; step = step_;
       if (first >= end) return;
       int page[2];
@@ -310,15 +309,16 @@ struct Stream {
       }
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const int8_t* at = keys(group(first, g), page[g]);
+        const size_t from = at(group(first, g), page[g]);
         read_fields(page[g], kf[g], vf[g]);
-        k[g].load(at, lane);
-        v.load(g, at + v_off, lane);
+        k[g].load(k_base + from, lane);
+        v.load(g, v_base + from, lane);
       }
     }
   };
   // full_from, full_to: keys from and up to here are seen by every row that exists.
   __device__ __forceinline__ void run(const Kv8Args& a, Walk& w, int full_from, int full_to, int lane) {
+    const float scale64 = a.scale * 0.015625f;
     for (int t = w.first; t < w.end; t += w.step) {
       const bool more = t + w.step < w.end;
       float s[2][NT][4];
@@ -326,19 +326,18 @@ struct Stream {
       int vf[2];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        // (a page whose values are NaN makes the scores NaN that see it, and with them the row)
-        const float ks = kv8_step(w.vf[g] == 255 ? 255u : (uint32_t)w.kf[g]) * a.scale;
-        vf[g] = w.vf[g] == 255 ? 0 : w.vf[g];
+        const float ks = kv8_score_step(w.kf[g], w.vf[g], scale64);
+        vf[g] = kv8_value_field(w.vf[g]);
         if (whole) scores<false>(w.k[g], ks, t * TILE + g * 16, a.window, s[g], lane);
         else scores<true>(w.k[g], ks, t * TILE + g * 16, a.window, s[g], lane);
       }
-      const int8_t* next[2] = {w.base, w.base};
+      size_t next[2] = {0, 0};
       if (more) {                                                       // the next keys while these values are multiplied
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          next[g] = w.keys(w.group(t + w.step, g), w.next_page[g]);
+          next[g] = w.at(w.group(t + w.step, g), w.next_page[g]);
           w.read_fields(w.next_page[g], w.kf[g], w.vf[g]);
-          w.k[g].load(next[g], lane);
+          w.k[g].load(w.k_base + next[g], lane);
         }
         if (t + 2 * w.step < w.end) {
 #pragma unroll
@@ -348,7 +347,7 @@ struct Stream {
       weigh(s, w.v, vf[0], vf[1]);
       if (more) {                                                       // and the next values while the next scores are formed
 #pragma unroll
-        for (int g = 0; g < 2; ++g) w.v.load(g, next[g] + w.v_off, lane);
+        for (int g = 0; g < 2; ++g) w.v.load(g, w.v_base + next[g], lane);
       }
     }
   }
