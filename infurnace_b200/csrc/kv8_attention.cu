@@ -15,9 +15,11 @@
 // half-precision numbers down to 2^-32 of it still count.  A weight enters the product times its page's step over the largest
 // step so far.  Sums are float32.
 //
-// What bounds it: a warp takes some 380 instructions for 16 keys of 128, 260 of them on the integer pipe, most for the bytes of keys
-// and values; the loop brings 4.8 to 5.8 TB/s, and a call has some 9 us beside it (the look at the lengths, the first trip, the joins).
-// Eight requests of 3,967 to 8,095 keys (32 heads on 8) 28 us, 3.5 TB/s; 64 of 129 to 383 (16 on 8) 16 us.
+// What bounds it: the integer pipe, for the bytes of keys and values (half of its time over a whole call), and the registers, with 128 of which four CTAs
+// fit on an SM: what does not have to stay in one over the loop is named anew or uniform (46.1 to 42.2 us in the third figure).  A call has some
+// 8 us beside the loop: the look at the lengths, the first trip, the joins.  Eight requests of 3,967 to 8,095 keys (32 heads on 8)
+// 26.5 us, 3.7 TB/s; 64 of 129 to 383 (16 on 8) 14.5; 64 of 1,500 (32 on 8) 42.2, 4.7 TB/s.  Slower were: copies to shared memory some tiles
+// ahead, requests to the second level of cache two tiles ahead, values requested with the keys, three CTAs with more registers (59 us).
 #define KV8_F32 0
 #include "kv8_attention.cuh"
 #include <cuda_fp16.h>
@@ -77,9 +79,9 @@ struct Stream {
   uint32_t qf[NT][KS][2];
   float qscale[NT][2], qoff[NT][2];      // what turns a product into a number of real units: times qscale, and qoff
   int last[NT][2];                       // position of the row's query (NO_ROW: no such row)
-  // m: reference of the row's scores; rise: what a score has to exceed to move it; shift: what is added to a score for its weight;
-  // l, wsum: this lane's part of the sums of the weights, and of weights times steps
-  float m[NT][2], rise[NT][2], shift[NT][2], l[NT][2], wsum[NT][2];
+  // m: reference of the row's scores, finite (a score has to exceed m + 6 to move it, and a weight is 2^(score + (8 - m))); l, wsum: this lane's
+  // part of the sums of the weights, and of weights times steps
+  float m[NT][2], l[NT][2], wsum[NT][2];
   float o[KS][NT][4];
   int v_ref;                             // exponent field that the sums of weighted values are in units of
 
@@ -88,7 +90,7 @@ struct Stream {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) { m[n][e] = rise[n][e] = -INFINITY; shift[n][e] = 8.f; l[n][e] = 0.f; wsum[n][e] = 0.f; }
+      for (int e = 0; e < 2; ++e) { m[n][e] = NO_SCORE; l[n][e] = 0.f; wsum[n][e] = 0.f; }
 #pragma unroll
       for (int i = 0; i < KS; ++i) { o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f; }
     }
@@ -162,7 +164,7 @@ struct Stream {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) up |= fmaxf(s[n][e], s[n][2 + e]) > rise[n][e];
+      for (int e = 0; e < 2; ++e) up |= fmaxf(s[n][e], s[n][2 + e]) > m[n][e] + 6.f;
     const bool larger = vf > v_ref;                                     // uniform
     if (__any_sync(0xffffffffu, up) || larger) {
       float fv = 1.f;
@@ -180,10 +182,8 @@ struct Stream {
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
           mx = fmaxf(mx, m[n][e]);
-          f[e] = mx == m[n][e] ? 1.f : kv8_exp2(m[n][e] - mx);
+          f[e] = kv8_exp2(m[n][e] - mx);
           m[n][e] = mx;
-          rise[n][e] = mx + 6.f;
-          shift[n][e] = mx == -INFINITY ? 8.f : 8.f - mx;
           l[n][e] *= f[e];
           f[e] *= fv;
           wsum[n][e] *= f[e];
@@ -199,7 +199,7 @@ struct Stream {
     for (int n = 0; n < NT; ++n) {
       float w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = kv8_exp2(s[n][j] + shift[n][j & 1]);
+      for (int j = 0; j < 4; ++j) w[j] = kv8_exp2(s[n][j] + (8.f - m[n][j & 1]));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float both = w[e] + w[2 + e];
@@ -221,8 +221,8 @@ struct Stream {
     Keys k;
     Values<D> v;
     __device__ __forceinline__ Walk(const Kv8Args& a, const int* table_, int kv_head, int, int, int first_, int end_, int step_, int lane)
-        : Kv8Pages(a, table_, kv_head, lane) {
-      first = first_; end = end_; step = step_; next_page = 0;
+        : Kv8Pages(a, table_, kv8_uniform(kv_head), lane) {
+      first = kv8_uniform(first_); end = kv8_uniform(end_); step = step_; next_page = 0;
       if (first >= end) return;
       const int page = page_of(first);
       if (first + step < end) next_page = page_of(first + step);

@@ -37,6 +37,7 @@ constexpr int WARPS = 4;
 constexpr int K64 = D / 64;              // pieces of 64 dimensions of a key that a quad of lanes takes 16 bytes a lane at a time
 constexpr int TILES = D <= 128 ? 2 : 1;  // tiles of 8 score rows that a warp has at most (wider heads leave no registers for a second)
 constexpr int NO_ROW = -1000000000;
+constexpr float NO_SCORE = -3.402823466e38f;      // the lowest float
 
 struct Kv8Args {
   const qtype* q;
@@ -56,6 +57,9 @@ struct Kv8Args {
   int tiles;                             // split form: tiles of score rows that any request has at most
   int most;                              // split form: CTAs that run on the device at a time
 };
+
+// A number that all lanes of a warp have, so that it may live in a uniform register: those of the loops over keys are scarce.
+__device__ __forceinline__ int kv8_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 __device__ __forceinline__ float kv8_exp2(float x) {
   float y;
@@ -161,15 +165,14 @@ __device__ __forceinline__ void request_queries(Queries<NT>& raw, const Kv8Args&
 struct Kv8Pages {
   const int* table;
   const int8_t *k_base, *v_base;
-  const uint8_t *k_fields, *v_fields;
+  const uint8_t* fields;
   uint32_t page_bytes, page_fields, per_page, inverse;
   __device__ __forceinline__ Kv8Pages(const Kv8Args& a, const int* table_, int kv_head, int lane) {
     table = table_;
     page_bytes = 2u * (uint32_t)a.kv_heads * (uint32_t)a.page_size * D;
     k_base = a.codes + (size_t)kv_head * a.page_size * D + Keys::offset(lane);
     v_base = a.codes + (size_t)(a.kv_heads + kv_head) * a.page_size * D + value_offset(lane);
-    k_fields = a.exponents + kv_head;
-    v_fields = k_fields + a.kv_heads;
+    fields = a.exponents + kv_head;
     page_fields = 2u * (uint32_t)a.kv_heads;
     per_page = (uint32_t)a.page_size / 16;
     inverse = per_page > 1 ? 0xffffffffu / per_page + 1 : 0;
@@ -182,8 +185,9 @@ struct Kv8Pages {
     return (size_t)(uint32_t)page * page_bytes + (uint32_t)(group - place(group) * (int)per_page) * (16 * D);
   }
   __device__ __forceinline__ void read_fields(int page, int& kf, int& vf) const {
-    kf = k_fields[(size_t)(uint32_t)page * page_fields];
-    vf = v_fields[(size_t)(uint32_t)page * page_fields];
+    const uint8_t* at = fields + (size_t)(uint32_t)page * page_fields;
+    kf = at[0];
+    vf = at[page_fields >> 1];
   }
 };
 // The factor of a page's scores: its keys' step times `scale64`, the scores' scale over 64 (a step is 2^-6 of what its field says as a float's).  A page

@@ -9,8 +9,8 @@
 // each; everything outside of the products is float32.
 // Errors against 64 bits 3 to 5e-7 of the output, below those of plain float32 sums; with queries and weights of two
 // half-precision terms each, in the same time, 1.4 to 2.4e-6 (the running sums of half-precision products are cut off, not
-// rounded).  For bfloat16 the two are not of the same time: eight requests of 4,000 to 8,100 keys 33 us so, 28 as in
-// kv8_attention.cu.
+// rounded).  For bfloat16 the two are not of the same time: eight requests of 3,967 to 8,095 keys 32 us here, 26.5
+// as in kv8_attention.cu.
 #define KV8_F32 1
 #include "kv8_attention.cuh"
 
@@ -298,8 +298,8 @@ struct Stream {
     Values<D> v;
     __device__ __forceinline__ int group(int t, int g) const { return min(max(2 * t + g, low), high - 1); }
     __device__ __forceinline__ Walk(const Kv8Args& a, const int* table_, int kv_head, int low_, int high_, int first_, int end_, int step_, int lane)
-        : Kv8Pages(a, table_, kv_head, lane) {
-      low = low_; high = high_; first = first_; end = end_; step = step_;
+        : Kv8Pages(a, table_, kv8_uniform(kv_head), lane) {
+      low = low_; high = high_; first = kv8_uniform(first_); end = kv8_uniform(end_); step = step_;
       if (first >= end) return;
       int page[2];
 #pragma unroll
