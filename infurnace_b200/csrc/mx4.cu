@@ -268,6 +268,9 @@ IFB_EXPORT int ifb_mx4_values(const void* codes, const void* scales, void* out, 
 // beside its part of the matrix, and a launch and a trip through memory are saved.  The numbers are requested some stages ahead
 // (one ahead: 8 rows of 12,288 by 4,096 11.1 us, four 8.3; with a kernel of its own for the rounding 8.9).  From 33 rows on the
 // rounding takes longer than the matrix (24,576 x 4,096: 25 us, 15.5 with the kernel of its own).
+// What bounds it: few tokens, the matrix's bytes and what a CTA does beside them, its start, its first stages and the sum over its cluster (8 rows
+// of 12,288 by 4,096: 8.2 us, 3.3 TB/s; 33 rows by gate and up of 12,288 x 4,096, rows rounded first: 15.6 us, 3.5 TB/s; 1 row of 1,024 by
+// 4,096: 3.3 us, latency).
 // Waits are bounded: after a limit a thread records a code in `*err`, raises the CTA's abort flag, and all fall through to the
 // end, where the tensor memory is given back.
 // ---------------------------------------------------------------------------------------------
@@ -401,7 +404,7 @@ __device__ __forceinline__ uint4 mx_round32(const uint32_t (&w)[32], uint32_t& s
 }
 
 // What becomes of a sum.  The function is chosen at compile time, or is one call: copies of every function's code for every
-// element of an unrolled loop are fetched by every SM (33 rows of gated 4,096 x 12,288: 38 us for 16).
+// element of an unrolled loop are fetched by every SM (33 rows of gated 4,096 x 12,288: 38 us then, 20 so, before other steps).
 //   MX_PLAIN: nothing; MX_SILU: silu(gate) * up with the hardware's exp2 and reciprocal (relative error about 2^-21; outputs of
 //   16 bits); MX_UNARY, MX_GATED: any function of common.cuh.
 enum { MX_PLAIN, MX_SILU, MX_UNARY, MX_GATED };
@@ -667,7 +670,9 @@ static int mx_launch_any(const CUtensorMap& xm, const CUtensorMap& wm, const MxP
 // The product of many rows, over pairs of SMs: a cluster of two CTAs owns 256 rows of w by 256 tokens.  Each CTA brings 128 rows
 // of either operand (and the scales of its rows of w and of all 256 tokens), one tcgen05.mma of the pair (M = 256), issued by the
 // first CTA, multiplies out of both shared memories into both tensor memories, where a CTA finds its 128 rows of w.  What bounds
-// these products is the bytes that reach an SM: 8 KB for the 128 cycles of 128 x 256 x 64, where a CTA alone would bring 12.
+// these products is the bytes that reach an SM: 8 KB for the 128 cycles of 128 x 256 x 64, where a CTA alone would bring 12 (2,048 rows by gate
+// and up of 12,288 x 4,096: 88 us with the rows' rounding, 4.7 PFLOP/s, the tensor pipe busy for 63 % of the time, 46 bytes a cycle into an SM; by
+// CTAs alone 150).
 // Persistent, one accumulator (the scales leave no room for two): the epilogue's warps take it to registers at once (256
 // columns in some hundred cycles) and let the next tile's products begin, which run while they finish and store.
 // The "full" barriers are the first CTA's and count both CTAs' bytes; "empty" and "accumulator ready" are each CTA's own, by

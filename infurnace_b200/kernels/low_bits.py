@@ -331,16 +331,16 @@ class LowBitKernels:
 
     kv8_expand_bytes = 4 << 30       # room for expanded pages that a call may take
     # Which form attends to requests of more than 16 score rows (queries x query heads of a key head) in bfloat16.  The split form's time
-    # grows with the rows, 3.7 ns for 1,000 keys and row in all (heads of 128).  The tcgen05 kernel has a tile of 128 rows per SM: 10.7 ns
+    # grows with the rows, 3.5 ns for 1,000 keys and row in all (heads of 128).  The tcgen05 kernel has a tile of 128 rows per SM: 10.7 ns
     # for a key and round of tiles, and the pages' expansion, 0.12 ns for a key and key head.  So up to 24 rows of an SM in
     # every round of tiles, and 32 of every request's key head, the split form is the shorter.  Measured, split and tcgen05, 32 query and
-    # 8 key heads of 128: a request of 16 queries over 5,000 and 16,000 keys 22 and 60, 38 and 172 us; of 64 queries 45 and 61, 114 and 174; of
-    # 128 queries 72 and 62, 211 and 175; 16 requests of 8 and of 32 queries over 1,200 keys 24 and 43, 76 and 44 us.
+    # 8 key heads of 128: a request of 16 queries over 5,000 and 16,000 keys 22 and 60, 36 and 172 us; of 64 queries 43 and 61, 110 and 173; of
+    # 128 queries 69 and 62, 201 and 175; 16 requests of 8 and of 32 queries over 1,200 keys 23 and 42, 71 and 44 us.
     kv8_split_rows = (24, 32)
     # Where that kernel does not fit (float32, heads wider than 128, other pages) all requests run split, but those of more than 64 rows
     # whole where the device has plenty of rows and the keys are few, so that an item's beginning and end count.  Measured, split and whole,
-    # float32, 8 key heads of 128: 8 requests of 64 queries over 300 keys 53 and 38 us, of 1,024 over 1,200 keys 1,210 and 1,032, of 256 over
-    # 5,000 keys 1,512 and 1,826; one of 64 over 300 keys 16 and 30.
+    # float32, 8 key heads of 128: 8 requests of 64 queries over 300 keys 50 and 37 us, of 1,024 over 1,200 keys 1,122 and 1,009, of 256 over
+    # 5,000 keys 1,416 and 1,805; one of 64 over 300 keys 18 and 29.
     kv8_whole_rows, kv8_whole_keys = 64, 2048      # rows of an SM from which, keys up to which
 
     def _kv8_expand(self, pages, block_tables, cu_q, seq_lens, window, r, group, most, room, stream):
