@@ -603,24 +603,63 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
     asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
     const int tokens = min(C::NT, p.rows - n0);
-    // two rows of w (one output, if gated) per thread and turn
-    for (int i = blockIdx.z * C::THREADS + threadIdx.x; i < tokens * 64; i += splits * C::THREADS) {
-      const int token = i >> 6, pair = (i & 63) * 2, row = o0 + pair;
-      float a = 0.f, b = 0.f;
-      for (int r = 0; r < splits; ++r) {
-        uint32_t remote;
-        float2 f;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(mx_smem(mine + token * 128 + pair)), "r"(r));
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(f.x), "=f"(f.y) : "r"(remote) : "memory");
-        a += f.x;
-        b += f.y;
-      }
-      TO* to = out + (size_t)(n0 + token) * p.out_features;
+    // two rows of w (one output, if gated) per thread and turn, the ranks' numbers added in their order
+    const int step = splits * C::THREADS;
+    auto put = [&](int i, float2 sum) {
+      const int row = o0 + (i & 63) * 2;
+      TO* to = out + (size_t)(n0 + (i >> 6)) * p.out_features;
       if (GATED) {
-        if (row < p.w_rows) to[row >> 1] = from_f32<TO>(mx_gate<EPI>(a, b, p.unary));
+        if (row < p.w_rows) to[row >> 1] = from_f32<TO>(mx_gate<EPI>(sum.x, sum.y, p.unary));
       } else {
-        if (row < p.w_rows) to[row] = from_f32<TO>(mx_apply<EPI>(a, p.unary));
-        if (row + 1 < p.w_rows) to[row + 1] = from_f32<TO>(mx_apply<EPI>(b, p.unary));
+        if (row < p.w_rows) to[row] = from_f32<TO>(mx_apply<EPI>(sum.x, p.unary));
+        if (row + 1 < p.w_rows) to[row + 1] = from_f32<TO>(mx_apply<EPI>(sum.y, p.unary));
+      }
+    };
+    auto from = [&](int r) {
+      uint32_t remote;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(mx_smem(mine)), "r"(r));
+      return remote;
+    };
+    auto get = [](float2& f, uint32_t remote) {
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(f.x), "=f"(f.y) : "r"(remote) : "memory");
+    };
+    if constexpr (C::NT == 16) {                                        // one or two turns in all
+      for (int i = blockIdx.z * C::THREADS + threadIdx.x; i < tokens * 64; i += step) {
+        float2 sum = make_float2(0.f, 0.f);
+        for (int r = 0; r < splits; ++r) {
+          float2 f;
+          get(f, from(r) + i * 8);
+          sum.x += f.x;
+          sum.y += f.y;
+        }
+        put(i, sum);
+      }
+    } else {
+      // the numbers of four ranks and TURN turns are requested together (one by one: 128 rows of 1,024, shared by two, 7.0 us for 5.5)
+      constexpr int TURN = C::NT >= 64 ? 4 : 2;
+      for (int i0 = blockIdx.z * C::THREADS + threadIdx.x; i0 < tokens * 64; i0 += TURN * step) {
+        float2 sum[TURN];
+#pragma unroll
+        for (int u = 0; u < TURN; ++u) sum[u] = make_float2(0.f, 0.f);
+        for (int r0 = 0; r0 < splits; r0 += 4) {
+          float2 f[4][TURN];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (r0 + r >= splits) break;
+            const uint32_t remote = from(r0 + r);
+#pragma unroll
+            for (int u = 0; u < TURN; ++u) get(f[r][u], remote + min(i0 + u * step, tokens * 64 - 1) * 8);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (r0 + r >= splits) break;
+#pragma unroll
+            for (int u = 0; u < TURN; ++u) { sum[u].x += f[r][u].x; sum[u].y += f[r][u].y; }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < TURN; ++u)
+          if (i0 + u * step < tokens * 64) put(i0 + u * step, sum[u]);
       }
     }
     asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
@@ -635,15 +674,48 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
   }
 }
 
+// Clusters of s CTAs that find SMs at a time (33 of four, not 37: a cluster stays in one part of the device).
+template <typename K> static int mx_clusters(K kernel, cudaLaunchConfig_t cfg, int s) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = s;
+  cfg.gridDim.z = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+  return n;
+}
 template <typename C, int EPI, typename TO, typename TX>
-static int mx_launch(const CUtensorMap& xm, const CUtensorMap& wm, const MxProduct& p, int splits, int* err, cudaStream_t stream) {
+static int mx_launch(const CUtensorMap& xm, const CUtensorMap& wm, MxProduct p, int splits, int* err, cudaStream_t stream) {
   auto kernel = mx4_linear_kernel<C, EPI, TO, TX>;
   IFB_ALLOW_SMEM(kernel, C::SMEM);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.w_rows + 127) / 128, (p.rows + C::NT - 1) / C::NT, splits);
+  cfg.gridDim = dim3((p.w_rows + 127) / 128, (p.rows + C::NT - 1) / C::NT, 1);
   cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = stream;
+  const int stages = (p.k + MX_KSTAGE - 1) / MX_KSTAGE, tiles = cfg.gridDim.x * cfg.gridDim.y;
+  if (!splits) {
+    // The k range of a tile is shared by up to four CTAs, if all find an SM at once, in as many stages of a CTA and, for the sum, two to four more as are
+    // the fewest.  (8 rows, k = 4,096, on 1, 2, 3, 4 CTAs: 16 tiles 8.1, 6.4, 5.7 and 4.7 us, 36 tiles 8.0, 6.4, 5.9 and, in two rounds, 9.2, 48 tiles 8.4,
+    // 6.8, 11.5 and 10.2; 128 rows: 16 tiles 8.8, 7.3, 7.1, 6.3, 48 tiles 9.0, 7.9, 14.3, 13.3; k = 1,024, 48 tiles: 8 rows 3.8, 4.3, 4.3, 7.8.
+    // More than four leave SMs without one: 16 tiles of 128 rows, k = 2,048, eight 8.8.)
+    static int clusters[IFB_MAX_DEVICES][5] = {};
+    int dev = 0, least = stages;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= IFB_MAX_DEVICES) return IFB_ERR_ARG;
+    splits = 1;
+    for (int s = 4; s > 1; --s) {
+      int& fit = clusters[dev][s];
+      if (!fit) fit = 1 + mx_clusters(kernel, cfg, s);
+      const int cost = (stages + s - 1) / s + (s == 4 ? (C::NT == 32 ? 2 : 3) : C::NT <= 32 ? 2 : 4);
+      if (tiles < fit && cost < least) { splits = s; least = cost; }
+    }
+  }
+  if (splits < 1 || splits > 8 || splits > stages) return IFB_ERR_ARG;
+  p.per_split = (stages + splits - 1) / splits;
+  splits = (stages + p.per_split - 1) / p.per_split;                   // every CTA has a stage
+  cfg.gridDim.z = splits;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = splits;
@@ -994,19 +1066,7 @@ IFB_EXPORT int ifb_mx4_linear(const void* x, int x_dtype, long long x_row, void*
   const bool pair = nt ? nt == 256 : many;
   if (!nt || round) nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   if (nt < rows && nt < 128) return IFB_ERR_ARG;
-  const int stages = (k + MX_KSTAGE - 1) / MX_KSTAGE, tiles = (w_rows + 127) / 128 * ((rows + nt - 1) / nt);
-  // The k range of a tile is shared by the most CTAs, up to 8, that have two stages each and find an SM each; clusters of more
-  // than 4 leave SMs without one (16 tiles of 128 x 128, k = 2,048: 1, 4 and 8 CTAs per tile 5.9, 5.3 and 8.8 us; 32 tiles, k = 4,096: 1, 4, 6:
-  // 7.4, 4.9 to 5.3, 9.8; k = 1,024, four stages: 1, 2, 4: 2.9, 2.9, 3.4).
-  if (!splits) {
-    splits = 1;
-    for (int s = 4; s > 1; --s)
-      if (2 * s <= stages && tiles * s <= ifb_sm_count()) { splits = s; break; }
-  }
-  if (splits < 1 || splits > 8 || splits > stages) return IFB_ERR_ARG;
-  MxProduct p = {(const uint8_t*)x_scales, (const uint8_t*)w_scales, out, rows, k, w_rows, gated ? w_rows / 2 : w_rows, unary,
-                 (stages + splits - 1) / splits, x, x_row};
-  splits = (stages + p.per_split - 1) / p.per_split;                   // every CTA has a stage
+  const MxProduct p = {(const uint8_t*)x_scales, (const uint8_t*)w_scales, out, rows, k, w_rows, gated ? w_rows / 2 : w_rows, unary, 0, x, x_row};
   // the maps see pairs of bytes as one number of 16 bits: only widths and strides in bytes count
   const unsigned long long xd[2] = {(unsigned long long)k / 4, (unsigned long long)rows}, xs[1] = {(unsigned long long)k / 2};
   const unsigned long long wd[2] = {(unsigned long long)k / 4, (unsigned long long)w_rows}, ws[1] = {(unsigned long long)k / 2};
