@@ -10,10 +10,11 @@
 // integer instructions make two of them.  Keys stay so (q . (u - 127.5) = q . u - 127.5 sum(q), the second known per row);
 // for values 128 is taken off again: a sum over thousands of keys would lose what the offset swamps.
 //
-// Softmax: weights are 2^(score - m + 8) with a reference m per row that moves (and then rescales the sums) only when a score
-// exceeds it by 6 in the exponent, so that most tiles need no maximum over lanes; 2^14 is then the largest weight, and
-// half-precision numbers down to 2^-32 of it still count.  A weight enters the product times its page's step over the largest
-// step so far.  Sums are float32.
+// Softmax: weights are 2^(score - m + 8) with a reference m per row that moves (and then rescales the sums) only when a weight, times its
+// page's step over the largest step that the warp has met, exceeds it by 6 in the exponent, so that most tiles need no maximum
+// over lanes.  That product is what enters the second product: 2^14 is the largest, and half-precision numbers down to 2^-32 of it
+// still count, for steps up to 2^80 apart.  (A reference of the scores alone: rows that do not see a page of values 2^24 larger than
+// their own, but whose warp does, lose bits, and from 2^33 on are zero.)  Sums are float32.
 //
 // What bounds it: the integer pipe, for the bytes of keys and values (half of its time over a whole call), and the registers, with 128 of which four CTAs
 // fit on an SM: what does not have to stay in one over the loop is named anew or uniform (46.1 to 42.2 us in the third figure).  A call has some
@@ -79,11 +80,12 @@ struct Stream {
   uint32_t qf[NT][KS][2];
   float qscale[NT][2], qoff[NT][2];      // what turns a product into a number of real units: times qscale, and qoff
   int last[NT][2];                       // position of the row's query (NO_ROW: no such row)
-  // m: reference of the row's scores, finite (a score has to exceed m + 6 to move it, and a weight is 2^(score + (8 - m))); l, wsum: this lane's
-  // part of the sums of the weights, and of weights times steps
+  // m: reference of the row's scores, finite (`weigh`; a weight is 2^(score + (8 - m))); l, wsum: this lane's part of the sums of the weights,
+  // and of weights times steps
   float m[NT][2], l[NT][2], wsum[NT][2];
   float o[KS][NT][4];
   int v_ref;                             // exponent field that the sums of weighted values are in units of
+  static constexpr int SPREAD = 80;      // what a row's reference lies below its largest score at most, in log2, beside the 6
 
   __device__ __forceinline__ void reset() {
     v_ref = 0;
@@ -159,14 +161,20 @@ struct Stream {
       }
   }
   // vf: the exponent field of the values; 0 also for a page of NaN, whose scores are NaN where they are seen.
+  // A row's reference is that of its weights times their steps, in units of 2^v_ref: a score may exceed it by what its page's step lies below
+  // v_ref (by SPREAD at most), and when a page raises v_ref, the reference falls as much.  So a row keeps the bits of its products
+  // whatever steps the warp has met that the row does not see or gives no weight.
   __device__ __forceinline__ void weigh(float (&s)[NT][4], const Values<D>& v, int vf) {
+    const bool larger = vf > v_ref;                                     // uniform
+    const int below = min(max(v_ref - vf, 0), SPREAD);
+    const float lag = __int_as_float(0x4b400000 + below) - 12582906.f;  // below + 6
     bool up = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) up |= fmaxf(s[n][e], s[n][2 + e]) > m[n][e] + 6.f;
-    const bool larger = vf > v_ref;                                     // uniform
+      for (int e = 0; e < 2; ++e) up |= fmaxf(s[n][e], s[n][2 + e]) > m[n][e] + lag;
     if (__any_sync(0xffffffffu, up) || larger) {
+      const int raise = larger ? min(vf - v_ref, SPREAD) : 0;
       float fv = 1.f;
       if (larger) {
         fv = v_ref ? __uint_as_float((uint32_t)max(0, 127 + v_ref - vf) << 23) : 0.f;
@@ -177,11 +185,14 @@ struct Stream {
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(s[n][e], s[n][2 + e]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = fmaxf(mx, m[n][e]);
+          float mx = fmaxf(s[n][e], s[n][2 + e]), sum = l[n][e];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            sum += __shfl_xor_sync(0xffffffffu, sum, x);
+          }
+          const int room = max(0, min(raise, 214 - (int)(__float_as_uint(sum) >> 23)));      // the row's sum stays below 2^88
+          mx = fmaxf(mx - (lag - 6.f), m[n][e] - (float)room);
           f[e] = kv8_exp2(m[n][e] - mx);
           m[n][e] = mx;
           l[n][e] *= f[e];
