@@ -269,17 +269,23 @@ struct Stream {
     const float unit = kv8_step((uint32_t)v_ref);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      float less[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) {
           l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
           wsum[n][e] += __shfl_xor_sync(0xffffffffu, wsum[n][e], x);
         }
+        const int by = kv8_excess(l[n][e], wsum[n][e], (float)v_ref);
+        less[e] = __uint_as_float((uint32_t)(127 - by) << 23);
+        l[n][e] *= less[e];
+        m[n][e] += (float)by;
+      }
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][n][j] = fmaf(o[i][n][j], 16777216.f, 0.5f * wsum[n][j & 1]) * unit;
+        for (int j = 0; j < 4; ++j) o[i][n][j] = fmaf(o[i][n][j], 16777216.f, 0.5f * wsum[n][j & 1]) * less[j & 1] * unit;
     }
   }
 };

@@ -199,6 +199,13 @@ __device__ __forceinline__ int kv8_value_field(int vf) { return vf == 255 ? 0 : 
 
 __device__ __forceinline__ void kv8_store_pair(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
 __device__ __forceinline__ void kv8_store_pair(bf16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
+// What a row's reference is raised by at the end (0: as it is).  Sums of weighted values are 127.5 wsum 2^(unit - 133) at most: from 2^118 on the
+// weights' sum l is brought to [2^-10, 2^-9), which leaves the joins room.  (Raised always, a reference with a fraction would be
+// rounded once more.)
+__device__ __forceinline__ int kv8_excess(float l, float wsum, float unit) {
+  const int at = (int)(__float_as_uint(wsum) >> 23) - 127;
+  return (float)at + unit >= 244.f ? min((int)(__float_as_uint(l) >> 23), 243) - 117 : 0;
+}
 __device__ __forceinline__ float kv8_ratio(float o, float l) { return l == 0.f ? 0.f : o / l; }
 
 // --------------------------------------------------------------------------------------------

@@ -363,7 +363,10 @@ struct Stream {
           l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
           wsum[n][e] += __shfl_xor_sync(0xffffffffu, wsum[n][e], x);
         }
-        unit[e] = r[n][e] == -INFINITY ? 0.f : kv8_exp2(r[n][e] - 133.f);
+        const int by = kv8_excess(l[n][e], wsum[n][e], r[n][e]);
+        unit[e] = r[n][e] == -INFINITY ? 0.f : kv8_exp2(r[n][e] - 133.f - (float)by);
+        l[n][e] *= __uint_as_float((uint32_t)(127 - by) << 23);
+        m[n][e] += (float)by;
       }
 #pragma unroll
       for (int i = 0; i < KS; ++i)
