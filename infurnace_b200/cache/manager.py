@@ -114,10 +114,11 @@ class CacheLayout:
 
 class CacheManager:
     def __init__(self, plan: ModelPlan, page_size: int, num_pages, max_requests: int,
-                 dtype=None, device=None, allocate_tensors: bool = True, cache_format: str = "dtype"):
+                 dtype=None, device=None, allocate_tensors: bool = True, cache_format: str = "dtype", room_bytes: int = 0):
         """``num_pages``: pages of every key/value group (an int), or a dict from group key
         to its count.  ``allocate_tensors`` False gives a manager that only does the
-        accounting (tests without a device)."""
+        accounting (tests without a device).  ``room_bytes``: of the room that all 8-bit entries share for
+        what attention expands of their pages (0: none)."""
         if page_size < 1:
             raise CacheError("page_size must be positive")
         if max_requests < 1:
@@ -146,6 +147,7 @@ class CacheManager:
         self._lives = 0
         if allocate_tensors:
             import torch
+            room = torch.empty(room_bytes, dtype=torch.uint8, device=device) if room_bytes else None
             for g in self.kv_groups:
                 st = g.need.streams
                 for cid in g.cache_ids:
@@ -154,6 +156,7 @@ class CacheManager:
                         if not g.uniform or len(st) != 2:
                             raise CacheError(f"cache entry {cid}: pages of 8 bits hold keys and values of one shape")
                         t = Kv8Pages.empty(g.pool.num_pages, st[0].heads, page_size, st[0].width, device)
+                        t.room, t.shared = room, False
                         g.tensors[cid] = t
                         g.streams[cid] = {x.name: t.codes[:, i] for i, x in enumerate(st)}
                     elif g.uniform:

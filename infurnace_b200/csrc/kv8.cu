@@ -223,10 +223,13 @@ kv8_values_kernel(const int8_t* codes, const uint8_t* exponents, T* out, long lo
 }
 
 // The pages of the requests with more than `above` score rows as bfloat16 pages, for a kernel that reads those: the pages that a
-// request's keys lie in, one after the other over all such requests, and a table of them.  Exact, but for a block of NaN:
+// request's queries see, one after the other over all such requests, and a table of them.  Exact, but for a block of NaN:
 // either kind's makes the page's keys NaN and its values 0, so that rows that do not see the page keep their numbers (a weight
 // of 0 times NaN would not be 0) and rows that see it are NaN.  Grid (pages of a request, 2 kinds, requests).  Bound by memory: a byte read and
 // two written for each number: 2,000 pages of 16 tokens of 8 heads of 128 35 us, 5.6 TB/s.
+__device__ __forceinline__ int kv8_first_page(int L, int q_len, int window, int page_size) {
+  return window > 0 ? max(0, L - q_len - window + 1) / page_size : 0;
+}
 __global__ void __launch_bounds__(256)
 kv8_expand_kernel(const int8_t* codes, const uint8_t* exponents, const int* tables, int table_stride, const int* cu_q, const int* seq_lens, bf16* out,
                   int* out_tables, int out_pages, int heads, int group, int page_size, int dim, int window, int above) {
@@ -234,18 +237,19 @@ kv8_expand_kernel(const int8_t* codes, const uint8_t* exponents, const int* tabl
   ifb_pdl_wait();
   ifb_pdl_trigger();
   const int r = blockIdx.z, kind = blockIdx.y, p = blockIdx.x;
-  const int q_len = cu_q[r + 1] - cu_q[r], L = seq_lens[r];
-  if (q_len * group <= above || p * page_size >= L) return;
-  if (window > 0 && (p + 1) * page_size <= L - q_len - window + 1) return;
+  const int q_len = cu_q[r + 1] - cu_q[r], L = seq_lens[r], first = kv8_first_page(L, q_len, window, page_size);
+  if (q_len * group <= above || p * page_size >= L || p < first) return;
   if (threadIdx.x < 32) {
     int sum = 0;
-    for (int i = threadIdx.x; i < r; i += 32)
-      if ((cu_q[i + 1] - cu_q[i]) * group > above) sum += (max(0, seq_lens[i]) + page_size - 1) / page_size;
+    for (int i = threadIdx.x; i < r; i += 32) {
+      const int n = cu_q[i + 1] - cu_q[i], l = max(0, seq_lens[i]);
+      if (n * group > above) sum += (l + page_size - 1) / page_size - kv8_first_page(l, n, window, page_size);
+    }
     sum = __reduce_add_sync(0xffffffffu, sum);
     if (threadIdx.x == 0) first_sum = sum;
   }
   __syncthreads();
-  const int to = first_sum + p;
+  const int to = first_sum + p - first;
   if (to >= out_pages) return;                                          // (more keys than the caller said)
   const int page = tables[(size_t)r * table_stride + p];
   if (kind == 0 && threadIdx.x == 0) out_tables[(size_t)r * gridDim.x + p] = to;

@@ -6,9 +6,10 @@ from typing import Optional
 
 import torch
 
-from ..cache import CacheManager
+from ..cache import CacheLayout, CacheManager
 from ..errors import ModelConfigError
 from ..config.specs import AttentionSpec, DenseMLPSpec, GatedMLPSpec, KVCacheNeed, PagedCacheNeed
+from ..kernels.low_bits import kv8_room_bytes
 from ..models import plan_for, read_config
 from ..parts import DecoderModel, Runtime
 from ..weights.loader import load_weights
@@ -77,8 +78,9 @@ def build_runner(model_dir: Optional[str], options: EngineOptions, kernels=None,
     num_pages = options.num_pages
     if num_pages is None:
         num_pages = default_num_pages(plan, options, dtype, runtime.device, max_len)
+    room = room_bytes(plan, options, dtype, max_len, num_pages) if getattr(kernels, "attention_tc", False) else 0
     cache = CacheManager(plan, options.page_size, num_pages, options.max_num_seqs, dtype=dtype, device=runtime.device,
-                         cache_format=options.cache_format)
+                         cache_format=options.cache_format, room_bytes=room)
     runner = ModelRunner(model, cache, runtime, options.max_num_batched_tokens, max_len)
     return config, plan, runner
 
@@ -113,10 +115,19 @@ def check_plan(plan, options) -> None:
                         raise ModelConfigError(f"cache_format int8: head_dim is a multiple of 16 up to 256, not {mixer.head_dim}")
 
 
+def room_bytes(plan, options, dtype, max_len, num_pages) -> int:
+    """Bytes of the room for expanded 8-bit pages that an engine's layers share (``num_pages``: as in the cache manager)."""
+    if options.cache_format != "int8":
+        return 0
+    each = -(-max_len // options.page_size)
+    return max((kv8_room_bytes(num_pages[key] if isinstance(num_pages, dict) else num_pages, options.max_num_seqs, each,
+                               need.streams[0].heads, options.page_size, need.streams[0].width, dtype)
+                for key, (need, _) in CacheLayout(plan).kv.items()), default=0)
+
+
 def default_num_pages(plan, options, dtype, device, max_len) -> int:
     """Pages for ``max_num_seqs`` sequences of ``max_model_len``, capped by the share of
-    free device memory that ``memory_fraction`` allows."""
-    from ..cache import CacheLayout
+    free device memory that ``memory_fraction`` allows, the room for expanded 8-bit pages counted."""
     layout = CacheLayout(plan)
     per_page = 0
     esize = 1 if options.cache_format == "int8" else torch.empty((), dtype=dtype).element_size()
@@ -127,6 +138,8 @@ def default_num_pages(plan, options, dtype, device, max_len) -> int:
         return 1
     if device.type == "cuda":
         free, _ = torch.cuda.mem_get_info(device)
-        fit = int(free * options.memory_fraction) // per_page
+        free = int(free * options.memory_fraction)
+        room = [room_bytes(plan, options, dtype, max_len, n) for n in (0, 1, want)]
+        fit = max((free - room[2]) // per_page, (free - room[0]) // (per_page + room[1] - room[0]))
         want = max(1, min(want, fit))
     return want

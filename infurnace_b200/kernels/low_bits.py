@@ -108,7 +108,15 @@ class Kv8Pages:
     [pages, 2, kv_heads], one for the keys (or values) of a page and head.
 
     A number is (code + 1/2) step with step = 2^(exponent - 133); ``exponent`` is the exponent field of the block's largest
-    number as a float32, 0 where all are zero (the values are then 0), 255 where one is infinite or NaN (the values are NaN)."""
+    number as a float32, 0 where all are zero (the values are then 0), 255 where one is infinite or NaN (the values are NaN).
+
+    ``room``: None, or a uint8 tensor beside the codes in which ``kv8_attention`` lays out the pages that it expands, in place of
+    memory of the allocator's for each call (and, within a recording, of the graph's own pool for each graph).  Several ``Kv8Pages``
+    may have one room, as an engine's layers have, if the calls over them, and the replays of recorded ones, follow one another.
+    A call that would need more than the room takes another form.  ``shared``: whether a page may be in the tables of two requests, or
+    twice in one; where none is (False), there are no more pages to expand than the pool has."""
+
+    room, shared = None, True
 
     def __init__(self, codes, exponents):
         if codes.dtype != torch.int8 or codes.dim() != 5 or codes.shape[1] != 2 or not codes.is_contiguous() or codes.data_ptr() % 16:
@@ -128,6 +136,21 @@ class Kv8Pages:
     def empty(cls, pages, kv_heads, page_size, head_dim, device="cuda"):
         return cls(torch.zeros((pages, 2, kv_heads, page_size, head_dim), dtype=torch.int8, device=device),
                    torch.zeros((pages, 2, kv_heads), dtype=torch.uint8, device=device))
+
+
+KV8_EXPAND_BYTES = 4 << 30       # room for expanded pages that a call takes at most
+
+
+def kv8_room_bytes(pages, requests, pages_each, kv_heads, page_size, head_dim, dtype):
+    """Bytes of a room (``Kv8Pages.room``) with which no call over a pool of ``pages`` pages, none of which two requests share, is
+    short of it: for so many requests of so many pages at most.  0 where no call expands pages of these sizes."""
+    if dtype != torch.bfloat16 or head_dim > 128 or page_size not in (16, 32, 64):
+        return 0
+    return min(KV8_EXPAND_BYTES, _expanded_bytes(pages, requests * pages_each, kv_heads, page_size, head_dim))
+
+
+def _expanded_bytes(pages, entries, kv_heads, page_size, head_dim):
+    return pages * 4 * kv_heads * page_size * head_dim + -(-entries // 64) * 256
 
 
 class LowBitKernels:
@@ -329,7 +352,7 @@ class LowBitKernels:
                     self.scratch_generation += 1
         return held["graph" if capturing else stream][2:4]
 
-    kv8_expand_bytes = 4 << 30       # room for expanded pages that a call may take
+    kv8_expand_bytes = KV8_EXPAND_BYTES
     # Which form attends to requests of more than 16 score rows (queries x query heads of a key head) in bfloat16.  The split form's time
     # grows with the rows, 3.5 ns for 1,000 keys and row in all (heads of 128).  The tcgen05 kernel has a tile of 128 rows per SM: 10.7 ns
     # for a key and round of tiles, and the pages' expansion, 0.12 ns for a key and key head.  So up to 24 rows of an SM in
@@ -343,11 +366,24 @@ class LowBitKernels:
     # 5,000 keys 1,416 and 1,805; one of 64 over 300 keys 18 and 29.
     kv8_whole_rows, kv8_whole_keys = 64, 2048      # rows of an SM from which, keys up to which
 
+    def _kv8_room_size(self, pages):
+        """Bytes that the pages which a call expands may take."""
+        room = pages.room
+        if room is None:
+            return self.kv8_expand_bytes
+        if room.dtype != torch.uint8 or room.dim() != 1 or not room.is_contiguous() or room.data_ptr() % 128 or room.get_device() != pages._index:
+            raise KernelError("kv8_attention: a room is uint8 [bytes], contiguous, on 128 bytes, on the pages' device")
+        return room.numel()
+
     def _kv8_expand(self, pages, block_tables, cu_q, seq_lens, window, r, group, most, room, stream):
         """The pages of the requests with more than 16 score rows as bfloat16 (exact), and tables of them."""
         kv_heads, ps, dim = pages.kv_heads, pages.page_size, pages.head_dim
-        wide = torch.empty((room, 2, kv_heads, ps, dim), dtype=torch.bfloat16, device=pages.codes.device)
-        tables = torch.empty((r, most), dtype=torch.int32, device=pages.codes.device)
+        held = pages.room
+        if held is None:
+            held = torch.empty(_expanded_bytes(room, r * most, kv_heads, ps, dim), dtype=torch.uint8, device=pages.codes.device)
+        split = room * 4 * kv_heads * ps * dim
+        wide = held[:split].view(torch.bfloat16).view(room, 2, kv_heads, ps, dim)
+        tables = held[split:split + 4 * r * most].view(torch.int32).view(r, most)
         self.launches += 1
         status = self._kv8_lib().ifb_kv8_expand(*pages._at, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(), seq_lens.data_ptr(),
                                                 wide.data_ptr(), tables.data_ptr(), room, r, most, kv_heads, group, ps, dim, window, 16, stream)
@@ -362,7 +398,8 @@ class LowBitKernels:
         (``window`` 0: from 0); request r has the rows cu_q[r] .. cu_q[r + 1] - 1 and ``seq_lens[r]`` keys, these queries' own
         among them.  A row that sees no key becomes zero.  No request has more than ``max_q_len`` queries or ``max_seq_len``
         keys, none fewer than ``min_q_len`` queries; ``exact_lens``: some request has ``max_q_len``, and ``q`` no other rows than
-        theirs, which bounds how many are long."""
+        theirs, which bounds how many are long.  Numbers of queries, keys and values are below 2^100 in size, or infinite or NaN
+        (which the rows that see them become): sums of larger ones may overflow."""
         code = _CODES.get(q.dtype)
         shape, pitch, index = q.shape, q.stride(), pages._index
         n, heads, dim = shape if len(shape) == 3 else (0, 0, 0)
@@ -397,7 +434,9 @@ class LowBitKernels:
                 # (a long request has more than 16 score rows)
                 most = -(-max_seq_len // pages.page_size)
                 room = most * (self.long_requests(n, r, group, max_q_len, min_q_len) if exact_lens else min(r, n // (16 // group + 1)))
-                tc = room * pages.page_size * kv_heads * dim * 4 <= self.kv8_expand_bytes
+                if not pages.shared:
+                    room = min(room, pages.pages)
+                tc = _expanded_bytes(room, r * most, kv_heads, pages.page_size, dim) <= self._kv8_room_size(pages)
         if tc:
             wide, wide_tables = self._kv8_expand(pages, block_tables, cu_q, seq_lens, window, r, group, most, room, stream)
             rows = 16
