@@ -74,6 +74,7 @@ def build_runner(model_dir: Optional[str], options: EngineOptions, kernels=None,
         weights = DeviceRandomWeights(plan, random[1], dtype, runtime.device, kernels, store_dtype=parse_dtype(random[2]))
     model = DecoderModel(plan, weights, runtime)
     del weights
+    runtime.share_row_room(max(options.max_num_batched_tokens, options.max_num_seqs))
     max_len = min(options.max_model_len or plan.max_positions, plan.max_positions)
     num_pages = options.num_pages
     if num_pages is None:

@@ -31,7 +31,13 @@ class Mx4Matrix:
 
     ``codes`` uint8 [rows, k / 2], element 2 i in the low half of a byte; ``scales`` uint8, in tiles of 128 rows x 128 of k as
     the tensor core takes them.  ``gated``: the rows are pairs (gate row i, up row i) of a matrix that had all gate rows before
-    all up rows, which is the order that the gated epilogues of a product want."""
+    all up rows, which is the order that the gated epilogues of a product want.
+
+    ``room``: None, or a uint8 tensor beside the codes for the rows that a product with the matrix rounds first (``row_bytes`` of
+    them), in place of memory kept per stream (and, within a recording, of the graph's own pool for each graph).  Several matrices may
+    have one room, as an engine's have, if the products with them, and the replays of recorded ones, follow one another."""
+
+    _room, _room_at = None, (0, 0)
 
     def __init__(self, codes, scales, rows, k, gated=False):
         if codes.dtype != torch.uint8 or codes.shape != (rows, k // 2) or not codes.is_contiguous() or codes.data_ptr() % 16:
@@ -49,6 +55,22 @@ class Mx4Matrix:
         if rows < 1 or k < MX4_BLOCK or k % MX4_BLOCK:
             raise KernelError(f"Mx4Matrix: {rows} rows of {k}: rows are positive and k is a multiple of {MX4_BLOCK}")
         return -(-rows // 256) * 2 * -(-k // 128) * 512
+
+    @property
+    def room(self):
+        return self._room
+
+    @room.setter
+    def room(self, room):
+        if room is not None and (room.dtype != torch.uint8 or room.dim() != 1 or not room.is_contiguous() or room.data_ptr() % 256
+                                 or room.device != self.codes.device):
+            raise KernelError("Mx4Matrix: a room is uint8 [bytes], contiguous, on 256 bytes, beside the codes")
+        self._room, self._room_at = room, (0, 0) if room is None else (room.data_ptr(), room.numel())
+
+    @classmethod
+    def row_bytes(cls, rows, k):
+        """Bytes of a room for ``rows`` rows of ``k`` numbers: codes to a multiple of 256 bytes, then scales."""
+        return -(-rows * k // 512) * 256 + cls.scale_bytes(rows, k)
 
     @classmethod
     def empty(cls, rows, k, device="cuda", gated=False):
@@ -209,8 +231,13 @@ class LowBitKernels:
             raise KernelError("mx4_matrix: w is [rows, k], a gated one of an even number of rows")
         return self.mx4_quantize(w, Mx4Matrix.empty(w.shape[0], w.shape[1], w.device, gated))
 
-    def _mx4_room(self, stream, size, device):
-        """Address of room for rounded rows: of a stream each, whose launches follow one another; memory of its own in a recording."""
+    def _mx4_room(self, w, stream, size):
+        """Address of room for rounded rows: the matrix's, if it suffices; else of a stream each, whose launches follow one another, and
+        memory of its own in a recording."""
+        at, held = w._room_at
+        if held >= size:
+            return at
+        device = w.codes.device
         if _capturing():
             held = self._mx4_recorded = torch.empty(size, dtype=torch.uint8, device=device)      # the graph's own pool keeps it for its replays
             return held.data_ptr()
@@ -255,9 +282,8 @@ class LowBitKernels:
             if n <= self._mx4_round_rows[x_code]:
                 rows = (x.data_ptr(), x_code, pitch, 0, 0)
             else:
-                codes = -(-n * k // 512) * 256                             # half a byte an element, to a multiple of 256
-                room = self._mx4_room(_raw_stream(index), codes + Mx4Matrix.scale_bytes(n, k), w.codes.device)
-                rows = (x.data_ptr(), x_code, pitch, room, room + codes)
+                room = self._mx4_room(w, _raw_stream(index), Mx4Matrix.row_bytes(n, k))
+                rows = (x.data_ptr(), x_code, pitch, room, room + -(-n * k // 512) * 256)
         self.launches += 1 if rows[1] < 0 or n <= self._mx4_round_rows[rows[1]] else 2
         self._err_armed = True
         status = lib.ifb_mx4_linear(*rows, *w._at, out.data_ptr(), code, n, k, w.rows, epi, nt, splits, self._dev_err_at, _raw_stream(index))

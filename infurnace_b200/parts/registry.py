@@ -33,7 +33,7 @@ product that reads it can multiply its rows by r at the end: no kernel runs for 
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Any, Dict
 
 _PARTS: Dict[type, Any] = {}
@@ -103,7 +103,20 @@ class Runtime:
     act_dtype: Any
     kernels: Any
     weight_format: str = "stored"      # "mx4": the matrices that parts pass through ``matrix`` are kept in 4 bits
+    matrices: list = field(default_factory=list)      # those
 
     def matrix(self, w, gated=False):
         """A matrix as the products take it: the tensor, or its 4-bit form (``gated``: gate rows, then up rows)."""
-        return self.kernels.mx4_matrix(w, gated=gated) if self.weight_format == "mx4" else w
+        if self.weight_format != "mx4":
+            return w
+        self.matrices.append(self.kernels.mx4_matrix(w, gated=gated))
+        return self.matrices[-1]
+
+    def share_row_room(self, rows):
+        """One room for what products with the 4-bit matrices round of up to ``rows`` rows."""
+        sizes = [m.row_bytes(rows, m.k) for m in self.matrices if hasattr(m, "row_bytes")]
+        if sizes:
+            import torch
+            room = torch.empty(max(sizes), dtype=torch.uint8, device=self.device)
+            for m in self.matrices:
+                m.room = room
