@@ -9,6 +9,7 @@ from __future__ import annotations
 from ctypes import c_char_p, c_int, c_longlong, c_void_p
 
 import struct
+import threading
 
 import torch
 
@@ -178,6 +179,9 @@ def _expanded_bytes(pages, entries, kv_heads, page_size, head_dim):
 class LowBitKernels:
     """The calls over 4-bit matrices; mixed into the kernel set, which gives streams, counters and the error word."""
 
+    # Held by a call of several launches over one room, or of memory kept per stream, until the last is launched: the library's calls let
+    # other threads run, and one on the same stream would write the room in between.
+    _low_bit_lock = threading.RLock()
     _mx4 = None
 
     def _mx4_lib(self):
@@ -282,14 +286,19 @@ class LowBitKernels:
             if n <= self._mx4_round_rows[x_code]:
                 rows = (x.data_ptr(), x_code, pitch, 0, 0)
             else:
-                room = self._mx4_room(w, _raw_stream(index), Mx4Matrix.row_bytes(n, k))
-                rows = (x.data_ptr(), x_code, pitch, room, room + -(-n * k // 512) * 256)
-        self.launches += 1 if rows[1] < 0 or n <= self._mx4_round_rows[rows[1]] else 2
+                with self._low_bit_lock:
+                    room = self._mx4_room(w, _raw_stream(index), Mx4Matrix.row_bytes(n, k))
+                    self._mx4_product(lib, (x.data_ptr(), x_code, pitch, room, room + -(-n * k // 512) * 256), w, out, code, n, k, epi, nt, splits, 2)
+                return out
+        self._mx4_product(lib, rows, w, out, code, n, k, epi, nt, splits, 1)
+        return out
+
+    def _mx4_product(self, lib, rows, w, out, code, n, k, epi, nt, splits, launches):
+        self.launches += launches
         self._err_armed = True
-        status = lib.ifb_mx4_linear(*rows, *w._at, out.data_ptr(), code, n, k, w.rows, epi, nt, splits, self._dev_err_at, _raw_stream(index))
+        status = lib.ifb_mx4_linear(*rows, *w._at, out.data_ptr(), code, n, k, w.rows, epi, nt, splits, self._dev_err_at, _raw_stream(w._index))
         if status:
             self._low_bit_status(status, "mx4_linear")
-        return out
 
     # ------------------------------------------------------------------ keys and values of 8 bits
     _kv8 = None
@@ -463,30 +472,31 @@ class LowBitKernels:
                 if not pages.shared:
                     room = min(room, pages.pages)
                 tc = _expanded_bytes(room, r * most, kv_heads, pages.page_size, dim) <= self._kv8_room_size(pages)
-        if tc:
-            wide, wide_tables = self._kv8_expand(pages, block_tables, cu_q, seq_lens, window, r, group, most, room, stream)
-            rows = 16
-        # score rows up to which a request runs split
-        limit = min(rows, 64) if n * heads > self.kv8_whole_rows * self.sm_count and max_seq_len <= self.kv8_whole_keys else rows
-        nt = 1 if rows <= 8 or dim > 128 or tc and group <= 8 else 2      # (beside prompts the short requests decode)
-        fixed = (q.data_ptr(), code, pitch[0], *pages._at, block_tables.data_ptr(), table_pitch[0], cu_q.data_ptr(), seq_lens.data_ptr(),
-                 out.data_ptr())
-        sizes = (r, heads, kv_heads, pages.page_size, dim, window, max_q_len)
-        status = 0
-        if least <= limit:
-            tiles = -(-limit // (8 * nt))
-            items = min(r * tiles, r + n * group // (8 * nt)) * kv_heads
-            self.launches += 1
-            status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, *self._kv8_scratch(stream, lib.scratch_floats[nt], r * tiles * kv_heads), *sizes, 0, limit,
-                                                     tiles, nt, 0, items, stream, scale))
-        if rows > limit and not status:
-            self.launches += 1
-            status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, 0, 0, *sizes, limit + 1, (1 << 31) - 1, 1, nt, 1, 0, stream, scale))
-        if status:
-            self._low_bit_status(status, "kv8_attention")
-        if tc:
-            at, step, block = wide.data_ptr(), wide.stride(0), 2 * kv_heads * pages.page_size * dim
-            self._attention_tc_streams(q.as_strided((n, heads * dim), (pitch[0], 1)), heads, kv_heads, 1, dim, dim, (at, step, pages.page_size),
-                                       (at + block, step, pages.page_size), room, wide_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r,
-                                       2, None, None, kind=0)
+        with self._low_bit_lock:
+            if tc:
+                wide, wide_tables = self._kv8_expand(pages, block_tables, cu_q, seq_lens, window, r, group, most, room, stream)
+                rows = 16
+            # score rows up to which a request runs split
+            limit = min(rows, 64) if n * heads > self.kv8_whole_rows * self.sm_count and max_seq_len <= self.kv8_whole_keys else rows
+            nt = 1 if rows <= 8 or dim > 128 or tc and group <= 8 else 2      # (beside prompts the short requests decode)
+            fixed = (q.data_ptr(), code, pitch[0], *pages._at, block_tables.data_ptr(), table_pitch[0], cu_q.data_ptr(), seq_lens.data_ptr(),
+                     out.data_ptr())
+            sizes = (r, heads, kv_heads, pages.page_size, dim, window, max_q_len)
+            status = 0
+            if least <= limit:
+                tiles = -(-limit // (8 * nt))
+                items = min(r * tiles, r + n * group // (8 * nt)) * kv_heads
+                self.launches += 1
+                status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, *self._kv8_scratch(stream, lib.scratch_floats[nt], r * tiles * kv_heads), *sizes, 0, limit,
+                                                         tiles, nt, 0, items, stream, scale))
+            if rows > limit and not status:
+                self.launches += 1
+                status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, 0, 0, *sizes, limit + 1, (1 << 31) - 1, 1, nt, 1, 0, stream, scale))
+            if status:
+                self._low_bit_status(status, "kv8_attention")
+            if tc:
+                at, step, block = wide.data_ptr(), wide.stride(0), 2 * kv_heads * pages.page_size * dim
+                self._attention_tc_streams(q.as_strided((n, heads * dim), (pitch[0], 1)), heads, kv_heads, 1, dim, dim, (at, step, pages.page_size),
+                                           (at + block, step, pages.page_size), room, wide_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r,
+                                           2, None, None, kind=0)
         return out
