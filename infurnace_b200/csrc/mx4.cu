@@ -81,7 +81,7 @@ template <> struct MxSixteen<float> {
 // at once (a large matrix: one row per thread is a load's latency per CTA of little work).  Bound by memory: 24,576 x 4,096 of bfloat16 38 us,
 // 6.7 TB/s, and the way back 40 us, 6.4 TB/s.
 // early: the next kernel may begin at once.  The product that rounds its rows with this kernel reads them behind its wait; but what may become a
-// product's matrix is read before that wait, so nothing may begin ahead of these writes but mx4_written_kernel.
+// product's matrix is read before that wait, so nothing may begin ahead of these writes but mx4_written_kernel (nor ahead of other kernels' writes: ifb_mx4_written).
 template <typename T, int PER>
 __global__ void __launch_bounds__(256)
 mx4_quantize_kernel(const T* x, long long row_stride, uint8_t* codes, uint8_t* scales, int rows, int k, int gated_rows, int early) {
@@ -179,6 +179,8 @@ __global__ void mx4_written_kernel() {
   ifb_pdl_trigger();
 }
 static int mx_written(cudaStream_t stream) { return ifb_launch(mx4_written_kernel, dim3(1), dim3(32), 0, stream); }
+// For matrices that other kernels wrote.
+IFB_EXPORT int ifb_mx4_written(void* stream) { return mx_written((cudaStream_t)stream); }
 
 static int mx_sizes(int rows, int k, int gated) {
   if (rows < 1 || k < MX_BLOCK || k % MX_BLOCK || (gated && (rows & 1))) return IFB_ERR_SIZE;

@@ -34,6 +34,9 @@ class Mx4Matrix:
     the tensor core takes them.  ``gated``: the rows are pairs (gate row i, up row i) of a matrix that had all gate rows before
     all up rows, which is the order that the gated epilogues of a product want.
 
+    A product asks for its matrix before the kernel ahead of it in the stream has ended.  ``mx4_quantize`` and ``from_parts`` take care
+    of that; who writes ``codes`` or ``scales`` in another way calls :meth:`written` on that stream before the next product.
+
     ``room``: None, or a uint8 tensor beside the codes for the rows that a product with the matrix rounds first (``row_bytes`` of
     them), in place of memory kept per stream (and, within a recording, of the graph's own pool for each graph).  Several matrices may
     have one room, as an engine's have, if the products with them, and the replays of recorded ones, follow one another."""
@@ -94,7 +97,18 @@ class Mx4Matrix:
         padded = torch.zeros((rt * 128, kt * 4), dtype=torch.uint8, device=codes.device)
         padded[:rows, :k // MX4_BLOCK] = scales
         tiles = padded.view(rt, 4, 32, kt, 4).permute(0, 3, 2, 1, 4).contiguous().view(size)
-        return cls(codes.contiguous(), tiles, rows, k, gated)
+        return cls(codes.contiguous(), tiles, rows, k, gated).written()
+
+    def written(self):
+        """What the current stream has written so far into ``codes`` and ``scales`` is there before a product of that stream asks
+        for it.  Returns the matrix."""
+        if self._index >= 0:
+            lib = load_library("mx4")
+            lib.ifb_mx4_written.argtypes = [c_void_p]
+            status = lib.ifb_mx4_written(_raw_stream(self._index))
+            if status:
+                LowBitKernels._low_bit_status(status, "Mx4Matrix.written")
+        return self
 
     def parts(self):
         """(codes [rows, k / 2], scales [rows, k / 32]) in the order of the rows: what ``from_parts`` takes."""
