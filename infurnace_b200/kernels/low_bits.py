@@ -373,17 +373,18 @@ class LowBitKernels:
             lib.ifb_kv8_attention.argtypes = [c_char_p]
             lib.ifb_kv8_attention_scratch.restype = c_longlong
             lib.ifb_kv8_attention_scratch.argtypes = [c_int]
-            lib.scratch_floats = {nt: int(lib.ifb_kv8_attention_scratch(nt)) for nt in range(1, lib.ifb_kv8_attention_tiles() + 1)}
-            for floats in lib.scratch_floats.values():
-                if floats < 0:
-                    raise KernelError(f"kv8_attention: the device cannot be asked for its size (error {floats})")
+            floats = [int(lib.ifb_kv8_attention_scratch(nt)) for nt in range(1, lib.ifb_kv8_attention_tiles() + 1)]
+            if min(floats) < 0:
+                raise KernelError(f"kv8_attention: the device cannot be asked for its size (error {min(floats)})")
+            lib.most_floats = max(floats)
             libs[(dim, dtype)] = lib
         return lib
 
     def _kv8_scratch(self, stream, floats, counters):
         """Addresses of (sums, counters) of the split form: of a stream each, and one pair for recorded graphs, whose replays follow
         one another.  The counters are zero between launches; a recording could not clear new ones, so what it uses is made
-        before, with the first call outside of one; what an older recording uses is kept when room grows."""
+        before, with the first call outside of one; what an older recording uses is kept when room grows.  The counters' number goes by
+        powers of two: new ones make recorded steps stale."""
         held = self.__dict__.setdefault("_kv8_held", {})
         capturing = _capturing()
         for key in (("graph",) if capturing else (stream, "graph")):
@@ -391,7 +392,7 @@ class LowBitKernels:
             if have is None or have[0] < floats or have[1] < counters:
                 if capturing:
                     raise KernelError("kv8_attention: run the call once before it is recorded into a graph")
-                floats_, counters_ = max(floats, have[0] if have else 0), max(counters, have[1] if have else 4096)
+                floats_, counters_ = max(floats, have[0] if have else 0), max(1 << (counters - 1).bit_length(), have[1] if have else 4096)
                 sums = torch.empty(floats_, dtype=torch.float32, device="cuda")
                 zeros = torch.zeros(counters_, dtype=torch.int32, device="cuda")
                 held[key] = (floats_, counters_, sums.data_ptr(), zeros.data_ptr(), sums, zeros)
@@ -501,7 +502,7 @@ class LowBitKernels:
                 tiles = -(-limit // (8 * nt))
                 items = min(r * tiles, r + n * group // (8 * nt)) * kv_heads
                 self.launches += 1
-                status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, *self._kv8_scratch(stream, lib.scratch_floats[nt], r * tiles * kv_heads), *sizes, 0, limit,
+                status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, *self._kv8_scratch(stream, lib.most_floats, r * tiles * kv_heads), *sizes, 0, limit,
                                                          tiles, nt, 0, items, stream, scale))
             if rows > limit and not status:
                 self.launches += 1

@@ -75,3 +75,22 @@ def test_threads_on_one_stream_do_not_share_a_room_at_a_time(monkeypatch, own):
     for t in threads:
         t.join()
     assert library.calls == 24 and library.broken == 0
+
+
+class Scratch(LowBitKernels):
+    scratch_generation = 0
+
+
+def test_scratch_grows_by_doubling(monkeypatch):
+    """Calls that need more counters each time (prompts that grow, say) move the scratch, which makes recordings stale, few times."""
+    monkeypatch.setattr(low_bits, "_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: type("S", (), {"synchronize": lambda self: None})())
+    real = {"empty": torch.empty, "zeros": torch.zeros}
+    for name, make in real.items():
+        monkeypatch.setattr(torch, name, lambda n, dtype=None, device=None, make=make: make(n, dtype=dtype))
+    kernels = Scratch()
+    for counters in range(100, 60000, 700):
+        sums, zeros = kernels._kv8_scratch(7, 1000, counters)
+        held = kernels._kv8_held[7]
+        assert held[0] >= 1000 and held[1] >= counters and (sums, zeros) == held[2:4] and held[5].numel() == held[1]
+    assert kernels.scratch_generation <= 5                              # 4,096 and up to 65,536
