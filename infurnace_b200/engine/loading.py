@@ -37,8 +37,8 @@ class EngineOptions:
             raise ModelConfigError(f"weight_format {self.weight_format!r}: choose stored or mx4")
         if self.cache_format not in ("dtype", "int8"):
             raise ModelConfigError(f"cache_format {self.cache_format!r}: choose dtype or int8")
-        if self.cache_format == "int8" and (self.page_size % 16 or self.page_size < 16):
-            raise ModelConfigError(f"cache_format int8 wants pages of a multiple of 16 tokens, not {self.page_size}")
+        if self.cache_format == "int8" and (self.page_size % 16 or not 16 <= self.page_size <= 4096):
+            raise ModelConfigError(f"cache_format int8 wants pages of a multiple of 16 tokens up to 4,096, not {self.page_size}")
 
 
 def parse_dtype(name):
