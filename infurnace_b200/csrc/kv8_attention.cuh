@@ -505,13 +505,12 @@ template <typename S1, typename S2> static long long kv8_scratch(int nt) {
   return bad ? (bad > 0 ? -bad : bad) : (long long)ctas * 8 * nt * (D + 2);
 }
 
-template <typename S>
-static int kv8_launch(const Kv8Args& a, bool whole, int max_q, long long items, cudaStream_t stream) {
-  if (whole) {
-    const int rows = max_q * (a.heads / a.kv_heads);
-    const dim3 grid((rows + 8 * S::ROW_TILES * WARPS - 1) / (8 * S::ROW_TILES * WARPS), a.kv_heads, a.requests);
-    return ifb_launch(kv8_attention_whole_kernel<S>, grid, dim3(32 * WARPS), 0, stream, a);
-  }
+template <typename S> static int kv8_launch_whole(const Kv8Args& a, int max_q, cudaStream_t stream) {
+  const int rows = max_q * (a.heads / a.kv_heads);
+  const dim3 grid((rows + 8 * S::ROW_TILES * WARPS - 1) / (8 * S::ROW_TILES * WARPS), a.kv_heads, a.requests);
+  return ifb_launch(kv8_attention_whole_kernel<S>, grid, dim3(32 * WARPS), 0, stream, a);
+}
+template <typename S> static int kv8_launch_split(const Kv8Args& a, long long items, cudaStream_t stream) {
   int ctas = 0;
   const int bad = kv8_split_ctas<S>(&ctas);
   if (bad) return bad;
@@ -522,7 +521,7 @@ static int kv8_launch(const Kv8Args& a, bool whole, int max_q, long long items, 
   return ifb_launch(kv8_attention_split_kernel<S>, dim3(items > ctas ? (unsigned)items : (unsigned)ctas), dim3(32 * WARPS), kv8_split_smem<S>(), stream, b);
 }
 
-// nt: tiles of 8 score rows per warp.  whole: the whole form.  Requests of min_rows .. max_rows score rows are worked on.  Split form:
+// nt: tiles of 8 score rows per warp (split form).  whole: the whole form, of TILES such tiles.  Requests of min_rows .. max_rows score rows are worked on.  Split form:
 // `tiles` tiles of a request at most, `items` (tiles x key heads) of all requests.
 // One argument, since a call's price on the host is that of its arguments.
 struct Kv8Call {
@@ -550,7 +549,8 @@ template <typename S1, typename S2> static int kv8_call(const Kv8Call* c) {
                      (int)c->kv_heads, (int)c->page_size, (int)c->window, (float)c->scale * 1.4426950408889634f, (int)c->min_rows, (int)c->max_rows,
                      (int)c->tiles, 0};
   cudaStream_t stream = (cudaStream_t)c->stream;
-  return c->nt == 1 ? kv8_launch<S1>(a, whole, (int)c->max_q, c->items, stream) : kv8_launch<S2>(a, whole, (int)c->max_q, c->items, stream);
+  if (whole) return kv8_launch_whole<S2>(a, (int)c->max_q, stream);
+  return c->nt == 1 ? kv8_launch_split<S1>(a, c->items, stream) : kv8_launch_split<S2>(a, c->items, stream);
 }
 
 // The library's calls over the file's streams of one and of TILES row tiles.

@@ -344,16 +344,15 @@ __device__ __forceinline__ void mx_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) 
 
 template <int NT_, int STAGES_> struct MxCfg {
   static constexpr int NT = NT_, STAGES = STAGES_;
-  static constexpr int RT = NT > 128 ? 2 : 1;                          // scale tiles of 128 tokens
   static constexpr int B_BYTES = NT * 128;
-  static constexpr int SA = MX_A_BYTES + B_BYTES, SB = SA + 1024, STAGE_BYTES = SB + RT * 1024;      // where the scales lie
-  static constexpr int S_COLS = 8 + 8 * RT;                            // columns of a stage's scales
+  static constexpr int SA = MX_A_BYTES + B_BYTES, SB = SA + 1024, STAGE_BYTES = SB + 1024;      // where the scales lie
+  static constexpr int S_COLS = 16;                                    // columns of a stage's scales
   static constexpr int COLS = NT + STAGES * S_COLS;
   static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static constexpr int EPI_WARPS = NT >= 128 ? 8 : 4, THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;
   static_assert(COLS <= 512 && STAGE_BYTES % 1024 == 0, "tensor memory and alignment");
-  static_assert(STAGES * STAGE_BYTES >= NT * 128 * 4 || NT > 128, "the float32 tile of a shared k range lies in the stages");
+  static_assert(NT <= 128 && STAGES * STAGE_BYTES >= NT * 128 * 4, "one tile of the tokens' scales; the float32 tile of a shared k range lies in the stages");
   // 4-bit elements of both operands (format 1), scales as powers of two, M = 128, N = NT, k = 64, both K-major
   static constexpr uint32_t IDESC = (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | (1u << 23) | ((uint32_t)(128 >> 4) << 24);
 };
@@ -457,15 +456,14 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
     auto bytes = [&](int s) { return (uint32_t)min(2, k_tiles - 2 * s) * 512u; };      // of one tile of rows' scales
     auto load_w = [&](int s, int i) {
       const uint32_t at = base + i * C::STAGE_BYTES;
-      mx_expect_tx(&full[i], ROUND ? MX_A_BYTES + bytes(s) : MX_A_BYTES + C::B_BYTES + bytes(s) * (1 + C::RT));
+      mx_expect_tx(&full[i], ROUND ? MX_A_BYTES + bytes(s) : MX_A_BYTES + C::B_BYTES + bytes(s) * 2);
       mx_tma_2d(at, &w_map, &full[i], s * 64, o0);
       mx_bulk(at + C::SA, p.w_scales + ((size_t)(o0 >> 7) * k_tiles + 2 * s) * 512, bytes(s), &full[i]);
     };
     auto load_x = [&](int s, int i) {
       const uint32_t at = base + i * C::STAGE_BYTES;
       mx_tma_2d(at + MX_A_BYTES, &x_map, &full[i], s * 64, n0);
-      for (int t = 0; t < C::RT; ++t)
-        mx_bulk(at + C::SB + t * 1024, p.x_scales + ((size_t)((n0 >> 7) + t) * k_tiles + 2 * s) * 512, bytes(s), &full[i]);
+      mx_bulk(at + C::SB, p.x_scales + ((size_t)(n0 >> 7) * k_tiles + 2 * s) * 512, bytes(s), &full[i]);
     };
     const int ahead = min(C::STAGES, s1 - s0);
     if (mx_elect())
@@ -542,15 +540,14 @@ mx4_linear_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
           const int tiles = min(2, k_tiles - 2 * s), products = min(4, (p.k - s * MX_KSTAGE + 63) / 64);
           for (int t = 0; t < tiles; ++t) {
             mx_copy_scales(sc + t * 4, at + C::SA + t * 512);
-#pragma unroll
-            for (int r = 0; r < C::RT; ++r) mx_copy_scales(sc + 8 + t * 4 * C::RT + r * 4, at + C::SB + r * 1024 + t * 512);
+            mx_copy_scales(sc + 8 + t * 4, at + C::SB + t * 512);
           }
           const uint64_t a = mx_desc(at), b = mx_desc(at + MX_A_BYTES);
 #pragma unroll
           for (int m = 0; m < 4; ++m)
             if (m < products) {
               const uint32_t id = (uint32_t)(m & 1) * 2;               // which two of the four scales of a word
-              mx_mma(tmem, a + m * 2, b + m * 2, C::IDESC | (id << 4) | (id << 29), sc + (m >> 1) * 4, sc + 8 + (m >> 1) * 4 * C::RT,
+              mx_mma(tmem, a + m * 2, b + m * 2, C::IDESC | (id << 4) | (id << 29), sc + (m >> 1) * 4, sc + 8 + (m >> 1) * 4,
                      (j | m) != 0);
             }
           mx_commit(&empty[i]);
@@ -1079,9 +1076,7 @@ IFB_EXPORT int ifb_mx4_linear(const void* x, int x_dtype, long long x_row, void*
   cudaStream_t st = (cudaStream_t)stream;
   int* e = (int*)err;
   if (round) {
-    if (x_dtype == IFB_F32)
-      return nt == 16 ? mx_launch_any<MxCfg<16, 6>, float>(wm, wm, p, gated, out_dtype, splits, e, st)
-                      : mx_launch_any<MxCfg<32, 6>, float>(wm, wm, p, gated, out_dtype, splits, e, st);
+    if (x_dtype == IFB_F32) return mx_launch_any<MxCfg<16, 6>, float>(wm, wm, p, gated, out_dtype, splits, e, st);      // (16 rows at most)
     return nt == 16 ? mx_launch_any<MxCfg<16, 6>, bf16>(wm, wm, p, gated, out_dtype, splits, e, st)
                     : mx_launch_any<MxCfg<32, 6>, bf16>(wm, wm, p, gated, out_dtype, splits, e, st);
   }

@@ -506,7 +506,7 @@ class LowBitKernels:
                                                          tiles, nt, 0, items, stream, scale))
             if rows > limit and not status:
                 self.launches += 1
-                status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, 0, 0, *sizes, limit + 1, (1 << 31) - 1, 1, nt, 1, 0, stream, scale))
+                status = lib.ifb_kv8_attention(_KV8_CALL(*fixed, 0, 0, *sizes, limit + 1, (1 << 31) - 1, 1, 1, 1, 0, stream, scale))
             if status:
                 self._low_bit_status(status, "kv8_attention")
             if tc:
