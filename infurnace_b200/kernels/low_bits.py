@@ -224,7 +224,7 @@ class LowBitKernels:
             raise KernelError(f"mx4_quantize: x is bfloat16 or float32 [{matrix.rows}, {matrix.k}] with unit stride along k, on the "
                               f"matrix's device; got {x.dtype} {tuple(x.shape)} on {x.device}")
         self.launches += 1
-        status = self._mx4_lib().ifb_mx4_quantize(x.data_ptr(), code, x.stride(0), *matrix._at, matrix.rows, matrix.k, matrix.gated,
+        status = self._mx4_lib().ifb_mx4_quantize(x.data_ptr(), code, x.stride(0) if matrix.rows > 1 else matrix.k, *matrix._at, matrix.rows, matrix.k, matrix.gated,
                                                   _raw_stream(index))
         if status:
             self._low_bit_status(status, "mx4_quantize")
@@ -297,6 +297,8 @@ class LowBitKernels:
             pitch, unit = x.stride()
             if x_code is None or unit != 1 or x.get_device() != index:
                 raise KernelError("mx4_linear: x is bfloat16 or float32 with unit stride along k on w's device, or an Mx4Matrix")
+            if n == 1:
+                pitch = k                                                  # (one row's pitch leads nowhere)
             if n <= self._mx4_round_rows[x_code]:
                 rows = (x.data_ptr(), x_code, pitch, 0, 0)
             else:
@@ -347,7 +349,8 @@ class LowBitKernels:
         if n == 0:
             return
         self.launches += 1
-        status = self._kv8_lib().ifb_kv8_store(k.data_ptr(), v.data_ptr(), code, pitch[0], v_pitch[0], slot_mapping.data_ptr(), *pages._at, n, heads,
+        k_row, v_row = (pitch[0], v_pitch[0]) if n > 1 else (heads * dim, heads * dim)
+        status = self._kv8_lib().ifb_kv8_store(k.data_ptr(), v.data_ptr(), code, k_row, v_row, slot_mapping.data_ptr(), *pages._at, n, heads,
                                                pages.page_size, dim, _raw_stream(index))
         if status:
             self._low_bit_status(status, "kv8_store")
@@ -462,7 +465,7 @@ class LowBitKernels:
         r = seq_lens.numel()
         table_shape, table_pitch = block_tables.shape, block_tables.stride()
         if cu_q.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_tables.dtype != torch.int32 or cu_q.numel() != r + 1 \
-                or len(table_shape) != 2 or table_shape[0] < r or table_pitch[1] != 1 or not cu_q.is_contiguous() or not seq_lens.is_contiguous():
+                or len(table_shape) != 2 or table_shape[0] < r or (table_pitch[1] != 1 and table_shape[1] > 1) or not cu_q.is_contiguous() or not seq_lens.is_contiguous():
             raise KernelError("kv8_attention: cu_q, seq_lens and block_tables are int32 for the same requests, dense along their last axis")
         if table_shape[1] * pages.page_size < max_seq_len:
             raise KernelError(f"kv8_attention: block tables of {table_shape[1]} pages do not hold {max_seq_len} keys")
@@ -474,6 +477,7 @@ class LowBitKernels:
         if window < 0 or max_q_len < 1 or not 1 <= min_q_len <= max_q_len:
             raise KernelError("kv8_attention: window is not negative, and 1 <= min_q_len <= max_q_len")
         lib, stream, group = self._kv8_attention_lib(dim, q.dtype), _raw_stream(index), heads // kv_heads
+        q_row = pitch[0] if n > 1 else heads * dim
         rows, least = max_q_len * group, min_q_len * group
         tc = False
         if rows > 16 and q.dtype == torch.bfloat16 and dim <= 128 and group <= 128 and pages.page_size in (16, 32, 64) and self.attention_tc:
@@ -494,7 +498,7 @@ class LowBitKernels:
             # score rows up to which a request runs split
             limit = min(rows, 64) if n * heads > self.kv8_whole_rows * self.sm_count and max_seq_len <= self.kv8_whole_keys else rows
             nt = 1 if rows <= 8 or dim > 128 or tc and group <= 8 else 2      # (beside prompts the short requests decode)
-            fixed = (q.data_ptr(), code, pitch[0], *pages._at, block_tables.data_ptr(), table_pitch[0], cu_q.data_ptr(), seq_lens.data_ptr(),
+            fixed = (q.data_ptr(), code, q_row, *pages._at, block_tables.data_ptr(), table_pitch[0], cu_q.data_ptr(), seq_lens.data_ptr(),
                      out.data_ptr())
             sizes = (r, heads, kv_heads, pages.page_size, dim, window, max_q_len)
             status = 0
@@ -511,7 +515,7 @@ class LowBitKernels:
                 self._low_bit_status(status, "kv8_attention")
             if tc:
                 at, step, block = wide.data_ptr(), wide.stride(0), 2 * kv_heads * pages.page_size * dim
-                self._attention_tc_streams(q.as_strided((n, heads * dim), (pitch[0], 1)), heads, kv_heads, 1, dim, dim, (at, step, pages.page_size),
+                self._attention_tc_streams(q.as_strided((n, heads * dim), (q_row, 1)), heads, kv_heads, 1, dim, dim, (at, step, pages.page_size),
                                            (at + block, step, pages.page_size), room, wide_tables, cu_q, seq_lens, out, scale, window, max_q_len, n, r,
                                            2, None, None, kind=0)
         return out
