@@ -4,8 +4,8 @@
 // The definition.  A block is what a page holds of one head's keys or values; f is the exponent field of its largest magnitude
 // as a float32 number, step = 2^(f - 133), a code is floor(x / step), which lies in [-128, 127], and stands for (code + 1/2)
 // step.  Floors nest: floor(floor(x / s) / 2^d) = floor(x / (s 2^d)), so when a token with a larger number joins a page, a
-// shift of the older codes to the right makes them what they would be had all been stored at once, and how a prompt was cut
-// leaves no trace in a page's bits.  (With rounding to nearest in place of floor, the second rounding would.)  f = 0 (all
+// shift of the older codes to the right makes them what they would be had all been stored at once, and how the same numbers
+// are cut over calls leaves no trace in a page's bits.  (With rounding to nearest in place of floor, the second rounding would.)  f = 0 (all
 // numbers zero or subnormal): the values are 0; f = 255 (an infinity or NaN): they are NaN.
 //
 // Layout: codes int8 [pages][2][heads][page_size][dim], exponents uint8 [pages][2][heads].

@@ -16,8 +16,9 @@
 // still count, for steps up to 2^80 apart.  (A reference of the scores alone: rows that do not see a page of values 2^24 larger than
 // their own, but whose warp does, lose bits, and from 2^33 on are zero.)  Sums are float32.
 //
-// What bounds it: the integer pipe, for the bytes of keys and values (half of its time over a whole call), and the registers, with 128 of which four CTAs
-// fit on an SM: what does not have to stay in one over the loop is named anew or uniform (46.1 to 42.2 us in the third figure).  A call has some
+// What bounds it: no one unit.  Over a whole call the integer pipe (for the bytes of keys and values) and the issue slots are half busy, and a third of
+// the warps' time is waiting for memory, with the four CTAs on an SM that 128 registers allow: what does not have to stay in one over the
+// loop is named anew or uniform (46.1 to 42.2 us in the third figure).  A call has some
 // 8 us beside the loop: the look at the lengths, the first trip, the joins.  Eight requests of 3,967 to 8,095 keys (32 heads on 8)
 // 26.5 us, 3.7 TB/s; 64 of 129 to 383 (16 on 8) 14.5; 64 of 1,500 (32 on 8) 42.2, 4.7 TB/s.  Slower were: copies to shared memory some tiles
 // ahead, requests to the second level of cache two tiles ahead, values requested with the keys, three CTAs with more registers (59 us).

@@ -271,7 +271,7 @@ IFB_EXPORT int ifb_mx4_values(const void* codes, const void* scales, void* out, 
 // (one ahead: 8 rows of 12,288 by 4,096 11.1 us, four 8.3; with a kernel of its own for the rounding 8.9).  From 33 rows on the
 // rounding takes longer than the matrix (24,576 x 4,096: 25 us, 15.5 with the kernel of its own).
 // What bounds it: few tokens, the matrix's bytes and what a CTA does beside them, its start, its first stages and the sum over its cluster (8 rows
-// of 12,288 by 4,096: 8.2 us, 3.3 TB/s; 33 rows by gate and up of 12,288 x 4,096, rows rounded first: 15.6 us, 3.5 TB/s; 1 row of 1,024 by
+// of 12,288 by 4,096: 8.2 us, 3.3 TB/s; 33 rows by gate and up of 12,288 x 4,096, rows rounded first: 15.6 us, 3.5 TB/s, 192 tiles at once of which 44 SMs have two; 1 row of 1,024 by
 // 4,096: 3.3 us, latency).
 // Waits are bounded: after a limit a thread records a code in `*err`, raises the CTA's abort flag, and all fall through to the
 // end, where the tensor memory is given back.
@@ -742,7 +742,7 @@ static int mx_launch_any(const CUtensorMap& xm, const CUtensorMap& wm, const MxP
 // of either operand (and the scales of its rows of w and of all 256 tokens), one tcgen05.mma of the pair (M = 256), issued by the
 // first CTA, multiplies out of both shared memories into both tensor memories, where a CTA finds its 128 rows of w.  What bounds
 // these products is the bytes that reach an SM: 8 KB for the 128 cycles of 128 x 256 x 64, where a CTA alone would bring 12 (2,048 rows by gate
-// and up of 12,288 x 4,096: 88 us with the rows' rounding, 4.7 PFLOP/s, the tensor pipe busy for 63 % of the time, 46 bytes a cycle into an SM; by
+// and up of 12,288 x 4,096: 89 us with the rows' rounding, 4.6 PFLOP/s, 103 in the long run, at the clocks of the power limit; the tensor pipe busy for 63 % of the time, 46 bytes a cycle into an SM; by
 // CTAs alone 150).
 // Persistent, one accumulator (the scales leave no room for two): the epilogue's warps take it to registers at once (256
 // columns in some hundred cycles) and let the next tile's products begin, which run while they finish and store.

@@ -452,7 +452,8 @@ class LowBitKernels:
         among them.  A row that sees no key becomes zero.  No request has more than ``max_q_len`` queries or ``max_seq_len``
         keys, none fewer than ``min_q_len`` queries; ``exact_lens``: some request has ``max_q_len``, and ``q`` no other rows than
         theirs, which bounds how many are long.  Numbers of queries, keys and values are below 2^100 in size, or infinite or NaN
-        (which the rows that see them become): sums of larger ones may overflow."""
+        (which the rows that see them become): sums of larger ones may overflow.  Recorded calls share memory for the split form's sums:
+        run the call once before a recording, and let replays follow one another."""
         code = _CODES.get(q.dtype)
         shape, pitch, index = q.shape, q.stride(), pages._index
         n, heads, dim = shape if len(shape) == 3 else (0, 0, 0)
