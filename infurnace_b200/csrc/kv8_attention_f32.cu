@@ -104,7 +104,9 @@ struct Stream {
   // r: log2 of the unit of o and wsum, 2^m apart; wsum: this lane's part of the sum of weights times steps, whose half o lacks
   float m[NT][2], l[NT][2], r[NT][2], wsum[NT][2];
   float o[KS][NT][4];
-  static constexpr float TOP = 23.9999f; // log2 of the largest weight as a whole number
+  // log2 of the largest weight as a whole number, 24 - 2^-12: differences to `top`, a number of up to 2^8 and more, are exact (23.9999 is
+  // rounded to 2^-17 there, and all weights with it, 5e-6 beside their sum)
+  static constexpr float TOP = 23.999755859375f;
 
   __device__ __forceinline__ void reset() {
 #pragma unroll

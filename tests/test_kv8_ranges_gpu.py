@@ -93,3 +93,14 @@ def test_sums_of_large_values(K, monkeypatch, form, dtype, q_len, field, rise):
         codes[tables[:, i].long(), 0, :, :, 0] = i - 10
     codes[:, 1].clamp_(-126, 125)                                      # (a weighted mean's rounding stays below the largest float)
     within(K, s, dim, n, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("field", [20, 90, 127, 150, 190, 220])
+@pytest.mark.parametrize("keys", [1, 2, 9, 40])
+def test_few_keys_with_values_of_any_size(K, dtype, field, keys):
+    """Where few keys leave little to the bound but the weights' own rounding: a weight's unit is the same in the products and beside them."""
+    n = 40
+    s = scene([1] * n, [keys] * n, 2, 4, 64, 16, dtype, seed=field + keys)
+    s[2][:, 1] = field + torch.randint(0, 20, s[2][:, 1].shape, generator=torch.Generator().manual_seed(keys)).to(torch.uint8)
+    within(K, s, 64, keys, dtype)
