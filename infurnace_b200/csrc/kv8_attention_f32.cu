@@ -357,7 +357,7 @@ struct Stream {
   __device__ __forceinline__ void finish() {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float unit[2];
+      float unit[2], rest[2];                                           // 2^(r - 133) in two factors: of its own it may be no float
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -366,14 +366,16 @@ struct Stream {
           wsum[n][e] += __shfl_xor_sync(0xffffffffu, wsum[n][e], x);
         }
         const int by = kv8_excess(l[n][e], wsum[n][e], r[n][e]);
-        unit[e] = r[n][e] == -INFINITY ? 0.f : kv8_exp2(r[n][e] - 133.f - (float)by);
+        const float to = r[n][e] == -INFINITY ? -1000.f : r[n][e] - 133.f - (float)by;
+        unit[e] = kv8_exp2(fmaxf(to, -100.f));
+        rest[e] = kv8_exp2(fminf(to + 100.f, 0.f));
         l[n][e] *= __uint_as_float((uint32_t)(127 - by) << 23);
         m[n][e] += (float)by;
       }
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][n][j] = fmaf(0.5f, wsum[n][j & 1], o[i][n][j]) * unit[j & 1];
+        for (int j = 0; j < 4; ++j) o[i][n][j] = fmaf(0.5f, wsum[n][j & 1], o[i][n][j]) * unit[j & 1] * rest[j & 1];
     }
   }
 };

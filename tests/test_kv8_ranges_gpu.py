@@ -104,3 +104,20 @@ def test_few_keys_with_values_of_any_size(K, dtype, field, keys):
     s = scene([1] * n, [keys] * n, 2, 4, 64, 16, dtype, seed=field + keys)
     s[2][:, 1] = field + torch.randint(0, 20, s[2][:, 1].shape, generator=torch.Generator().manual_seed(keys)).to(torch.uint8)
     within(K, s, 64, keys, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("q_len", [1, 20])
+def test_small_weights_beside_zeros(K, dtype, q_len):
+    """The keys of all the weight have values of zero; of the others, 2^-150 and 2^-92 of it, in this order, the larger make the output."""
+    n, dim, requests = 9 * 16, 64, 600 if q_len == 1 else 40
+    s = scene([q_len] * requests, [n] * requests, 1, 2, dim, 16, dtype, seed=7)
+    q, codes, fields, tables = s[:4]
+    q.zero_()
+    q[:, :, 0] = 8 * math.log(2.0)
+    fields[:, 0], fields[:, 1] = 133, 125
+    codes[:, 0, :, :, 0] = -128
+    for page, code in ((0, 100), (1, -50), (8, 8)):
+        codes[tables[:, page].long(), 0, :, :, 0] = code
+    fields[tables[:, 0].long(), 1] = 0
+    within(K, s, dim, n, dtype)
