@@ -287,7 +287,7 @@ class LowBitKernels:
             raise KernelError("mx4_linear: out is bfloat16 or float32, contiguous, and all is on the matrix's device")
         if n == 0:
             return out
-        lib = self._mx4_lib()
+        lib, stream, launches, lock = self._mx4_lib(), _raw_stream(index), 1, None
         if isinstance(x, Mx4Matrix):
             if x.gated or x._index != index:
                 raise KernelError("mx4_linear: x is a plain matrix on w's device")
@@ -297,24 +297,25 @@ class LowBitKernels:
             pitch, unit = x.stride()
             if x_code is None or unit != 1 or x.get_device() != index:
                 raise KernelError("mx4_linear: x is bfloat16 or float32 with unit stride along k on w's device, or an Mx4Matrix")
-            if n == 1:
-                pitch = k                                                  # (one row's pitch leads nowhere)
-            if n <= self._mx4_round_rows[x_code]:
-                rows = (x.data_ptr(), x_code, pitch, 0, 0)
-            else:
-                with self._low_bit_lock:
-                    room = self._mx4_room(w, _raw_stream(index), Mx4Matrix.row_bytes(n, k))
-                    self._mx4_product(lib, (x.data_ptr(), x_code, pitch, room, room + -(-n * k // 512) * 256), w, out, code, n, k, epi, nt, splits, 2)
-                return out
-        self._mx4_product(lib, rows, w, out, code, n, k, epi, nt, splits, 1)
-        return out
-
-    def _mx4_product(self, lib, rows, w, out, code, n, k, epi, nt, splits, launches):
-        self.launches += launches
-        self._err_armed = True
-        status = lib.ifb_mx4_linear(*rows, *w._at, out.data_ptr(), code, n, k, w.rows, epi, nt, splits, self._dev_err_at, _raw_stream(w._index))
+            rows = (x.data_ptr(), x_code, pitch if n > 1 else k, 0, 0)      # (one row's pitch leads nowhere)
+            if n > self._mx4_round_rows[x_code]:
+                launches, lock = 2, self._low_bit_lock
+        if lock is not None:
+            lock.acquire()
+        try:
+            if lock is not None:
+                codes = -(-n * k // 512) * 256                             # half a byte an element, to a multiple of 256
+                room = self._mx4_room(w, stream, codes + Mx4Matrix.scale_bytes(n, k))
+                rows = (*rows[:3], room, room + codes)
+            self.launches += launches
+            self._err_armed = True
+            status = lib.ifb_mx4_linear(*rows, *w._at, out.data_ptr(), code, n, k, w.rows, epi, nt, splits, self._dev_err_at, stream)
+        finally:
+            if lock is not None:
+                lock.release()
         if status:
             self._low_bit_status(status, "mx4_linear")
+        return out
 
     # ------------------------------------------------------------------ keys and values of 8 bits
     _kv8 = None
@@ -433,10 +434,12 @@ class LowBitKernels:
         kv_heads, ps, dim = pages.kv_heads, pages.page_size, pages.head_dim
         held = pages.room
         if held is None:
-            held = torch.empty(_expanded_bytes(room, r * most, kv_heads, ps, dim), dtype=torch.uint8, device=pages.codes.device)
-        split = room * 4 * kv_heads * ps * dim
-        wide = held[:split].view(torch.bfloat16).view(room, 2, kv_heads, ps, dim)
-        tables = held[split:split + 4 * r * most].view(torch.int32).view(r, most)
+            wide = torch.empty((room, 2, kv_heads, ps, dim), dtype=torch.bfloat16, device=pages.codes.device)
+            tables = torch.empty((r, most), dtype=torch.int32, device=pages.codes.device)
+        else:
+            split = room * 4 * kv_heads * ps * dim
+            wide = held[:split].view(torch.bfloat16).view(room, 2, kv_heads, ps, dim)
+            tables = held[split:split + 4 * r * most].view(torch.int32).view(r, most)
         self.launches += 1
         status = self._kv8_lib().ifb_kv8_expand(*pages._at, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(), seq_lens.data_ptr(),
                                                 wide.data_ptr(), tables.data_ptr(), room, r, most, kv_heads, group, ps, dim, window, 16, stream)
