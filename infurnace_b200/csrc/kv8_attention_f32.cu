@@ -7,9 +7,9 @@
 // over 2^24, so that a long row of small weights beside one large one keeps all bits.  A page's step is a factor of its keys'
 // scores; half a step beside each code is half the sum of the row's queries or weights.  Queries and weights are rounded once
 // each; everything outside of the products is float32.
-// Errors against 64 bits 3 to 5e-7 of the output, below those of plain float32 sums; with queries and weights of two
+// Errors against 64 bits 4 to 6e-7 of the output, below those of plain float32 sums (6e-7 to 1.4e-6); with queries and weights of two
 // half-precision terms each, in the same time, 1.4 to 2.4e-6 (the running sums of half-precision products are cut off, not
-// rounded).  For bfloat16 the two are not of the same time: eight requests of 3,967 to 8,095 keys 32 us here, 26.5
+// rounded).  For bfloat16 the two are not of the same time: eight requests of 3,967 to 8,095 keys 31 us here, 26.5
 // as in kv8_attention.cu.
 #define KV8_F32 1
 #include "kv8_attention.cuh"
