@@ -1,0 +1,763 @@
+// Drawing a token for each row of logits under top-k, top-p and min-p, and the log probability and rank of given tokens.
+//
+// sample_cut.  With m the row's largest logit (NaN counts as -inf throughout) w_i = exp((l_i - m) / T); tokens are ordered by falling logit,
+// equal ones by rising index.  A: the first k of the order (k < 1 or >= the vocabulary: all).  B: those of A before which A has less than p of its weight
+// (p >= 1: all; at least the first).  C: those of B with w_i >= min_p (or l_i = m).  The token is the smallest index i of C with
+// sum_{j <= i, j in C} w_j > u sum_C w; its log probability under C is (l_i - m) / T - log sum_C w.  T = 0 (or not above 0): the first of
+// the order, log probability 0.  A row without a number above -inf: token 0, NaN.
+//
+// Weights are whole numbers W_i = round(2^44 w_i), from 64-bit arithmetic (so what is below 2^-45 of the largest is never drawn).  The borders between 150,000 tokens lie some 1e-6 of the sum apart, so that
+// 32-bit sums (1e-7) would move one draw in tens to another token; with W one row in some 100,000 comes near a border (the errors of 150,000
+// roundings add up to 1e-11).  And sums of whole numbers do not depend on their order: a row's token depends on the row alone, not on how many CTAs or
+// threads share it.  2^44 times the largest vocabulary stays below 2^63.
+//
+// A row is shared by a cluster of C CTAs, which keep its slices in shared memory as float32: it is read from memory once.  A cut is found by counts (top-k)
+// or weights (top-p) in bins of equal width over (l - m) / T; the bin that the cut runs through is divided once more if it
+// has many members; the members left are put in order by one CTA.  Where too many are left (ties), a search over the ordered bits of their
+// values finds the last value that is kept, and a count in index order the last of its tokens.
+#include "common.cuh"
+#include <math.h>
+#include <type_traits>
+
+typedef unsigned long long u64;
+typedef __nv_bfloat16 bf16;
+
+constexpr int NT = 512;                  // threads of a CTA
+constexpr int NW = NT / 32;
+constexpr int BINS = 1024;               // over REACH factors of two below the largest weight: beyond them a weight is 0
+constexpr float REACH = 46.f;
+constexpr int SUBS = 256;                // parts of a bin
+constexpr int LIST = NT;                 // members that are put in order, one a thread
+constexpr int MAX_CLUSTER = 8;
+constexpr int SLICE = 46080;             // most logits of a CTA: 180 KB
+constexpr int SHARED_SLICE = 20480;      // up to here two CTAs fit on an SM
+constexpr double UNIT = 17592186044416.0;      // 2^44
+constexpr u64 ALL = ~0ull;
+
+// ---------------------------------------------------------------------------------------------------- clusters
+__device__ __forceinline__ uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint32_t peer(const void* p, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(s_addr(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ uint32_t peer_u32(const uint32_t* p, int rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(peer(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ u64 peer_u64(const u64* p, int rank) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];\n" : "=l"(v) : "r"(peer(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void put_u32(uint32_t* p, int rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(peer(p, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void put_u64(u64* p, int rank, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;\n" ::"r"(peer(p, rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t add_peer(uint32_t* p, int rank, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;\n" : "=r"(old) : "r"(peer(p, rank)), "r"(v) : "memory");
+  return old;
+}
+__device__ __forceinline__ int cluster_rank() { int r; asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r)); return r; }
+__device__ __forceinline__ int cluster_size() { int r; asm("mov.u32 %0, %%cluster_nctaid.x;\n" : "=r"(r)); return r; }
+// All threads of all CTAs of the row; what was written to shared memory before it, one's own or a peer's, is seen after it.
+__device__ __forceinline__ void row_sync(int ctas) {
+  if (ctas == 1) { __syncthreads(); return; }
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------------------------------- weights
+// 2^(j / 32), in shared memory.
+struct Exp2Table { double t[32]; };
+// round(2^44 2^y) for y <= 0 as a whole number; `w`: before rounding.  y = (n + f) / 32, n whole, |f| <= 1/2: 2^y = 2^(n / 32) e^(f ln 2 / 32), the
+// latter by its Taylor series, whose sixth power is below 3e-15.  Weights below 2^-46 are 0.
+__device__ __forceinline__ u64 weight_of(double y, const Exp2Table& tab, double& w) {
+  if (!(y >= -46.0)) { w = 0.0; return 0; }
+  constexpr double MAGIC = 6755399441055744.0 / 32.0;      // 1.5 2^52 / 32: the sum's last bit is 1/32
+  constexpr double LN2 = 0.693147180559945309417;
+  constexpr double C1 = LN2, C2 = LN2 * LN2 / 2, C3 = LN2 * LN2 * LN2 / 6, C4 = C3 * LN2 / 4, C5 = C4 * LN2 / 5;
+  const double t = y + MAGIC;
+  const double r = y - (t - MAGIC);
+  const int n = __double2loint(t);
+  const double scale = tab.t[n & 31];
+  double p = fma(r, C5, C4);
+  p = fma(r, p, C3);
+  p = fma(r, p, C2);
+  p = fma(r, p, C1);
+  p = fma(r, p, 1.0);
+  w = p * __hiloint2double(__double2hiint(scale) + (((n >> 5) + 44) << 20), __double2loint(scale));
+  return (u64)__double_as_longlong(w + 4503599627370496.0) & ((1ull << 52) - 1);
+}
+
+// How a row's numbers become weights.
+struct RowScale {
+  float m;          // the largest logit
+  float to_bin;     // bins per unit of m - l
+  double s;         // log2(e) / T
+};
+__device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp2Table& tab, double& w) {
+  const double y = l == rs.m ? 0.0 : ((double)l - (double)rs.m) * rs.s;      // (infinities too)
+  return weight_of(y, tab, w);
+}
+// The place of a number in bins of equal width; BINS or more (NaN included): its weight is 0.
+__device__ __forceinline__ float row_bin(float l, const RowScale& rs) { return l == rs.m ? 0.f : (rs.m - l) * rs.to_bin; }
+
+// An order-preserving whole number of a float32 number that is not NaN (-0 was made 0).
+__device__ __forceinline__ uint32_t ordered(float l) {
+  const uint32_t b = __float_as_uint(l);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+// ---------------------------------------------------------------------------------------------------- sums over a row
+struct Exchange { u64 a, b; };
+struct CutShared {
+  Exp2Table tab;
+  Exchange swap[2][MAX_CLUSTER];        // what the CTAs of a row tell each other, in turn
+  u64 warp_a[NW], warp_b[NW];
+  u64 found[4];
+  uint32_t listed, chosen;
+  float best_val;
+  uint32_t best_idx;
+};
+
+__device__ __forceinline__ u64 warp_add(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+struct Row {
+  CutShared* sh;
+  int ctas, rank, turn;
+  // Every CTA's (a, b) to every CTA; read with got(r) until the call after the next.
+  __device__ __forceinline__ const Exchange* tell(u64 a, u64 b) {      // called by all threads, with the CTA's numbers in thread 0
+    Exchange* box = sh->swap[turn];
+    turn ^= 1;
+    if (threadIdx.x == 0)
+      for (int r = 0; r < ctas; ++r) { put_u64(&box[rank].a, r, a); put_u64(&box[rank].b, r, b); }
+    row_sync(ctas);
+    return box;
+  }
+  // Sums of (a, b) over all threads of the row.
+  __device__ __forceinline__ void sum(u64& a, u64& b) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    a = warp_add(a); b = warp_add(b);
+    __syncthreads();
+    if (lane == 0) { sh->warp_a[warp] = a; sh->warp_b[warp] = b; }
+    __syncthreads();
+    a = b = 0;
+    if (threadIdx.x == 0)
+      for (int w = 0; w < NW; ++w) { a += sh->warp_a[w]; b += sh->warp_b[w]; }
+    const Exchange* box = tell(a, b);
+    a = b = 0;
+    for (int r = 0; r < ctas; ++r) { a += box[r].a; b += box[r].b; }
+  }
+  // Largest a and smallest b over all threads of the row.
+  __device__ __forceinline__ void extremes(u64& a, u64& b) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const u64 x = __shfl_xor_sync(0xffffffffu, a, o), y = __shfl_xor_sync(0xffffffffu, b, o);
+      a = a > x ? a : x; b = b < y ? b : y;
+    }
+    __syncthreads();
+    if (lane == 0) { sh->warp_a[warp] = a; sh->warp_b[warp] = b; }
+    __syncthreads();
+    if (threadIdx.x == 0)
+      for (int w = 0; w < NW; ++w) { a = a > sh->warp_a[w] ? a : sh->warp_a[w]; b = b < sh->warp_b[w] ? b : sh->warp_b[w]; }
+    const Exchange* box = tell(a, b);
+    a = 0; b = ALL;
+    for (int r = 0; r < ctas; ++r) { a = a > box[r].a ? a : box[r].a; b = b < box[r].b ? b : box[r].b; }
+  }
+  // The sum of v over the threads of this CTA before this one and the CTAs before it (`total`: over all).
+  __device__ __forceinline__ u64 before(u64 v, u64& total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    u64 run = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const u64 x = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += x; }
+    __syncthreads();
+    if (lane == 31) sh->warp_a[warp] = run;
+    __syncthreads();
+    u64 mine = 0, at = run - v;
+    for (int w = 0; w < NW; ++w) { const u64 x = sh->warp_a[w]; if (w < warp) at += x; mine += x; }
+    const Exchange* box = tell(mine, 0);
+    total = 0;
+    for (int r = 0; r < ctas; ++r) { if (r < rank) at += box[r].a; total += box[r].a; }
+    return at;
+  }
+};
+
+// The counts and weights of `n` bins over all CTAs of the row, from each CTA's own (weights in two halves): to every CTA.
+__device__ __forceinline__ void merge_bins(const Row& row, int n, const uint32_t* own_count, const uint32_t* own_lo, const uint32_t* own_hi,
+                                           uint32_t* count, u64* mass, bool weighted) {
+  row_sync(row.ctas);
+  const int share = (n + row.ctas - 1) / row.ctas, first = row.rank * share, last = min(n, first + share);
+  for (int b = first + threadIdx.x; b < last; b += NT) {
+    uint32_t c = 0;
+    u64 w = 0;
+    for (int r = 0; r < row.ctas; ++r) {
+      c += peer_u32(own_count + b, r);
+      if (weighted) w += ((u64)peer_u32(own_hi + b, r) << 32) + peer_u32(own_lo + b, r);
+    }
+    for (int r = 0; r < row.ctas; ++r) {
+      put_u32(count + b, r, c);
+      if (weighted) put_u64(mass + b, r, w);
+    }
+  }
+  row_sync(row.ctas);
+}
+
+// The bin that the cut runs through: the first with count (by_mass: weight) before it below `goal` and with it at least that.
+// Returns it, and what lies before it; n where the whole lies below the goal.  All threads of a CTA call it.
+__device__ __forceinline__ int find_bin(CutShared* sh, int n, const uint32_t* count, const u64* mass, bool by_mass, u64 goal, u64& before_count,
+                                        u64& before_mass, bool weighted) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (n + NT - 1) / NT;      // bins of a thread, one after the other
+  u64 c = 0, w = 0;
+  for (int j = 0; j < per; ++j) {
+    const int b = threadIdx.x * per + j;
+    if (b < n) { c += count[b]; if (weighted) w += mass[b]; }
+  }
+  u64 rc = c, rw = w;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, rc, o), y = __shfl_up_sync(0xffffffffu, rw, o);
+    if (lane >= o) { rc += x; rw += y; }
+  }
+  __syncthreads();
+  if (lane == 31) { sh->warp_a[warp] = rc; sh->warp_b[warp] = rw; }
+  if (threadIdx.x == 0) { sh->found[0] = n; sh->found[1] = sh->found[2] = 0; }
+  __syncthreads();
+  rc -= c; rw -= w;
+  for (int v = 0; v < warp; ++v) { rc += sh->warp_a[v]; rw += sh->warp_b[v]; }
+  for (int j = 0; j < per; ++j) {
+    const int b = threadIdx.x * per + j;
+    if (b >= n) break;
+    const u64 dc = count[b], dw = weighted ? mass[b] : 0;
+    const u64 at = by_mass ? rw : rc, d = by_mass ? dw : dc;
+    if (at < goal && at + d >= goal) { sh->found[0] = b; sh->found[1] = rc; sh->found[2] = rw; }
+    rc += dc; rw += dw;
+  }
+  __syncthreads();
+  before_count = sh->found[1]; before_mass = sh->found[2];
+  return (int)sh->found[0];
+}
+
+// The last token that a cut keeps, and the weight that it keeps in all.
+struct Cut { float l; int i; u64 mass; };
+__device__ __forceinline__ bool kept(float l, int i, const Cut& c) { return l > c.l || (l == c.l && i <= c.i); }
+
+struct CutMemory {      // of a CTA, behind its slice of the row
+  uint32_t* count; uint32_t* lo; uint32_t* hi;             // its own bins [BINS] each; one CTA's list of members lies over them
+  uint32_t* row_count; u64* row_mass;                      // the row's bins [BINS]
+  uint32_t* sub_count; u64* sub_mass;                      // the row's parts of a bin [SUBS]
+};
+constexpr size_t CUT_BYTES = (size_t)BINS * 12 + (size_t)BINS * 12 + (size_t)SUBS * 12;
+static_assert(LIST * (8 + 4 + 4) <= BINS * 12, "a list of members must fit over a CTA's own bins");
+
+__device__ __forceinline__ void add_mass(uint32_t* lo, uint32_t* hi, int b, u64 w) {
+  const uint32_t x = (uint32_t)w, old = atomicAdd(lo + b, x);
+  const uint32_t up = (uint32_t)(w >> 32) + (old + x < old ? 1u : 0u);
+  if (up) atomicAdd(hi + b, up);
+}
+
+// The cut through the row's bins after which `goal` tokens (by_mass: at least `goal` of weight) are kept.  `all`: the answer where that is everything.
+__device__ Cut find_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, bool by_mass, u64 goal, bool weighted,
+                        const Cut& all) {
+  CutShared* sh = row.sh;
+  u64 bc, bm;
+  const int b0 = find_bin(sh, BINS, mem.row_count, mem.row_mass, by_mass, goal, bc, bm, weighted);
+  if (b0 >= BINS) return all;
+  uint32_t members = mem.row_count[b0];
+  int b1 = -1;
+  if (members > LIST) {
+    __syncthreads();
+    for (int b = threadIdx.x; b < SUBS; b += NT) mem.count[b] = mem.lo[b] = mem.hi[b] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const float f = row_bin(vals[i], rs);
+      if (!(f < BINS) || (int)f != b0) continue;
+      const int b = (int)((f - b0) * SUBS);      // exact until the last step
+      atomicAdd(mem.count + b, 1u);
+      if (weighted) { double w; add_mass(mem.lo, mem.hi, b, row_weight(vals[i], rs, sh->tab, w)); }
+    }
+    merge_bins(row, SUBS, mem.count, mem.lo, mem.hi, mem.sub_count, mem.sub_mass, weighted);
+    u64 c1, m1;
+    b1 = find_bin(sh, SUBS, mem.sub_count, mem.sub_mass, by_mass, goal - (by_mass ? bm : bc), c1, m1, weighted);
+    if (b1 >= SUBS) return all;      // (never: the parts have what the bin has)
+    bc += c1; bm += m1;
+    members = mem.sub_count[b1];
+  }
+  auto member = [&](float l) {
+    const float f = row_bin(l, rs);
+    return f < BINS && (int)f == b0 && (b1 < 0 || (int)((f - b0) * SUBS) == b1);
+  };
+  if (members <= LIST) {
+    u64* lw = reinterpret_cast<u64*>(mem.count);
+    float* ll = reinterpret_cast<float*>(lw + LIST);
+    uint32_t* li = reinterpret_cast<uint32_t*>(ll + LIST);
+    if (threadIdx.x == 0) sh->listed = 0;
+    row_sync(row.ctas);      // nobody reads its bins any more
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const float l = vals[i];
+      if (!member(l)) continue;
+      const uint32_t at = add_peer(&sh->listed, 0, 1u);
+      if (at >= LIST) continue;      // (never: the members were counted)
+      double w;
+      put_u64(lw + at, 0, weighted ? row_weight(l, rs, sh->tab, w) : 0);
+      put_u32(reinterpret_cast<uint32_t*>(ll) + at, 0, __float_as_uint(l));
+      put_u32(li + at, 0, (uint32_t)(base + i));
+    }
+    row_sync(row.ctas);
+    if (row.rank == 0) {
+      const int i = threadIdx.x;
+      if (i < (int)members) {
+        const float l = ll[i];
+        const uint32_t idx = li[i];
+        u64 pos = bc, mass = bm;
+        for (int j = 0; j < (int)members; ++j)
+          if (ll[j] > l || (ll[j] == l && li[j] < idx)) { ++pos; mass += lw[j]; }
+        const u64 at = by_mass ? mass : pos, next = at + (by_mass ? lw[i] : 1);
+        if (at < goal && (next >= goal || pos + 1 == bc + members)) {
+          for (int r = 0; r < row.ctas; ++r) {
+            put_u64(&sh->found[0], r, ((u64)__float_as_uint(l) << 32) | idx);
+            put_u64(&sh->found[1], r, mass + lw[i]);
+          }
+        }
+      }
+    }
+    row_sync(row.ctas);
+    Cut c;
+    c.l = __uint_as_float((uint32_t)(sh->found[0] >> 32));
+    c.i = (int)(uint32_t)sh->found[0];
+    c.mass = sh->found[1];
+    __syncthreads();
+    return c;
+  }
+  // Many members within a hundred-thousandth of a factor of two: the smallest key above which less than the goal lies, by halving, then its ties in order.
+  u64 top = 0, low = ALL;
+  for (int i = threadIdx.x; i < n; i += NT)
+    if (member(vals[i])) { const u64 k = ordered(vals[i]); top = top > k ? top : k; low = low < k ? low : k; }
+  row.extremes(top, low);
+  auto above = [&](u64 key, u64& c, u64& w, u64& ties) {      // what lies above a key among the members, and before them
+    c = w = 0;
+    u64 t = 0, unused = 0;
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const float l = vals[i];
+      if (!member(l)) continue;
+      const u64 k = ordered(l);
+      if (k > key) { ++c; if (weighted) { double x; w += row_weight(l, rs, sh->tab, x); } }
+      t += k == key;
+    }
+    row.sum(c, w);
+    row.sum(t, unused);
+    c += bc; w += bm; ties = t;
+  };
+  u64 c = 0, w = 0, ties = 0;
+  while (low < top) {
+    const u64 mid = (low + top) >> 1;
+    above(mid, c, w, ties);
+    if ((by_mass ? w : c) < goal) top = mid; else low = mid + 1;
+  }
+  above(top, c, w, ties);
+  Cut cut;
+  cut.l = unordered((uint32_t)top);
+  double x;
+  const u64 each = weighted ? row_weight(cut.l, rs, sh->tab, x) : 0;
+  u64 take = by_mass ? (each ? (goal - w + each - 1) / each : ties) : goal - c;
+  if (take > ties) take = ties;
+  cut.mass = w + take * each;
+  // the take-th tie in the order of indices
+  const int chunk = ((n + NT - 1) / NT) | 1, first = min(n, (int)threadIdx.x * chunk), last = min(n, first + chunk);
+  u64 mine = 0, total;
+  for (int i = first; i < last; ++i) mine += vals[i] == cut.l;
+  u64 at = row.before(mine, total);
+  if (at < take && at + mine >= take)
+    for (int i = first; i < last; ++i)
+      if (vals[i] == cut.l && ++at == take)
+        for (int r = 0; r < row.ctas; ++r) put_u64(&sh->found[0], r, (u64)(base + i));
+  row_sync(row.ctas);
+  cut.i = (int)sh->found[0];
+  __syncthreads();
+  return cut;
+}
+
+template <typename T> struct Vec16;
+template <> struct Vec16<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void read(const float* p, float (&v)[4]) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  }
+};
+template <> struct Vec16<bf16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void read(const bf16* p, float (&v)[8]) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+  }
+};
+
+struct CutArgs {
+  long long pitch;
+  int vocab, per;      // of a CTA's slice
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* uniform;
+  int* out;
+  float* logprobs;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutArgs a) {
+  extern __shared__ __align__(16) unsigned char cut_smem[];
+  __shared__ CutShared shared;
+  CutShared* sh = &shared;
+  float* vals = reinterpret_cast<float*>(cut_smem);
+  CutMemory mem;
+  mem.row_mass = reinterpret_cast<u64*>(cut_smem + (size_t)((a.per + 3) & ~3) * 4);
+  mem.sub_mass = mem.row_mass + BINS;
+  mem.count = reinterpret_cast<uint32_t*>(mem.sub_mass + SUBS);
+  mem.lo = mem.count + BINS;
+  mem.hi = mem.lo + BINS;
+  mem.row_count = mem.hi + BINS;
+  mem.sub_count = mem.row_count + BINS;
+  Row row = {sh, cluster_size(), cluster_rank(), 0};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long long r = blockIdx.x / row.ctas;
+  const int base = min((long long)a.vocab, (long long)row.rank * a.per), n = min(a.vocab - base, a.per);
+  if (tid < 32) sh->tab.t[tid] = exp2(tid / 32.0);
+  for (int b = tid; b < BINS; b += NT) mem.count[b] = mem.lo[b] = mem.hi[b] = 0;
+  if (row.ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+
+  // ---- the slice into shared memory, and its best token
+  const T* src = logits + r * a.pitch + base;
+  float bv = -INFINITY;
+  int bi = 0x7fffffff;
+  auto take = [&](float v, int i) {
+    v = v == v ? v + 0.f : -INFINITY;      // -0 becomes 0
+    if (v > bv) { bv = v; bi = i; }
+    vals[i] = v;
+  };
+  constexpr int N = Vec16<T>::N;
+  int done = 0;
+  if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    done = n / N * N;
+#pragma unroll 4
+    for (int i = tid * N; i < done; i += NT * N) {
+      float v[N];
+      Vec16<T>::read(src + i, v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) take(v[j], i + j);
+    }
+  }
+  for (int i = done + tid; i < n; i += NT) take(to_f32<T>(src[i]), i);
+  bi = bi == 0x7fffffff ? bi : bi + base;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
+    const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+    if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
+  }
+  if (row.ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // every peer has begun: its shared memory may be written
+  // (largest first, then lowest index, as one whole number)
+  u64 best = ((u64)ordered(bv) << 32) | (uint32_t)~bi, dummy = ALL;
+  row.extremes(best, dummy);
+  const float m = unordered((uint32_t)(best >> 32));
+  const int first_token = (int)~(uint32_t)best;
+
+  const float temp = a.temperature[r];
+  if (!(temp > 0.f) || m == -INFINITY) {
+    if (row.rank == 0 && tid == 0) {
+      a.out[r] = m == -INFINITY ? 0 : first_token;
+      if (a.logprobs) a.logprobs[r] = m == -INFINITY ? __uint_as_float(0x7fc00000u) : 0.f;
+    }
+    row_sync(row.ctas);      // nobody leaves while a peer may write to it
+    return;
+  }
+  RowScale rs;
+  rs.m = m;
+  rs.s = 1.4426950408889634074 / (double)temp;
+  rs.to_bin = (float)fmin(rs.s * (BINS / (double)REACH), 3e38);
+  const int k = a.top_k ? a.top_k[r] : 0;
+  const float p = a.top_p ? a.top_p[r] : 1.f;
+  const double least = a.min_p ? (double)a.min_p[r] * UNIT : 0.0;
+  const bool by_count = k >= 1 && k < a.vocab, by_mass = p < 1.f;
+
+  // ---- what top-k and top-p keep
+  Cut cut = {-INFINITY, 0x7fffffff, 0};
+  if (by_count || by_mass) {
+    for (int i = tid; i < n; i += NT) {
+      const float l = vals[i], f = row_bin(l, rs);
+      if (!(f < BINS)) continue;
+      atomicAdd(mem.count + (int)f, 1u);
+      if (by_mass) { double w; add_mass(mem.lo, mem.hi, (int)f, row_weight(l, rs, sh->tab, w)); }
+    }
+    merge_bins(row, BINS, mem.count, mem.lo, mem.hi, mem.row_count, mem.row_mass, by_mass);
+    if (by_mass) {
+      u64 x = 0, unused = 0;
+      for (int b = tid; b < BINS; b += NT) x += mem.row_mass[b];
+      // (every CTA has the row's bins: their sum needs no peer)
+      x = warp_add(x);
+      __syncthreads();
+      if (lane == 0) sh->warp_a[warp] = x;
+      __syncthreads();
+      for (int w = 0; w < NW; ++w) unused += sh->warp_a[w];
+      cut.mass = unused;
+      __syncthreads();
+    }
+    if (by_count) cut = find_cut(row, mem, vals, n, base, rs, false, (u64)k, by_mass, cut);
+    if (by_mass) {
+      const double want = ceil((double)p * (double)cut.mass);
+      cut = find_cut(row, mem, vals, n, base, rs, true, want >= 1.0 ? (u64)want : 1, true, cut);
+    }
+  }
+
+  // ---- the draw: a thread has tokens one after the other
+  const int chunk = ((n + NT - 1) / NT) | 1, first = min(n, tid * chunk), last = min(n, first + chunk);      // (odd: no two threads of a warp on a bank)
+  auto weigh = [&](int i) -> u64 {
+    const float l = vals[i];
+    if (!kept(l, base + i, cut)) return 0;
+    double w;
+    const u64 whole = row_weight(l, rs, sh->tab, w);
+    return w >= least || l == m ? whole : 0;
+  };
+  u64 mine = 0, total;
+  for (int i = first; i < last; ++i) mine += weigh(i);
+  u64 at = row.before(mine, total);
+  const float u = a.uniform[r];
+  u64 goal = u > 0.f ? (u64)((double)u * (double)total) : 0;
+  if (goal >= total) goal = total - 1;
+  if (at <= goal && at + mine > goal) {
+    for (int i = first; i < last; ++i) {
+      at += weigh(i);
+      if (at > goal) {
+        a.out[r] = base + i;
+        if (a.logprobs) {
+          const float l = vals[i];
+          a.logprobs[r] = (float)((l == m ? 0.0 : ((double)l - (double)m) / (double)temp) - log((double)total / UNIT));
+        }
+        break;
+      }
+    }
+  }
+  row_sync(row.ctas);
+}
+
+// logits [rows, vocab] with rows `pitch` elements apart (dtype IFB_F32 or IFB_BF16); per row: temperature, uniform number, and top_k, top_p, min_p (each or
+// null); out int32, logprobs float32 or null.
+IFB_EXPORT int ifb_sample_cut_max_vocab() { return MAX_CLUSTER * SLICE; }
+IFB_EXPORT int ifb_sample_cut(const void* logits, int dtype, long long pitch, int rows, int vocab, const float* temperature, const float* uniform,
+                              const int* top_k, const float* top_p, const float* min_p, int* out, float* logprobs, cudaStream_t stream) {
+  if (rows <= 0) return IFB_OK;
+  if (vocab < 1 || vocab > MAX_CLUSTER * SLICE || rows > (1 << 27)) return IFB_ERR_SIZE;
+  if (!temperature || !uniform || !out) return IFB_ERR_ARG;
+  // As few CTAs of a row as let two share an SM; more while the rows leave SMs idle.
+  const int sms = ifb_sm_count();
+  int ctas = 1;
+  while (ctas < MAX_CLUSTER && ((vocab + ctas - 1) / ctas > SHARED_SLICE || ((long long)rows * ctas * 2 <= 2 * sms && vocab / ctas >= 2048))) ctas *= 2;
+  CutArgs a = {pitch, vocab, ((vocab + ctas - 1) / ctas + 7) & ~7, temperature, top_k, top_p, min_p, uniform, out, logprobs};
+  const size_t smem = (size_t)a.per * 4 + CUT_BYTES;
+  auto go = [&](auto kernel, auto typed) -> int {
+    IFB_ALLOW_SMEM(kernel, smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)rows * ctas);
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ifb_pdl_enabled() ? 2 : 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, typed, a);
+    if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
+    return IFB_OK;
+  };
+  if (dtype == IFB_F32) return go(sample_cut_kernel<float>, (const float*)logits);
+  if (dtype == IFB_BF16) return go(sample_cut_kernel<bf16>, (const bf16*)logits);
+  return IFB_ERR_DTYPE;
+}
+
+// ---------------------------------------------------------------------------------------------------- log probabilities
+// token_logprobs.  log p = l_t - m - log(1 + s), m the row's largest logit and s the sum of e^(l - m) over all tokens but one of the largest: with
+// log(1 + s) apart from the leading 1 a token that is nearly certain keeps its digits.  The rank is the number of tokens that come before t in the order of
+// falling logits, equal ones by rising index.  One pass over the row: running maximum and sum (32 bits, combined in 64 at the end), and two counts:
+// what lies at or above l_t ahead of t, and above it behind t.  A row with a NaN or +inf, or with no number above -inf, gives NaN; a token outside the
+// vocabulary NaN and -1.
+constexpr int LP_NT = 256;
+constexpr int LP_NW = LP_NT / 32;
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float lp_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+struct LpSum { float m, s; };      // the largest number so far, and the sum over all but one of it
+__device__ __forceinline__ LpSum lp_join(LpSum a, LpSum b) {
+  if (a.m < b.m) { const LpSum t = a; a = b; b = t; }
+  if (b.m != -INFINITY) a.s += (1.f + b.s) * lp_exp2((b.m - a.m) * LOG2E);
+  else a.s += b.s;      // (0, or NaN)
+  return a;
+}
+template <int N> __device__ __forceinline__ void lp_take(LpSum& t, const float (&v)[N]) {
+  float top = v[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) top = fmaxf(top, v[j]);
+  if (top > t.m) {
+    t.s = t.m == -INFINITY ? t.s : (1.f + t.s) * lp_exp2((t.m - top) * LOG2E);
+    t.m = top;
+    int ties = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const bool tie = v[j] == top;
+      ties += tie;
+      t.s += tie ? 0.f : lp_exp2((v[j] - top) * LOG2E);
+    }
+    t.s += (float)(ties - 1);
+  } else {
+    const float m = t.m == -INFINITY ? 0.f : t.m;
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < N; ++j) s[j & 1] += lp_exp2((v[j] - m) * LOG2E);
+    t.s += s[0] + s[1];
+  }
+}
+struct LpBox { LpSum sum; int count; int pad; };
+
+template <typename T>
+__global__ void __launch_bounds__(LP_NT) token_logprob_kernel(const T* logits, long long pitch, int vocab, int per, const int* tokens, float* out, int* ranks) {
+  __shared__ LpBox warps[LP_NW];
+  __shared__ LpBox boxes[MAX_CLUSTER];
+  const int ctas = cluster_size(), rank = cluster_rank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long long r = blockIdx.x / ctas;
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  const int token = tokens[r];
+  const T* row = logits + r * pitch;
+  const int base = min((long long)vocab, (long long)rank * per), n = min(vocab - base, per);
+  const bool valid = token >= 0 && token < vocab;
+  const float lt = valid ? to_f32<T>(row[token]) : 0.f;
+  const T* src = row + base;
+  const int t = max(0, min(n, token - base));      // numbers of this slice ahead of the token
+  constexpr int N = Vec16<T>::N;
+  LpSum sum = {-INFINITY, 0.f};
+  int count = 0;
+  const int vecs = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? n / N : 0;
+  // whole vectors ahead of the token, then those behind it
+  auto run = [&](int from, int to, auto ahead) {
+    constexpr int U = sizeof(T) == 4 ? 4 : 2;      // vectors at a time: 16 numbers
+    int i = from + tid;
+    for (; i + (U - 1) * LP_NT < to; i += U * LP_NT) {
+      float v[U * N];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float w[N];
+        Vec16<T>::read(src + (size_t)(i + u * LP_NT) * N, w);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[u * N + j] = w[j];
+      }
+      lp_take(sum, v);
+#pragma unroll
+      for (int j = 0; j < U * N; ++j) count += decltype(ahead)::value ? v[j] >= lt : v[j] > lt;
+    }
+    for (; i < to; i += LP_NT) {
+      float v[N];
+      Vec16<T>::read(src + (size_t)i * N, v);
+      lp_take(sum, v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) count += decltype(ahead)::value ? v[j] >= lt : v[j] > lt;
+    }
+  };
+  auto one = [&](int i) {
+    const float v[1] = {to_f32<T>(src[i])};
+    lp_take(sum, v);
+    count += i < t ? v[0] >= lt : v[0] > lt;
+  };
+  const int split = min(vecs, t / N);
+  run(0, split, std::true_type());
+  if (split < vecs && tid < N) one(split * N + tid);      // the vector that the token may be in
+  run(split + 1, vecs, std::false_type());
+  for (int i = vecs * N + tid; i < n; i += LP_NT) one(i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const LpSum x = {__shfl_xor_sync(0xffffffffu, sum.m, o), __shfl_xor_sync(0xffffffffu, sum.s, o)};
+    sum = lp_join(sum, x);
+    count += __shfl_xor_sync(0xffffffffu, count, o);
+  }
+  if (lane == 0) warps[warp] = {sum, count, 0};
+  if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < LP_NW; ++w) { sum = lp_join(sum, warps[w].sum); count += warps[w].count; }
+    if (ctas > 1) {
+      put_u64(reinterpret_cast<u64*>(&boxes[rank].sum), 0, ((u64)__float_as_uint(sum.s) << 32) | __float_as_uint(sum.m));
+      put_u32(reinterpret_cast<uint32_t*>(&boxes[rank].count), 0, (uint32_t)count);
+    }
+  }
+  if (ctas > 1) {
+    row_sync(ctas);
+    if (rank != 0) return;
+  }
+  if (tid == 0) {
+    if (ctas > 1) {
+      sum = boxes[0].sum; count = boxes[0].count;
+      for (int c = 1; c < ctas; ++c) { sum = lp_join(sum, boxes[c].sum); count += boxes[c].count; }
+    }
+    const bool nan = !valid || sum.m == INFINITY || sum.m == -INFINITY;
+    out[r] = nan ? __uint_as_float(0x7fc00000u) : (float)((double)lt - (double)sum.m - log1p((double)sum.s));
+    if (ranks) ranks[r] = valid ? count : -1;
+  }
+}
+
+IFB_EXPORT int ifb_token_logprobs(const void* logits, int dtype, long long pitch, int rows, int vocab, const int* tokens, float* out, int* ranks,
+                                  cudaStream_t stream) {
+  if (rows <= 0) return IFB_OK;
+  if (vocab < 1 || vocab > (1 << 30) || rows > (1 << 27)) return IFB_ERR_SIZE;
+  if (!tokens || !out) return IFB_ERR_ARG;
+  // several CTAs of a row while the rows leave room on the SMs (eight CTAs fit on each)
+  const int sms = ifb_sm_count();
+  int ctas = 1;
+  while (ctas < MAX_CLUSTER && (long long)rows * ctas * 2 <= 4 * sms && vocab / ctas >= 4096) ctas *= 2;
+  const int per = ((vocab + ctas - 1) / ctas + 7) & ~7;
+  auto go = [&](auto kernel, auto typed) -> int {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)rows * ctas);
+    cfg.blockDim = dim3(LP_NT);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ifb_pdl_enabled() ? 2 : 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, typed, pitch, vocab, per, tokens, out, ranks);
+    if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
+    return IFB_OK;
+  };
+  if (dtype == IFB_F32) return go(token_logprob_kernel<float>, (const float*)logits);
+  if (dtype == IFB_BF16) return go(token_logprob_kernel<bf16>, (const bf16*)logits);
+  return IFB_ERR_DTYPE;
+}

@@ -14,6 +14,7 @@ from ctypes import c_float, c_int, c_longlong, c_void_p
 import torch
 
 from ..errors import KernelError
+from .answers import AnswerKernels
 from .build import load_library
 from .low_bits import LowBitKernels, Mx4Matrix
 
@@ -62,7 +63,7 @@ def _dense(t, name, dtype=None):
     return t
 
 
-class CudaKernels(LowBitKernels):
+class CudaKernels(LowBitKernels, AnswerKernels):
     name = "cuda"
     takes_exact_lens = True        # paged_attention's ``exact_lens``
 
