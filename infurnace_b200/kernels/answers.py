@@ -1,10 +1,12 @@
-"""Several answers to one prompt: drawing tokens under top-k, top-p and min-p, and the log probabilities of tokens.
+"""Several answers to one prompt: drawing tokens under top-k, top-p and min-p, the log probabilities of tokens, and attention over
+pages that requests share.
 
-:class:`AnswerKernels` is the calls (a part of the kernel set).  What is drawn, and how, is defined at the head of ``csrc/sampling.cu``.
+:class:`AnswerKernels` is the calls (a part of the kernel set).  What is drawn, and how, is defined at the head of ``csrc/sampling.cu``, how
+attention is cut into pieces at the head of ``csrc/attention_shared.cuh``.
 """
 from __future__ import annotations
 
-from ctypes import c_int, c_longlong, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -104,4 +106,91 @@ class AnswerKernels:
         with torch.cuda.device(index):
             self.launches += 1
             _status(self._sampling_lib().ifb_token_logprobs(logits.data_ptr(), code, pitch, rows, vocab, *args, _raw_stream(index)), "token_logprobs")
+        return out
+
+    # ------------------------------------------------------------------ attention over shared pages
+    _shared = None
+
+    def _shared_lib(self):
+        if self._shared is None:
+            lib = load_library("attention_shared", progress=self._progress)
+            lib.ifb_attention_shared.argtypes = ([c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_int]
+                                                 + [c_void_p] * 7 + [c_int] * 7 + [c_float, c_int, c_void_p])
+            lib.ifb_attention_shared_room.argtypes = [c_int] * 6
+            lib.ifb_attention_shared_room.restype = c_longlong
+            self._shared = lib
+        return self._shared
+
+    def shared_prefix_room(self, tokens, requests, groups, heads, kv_heads, head_dim):
+        """Bytes of the room that ``shared_prefix_attention`` takes for a step of so many tokens, requests and groups."""
+        return int(self._shared_lib().ifb_attention_shared_room(tokens, requests, groups, kv_heads, heads // kv_heads, head_dim))
+
+    def shared_prefix_attention(self, q, kv_pages, block_tables, cu_q, seq_lens, cu_groups, shared_lens, out, scale, window, max_q_len, max_seq_len,
+                                room=None):
+        """``paged_attention`` for requests whose block tables share leading pages, which are then read once for all of them: answers to one
+        prompt, questions to one document, conversations behind one system prompt.
+
+        ``q`` and ``out`` are bfloat16 or float32 [tokens, heads, head_dim] (the rows of ``q`` may lie apart, those of ``out`` not), ``kv_pages`` [pages, 2,
+        kv_heads, page_size, head_dim] of the same type.  Request r has the rows cu_q[r] .. cu_q[r + 1] - 1 and ``seq_lens[r]`` keys, these
+        queries' own among them, in the pages of ``block_tables[r]``; the query at position p sees positions max(0, p - window + 1) .. p
+        (``window`` 0: from 0).  Group g is the requests cu_groups[g] .. cu_groups[g + 1] - 1, the first ``shared_lens[g]`` keys of which are the same: they are
+        read through the table of its first request.  (Any number of keys; beyond them each request's own table counts, also within
+        a page.)  Requests of no group share nothing.  A row that sees no key becomes zero; rows behind the last request stay as they are.
+        ``cu_q``, ``seq_lens``, ``block_tables``, ``cu_groups`` [groups + 1] and ``shared_lens`` [groups] are int32 on the device.  No request has more than
+        ``max_q_len`` queries or ``max_seq_len`` keys.  An entry of a table that is read and is no page of the pool counts as zeros and is recorded in the
+        kernels' error word.
+
+        ``room``: None, or a uint8 tensor of at least ``shared_prefix_room`` bytes for the pieces' sums, in place of memory of the allocator's (within
+        a recording: of the graph's own pool); calls that share one follow one another."""
+        code = _CODES.get(q.dtype)
+        shape, index = q.shape, q.get_device()
+        n, heads, dim = shape if len(shape) == 3 else (0, 0, 0)
+        pool = kv_pages.shape
+        if code is None or out.dtype != q.dtype or out.shape != shape or kv_pages.dtype != q.dtype or len(pool) != 5 or pool[1] != 2 \
+                or pool[4] != dim or pool[2] < 1 or heads % pool[2] or heads == 0:
+            raise KernelError(f"shared_prefix_attention: q and out are bfloat16 or float32 [tokens, heads, head_dim] and kv_pages [pages, 2, kv_heads, page_size, "
+                              f"head_dim] of one type, heads a multiple of kv_heads; got {q.dtype} {tuple(shape)}, {out.dtype} {tuple(out.shape)} and "
+                              f"{kv_pages.dtype} {tuple(pool)}")
+        pages, _, kv_heads, page_size, _ = pool
+        group = heads // kv_heads
+        if dim % 16 or not 16 <= dim <= 256 or group > 64:
+            raise KernelError(f"shared_prefix_attention: head_dim is a multiple of 16 up to 256, with up to 64 query heads for a key head; got {dim} and {group}")
+        if q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim) or not out.is_contiguous():
+            raise KernelError("shared_prefix_attention: the heads of a query lie one after the other, and out is contiguous")
+        block = 2 * kv_heads * page_size * dim
+        page_stride = kv_pages.stride(0) if pages > 1 else block
+        if pages < 1 or not kv_pages[0].is_contiguous() or page_stride < block:
+            raise KernelError("shared_prefix_attention: the numbers of a page lie one after the other")
+        r, groups = seq_lens.numel(), shared_lens.numel()
+        table = block_tables.shape
+        for t, name, count in ((cu_q, "cu_q", r + 1), (seq_lens, "seq_lens", r), (cu_groups, "cu_groups", groups + 1), (shared_lens, "shared_lens", groups)):
+            if t.dtype != torch.int32 or t.shape != (count,) or not t.is_contiguous():
+                raise KernelError(f"shared_prefix_attention: {name} is int32 [{count}], contiguous; got {t.dtype} {tuple(t.shape)}")
+        if block_tables.dtype != torch.int32 or len(table) != 2 or table[0] < r or (table[1] > 1 and block_tables.stride(1) != 1):
+            raise KernelError("shared_prefix_attention: block_tables is int32 [requests, pages] with unit stride along pages")
+        if index < 0 or any(t.get_device() != index for t in (kv_pages, out, block_tables, cu_q, seq_lens, cu_groups, shared_lens)):
+            raise KernelError("shared_prefix_attention: all tensors are on one CUDA device")
+        if window < 0 or max_q_len < 1 or max_seq_len < 0:
+            raise KernelError("shared_prefix_attention: window and max_seq_len are not negative, max_q_len is positive")
+        if table[1] * page_size < max_seq_len:
+            raise KernelError(f"shared_prefix_attention: block tables of {table[1]} pages do not hold {max_seq_len} keys")
+        if r + groups > 2048:
+            raise KernelError(f"shared_prefix_attention: {r} requests and {groups} groups; at most 2,048 together")
+        if n == 0 or r == 0:
+            return out
+        q_row = q.stride(0) if n > 1 else heads * dim
+        with torch.cuda.device(index):
+            lib = self._shared_lib()
+            size = lib.ifb_attention_shared_room(n, r, groups, kv_heads, group, dim)
+            if room is None:
+                room = torch.empty(size, dtype=torch.uint8, device=q.device)
+            elif room.dtype != torch.uint8 or room.dim() != 1 or not room.is_contiguous() or room.numel() < size or room.data_ptr() % 256 \
+                    or room.get_device() != index:
+                raise KernelError(f"shared_prefix_attention: a room is uint8 [{size} or more], contiguous, on 256 bytes, on the same device")
+            self.launches += 2
+            self._err_armed = True
+            _status(lib.ifb_attention_shared(q.data_ptr(), code, q_row, kv_pages.data_ptr(), page_stride, pages, block_tables.data_ptr(),
+                                             block_tables.stride(0), table[1], cu_q.data_ptr(), seq_lens.data_ptr(), cu_groups.data_ptr(),
+                                             shared_lens.data_ptr(), out.data_ptr(), room.data_ptr(), self._dev_err_at, n, r, groups, heads, kv_heads,
+                                             dim, page_size, scale, window, _raw_stream(index)), "shared_prefix_attention")
         return out

@@ -54,6 +54,8 @@ LIBRARIES: Dict[str, tuple] = {
     "kv8_attention_f32": (["kv8_attention_f32.cu"], []),
     # drawing tokens under top-k, top-p and min-p, log probabilities of tokens
     "sampling": (["sampling.cu"], []),
+    # attention over pages that requests share, in 32-bit arithmetic
+    "attention_shared": (["attention_shared.cu"], []),
     # compiled once per head size: defines={"HEAD_DIM": d}
     "attention_mma": (["attention_mma.cu"], []),
 }
@@ -220,7 +222,7 @@ def build_all(progress=None) -> List[str]:
     """Compile every library (used by the build check; needs no GPU)."""
     from concurrent.futures import ThreadPoolExecutor
     jobs = [("core", None), ("linear_tcgen05", None), ("linear_skinny_static", None), ("attention_tc", None),
-            ("mixers", None), ("hybrid", None), ("latent", None), ("mx4", None), ("kv8", None), ("sampling", None)] + DEFAULT_VARIANTS
+            ("mixers", None), ("hybrid", None), ("latent", None), ("mx4", None), ("kv8", None), ("sampling", None), ("attention_shared", None)] + DEFAULT_VARIANTS
     with ThreadPoolExecutor(max_workers=4) as pool:
         built = list(pool.map(lambda j: compile_library(j[0], j[1], progress), jobs))
     # objects of older sources are never loaded (their names carry another hash); take them out of the folder

@@ -375,6 +375,9 @@ class CudaKernels(LowBitKernels, AnswerKernels):
                 if code == 900:
                     raise KernelError("a token id outside the vocabulary reached the embedding (code 900): the step "
                                       "that sampled it had no valid logits; its output is not valid")
+                if code == 940:
+                    raise KernelError("attention over shared pages read a block-table entry that is no page of the pool (code 940): it "
+                                      "counted as zeros")
                 raise KernelError(f"a kernel gave up waiting on a barrier (code {code}); its output is not valid")
 
     def _linear_gemv(self, x, w, out, n, o, k, epi, row_scale=None, bias=None):

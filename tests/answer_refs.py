@@ -42,3 +42,31 @@ def logprob_row(logits, token):
         return math.nan, rank
     rest = torch.sort(x, descending=True)[0]
     return (x[token] - rest[0] - torch.log1p(torch.exp(rest[1:] - rest[0]).sum())).item(), rank
+
+
+def attention(q, pages, tables, cu_q, seq_lens, cu_groups, shared_lens, scale, window):
+    """Each request by itself, over the keys of its own table but for those that its group shares, which are its first request's."""
+    n, heads, dim = q.shape
+    _, _, kv_heads, page, _ = pages.shape
+    group = heads // kv_heads
+    out = torch.zeros((n, heads, dim), dtype=torch.float64)
+    weight_sum = torch.zeros((n, heads, dim), dtype=torch.float64)          # sum of |weight value|, for tolerances
+    for r, length in enumerate(seq_lens):
+        rows = range(cu_q[r], cu_q[r + 1])
+        if length == 0 or not len(rows):
+            continue
+        g = next((g for g in range(len(shared_lens)) if cu_groups[g] <= r < cu_groups[g + 1]), None)
+        slots = [int(tables[r if g is None or i >= shared_lens[g] else cu_groups[g], i // page]) * page + i % page for i in range(length)]
+        slots = torch.tensor(slots)
+        kv = pages[slots // page, :, :, slots % page].double()               # [keys, 2, kv_heads, dim]
+        for i, row in enumerate(rows):
+            p = length - len(rows) + i
+            lo = max(0, p - window + 1) if window else 0
+            if p < lo:
+                continue
+            for h in range(heads):
+                k, v = kv[lo:p + 1, 0, h // group], kv[lo:p + 1, 1, h // group]
+                w = torch.softmax(k @ q[row, h].double() * scale, 0)
+                out[row, h] = w @ v
+                weight_sum[row, h] = w @ v.abs()
+    return out, weight_sum
