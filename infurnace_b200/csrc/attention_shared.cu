@@ -27,23 +27,22 @@ __device__ __forceinline__ void sh_row4(float* dst, const T* src, bool valid) { 
 template <typename T, int DC>
 __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(Call c, const T* q, long long q_row, const T* pages, int dim) {
   extern __shared__ __align__(16) unsigned char sh_smem[];
-  __shared__ long long warp_sums[SH_THREADS / 32];
-  long long* starts = reinterpret_cast<long long*>(sh_smem);
+  const Plan plan = plan_at(sh_smem, c.n_groups + c.n_req);
   const int pitch = dim + 4;
-  float* Q = reinterpret_cast<float*>(starts + ((c.n_groups + c.n_req + 2) & ~1));      // [64][pitch]
+  float* Q = reinterpret_cast<float*>(sh_smem + plan_bytes(c.n_groups + c.n_req));      // [64][pitch]
   float* Ks = Q + SH_ROWS * pitch;                                                      // [32][pitch]
   float* Vs = Ks + SH_UNIT * pitch;
   float* P = Vs + SH_UNIT * pitch;                                                      // [64][33]
   ifb_pdl_wait();
   ifb_pdl_trigger();
-  plan(c, starts, warp_sums);
+  make_plan(c, plan);
   Walk walk;
-  walk.begin(c, starts, blockIdx.x);
+  walk.begin(c, plan, blockIdx.x);
   const int tid = threadIdx.x, x = tid & 7, y = tid >> 3, quads = dim / 4;
   const int group = c.heads / c.kv_heads;
   const long long values = (long long)c.kv_heads * c.page_size * dim;      // from a page's keys to its values
   Piece p;
-  while (walk.next(c, starts, p)) {
+  while (walk.next(c, plan, p)) {
     const int rows = p.tokens * group;
     __syncthreads();      // the piece before has read its tiles
     for (int i = tid; i < SH_ROWS * quads; i += SH_THREADS) {
@@ -55,7 +54,7 @@ __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(Call c, const T
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int row = 2 * y + e;
-      const int pos = row < rows ? row_position(c, p.w, p.row0 + row / group) : NO_POSITION;
+      const int pos = row < rows ? row_position(c, plan, p.w, p.row0 + row / group) : NO_POSITION;
       hi[e] = min(pos + 1, p.last);      // the row sees lo .. hi - 1 of the piece
       lo[e] = max(p.lo, c.window > 0 ? pos - c.window + 1 : 0);
 #pragma unroll
@@ -162,14 +161,14 @@ static Call sh_call(int n_tokens, int n_req, int n_groups, int kv_heads, int gro
   Call c = {};
   c.n_tokens = n_tokens; c.n_req = n_req; c.n_groups = n_groups;
   c.kv_heads = kv_heads; c.heads = kv_heads * group;
-  c.tokens = SH_ROWS / group; c.unit = SH_UNIT; c.rows = SH_ROWS;
+  c.tokens = SH_ROWS / group; c.unit = SH_UNIT; c.rows = SH_ROWS; c.align = 1;
   c.ctas = ifb_sm_count();
   return c;
 }
 // (one function for each kernel: what IFB_ALLOW_SMEM remembers is a kernel's)
 template <typename T, int DC>
 static int sh_main(const Call& c, const T* q, long long q_row, const T* pages, int dim, cudaStream_t stream) {
-  const size_t smem = (size_t)((c.n_req + c.n_groups + 2) & ~1) * 8 + (size_t)((SH_ROWS + 2 * SH_UNIT) * (dim + 4) + SH_ROWS * 33) * 4;
+  const size_t smem = plan_bytes(c.n_req + c.n_groups) + (size_t)((SH_ROWS + 2 * SH_UNIT) * (dim + 4) + SH_ROWS * 33) * 4;
   IFB_ALLOW_SMEM((shared_simt_kernel<T, DC>), smem);
   return ifb_launch(shared_simt_kernel<T, DC>, dim3(c.ctas), dim3(SH_THREADS), smem, stream, c, q, q_row, pages, dim);
 }

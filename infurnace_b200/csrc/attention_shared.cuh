@@ -37,6 +37,7 @@ struct Call {
   int table_pages, page_size, window;
   float scale_log2;
   int tokens, unit, rows;                // of a tile (rows = tokens x heads of a key head, at most), of a unit
+  int align;                             // an item's first key is a multiple of this
   int ctas;
   float* part_o;                         // [slots][rows][dim]
   float2* part_ml;                       // [slots][rows]: largest score (base 2), sum of weights
@@ -54,8 +55,8 @@ struct Owner {
   int row0, row1;            // query rows
   int request;               // whose table holds the keys (a group: its first request's)
   int lo, hi;                // keys lo .. hi - 1 at most
-  int p_first;               // a request: the position of its first row; a group: of no use
-  bool group;
+  int group;                 // whether it is one
+  __device__ __forceinline__ int p_first() const { return hi - (row1 - row0); }      // a request: the position of its first row
 };
 __device__ __forceinline__ int request_row(const Call& c, int r) { return clamp(c.cu_q[r], 0, c.n_tokens); }
 __device__ __forceinline__ int request_len(const Call& c, int r) { return clamp(c.seq_lens[r], 0, (int)min((long long)c.table_pages * c.page_size, 0x7fffff00LL)); }
@@ -72,16 +73,6 @@ __device__ __forceinline__ int group_of(const Call& c, int r) {
   }
   return lo;
 }
-// The request of a query row, the first in [r0, r1) whose rows end behind it.
-__device__ __forceinline__ int request_of(const Call& c, int row, int r0, int r1) {
-  int lo = r0, hi = r1 - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (request_row(c, mid + 1) <= row) lo = mid + 1; else hi = mid;
-  }
-  return lo;
-}
-
 __device__ __forceinline__ Owner owner_at(const Call& c, int o) {
   Owner w;
   w.group = o < c.n_groups;
@@ -92,7 +83,6 @@ __device__ __forceinline__ Owner owner_at(const Call& c, int o) {
     w.row1 = max(w.row0, request_row(c, r1));
     w.lo = 0;
     w.hi = shared_len(c, o);
-    w.p_first = 0;
     if (c.window > 0) {      // no row sees a key before this
       int first = w.hi;
       for (int r = r0; r < r1; ++r) first = min(first, request_len(c, r) - (request_row(c, r + 1) - request_row(c, r)) - c.window + 1);
@@ -106,7 +96,6 @@ __device__ __forceinline__ Owner owner_at(const Call& c, int o) {
     w.row1 = max(w.row0, request_row(c, r + 1));
     w.lo = g >= 0 ? shared_len(c, g) : 0;
     w.hi = request_len(c, r);
-    w.p_first = w.hi - (w.row1 - w.row0);
   }
   return w;
 }
@@ -115,7 +104,7 @@ __device__ __forceinline__ int owner_item(const Call& c, const Owner& w, int o) 
   return w.group ? (w.row0 / c.tokens + o) * c.kv_heads : prefix_items(c) + (w.row0 / c.tokens + o - c.n_groups) * c.kv_heads;
 }
 
-// The keys that a tile's rows can see (first .. last - 1), the first rounded down to a unit.
+// The keys that a tile's rows can see (lo .. last - 1), and where their units begin.
 struct Span { int first, last, lo, units; };
 __device__ __forceinline__ Span tile_span(const Call& c, const Owner& w, int tile) {
   Span s;
@@ -123,10 +112,10 @@ __device__ __forceinline__ Span tile_span(const Call& c, const Owner& w, int til
   s.last = w.hi;
   if (!w.group) {
     const int t0 = tile * c.tokens, t1 = min(w.row1 - w.row0, t0 + c.tokens);
-    if (c.window > 0) s.lo = max(s.lo, w.p_first + t0 - c.window + 1);
-    s.last = min(s.last, w.p_first + t1);
+    if (c.window > 0) s.lo = max(s.lo, w.p_first() + t0 - c.window + 1);
+    s.last = min(s.last, w.p_first() + t1);
   }
-  s.first = s.lo / c.unit * c.unit;
+  s.first = s.lo / c.align * c.align;
   s.units = s.last > s.lo ? (s.last - s.first + c.unit - 1) / c.unit : 0;
   return s;
 }
@@ -139,15 +128,33 @@ __device__ inline long long owner_units(const Call& c, const Owner& w) {
   return u * c.kv_heads;
 }
 
-// The owners' first units, in shared memory: starts[o], and the sum of all in starts[owners].  All threads of a CTA (up to 1,024, whole warps) call it.
-// The kernel before this one has ended (the call's numbers are its to write).
-__device__ inline void plan(const Call& c, long long* starts, long long* warp_sums) {
+// What a CTA knows of all owners, in shared memory: what they are, their first units, and behind those the sum of all.
+struct Plan {
+  long long* starts;      // [owners + 1]
+  Owner* owners;          // [owners]
+  long long* sums;        // [32]
+};
+__host__ __device__ inline size_t plan_bytes(int owners) { return ((size_t)(owners + 1) * (8 + sizeof(Owner)) + 32 * 8 + 15) & ~(size_t)15; }
+__device__ __forceinline__ Plan plan_at(unsigned char* at, int owners) {
+  Plan p;
+  p.starts = reinterpret_cast<long long*>(at);
+  p.sums = p.starts + owners + 1;
+  p.owners = reinterpret_cast<Owner*>(p.sums + 32);
+  return p;
+}
+// All threads of a CTA (up to 1,024, whole warps) call it.  The kernel before this one has ended (the call's numbers are its to write).
+__device__ inline void make_plan(const Call& c, const Plan& plan) {
+  long long *starts = plan.starts, *warp_sums = plan.sums;
   const int owners = c.n_groups + c.n_req, tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
   long long base = 0;
   for (int o0 = 0; o0 < owners; o0 += nt) {
     const int o = o0 + tid;
     long long u = 0;
-    if (o < owners) u = owner_units(c, owner_at(c, o));
+    if (o < owners) {
+      const Owner w = owner_at(c, o);
+      plan.owners[o] = w;
+      u = owner_units(c, w);
+    }
     long long run = u;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += x; }
@@ -176,7 +183,8 @@ struct Walk {
   long long tile_start;     // the first unit of the tile
   int open;                 // the owner whose numbers are in w
   Owner w;
-  __device__ __forceinline__ void begin(const Call& c, const long long* starts, int cta) {
+  __device__ __forceinline__ void begin(const Call& c, const Plan& plan, int cta) {
+    const long long* starts = plan.starts;
     total = starts[c.n_groups + c.n_req];
     ctas = min((long long)c.ctas, total);      // each has a unit: an item's pieces leave no CTA out
     at = end = 0;
@@ -196,11 +204,12 @@ struct Walk {
     tile_start = starts[o];
   }
   // The next piece; false: there is none.
-  __device__ __forceinline__ bool next(const Call& c, const long long* starts, Piece& p) {
+  __device__ __forceinline__ bool next(const Call& c, const Plan& plan, Piece& p) {
+    const long long* starts = plan.starts;
     if (at >= end) return false;
     while (at >= starts[o + 1]) { ++o; tile = 0; tile_start = starts[o]; }
     if (open != o) {
-      w = owner_at(c, o);
+      w = plan.owners[o];
       open = o;
       if (w.group && at > tile_start) {      // tiles of a group are alike
         const long long per = (long long)tile_span(c, w, 0).units * c.kv_heads;
@@ -237,11 +246,16 @@ struct Walk {
   }
 };
 
-// The position of a query row of a tile and the first key that it sees: of a group's row by its request.
-__device__ __forceinline__ int row_position(const Call& c, const Owner& w, int row) {
-  if (!w.group) return w.p_first + row - w.row0;
-  const int r = request_of(c, row, w.request, c.n_req);
-  return request_len(c, r) - (request_row(c, r + 1) - row);
+// The position of a query row of an owner: of a group's row by its request.
+__device__ __forceinline__ int row_position(const Call& c, const Plan& plan, const Owner& w, int row) {
+  if (!w.group) return w.p_first() + row - w.row0;
+  const Owner* requests = plan.owners + c.n_groups;      // the first whose rows end behind it
+  int lo = w.request, hi = c.n_req - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (requests[mid].row1 <= row) lo = mid + 1; else hi = mid;
+  }
+  return requests[lo].hi - (requests[lo].row1 - row);
 }
 
 // The first elements of a page's keys (values: `kv_heads` page_size dim further on); -1: not a page of the pool.

@@ -56,6 +56,8 @@ LIBRARIES: Dict[str, tuple] = {
     "sampling": (["sampling.cu"], []),
     # attention over pages that requests share, in 32-bit arithmetic
     "attention_shared": (["attention_shared.cu"], []),
+    # the same on tensor cores: heads of 128, or defines={"HEAD_DIM": d}
+    "attention_shared_tc": (["attention_shared_tc.cu"], []),
     # compiled once per head size: defines={"HEAD_DIM": d}
     "attention_mma": (["attention_mma.cu"], []),
 }
@@ -71,6 +73,8 @@ DEFAULT_VARIANTS += [("attention_tc", {"HEAD_DIM": 128, "WEIGHT_TERMS": 2, "SOFT
 DEFAULT_VARIANTS += [("attention_tc", {"HEAD_DIM": d, "WEIGHT_TERMS": 2}) for d in (128, 64, 32)]
 # attention over 8-bit pages: heads of 128 (bfloat16), the sizes that the tests of the engine run, float32
 DEFAULT_VARIANTS += [(name, {"HEAD_DIM": d}) for name in ("kv8_attention", "kv8_attention_f32") for d in (128, 64, 256, 16)]
+
+DEFAULT_VARIANTS += [("attention_shared_tc", {"HEAD_DIM": d}) for d in (64, 32)]
 
 def register_library(name: str, sources: Sequence[str], flags: Sequence[str] = (), *, replace: bool = False) -> None:
     """Make a library of CUDA sources from outside the package known to :func:`load_library`, so that a
@@ -222,7 +226,8 @@ def build_all(progress=None) -> List[str]:
     """Compile every library (used by the build check; needs no GPU)."""
     from concurrent.futures import ThreadPoolExecutor
     jobs = [("core", None), ("linear_tcgen05", None), ("linear_skinny_static", None), ("attention_tc", None),
-            ("mixers", None), ("hybrid", None), ("latent", None), ("mx4", None), ("kv8", None), ("sampling", None), ("attention_shared", None)] + DEFAULT_VARIANTS
+            ("mixers", None), ("hybrid", None), ("latent", None), ("mx4", None), ("kv8", None), ("sampling", None), ("attention_shared", None),
+            ("attention_shared_tc", None)] + DEFAULT_VARIANTS
     with ThreadPoolExecutor(max_workers=4) as pool:
         built = list(pool.map(lambda j: compile_library(j[0], j[1], progress), jobs))
     # objects of older sources are never loaded (their names carry another hash); take them out of the folder
