@@ -7,12 +7,14 @@
 // with m the largest score (base 2), l the sum of weights 2^(s - m) and O their sum with the values; so it is for any number of pieces.  The rows of a
 // group over its shared keys are one matrix product, in which a key is read once for all of them.
 //
-// Owners: the groups, then the requests.  An owner's rows are cut into tiles of `tokens` query tokens (times the heads of a key head's group), an owner's
-// keys into units of `unit` keys; a tile of one key head is an item.  All units of all items lie in one line, in the order of owner, tile, key
-// head and key, and CTA c of n takes those from c U / n to (c + 1) U / n: every CTA has the same number but for one, however uneven the requests.  A
-// stretch of one item's units within a CTA is a piece; its sums go to slot (item + c), which no two pieces share, for along the line
-// either the item or the CTA moves on.  A second kernel joins a row's pieces in their order.  Item numbers leave gaps
-// (an owner's first is floor(first row / tokens) + its place) so that they need no sum over the owners.
+// Owners: the groups, then the requests.  An owner of at most 16 score rows (rows times the heads of a key head's group) is narrow, the others
+// are wide: narrow ones are worked on by warps, sixteen rows each, wide ones by CTAs with larger tiles, in kernels of their own that run beside one another.
+// For either an owner's rows are cut into tiles of `tokens` query tokens (a narrow owner is one tile), its keys into units of `unit` keys; a tile of one key
+// head is an item.  All units of all items lie in one line, in the order of owner, tile, key head and key, and worker c of n takes those from
+// c U / n to (c + 1) U / n: every worker has the same number but for one, however uneven the requests.  A stretch of one item's units within a worker
+// is a piece; its sums go to slot (item + c), which no two pieces share, for along the line either the item or the worker moves on.  A last
+// kernel joins a row's pieces in their order.  Item numbers leave gaps (an owner's first is floor(first row / tokens) + its place) so that they
+// need no sum over the owners.
 #pragma once
 #include "common.cuh"
 #include <math.h>
@@ -23,6 +25,9 @@ namespace shared_attention {
 
 constexpr int MAX_OWNERS = 2048;      // groups and requests of a call
 constexpr int NO_POSITION = -1;
+
+enum Class { EVERY, WIDE, NARROW };   // whose owners a kernel works on
+constexpr int NARROW_ROWS = 16;
 
 struct Call {
   const int* block_tables;
@@ -36,17 +41,32 @@ struct Call {
   int heads, kv_heads;
   int table_pages, page_size, window;
   float scale_log2;
+  int* err;
+  // of one class's kernel
+  int which;
   int tokens, unit, rows;                // of a tile (rows = tokens x heads of a key head, at most), of a unit
   int align;                             // an item's first key is a multiple of this
-  int ctas;
+  int workers;                           // at most
+  int cost;                              // of a unit, to the other class's
   float* part_o;                         // [slots][rows][dim]
   float2* part_ml;                       // [slots][rows]: largest score (base 2), sum of weights
-  int2* pieces;                          // [items]: first and last CTA of an item that has units
-  int* err;
+  int2* pieces;                          // [items]: first and last worker of an item that has units
 };
 
 __host__ __device__ inline int prefix_items(const Call& c) { return (c.n_tokens / c.tokens + c.n_groups + 1) * c.kv_heads; }
 __host__ __device__ inline int all_items(const Call& c) { return prefix_items(c) + (c.n_tokens / c.tokens + c.n_req + 1) * c.kv_heads; }
+__host__ inline long long room_align(long long x) { return (x + 255) & ~255LL; }
+// The room of one class's kernel, in three parts.
+__host__ inline long long room_bytes(const Call& c, int dim) {
+  const long long slots = (long long)all_items(c) + c.workers;
+  return room_align(slots * c.rows * dim * 4) + room_align(slots * c.rows * 8) + room_align((long long)all_items(c) * 8);
+}
+__host__ inline void room_at(Call& c, int dim, void* room) {
+  const long long slots = (long long)all_items(c) + c.workers;
+  c.part_o = (float*)room;
+  c.part_ml = (float2*)((char*)room + room_align(slots * c.rows * dim * 4));
+  c.pieces = (int2*)((char*)c.part_ml + room_align(slots * c.rows * 8));
+}
 
 __device__ __forceinline__ int clamp(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
@@ -119,6 +139,7 @@ __device__ __forceinline__ Span tile_span(const Call& c, const Owner& w, int til
   s.units = s.last > s.lo ? (s.last - s.first + c.unit - 1) / c.unit : 0;
   return s;
 }
+__device__ __forceinline__ bool is_narrow(const Call& c, const Owner& w) { return (w.row1 - w.row0) * (c.heads / c.kv_heads) <= NARROW_ROWS; }
 __device__ inline long long owner_units(const Call& c, const Owner& w) {
   const int n = owner_tiles(c, w);
   if (n == 0) return 0;
@@ -132,7 +153,7 @@ __device__ inline long long owner_units(const Call& c, const Owner& w) {
 struct Plan {
   long long* starts;      // [owners + 1]
   Owner* owners;          // [owners]
-  long long* sums;        // [32]
+  long long* sums;        // [32]: of warps; the last: units of the other class
 };
 __host__ __device__ inline size_t plan_bytes(int owners) { return ((size_t)(owners + 1) * (8 + sizeof(Owner)) + 32 * 8 + 15) & ~(size_t)15; }
 __device__ __forceinline__ Plan plan_at(unsigned char* at, int owners) {
@@ -142,18 +163,20 @@ __device__ __forceinline__ Plan plan_at(unsigned char* at, int owners) {
   p.owners = reinterpret_cast<Owner*>(p.sums + 32);
   return p;
 }
-// All threads of a CTA (up to 1,024, whole warps) call it.  The kernel before this one has ended (the call's numbers are its to write).
-__device__ inline void make_plan(const Call& c, const Plan& plan) {
+// All threads of a CTA (up to 31 warps) call it.  The kernel before this one has ended (the call's numbers are its to write).  `other`: the other class's call.
+__device__ inline void make_plan(const Call& c, const Call& other, const Plan& plan) {
   long long *starts = plan.starts, *warp_sums = plan.sums;
   const int owners = c.n_groups + c.n_req, tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
   long long base = 0;
+  if (tid == 0) plan.sums[31] = 0;
   for (int o0 = 0; o0 < owners; o0 += nt) {
     const int o = o0 + tid;
-    long long u = 0;
+    long long u = 0, theirs = 0;
     if (o < owners) {
       const Owner w = owner_at(c, o);
       plan.owners[o] = w;
-      u = owner_units(c, w);
+      if (c.which == EVERY || (c.which == NARROW) == is_narrow(c, w)) u = owner_units(c, w);
+      else theirs += owner_units(other, w);
     }
     long long run = u;
 #pragma unroll
@@ -163,6 +186,7 @@ __device__ inline void make_plan(const Call& c, const Plan& plan) {
     long long all = 0, before = 0;
     for (int v = 0; v < warps; ++v) { if (v < warp) before += warp_sums[v]; all += warp_sums[v]; }
     if (o < owners) starts[o] = base + before + run - u;
+    if (theirs) atomicAdd(reinterpret_cast<unsigned long long*>(plan.sums + 31), (unsigned long long)theirs);
     base += all;
     __syncthreads();
   }
@@ -170,7 +194,14 @@ __device__ inline void make_plan(const Call& c, const Plan& plan) {
   __syncthreads();
 }
 
-// A CTA's walk over its pieces.
+// How many of `sms` SMs the wide owners' kernel has: as much of them as of the cost; one at least where there is something to do, also for the other.
+__device__ __forceinline__ int wide_sms(int sms, long long wide, long long narrow) {
+  if (wide == 0) return 0;
+  if (narrow == 0) return sms;
+  return (int)max(1LL, min((long long)sms - 1, (sms * wide + (wide + narrow) / 2) / (wide + narrow)));
+}
+
+// A worker's walk over its pieces; `limit`: how many workers there are.
 struct Piece {
   Owner w;
   int tile, kv_head, item;
@@ -178,19 +209,19 @@ struct Piece {
   int row0, tokens;         // of the tile
 };
 struct Walk {
-  long long at, end, total, ctas;
+  long long at, end, total, workers;
   int o, tile;              // where `at` lies
   long long tile_start;     // the first unit of the tile
   int open;                 // the owner whose numbers are in w
   Owner w;
-  __device__ __forceinline__ void begin(const Call& c, const Plan& plan, int cta) {
+  __device__ __forceinline__ void begin(const Call& c, const Plan& plan, int worker, int limit) {
     const long long* starts = plan.starts;
     total = starts[c.n_groups + c.n_req];
-    ctas = min((long long)c.ctas, total);      // each has a unit: an item's pieces leave no CTA out
+    workers = min((long long)limit, total);      // each has a unit: an item's pieces leave none out
     at = end = 0;
-    if (cta < ctas) {
-      at = cta * total / ctas;
-      end = (cta + 1) * total / ctas;
+    if (worker < workers) {
+      at = worker * total / workers;
+      end = (worker + 1) * total / workers;
     }
     open = -1;
     if (at >= end) return;
@@ -238,11 +269,11 @@ struct Walk {
     at += u1 - u0;
     return true;
   }
-  // The CTAs that have pieces of the item whose piece came last (its first unit, and how many it has).
-  __device__ __forceinline__ int2 item_ctas(const Call& c, const Piece& p) const {
+  // The workers that have pieces of the item whose piece came last.
+  __device__ __forceinline__ int2 item_workers(const Call& c, const Piece& p) const {
     const Span s = tile_span(c, p.w, p.tile);
     const long long a = tile_start + (long long)p.kv_head * s.units, b = a + s.units - 1;
-    return make_int2((int)(((a + 1) * ctas - 1) / total), (int)(((b + 1) * ctas - 1) / total));
+    return make_int2((int)(((a + 1) * workers - 1) / total), (int)(((b + 1) * workers - 1) / total));
   }
 };
 
@@ -266,42 +297,50 @@ __device__ __forceinline__ long long page_at(const Call& c, int request, int pag
 }
 
 // ---------------------------------------------------------------------------------------------------- the join
-// A block takes a token's heads, eight warps of one head each at a time; a lane has columns lane, lane + 32, ...
+// A block takes a token's heads, a warp one head at a time; a lane has columns lane, lane + 32, ...  `wide` and `narrow`: the classes' calls (of
+// `wide.which` EVERY there is no other).
 constexpr int JOIN_WARPS = 8;
 template <typename T>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Call c, int dim, T* out) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ Call wide, const __grid_constant__ Call narrow, int dim, T* out) {
   __shared__ int found[1];
   ifb_pdl_wait();
   ifb_pdl_trigger();
   const int token = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
   if (tid == 0) found[0] = -1;
   __syncthreads();
-  for (int r = tid; r < c.n_req; r += JOIN_WARPS * 32)
-    if (request_row(c, r) <= token && token < request_row(c, r + 1)) found[0] = r;
+  for (int r = tid; r < wide.n_req; r += JOIN_WARPS * 32)
+    if (request_row(wide, r) <= token && token < request_row(wide, r + 1)) found[0] = r;
   __syncthreads();
   const int r = found[0];
   if (r < 0) return;      // a row of no request: left as it is
-  const int g = group_of(c, r), group = c.heads / c.kv_heads;
+  const int g = group_of(wide, r), group = wide.heads / wide.kv_heads;
   const int head = blockIdx.y * JOIN_WARPS + (tid >> 5);
-  if (head >= c.heads) return;
+  if (head >= wide.heads) return;
   const int kv_head = head / group;
-  int first[2] = {0, 0}, last[2] = {-1, -1}, item[2] = {0, 0}, row[2] = {0, 0};
+  int first[2] = {0, 0}, last[2] = {-1, -1};
+  const float2* ml_at[2] = {nullptr, nullptr};      // of the item's slot for worker 0
+  const float* o_at[2] = {nullptr, nullptr};
+  int rows[2] = {0, 0};
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int o = k == 0 ? g : c.n_groups + r;
+    const int o = k == 0 ? g : wide.n_groups + r;
     if (o < 0) continue;
-    const Owner w = owner_at(c, o);
+    const Owner w = owner_at(wide, o);
+    const Call& c = wide.which != EVERY && is_narrow(wide, w) ? narrow : wide;
     const int tile = (token - w.row0) / c.tokens;
     if (tile_span(c, w, tile).units == 0) continue;
-    item[k] = owner_item(c, w, o) + tile * c.kv_heads + kv_head;
-    const int2 ctas = c.pieces[item[k]];
-    first[k] = max(0, ctas.x); last[k] = min(ctas.y, c.ctas - 1);
-    row[k] = (token - w.row0 - tile * c.tokens) * group + head % group;
+    const int item = owner_item(c, w, o) + tile * c.kv_heads + kv_head;
+    const int2 workers = c.pieces[item];
+    first[k] = max(0, workers.x); last[k] = min(workers.y, c.workers - 1);
+    rows[k] = c.rows;
+    const long long at = (long long)item * c.rows + (token - w.row0 - tile * c.tokens) * group + head % group;
+    ml_at[k] = c.part_ml + at;
+    o_at[k] = c.part_o + at * dim;
   }
   float m = -INFINITY;
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    for (int x = first[k] + lane; x <= last[k]; x += 32) m = fmaxf(m, c.part_ml[(long long)(item[k] + x) * c.rows + row[k]].x);
+    for (int x = first[k] + lane; x <= last[k]; x += 32) m = fmaxf(m, ml_at[k][(long long)x * rows[k]].x);
   m = warp_max(m);
   constexpr int PER = 256 / 32;
   float acc[PER], den = 0.f;
@@ -311,25 +350,24 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Call c, int dim, 
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     for (int x = first[k]; x <= last[k]; ++x) {
-      const long long at = (long long)(item[k] + x) * c.rows + row[k];
-      const float2 ml = c.part_ml[at];
+      const float2 ml = ml_at[k][(long long)x * rows[k]];
       if (ml.y == 0.f) continue;      // a piece of which the row sees nothing
       const float f = exp2f(ml.x - m);
       den = fmaf(f, ml.y, den);
-      const float* o = c.part_o + at * dim;
+      const float* o = o_at[k] + (long long)x * rows[k] * dim;
 #pragma unroll
       for (int j = 0; j < PER; ++j)
         if (lane + j * 32 < dim) acc[j] = fmaf(f, o[lane + j * 32], acc[j]);
     }
   const float inv = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den;      // (NaN stays)
-  T* dst = out + ((long long)token * c.heads + head) * dim;
+  T* dst = out + ((long long)token * wide.heads + head) * dim;
 #pragma unroll
   for (int j = 0; j < PER; ++j)
     if (lane + j * 32 < dim) dst[lane + j * 32] = from_f32<T>(acc[j] * inv);
 }
 
-template <typename T> static int join(const Call& c, int dim, T* out, cudaStream_t stream) {
-  return ifb_launch(join_kernel<T>, dim3(c.n_tokens, (c.heads + JOIN_WARPS - 1) / JOIN_WARPS), dim3(JOIN_WARPS * 32), 0, stream, c, dim, out);
+template <typename T> static int join(const Call& wide, const Call& narrow, int dim, T* out, cudaStream_t stream) {
+  return ifb_launch(join_kernel<T>, dim3(wide.n_tokens, (wide.heads + JOIN_WARPS - 1) / JOIN_WARPS), dim3(JOIN_WARPS * 32), 0, stream, wide, narrow, dim, out);
 }
 
 }  // namespace shared_attention

@@ -1,5 +1,5 @@
-// Attention over shared pages on the fifth-generation tensor cores: bfloat16 heads of up to 128 in pages of 16, 32 or 64.  Compiled for one head size:
-// -DHEAD_DIM=<multiple of 16, at most 128> (default 128).  attention_shared.cuh says how the work is cut and joined.
+// Attention over shared pages on the fifth-generation tensor cores: wide owners of bfloat16 heads of HEAD_DIM, a multiple of 16 up to 128, in
+// pages of 16, 32 or 64.  attention_shared.cuh says how the work is cut and joined.
 //
 // A tile is 128 score rows (query tokens times the heads of a key head's group: row = token * G + head-in-group), a unit 128 keys.  Decoded tokens
 // of all requests of a group fill a tile together over the keys that they share; over its own keys a request has a tile to itself, most rows of
@@ -14,20 +14,13 @@
 // What no row sees may be anything: keys outside of a piece's are masked as scores; their values, which the product would multiply by a weight of zero, are
 // overwritten with zeros in shared memory by the warp that issues it.  (Within a request's own keys a value that only later queries see is in the product of
 // the earlier ones with weight zero: where it is infinite or NaN they become NaN with them.)
+#pragma once
 #include "tc_ops.cuh"
 #include "attention_shared.cuh"
-
-#ifndef HEAD_DIM
-#define HEAD_DIM 128
-#endif
-#if HEAD_DIM % 16 || HEAD_DIM < 16 || HEAD_DIM > 128
-#error "attention_shared_tc.cu takes head sizes up to 128, multiples of 16"
-#endif
 
 using namespace shared_attention;
 typedef __nv_bfloat16 bf16;
 
-constexpr int D = HEAD_DIM;
 constexpr int DH = (D + 63) / 64;                // swizzle rows of 64 columns that a row has
 constexpr int DN = DH * 64;                      // columns of the output accumulator
 constexpr int ROWS = 128, UNIT = 128, SUB = 64;
@@ -35,6 +28,7 @@ constexpr int THREADS = 384;
 constexpr int HALF_BYTES = 128 * 128;            // [128 rows][64 columns] in the 128-byte swizzle
 constexpr int TILE_BYTES = DH * HALF_BYTES;
 constexpr int TILES_BYTES = 5 * TILE_BYTES + 1024;      // Q, two stages of K and of V, alignment
+constexpr int STAGES_BYTES = 8 * 32 * 36 * 4;     // where sums turn from rows of a thread to rows of eight lanes
 constexpr int COL_S = 0, COL_O = 128, COLS_PER_STREAM = 256, TMEM_COLS = 512;
 constexpr uint64_t DESC = (1ull << 46) | (2ull << 61) | ((uint64_t)(1024 >> 4) << 32);      // 128-byte swizzle, groups of 8 rows 1,024 bytes apart
 __device__ __forceinline__ uint64_t desc_k_major(uint32_t a) { return (uint64_t)((a >> 4) & 0x3FFF) | (1ull << 16) | DESC; }
@@ -58,7 +52,7 @@ struct PageRows { int page, total; };      // the pool as a matrix of rows: rows
 
 __global__ void __launch_bounds__(THREADS, 1)
 shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                 PageRows mrows, const Call c) {
+                 PageRows mrows, const __grid_constant__ Call c, const __grid_constant__ Call other) {
   extern __shared__ unsigned char tc_smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t tmem_slot;
@@ -69,7 +63,8 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   const uint32_t raw = tc_smem_u32(tc_smem_raw);
   unsigned char* smem = tc_smem_raw + (((raw + 1023u) & ~1023u) - raw);
   unsigned char *Qs = smem, *Ks = smem + TILE_BYTES, *Vs = smem + 3 * TILE_BYTES;
-  const Plan plan = plan_at(smem + 5 * TILE_BYTES, c.n_groups + c.n_req);
+  const Plan plan = plan_at(smem + 5 * TILE_BYTES + STAGES_BYTES, c.n_groups + c.n_req);
+  float* stages = reinterpret_cast<float*>(smem + 5 * TILE_BYTES);      // [8 warps][32][36]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int G = c.heads / c.kv_heads;
 
@@ -101,13 +96,13 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   }
   ifb_pdl_wait();
   ifb_pdl_trigger();
-  make_plan(c, plan);
+  make_plan(c, other, plan);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   Walk walk;
-  walk.begin(c, plan, blockIdx.x);
+  walk.begin(c, plan, blockIdx.x, wide_sms(c.workers, plan.starts[c.n_groups + c.n_req] * c.cost, plan.sums[31] * other.cost));
   Piece p;
 
   if (warp == 0 || warp == 3) {
@@ -238,6 +233,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     const int row = qd * 32 + lane;
     const uint32_t lane_addr = tmem + ((uint32_t)(qd * 32) << 16) + x * COLS_PER_STREAM;
     uint64_t* o_done = &bars.o_done[x];
+    float* stage = stages + (warp - 4) * 32 * 36;
     bool ok = true;
     int hc = 0, ic = 0;                                      // this stream's halves and the pieces so far
     const float scale_log2 = c.scale_log2;
@@ -317,15 +313,22 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) {
             uint32_t pk[16], pr[16];
+            if (interior) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float e0 = tc_exp2(fmaf(__uint_as_float(v[cc][i]), scale_log2, -ref)), e1 = tc_exp2(fmaf(__uint_as_float(v[cc][i + 1]), scale_log2, -ref));
-              if (!interior) {
-                e0 = cc * 32 + i < vis_hi && cc * 32 + i >= vis_lo ? e0 : 0.f;
-                e1 = cc * 32 + i + 1 < vis_hi && cc * 32 + i + 1 >= vis_lo ? e1 : 0.f;
+              for (int i = 0; i < 32; i += 2) {
+                const float e0 = tc_exp2(fmaf(__uint_as_float(v[cc][i]), scale_log2, -ref)), e1 = tc_exp2(fmaf(__uint_as_float(v[cc][i + 1]), scale_log2, -ref));
+                lc[i & 2] += e0; lc[(i & 2) + 1] += e1;
+                weight_terms(e0, e1, pk[i >> 1], pr[i >> 1]);
               }
-              lc[i & 2] += e0; lc[(i & 2) + 1] += e1;
-              weight_terms(e0, e1, pk[i >> 1], pr[i >> 1]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const bool v0 = cc * 32 + i < vis_hi && cc * 32 + i >= vis_lo, v1 = cc * 32 + i + 1 < vis_hi && cc * 32 + i + 1 >= vis_lo;
+                const float e0 = v0 ? tc_exp2(fmaf(__uint_as_float(v[cc][i]), scale_log2, -ref)) : 0.f;
+                const float e1 = v1 ? tc_exp2(fmaf(__uint_as_float(v[cc][i + 1]), scale_log2, -ref)) : 0.f;
+                lc[i & 2] += e0; lc[(i & 2) + 1] += e1;
+                weight_terms(e0, e1, pk[i >> 1], pr[i >> 1]);
+              }
             }
             tc_st16(s_addr + cc * 16, pk);
             tc_st16(s_addr + 32 + cc * 16, pr);
@@ -357,7 +360,8 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         const bool two = n_half > 1;                             // stream 1's accumulator holds something of this piece
         const uint32_t o_addr = tmem + ((uint32_t)(qd * 32) << 16) + COL_O;
         const long long slot = (long long)(p.item + blockIdx.x) * ROWS + row;
-        float* dst = c.part_o + slot * D;
+        float* dst = c.part_o + (slot - lane) * D;               // of the warp's first row
+        const int count = min(32, p.tokens * G - qd * 32);       // its rows that exist
         if (x == 0 && exists) c.part_ml[slot] = make_float2(m, (m0 == -INFINITY ? l0 : a0 * l0) + (m1 == -INFINITY ? l1 : a1 * l1));
 #pragma unroll 1
         for (int cc = 0; cc < DN / 64; ++cc) {
@@ -374,14 +378,18 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
 #pragma unroll
             for (int i = 0; i < 32; ++i) y[i] = fmaf(__uint_as_float(ob[i]), a1, y[i]);
           }
-          if (exists) {
+          // a row's 128 bytes by eight lanes: through shared memory, a row of it 36 numbers long (no two lanes of a quarter on a bank)
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              if (DN == D || col0 + i < D) *reinterpret_cast<float4*>(dst + col0 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
-          }
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(stage + lane * 36 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+          __syncwarp();
+          const int col = lane % 8 * 4;
+          if (DN == D || col0 + col < D)
+            for (int q = lane / 8; q < count; q += 4)
+              *reinterpret_cast<float4*>(dst + q * D + col0 + col) = *reinterpret_cast<const float4*>(stage + q * 36 + col);
+          __syncwarp();
         }
       }
-      if (threadIdx.x == 128 && go) c.pieces[p.item] = walk.item_ctas(c, p);
+      if (threadIdx.x == 128 && go) c.pieces[p.item] = walk.item_workers(c, p);
       tc_fence_before();
       tc_mbar_arrive(&bars.o_free);            // this piece's sums have been read
       if (!go) break;
@@ -400,60 +408,31 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   }
 }
 
-static Call tc_call(int n_tokens, int n_req, int n_groups, int kv_heads, int group) {
+static inline Call tc_call(int n_tokens, int n_req, int n_groups, int kv_heads, int group, int page_size) {
   Call c = {};
+  c.which = WIDE;
   c.n_tokens = n_tokens; c.n_req = n_req; c.n_groups = n_groups;
   c.kv_heads = kv_heads; c.heads = kv_heads * group;
-  c.tokens = ROWS / group; c.unit = UNIT; c.rows = ROWS;
-  c.ctas = ifb_sm_count();
+  c.tokens = ROWS / group; c.unit = UNIT; c.rows = ROWS; c.align = page_size;
+  c.workers = ifb_sm_count();
+  c.cost = 8;
   return c;
 }
-static long long tc_align(long long x) { return (x + 255) & ~255LL; }
-
-// Bytes of room for a call's sums, in three parts: sums, maxima and denominators, items' pieces.
-IFB_EXPORT long long ifb_attention_shared_tc_room(int n_tokens, int n_req, int n_groups, int kv_heads, int group) {
-  const Call c = tc_call(n_tokens, n_req, n_groups, kv_heads, group);
-  const long long slots = (long long)all_items(c) + c.ctas;
-  return tc_align(slots * ROWS * D * 4) + tc_align(slots * ROWS * 8) + tc_align((long long)all_items(c) * 8);
-}
-
-// As ifb_attention_shared, for bfloat16, heads of D, at most 128 query heads a key head, pages of 16, 32 or 64 and a positive scale.
-IFB_EXPORT int ifb_attention_shared_tc(const void* q, long long q_row, const void* pages, long long page_stride, long long num_pages,
-                                       const int* block_tables, long long bt_stride, int table_pages, const int* cu_q, const int* seq_lens,
-                                       const int* cu_groups, const int* shared_lens, void* out, void* room, int* err, int n_tokens, int n_req, int n_groups,
-                                       int heads, int kv_heads, int page_size, float scale, int window, cudaStream_t stream) {
-  if (n_tokens <= 0 || n_req <= 0) return IFB_OK;
-  if (kv_heads < 1 || heads % kv_heads || heads / kv_heads > ROWS || n_groups < 0 || n_req + n_groups > MAX_OWNERS || num_pages < 1 ||
-      (page_size != 16 && page_size != 32 && page_size != 64))
-    return IFB_ERR_SIZE;
-  if ((((uintptr_t)q | (uintptr_t)pages) & 15) || q_row % 8 || page_stride % D || ((uintptr_t)room & 255)) return IFB_ERR_ALIGN;
-  if (window < 0 || !err || !(scale > 0.f) || page_stride < 2LL * kv_heads * page_size * D) return IFB_ERR_ARG;
-  const long long page_rows = page_stride / D, rows = (num_pages - 1) * page_rows + (long long)kv_heads * page_size;
-  if (rows >= 0x7fffffffLL) return IFB_ERR_SIZE;
-  Call c = tc_call(n_tokens, n_req, n_groups, kv_heads, heads / kv_heads);
-  c.align = page_size;
-  c.block_tables = block_tables; c.cu_q = cu_q; c.seq_lens = seq_lens; c.cu_groups = cu_groups; c.shared_lens = shared_lens;
-  c.bt_stride = bt_stride; c.num_pages = num_pages; c.page_stride = page_stride;
-  c.table_pages = table_pages; c.page_size = page_size; c.window = window;
-  c.scale_log2 = scale * 1.4426950408889634f;
-  const long long slots = (long long)all_items(c) + c.ctas;
-  c.part_o = (float*)room;
-  c.part_ml = (float2*)((char*)room + tc_align(slots * ROWS * D * 4));
-  c.pieces = (int2*)((char*)c.part_ml + tc_align(slots * ROWS * 8));
-  c.err = err;
+static int tc_main(const Call& c, const Call& other, const bf16* q, long long q_row, const bf16* pages, cudaStream_t stream) {
+  const int group = c.heads / c.kv_heads;
+  const long long page_rows = c.page_stride / D, rows = (c.num_pages - 1) * page_rows + (long long)c.kv_heads * c.page_size;
   CUtensorMap q_map, k_map, v_map;
   {
-    const unsigned long long dims[3] = {(unsigned long long)D, (unsigned long long)heads, (unsigned long long)n_tokens};
+    const unsigned long long dims[3] = {(unsigned long long)D, (unsigned long long)c.heads, (unsigned long long)c.n_tokens};
     const unsigned long long strides[2] = {(unsigned long long)D * 2, (unsigned long long)q_row * 2};
-    const unsigned box[3] = {64, (unsigned)(heads / kv_heads), (unsigned)c.tokens};
+    const unsigned box[3] = {64, (unsigned)group, (unsigned)c.tokens};
     if (ifb_tensor_map_bf16(&q_map, q, 3, dims, strides, box)) return IFB_ERR_ARG;
   }
   const unsigned long long dims[2] = {(unsigned long long)D, (unsigned long long)rows}, strides[1] = {(unsigned long long)D * 2};
-  const unsigned box[2] = {64, (unsigned)page_size};
+  const unsigned box[2] = {64, (unsigned)c.page_size};
   if (ifb_tensor_map_bf16(&k_map, pages, 2, dims, strides, box)) return IFB_ERR_ARG;
-  if (ifb_tensor_map_bf16(&v_map, (const bf16*)pages + (long long)kv_heads * page_size * D, 2, dims, strides, box)) return IFB_ERR_ARG;
-  const size_t smem = TILES_BYTES + plan_bytes(n_req + n_groups);
+  if (ifb_tensor_map_bf16(&v_map, pages + (long long)c.kv_heads * c.page_size * D, 2, dims, strides, box)) return IFB_ERR_ARG;
+  const size_t smem = TILES_BYTES + STAGES_BYTES + plan_bytes(c.n_req + c.n_groups);
   IFB_ALLOW_SMEM(shared_tc_kernel, smem);
-  const int st = ifb_launch(shared_tc_kernel, dim3(c.ctas), dim3(THREADS), smem, stream, q_map, k_map, v_map, PageRows{(int)page_rows, (int)rows}, c);
-  return st ? st : join<bf16>(c, D, (bf16*)out, stream);
+  return ifb_launch(shared_tc_kernel, dim3(c.workers), dim3(THREADS), smem, stream, q_map, k_map, v_map, PageRows{(int)page_rows, (int)rows}, c, other);
 }

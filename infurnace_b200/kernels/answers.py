@@ -109,38 +109,27 @@ class AnswerKernels:
         return out
 
     # ------------------------------------------------------------------ attention over shared pages
-    _shared = None
+    def _shared_lib(self, dtype, dim):
+        """(call, size of its room) for a type and head size."""
+        libs = self.__dict__.setdefault("_shared", {})
+        held = libs.get((dtype, dim))
+        if held is None:
+            if dtype == torch.float32:
+                lib = load_library("attention_shared", progress=self._progress)
+                call, room = lib.ifb_attention_shared, lib.ifb_attention_shared_room
+            else:
+                lib = load_library("attention_shared_bf16", {"HEAD_DIM": dim}, progress=self._progress)
+                call, room = lib.ifb_attention_shared_bf16, lib.ifb_attention_shared_bf16_room
+            call.argtypes = [c_void_p, c_longlong, c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_int] + [c_void_p] * 7 + [c_int] * 7 + [
+                c_float, c_int, c_void_p]
+            room.argtypes, room.restype = [c_int] * (6 if dtype == torch.float32 else 5), c_longlong
+            held = libs[(dtype, dim)] = (call, room)
+        return held
 
-    def _shared_lib(self):
-        if self._shared is None:
-            lib = load_library("attention_shared", progress=self._progress)
-            lib.ifb_attention_shared.argtypes = ([c_void_p, c_int, c_longlong, c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_int]
-                                                 + [c_void_p] * 7 + [c_int] * 7 + [c_float, c_int, c_void_p])
-            lib.ifb_attention_shared_room.argtypes = [c_int] * 6
-            lib.ifb_attention_shared_room.restype = c_longlong
-            self._shared = lib
-        return self._shared
-
-    def _shared_tc_lib(self, dim):
-        libs = self.__dict__.setdefault("_shared_tc", {})
-        lib = libs.get(dim)
-        if lib is None:
-            lib = libs[dim] = load_library("attention_shared_tc", {"HEAD_DIM": dim} if dim != 128 else None, progress=self._progress)
-            lib.ifb_attention_shared_tc.argtypes = ([c_void_p, c_longlong, c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_int]
-                                                    + [c_void_p] * 7 + [c_int] * 6 + [c_float, c_int, c_void_p])
-            lib.ifb_attention_shared_tc_room.argtypes = [c_int] * 5
-            lib.ifb_attention_shared_tc_room.restype = c_longlong
-        return lib
-
-    SHARED_TC_OWNERS = 1024       # groups and requests whose numbers the tcgen05 form holds beside its tiles
-
-    def shared_prefix_room(self, tokens, requests, groups, heads, kv_heads, head_dim):
-        """Bytes of the room that ``shared_prefix_attention`` takes at most for a step of so many tokens, requests and groups."""
-        group = heads // kv_heads
-        size = int(self._shared_lib().ifb_attention_shared_room(tokens, requests, groups, kv_heads, group, head_dim))
-        if head_dim <= 128:
-            size = max(size, int(self._shared_tc_lib(head_dim).ifb_attention_shared_tc_room(tokens, requests, groups, kv_heads, group)))
-        return size
+    def shared_prefix_room(self, tokens, requests, groups, heads, kv_heads, head_dim, dtype):
+        """Bytes of the room that ``shared_prefix_attention`` takes for a step of so many tokens, requests and groups."""
+        sizes = (tokens, requests, groups, kv_heads, heads // kv_heads)
+        return int(self._shared_lib(dtype, head_dim)[1](*sizes, *((head_dim,) if dtype == torch.float32 else ())))
 
     def shared_prefix_attention(self, q, kv_pages, block_tables, cu_q, seq_lens, cu_groups, shared_lens, out, scale, window, max_q_len, max_seq_len,
                                 room=None):
@@ -197,29 +186,17 @@ class AnswerKernels:
             return out
         q_row = q.stride(0) if n > 1 else heads * dim
         with torch.cuda.device(index):
-            # bfloat16 heads up to 128 in pages that are boxes of a copy: tensor cores.  (The 32-bit form for the same: 64 answers to 8,000 keys 1,524 us.)
-            tc = (q.dtype == torch.bfloat16 and dim <= 128 and page_size in (16, 32, 64) and r + groups <= self.SHARED_TC_OWNERS and scale > 0
-                  and q.data_ptr() % 16 == 0 and kv_pages.data_ptr() % 16 == 0 and q_row % 8 == 0 and page_stride % dim == 0
-                  and pages * page_stride // dim < (1 << 31) - 1)
-            if tc:
-                lib = self._shared_tc_lib(dim)
-                size = lib.ifb_attention_shared_tc_room(n, r, groups, kv_heads, group)
-            else:
-                lib = self._shared_lib()
-                size = lib.ifb_attention_shared_room(n, r, groups, kv_heads, group, dim)
+            call, room_of = self._shared_lib(q.dtype, dim)
+            size = room_of(n, r, groups, kv_heads, group, dim) if q.dtype == torch.float32 else room_of(n, r, groups, kv_heads, group)
             if room is None:
                 room = torch.empty(size, dtype=torch.uint8, device=q.device)
             elif room.dtype != torch.uint8 or room.dim() != 1 or not room.is_contiguous() or room.numel() < size or room.data_ptr() % 256 \
                     or room.get_device() != index:
                 raise KernelError(f"shared_prefix_attention: a room is uint8 [{size} or more], contiguous, on 256 bytes, on the same device")
-            self.launches += 2
+            self.launches += 2 if q.dtype == torch.float32 or group > 16 or n * group <= 16 else 3
             self._err_armed = True
-            pool = (kv_pages.data_ptr(), page_stride, pages, block_tables.data_ptr(), block_tables.stride(0), table[1], cu_q.data_ptr(),
-                    seq_lens.data_ptr(), cu_groups.data_ptr(), shared_lens.data_ptr(), out.data_ptr(), room.data_ptr(), self._dev_err_at, n, r, groups,
-                    heads, kv_heads)
-            if tc:
-                status = lib.ifb_attention_shared_tc(q.data_ptr(), q_row, *pool, page_size, scale, window, _raw_stream(index))
-            else:
-                status = lib.ifb_attention_shared(q.data_ptr(), code, q_row, *pool, dim, page_size, scale, window, _raw_stream(index))
+            status = call(q.data_ptr(), q_row, kv_pages.data_ptr(), page_stride, pages, block_tables.data_ptr(), block_tables.stride(0), table[1],
+                          cu_q.data_ptr(), seq_lens.data_ptr(), cu_groups.data_ptr(), shared_lens.data_ptr(), out.data_ptr(), room.data_ptr(),
+                          self._dev_err_at, n, r, groups, heads, kv_heads, dim, page_size, scale, window, _raw_stream(index))
             _status(status, "shared_prefix_attention")
         return out

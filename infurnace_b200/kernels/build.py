@@ -54,10 +54,9 @@ LIBRARIES: Dict[str, tuple] = {
     "kv8_attention_f32": (["kv8_attention_f32.cu"], []),
     # drawing tokens under top-k, top-p and min-p, log probabilities of tokens
     "sampling": (["sampling.cu"], []),
-    # attention over pages that requests share, in 32-bit arithmetic
+    # attention over pages that requests share: float32; bfloat16, compiled once per head size: defines={"HEAD_DIM": d}
     "attention_shared": (["attention_shared.cu"], []),
-    # the same on tensor cores: heads of 128, or defines={"HEAD_DIM": d}
-    "attention_shared_tc": (["attention_shared_tc.cu"], []),
+    "attention_shared_bf16": (["attention_shared_bf16.cu"], []),
     # compiled once per head size: defines={"HEAD_DIM": d}
     "attention_mma": (["attention_mma.cu"], []),
 }
@@ -74,7 +73,8 @@ DEFAULT_VARIANTS += [("attention_tc", {"HEAD_DIM": d, "WEIGHT_TERMS": 2}) for d 
 # attention over 8-bit pages: heads of 128 (bfloat16), the sizes that the tests of the engine run, float32
 DEFAULT_VARIANTS += [(name, {"HEAD_DIM": d}) for name in ("kv8_attention", "kv8_attention_f32") for d in (128, 64, 256, 16)]
 
-DEFAULT_VARIANTS += [("attention_shared_tc", {"HEAD_DIM": d}) for d in (64, 32)]
+# attention over shared pages in bfloat16: heads of 128 and what the tests run most
+DEFAULT_VARIANTS += [("attention_shared_bf16", {"HEAD_DIM": d}) for d in (128, 64, 32)]
 
 def register_library(name: str, sources: Sequence[str], flags: Sequence[str] = (), *, replace: bool = False) -> None:
     """Make a library of CUDA sources from outside the package known to :func:`load_library`, so that a
@@ -226,8 +226,7 @@ def build_all(progress=None) -> List[str]:
     """Compile every library (used by the build check; needs no GPU)."""
     from concurrent.futures import ThreadPoolExecutor
     jobs = [("core", None), ("linear_tcgen05", None), ("linear_skinny_static", None), ("attention_tc", None),
-            ("mixers", None), ("hybrid", None), ("latent", None), ("mx4", None), ("kv8", None), ("sampling", None), ("attention_shared", None),
-            ("attention_shared_tc", None)] + DEFAULT_VARIANTS
+            ("mixers", None), ("hybrid", None), ("latent", None), ("mx4", None), ("kv8", None), ("sampling", None), ("attention_shared", None)] + DEFAULT_VARIANTS
     with ThreadPoolExecutor(max_workers=4) as pool:
         built = list(pool.map(lambda j: compile_library(j[0], j[1], progress), jobs))
     # objects of older sources are never loaded (their names carry another hash); take them out of the folder

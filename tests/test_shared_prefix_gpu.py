@@ -191,7 +191,7 @@ def test_bits_repeat_and_a_room_may_be_the_callers(K, dtype):
     s = Scene(**SCENES["uneven"], dtype=dtype)
     first = s.run(K)
     heads, dim = s.q.shape[1:]
-    size = K.shared_prefix_room(s.rows, len(s.lens), len(s.shared), heads, 2, dim)
+    size = K.shared_prefix_room(s.rows, len(s.lens), len(s.shared), heads, 2, dim, dtype)
     room = torch.full((size,), 255, dtype=torch.uint8, device="cuda")              # NaN wherever it is read as numbers
     for _ in range(3):
         assert torch.equal(s.run(K, room=room), first)
