@@ -3,7 +3,7 @@
 
 // Bytes of room for a call's sums.
 IFB_EXPORT long long ifb_attention_shared_room(int n_tokens, int n_req, int n_groups, int kv_heads, int group, int dim) {
-  return room_bytes(sh_call(n_tokens, n_req, n_groups, kv_heads, group, EVERY), dim);
+  return parts_bytes(n_tokens) + room_bytes(sh_call(n_tokens, n_req, n_groups, kv_heads, group, EVERY), dim);
 }
 
 // q [n_tokens, heads, dim] with rows `q_row` elements apart; pages [num_pages][2][kv_heads][page_size][dim], pages `page_stride` elements apart; out dense.
@@ -23,8 +23,11 @@ IFB_EXPORT int ifb_attention_shared(const float* q, long long q_row, const float
   c.table_pages = table_pages; c.page_size = page_size; c.window = window;
   c.scale_log2 = scale * 1.4426950408889634f;
   c.err = err;
-  room_at(c, dim, room);
-  const int st = dim <= 64 ? sh_main<float, 8>(c, c, q, q_row, pages, dim, stream) : dim <= 128 ? sh_main<float, 16>(c, c, q, q_row, pages, dim, stream)
-                                                                                              : sh_main<float, 32>(c, c, q, q_row, pages, dim, stream);
-  return st ? st : join<float>(c, c, dim, out, stream);
+  c.out = out;
+  c.parts = (int4*)room;
+  room_at(c, dim, (char*)room + parts_bytes(n_tokens));
+  const int st = dim <= 64    ? sh_main<float, 8>(c, c, q, q_row, pages, dim, true, stream)
+                 : dim <= 128 ? sh_main<float, 16>(c, c, q, q_row, pages, dim, true, stream)
+                              : sh_main<float, 32>(c, c, q, q_row, pages, dim, true, stream);
+  return st ? st : join<float>(c, c, dim, stream);
 }

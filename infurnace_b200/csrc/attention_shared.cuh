@@ -7,14 +7,17 @@
 // with m the largest score (base 2), l the sum of weights 2^(s - m) and O their sum with the values; so it is for any number of pieces.  The rows of a
 // group over its shared keys are one matrix product, in which a key is read once for all of them.
 //
-// Owners: the groups, then the requests.  An owner of at most 16 score rows (rows times the heads of a key head's group) is narrow, the others
-// are wide: narrow ones are worked on by warps, sixteen rows each, wide ones by CTAs with larger tiles, in kernels of their own that run beside one another.
+// Owners: the groups, then the requests.  Where the requests of a group bring many rows each (64 score rows on average, half a tile), their tiles are full
+// without it: the group has no rows then, and each request has all its keys, the shared ones through the first request's table ("split" below).
+// An owner of at most 16 score rows (rows times the heads of a key head's group) is narrow, the others are wide: narrow ones are worked on by warps,
+// sixteen rows each, wide ones by CTAs with larger tiles, in kernels of their own that run beside one another.
 // For either an owner's rows are cut into tiles of `tokens` query tokens (a narrow owner is one tile), its keys into units of `unit` keys; a tile of one key
-// head is an item.  All units of all items lie in one line, in the order of owner, tile, key head and key, and worker c of n takes those from
-// c U / n to (c + 1) U / n: every worker has the same number but for one, however uneven the requests.  A stretch of one item's units within a worker
-// is a piece; its sums go to slot (item + c), which no two pieces share, for along the line either the item or the worker moves on.  A last
-// kernel joins a row's pieces in their order.  Item numbers leave gaps (an owner's first is floor(first row / tokens) + its place) so that they
-// need no sum over the owners.
+// head is an item.  All units of all items, and `extra` ones for an item's beginning and end, lie in one line, in the order of owner, tile, key
+// head and key, and worker c of n takes those from c U / n to (c + 1) U / n: every worker has the same number but for one, however uneven the requests.
+// A stretch of one item's units within a worker is a piece; its sums go to slot (item + c), which no two pieces share, for along the line
+// either the item or the worker moves on.  A last kernel joins a row's pieces in their order; an item that is one piece, and the only one of its
+// rows, is written out where it is worked on.  Item numbers leave gaps (an owner's first is floor(first row / tokens) + its place) so that they need no
+// sum over the owners.
 #pragma once
 #include "common.cuh"
 #include <math.h>
@@ -25,9 +28,9 @@ namespace shared_attention {
 
 constexpr int MAX_OWNERS = 2048;      // groups and requests of a call
 constexpr int NO_POSITION = -1;
-
 enum Class { EVERY, WIDE, NARROW };   // whose owners a kernel works on
 constexpr int NARROW_ROWS = 16;
+constexpr int FULL_ROWS = 64;         // score rows of a request, on average, from which a group is given up
 
 struct Call {
   const int* block_tables;
@@ -41,10 +44,13 @@ struct Call {
   int heads, kv_heads;
   int table_pages, page_size, window;
   float scale_log2;
+  void* out;                             // [n_tokens, heads, dim]
+  int4* parts;                           // [n_tokens]: where a row's pieces are (RowParts)
   int* err;
   // of one class's kernel
   int which;
   int tokens, unit, rows;                // of a tile (rows = tokens x heads of a key head, at most), of a unit
+  int extra;                             // units that an item's beginning and end cost
   int align;                             // an item's first key is a multiple of this
   int workers;                           // at most
   int cost;                              // of a unit, to the other class's
@@ -61,6 +67,7 @@ __host__ inline long long room_bytes(const Call& c, int dim) {
   const long long slots = (long long)all_items(c) + c.workers;
   return room_align(slots * c.rows * dim * 4) + room_align(slots * c.rows * 8) + room_align((long long)all_items(c) * 8);
 }
+__host__ inline long long parts_bytes(int n_tokens) { return room_align((long long)n_tokens * 16); }
 __host__ inline void room_at(Call& c, int dim, void* room) {
   const long long slots = (long long)all_items(c) + c.workers;
   c.part_o = (float*)room;
@@ -73,56 +80,13 @@ __device__ __forceinline__ int clamp(int x, int lo, int hi) { return min(max(x, 
 // What an owner's rows and keys are.
 struct Owner {
   int row0, row1;            // query rows
-  int request;               // whose table holds the keys (a group: its first request's)
   int lo, hi;                // keys lo .. hi - 1 at most
+  int request;               // whose table holds the keys (a group: its first request's)
+  int first, split;          // keys below `split`, a whole number of pages, are in the table of `first` instead
   int group;                 // whether it is one
   __device__ __forceinline__ int p_first() const { return hi - (row1 - row0); }      // a request: the position of its first row
+  __device__ __forceinline__ int table(int key) const { return key < split ? first : request; }
 };
-__device__ __forceinline__ int request_row(const Call& c, int r) { return clamp(c.cu_q[r], 0, c.n_tokens); }
-__device__ __forceinline__ int request_len(const Call& c, int r) { return clamp(c.seq_lens[r], 0, (int)min((long long)c.table_pages * c.page_size, 0x7fffff00LL)); }
-__device__ __forceinline__ int group_start(const Call& c, int g) { return clamp(c.cu_groups[g], 0, c.n_req); }
-__device__ __forceinline__ int shared_len(const Call& c, int g) { return clamp(c.shared_lens[g], 0, (int)min((long long)c.table_pages * c.page_size, 0x7fffff00LL)); }
-
-// The group of a request, or -1.
-__device__ __forceinline__ int group_of(const Call& c, int r) {
-  if (c.n_groups == 0 || r < group_start(c, 0) || r >= group_start(c, c.n_groups)) return -1;
-  int lo = 0, hi = c.n_groups - 1;      // the last group that begins at or before r
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (group_start(c, mid) <= r) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
-__device__ __forceinline__ Owner owner_at(const Call& c, int o) {
-  Owner w;
-  w.group = o < c.n_groups;
-  if (w.group) {
-    const int r0 = group_start(c, o), r1 = max(r0, group_start(c, o + 1));
-    w.request = min(r0, c.n_req - 1);
-    w.row0 = request_row(c, r0);
-    w.row1 = max(w.row0, request_row(c, r1));
-    w.lo = 0;
-    w.hi = shared_len(c, o);
-    if (c.window > 0) {      // no row sees a key before this
-      int first = w.hi;
-      for (int r = r0; r < r1; ++r) first = min(first, request_len(c, r) - (request_row(c, r + 1) - request_row(c, r)) - c.window + 1);
-      w.lo = max(0, first);
-    }
-  } else {
-    const int r = o - c.n_groups;
-    const int g = group_of(c, r);
-    w.request = r;
-    w.row0 = request_row(c, r);
-    w.row1 = max(w.row0, request_row(c, r + 1));
-    w.lo = g >= 0 ? shared_len(c, g) : 0;
-    w.hi = request_len(c, r);
-  }
-  return w;
-}
-__device__ __forceinline__ int owner_tiles(const Call& c, const Owner& w) { return (w.row1 - w.row0 + c.tokens - 1) / c.tokens; }
-__device__ __forceinline__ int owner_item(const Call& c, const Owner& w, int o) {
-  return w.group ? (w.row0 / c.tokens + o) * c.kv_heads : prefix_items(c) + (w.row0 / c.tokens + o - c.n_groups) * c.kv_heads;
-}
 
 // The keys that a tile's rows can see (lo .. last - 1), and where their units begin.
 struct Span { int first, last, lo, units; };
@@ -139,58 +103,120 @@ __device__ __forceinline__ Span tile_span(const Call& c, const Owner& w, int til
   s.units = s.last > s.lo ? (s.last - s.first + c.unit - 1) / c.unit : 0;
   return s;
 }
+__device__ __forceinline__ int span_cost(const Call& c, const Span& s) { return s.units ? s.units + c.extra : 0; }
+__device__ __forceinline__ int owner_tiles(const Call& c, const Owner& w) { return (w.row1 - w.row0 + c.tokens - 1) / c.tokens; }
+__device__ __forceinline__ int owner_item(const Call& c, const Owner& w, int o) {
+  return w.group ? (w.row0 / c.tokens + o) * c.kv_heads : prefix_items(c) + (w.row0 / c.tokens + o - c.n_groups) * c.kv_heads;
+}
 __device__ __forceinline__ bool is_narrow(const Call& c, const Owner& w) { return (w.row1 - w.row0) * (c.heads / c.kv_heads) <= NARROW_ROWS; }
-__device__ inline long long owner_units(const Call& c, const Owner& w) {
+__device__ inline long long owner_cost(const Call& c, const Owner& w) {
   const int n = owner_tiles(c, w);
   if (n == 0) return 0;
-  if (w.group) return (long long)n * tile_span(c, w, 0).units * c.kv_heads;
+  if (w.group) return (long long)n * span_cost(c, tile_span(c, w, 0)) * c.kv_heads;
   long long u = 0;
-  for (int t = 0; t < n; ++t) u += tile_span(c, w, t).units;
+  for (int t = 0; t < n; ++t) u += span_cost(c, tile_span(c, w, t));
   return u * c.kv_heads;
 }
 
 // What a CTA knows of all owners, in shared memory: what they are, their first units, and behind those the sum of all.
 struct Plan {
-  long long* starts;      // [owners + 1]
+  long long* starts;      // [owners + 1]; before it is made, the call's numbers lie there
+  long long* sums;        // [32]: of warps; the last: cost of the other class
   Owner* owners;          // [owners]
-  long long* sums;        // [32]: of warps; the last: units of the other class
 };
-__host__ __device__ inline size_t plan_bytes(int owners) { return ((size_t)(owners + 1) * (8 + sizeof(Owner)) + 32 * 8 + 15) & ~(size_t)15; }
+__host__ __device__ inline size_t plan_bytes(int owners) { return (((size_t)(owners + 1) + 32) * 8 + 15 & ~(size_t)15) + (size_t)owners * sizeof(Owner); }
 __device__ __forceinline__ Plan plan_at(unsigned char* at, int owners) {
   Plan p;
   p.starts = reinterpret_cast<long long*>(at);
   p.sums = p.starts + owners + 1;
-  p.owners = reinterpret_cast<Owner*>(p.sums + 32);
+  p.owners = reinterpret_cast<Owner*>(at + (((size_t)(owners + 1) + 32) * 8 + 15 & ~(size_t)15));
   return p;
 }
-// All threads of a CTA (up to 31 warps) call it.  The kernel before this one has ended (the call's numbers are its to write).  `other`: the other class's call.
+// All threads of a CTA (up to 31 warps) call it.  The kernel before this one has ended (the call's numbers are its to write).  `other`: the other class's
+// call.  The numbers are brought to shared memory first, all at once: read where they are needed they were a chain of seven trips to L2 (5 us).
 __device__ inline void make_plan(const Call& c, const Call& other, const Plan& plan) {
-  long long *starts = plan.starts, *warp_sums = plan.sums;
-  const int owners = c.n_groups + c.n_req, tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
+  const int R = c.n_req, N = c.n_groups, owners = N + R;
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
+  {
+    int* rows = reinterpret_cast<int*>(plan.starts);      // [R + 1] first rows, [R] lengths, [N + 1] first requests, [N] shared lengths
+    int *lens = rows + R + 1, *members = lens + R, *shared = members + N + 1;
+    const int most = (int)min((long long)c.table_pages * c.page_size, 0x7fffff00LL);
+    for (int i = tid; i <= R; i += nt) {
+      const int row = c.cu_q[i], len = i < R ? c.seq_lens[i] : 0;
+      rows[i] = clamp(row, 0, c.n_tokens);
+      if (i < R) lens[i] = clamp(len, 0, most);
+    }
+    for (int i = tid; i <= N; i += nt) {
+      const int r = c.cu_groups[i], len = i < N ? c.shared_lens[i] : 0;
+      members[i] = clamp(r, 0, R);
+      if (i < N) shared[i] = clamp(len, 0, most);
+    }
+    __syncthreads();
+    const int G = c.heads / c.kv_heads;
+    auto full = [&](int g) {      // a group that is given up
+      const int n = members[g + 1] - members[g];
+      return n > 0 && (long long)(rows[members[g + 1]] - rows[members[g]]) * G >= (long long)FULL_ROWS * n && shared[g] % c.page_size == 0;
+    };
+    for (int o = tid; o < owners; o += nt) {
+      Owner w;
+      w.group = o < N;
+      w.first = w.split = 0;
+      if (w.group) {
+        const int r0 = members[o], r1 = max(r0, members[o + 1]);
+        w.request = min(r0, R - 1);
+        w.row0 = rows[r0];
+        w.row1 = full(o) ? w.row0 : max(w.row0, rows[r1]);
+        w.lo = 0;
+        w.hi = shared[o];
+        if (c.window > 0) {      // no row sees a key before this
+          int first = w.hi;
+          for (int r = r0; r < r1; ++r) first = min(first, lens[r] - (rows[r + 1] - rows[r]) - c.window + 1);
+          w.lo = max(0, first);
+        }
+      } else {
+        const int r = o - N;
+        w.request = r;
+        w.row0 = rows[r];
+        w.row1 = max(w.row0, rows[r + 1]);
+        w.lo = 0;
+        w.hi = lens[r];
+        if (N > 0 && r >= members[0] && r < members[N]) {
+          int a = 0, b = N - 1;      // the last group that begins at or before r
+          while (a < b) {
+            const int mid = (a + b + 1) >> 1;
+            if (members[mid] <= r) a = mid; else b = mid - 1;
+          }
+          if (full(a)) { w.first = members[a]; w.split = shared[a]; }
+          else w.lo = shared[a];
+        }
+      }
+      plan.owners[o] = w;
+    }
+    if (tid == 0) plan.sums[31] = 0;
+    __syncthreads();
+  }
   long long base = 0;
-  if (tid == 0) plan.sums[31] = 0;
   for (int o0 = 0; o0 < owners; o0 += nt) {
     const int o = o0 + tid;
     long long u = 0, theirs = 0;
     if (o < owners) {
-      const Owner w = owner_at(c, o);
-      plan.owners[o] = w;
-      if (c.which == EVERY || (c.which == NARROW) == is_narrow(c, w)) u = owner_units(c, w);
-      else theirs += owner_units(other, w);
+      const Owner w = plan.owners[o];
+      if (c.which == EVERY || (c.which == NARROW) == is_narrow(c, w)) u = owner_cost(c, w);
+      else theirs = owner_cost(other, w);
     }
     long long run = u;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += x; }
-    if (lane == 31) warp_sums[warp] = run;
+    if (lane == 31) plan.sums[warp] = run;
+    if (theirs) atomicAdd(reinterpret_cast<unsigned long long*>(plan.sums + 31), (unsigned long long)theirs);
     __syncthreads();
     long long all = 0, before = 0;
-    for (int v = 0; v < warps; ++v) { if (v < warp) before += warp_sums[v]; all += warp_sums[v]; }
-    if (o < owners) starts[o] = base + before + run - u;
-    if (theirs) atomicAdd(reinterpret_cast<unsigned long long*>(plan.sums + 31), (unsigned long long)theirs);
+    for (int v = 0; v < warps; ++v) { if (v < warp) before += plan.sums[v]; all += plan.sums[v]; }
+    if (o < owners) plan.starts[o] = base + before + run - u;
     base += all;
     __syncthreads();
   }
-  if (tid == 0) starts[owners] = base;
+  if (tid == 0) plan.starts[owners] = base;
   __syncthreads();
 }
 
@@ -205,12 +231,12 @@ __device__ __forceinline__ int wide_sms(int sms, long long wide, long long narro
 struct Piece {
   Owner w;
   int tile, kv_head, item;
-  int first, last, lo;      // keys first .. last - 1 of whole units; visible ones are lo .. Span.last - 1 of these
+  int first, last, lo;      // keys first .. last - 1 of whole units; visible ones are lo .. last - 1 of these
   int row0, tokens;         // of the tile
 };
 struct Walk {
   long long at, end, total, workers;
-  int o, tile;              // where `at` lies
+  int o, tile, cost;        // where the last piece was; what an item of the tile costs
   long long tile_start;     // the first unit of the tile
   int open;                 // the owner whose numbers are in w
   Owner w;
@@ -237,45 +263,50 @@ struct Walk {
   // The next piece; false: there is none.
   __device__ __forceinline__ bool next(const Call& c, const Plan& plan, Piece& p) {
     const long long* starts = plan.starts;
-    if (at >= end) return false;
-    while (at >= starts[o + 1]) { ++o; tile = 0; tile_start = starts[o]; }
-    if (open != o) {
-      w = plan.owners[o];
-      open = o;
-      if (w.group && at > tile_start) {      // tiles of a group are alike
-        const long long per = (long long)tile_span(c, w, 0).units * c.kv_heads;
-        tile = (int)((at - tile_start) / per);
-        tile_start += tile * per;
+    while (at < end) {
+      while (at >= starts[o + 1]) { ++o; tile = 0; tile_start = starts[o]; }
+      if (open != o) {
+        w = plan.owners[o];
+        open = o;
+        if (w.group && at > tile_start) {      // tiles of a group are alike
+          const long long per = (long long)span_cost(c, tile_span(c, w, 0)) * c.kv_heads;
+          tile = (int)((at - tile_start) / per);
+          tile_start += tile * per;
+        }
       }
+      Span s = tile_span(c, w, tile);
+      cost = span_cost(c, s);
+      while (at >= tile_start + (long long)cost * c.kv_heads) {
+        tile_start += (long long)cost * c.kv_heads;
+        s = tile_span(c, w, ++tile);
+        cost = span_cost(c, s);
+      }
+      const int in_tile = (int)(at - tile_start), head = in_tile / cost, v0 = in_tile % cost;
+      const int v1 = (int)min((long long)cost, v0 + (end - at));
+      const int u0 = max(0, v0 - c.extra), u1 = v1 - c.extra;
+      at += v1 - v0;
+      if (u1 <= u0) continue;      // the worker's share is of the item's extra units
+      p.w = w;
+      p.tile = tile;
+      p.kv_head = head;
+      p.item = owner_item(c, w, o) + tile * c.kv_heads + head;
+      p.first = s.first + u0 * c.unit;
+      p.last = min(s.last, s.first + u1 * c.unit);
+      p.lo = max(s.lo, p.first);
+      p.row0 = w.row0 + tile * c.tokens;
+      p.tokens = min(c.tokens, w.row1 - p.row0);
+      return true;
     }
-    Span s = tile_span(c, w, tile);
-    while (at >= tile_start + (long long)s.units * c.kv_heads) {
-      tile_start += (long long)s.units * c.kv_heads;
-      s = tile_span(c, w, ++tile);
-    }
-    const int in_tile = (int)(at - tile_start);
-    p.w = w;
-    p.tile = tile;
-    p.kv_head = in_tile / s.units;
-    const int u0 = in_tile % s.units;
-    const long long rest = end - at;
-    const int u1 = (int)min((long long)s.units, u0 + rest);
-    p.item = owner_item(c, w, o) + tile * c.kv_heads + p.kv_head;
-    p.first = s.first + u0 * c.unit;
-    p.last = min(s.last, s.first + u1 * c.unit);
-    p.lo = max(s.lo, p.first);
-    p.row0 = w.row0 + tile * c.tokens;
-    p.tokens = min(c.tokens, w.row1 - p.row0);
-    at += u1 - u0;
-    return true;
+    return false;
   }
   // The workers that have pieces of the item whose piece came last.
   __device__ __forceinline__ int2 item_workers(const Call& c, const Piece& p) const {
-    const Span s = tile_span(c, p.w, p.tile);
-    const long long a = tile_start + (long long)p.kv_head * s.units, b = a + s.units - 1;
-    return make_int2((int)(((a + 1) * workers - 1) / total), (int)(((b + 1) * workers - 1) / total));
+    const long long a = tile_start + (long long)p.kv_head * cost, b = a + cost;
+    return make_int2((int)(((a + c.extra + 1) * workers - 1) / total), (int)((b * workers - 1) / total));
   }
 };
+// Whether a piece is all that its rows have (`at`: its item's workers): it is written out where it is worked on.
+__device__ __forceinline__ bool is_sole(const Piece& p, int2 at) { return !p.w.group && p.w.lo == 0 && at.x == at.y; }
 
 // The position of a query row of an owner: of a group's row by its request.
 __device__ __forceinline__ int row_position(const Call& c, const Plan& plan, const Owner& w, int row) {
@@ -296,78 +327,120 @@ __device__ __forceinline__ long long page_at(const Call& c, int request, int pag
   return id * c.page_stride;
 }
 
-// ---------------------------------------------------------------------------------------------------- the join
-// A block takes a token's heads, a warp one head at a time; a lane has columns lane, lane + 32, ...  `wide` and `narrow`: the classes' calls (of
-// `wide.which` EVERY there is no other).
-constexpr int JOIN_WARPS = 8;
-template <typename T>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ Call wide, const __grid_constant__ Call narrow, int dim, T* out) {
-  __shared__ int found[1];
-  ifb_pdl_wait();
-  ifb_pdl_trigger();
-  const int token = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  for (int r = tid; r < wide.n_req; r += JOIN_WARPS * 32)
-    if (request_row(wide, r) <= token && token < request_row(wide, r + 1)) found[0] = r;
-  __syncthreads();
-  const int r = found[0];
-  if (r < 0) return;      // a row of no request: left as it is
-  const int g = group_of(wide, r), group = wide.heads / wide.kv_heads;
-  const int head = blockIdx.y * JOIN_WARPS + (tid >> 5);
-  if (head >= wide.heads) return;
-  const int kv_head = head / group;
-  int first[2] = {0, 0}, last[2] = {-1, -1};
-  const float2* ml_at[2] = {nullptr, nullptr};      // of the item's slot for worker 0
-  const float* o_at[2] = {nullptr, nullptr};
-  int rows[2] = {0, 0};
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int o = k == 0 ? g : wide.n_groups + r;
-    if (o < 0) continue;
-    const Owner w = owner_at(wide, o);
-    const Call& c = wide.which != EVERY && is_narrow(wide, w) ? narrow : wide;
-    const int tile = (token - w.row0) / c.tokens;
-    if (tile_span(c, w, tile).units == 0) continue;
-    const int item = owner_item(c, w, o) + tile * c.kv_heads + kv_head;
-    const int2 workers = c.pieces[item];
-    first[k] = max(0, workers.x); last[k] = min(workers.y, c.workers - 1);
-    rows[k] = c.rows;
-    const long long at = (long long)item * c.rows + (token - w.row0 - tile * c.tokens) * group + head % group;
-    ml_at[k] = c.part_ml + at;
-    o_at[k] = c.part_o + at * dim;
-  }
-  float m = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    for (int x = first[k] + lane; x <= last[k]; x += 32) m = fmaxf(m, ml_at[k][(long long)x * rows[k]].x);
-  m = warp_max(m);
-  constexpr int PER = 256 / 32;
-  float acc[PER], den = 0.f;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) acc[j] = 0.f;
-  if (m == -INFINITY) m = 0.f;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    for (int x = first[k]; x <= last[k]; ++x) {
-      const float2 ml = ml_at[k][(long long)x * rows[k]];
-      if (ml.y == 0.f) continue;      // a piece of which the row sees nothing
-      const float f = exp2f(ml.x - m);
-      den = fmaf(f, ml.y, den);
-      const float* o = o_at[k] + (long long)x * rows[k] * dim;
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (lane + j * 32 < dim) acc[j] = fmaf(f, o[lane + j * 32], acc[j]);
+// Where a row's pieces are, for the join: of its group's item (x, y) and its request's (z, w).  The item of key head 0, or -1: none (x = -2: no request's
+// row); row of head 0 in the tile, NARROW_PART if its class is that, SOLE_PART if one piece of it would be all.
+constexpr int NARROW_PART = 1 << 16, SOLE_PART = 1 << 17;
+// The threads of all CTAs of a kernel call it together, each for some rows.
+__device__ inline void write_parts(const Call& wide, const Call& narrow, const Plan& plan) {
+  const int N = wide.n_groups, G = wide.heads / wide.kv_heads;
+  auto find = [&](const Owner* owners, int n, int token) {      // the first that ends behind it, if it begins at or before it
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (owners[mid].row1 <= token) lo = mid + 1; else hi = mid;
     }
-  const float inv = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den;      // (NaN stays)
-  T* dst = out + ((long long)token * wide.heads + head) * dim;
+    return lo < n && owners[lo].row0 <= token ? lo : -1;
+  };
+  for (int token = blockIdx.x * blockDim.x + threadIdx.x; token < wide.n_tokens; token += gridDim.x * blockDim.x) {
+    int at[4] = {-1, 0, -1, 0};
+    const int r = find(plan.owners + N, wide.n_req, token), g = find(plan.owners, N, token);
+    if (r < 0) at[0] = -2;
 #pragma unroll
-  for (int j = 0; j < PER; ++j)
-    if (lane + j * 32 < dim) dst[lane + j * 32] = from_f32<T>(acc[j] * inv);
+    for (int k = 0; k < 2; ++k) {
+      if (r < 0 || (k == 0 && g < 0)) continue;
+      const int o = k == 0 ? g : N + r;
+      const Owner w = plan.owners[o];
+      const bool few = wide.which != EVERY && is_narrow(wide, w);
+      const Call& c = few ? narrow : wide;
+      const int tile = (token - w.row0) / c.tokens;
+      if (tile_span(c, w, tile).units == 0) continue;
+      at[2 * k] = owner_item(c, w, o) + tile * c.kv_heads;
+      at[2 * k + 1] = (token - w.row0 - tile * c.tokens) * G | (few ? NARROW_PART : 0) | (k == 1 && w.lo == 0 ? SOLE_PART : 0);
+    }
+    wide.parts[token] = make_int4(at[0], at[1], at[2], at[3]);
+  }
 }
 
-template <typename T> static int join(const Call& wide, const Call& narrow, int dim, T* out, cudaStream_t stream) {
-  return ifb_launch(join_kernel<T>, dim3(wide.n_tokens, (wide.heads + JOIN_WARPS - 1) / JOIN_WARPS), dim3(JOIN_WARPS * 32), 0, stream, wide, narrow, dim, out);
+// ---------------------------------------------------------------------------------------------------- the join
+// A warp takes a head of a token; a lane has the columns from 4 lane and 128 + 4 lane on.  `wide` and `narrow`: the classes' calls (the same one where
+// there is one kernel only).  Lane x first has piece x: its maximum and denominator, from which the factor that its sums get.
+constexpr int JOIN_WARPS = 8;
+template <typename T>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ Call wide, const __grid_constant__ Call narrow, int dim) {
+  ifb_pdl_wait();
+  ifb_pdl_trigger();
+  const int token = blockIdx.x, lane = threadIdx.x & 31, head = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5);
+  if (head >= wide.heads) return;
+  const int4 at = wide.parts[token];
+  if (at.x == -2) return;      // a row of no request: left as it is
+  const int group = wide.heads / wide.kv_heads, kv_head = head / group;
+  int first[2] = {0, 0}, count[2] = {0, 0}, rows[2] = {0, 0};
+  const float2* ml_at[2] = {nullptr, nullptr};      // of the item's slot for its first worker
+  const float* o_at[2] = {nullptr, nullptr};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int item = (k ? at.z : at.x) + kv_head, how = k ? at.w : at.y;
+    if (item < kv_head) continue;
+    const Call& c = how & NARROW_PART ? narrow : wide;
+    const int2 workers = c.pieces[item];
+    if (how & SOLE_PART && workers.x == workers.y) return;      // it is written already
+    first[k] = clamp(workers.x, 0, c.workers - 1);
+    count[k] = clamp(workers.y, 0, c.workers - 1) - first[k] + 1;
+    rows[k] = c.rows;
+    const long long slot = (long long)(item + first[k]) * c.rows + (how & 0xffff) + head % group;
+    ml_at[k] = c.part_ml + slot;
+    o_at[k] = c.part_o + slot * dim;
+  }
+  const int n = max(0, count[0]) + max(0, count[1]);
+  // in turns of 32 pieces, against a running maximum
+  float m = -INFINITY, den = 0.f;
+  float4 acc[2] = {};
+  for (int x0 = 0; x0 < n; x0 += 32) {
+    const int x = x0 + lane;
+    const bool k = x >= count[0];
+    const long long i = (long long)(k ? x - count[0] : x) * (k ? rows[1] : rows[0]);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    const float* src = nullptr;
+    if (x < n) {
+      ml = (k ? ml_at[1] : ml_at[0])[i];
+      src = (k ? o_at[1] : o_at[0]) + i * dim;
+    }
+    const float next = fmaxf(m, warp_max(ml.y == 0.f ? -INFINITY : ml.x)), ref = next == -INFINITY ? 0.f : next;
+    const float keep = exp2f(m - ref), f = ml.y == 0.f ? 0.f : exp2f(ml.x - ref);      // (a piece of which the row sees nothing has weight 0)
+    m = next;
+    den = fmaf(den, keep, warp_sum(f * ml.y));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) { acc[j].x *= keep; acc[j].y *= keep; acc[j].z *= keep; acc[j].w *= keep; }
+    const int turn = min(32, n - x0);
+#pragma unroll 4
+    for (int t = 0; t < turn; ++t) {
+      const float g = __shfl_sync(0xffffffffu, f, t);
+      const float* o = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, t));
+      if (g == 0.f) continue;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int col = j * 128 + lane * 4;
+        if (col < dim) {
+          const float4 v = *reinterpret_cast<const float4*>(o + col);
+          acc[j].x = fmaf(g, v.x, acc[j].x); acc[j].y = fmaf(g, v.y, acc[j].y); acc[j].z = fmaf(g, v.z, acc[j].z); acc[j].w = fmaf(g, v.w, acc[j].w);
+        }
+      }
+    }
+  }
+  const float inv = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den;      // (NaN stays)
+  T* dst = reinterpret_cast<T*>(wide.out) + ((long long)token * wide.heads + head) * dim;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int col = j * 128 + lane * 4;
+    if (col < dim) {
+      dst[col] = from_f32<T>(acc[j].x * inv); dst[col + 1] = from_f32<T>(acc[j].y * inv);
+      dst[col + 2] = from_f32<T>(acc[j].z * inv); dst[col + 3] = from_f32<T>(acc[j].w * inv);
+    }
+  }
+}
+
+template <typename T> static int join(const Call& wide, const Call& narrow, int dim, cudaStream_t stream) {
+  return ifb_launch(join_kernel<T>, dim3(wide.n_tokens, (wide.heads + JOIN_WARPS - 1) / JOIN_WARPS), dim3(JOIN_WARPS * 32), 0, stream, wide, narrow, dim);
 }
 
 }  // namespace shared_attention

@@ -36,7 +36,7 @@ static Call wide_call(bool tc, int n_tokens, int n_req, int n_groups, int kv_hea
 IFB_EXPORT long long ifb_attention_shared_bf16_room(int n_tokens, int n_req, int n_groups, int kv_heads, int group) {
   const long long a = room_bytes(wide_call(true, n_tokens, n_req, n_groups, kv_heads, group, 16), D);
   const long long b = room_bytes(wide_call(false, n_tokens, n_req, n_groups, kv_heads, group, 16), D);
-  return (a > b ? a : b) + room_bytes(narrow::call(n_tokens, n_req, n_groups, kv_heads, group), D);
+  return parts_bytes(n_tokens) + (a > b ? a : b) + room_bytes(narrow::call(n_tokens, n_req, n_groups, kv_heads, group), D);
 }
 
 // As ifb_attention_shared.
@@ -59,22 +59,26 @@ IFB_EXPORT int ifb_attention_shared_bf16(const __nv_bfloat16* q, long long q_row
     c->table_pages = table_pages; c->page_size = page_size; c->window = window;
     c->scale_log2 = scale * 1.4426950408889634f;
     c->err = err;
+    c->out = out;
+    c->parts = (int4*)room;
   }
-  room_at(wide, D, room);
-  room_at(few, D, (char*)room + room_bytes(wide, D));
+  char* rest = (char*)room + parts_bytes(n_tokens);
+  room_at(wide, D, rest);
+  room_at(few, D, rest + room_bytes(wide, D));
   const bool any_wide = (long long)n_tokens * group > NARROW_ROWS;      // no owner has more rows than all
+  const bool any_narrow = group <= NARROW_ROWS;
   int st = IFB_OK;
   if (any_wide) {
 #if HEAD_DIM <= 128
-    if (tc) st = tc_main(wide, few, q, q_row, pages, stream);
+    if (tc) st = tc_main(wide, few, q, q_row, pages, !any_narrow, stream);
     else
 #endif
-      st = sh_main<__nv_bfloat16, (D <= 64 ? 8 : D <= 128 ? 16 : 32)>(wide, few, q, q_row, pages, D, stream);
+      st = sh_main<__nv_bfloat16, (D <= 64 ? 8 : D <= 128 ? 16 : 32)>(wide, few, q, q_row, pages, D, !any_narrow, stream);
     if (st) return st;
   }
-  if (group <= NARROW_ROWS) {
+  if (any_narrow) {
     st = narrow::run(few, wide, q, q_row, pages, any_wide, stream);
     if (st) return st;
   }
-  return join<__nv_bfloat16>(wide, few, D, out, stream);
+  return join<__nv_bfloat16>(wide, few, D, stream);
 }

@@ -35,7 +35,7 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void* 
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)) : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -76,18 +76,25 @@ shared_narrow_kernel(const __grid_constant__ Call c, const __grid_constant__ Cal
   int akey = 0;
   bool more = ahead.next(c, plan, ap);
   if (more) akey = ap.first;
-  int put = 0;
+  int put = 0, page0 = 0, id = 0;      // the piece's pages page0 .. page0 + 31, one a lane
+  bool fresh = true;
   auto request = [&]() {      // the next chunk of 16 keys, if there is one; a group of copies in any case
     if (more) {
       bf16* st = stages + put * STAGE_ELEMENTS;
       put = put + 1 == STAGES ? 0 : put + 1;
-      // lanes 0 .. 15 find the places of the chunk's keys
+      // lanes 0 .. 15 (16 .. 31 likewise) find the places of the chunk's keys; the table is asked once for 32 pages
+      const int key = akey + (lane & 15), page = key / c.page_size;
+      if (fresh || __shfl_sync(0xffffffffu, page, 15) >= page0 + 32) {
+        page0 = __shfl_sync(0xffffffffu, page, 0);
+        const int first = (page0 + lane) * c.page_size;      // of the lane's page
+        id = first < ap.last ? c.block_tables[ap.w.table(first) * c.bt_stride + page0 + lane] : -1;
+        fresh = false;
+      }
+      const int mine = __shfl_sync(0xffffffffu, id, page - page0 & 31);
       long long at = -1;
-      const int key = akey + (lane & 15);
       if (key >= ap.lo && key < ap.last) {
-        at = page_at(c, ap.w.request, key / c.page_size);
-        if (at < 0) atomicExch(c.err, IFB_DEV_ERR_SHARED_PAGE);
-        else at += ((long long)ap.kv_head * c.page_size + key % c.page_size) * D;
+        if (mine < 0 || mine >= c.num_pages) atomicExch(c.err, IFB_DEV_ERR_SHARED_PAGE);
+        else at = mine * c.page_stride + ((long long)ap.kv_head * c.page_size + key - page * c.page_size) * D;
       }
       constexpr int PARTS = D / 8;      // 16-byte parts of a row
 #pragma unroll
@@ -104,12 +111,14 @@ shared_narrow_kernel(const __grid_constant__ Call c, const __grid_constant__ Cal
       if (akey >= ap.last) {
         more = ahead.next(c, plan, ap);
         if (more) akey = ap.first;
+        fresh = true;
       }
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) request();
+  write_parts(other, c, plan);
 
   // ---- products
   Walk walk;
@@ -149,16 +158,20 @@ shared_narrow_kernel(const __grid_constant__ Call c, const __grid_constant__ Cal
       request();                       // over that one
       const bf16 *Ks = stages + get * STAGE_ELEMENTS, *Vs = Ks + CHUNK * PITCH;
       get = get + 1 == STAGES ? 0 : get + 1;
-      float s[2][4];
+      float s[2][4], odd[2][4];      // of even and of odd steps along the head: two chains of products in place of one
 #pragma unroll
-      for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = odd[n][0] = odd[n][1] = odd[n][2] = odd[n][3] = 0.f;
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
         uint32_t b[4];
         ldmatrix_x4(b, Ks + ((lane & 7) + ((lane >> 4) << 3)) * PITCH + k * 16 + (((lane >> 3) & 1) << 3));
-        mma(s[0], qf[k], b[0], b[1]);
-        mma(s[1], qf[k], b[2], b[3]);
+        mma(k & 1 ? odd[0] : s[0], qf[k], b[0], b[1]);
+        mma(k & 1 ? odd[1] : s[1], qf[k], b[2], b[3]);
       }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += odd[n][e];
       // rows A and B of the scores, keys key0 + 8 n + 2 (lane & 3) + j
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -215,20 +228,27 @@ shared_narrow_kernel(const __grid_constant__ Call c, const __grid_constant__ Cal
         mma(o[2 * n + 1], a2, b[2], b[3]);
       }
     }
+    const int2 workers = walk.item_workers(c, p);
+    const bool sole = is_sole(p, workers);
     const long long slot = (long long)(p.item + worker) * c.rows;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       const int row = r ? rowB : rowA;
-      if (row < rows) {
+      if (row < rows && sole) {
+        const float inv = l[r] > 0.f ? 1.f / l[r] : l[r] == 0.f ? 0.f : l[r];      // (NaN stays)
+        bf16* dst = reinterpret_cast<bf16*>(c.out) + ((long long)(p.row0 + row / G) * c.heads + p.kv_head * G + row % G) * D + ((lane & 3) << 1);
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) *reinterpret_cast<__nv_bfloat162*>(dst + n * 8) = __floats2bfloat162_rn(o[n][2 * r] * inv, o[n][2 * r + 1] * inv);
+      } else if (row < rows) {
         if ((lane & 3) == 0) c.part_ml[slot + row] = make_float2(m[r], l[r]);
         float* dst = c.part_o + (slot + row) * D + ((lane & 3) << 1);
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
       }
     }
-    if (lane == 0) c.pieces[p.item] = walk.item_workers(c, p);
+    if (lane == 0) c.pieces[p.item] = workers;
   }
   asm volatile("cp.async.wait_all;\n" ::: "memory");
   if (beside && (blockIdx.x == 0 || (int)blockIdx.x * WARPS < limit)) ifb_pdl_wait();      // (one CTA that waits is enough for the grid)
@@ -242,6 +262,7 @@ static inline Call call(int n_tokens, int n_req, int n_groups, int kv_heads, int
   c.tokens = group <= NARROW_ROWS ? NARROW_ROWS / group : 1; c.unit = UNIT; c.rows = NARROW_ROWS; c.align = 1;
   c.workers = ifb_sm_count() * CTAS_PER_SM * WARPS;
   c.cost = 1;
+  c.extra = 1;
   return c;
 }
 static int run(const Call& c, const Call& other, const bf16* q, long long q_row, const bf16* pages, bool beside, cudaStream_t stream) {

@@ -24,9 +24,9 @@ __device__ __forceinline__ void sh_row4(float* dst, const T* src, bool valid) { 
   *reinterpret_cast<float4*>(dst) = v;
 }
 
-// DC: columns of a thread, the head size over eight rounded up to 8, 16 or 32.
+// parts: whether this kernel writes where the rows' pieces are.  DC: columns of a thread, the head size over eight rounded up to 8, 16 or 32.
 template <typename T, int DC>
-__global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_constant__ Call c, const __grid_constant__ Call other, const T* q, long long q_row, const T* pages, int dim) {
+__global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_constant__ Call c, const __grid_constant__ Call other, const T* q, long long q_row, const T* pages, int dim, int parts) {
   extern __shared__ __align__(16) unsigned char sh_smem[];
   const Plan plan = plan_at(sh_smem, c.n_groups + c.n_req);
   const int pitch = dim + 4;
@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_co
   Walk walk;
   const int ctas = c.which == EVERY ? c.workers : wide_sms(c.workers, plan.starts[c.n_groups + c.n_req] * c.cost, plan.sums[31] * other.cost);
   walk.begin(c, plan, blockIdx.x, ctas);
+  if (parts) write_parts(c, other, plan);
   const int tid = threadIdx.x, x = tid & 7, y = tid >> 3, quads = dim / 4;
   const int group = c.heads / c.kv_heads;
   const long long values = (long long)c.kv_heads * c.page_size * dim;      // from a page's keys to its values
@@ -71,7 +72,7 @@ __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_co
         long long at = 0;
         bool valid = in;
         if (in) {
-          at = page_at(c, p.w.request, key / c.page_size);
+          at = page_at(c, p.w.table(key), key / c.page_size);
           valid = at >= 0;
           if (!valid) atomicExch(c.err, IFB_DEV_ERR_SHARED_PAGE);
           at += ((long long)p.kv_head * c.page_size + key % c.page_size) * dim + col;
@@ -143,6 +144,8 @@ __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_co
       }
       __syncwarp();
     }
+    const int2 workers = walk.item_workers(c, p);
+    const bool sole = is_sole(p, workers);
     const long long slot = (long long)(p.item + blockIdx.x) * c.rows;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -150,12 +153,20 @@ __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_co
 #pragma unroll
       for (int d = 1; d < 8; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
       if (row >= rows) continue;
+      if (sole) {
+        const float inv = l[e] > 0.f ? 1.f / l[e] : l[e] == 0.f ? 0.f : l[e];      // (NaN stays)
+        T* dst = reinterpret_cast<T*>(c.out) + ((long long)(p.row0 + row / group) * c.heads + p.kv_head * group + row % group) * dim;
+#pragma unroll
+        for (int j = 0; j < DC; ++j)
+          if (x + 8 * j < dim) dst[x + 8 * j] = from_f32<T>(o[e][j] * inv);
+        continue;
+      }
       if (x == 0) c.part_ml[slot + row] = make_float2(m[e], l[e]);
 #pragma unroll
       for (int j = 0; j < DC; ++j)
         if (x + 8 * j < dim) c.part_o[(slot + row) * dim + x + 8 * j] = o[e][j];
     }
-    if (tid == 0) c.pieces[p.item] = walk.item_workers(c, p);
+    if (tid == 0) c.pieces[p.item] = workers;
   }
 }
 
@@ -167,12 +178,13 @@ static inline Call sh_call(int n_tokens, int n_req, int n_groups, int kv_heads, 
   c.tokens = SH_ROWS / group; c.unit = SH_UNIT; c.rows = SH_ROWS; c.align = 1;
   c.workers = ifb_sm_count();
   c.cost = 16;
+  c.extra = 1;
   return c;
 }
 // (one function for each kernel: what IFB_ALLOW_SMEM remembers is a kernel's)
 template <typename T, int DC>
-static int sh_main(const Call& c, const Call& other, const T* q, long long q_row, const T* pages, int dim, cudaStream_t stream) {
+static int sh_main(const Call& c, const Call& other, const T* q, long long q_row, const T* pages, int dim, bool parts, cudaStream_t stream) {
   const size_t smem = plan_bytes(c.n_req + c.n_groups) + (size_t)((SH_ROWS + 2 * SH_UNIT) * (dim + 4) + SH_ROWS * 33) * 4;
   IFB_ALLOW_SMEM((shared_simt_kernel<T, DC>), smem);
-  return ifb_launch(shared_simt_kernel<T, DC>, dim3(c.workers), dim3(SH_THREADS), smem, stream, c, other, q, q_row, pages, dim);
+  return ifb_launch(shared_simt_kernel<T, DC>, dim3(c.workers), dim3(SH_THREADS), smem, stream, c, other, q, q_row, pages, dim, parts ? 1 : 0);
 }

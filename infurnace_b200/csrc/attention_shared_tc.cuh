@@ -52,7 +52,7 @@ struct PageRows { int page, total; };      // the pool as a matrix of rows: rows
 
 __global__ void __launch_bounds__(THREADS, 1)
 shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                 PageRows mrows, const __grid_constant__ Call c, const __grid_constant__ Call other) {
+                 PageRows mrows, const __grid_constant__ Call c, const __grid_constant__ Call other, int parts) {
   extern __shared__ unsigned char tc_smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t tmem_slot;
@@ -104,6 +104,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   Walk walk;
   walk.begin(c, plan, blockIdx.x, wide_sms(c.workers, plan.starts[c.n_groups + c.n_req] * c.cost, plan.sums[31] * other.cost));
   Piece p;
+  if (parts) write_parts(c, other, plan);
 
   if (warp == 0 || warp == 3) {
     // ---------------- producers: queries and keys, and values
@@ -130,7 +131,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         const int pg = lane / DH, half = lane % DH, key0 = p.first + j * UNIT + pg * c.page_size;
         int y = mrows.total;                                 // beyond the pool: zeros
         if (lane < n_ops && key0 < p.last && key0 + c.page_size > p.lo) {
-          const int id = c.block_tables[p.w.request * c.bt_stride + (key0 >> ps_shift)];
+          const int id = c.block_tables[p.w.table(key0) * c.bt_stride + (key0 >> ps_shift)];
           if (id >= 0 && id < c.num_pages) y = id * mrows.page + p.kv_head * c.page_size;
           else atomicExch(err, IFB_DEV_ERR_SHARED_PAGE);
         }
@@ -353,16 +354,21 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       asm volatile("bar.sync 2, 256;\n" ::: "memory");          // the eight softmax warps, on every path
       tc_fence_after();
       const bool go = __all_sync(0xffffffffu, !*abort_flag) != 0;
+      const int2 workers = walk.item_workers(c, p);
       if (go && work) {
         const float m0 = merge_m[par][0][row], m1 = merge_m[par][1][row], l0 = merge_l[par][0][row], l1 = merge_l[par][1][row];
         const float m = fmaxf(m0, m1);
         const float a0 = m0 == -INFINITY ? 0.f : tc_exp2(m0 - m), a1 = m1 == -INFINITY ? 0.f : tc_exp2(m1 - m);
         const bool two = n_half > 1;                             // stream 1's accumulator holds something of this piece
         const uint32_t o_addr = tmem + ((uint32_t)(qd * 32) << 16) + COL_O;
+        const float ml = (m0 == -INFINITY ? l0 : a0 * l0) + (m1 == -INFINITY ? l1 : a1 * l1);
+        const bool sole = is_sole(p, workers);
+        const float inv = !sole ? 1.f : ml > 0.f ? 1.f / ml : ml == 0.f ? 0.f : ml;      // (NaN stays)
+        const float w0 = a0 * inv, w1 = a1 * inv;
         const long long slot = (long long)(p.item + blockIdx.x) * ROWS + row;
         float* dst = c.part_o + (slot - lane) * D;               // of the warp's first row
         const int count = min(32, p.tokens * G - qd * 32);       // its rows that exist
-        if (x == 0 && exists) c.part_ml[slot] = make_float2(m, (m0 == -INFINITY ? l0 : a0 * l0) + (m1 == -INFINITY ? l1 : a1 * l1));
+        if (x == 0 && exists && !sole) c.part_ml[slot] = make_float2(m, ml);
 #pragma unroll 1
         for (int cc = 0; cc < DN / 64; ++cc) {
           const int col0 = x * (DN / 2) + cc * 32;
@@ -373,23 +379,34 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           float y[32];
           // (a stream in which the row sees nothing has sums of zero)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(oa[i]) * a0;
+          for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(oa[i]) * w0;
           if (two) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = fmaf(__uint_as_float(ob[i]), a1, y[i]);
+            for (int i = 0; i < 32; ++i) y[i] = fmaf(__uint_as_float(ob[i]), w1, y[i]);
           }
           // a row's 128 bytes by eight lanes: through shared memory, a row of it 36 numbers long (no two lanes of a quarter on a bank)
 #pragma unroll
           for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(stage + lane * 36 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
           __syncwarp();
           const int col = lane % 8 * 4;
-          if (DN == D || col0 + col < D)
-            for (int q = lane / 8; q < count; q += 4)
-              *reinterpret_cast<float4*>(dst + q * D + col0 + col) = *reinterpret_cast<const float4*>(stage + q * 36 + col);
+          if (DN == D || col0 + col < D) {
+            if (!sole) {
+              for (int q = lane / 8; q < count; q += 4)
+                *reinterpret_cast<float4*>(dst + q * D + col0 + col) = *reinterpret_cast<const float4*>(stage + q * 36 + col);
+            } else {
+              for (int q = lane / 8; q < count; q += 4) {
+                const int r = qd * 32 + q;
+                const float4 v = *reinterpret_cast<const float4*>(stage + q * 36 + col);
+                const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+                bf16* to = reinterpret_cast<bf16*>(c.out) + ((long long)(p.row0 + r / G) * c.heads + p.kv_head * G + r % G) * D + col0 + col;
+                *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+              }
+            }
+          }
           __syncwarp();
         }
       }
-      if (threadIdx.x == 128 && go) c.pieces[p.item] = walk.item_workers(c, p);
+      if (threadIdx.x == 128 && go) c.pieces[p.item] = workers;
       tc_fence_before();
       tc_mbar_arrive(&bars.o_free);            // this piece's sums have been read
       if (!go) break;
@@ -416,9 +433,10 @@ static inline Call tc_call(int n_tokens, int n_req, int n_groups, int kv_heads, 
   c.tokens = ROWS / group; c.unit = UNIT; c.rows = ROWS; c.align = page_size;
   c.workers = ifb_sm_count();
   c.cost = 8;
+  c.extra = 2;
   return c;
 }
-static int tc_main(const Call& c, const Call& other, const bf16* q, long long q_row, const bf16* pages, cudaStream_t stream) {
+static int tc_main(const Call& c, const Call& other, const bf16* q, long long q_row, const bf16* pages, bool parts, cudaStream_t stream) {
   const int group = c.heads / c.kv_heads;
   const long long page_rows = c.page_stride / D, rows = (c.num_pages - 1) * page_rows + (long long)c.kv_heads * c.page_size;
   CUtensorMap q_map, k_map, v_map;
@@ -434,5 +452,5 @@ static int tc_main(const Call& c, const Call& other, const bf16* q, long long q_
   if (ifb_tensor_map_bf16(&v_map, pages + (long long)c.kv_heads * c.page_size * D, 2, dims, strides, box)) return IFB_ERR_ARG;
   const size_t smem = TILES_BYTES + STAGES_BYTES + plan_bytes(c.n_req + c.n_groups);
   IFB_ALLOW_SMEM(shared_tc_kernel, smem);
-  return ifb_launch(shared_tc_kernel, dim3(c.workers), dim3(THREADS), smem, stream, q_map, k_map, v_map, PageRows{(int)page_rows, (int)rows}, c, other);
+  return ifb_launch(shared_tc_kernel, dim3(c.workers), dim3(THREADS), smem, stream, q_map, k_map, v_map, PageRows{(int)page_rows, (int)rows}, c, other, parts ? 1 : 0);
 }

@@ -94,6 +94,8 @@ SCENES = {
     "no-groups": dict(groups=[], alone=[(5, 1), (130, 1), (257, 1), (64, 30)]),
     "nothing-of-its-own": dict(groups=[(64, [(64, 1), (64, 1), (64, 3)])]),
     "questions": dict(groups=[(300, [(330, 30), (341, 41), (301, 1)]), (128, [(200, 72), (128, 2)])]),
+    "full-tiles": dict(groups=[(208, [(330, 90), (208, 70), (200, 60), (209, 1)]), (37, [(150, 100), (120, 80)]), (64, [(64, 64)])], alone=[(130, 130)]),
+    "full-tiles-window": dict(groups=[(208, [(330, 90), (208, 70), (200, 60), (209, 1)])], window=77, page=32),
     "empty-requests": dict(groups=[(48, [(50, 1), (0, 1), (49, 0), (51, 2)]), (20, [(0, 0)])], alone=[(0, 1), (3, 3)], rows_behind=5),
     "in-the-shared-part": dict(groups=[(200, [(200, 60), (150, 10), (260, 20)])]),
     "window": dict(groups=[(300, [(310, 1), (420, 1), (305, 5)]), (64, [(500, 1)])], alone=[(90, 40)], window=100),
