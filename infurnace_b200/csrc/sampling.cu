@@ -12,9 +12,10 @@
 // threads share it.  2^44 times the largest vocabulary stays below 2^63.
 //
 // A row is shared by a cluster of C CTAs, which keep its slices in shared memory as float32: it is read from memory once.  A cut is found by counts (top-k)
-// or weights (top-p) in bins of equal width over (l - m) / T; the bin that the cut runs through is divided once more if it
-// has many members; the members left are put in order by one CTA.  Where too many are left (ties), a search over the ordered bits of their
-// values finds the last value that is kept, and a count in index order the last of its tokens.
+// or weights (top-p) in bins of equal width over (l - m) / T.  At first the bins reach 14 factors of two down, where nearly all cuts are and few tokens, so
+// that few take part in the bins' atomics (what lies below is one sum); a cut that is not there is looked for over all 46.  The bin that the cut
+// runs through is divided once more if it has many members; the members left are put in order by one CTA.  Where too many are left (ties), a
+// search over the ordered bits of their values finds the last value that is kept, and a count in index order the last of its tokens.
 #include "common.cuh"
 #include <math.h>
 #include <type_traits>
@@ -24,13 +25,13 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int NT = 512;                  // threads of a CTA
 constexpr int NW = NT / 32;
-constexpr int BINS = 1024;               // over REACH factors of two below the largest weight: beyond them a weight is 0
-constexpr float REACH = 46.f;
+constexpr int BINS = 1023;               // over a reach of factors of two below the largest weight; place BINS holds the sum of what lies beyond
+constexpr float NEAR = 14.f, REACH = 46.f;      // (beyond the latter a weight is 0)
 constexpr int SUBS = 256;                // parts of a bin
 constexpr int LIST = NT;                 // members that are put in order, one a thread
 constexpr int MAX_CLUSTER = 8;
 constexpr int SLICE = 46080;             // most logits of a CTA: 180 KB
-constexpr int SHARED_SLICE = 20480;      // up to here two CTAs fit on an SM
+constexpr int SHARED_SLICE = 19072;      // up to here two CTAs fit on an SM
 constexpr double UNIT = 17592186044416.0;      // 2^44
 constexpr u64 ALL = ~0ull;
 
@@ -73,40 +74,44 @@ __device__ __forceinline__ void row_sync(int ctas) {
 }
 
 // ---------------------------------------------------------------------------------------------------- weights
-// 2^(j / 32), in shared memory.
-struct Exp2Table { double t[32]; };
-// round(2^44 2^y) for y <= 0 as a whole number; `w`: before rounding.  y = (n + f) / 32, n whole, |f| <= 1/2: 2^y = 2^(n / 32) e^(f ln 2 / 32), the
-// latter by its Taylor series, whose sixth power is below 3e-15.  Weights below 2^-46 are 0.
-__device__ __forceinline__ u64 weight_of(double y, const Exp2Table& tab, double& w) {
-  if (!(y >= -46.0)) { w = 0.0; return 0; }
-  constexpr double MAGIC = 6755399441055744.0 / 32.0;      // 1.5 2^52 / 32: the sum's last bit is 1/32
-  constexpr double LN2 = 0.693147180559945309417;
-  constexpr double C1 = LN2, C2 = LN2 * LN2 / 2, C3 = LN2 * LN2 * LN2 / 6, C4 = C3 * LN2 / 4, C5 = C4 * LN2 / 5;
-  const double t = y + MAGIC;
-  const double r = y - (t - MAGIC);
-  const int n = __double2loint(t);
-  const double scale = tab.t[n & 31];
-  double p = fma(r, C5, C4);
-  p = fma(r, p, C3);
-  p = fma(r, p, C2);
-  p = fma(r, p, C1);
-  p = fma(r, p, 1.0);
-  w = p * __hiloint2double(__double2hiint(scale) + (((n >> 5) + 44) << 20), __double2loint(scale));
-  return (u64)__double_as_longlong(w + 4503599627370496.0) & ((1ull << 52) - 1);
-}
+// 2^(j / 256), in shared memory.
+constexpr int STEPS = 256;
+struct Exp2Table { double t[STEPS]; };
 
 // How a row's numbers become weights.
 struct RowScale {
-  float m;          // the largest logit
+  double m, s;      // the largest logit, log2(e) / T
+  float top;        // the largest logit
   float to_bin;     // bins per unit of m - l
-  double s;         // log2(e) / T
+  float to_log2;    // s
 };
-__device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp2Table& tab, double& w) {
-  const double y = l == rs.m ? 0.0 : ((double)l - (double)rs.m) * rs.s;      // (infinities too)
-  return weight_of(y, tab, w);
+// round(2^44 2^y), y = (l - m) s <= 0, as a whole number; `w`, if wanted: before rounding.  y = (n + f) / 256, n whole, |f| <= 1/2: 2^y = 2^(n / 256) e^x,
+// x = f ln 2 / 256, by the first terms of its Taylor series (x^4 / 24 < 2e-13).  Weights below 2^-46 are 0.  Eight operations in 64 bits.
+__device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp2Table& tab, double* w = nullptr) {
+  if (l == rs.top) {      // (infinities too)
+    if (w) *w = UNIT;
+    return (u64)UNIT;
+  }
+  if (!((rs.top - l) * rs.to_log2 < REACH)) {
+    if (w) *w = 0.0;
+    return 0;
+  }
+  constexpr double MAGIC = 6755399441055744.0 / STEPS;      // 1.5 2^52 / 256: the sum's last bit is 1/256
+  constexpr double LN2 = 0.693147180559945309417;
+  const double d = (double)l - rs.m;
+  const double t = fma(d, rs.s, MAGIC);
+  const double r = fma(d, rs.s, -(t - MAGIC));
+  const int n = __double2loint(t);
+  const double step = tab.t[n & (STEPS - 1)];
+  const double scale = __hiloint2double(__double2hiint(step) + (((n >> 8) + 44) << 20), __double2loint(step));
+  double p = fma(r, LN2 * LN2 * LN2 / 6, LN2 * LN2 / 2);
+  p = fma(r, p, LN2);
+  p = fma(r, p, 1.0);
+  if (w) *w = p * scale;
+  return (u64)__double_as_longlong(fma(p, scale, 4503599627370496.0)) & ((1ull << 52) - 1);
 }
 // The place of a number in bins of equal width; BINS or more (NaN included): its weight is 0.
-__device__ __forceinline__ float row_bin(float l, const RowScale& rs) { return l == rs.m ? 0.f : (rs.m - l) * rs.to_bin; }
+__device__ __forceinline__ float row_bin(float l, const RowScale& rs) { return l == rs.top ? 0.f : (rs.top - l) * rs.to_bin; }
 
 // An order-preserving whole number of a float32 number that is not NaN (-0 was made 0).
 __device__ __forceinline__ uint32_t ordered(float l) {
@@ -255,12 +260,12 @@ struct Cut { float l; int i; u64 mass; };
 __device__ __forceinline__ bool kept(float l, int i, const Cut& c) { return l > c.l || (l == c.l && i <= c.i); }
 
 struct CutMemory {      // of a CTA, behind its slice of the row
-  uint32_t* count; uint32_t* lo; uint32_t* hi;             // its own bins [BINS] each; one CTA's list of members lies over them
-  uint32_t* row_count; u64* row_mass;                      // the row's bins [BINS]
+  uint32_t* count; uint32_t* lo; uint32_t* hi;             // its own bins [BINS + 1] each
+  uint32_t* row_count; u64* row_mass;                      // the row's bins [BINS + 1]
   uint32_t* sub_count; u64* sub_mass;                      // the row's parts of a bin [SUBS]
+  u64* list_mass; float* list_l; uint32_t* list_i;         // the members of a bin [LIST]
 };
-constexpr size_t CUT_BYTES = (size_t)BINS * 12 + (size_t)BINS * 12 + (size_t)SUBS * 12;
-static_assert(LIST * (8 + 4 + 4) <= BINS * 12, "a list of members must fit over a CTA's own bins");
+constexpr size_t CUT_BYTES = (size_t)(BINS + 1) * 24 + (size_t)SUBS * 12 + (size_t)LIST * 16;
 
 __device__ __forceinline__ void add_mass(uint32_t* lo, uint32_t* hi, int b, u64 w) {
   const uint32_t x = (uint32_t)w, old = atomicAdd(lo + b, x);
@@ -268,13 +273,13 @@ __device__ __forceinline__ void add_mass(uint32_t* lo, uint32_t* hi, int b, u64 
   if (up) atomicAdd(hi + b, up);
 }
 
-// The cut through the row's bins after which `goal` tokens (by_mass: at least `goal` of weight) are kept.  `all`: the answer where that is everything.
-__device__ Cut find_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, bool by_mass, u64 goal, bool weighted,
-                        const Cut& all) {
+// The cut through the row's bins after which `goal` tokens (by_mass: at least `goal` of weight) are kept.  False: it does not run through them.
+__device__ bool find_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, bool by_mass, u64 goal, bool weighted,
+                         Cut& cut) {
   CutShared* sh = row.sh;
   u64 bc, bm;
   const int b0 = find_bin(sh, BINS, mem.row_count, mem.row_mass, by_mass, goal, bc, bm, weighted);
-  if (b0 >= BINS) return all;
+  if (b0 >= BINS) return false;
   uint32_t members = mem.row_count[b0];
   int b1 = -1;
   if (members > LIST) {
@@ -286,12 +291,12 @@ __device__ Cut find_cut(Row& row, const CutMemory& mem, const float* vals, int n
       if (!(f < BINS) || (int)f != b0) continue;
       const int b = (int)((f - b0) * SUBS);      // exact until the last step
       atomicAdd(mem.count + b, 1u);
-      if (weighted) { double w; add_mass(mem.lo, mem.hi, b, row_weight(vals[i], rs, sh->tab, w)); }
+      if (weighted) add_mass(mem.lo, mem.hi, b, row_weight(vals[i], rs, sh->tab));
     }
     merge_bins(row, SUBS, mem.count, mem.lo, mem.hi, mem.sub_count, mem.sub_mass, weighted);
     u64 c1, m1;
     b1 = find_bin(sh, SUBS, mem.sub_count, mem.sub_mass, by_mass, goal - (by_mass ? bm : bc), c1, m1, weighted);
-    if (b1 >= SUBS) return all;      // (never: the parts have what the bin has)
+    if (b1 >= SUBS) return false;      // (never: the parts have what the bin has)
     bc += c1; bm += m1;
     members = mem.sub_count[b1];
   }
@@ -300,24 +305,22 @@ __device__ Cut find_cut(Row& row, const CutMemory& mem, const float* vals, int n
     return f < BINS && (int)f == b0 && (b1 < 0 || (int)((f - b0) * SUBS) == b1);
   };
   if (members <= LIST) {
-    u64* lw = reinterpret_cast<u64*>(mem.count);
-    float* ll = reinterpret_cast<float*>(lw + LIST);
-    uint32_t* li = reinterpret_cast<uint32_t*>(ll + LIST);
-    if (threadIdx.x == 0) sh->listed = 0;
-    row_sync(row.ctas);      // nobody reads its bins any more
+    u64* lw = mem.list_mass;
+    float* ll = mem.list_l;
+    uint32_t* li = mem.list_i;
     for (int i = threadIdx.x; i < n; i += NT) {
       const float l = vals[i];
       if (!member(l)) continue;
-      const uint32_t at = add_peer(&sh->listed, 0, 1u);
+      const uint32_t at = add_peer(&sh->listed, 0, 1u);      // (0 whenever a list begins: set before the kernel's first barrier and by the one who reads it)
       if (at >= LIST) continue;      // (never: the members were counted)
-      double w;
-      put_u64(lw + at, 0, weighted ? row_weight(l, rs, sh->tab, w) : 0);
+      put_u64(lw + at, 0, weighted ? row_weight(l, rs, sh->tab) : 0);
       put_u32(reinterpret_cast<uint32_t*>(ll) + at, 0, __float_as_uint(l));
       put_u32(li + at, 0, (uint32_t)(base + i));
     }
     row_sync(row.ctas);
     if (row.rank == 0) {
       const int i = threadIdx.x;
+      if (i == 0) sh->listed = 0;
       if (i < (int)members) {
         const float l = ll[i];
         const uint32_t idx = li[i];
@@ -334,12 +337,11 @@ __device__ Cut find_cut(Row& row, const CutMemory& mem, const float* vals, int n
       }
     }
     row_sync(row.ctas);
-    Cut c;
-    c.l = __uint_as_float((uint32_t)(sh->found[0] >> 32));
-    c.i = (int)(uint32_t)sh->found[0];
-    c.mass = sh->found[1];
+    cut.l = __uint_as_float((uint32_t)(sh->found[0] >> 32));
+    cut.i = (int)(uint32_t)sh->found[0];
+    cut.mass = sh->found[1];
     __syncthreads();
-    return c;
+    return true;
   }
   // Many members within a hundred-thousandth of a factor of two: the smallest key above which less than the goal lies, by halving, then its ties in order.
   u64 top = 0, low = ALL;
@@ -353,7 +355,7 @@ __device__ Cut find_cut(Row& row, const CutMemory& mem, const float* vals, int n
       const float l = vals[i];
       if (!member(l)) continue;
       const u64 k = ordered(l);
-      if (k > key) { ++c; if (weighted) { double x; w += row_weight(l, rs, sh->tab, x); } }
+      if (k > key) { ++c; if (weighted) w += row_weight(l, rs, sh->tab); }
       t += k == key;
     }
     row.sum(c, w);
@@ -367,10 +369,8 @@ __device__ Cut find_cut(Row& row, const CutMemory& mem, const float* vals, int n
     if ((by_mass ? w : c) < goal) top = mid; else low = mid + 1;
   }
   above(top, c, w, ties);
-  Cut cut;
   cut.l = unordered((uint32_t)top);
-  double x;
-  const u64 each = weighted ? row_weight(cut.l, rs, sh->tab, x) : 0;
+  const u64 each = weighted ? row_weight(cut.l, rs, sh->tab) : 0;
   u64 take = by_mass ? (each ? (goal - w + each - 1) / each : ties) : goal - c;
   if (take > ties) take = ties;
   cut.mass = w + take * each;
@@ -386,7 +386,7 @@ __device__ Cut find_cut(Row& row, const CutMemory& mem, const float* vals, int n
   row_sync(row.ctas);
   cut.i = (int)sh->found[0];
   __syncthreads();
-  return cut;
+  return true;
 }
 
 template <typename T> struct Vec16;
@@ -427,18 +427,22 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   float* vals = reinterpret_cast<float*>(cut_smem);
   CutMemory mem;
   mem.row_mass = reinterpret_cast<u64*>(cut_smem + (size_t)((a.per + 3) & ~3) * 4);
-  mem.sub_mass = mem.row_mass + BINS;
-  mem.count = reinterpret_cast<uint32_t*>(mem.sub_mass + SUBS);
-  mem.lo = mem.count + BINS;
-  mem.hi = mem.lo + BINS;
-  mem.row_count = mem.hi + BINS;
-  mem.sub_count = mem.row_count + BINS;
+  mem.sub_mass = mem.row_mass + BINS + 1;
+  mem.list_mass = mem.sub_mass + SUBS;
+  mem.list_l = reinterpret_cast<float*>(mem.list_mass + LIST);
+  mem.list_i = reinterpret_cast<uint32_t*>(mem.list_l + LIST);
+  mem.count = mem.list_i + LIST;
+  mem.lo = mem.count + BINS + 1;
+  mem.hi = mem.lo + BINS + 1;
+  mem.row_count = mem.hi + BINS + 1;
+  mem.sub_count = mem.row_count + BINS + 1;
   Row row = {sh, cluster_size(), cluster_rank(), 0};
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long r = blockIdx.x / row.ctas;
   const int base = min((long long)a.vocab, (long long)row.rank * a.per), n = min(a.vocab - base, a.per);
-  if (tid < 32) sh->tab.t[tid] = exp2(tid / 32.0);
-  for (int b = tid; b < BINS; b += NT) mem.count[b] = mem.lo[b] = mem.hi[b] = 0;
+  if (tid < STEPS) sh->tab.t[tid] = exp2(tid / (double)STEPS);
+  if (tid == 0) sh->listed = 0;
+  for (int b = tid; b <= BINS; b += NT) mem.count[b] = mem.lo[b] = mem.hi[b] = 0;
   if (row.ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
   ifb_pdl_wait();
   ifb_pdl_trigger();
@@ -489,40 +493,56 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
     return;
   }
   RowScale rs;
-  rs.m = m;
+  rs.top = m;
+  rs.m = (double)m;
   rs.s = 1.4426950408889634074 / (double)temp;
-  rs.to_bin = (float)fmin(rs.s * (BINS / (double)REACH), 3e38);
+  rs.to_log2 = (float)fmin(rs.s, 3e38);
   const int k = a.top_k ? a.top_k[r] : 0;
-  const float p = a.top_p ? a.top_p[r] : 1.f;
-  const double least = a.min_p ? (double)a.min_p[r] * UNIT : 0.0;
-  const bool by_count = k >= 1 && k < a.vocab, by_mass = p < 1.f;
+  const float p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
+  const bool by_count = k >= 1 && k < a.vocab, by_mass = p < 1.f, by_least = least > 0.f;
 
   // ---- what top-k and top-p keep
   Cut cut = {-INFINITY, 0x7fffffff, 0};
   if (by_count || by_mass) {
-    for (int i = tid; i < n; i += NT) {
-      const float l = vals[i], f = row_bin(l, rs);
-      if (!(f < BINS)) continue;
-      atomicAdd(mem.count + (int)f, 1u);
-      if (by_mass) { double w; add_mass(mem.lo, mem.hi, (int)f, row_weight(l, rs, sh->tab, w)); }
-    }
-    merge_bins(row, BINS, mem.count, mem.lo, mem.hi, mem.row_count, mem.row_mass, by_mass);
-    if (by_mass) {
-      u64 x = 0, unused = 0;
-      for (int b = tid; b < BINS; b += NT) x += mem.row_mass[b];
-      // (every CTA has the row's bins: their sum needs no peer)
-      x = warp_add(x);
-      __syncthreads();
-      if (lane == 0) sh->warp_a[warp] = x;
-      __syncthreads();
-      for (int w = 0; w < NW; ++w) unused += sh->warp_a[w];
-      cut.mass = unused;
-      __syncthreads();
-    }
-    if (by_count) cut = find_cut(row, mem, vals, n, base, rs, false, (u64)k, by_mass, cut);
-    if (by_mass) {
-      const double want = ceil((double)p * (double)cut.mass);
-      cut = find_cut(row, mem, vals, n, base, rs, true, want >= 1.0 ? (u64)want : 1, true, cut);
+    bool counted = !by_count, done = false;
+    for (int far = 0; far < 2 && !done; ++far) {
+      rs.to_bin = (float)fmin(rs.s * (BINS / (double)(far ? REACH : NEAR)), 3e38);
+      if (far) {      // (no peer reads these any more)
+        for (int b = tid; b <= BINS; b += NT) mem.count[b] = mem.lo[b] = mem.hi[b] = 0;
+        __syncthreads();
+      }
+      u64 beyond = 0;
+      for (int i = tid; i < n; i += NT) {
+        const float l = vals[i], f = row_bin(l, rs);
+        if (f < BINS) {
+          atomicAdd(mem.count + (int)f, 1u);
+          if (by_mass) add_mass(mem.lo, mem.hi, (int)f, row_weight(l, rs, sh->tab));
+        } else if (by_mass) {
+          beyond += row_weight(l, rs, sh->tab);
+        }
+      }
+      beyond = warp_add(beyond);
+      if (lane == 0 && beyond) add_mass(mem.lo, mem.hi, BINS, beyond);
+      merge_bins(row, BINS + 1, mem.count, mem.lo, mem.hi, mem.row_count, mem.row_mass, by_mass);
+      u64 all = 0;
+      if (by_mass) {      // every CTA has the row's bins: their sum needs no peer
+        u64 x = 0;
+        for (int b = tid; b <= BINS; b += NT) x += mem.row_mass[b];
+        x = warp_add(x);
+        __syncthreads();
+        if (lane == 0) sh->warp_a[warp] = x;
+        __syncthreads();
+        for (int w = 0; w < NW; ++w) all += sh->warp_a[w];
+        __syncthreads();
+      }
+      cut.mass = all;
+      if (by_count) counted = find_cut(row, mem, vals, n, base, rs, false, (u64)k, by_mass, cut);
+      if (!counted && !far) continue;      // (with fewer than k tokens in all the bins top-k keeps everything)
+      done = true;
+      if (by_mass) {
+        const double want = ceil((double)p * (double)cut.mass);
+        done = find_cut(row, mem, vals, n, base, rs, true, want >= 1.0 ? (u64)want : 1, true, cut);
+      }
     }
   }
 
@@ -531,30 +551,67 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   auto weigh = [&](int i) -> u64 {
     const float l = vals[i];
     if (!kept(l, base + i, cut)) return 0;
+    if (!by_least) return row_weight(l, rs, sh->tab);
     double w;
-    const u64 whole = row_weight(l, rs, sh->tab, w);
-    return w >= least || l == m ? whole : 0;
+    const u64 whole = row_weight(l, rs, sh->tab, &w);
+    return w >= (double)least * UNIT || l == m ? whole : 0;
   };
   u64 mine = 0, total;
   for (int i = first; i < last; ++i) mine += weigh(i);
-  u64 at = row.before(mine, total);
+  const u64 at = row.before(mine, total);
   const float u = a.uniform[r];
   u64 goal = u > 0.f ? (u64)((double)u * (double)total) : 0;
   if (goal >= total) goal = total - 1;
-  if (at <= goal && at + mine > goal) {
-    for (int i = first; i < last; ++i) {
-      at += weigh(i);
-      if (at > goal) {
+  const unsigned owner = __ballot_sync(0xffffffffu, at <= goal && at + mine > goal);
+  if (owner) {      // the warp weighs that thread's tokens anew, a lane each
+    const int from = __ffs(owner) - 1, i0 = __shfl_sync(0xffffffffu, first, from), i1 = __shfl_sync(0xffffffffu, last, from);
+    u64 run = __shfl_sync(0xffffffffu, at, from);
+    for (int j = i0; j < i1; j += 32) {
+      const int i = j + lane;
+      const u64 w = i < i1 ? weigh(i) : 0;
+      u64 x = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const u64 y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+      if (run + x > goal && run + x - w <= goal) {
         a.out[r] = base + i;
         if (a.logprobs) {
           const float l = vals[i];
           a.logprobs[r] = (float)((l == m ? 0.0 : ((double)l - (double)m) / (double)temp) - log((double)total / UNIT));
         }
-        break;
       }
+      run += __shfl_sync(0xffffffffu, x, 31);
     }
   }
   row_sync(row.ctas);
+}
+
+// How many clusters of `ctas` CTAs with so much shared memory the device holds at a time (remembered by what they fit: two of them on an SM, or one); negative: an
+// error.
+static int cut_clusters(const void* kernel, int dtype, int ctas, size_t smem) {
+  static int known[IFB_MAX_DEVICES][2][2][MAX_CLUSTER + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= IFB_MAX_DEVICES) return 0;
+  const bool pair = smem <= (size_t)SHARED_SLICE * 4 + CUT_BYTES;
+  int& n = known[dev][dtype][pair][ctas];
+  if (n) return n;
+  const size_t size = pair ? (size_t)SHARED_SLICE * 4 + CUT_BYTES : (size_t)SLICE * 4 + CUT_BYTES;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((size_t)SLICE * 4 + CUT_BYTES));
+  if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = size;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int found = 0;
+  e = cudaOccupancyMaxActiveClusters(&found, kernel, &cfg);
+  if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
+  return n = found;
 }
 
 // logits [rows, vocab] with rows `pitch` elements apart (dtype IFB_F32 or IFB_BF16); per row: temperature, uniform number, and top_k, top_p, min_p (each or
@@ -565,11 +622,19 @@ IFB_EXPORT int ifb_sample_cut(const void* logits, int dtype, long long pitch, in
   if (rows <= 0) return IFB_OK;
   if (vocab < 1 || vocab > MAX_CLUSTER * SLICE || rows > (1 << 27)) return IFB_ERR_SIZE;
   if (!temperature || !uniform || !out) return IFB_ERR_ARG;
-  // As few CTAs of a row as let two share an SM; more while the rows leave SMs idle.
-  const int sms = ifb_sm_count();
+  // As few CTAs of a row as let two share an SM; more while all rows' clusters find their SMs at once.
+  const void* kernel = dtype == IFB_F32 ? (const void*)sample_cut_kernel<float> : dtype == IFB_BF16 ? (const void*)sample_cut_kernel<bf16> : nullptr;
+  if (!kernel) return IFB_ERR_DTYPE;
+  auto slice = [&](int n) { return ((vocab + n - 1) / n + 7) & ~7; };
   int ctas = 1;
-  while (ctas < MAX_CLUSTER && ((vocab + ctas - 1) / ctas > SHARED_SLICE || ((long long)rows * ctas * 2 <= 2 * sms && vocab / ctas >= 2048))) ctas *= 2;
-  CutArgs a = {pitch, vocab, ((vocab + ctas - 1) / ctas + 7) & ~7, temperature, top_k, top_p, min_p, uniform, out, logprobs};
+  while (ctas < MAX_CLUSTER && slice(ctas) > SHARED_SLICE) ctas *= 2;
+  while (ctas < MAX_CLUSTER && vocab / ctas >= 2048) {
+    const int clusters = cut_clusters(kernel, dtype, ctas * 2, (size_t)slice(ctas * 2) * 4 + CUT_BYTES);
+    if (clusters < 0) return clusters;
+    if (rows > clusters) break;
+    ctas *= 2;
+  }
+  CutArgs a = {pitch, vocab, slice(ctas), temperature, top_k, top_p, min_p, uniform, out, logprobs};
   const size_t smem = (size_t)a.per * 4 + CUT_BYTES;
   auto go = [&](auto kernel, auto typed) -> int {
     IFB_ALLOW_SMEM(kernel, smem);
