@@ -86,16 +86,10 @@ struct RowScale {
   float to_log2;    // s
 };
 // round(2^44 2^y), y = (l - m) s <= 0, as a whole number; `w`, if wanted: before rounding.  y = (n + f) / 256, n whole, |f| <= 1/2: 2^y = 2^(n / 256) e^x,
-// x = f ln 2 / 256, by the first terms of its Taylor series (x^4 / 24 < 2e-13).  Weights below 2^-46 are 0.  Eight operations in 64 bits.
+// x = f ln 2 / 256, by the first terms of its Taylor series (x^4 / 24 < 2e-13).  Weights below 2^-46 are 0.  Eight operations in 64 bits and a conversion,
+// without a branch, so that a thread has several numbers under way (one after the other they take 250 cycles each, four together 115).
 __device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp2Table& tab, double* w = nullptr) {
-  if (l == rs.top) {      // (infinities too)
-    if (w) *w = UNIT;
-    return (u64)UNIT;
-  }
-  if (!((rs.top - l) * rs.to_log2 < REACH)) {
-    if (w) *w = 0.0;
-    return 0;
-  }
+  const bool none = !((rs.top - l) * rs.to_log2 < REACH), best = l == rs.top;      // (infinities too)
   constexpr double MAGIC = 6755399441055744.0 / STEPS;      // 1.5 2^52 / 256: the sum's last bit is 1/256
   constexpr double LN2 = 0.693147180559945309417;
   const double d = (double)l - rs.m;
@@ -107,8 +101,9 @@ __device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp
   double p = fma(r, LN2 * LN2 * LN2 / 6, LN2 * LN2 / 2);
   p = fma(r, p, LN2);
   p = fma(r, p, 1.0);
-  if (w) *w = p * scale;
-  return (u64)__double_as_longlong(fma(p, scale, 4503599627370496.0)) & ((1ull << 52) - 1);
+  if (w) *w = best ? UNIT : none ? 0.0 : p * scale;
+  const u64 whole = (u64)__double_as_longlong(fma(p, scale, 4503599627370496.0)) & ((1ull << 52) - 1);
+  return best ? (u64)UNIT : none ? 0 : whole;
 }
 // The place of a number in bins of equal width; BINS or more (NaN included): its weight is 0.
 __device__ __forceinline__ float row_bin(float l, const RowScale& rs) { return l == rs.top ? 0.f : (rs.top - l) * rs.to_bin; }
@@ -319,14 +314,25 @@ __device__ bool find_cut(Row& row, const CutMemory& mem, const float* vals, int 
     }
     row_sync(row.ctas);
     if (row.rank == 0) {
-      const int i = threadIdx.x;
-      if (i == 0) sh->listed = 0;
-      if (i < (int)members) {
-        const float l = ll[i];
-        const uint32_t idx = li[i];
-        u64 pos = bc, mass = bm;
-        for (int j = 0; j < (int)members; ++j)
-          if (ll[j] > l || (ll[j] == l && li[j] < idx)) { ++pos; mass += lw[j]; }
+      if (threadIdx.x == 0) sh->listed = 0;
+      const int sub = threadIdx.x & 3;      // four threads count what comes before a member
+      for (int i0 = 0; i0 < (int)members; i0 += NT / 4) {
+        const int i = i0 + (int)(threadIdx.x >> 2);
+        const bool in = i < (int)members;
+        const float l = in ? ll[i] : INFINITY;
+        const uint32_t idx = in ? li[i] : 0;
+        u64 pos = 0, mass = 0;
+#pragma unroll 4
+        for (int j = sub; j < (int)members; j += 4) {
+          const float other = ll[j];
+          const bool first = other > l || (other == l && li[j] < idx);
+          pos += first;
+          mass += first ? lw[j] : 0;
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) { pos += __shfl_xor_sync(0xffffffffu, pos, o); mass += __shfl_xor_sync(0xffffffffu, mass, o); }
+        pos += bc; mass += bm;
+        if (!in || sub) continue;
         const u64 at = by_mass ? mass : pos, next = at + (by_mass ? lw[i] : 1);
         if (at < goal && (next >= goal || pos + 1 == bc + members)) {
           for (int r = 0; r < row.ctas; ++r) {
@@ -512,13 +518,24 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
         __syncthreads();
       }
       u64 beyond = 0;
-      for (int i = tid; i < n; i += NT) {
-        const float l = vals[i], f = row_bin(l, rs);
-        if (f < BINS) {
-          atomicAdd(mem.count + (int)f, 1u);
-          if (by_mass) add_mass(mem.lo, mem.hi, (int)f, row_weight(l, rs, sh->tab));
-        } else if (by_mass) {
-          beyond += row_weight(l, rs, sh->tab);
+      for (int i0 = tid; i0 < n; i0 += 4 * NT) {
+        float f[4];
+        u64 w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = i0 + j * NT;
+          const float l = i < n ? vals[i] : -INFINITY;
+          f[j] = row_bin(l, rs);
+          if (by_mass) w[j] = row_weight(l, rs, sh->tab);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (f[j] < BINS) {
+            atomicAdd(mem.count + (int)f[j], 1u);
+            if (by_mass) add_mass(mem.lo, mem.hi, (int)f[j], w[j]);
+          } else {
+            beyond += w[j];
+          }
         }
       }
       beyond = warp_add(beyond);
@@ -557,7 +574,20 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
     return w >= (double)least * UNIT || l == m ? whole : 0;
   };
   u64 mine = 0, total;
-  for (int i = first; i < last; ++i) mine += weigh(i);
+  int i = first;
+  if (!by_count && !by_mass && !by_least) {
+    for (; i + 4 <= last; i += 4)
+      mine += (row_weight(vals[i], rs, sh->tab) + row_weight(vals[i + 1], rs, sh->tab)) + (row_weight(vals[i + 2], rs, sh->tab) + row_weight(vals[i + 3], rs, sh->tab));
+  } else {      // most are not kept
+    float floor = cut.l;
+    if (by_least) {      // what min_p asks, and a little less
+      const float l = m - (0.01f - log2f(fminf(least, 1.f))) / rs.to_log2;
+      floor = fmaxf(floor, l - fabsf(l) * 2.4e-7f);
+    }
+    for (; i + 4 <= last; i += 4)
+      if (fmaxf(fmaxf(vals[i], vals[i + 1]), fmaxf(vals[i + 2], vals[i + 3])) >= floor) mine += (weigh(i) + weigh(i + 1)) + (weigh(i + 2) + weigh(i + 3));
+  }
+  for (; i < last; ++i) mine += weigh(i);
   const u64 at = row.before(mine, total);
   const float u = a.uniform[r];
   u64 goal = u > 0.f ? (u64)((double)u * (double)total) : 0;
