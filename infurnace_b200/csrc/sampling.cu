@@ -13,7 +13,7 @@
 //
 // A row is shared by a cluster of C CTAs, which keep its slices in shared memory as float32: it is read from memory once.  A cut is found by counts (top-k)
 // or weights (top-p) in bins of equal width over (l - m) / T.  At first the bins reach 14 factors of two down, where nearly all cuts are and few tokens, so
-// that few take part in the bins' atomics (what lies below is one sum); a cut that is not there is looked for over all 46.  The bin that the cut
+// that few take part in the bins' atomics (what lies below is one sum); a cut that is not there is looked for over 24, and then over all 46.  The bin that the cut
 // runs through is divided once more if it has many members; the members left are put in order by one CTA.  Where too many are left (ties), a
 // search over the ordered bits of their values finds the last value that is kept, and a count in index order the last of its tokens.
 #include "common.cuh"
@@ -26,10 +26,13 @@ typedef __nv_bfloat16 bf16;
 constexpr int NT = 512;                  // threads of a CTA
 constexpr int NW = NT / 32;
 constexpr int BINS = 1023;               // over a reach of factors of two below the largest weight; place BINS holds the sum of what lies beyond
-constexpr float NEAR = 14.f, REACH = 46.f;      // (beyond the latter a weight is 0)
+constexpr float REACH = 46.f;            // beyond it a weight is 0
+constexpr int TRIES = 3;                 // reaches of the bins: 14, 24, 46
+__device__ __forceinline__ float reach_of(int t) { return t == 0 ? 14.f : t == 1 ? 24.f : REACH; }
 constexpr int SUBS = 256;                // parts of a bin
 constexpr int LIST = NT;                 // members that are put in order, one a thread
-constexpr int MAX_CLUSTER = 8;
+constexpr int MAX_CLUSTER = 16;          // (beyond 8 a device may refuse: then no such cluster is taken)
+constexpr int SURE_CLUSTER = 8;
 constexpr int SLICE = 46080;             // most logits of a CTA: 180 KB
 constexpr int SHARED_SLICE = 19072;      // up to here two CTAs fit on an SM
 constexpr double UNIT = 17592186044416.0;      // 2^44
@@ -198,18 +201,24 @@ struct Row {
 __device__ __forceinline__ void merge_bins(const Row& row, int n, const uint32_t* own_count, const uint32_t* own_lo, const uint32_t* own_hi,
                                            uint32_t* count, u64* mass, bool weighted) {
   row_sync(row.ctas);
-  const int share = (n + row.ctas - 1) / row.ctas, first = row.rank * share, last = min(n, first + share);
-  for (int b = first + threadIdx.x; b < last; b += NT) {
+  // a CTA has a share of the bins, four threads each of these: each takes a quarter of the CTAs
+  const int share = (n + row.ctas - 1) / row.ctas, first = row.rank * share, last = min(n, first + share), q = threadIdx.x & 3;
+  for (int b0 = first; b0 < last; b0 += NT / 4) {
+    const int b = b0 + (int)(threadIdx.x >> 2);
     uint32_t c = 0;
     u64 w = 0;
-    for (int r = 0; r < row.ctas; ++r) {
-      c += peer_u32(own_count + b, r);
-      if (weighted) w += ((u64)peer_u32(own_hi + b, r) << 32) + peer_u32(own_lo + b, r);
-    }
-    for (int r = 0; r < row.ctas; ++r) {
-      put_u32(count + b, r, c);
-      if (weighted) put_u64(mass + b, r, w);
-    }
+    if (b < last)
+      for (int r = q; r < row.ctas; r += 4) {
+        c += peer_u32(own_count + b, r);
+        if (weighted) w += ((u64)peer_u32(own_hi + b, r) << 32) + peer_u32(own_lo + b, r);
+      }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) { c += __shfl_xor_sync(0xffffffffu, c, o); w += __shfl_xor_sync(0xffffffffu, w, o); }
+    if (b < last)
+      for (int r = q; r < row.ctas; r += 4) {
+        put_u32(count + b, r, c);
+        if (weighted) put_u64(mass + b, r, w);
+      }
   }
   row_sync(row.ctas);
 }
@@ -303,14 +312,25 @@ __device__ bool find_cut(Row& row, const CutMemory& mem, const float* vals, int 
     u64* lw = mem.list_mass;
     float* ll = mem.list_l;
     uint32_t* li = mem.list_i;
-    for (int i = threadIdx.x; i < n; i += NT) {
-      const float l = vals[i];
-      if (!member(l)) continue;
-      const uint32_t at = add_peer(&sh->listed, 0, 1u);      // (0 whenever a list begins: set before the kernel's first barrier and by the one who reads it)
-      if (at >= LIST) continue;      // (never: the members were counted)
-      put_u64(lw + at, 0, weighted ? row_weight(l, rs, sh->tab) : 0);
-      put_u32(reinterpret_cast<uint32_t*>(ll) + at, 0, __float_as_uint(l));
-      put_u32(li + at, 0, (uint32_t)(base + i));
+    const float f0 = b1 < 0 ? (float)b0 : b0 + b1 * (1.f / SUBS), f1 = b1 < 0 ? b0 + 1.f : b0 + (b1 + 1) * (1.f / SUBS);      // (exact)
+    for (int i0 = threadIdx.x; i0 < n; i0 += 4 * NT) {
+      bool in[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = i0 + j * NT < n ? row_bin(vals[i0 + j * NT], rs) : INFINITY;
+        in[j] = f >= f0 && f < f1;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!in[j]) continue;
+        const int i = i0 + j * NT;
+        const float l = vals[i];
+        const uint32_t at = add_peer(&sh->listed, 0, 1u);      // (0 whenever a list begins: set before the kernel's first barrier and by the one who reads it)
+        if (at >= LIST) continue;      // (never: the members were counted)
+        put_u64(lw + at, 0, weighted ? row_weight(l, rs, sh->tab) : 0);
+        put_u32(reinterpret_cast<uint32_t*>(ll) + at, 0, __float_as_uint(l));
+        put_u32(li + at, 0, (uint32_t)(base + i));
+      }
     }
     row_sync(row.ctas);
     if (row.rank == 0) {
@@ -453,6 +473,9 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   ifb_pdl_wait();
   ifb_pdl_trigger();
 
+  const float temp = a.temperature[r], u = a.uniform[r], p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
+  const int k = a.top_k ? a.top_k[r] : 0;
+
   // ---- the slice into shared memory, and its best token
   const T* src = logits + r * a.pitch + base;
   float bv = -INFINITY;
@@ -489,31 +512,28 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   const float m = unordered((uint32_t)(best >> 32));
   const int first_token = (int)~(uint32_t)best;
 
-  const float temp = a.temperature[r];
   if (!(temp > 0.f) || m == -INFINITY) {
     if (row.rank == 0 && tid == 0) {
       a.out[r] = m == -INFINITY ? 0 : first_token;
       if (a.logprobs) a.logprobs[r] = m == -INFINITY ? __uint_as_float(0x7fc00000u) : 0.f;
     }
-    row_sync(row.ctas);      // nobody leaves while a peer may write to it
-    return;
+    return;      // (what peers write to one another they have read behind a barrier: nobody need wait)
   }
   RowScale rs;
   rs.top = m;
   rs.m = (double)m;
   rs.s = 1.4426950408889634074 / (double)temp;
   rs.to_log2 = (float)fmin(rs.s, 3e38);
-  const int k = a.top_k ? a.top_k[r] : 0;
-  const float p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
   const bool by_count = k >= 1 && k < a.vocab, by_mass = p < 1.f, by_least = least > 0.f;
 
   // ---- what top-k and top-p keep
   Cut cut = {-INFINITY, 0x7fffffff, 0};
   if (by_count || by_mass) {
     bool counted = !by_count, done = false;
-    for (int far = 0; far < 2 && !done; ++far) {
-      rs.to_bin = (float)fmin(rs.s * (BINS / (double)(far ? REACH : NEAR)), 3e38);
-      if (far) {      // (no peer reads these any more)
+    for (int t = 0; t < TRIES && !done; ++t) {
+      const bool last_try = t == TRIES - 1;
+      rs.to_bin = (float)fmin(rs.s * (BINS / (double)reach_of(t)), 3e38);
+      if (t) {      // (no peer reads these any more)
         for (int b = tid; b <= BINS; b += NT) mem.count[b] = mem.lo[b] = mem.hi[b] = 0;
         __syncthreads();
       }
@@ -554,7 +574,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
       }
       cut.mass = all;
       if (by_count) counted = find_cut(row, mem, vals, n, base, rs, false, (u64)k, by_mass, cut);
-      if (!counted && !far) continue;      // (with fewer than k tokens in all the bins top-k keeps everything)
+      if (!counted && !last_try) continue;      // (with fewer than k tokens in the last try's bins top-k keeps everything)
       done = true;
       if (by_mass) {
         const double want = ceil((double)p * (double)cut.mass);
@@ -567,11 +587,9 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   const int chunk = ((n + NT - 1) / NT) | 1, first = min(n, tid * chunk), last = min(n, first + chunk);      // (odd: no two threads of a warp on a bank)
   auto weigh = [&](int i) -> u64 {
     const float l = vals[i];
-    if (!kept(l, base + i, cut)) return 0;
-    if (!by_least) return row_weight(l, rs, sh->tab);
     double w;
     const u64 whole = row_weight(l, rs, sh->tab, &w);
-    return w >= (double)least * UNIT || l == m ? whole : 0;
+    return kept(l, base + i, cut) && (!by_least || w >= (double)least * UNIT || l == m) ? whole : 0;
   };
   u64 mine = 0, total;
   int i = first;
@@ -589,7 +607,6 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   }
   for (; i < last; ++i) mine += weigh(i);
   const u64 at = row.before(mine, total);
-  const float u = a.uniform[r];
   u64 goal = u > 0.f ? (u64)((double)u * (double)total) : 0;
   if (goal >= total) goal = total - 1;
   const unsigned owner = __ballot_sync(0xffffffffu, at <= goal && at + mine > goal);
@@ -612,7 +629,6 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
       run += __shfl_sync(0xffffffffu, x, 31);
     }
   }
-  row_sync(row.ctas);
 }
 
 // How many clusters of `ctas` CTAs with so much shared memory the device holds at a time (remembered by what they fit: two of them on an SM, or one); negative: an
@@ -626,6 +642,7 @@ static int cut_clusters(const void* kernel, int dtype, int ctas, size_t smem) {
   if (n) return n;
   const size_t size = pair ? (size_t)SHARED_SLICE * 4 + CUT_BYTES : (size_t)SLICE * 4 + CUT_BYTES;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((size_t)SLICE * 4 + CUT_BYTES));
+  if (e == cudaSuccess && ctas > SURE_CLUSTER) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
@@ -646,18 +663,18 @@ static int cut_clusters(const void* kernel, int dtype, int ctas, size_t smem) {
 
 // logits [rows, vocab] with rows `pitch` elements apart (dtype IFB_F32 or IFB_BF16); per row: temperature, uniform number, and top_k, top_p, min_p (each or
 // null); out int32, logprobs float32 or null.
-IFB_EXPORT int ifb_sample_cut_max_vocab() { return MAX_CLUSTER * SLICE; }
+IFB_EXPORT int ifb_sample_cut_max_vocab() { return SURE_CLUSTER * SLICE; }
 IFB_EXPORT int ifb_sample_cut(const void* logits, int dtype, long long pitch, int rows, int vocab, const float* temperature, const float* uniform,
                               const int* top_k, const float* top_p, const float* min_p, int* out, float* logprobs, cudaStream_t stream) {
   if (rows <= 0) return IFB_OK;
-  if (vocab < 1 || vocab > MAX_CLUSTER * SLICE || rows > (1 << 27)) return IFB_ERR_SIZE;
+  if (vocab < 1 || vocab > SURE_CLUSTER * SLICE || rows > (1 << 27)) return IFB_ERR_SIZE;
   if (!temperature || !uniform || !out) return IFB_ERR_ARG;
   // As few CTAs of a row as let two share an SM; more while all rows' clusters find their SMs at once.
   const void* kernel = dtype == IFB_F32 ? (const void*)sample_cut_kernel<float> : dtype == IFB_BF16 ? (const void*)sample_cut_kernel<bf16> : nullptr;
   if (!kernel) return IFB_ERR_DTYPE;
   auto slice = [&](int n) { return ((vocab + n - 1) / n + 7) & ~7; };
   int ctas = 1;
-  while (ctas < MAX_CLUSTER && slice(ctas) > SHARED_SLICE) ctas *= 2;
+  while (ctas < SURE_CLUSTER && slice(ctas) > SHARED_SLICE) ctas *= 2;
   while (ctas < MAX_CLUSTER && vocab / ctas >= 2048) {
     const int clusters = cut_clusters(kernel, dtype, ctas * 2, (size_t)slice(ctas * 2) * 4 + CUT_BYTES);
     if (clusters < 0) return clusters;
@@ -832,7 +849,7 @@ IFB_EXPORT int ifb_token_logprobs(const void* logits, int dtype, long long pitch
   // several CTAs of a row while the rows leave room on the SMs (eight CTAs fit on each)
   const int sms = ifb_sm_count();
   int ctas = 1;
-  while (ctas < MAX_CLUSTER && (long long)rows * ctas * 2 <= 4 * sms && vocab / ctas >= 4096) ctas *= 2;
+  while (ctas < SURE_CLUSTER && (long long)rows * ctas * 2 <= 4 * sms && vocab / ctas >= 4096) ctas *= 2;
   const int per = ((vocab + ctas - 1) / ctas + 7) & ~7;
   auto go = [&](auto kernel, auto typed) -> int {
     cudaLaunchConfig_t cfg = {};
