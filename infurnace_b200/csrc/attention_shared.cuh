@@ -121,15 +121,15 @@ __device__ inline long long owner_cost(const Call& c, const Owner& w) {
 // What a CTA knows of all owners, in shared memory: what they are, their first units, and behind those the sum of all.
 struct Plan {
   long long* starts;      // [owners + 1]; before it is made, the call's numbers lie there
-  long long* sums;        // [32]: of warps; the last: cost of the other class
+  long long* sums;        // [64]: of warps; the second half: of the other class, its sum in the last
   Owner* owners;          // [owners]
 };
-__host__ __device__ inline size_t plan_bytes(int owners) { return (((size_t)(owners + 1) + 32) * 8 + 15 & ~(size_t)15) + (size_t)owners * sizeof(Owner); }
+__host__ __device__ inline size_t plan_bytes(int owners) { return (((size_t)(owners + 1) + 64) * 8 + 15 & ~(size_t)15) + (size_t)owners * sizeof(Owner); }
 __device__ __forceinline__ Plan plan_at(unsigned char* at, int owners) {
   Plan p;
   p.starts = reinterpret_cast<long long*>(at);
   p.sums = p.starts + owners + 1;
-  p.owners = reinterpret_cast<Owner*>(at + (((size_t)(owners + 1) + 32) * 8 + 15 & ~(size_t)15));
+  p.owners = reinterpret_cast<Owner*>(at + (((size_t)(owners + 1) + 64) * 8 + 15 & ~(size_t)15));
   return p;
 }
 // All threads of a CTA (up to 31 warps) call it.  The kernel before this one has ended (the call's numbers are its to write).  `other`: the other class's
@@ -192,10 +192,9 @@ __device__ inline void make_plan(const Call& c, const Call& other, const Plan& p
       }
       plan.owners[o] = w;
     }
-    if (tid == 0) plan.sums[31] = 0;
     __syncthreads();
   }
-  long long base = 0;
+  long long base = 0, other_base = 0;
   for (int o0 = 0; o0 < owners; o0 += nt) {
     const int o = o0 + tid;
     long long u = 0, theirs = 0;
@@ -207,16 +206,17 @@ __device__ inline void make_plan(const Call& c, const Call& other, const Plan& p
     long long run = u;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += x; }
-    if (lane == 31) plan.sums[warp] = run;
-    if (theirs) atomicAdd(reinterpret_cast<unsigned long long*>(plan.sums + 31), (unsigned long long)theirs);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) theirs += __shfl_xor_sync(0xffffffffu, theirs, d);
+    if (lane == 31) { plan.sums[warp] = run; plan.sums[32 + warp] = theirs; }
     __syncthreads();
     long long all = 0, before = 0;
-    for (int v = 0; v < warps; ++v) { if (v < warp) before += plan.sums[v]; all += plan.sums[v]; }
+    for (int v = 0; v < warps; ++v) { if (v < warp) before += plan.sums[v]; all += plan.sums[v]; other_base += plan.sums[32 + v]; }
     if (o < owners) plan.starts[o] = base + before + run - u;
     base += all;
     __syncthreads();
   }
-  if (tid == 0) plan.starts[owners] = base;
+  if (tid == 0) { plan.starts[owners] = base; plan.sums[63] = other_base; }
   __syncthreads();
 }
 
@@ -233,6 +233,7 @@ struct Piece {
   int tile, kv_head, item;
   int first, last, lo;      // keys first .. last - 1 of whole units; visible ones are lo .. last - 1 of these
   int row0, tokens;         // of the tile
+  bool whole;               // the item is this piece
 };
 struct Walk {
   long long at, end, total, workers;
@@ -295,12 +296,14 @@ struct Walk {
       p.lo = max(s.lo, p.first);
       p.row0 = w.row0 + tile * c.tokens;
       p.tokens = min(c.tokens, w.row1 - p.row0);
+      p.whole = u0 == 0 && u1 == s.units;
       return true;
     }
     return false;
   }
-  // The workers that have pieces of the item whose piece came last.
-  __device__ __forceinline__ int2 item_workers(const Call& c, const Piece& p) const {
+  // The workers that have pieces of the item whose piece came last, this worker being one.
+  __device__ __forceinline__ int2 item_workers(const Call& c, const Piece& p, int worker) const {
+    if (p.whole) return make_int2(worker, worker);
     const long long a = tile_start + (long long)p.kv_head * cost, b = a + cost;
     return make_int2((int)(((a + c.extra + 1) * workers - 1) / total), (int)((b * workers - 1) / total));
   }
@@ -412,17 +415,24 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
 #pragma unroll
     for (int j = 0; j < 2; ++j) { acc[j].x *= keep; acc[j].y *= keep; acc[j].z *= keep; acc[j].w *= keep; }
     const int turn = min(32, n - x0);
-#pragma unroll 4
-    for (int t = 0; t < turn; ++t) {
-      const float g = __shfl_sync(0xffffffffu, f, t);
-      const float* o = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, t));
-      if (g == 0.f) continue;
+    // eight pieces' sums are asked for at once
+    for (int t0 = 0; t0 < turn; t0 += 8) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int col = j * 128 + lane * 4;
-        if (col < dim) {
-          const float4 v = *reinterpret_cast<const float4*>(o + col);
-          acc[j].x = fmaf(g, v.x, acc[j].x); acc[j].y = fmaf(g, v.y, acc[j].y); acc[j].z = fmaf(g, v.z, acc[j].z); acc[j].w = fmaf(g, v.w, acc[j].w);
+        if (j * 128 >= dim) break;
+        float4 v[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const float* o = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, t0 + t & 31));
+          v[t] = t0 + t < turn && col < dim ? *reinterpret_cast<const float4*>(o + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const float g = __shfl_sync(0xffffffffu, f, t0 + t & 31);
+          if (g != 0.f && t0 + t < turn) {      // (what has weight 0 may be infinite or NaN)
+            acc[j].x = fmaf(g, v[t].x, acc[j].x); acc[j].y = fmaf(g, v[t].y, acc[j].y); acc[j].z = fmaf(g, v[t].z, acc[j].z); acc[j].w = fmaf(g, v[t].w, acc[j].w);
+          }
         }
       }
     }

@@ -3,7 +3,10 @@
 //
 // The work is the reading of keys and values.  Every warp is a worker of its own: it walks over its pieces in chunks of 16 keys, which it brings to its part
 // of shared memory by asynchronous copies of 16 bytes (any page size), two chunks ahead and across the ends of pieces, so that no warp waits for
-// another and 2 x 4 warps of an SM have 130 KB on their way.  The 16 score rows meet 16 keys in mma.sync products of bfloat16; a row's weights
+// another and 2 x 4 warps of an SM have 130 KB on their way.  Products are mma.sync of bfloat16 with the keys, and then the columns of the values, on the
+// side of 16 and the score rows on the side of eight, one or two times: S^T = K Q^T, O^T += V^T P^T.  (With the rows on the side of 16 a chunk of four rows
+// took 48 products in place of 24, and their issue, some 16 cycles each, was the longest part of it.)  In both a thread has rows 2 (lane mod 4) and
+// the next, so that the factors of a row's maximum need no exchange; weights cross over from accumulator to operand by movmatrix.  A row's weights
 // are formed in float32 against its running maximum and enter the second product as two bfloat16 terms (16 bits of a weight); sums are float32.
 #pragma once
 #include "attention_shared.cuh"
@@ -43,6 +46,12 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
+// An 8 x 8 matrix of 16-bit numbers, a row in four lanes, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
 // A pair of weights as bfloat16: rounded, and the rounding of what that left out.
 __device__ __forceinline__ void terms(float a, float b, uint32_t& first, uint32_t& second) {
   const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
@@ -65,13 +74,14 @@ shared_narrow_kernel(const __grid_constant__ Call c, const __grid_constant__ Cal
   make_plan(c, other, plan);
   const int G = c.heads / c.kv_heads;
   // the SMs that the wide owners' kernel leaves
-  const int mine = sms - wide_sms(sms, plan.sums[31] * other.cost, plan.starts[c.n_groups + c.n_req] * c.cost);
+  const int mine = sms - wide_sms(sms, plan.sums[63] * other.cost, plan.starts[c.n_groups + c.n_req] * c.cost);
   const int worker = blockIdx.x * WARPS + warp, limit = min(c.workers, mine * CTAS_PER_SM * WARPS);
   const long long values = (long long)c.kv_heads * c.page_size * D;
 
   // ---- the copies' walk, ahead of the products'
   Walk ahead;
   ahead.begin(c, plan, worker, limit);
+  Walk walk = ahead;      // the products'
   Piece ap;
   int akey = 0;
   bool more = ahead.next(c, plan, ap);
@@ -121,131 +131,137 @@ shared_narrow_kernel(const __grid_constant__ Call c, const __grid_constant__ Cal
   write_parts(other, c, plan);
 
   // ---- products
-  Walk walk;
-  walk.begin(c, plan, worker, limit);
   Piece p;
   int get = 0;
-  const int rowA = lane >> 2, rowB = rowA + 8;
+  const int pair = (lane & 3) << 1;      // the thread's rows of a tile of eight: pair, pair + 1
   while (walk.next(c, plan, p)) {
     const int rows = p.tokens * G;
-    uint32_t qf[KB][4];
-    {
-      const bool a = rowA < rows, b = rowB < rows;
-      const bf16* qa = q + (p.row0 + (a ? rowA / G : 0)) * q_row + (long long)(p.kv_head * G + (a ? rowA % G : 0)) * D + (lane & 3) * 2;
-      const bf16* qb = q + (p.row0 + (b ? rowB / G : 0)) * q_row + (long long)(p.kv_head * G + (b ? rowB % G : 0)) * D + (lane & 3) * 2;
+    const bool two = rows > 8;           // tiles of eight rows
+    uint32_t qf[2][KB][2];               // rows lane / 4 and lane / 4 + 8
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int row = (lane >> 2) + 8 * t;
+      const bool in = row < rows;
+      const bf16* src = q + (p.row0 + (in ? row / G : 0)) * q_row + (long long)(p.kv_head * G + (in ? row % G : 0)) * D + pair;
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        qf[k][0] = a ? *reinterpret_cast<const uint32_t*>(qa + k * 16) : 0u;
-        qf[k][1] = b ? *reinterpret_cast<const uint32_t*>(qb + k * 16) : 0u;
-        qf[k][2] = a ? *reinterpret_cast<const uint32_t*>(qa + k * 16 + 8) : 0u;
-        qf[k][3] = b ? *reinterpret_cast<const uint32_t*>(qb + k * 16 + 8) : 0u;
+        qf[t][k][0] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16) : 0u;
+        qf[t][k][1] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8) : 0u;
       }
     }
-    int lo[2], hi[2];
+    int lo[2][2], hi[2][2];
+    float m[2][2], l[2][2], o[2][KB][4];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int row = e ? rowB : rowA;
-      const int pos = row < rows ? row_position(c, plan, p.w, p.row0 + row / G) : NO_POSITION;
-      lo[e] = max(p.lo, c.window > 0 ? pos - c.window + 1 : 0);
-      hi[e] = min(p.last, pos + 1);
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = 8 * t + pair + e;
+        const int pos = row < rows ? row_position(c, plan, p.w, p.row0 + row / G) : NO_POSITION;
+        lo[t][e] = max(p.lo, c.window > 0 ? pos - c.window + 1 : 0);
+        hi[t][e] = min(p.last, pos + 1);
+        m[t][e] = -INFINITY; l[t][e] = 0.f;
+      }
+#pragma unroll
+      for (int n = 0; n < KB; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     for (int key0 = p.first; key0 < p.last; key0 += CHUNK) {
       asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
       __syncwarp();                    // the chunk is there for all lanes, and all are done with the one before
       request();                       // over that one
       const bf16 *Ks = stages + get * STAGE_ELEMENTS, *Vs = Ks + CHUNK * PITCH;
       get = get + 1 == STAGES ? 0 : get + 1;
-      float s[2][4], odd[2][4];      // of even and of odd steps along the head: two chains of products in place of one
+      float s[2][2][4];                // of even and of odd steps along the head: two chains of products in place of one
 #pragma unroll
-      for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = odd[n][0] = odd[n][1] = odd[n][2] = odd[n][3] = 0.f;
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][0][e] = s[t][1][e] = 0.f;
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        uint32_t b[4];
-        ldmatrix_x4(b, Ks + ((lane & 7) + ((lane >> 4) << 3)) * PITCH + k * 16 + (((lane >> 3) & 1) << 3));
-        mma(k & 1 ? odd[0] : s[0], qf[k], b[0], b[1]);
-        mma(k & 1 ? odd[1] : s[1], qf[k], b[2], b[3]);
+        uint32_t a[4];
+        ldmatrix_x4(a, Ks + (lane & 15) * PITCH + k * 16 + ((lane >> 4) << 3));
+        mma(s[0][k & 1], a, qf[0][k][0], qf[0][k][1]);
+        if (two) mma(s[1][k & 1], a, qf[1][k][0], qf[1][k][1]);
       }
+      uint32_t b1[2][2], b2[2][2];     // weights as operands: [tile][keys 0 .. 7, 8 .. 15]
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] += odd[n][e];
-      // rows A and B of the scores, keys key0 + 8 n + 2 (lane & 3) + j
-      float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int t = 0; t < 2; ++t) {
+        if (t && !two) break;
+        // z[e + 2 h]: key key0 + 8 h + lane / 4, row pair + e
+        float z[4], top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = key0 + 8 * n + ((lane & 3) << 1) + (e & 1), r = e >> 1;
-          const bool sees = key >= lo[r] && key < hi[r];
-          s[n][e] = sees ? s[n][e] * c.scale_log2 : -INFINITY;
-          top[r] = fmaxf(top[r], s[n][e]);
-        }
-      float ref[2];
-      bool grew = false;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-        grew |= top[r] > m[r];
-      }
-      if (__any_sync(0xffffffffu, grew)) {
-        float f[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float next = fmaxf(m[r], top[r]);
-          f[r] = next == m[r] ? 1.f : fast_exp2(m[r] - next);
-          m[r] = next;
-          l[r] *= f[r];
+          const int key = key0 + 8 * (e >> 1) + (lane >> 2);
+          const bool sees = key >= lo[t][e & 1] && key < hi[t][e & 1];
+          z[e] = sees ? (s[t][0][e] + s[t][1][e]) * c.scale_log2 : -INFINITY;
+          top[e & 1] = fmaxf(top[e & 1], z[e]);
         }
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) { o[n][0] *= f[0]; o[n][1] *= f[0]; o[n][2] *= f[1]; o[n][3] *= f[1]; }
-      }
+        for (int d = 4; d < 32; d <<= 1)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) ref[r] = m[r] == -INFINITY ? 0.f : m[r];
+          for (int e = 0; e < 2; ++e) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], d));
+        if (__any_sync(0xffffffffu, top[0] > m[t][0] || top[1] > m[t][1])) {
+          float f[2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+          for (int e = 0; e < 2; ++e) {
+            const float next = fmaxf(m[t][e], top[e]);
+            f[e] = next == m[t][e] ? 1.f : fast_exp2(m[t][e] - next);
+            m[t][e] = next;
+            l[t][e] *= f[e];
+          }
+#pragma unroll
+          for (int n = 0; n < KB; ++n) { o[t][n][0] *= f[0]; o[t][n][1] *= f[1]; o[t][n][2] *= f[0]; o[t][n][3] *= f[1]; }
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = key0 + 8 * n + ((lane & 3) << 1) + (e & 1), r = e >> 1;
-          s[n][e] = key >= lo[r] && key < hi[r] ? fast_exp2(s[n][e] - ref[r]) : 0.f;
-          l[r] += s[n][e];
+          const int key = key0 + 8 * (e >> 1) + (lane >> 2);
+          const float ref = m[t][e & 1] == -INFINITY ? 0.f : m[t][e & 1];
+          z[e] = key >= lo[t][e & 1] && key < hi[t][e & 1] ? fast_exp2(z[e] - ref) : 0.f;
+          l[t][e & 1] += z[e];
         }
-      uint32_t a1[4], a2[4];
-      terms(s[0][0], s[0][1], a1[0], a2[0]);
-      terms(s[0][2], s[0][3], a1[1], a2[1]);
-      terms(s[1][0], s[1][1], a1[2], a2[2]);
-      terms(s[1][2], s[1][3], a1[3], a2[3]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t first, second;
+          terms(z[2 * h], z[2 * h + 1], first, second);
+          b1[t][h] = transposed(first);
+          b2[t][h] = transposed(second);
+        }
+      }
 #pragma unroll
       for (int n = 0; n < KB; ++n) {
-        uint32_t b[4];
-        ldmatrix_x4_trans(b, Vs + ((lane & 7) + (((lane >> 3) & 1) << 3)) * PITCH + n * 16 + ((lane >> 4) << 3));
-        mma(o[2 * n], a1, b[0], b[1]);
-        mma(o[2 * n + 1], a1, b[2], b[3]);
-        mma(o[2 * n], a2, b[0], b[1]);
-        mma(o[2 * n + 1], a2, b[2], b[3]);
+        uint32_t a[4];      // columns 16 n .. 16 n + 15 by 16 keys
+        ldmatrix_x4_trans(a, Vs + ((lane & 7) + ((lane >> 4) << 3)) * PITCH + n * 16 + (((lane >> 3) & 1) << 3));
+        mma(o[0][n], a, b1[0][0], b1[0][1]);
+        if (two) mma(o[1][n], a, b1[1][0], b1[1][1]);
+        mma(o[0][n], a, b2[0][0], b2[0][1]);
+        if (two) mma(o[1][n], a, b2[1][0], b2[1][1]);
       }
     }
-    const int2 workers = walk.item_workers(c, p);
+    const int2 workers = walk.item_workers(c, p, worker);
     const bool sole = is_sole(p, workers);
     const long long slot = (long long)(p.item + worker) * c.rows;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      const int row = r ? rowB : rowA;
-      if (row < rows && sole) {
-        const float inv = l[r] > 0.f ? 1.f / l[r] : l[r] == 0.f ? 0.f : l[r];      // (NaN stays)
-        bf16* dst = reinterpret_cast<bf16*>(c.out) + ((long long)(p.row0 + row / G) * c.heads + p.kv_head * G + row % G) * D + ((lane & 3) << 1);
+    for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) *reinterpret_cast<__nv_bfloat162*>(dst + n * 8) = __floats2bfloat162_rn(o[n][2 * r] * inv, o[n][2 * r + 1] * inv);
-      } else if (row < rows) {
-        if ((lane & 3) == 0) c.part_ml[slot + row] = make_float2(m[r], l[r]);
-        float* dst = c.part_o + (slot + row) * D + ((lane & 3) << 1);
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+        for (int d = 4; d < 32; d <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], d);
+        const int row = 8 * t + pair + e;
+        if (row >= rows) continue;
+        // columns 16 n + lane / 4 and the one eight on: eight lanes write 32 bytes (16 of bfloat16) together
+        if (sole) {
+          const float inv = l[t][e] > 0.f ? 1.f / l[t][e] : l[t][e] == 0.f ? 0.f : l[t][e];      // (NaN stays)
+          bf16* dst = reinterpret_cast<bf16*>(c.out) + ((long long)(p.row0 + row / G) * c.heads + p.kv_head * G + row % G) * D + (lane >> 2);
+#pragma unroll
+          for (int n = 0; n < KB; ++n) {
+            dst[n * 16] = __float2bfloat16_rn(o[t][n][e] * inv);
+            dst[n * 16 + 8] = __float2bfloat16_rn(o[t][n][2 + e] * inv);
+          }
+        } else {
+          if (lane < 4) c.part_ml[slot + row] = make_float2(m[t][e], l[t][e]);
+          float* dst = c.part_o + (slot + row) * D + (lane >> 2);
+#pragma unroll
+          for (int n = 0; n < KB; ++n) { dst[n * 16] = o[t][n][e]; dst[n * 16 + 8] = o[t][n][2 + e]; }
+        }
       }
     }
     if (lane == 0) c.pieces[p.item] = workers;

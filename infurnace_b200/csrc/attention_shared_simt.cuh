@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_co
   ifb_pdl_trigger();
   make_plan(c, other, plan);
   Walk walk;
-  const int ctas = c.which == EVERY ? c.workers : wide_sms(c.workers, plan.starts[c.n_groups + c.n_req] * c.cost, plan.sums[31] * other.cost);
+  const int ctas = c.which == EVERY ? c.workers : wide_sms(c.workers, plan.starts[c.n_groups + c.n_req] * c.cost, plan.sums[63] * other.cost);
   walk.begin(c, plan, blockIdx.x, ctas);
   if (parts) write_parts(c, other, plan);
   const int tid = threadIdx.x, x = tid & 7, y = tid >> 3, quads = dim / 4;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_co
       }
       __syncwarp();
     }
-    const int2 workers = walk.item_workers(c, p);
+    const int2 workers = walk.item_workers(c, p, blockIdx.x);
     const bool sole = is_sole(p, workers);
     const long long slot = (long long)(p.item + blockIdx.x) * c.rows;
 #pragma unroll

@@ -102,7 +102,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   Walk walk;
-  walk.begin(c, plan, blockIdx.x, wide_sms(c.workers, plan.starts[c.n_groups + c.n_req] * c.cost, plan.sums[31] * other.cost));
+  walk.begin(c, plan, blockIdx.x, wide_sms(c.workers, plan.starts[c.n_groups + c.n_req] * c.cost, plan.sums[63] * other.cost));
   Piece p;
   if (parts) write_parts(c, other, plan);
 
@@ -354,7 +354,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       asm volatile("bar.sync 2, 256;\n" ::: "memory");          // the eight softmax warps, on every path
       tc_fence_after();
       const bool go = __all_sync(0xffffffffu, !*abort_flag) != 0;
-      const int2 workers = walk.item_workers(c, p);
+      const int2 workers = walk.item_workers(c, p, blockIdx.x);
       if (go && work) {
         const float m0 = merge_m[par][0][row], m1 = merge_m[par][1][row], l0 = merge_l[par][0][row], l1 = merge_l[par][1][row];
         const float m = fmaxf(m0, m1);
