@@ -75,6 +75,8 @@ __host__ inline void room_at(Call& c, int dim, void* room) {
   c.pieces = (int2*)((char*)c.part_ml + room_align(slots * c.rows * 8));
 }
 
+struct PageRows { int page, total; };      // the pool as a matrix of rows: rows of a page, rows in all
+
 __device__ __forceinline__ int clamp(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
 // What an owner's rows and keys are.

@@ -36,7 +36,7 @@ static Call wide_call(bool tc, int n_tokens, int n_req, int n_groups, int kv_hea
 IFB_EXPORT long long ifb_attention_shared_bf16_room(int n_tokens, int n_req, int n_groups, int kv_heads, int group) {
   const long long a = room_bytes(wide_call(true, n_tokens, n_req, n_groups, kv_heads, group, 16), D);
   const long long b = room_bytes(wide_call(false, n_tokens, n_req, n_groups, kv_heads, group, 16), D);
-  return parts_bytes(n_tokens) + (a > b ? a : b) + room_bytes(narrow::call(n_tokens, n_req, n_groups, kv_heads, group), D);
+  return parts_bytes(n_tokens) + (a > b ? a : b) + room_bytes(narrow::call(true, n_tokens, n_req, n_groups, kv_heads, group), D);      // (either has as many workers)
 }
 
 // As ifb_attention_shared.
@@ -52,7 +52,8 @@ IFB_EXPORT int ifb_attention_shared_bf16(const __nv_bfloat16* q, long long q_row
   if (window < 0 || !err || page_stride < 2LL * kv_heads * page_size * D) return IFB_ERR_ARG;
   const int group = heads / kv_heads;
   const bool tc = on_tc(page_size, n_req + n_groups, scale, page_stride, num_pages);
-  Call wide = wide_call(tc, n_tokens, n_req, n_groups, kv_heads, group, page_size), few = narrow::call(n_tokens, n_req, n_groups, kv_heads, group);
+  const bool by_tma = narrow::by_tma(page_size, page_stride, num_pages);
+  Call wide = wide_call(tc, n_tokens, n_req, n_groups, kv_heads, group, page_size), few = narrow::call(by_tma, n_tokens, n_req, n_groups, kv_heads, group);
   for (Call* c : {&wide, &few}) {
     c->block_tables = block_tables; c->cu_q = cu_q; c->seq_lens = seq_lens; c->cu_groups = cu_groups; c->shared_lens = shared_lens;
     c->bt_stride = bt_stride; c->num_pages = num_pages; c->page_stride = page_stride;
@@ -77,7 +78,7 @@ IFB_EXPORT int ifb_attention_shared_bf16(const __nv_bfloat16* q, long long q_row
     if (st) return st;
   }
   if (any_narrow) {
-    st = narrow::run(few, wide, q, q_row, pages, any_wide, stream);
+    st = narrow::run(by_tma, few, wide, q, q_row, pages, any_wide, stream);
     if (st) return st;
   }
   return join<__nv_bfloat16>(wide, few, D, stream);

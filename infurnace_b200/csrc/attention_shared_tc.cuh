@@ -48,7 +48,6 @@ __device__ __forceinline__ void weight_terms(float e0, float e1, uint32_t& first
 struct Bars {
   uint64_t q_full, q_empty, o_free, k_full[2], v_full[2], k_empty[2][2], v_empty[2][2], s_full[2][2], p_ready[2][2], o_done[2];
 };
-struct PageRows { int page, total; };      // the pool as a matrix of rows: rows of a page, rows in all
 
 __global__ void __launch_bounds__(THREADS, 1)
 shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
