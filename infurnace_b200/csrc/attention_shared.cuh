@@ -11,7 +11,7 @@
 // without it: the group has no rows then, and each request has all its keys, the shared ones through the first request's table ("split" below).
 // An owner of at most 16 score rows (rows times the heads of a key head's group) is narrow, the others are wide: narrow ones are worked on by warps,
 // sixteen rows each, wide ones by CTAs with larger tiles, in kernels of their own that run beside one another.
-// For either an owner's rows are cut into tiles of `tokens` query tokens (a narrow owner is one tile), its keys into units of `unit` keys; a tile of one key
+// For either an owner's rows are cut into tiles of `tokens` query tokens (a narrow owner is one tile), its keys into units; a tile of one key
 // head is an item.  All units of all items, and `extra` ones for an item's beginning and end, lie in one line, in the order of owner, tile, key
 // head and key, and worker c of n takes those from c U / n to (c + 1) U / n: every worker has the same number but for one, however uneven the requests.
 // A stretch of one item's units within a worker is a piece; its sums go to slot (item + c), which no two pieces share, for along the line
@@ -49,9 +49,9 @@ struct Call {
   int* err;
   // of one class's kernel
   int which;
-  int tokens, unit, rows;                // of a tile (rows = tokens x heads of a key head, at most), of a unit
+  int tokens, rows;                      // of a tile (rows = tokens x heads of a key head, at most)
+  int unit_log, align_log;               // keys of a unit; of which number an item's first key is a multiple: powers of two
   int extra;                             // units that an item's beginning and end cost
-  int align;                             // an item's first key is a multiple of this
   int workers;                           // at most
   int cost;                              // of a unit, to the other class's
   float* part_o;                         // [slots][rows][dim]
@@ -101,8 +101,8 @@ __device__ __forceinline__ Span tile_span(const Call& c, const Owner& w, int til
     if (c.window > 0) s.lo = max(s.lo, w.p_first() + t0 - c.window + 1);
     s.last = min(s.last, w.p_first() + t1);
   }
-  s.first = s.lo / c.align * c.align;
-  s.units = s.last > s.lo ? (s.last - s.first + c.unit - 1) / c.unit : 0;
+  s.first = s.lo >> c.align_log << c.align_log;
+  s.units = s.last > s.lo ? (s.last - s.first - 1 >> c.unit_log) + 1 : 0;
   return s;
 }
 __device__ __forceinline__ int span_cost(const Call& c, const Span& s) { return s.units ? s.units + c.extra : 0; }
@@ -293,8 +293,8 @@ struct Walk {
       p.tile = tile;
       p.kv_head = head;
       p.item = owner_item(c, w, o) + tile * c.kv_heads + head;
-      p.first = s.first + u0 * c.unit;
-      p.last = min(s.last, s.first + u1 * c.unit);
+      p.first = s.first + (u0 << c.unit_log);
+      p.last = min(s.last, s.first + (u1 << c.unit_log));
       p.lo = max(s.lo, p.first);
       p.row0 = w.row0 + tile * c.tokens;
       p.tokens = min(c.tokens, w.row1 - p.row0);
@@ -410,31 +410,37 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
       ml = (k ? ml_at[1] : ml_at[0])[i];
       src = (k ? o_at[1] : o_at[0]) + i * dim;
     }
+    const int turn = min(32, n - x0);
+    // eight pieces' sums are asked for at once, the first with the maxima
+    float4 v[2][8];
+    auto ask = [&](int t0) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const float* o = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, t0 + t & 31));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int col = j * 128 + lane * 4;
+          if (t0 + t < turn && col < dim) v[j][t] = *reinterpret_cast<const float4*>(o + col);
+        }
+      }
+    };
+    ask(0);
     const float next = fmaxf(m, warp_max(ml.y == 0.f ? -INFINITY : ml.x)), ref = next == -INFINITY ? 0.f : next;
     const float keep = exp2f(m - ref), f = ml.y == 0.f ? 0.f : exp2f(ml.x - ref);      // (a piece of which the row sees nothing has weight 0)
     m = next;
     den = fmaf(den, keep, warp_sum(f * ml.y));
 #pragma unroll
     for (int j = 0; j < 2; ++j) { acc[j].x *= keep; acc[j].y *= keep; acc[j].z *= keep; acc[j].w *= keep; }
-    const int turn = min(32, n - x0);
-    // eight pieces' sums are asked for at once
     for (int t0 = 0; t0 < turn; t0 += 8) {
+      if (t0) ask(t0);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int col = j * 128 + lane * 4;
-        if (j * 128 >= dim) break;
-        float4 v[8];
+      for (int t = 0; t < 8; ++t) {
+        const float g = __shfl_sync(0xffffffffu, f, t0 + t & 31);
+        if (g == 0.f || t0 + t >= turn) continue;      // (what has weight 0 may be infinite or NaN)
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          const float* o = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, t0 + t & 31));
-          v[t] = t0 + t < turn && col < dim ? *reinterpret_cast<const float4*>(o + col) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          const float g = __shfl_sync(0xffffffffu, f, t0 + t & 31);
-          if (g != 0.f && t0 + t < turn) {      // (what has weight 0 may be infinite or NaN)
-            acc[j].x = fmaf(g, v[t].x, acc[j].x); acc[j].y = fmaf(g, v[t].y, acc[j].y); acc[j].z = fmaf(g, v[t].z, acc[j].z); acc[j].w = fmaf(g, v[t].w, acc[j].w);
-          }
+        for (int j = 0; j < 2; ++j) {
+          acc[j].x = fmaf(g, v[j][t].x, acc[j].x); acc[j].y = fmaf(g, v[j][t].y, acc[j].y);
+          acc[j].z = fmaf(g, v[j][t].z, acc[j].z); acc[j].w = fmaf(g, v[j][t].w, acc[j].w);
         }
       }
     }

@@ -24,6 +24,7 @@ namespace narrow {
 typedef __nv_bfloat16 bf16;
 constexpr int WARPS = 4;
 constexpr int CHUNK = 16, UNIT = 32;
+static_assert(UNIT == 1 << 5 && CHUNK == 1 << 4, "unit_log, align_log");
 constexpr int STAGES = 3;
 constexpr int KB = D / 16;
 constexpr bool TMA_HEADS = D % 64 == 0;               // whole rows of 64 columns
@@ -101,6 +102,7 @@ shared_narrow_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
   unsigned char* stages = base + (size_t)warp * Room<TMA>::WARP;
   const Plan plan = plan_at(base + WARPS * Room<TMA>::WARP, c.n_groups + c.n_req);
   volatile int* abort_flag = &abort_words[warp];
+  if (TMA && threadIdx.x < 2) tc_prefetch_map(threadIdx.x ? &v_map : &k_map);
   if (lane == 0) {
     abort_words[warp] = 0;
     if (TMA) {
@@ -372,7 +374,7 @@ static inline Call call(bool tma, int n_tokens, int n_req, int n_groups, int kv_
   c.which = NARROW;
   c.n_tokens = n_tokens; c.n_req = n_req; c.n_groups = n_groups;
   c.kv_heads = kv_heads; c.heads = kv_heads * group;
-  c.tokens = group <= NARROW_ROWS ? NARROW_ROWS / group : 1; c.unit = UNIT; c.rows = NARROW_ROWS; c.align = tma ? CHUNK : 1;
+  c.tokens = group <= NARROW_ROWS ? NARROW_ROWS / group : 1; c.rows = NARROW_ROWS; c.unit_log = 5; c.align_log = tma ? 4 : 0;
   c.workers = ifb_sm_count() * (tma ? Room<true>::CTAS : Room<false>::CTAS) * WARPS;
   c.cost = 1;
   c.extra = 1;

@@ -10,6 +10,7 @@
 using namespace shared_attention;
 
 constexpr int SH_ROWS = 64, SH_UNIT = 32, SH_THREADS = 256;
+static_assert(SH_UNIT == 1 << 5, "unit_log");
 
 template <typename T>
 __device__ __forceinline__ void sh_row4(float* dst, const T* src, bool valid) {      // four numbers
@@ -175,7 +176,7 @@ static inline Call sh_call(int n_tokens, int n_req, int n_groups, int kv_heads, 
   c.which = which;
   c.n_tokens = n_tokens; c.n_req = n_req; c.n_groups = n_groups;
   c.kv_heads = kv_heads; c.heads = kv_heads * group;
-  c.tokens = SH_ROWS / group; c.unit = SH_UNIT; c.rows = SH_ROWS; c.align = 1;
+  c.tokens = SH_ROWS / group; c.rows = SH_ROWS; c.unit_log = 5; c.align_log = 0;
   c.workers = ifb_sm_count();
   c.cost = 16;
   c.extra = 1;

@@ -24,6 +24,7 @@ typedef __nv_bfloat16 bf16;
 constexpr int DH = (D + 63) / 64;                // swizzle rows of 64 columns that a row has
 constexpr int DN = DH * 64;                      // columns of the output accumulator
 constexpr int ROWS = 128, UNIT = 128, SUB = 64;
+static_assert(UNIT == 1 << 7, "unit_log");
 constexpr int THREADS = 384;
 constexpr int HALF_BYTES = 128 * 128;            // [128 rows][64 columns] in the 128-byte swizzle
 constexpr int TILE_BYTES = DH * HALF_BYTES;
@@ -67,6 +68,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int G = c.heads / c.kv_heads;
 
+  if (threadIdx.x < 3) tc_prefetch_map(threadIdx.x == 0 ? &q_map : threadIdx.x == 1 ? &k_map : &v_map);
   if (c.tokens * G < ROWS) {      // rows of the tile that no query fills: zeros, once
     for (int i = threadIdx.x; i < TILE_BYTES / 16; i += THREADS) reinterpret_cast<uint4*>(Qs)[i] = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -429,9 +431,9 @@ static inline Call tc_call(int n_tokens, int n_req, int n_groups, int kv_heads, 
   c.which = WIDE;
   c.n_tokens = n_tokens; c.n_req = n_req; c.n_groups = n_groups;
   c.kv_heads = kv_heads; c.heads = kv_heads * group;
-  c.tokens = ROWS / group; c.unit = UNIT; c.rows = ROWS; c.align = page_size;
+  c.tokens = ROWS / group; c.rows = ROWS; c.unit_log = 7; c.align_log = page_size == 16 ? 4 : page_size == 32 ? 5 : 6;
   c.workers = ifb_sm_count();
-  c.cost = 8;
+  c.cost = 7;
   c.extra = 2;
   return c;
 }

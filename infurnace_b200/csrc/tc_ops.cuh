@@ -41,6 +41,8 @@ __device__ __forceinline__ void tc_tma_3d(void* smem, const CUtensorMap* map, ui
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
                ::"r"(tc_smem_u32(smem)), "l"(map), "r"(tc_smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
 }
+// The description of a tensor, on its way to where copies look it up (a kernel's first copy waits for it otherwise).
+__device__ __forceinline__ void tc_prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory"); }
 // True in exactly one lane of a converged warp.  Code under it is known to the compiler as single-threaded, which lets
 // it keep the descriptors of the copies and products it issues in uniform registers.
 __device__ __forceinline__ bool tc_elect_one() {
