@@ -26,7 +26,8 @@
 
 namespace shared_attention {
 
-constexpr int MAX_OWNERS = 2048;      // groups and requests of a call
+constexpr int MAX_OWNERS = 2048;      // groups and requests of a call (512 for heads over 128, whose tiles leave less room beside them)
+constexpr size_t MOST_SMEM = 224 * 1024;      // of a kernel, beside what it declares
 constexpr int NO_POSITION = -1;
 enum Class { EVERY, WIDE, NARROW };   // whose owners a kernel works on
 constexpr int NARROW_ROWS = 16;
@@ -367,10 +368,10 @@ __device__ inline void write_parts(const Call& wide, const Call& narrow, const P
 }
 
 // ---------------------------------------------------------------------------------------------------- the join
-// A warp takes a head of a token; a lane has the columns from 4 lane and 128 + 4 lane on.  `wide` and `narrow`: the classes' calls (the same one where
+// A warp takes a head of a token; a lane has the columns from 4 lane on (WIDTH 2, heads over 128: and from 128 + 4 lane on).  `wide` and `narrow`: the classes' calls (the same one where
 // there is one kernel only).  Lane x first has piece x: its maximum and denominator, from which the factor that its sums get.
 constexpr int JOIN_WARPS = 8;
-template <typename T>
+template <typename T, int WIDTH>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ Call wide, const __grid_constant__ Call narrow, int dim) {
   ifb_pdl_wait();
   ifb_pdl_trigger();
@@ -399,7 +400,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
   const int n = max(0, count[0]) + max(0, count[1]);
   // in turns of 32 pieces, against a running maximum
   float m = -INFINITY, den = 0.f;
-  float4 acc[2] = {};
+  float4 acc[WIDTH] = {};
+  constexpr int ASK = 16 / WIDTH;      // pieces whose sums are asked for at once, the first with the maxima
   for (int x0 = 0; x0 < n; x0 += 32) {
     const int x = x0 + lane;
     const bool k = x >= count[0];
@@ -411,14 +413,13 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
       src = (k ? o_at[1] : o_at[0]) + i * dim;
     }
     const int turn = min(32, n - x0);
-    // eight pieces' sums are asked for at once, the first with the maxima
-    float4 v[2][8];
+    float4 v[WIDTH][ASK];
     auto ask = [&](int t0) {
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
+      for (int t = 0; t < ASK; ++t) {
         const float* o = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, t0 + t & 31));
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < WIDTH; ++j) {
           const int col = j * 128 + lane * 4;
           if (t0 + t < turn && col < dim) v[j][t] = *reinterpret_cast<const float4*>(o + col);
         }
@@ -430,15 +431,15 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
     m = next;
     den = fmaf(den, keep, warp_sum(f * ml.y));
 #pragma unroll
-    for (int j = 0; j < 2; ++j) { acc[j].x *= keep; acc[j].y *= keep; acc[j].z *= keep; acc[j].w *= keep; }
-    for (int t0 = 0; t0 < turn; t0 += 8) {
+    for (int j = 0; j < WIDTH; ++j) { acc[j].x *= keep; acc[j].y *= keep; acc[j].z *= keep; acc[j].w *= keep; }
+    for (int t0 = 0; t0 < turn; t0 += ASK) {
       if (t0) ask(t0);
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
+      for (int t = 0; t < ASK; ++t) {
         const float g = __shfl_sync(0xffffffffu, f, t0 + t & 31);
         if (g == 0.f || t0 + t >= turn) continue;      // (what has weight 0 may be infinite or NaN)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < WIDTH; ++j) {
           acc[j].x = fmaf(g, v[j][t].x, acc[j].x); acc[j].y = fmaf(g, v[j][t].y, acc[j].y);
           acc[j].z = fmaf(g, v[j][t].z, acc[j].z); acc[j].w = fmaf(g, v[j][t].w, acc[j].w);
         }
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
   const float inv = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den;      // (NaN stays)
   T* dst = reinterpret_cast<T*>(wide.out) + ((long long)token * wide.heads + head) * dim;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < WIDTH; ++j) {
     const int col = j * 128 + lane * 4;
     if (col < dim) {
       dst[col] = from_f32<T>(acc[j].x * inv); dst[col + 1] = from_f32<T>(acc[j].y * inv);
@@ -458,7 +459,39 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
 }
 
 template <typename T> static int join(const Call& wide, const Call& narrow, int dim, cudaStream_t stream) {
-  return ifb_launch(join_kernel<T>, dim3(wide.n_tokens, (wide.heads + JOIN_WARPS - 1) / JOIN_WARPS), dim3(JOIN_WARPS * 32), 0, stream, wide, narrow, dim);
+  const dim3 grid(wide.n_tokens, (wide.heads + JOIN_WARPS - 1) / JOIN_WARPS), block(JOIN_WARPS * 32);
+  return dim <= 128 ? ifb_launch(join_kernel<T, 1>, grid, block, 0, stream, wide, narrow, dim) : ifb_launch(join_kernel<T, 2>, grid, block, 0, stream, wide, narrow, dim);
+}
+
+// A call as the caller packs it: 8-byte fields first.
+struct Packed {
+  const void *q, *pages;
+  const int *block_tables, *cu_q, *seq_lens, *cu_groups, *shared_lens;
+  void *out, *room;
+  int* err;
+  cudaStream_t stream;
+  long long q_row, page_stride, num_pages, bt_stride;
+  double scale;
+  int table_pages, n_tokens, n_req, n_groups, heads, kv_heads, dim, page_size, window, spare;
+};
+// What either class's call has from it.
+static inline void fill(Call& c, const Packed& a) {
+  c.block_tables = a.block_tables; c.cu_q = a.cu_q; c.seq_lens = a.seq_lens; c.cu_groups = a.cu_groups; c.shared_lens = a.shared_lens;
+  c.bt_stride = a.bt_stride; c.num_pages = a.num_pages; c.page_stride = a.page_stride;
+  c.table_pages = a.table_pages; c.page_size = a.page_size; c.window = a.window;
+  c.scale_log2 = (float)(a.scale * 1.4426950408889634);
+  c.out = a.out;
+  c.parts = (int4*)a.room;
+  c.err = a.err;
+}
+// The checks that do not depend on the type; `least`: elements of 16 bytes.
+static inline int check(const Packed& a, int most_group, int least) {
+  if (a.kv_heads < 1 || a.heads % a.kv_heads || a.heads / a.kv_heads > most_group || a.dim < 16 || a.dim > 256 || a.dim % 16 || a.n_groups < 0 ||
+      a.n_req + a.n_groups > MAX_OWNERS || a.page_size < 1 || a.num_pages < 1)
+    return IFB_ERR_SIZE;
+  if ((((uintptr_t)a.q | (uintptr_t)a.pages) & 15) || a.q_row % least || a.page_stride % least || ((uintptr_t)a.room & 255)) return IFB_ERR_ALIGN;
+  if (a.window < 0 || !a.err || !a.room || a.page_stride < 2LL * a.kv_heads * a.page_size * a.dim) return IFB_ERR_ARG;
+  return IFB_OK;
 }
 
 }  // namespace shared_attention

@@ -40,46 +40,36 @@ IFB_EXPORT long long ifb_attention_shared_bf16_room(int n_tokens, int n_req, int
 }
 
 // As ifb_attention_shared.
-IFB_EXPORT int ifb_attention_shared_bf16(const __nv_bfloat16* q, long long q_row, const __nv_bfloat16* pages, long long page_stride, long long num_pages,
-                                         const int* block_tables, long long bt_stride, int table_pages, const int* cu_q, const int* seq_lens,
-                                         const int* cu_groups, const int* shared_lens, __nv_bfloat16* out, void* room, int* err, int n_tokens, int n_req,
-                                         int n_groups, int heads, int kv_heads, int dim, int page_size, float scale, int window, cudaStream_t stream) {
-  if (n_tokens <= 0 || n_req <= 0) return IFB_OK;
-  if (dim != D || kv_heads < 1 || heads % kv_heads || heads / kv_heads > SH_ROWS || n_groups < 0 || n_req + n_groups > MAX_OWNERS || page_size < 1 ||
-      num_pages < 1)
-    return IFB_ERR_SIZE;
-  if ((((uintptr_t)q | (uintptr_t)pages) & 15) || q_row % 8 || page_stride % 8 || ((uintptr_t)room & 255)) return IFB_ERR_ALIGN;
-  if (window < 0 || !err || page_stride < 2LL * kv_heads * page_size * D) return IFB_ERR_ARG;
-  const int group = heads / kv_heads;
-  const bool tc = on_tc(page_size, n_req + n_groups, scale, page_stride, num_pages);
-  const bool by_tma = narrow::by_tma(page_size, page_stride, num_pages);
-  Call wide = wide_call(tc, n_tokens, n_req, n_groups, kv_heads, group, page_size), few = narrow::call(by_tma, n_tokens, n_req, n_groups, kv_heads, group);
-  for (Call* c : {&wide, &few}) {
-    c->block_tables = block_tables; c->cu_q = cu_q; c->seq_lens = seq_lens; c->cu_groups = cu_groups; c->shared_lens = shared_lens;
-    c->bt_stride = bt_stride; c->num_pages = num_pages; c->page_stride = page_stride;
-    c->table_pages = table_pages; c->page_size = page_size; c->window = window;
-    c->scale_log2 = scale * 1.4426950408889634f;
-    c->err = err;
-    c->out = out;
-    c->parts = (int4*)room;
-  }
-  char* rest = (char*)room + parts_bytes(n_tokens);
+IFB_EXPORT int ifb_attention_shared_bf16(const Packed* call) {
+  const Packed& a = *call;
+  if (a.n_tokens <= 0 || a.n_req <= 0) return IFB_OK;
+  if (a.dim != D) return IFB_ERR_SIZE;
+  if (const int st = check(a, SH_ROWS, 8)) return st;
+  const __nv_bfloat16 *q = (const __nv_bfloat16*)a.q, *pages = (const __nv_bfloat16*)a.pages;
+  const int group = a.heads / a.kv_heads;
+  const bool tc = on_tc(a.page_size, a.n_req + a.n_groups, (float)a.scale, a.page_stride, a.num_pages);
+  const bool by_tma = narrow::by_tma(a.page_size, a.page_stride, a.num_pages);
+  Call wide = wide_call(tc, a.n_tokens, a.n_req, a.n_groups, a.kv_heads, group, a.page_size);
+  Call few = narrow::call(by_tma, a.n_tokens, a.n_req, a.n_groups, a.kv_heads, group);
+  fill(wide, a);
+  fill(few, a);
+  char* rest = (char*)a.room + parts_bytes(a.n_tokens);
   room_at(wide, D, rest);
   room_at(few, D, rest + room_bytes(wide, D));
-  const bool any_wide = (long long)n_tokens * group > NARROW_ROWS;      // no owner has more rows than all
+  const bool any_wide = (long long)a.n_tokens * group > NARROW_ROWS;      // no owner has more rows than all
   const bool any_narrow = group <= NARROW_ROWS;
   int st = IFB_OK;
   if (any_wide) {
 #if HEAD_DIM <= 128
-    if (tc) st = tc_main(wide, few, q, q_row, pages, !any_narrow, stream);
+    if (tc) st = tc_main(wide, few, q, a.q_row, pages, !any_narrow, a.stream);
     else
 #endif
-      st = sh_main<__nv_bfloat16, (D <= 64 ? 8 : D <= 128 ? 16 : 32)>(wide, few, q, q_row, pages, D, !any_narrow, stream);
+      st = sh_main<__nv_bfloat16, (D <= 64 ? 8 : D <= 128 ? 16 : 32)>(wide, few, q, a.q_row, pages, D, !any_narrow, a.stream);
     if (st) return st;
   }
   if (any_narrow) {
-    st = narrow::run(by_tma, few, wide, q, q_row, pages, any_wide, stream);
+    st = narrow::run(by_tma, few, wide, q, a.q_row, pages, any_wide, a.stream);
     if (st) return st;
   }
-  return join<__nv_bfloat16>(wide, few, D, stream);
+  return join<__nv_bfloat16>(wide, few, D, a.stream);
 }

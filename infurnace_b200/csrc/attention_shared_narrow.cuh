@@ -384,6 +384,7 @@ template <bool TMA>
 static int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, PageRows rows, const Call& c, const Call& other, const bf16* q, long long q_row,
                   const bf16* pages, bool beside, cudaStream_t stream) {
   const size_t smem = 1024 + plan_bytes(c.n_req + c.n_groups) + WARPS * Room<TMA>::WARP;
+  if (smem > MOST_SMEM) return IFB_ERR_SIZE;
   IFB_ALLOW_SMEM(shared_narrow_kernel<TMA>, smem);
   return ifb_launch(shared_narrow_kernel<TMA>, dim3(c.workers / WARPS), dim3(WARPS * 32), smem, stream, k_map, v_map, rows, c, other, q, q_row, pages,
                     ifb_sm_count(), beside ? 1 : 0);

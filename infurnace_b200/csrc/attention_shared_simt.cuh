@@ -186,6 +186,7 @@ static inline Call sh_call(int n_tokens, int n_req, int n_groups, int kv_heads, 
 template <typename T, int DC>
 static int sh_main(const Call& c, const Call& other, const T* q, long long q_row, const T* pages, int dim, bool parts, cudaStream_t stream) {
   const size_t smem = plan_bytes(c.n_req + c.n_groups) + (size_t)((SH_ROWS + 2 * SH_UNIT) * (dim + 4) + SH_ROWS * 33) * 4;
+  if (smem > MOST_SMEM) return IFB_ERR_SIZE;
   IFB_ALLOW_SMEM((shared_simt_kernel<T, DC>), smem);
   return ifb_launch(shared_simt_kernel<T, DC>, dim3(c.workers), dim3(SH_THREADS), smem, stream, c, other, q, q_row, pages, dim, parts ? 1 : 0);
 }

@@ -664,11 +664,22 @@ static int cut_clusters(const void* kernel, int dtype, int ctas, size_t smem) {
 // logits [rows, vocab] with rows `pitch` elements apart (dtype IFB_F32 or IFB_BF16); per row: temperature, uniform number, and top_k, top_p, min_p (each or
 // null); out int32, logprobs float32 or null.
 IFB_EXPORT int ifb_sample_cut_max_vocab() { return SURE_CLUSTER * SLICE; }
-IFB_EXPORT int ifb_sample_cut(const void* logits, int dtype, long long pitch, int rows, int vocab, const float* temperature, const float* uniform,
-                              const int* top_k, const float* top_p, const float* min_p, int* out, float* logprobs, cudaStream_t stream) {
+struct CutPacked {      // a call as the caller packs it: 8-byte fields first
+  const void* logits;
+  const float *temperature, *uniform;
+  const int* top_k;
+  const float *top_p, *min_p;
+  int* out;
+  float* logprobs;
+  cudaStream_t stream;
+  long long pitch;
+  int dtype, rows, vocab, spare;
+};
+IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
+  const int dtype = call->dtype, rows = call->rows, vocab = call->vocab;
   if (rows <= 0) return IFB_OK;
   if (vocab < 1 || vocab > SURE_CLUSTER * SLICE || rows > (1 << 27)) return IFB_ERR_SIZE;
-  if (!temperature || !uniform || !out) return IFB_ERR_ARG;
+  if (!call->temperature || !call->uniform || !call->out) return IFB_ERR_ARG;
   // As few CTAs of a row as let two share an SM; more while all rows' clusters find their SMs at once.
   const void* kernel = dtype == IFB_F32 ? (const void*)sample_cut_kernel<float> : dtype == IFB_BF16 ? (const void*)sample_cut_kernel<bf16> : nullptr;
   if (!kernel) return IFB_ERR_DTYPE;
@@ -681,7 +692,7 @@ IFB_EXPORT int ifb_sample_cut(const void* logits, int dtype, long long pitch, in
     if (rows > clusters) break;
     ctas *= 2;
   }
-  CutArgs a = {pitch, vocab, slice(ctas), temperature, top_k, top_p, min_p, uniform, out, logprobs};
+  CutArgs a = {call->pitch, vocab, slice(ctas), call->temperature, call->top_k, call->top_p, call->min_p, call->uniform, call->out, call->logprobs};
   const size_t smem = (size_t)a.per * 4 + CUT_BYTES;
   auto go = [&](auto kernel, auto typed) -> int {
     IFB_ALLOW_SMEM(kernel, smem);
@@ -689,7 +700,7 @@ IFB_EXPORT int ifb_sample_cut(const void* logits, int dtype, long long pitch, in
     cfg.gridDim = dim3((unsigned)rows * ctas);
     cfg.blockDim = dim3(NT);
     cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
+    cfg.stream = call->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = ctas;
@@ -703,8 +714,8 @@ IFB_EXPORT int ifb_sample_cut(const void* logits, int dtype, long long pitch, in
     if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
     return IFB_OK;
   };
-  if (dtype == IFB_F32) return go(sample_cut_kernel<float>, (const float*)logits);
-  if (dtype == IFB_BF16) return go(sample_cut_kernel<bf16>, (const bf16*)logits);
+  if (dtype == IFB_F32) return go(sample_cut_kernel<float>, (const float*)call->logits);
+  if (dtype == IFB_BF16) return go(sample_cut_kernel<bf16>, (const bf16*)call->logits);
   return IFB_ERR_DTYPE;
 }
 

@@ -6,7 +6,9 @@ attention is cut into pieces at the head of ``csrc/attention_shared.cuh``.
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_char_p, c_int, c_longlong, c_void_p
+
+import struct
 
 import torch
 
@@ -29,25 +31,30 @@ def _status(status, what):
 def _logit_rows(logits, what):
     """(dtype code, rows, vocabulary, elements between rows, device) of a call's logits."""
     code = _CODES.get(logits.dtype)
-    shape = logits.shape
-    if code is None or len(shape) != 2 or shape[1] < 1 or (shape[1] > 1 and logits.stride(1) != 1):
+    shape, pitch, index = logits.shape, logits.stride(), logits.get_device()
+    if code is None or len(shape) != 2 or shape[1] < 1 or (pitch[1] != 1 and shape[1] > 1):
         raise KernelError(f"{what}: logits are float32 or bfloat16 [rows, vocabulary] with unit stride along the vocabulary; got {logits.dtype} "
-                          f"{tuple(shape)} of strides {logits.stride()}")
-    index = logits.get_device()
+                          f"{tuple(shape)} of strides {pitch}")
     if index < 0:
         raise KernelError(f"{what}: logits are not on a CUDA device")
     rows, vocab = shape
-    pitch = logits.stride(0) if rows > 1 else vocab          # (one row's pitch leads nowhere)
-    return code, rows, vocab, pitch, index
+    return code, rows, vocab, pitch[0] if rows > 1 else vocab, index          # (one row's pitch leads nowhere)
 
 
-def _one_per_row(t, dtype, rows, index, what, name, optional=False):
-    """The address of a tensor with one number for each row (0: absent)."""
-    if t is None and optional:
-        return 0
-    if t.dtype != dtype or t.shape != (rows,) or (rows > 1 and t.stride(0) != 1) or t.get_device() != index:
+def _one_per_row(t, dtype, rows, index, what, name):
+    """The address of a tensor with one number for each row."""
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() != rows or not t.is_contiguous() or t.get_device() != index:
         raise KernelError(f"{what}: {name} is {dtype} [{rows}], contiguous, on the logits' device; got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
+
+
+def _device_of(index):
+    """The device that calls launch on, for the time of a call; None: it is the current one."""
+    return None if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+
+
+_CUT_CALL = struct.Struct("=10q4i").pack            # csrc/sampling.cu: CutPacked
+_SHARED_CALL = struct.Struct("=15qd10i").pack       # csrc/attention_shared.cuh: Packed
 
 
 class AnswerKernels:
@@ -58,7 +65,7 @@ class AnswerKernels:
     def _sampling_lib(self):
         if self._sampling is None:
             lib = load_library("sampling", progress=self._progress)
-            lib.ifb_sample_cut.argtypes = [c_void_p, c_int, c_longlong, c_int, c_int] + [c_void_p] * 8
+            lib.ifb_sample_cut.argtypes = [c_char_p]
             lib.ifb_token_logprobs.argtypes = [c_void_p, c_int, c_longlong, c_int, c_int] + [c_void_p] * 4
             self._sampling_max_vocab = int(lib.ifb_sample_cut_max_vocab())
             self._sampling = lib
@@ -74,22 +81,30 @@ class AnswerKernels:
         Among equal logits the lower index is the better; the draw is by inverse CDF in the order of indices.  NaN counts as -inf,
         which is never drawn; of infinities each is as likely as the other.  A row without a number above -inf gives token 0 and NaN.  A
         row's token depends on that row alone, and on its weights to 2^-44 of the largest."""
-        code, rows, vocab, pitch, index = _logit_rows(logits, "sample_filtered")
-        args = (_one_per_row(temperature, torch.float32, rows, index, "sample_filtered", "temperature"),
-                _one_per_row(uniform, torch.float32, rows, index, "sample_filtered", "uniform"),
-                _one_per_row(top_k, torch.int32, rows, index, "sample_filtered", "top_k", True),
-                _one_per_row(top_p, torch.float32, rows, index, "sample_filtered", "top_p", True),
-                _one_per_row(min_p, torch.float32, rows, index, "sample_filtered", "min_p", True),
-                _one_per_row(out, torch.int32, rows, index, "sample_filtered", "out"),
-                _one_per_row(logprobs, torch.float32, rows, index, "sample_filtered", "logprobs", True))
-        lib = self._sampling_lib()
+        what, f32 = "sample_filtered", torch.float32
+        code, rows, vocab, pitch, index = _logit_rows(logits, what)
+        args = (logits.data_ptr(), _one_per_row(temperature, f32, rows, index, what, "temperature"),
+                _one_per_row(uniform, f32, rows, index, what, "uniform"),
+                0 if top_k is None else _one_per_row(top_k, torch.int32, rows, index, what, "top_k"),
+                0 if top_p is None else _one_per_row(top_p, f32, rows, index, what, "top_p"),
+                0 if min_p is None else _one_per_row(min_p, f32, rows, index, what, "min_p"),
+                _one_per_row(out, torch.int32, rows, index, what, "out"),
+                0 if logprobs is None else _one_per_row(logprobs, f32, rows, index, what, "logprobs"))
+        lib = self._sampling or self._sampling_lib()
         if vocab > self._sampling_max_vocab:
             raise KernelError(f"sample_filtered: a vocabulary of {vocab}; at most {self._sampling_max_vocab}")
         if rows == 0:
             return out
-        with torch.cuda.device(index):
-            self.launches += 1
-            _status(lib.ifb_sample_cut(logits.data_ptr(), code, pitch, rows, vocab, *args, _raw_stream(index)), "sample_filtered")
+        self.launches += 1
+        call = _CUT_CALL(*args, _raw_stream(index), pitch, code, rows, vocab, 0)
+        other = _device_of(index)
+        if other is None:
+            status = lib.ifb_sample_cut(call)
+        else:
+            with other:
+                status = lib.ifb_sample_cut(call)
+        if status:
+            _status(status, what)
         return out
 
     def token_logprobs(self, logits, tokens, out, ranks=None):
@@ -97,18 +112,29 @@ class AnswerKernels:
         falling logit, equal ones by rising index, into ``ranks`` (int32).  ``logits`` float32 or bfloat16 [rows, vocabulary], rows may
         lie apart; ``tokens`` int32, one a row.  A token outside the vocabulary (padding) gives NaN and -1; a row with a NaN
         or +inf, or with no number above -inf, NaN."""
-        code, rows, vocab, pitch, index = _logit_rows(logits, "token_logprobs")
-        args = (_one_per_row(tokens, torch.int32, rows, index, "token_logprobs", "tokens"),
-                _one_per_row(out, torch.float32, rows, index, "token_logprobs", "out"),
-                _one_per_row(ranks, torch.int32, rows, index, "token_logprobs", "ranks", True))
+        what = "token_logprobs"
+        code, rows, vocab, pitch, index = _logit_rows(logits, what)
+        args = (_one_per_row(tokens, torch.int32, rows, index, what, "tokens"), _one_per_row(out, torch.float32, rows, index, what, "out"),
+                0 if ranks is None else _one_per_row(ranks, torch.int32, rows, index, what, "ranks"), _raw_stream(index))
         if rows == 0:
             return out
-        with torch.cuda.device(index):
-            self.launches += 1
-            _status(self._sampling_lib().ifb_token_logprobs(logits.data_ptr(), code, pitch, rows, vocab, *args, _raw_stream(index)), "token_logprobs")
+        self.launches += 1
+        call = (self._sampling or self._sampling_lib()).ifb_token_logprobs
+        other = _device_of(index)
+        if other is None:
+            status = call(logits.data_ptr(), code, pitch, rows, vocab, *args)
+        else:
+            with other:
+                status = call(logits.data_ptr(), code, pitch, rows, vocab, *args)
+        if status:
+            _status(status, what)
         return out
 
     # ------------------------------------------------------------------ attention over shared pages
+    @property
+    def _shared_sizes(self):
+        return self.__dict__.setdefault("_shared_sizes_held", {})
+
     def _shared_lib(self, dtype, dim):
         """(call, size of its room) for a type and head size."""
         libs = self.__dict__.setdefault("_shared", {})
@@ -120,8 +146,7 @@ class AnswerKernels:
             else:
                 lib = load_library("attention_shared_bf16", {"HEAD_DIM": dim}, progress=self._progress)
                 call, room = lib.ifb_attention_shared_bf16, lib.ifb_attention_shared_bf16_room
-            call.argtypes = [c_void_p, c_longlong, c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_int] + [c_void_p] * 7 + [c_int] * 7 + [
-                c_float, c_int, c_void_p]
+            call.argtypes = [c_char_p]
             room.argtypes, room.restype = [c_int] * (6 if dtype == torch.float32 else 5), c_longlong
             held = libs[(dtype, dim)] = (call, room)
         return held
@@ -148,55 +173,70 @@ class AnswerKernels:
 
         ``room``: None, or a uint8 tensor of at least ``shared_prefix_room`` bytes for the pieces' sums, in place of memory of the allocator's (within
         a recording: of the graph's own pool); calls that share one follow one another."""
-        code = _CODES.get(q.dtype)
-        shape, index = q.shape, q.get_device()
+        dtype, shape, pitch, index = q.dtype, q.shape, q.stride(), q.get_device()
+        pool, block = kv_pages.shape, kv_pages.stride()
         n, heads, dim = shape if len(shape) == 3 else (0, 0, 0)
-        pool = kv_pages.shape
-        if code is None or out.dtype != q.dtype or out.shape != shape or kv_pages.dtype != q.dtype or len(pool) != 5 or pool[1] != 2 \
-                or pool[4] != dim or pool[2] < 1 or heads % pool[2] or heads == 0:
+        if dtype not in _CODES or out.dtype is not dtype or out.shape != shape or kv_pages.dtype is not dtype or len(pool) != 5 or pool[1] != 2 \
+                or pool[4] != dim or pool[0] < 1 or pool[2] < 1 or pool[3] < 1 or heads % pool[2] or heads == 0:
             raise KernelError(f"shared_prefix_attention: q and out are bfloat16 or float32 [tokens, heads, head_dim] and kv_pages [pages, 2, kv_heads, page_size, "
-                              f"head_dim] of one type, heads a multiple of kv_heads; got {q.dtype} {tuple(shape)}, {out.dtype} {tuple(out.shape)} and "
+                              f"head_dim] of one type, heads a multiple of kv_heads; got {dtype} {tuple(shape)}, {out.dtype} {tuple(out.shape)} and "
                               f"{kv_pages.dtype} {tuple(pool)}")
         pages, _, kv_heads, page_size, _ = pool
         group = heads // kv_heads
         if dim % 16 or not 16 <= dim <= 256 or group > 64:
             raise KernelError(f"shared_prefix_attention: head_dim is a multiple of 16 up to 256, with up to 64 query heads for a key head; got {dim} and {group}")
-        if q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim) or not out.is_contiguous():
+        if pitch[2] != 1 or (heads > 1 and pitch[1] != dim) or not out.is_contiguous():
             raise KernelError("shared_prefix_attention: the heads of a query lie one after the other, and out is contiguous")
-        block = 2 * kv_heads * page_size * dim
-        page_stride = kv_pages.stride(0) if pages > 1 else block
-        if pages < 1 or not kv_pages[0].is_contiguous() or page_stride < block:
+        inner = page_size * dim
+        page_stride = block[0] if pages > 1 else 2 * kv_heads * inner
+        if block[4] != 1 or (page_size > 1 and block[3] != dim) or (kv_heads > 1 and block[2] != inner) or block[1] != kv_heads * inner \
+                or page_stride < 2 * kv_heads * inner:
             raise KernelError("shared_prefix_attention: the numbers of a page lie one after the other")
         r, groups = seq_lens.numel(), shared_lens.numel()
-        table = block_tables.shape
-        for t, name, count in ((cu_q, "cu_q", r + 1), (seq_lens, "seq_lens", r), (cu_groups, "cu_groups", groups + 1), (shared_lens, "shared_lens", groups)):
-            if t.dtype != torch.int32 or t.shape != (count,) or not t.is_contiguous():
-                raise KernelError(f"shared_prefix_attention: {name} is int32 [{count}], contiguous; got {t.dtype} {tuple(t.shape)}")
-        if block_tables.dtype != torch.int32 or len(table) != 2 or table[0] < r or (table[1] > 1 and block_tables.stride(1) != 1):
+        for t, count in ((cu_q, r + 1), (seq_lens, r), (cu_groups, groups + 1), (shared_lens, groups)):
+            if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != count or not t.is_contiguous() or t.get_device() != index:
+                raise KernelError(f"shared_prefix_attention: cu_q [requests + 1], seq_lens [requests], cu_groups [groups + 1] and shared_lens [groups] are int32, "
+                                  f"contiguous, on q's device; got {t.dtype} {tuple(t.shape)} on {t.device} for {count}")
+        table, table_pitch = block_tables.shape, block_tables.stride()
+        if block_tables.dtype is not torch.int32 or len(table) != 2 or table[0] < r or (table[1] > 1 and table_pitch[1] != 1):
             raise KernelError("shared_prefix_attention: block_tables is int32 [requests, pages] with unit stride along pages")
-        if index < 0 or any(t.get_device() != index for t in (kv_pages, out, block_tables, cu_q, seq_lens, cu_groups, shared_lens)):
+        if index < 0 or kv_pages.get_device() != index or out.get_device() != index or block_tables.get_device() != index:
             raise KernelError("shared_prefix_attention: all tensors are on one CUDA device")
+        q_row = pitch[0] if n > 1 else heads * dim
+        lines = 4 if dtype is torch.float32 else 8          # elements of 16 bytes
+        if q.data_ptr() % 16 or kv_pages.data_ptr() % 16 or q_row % lines or page_stride % lines:
+            raise KernelError("shared_prefix_attention: q's rows and the pages begin on 16 bytes")
         if window < 0 or max_q_len < 1 or max_seq_len < 0:
             raise KernelError("shared_prefix_attention: window and max_seq_len are not negative, max_q_len is positive")
         if table[1] * page_size < max_seq_len:
             raise KernelError(f"shared_prefix_attention: block tables of {table[1]} pages do not hold {max_seq_len} keys")
-        if r + groups > 2048:
-            raise KernelError(f"shared_prefix_attention: {r} requests and {groups} groups; at most 2,048 together")
+        if r + groups > (2048 if dim <= 128 else 512):
+            raise KernelError(f"shared_prefix_attention: {r} requests and {groups} groups; at most 2,048 together (512 for heads over 128)")
         if n == 0 or r == 0:
             return out
-        q_row = q.stride(0) if n > 1 else heads * dim
-        with torch.cuda.device(index):
-            call, room_of = self._shared_lib(q.dtype, dim)
-            size = room_of(n, r, groups, kv_heads, group, dim) if q.dtype == torch.float32 else room_of(n, r, groups, kv_heads, group)
-            if room is None:
-                room = torch.empty(size, dtype=torch.uint8, device=q.device)
-            elif room.dtype != torch.uint8 or room.dim() != 1 or not room.is_contiguous() or room.numel() < size or room.data_ptr() % 256 \
-                    or room.get_device() != index:
-                raise KernelError(f"shared_prefix_attention: a room is uint8 [{size} or more], contiguous, on 256 bytes, on the same device")
-            self.launches += 2 if q.dtype == torch.float32 or group > 16 or n * group <= 16 else 3
-            self._err_armed = True
-            status = call(q.data_ptr(), q_row, kv_pages.data_ptr(), page_stride, pages, block_tables.data_ptr(), block_tables.stride(0), table[1],
-                          cu_q.data_ptr(), seq_lens.data_ptr(), cu_groups.data_ptr(), shared_lens.data_ptr(), out.data_ptr(), room.data_ptr(),
-                          self._dev_err_at, n, r, groups, heads, kv_heads, dim, page_size, scale, window, _raw_stream(index))
+        call, room_of = self._shared_lib(dtype, dim)
+        key = (n, r, groups, kv_heads, group, dim, dtype)
+        size = self._shared_sizes.get(key)
+        if size is None:
+            if len(self._shared_sizes) > 4096:
+                self._shared_sizes.clear()
+            size = self._shared_sizes[key] = self.shared_prefix_room(n, r, groups, heads, kv_heads, dim, dtype)
+        if room is None:
+            room = torch.empty(size, dtype=torch.uint8, device=q.device)
+        elif room.dtype is not torch.uint8 or room.dim() != 1 or not room.is_contiguous() or room.numel() < size or room.data_ptr() % 256 \
+                or room.get_device() != index:
+            raise KernelError(f"shared_prefix_attention: a room is uint8 [{size} or more], contiguous, on 256 bytes, on the same device")
+        self.launches += 2 if dtype is torch.float32 or group > 16 or n * group <= 16 else 3
+        self._err_armed = True
+        packed = _SHARED_CALL(q.data_ptr(), kv_pages.data_ptr(), block_tables.data_ptr(), cu_q.data_ptr(), seq_lens.data_ptr(), cu_groups.data_ptr(),
+                              shared_lens.data_ptr(), out.data_ptr(), room.data_ptr(), self._dev_err_at, _raw_stream(index), q_row, page_stride, pages,
+                              table_pitch[0], scale, table[1], n, r, groups, heads, kv_heads, dim, page_size, window, 0)
+        other = _device_of(index)
+        if other is None:
+            status = call(packed)
+        else:
+            with other:
+                status = call(packed)
+        if status:
             _status(status, "shared_prefix_attention")
         return out
