@@ -34,6 +34,10 @@ def build_parser() -> argparse.ArgumentParser:
     gen = ap.add_argument_group("generation")
     gen.add_argument("--max-tokens", "--output-tokens", dest="max_tokens", type=int, default=32)
     gen.add_argument("--temperature", type=float, default=0.0)
+    gen.add_argument("--top-k", type=int, default=0, help="draw from the k likeliest tokens (0: all)")
+    gen.add_argument("--top-p", type=float, default=1.0, help="draw from the likeliest tokens that together have this share")
+    gen.add_argument("--min-p", type=float, default=0.0, help="draw from the tokens that have this share of the likeliest's probability")
+    gen.add_argument("--logprobs", action="store_true", help="the generated tokens' log probabilities under the model, in the JSON report")
     gen.add_argument("--seed", type=int, default=0, help="seed of sampling and of --prompt-len")
     eng = ap.add_argument_group("engine")
     eng.add_argument("--num-slots", "--max-num-seqs", dest="max_num_seqs", type=int, default=1,
@@ -103,7 +107,8 @@ def main(argv=None) -> int:
         t0 = time.perf_counter()
         engine = Engine.from_model_dir(model_dir, options, tokenizer=tokenizer)
         load_ms = (time.perf_counter() - t0) * 1000
-        sp = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, seed=args.seed)
+        sp = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, seed=args.seed, top_k=args.top_k, top_p=args.top_p,
+                            min_p=args.min_p, logprobs=args.logprobs)
         if args.prompt is not None:
             req = engine.add_text_request(args.prompt, sp, stop_strings=args.stop_strings)
         else:
@@ -150,6 +155,8 @@ def main(argv=None) -> int:
                 "generated_token_ids": list(req.output_token_ids),
                 "finish_reason": req.finish_reason,
             }
+            if args.logprobs:
+                report["logprobs"] = list(req.output_logprobs)
             if tokenizer is not None:
                 report["text"] = engine.final_text(req.request_id)
             print(json.dumps(report, ensure_ascii=False, indent=2))

@@ -4,7 +4,7 @@
 // equal ones by rising index.  A: the first k of the order (k < 1 or >= the vocabulary: all).  B: those of A before which A has less than p of its weight
 // (p >= 1: all; at least the first).  C: those of B with w_i >= min_p (or l_i = m).  The token is the smallest index i of C with
 // sum_{j <= i, j in C} w_j > u sum_C w; its log probability under C is (l_i - m) / T - log sum_C w.  T = 0 (or not above 0): the first of
-// the order, log probability 0.  A row without a number above -inf: token 0, NaN.
+// the order, log probability 0.  T NaN: the row is not drawn, nothing is written.  A row without a number above -inf: token 0, NaN.
 //
 // Weights are whole numbers W_i = round(2^44 w_i), from 64-bit arithmetic (so what is below 2^-45 of the largest is never drawn).  The borders between 150,000 tokens lie some 1e-6 of the sum apart, so that
 // 32-bit sums (1e-7) would move one draw in tens to another token; with W one row in some 100,000 comes near a border (the errors of 150,000
@@ -475,6 +475,10 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
 
   const float temp = a.temperature[r], u = a.uniform[r], p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
   const int k = a.top_k ? a.top_k[r] : 0;
+  if (temp != temp) {      // the row is not to be drawn
+    if (row.ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    return;
+  }
 
   // ---- the slice into shared memory, and its best token
   const T* src = logits + r * a.pitch + base;

@@ -50,6 +50,7 @@ class RawStep:
     handle: object = None                  # SampledTokens of the step (None: nothing was sampled)
     sampled: List[str] = field(default_factory=list)     # request ids, in the order of the handle's rows
     tokens: Dict[str, int] = field(default_factory=dict)
+    logprobs: Dict[str, float] = field(default_factory=dict)     # of requests that keep them
     error: Optional[str] = None
 
 
@@ -58,7 +59,7 @@ class Engine:
                  tokenizer: Optional[Tokenizer] = None, eos_token_ids: Sequence[int] = (), max_prefill_portion=None):
         self.runner = runner
         self.scheduler = scheduler or Scheduler(runner.cache, runner.max_requests, runner.max_tokens,
-                                                runner.max_model_len, max_prefill_portion)
+                                                runner.max_model_len, max_prefill_portion, cuts=getattr(runner, "draws_under_cuts", False))
         self.tokenizer = tokenizer
         self.eos_token_ids = list(eos_token_ids)
         self._detoks: Dict[str, StreamingDetokenizer] = {}
@@ -163,7 +164,11 @@ class Engine:
             temps = [r.sampling_params.effective_temperature for r in reqs]
             us = [uniform(r.sampling_params.seed, len(r.output_token_ids) + pending) if t > 0.0 else 0.0
                   for r, t in zip(reqs, temps)]
-            raw.handle = self.runner.step_and_sample(entries, temps, us, feed=feed)
+            cuts = [r.sampling_params.cuts for r in reqs]
+            more = {"cuts": cuts} if any(cuts) else {}
+            if any(r.sampling_params.logprobs for r in reqs):
+                more["logprobs"] = True
+            raw.handle = self.runner.step_and_sample(entries, temps, us, feed=feed, **more)
             raw.sampled = [e.request_id for e in sampled]
             for e in plan.entries:                 # the tokens' keys and values are in the pages now
                 self.scheduler.advance(e)
@@ -179,6 +184,9 @@ class Engine:
         plan, sch = raw.plan, self.scheduler
         if raw.error is None and raw.handle is not None:
             raw.tokens = {rid: int(t) for rid, t in zip(raw.sampled, raw.handle.tolist())}
+            if raw.handle.logprobs is not None:
+                raw.logprobs = {rid: x for rid, x in zip(raw.sampled, raw.handle.logprob_list())
+                                if sch.get_request(rid).sampling_params.logprobs}
         completed, failed = [], list(plan.failed)
         new_tokens: Dict[str, List[int]] = {}
         new_text: Dict[str, str] = {}
@@ -200,7 +208,7 @@ class Engine:
             if not e.sample:
                 continue
             tok = raw.tokens[e.request_id]
-            req.append_output_token(tok)
+            req.append_output_token(tok, raw.logprobs.get(e.request_id))
             sch.on_token(e.request_id)
             new_tokens.setdefault(e.request_id, []).append(tok)
             reason = req.check_finished(tok)

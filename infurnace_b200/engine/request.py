@@ -38,10 +38,11 @@ class SamplingParams:
     """The reference's fields (request.py:35-44) plus ``seed``.
 
     ``temperature`` 0 is greedy (the reference's only sampler, src/infurnace/sampler/greedy.py:21-22);
-    above 0 a token is drawn from softmax(logits / temperature).  ``top_k`` and ``top_p``
-    exist in the reference but nothing there reads them; here ``top_k`` may be 0 (off) or 1
-    (greedy whatever the temperature) and ``top_p`` must be 1.0; other values are refused
-    at admission."""
+    above 0 a token is drawn from softmax(logits / temperature), cut by ``top_k`` (the k likeliest; 0: off, 1: greedy whatever
+    the temperature), then by ``top_p`` (the likeliest that together have this share; 1.0: off) and by ``min_p`` (those that have
+    this share of the likeliest's probability; 0.0: off).  ``top_k`` and ``top_p`` exist in the reference but nothing there
+    reads them.  Cuts other than ``top_k`` 1 need a kernel set that draws under them; without one they are refused at admission, and so
+    is ``logprobs`` (whether the request keeps its tokens' log probabilities under the model, whatever temperature and cuts)."""
     temperature: float = 0.0
     top_k: int = 0
     top_p: float = 1.0
@@ -50,14 +51,21 @@ class SamplingParams:
     min_tokens: int = 0
     include_stop_str_in_output: bool = False
     seed: int = 0
+    min_p: float = 0.0
+    logprobs: bool = False
 
-    def problem(self) -> Optional[str]:
+    def problem(self, cuts: bool = False) -> Optional[str]:
+        """What is wrong with the options, or None.  ``cuts``: whether tokens can be drawn under cuts, and scored."""
         if not self.temperature >= 0.0:
             return f"temperature {self.temperature} is negative"
-        if self.top_k not in (0, 1):
-            return f"top_k {self.top_k} is not supported (0: off, 1: greedy)"
-        if self.top_p != 1.0:
-            return f"top_p {self.top_p} is not supported (1.0: off)"
+        if self.top_k not in (0, 1) and not (cuts and isinstance(self.top_k, int) and 0 <= self.top_k < 1 << 31):
+            return f"top_k {self.top_k} is not supported (0: off, 1: greedy" + (", or how many)" if cuts else ")")
+        if self.top_p != 1.0 and not (cuts and 0.0 <= self.top_p <= 1.0):
+            return f"top_p {self.top_p} is not supported (1.0: off" + (", or a share)" if cuts else ")")
+        if self.min_p != 0.0 and not (cuts and 0.0 <= self.min_p <= 1.0):
+            return f"min_p {self.min_p} is not supported (0.0: off" + (", or a share)" if cuts else ")")
+        if self.logprobs and not cuts:
+            return "logprobs are not supported"
         if self.max_tokens < 0:
             return f"max_tokens {self.max_tokens} is negative"
         return None
@@ -65,6 +73,13 @@ class SamplingParams:
     @property
     def effective_temperature(self) -> float:
         return 0.0 if self.top_k == 1 else float(self.temperature)
+
+    @property
+    def cuts(self):
+        """(top_k, top_p, min_p) where a token is drawn under one of them, else None."""
+        if self.effective_temperature == 0.0 or (self.top_k == 0 and self.top_p == 1.0 and self.min_p == 0.0):
+            return None
+        return int(self.top_k), float(self.top_p), float(self.min_p)
 
 
 @dataclass
@@ -103,11 +118,17 @@ class Request:
     def __post_init__(self):
         self.prompt_token_ids = [int(t) for t in self.prompt_token_ids]
         self._output: List[int] = []
+        self._logprobs: List[Optional[float]] = []
         self._all: List[int] = list(self.prompt_token_ids)
 
     @property
     def output_token_ids(self):
         return tuple(self._output)
+
+    @property
+    def output_logprobs(self):
+        """The output tokens' log probabilities under the model (of a request whose ``logprobs`` is set)."""
+        return tuple(self._logprobs)
 
     @property
     def all_token_ids(self):
@@ -130,10 +151,12 @@ class Request:
     def is_active(self) -> bool:
         return self.state in (RequestState.PREFILLING, RequestState.DECODING)
 
-    def append_output_token(self, token_id: int) -> None:
+    def append_output_token(self, token_id: int, logprob: Optional[float] = None) -> None:
         if self.metrics.first_token_time is None:
             self.metrics.first_token_time = monotonic()
         self._output.append(int(token_id))
+        if logprob is not None:
+            self._logprobs.append(logprob)
         self._all.append(int(token_id))
 
     def check_finished(self, new_token_id: int) -> Optional[str]:

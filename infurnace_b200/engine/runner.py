@@ -53,13 +53,19 @@ class SampledTokens:
     """The token ids one step sampled, on their way to the host: a device copy that the next step may
     take its input tokens from, and a pinned host copy that ``tolist`` waits for."""
 
-    def __init__(self, device, host, event, count, slot):
+    def __init__(self, device, host, event, count, slot, logprobs=None):
         self.device, self.host, self.event, self.count, self.slot = device, host, event, count, slot
+        self.logprobs = logprobs           # the tokens' log probabilities on the host, where they were asked for
 
     def tolist(self):
         if self.event is not None:
             self.event.synchronize()
         return self.host[: self.count].tolist()
+
+    def logprob_list(self):
+        if self.event is not None:
+            self.event.synchronize()
+        return self.logprobs[: self.count].tolist()
 
 
 @dataclass
@@ -174,7 +180,9 @@ class ModelRunner:
         self._pin = dev is not None and torch.device(dev).type == "cuda"
         n, r, g = self._n_cap, self.max_requests, len(cache.kv_groups)
         # one staging area: [ids n][pos n][req n][logit_rows n][cu_q r+1][seq r][slot r][first r] + g * [slots n]
-        self._small_len = 4 * n + 4 * r + 1 + g * n + 2 * r      # the last 2r words: temperatures, uniforms (float32)
+        # the last 6r words: temperatures, uniforms (float32), and what cuts draws: top_k (int32), top_p, min_p, temperatures of rows that are
+        # drawn under cuts (NaN: of the others)
+        self._small_len = 4 * n + 4 * r + 1 + g * n + 6 * r
         # behind it, from a multiple of 256 bytes on, the block tables [g][r][pages]: with one group one copy brings a step's share of both
         self._tables_at = -(-self._small_len // 64) * 64
         # two host staging sets used in turn: a set is rewritten only after the copy that
@@ -196,6 +204,8 @@ class ModelRunner:
         self._hist = [torch.zeros(max(r, 1), dtype=torch.int32, device=dev) for _ in range(2)]
         self._hist_host = [torch.zeros(max(r, 1), dtype=torch.int32, pin_memory=self._pin) for _ in range(2)]
         self._sampled_steps = 0
+        self.draws_under_cuts = hasattr(runtime.kernels, "sample_filtered")      # and scores tokens
+        self._logprobs = None          # buffers of the tokens' log probabilities, made when they are first asked for
         # decode-only steps are replayed from CUDA graphs, one per (batch bucket, context bucket)
         self.use_graphs = self._pin and bool(getattr(model, "graph_safe", False))
         self._graphs: Dict[tuple, tuple] = {}
@@ -298,10 +308,12 @@ class ModelRunner:
         return logits
 
     def step_and_sample(self, entries: Sequence[StepEntry], temperatures: Sequence[float],
-                        uniforms: Sequence[float], feed=None) -> Optional[SampledTokens]:
+                        uniforms: Sequence[float], feed=None, cuts=None, logprobs=False) -> Optional[SampledTokens]:
         """``step`` followed by the sampling kernel on the wanted rows: returns the sampled token
         ids as a :class:`SampledTokens` (None if nothing is wanted); nothing here waits for the
-        device.  ``temperatures`` and ``uniforms`` have one entry per wanted row.
+        device.  ``temperatures`` and ``uniforms`` have one entry per wanted row.  ``cuts``: for each wanted row None or
+        (top_k, top_p, min_p), under which it is drawn (rows without are drawn as in a step without any).  ``logprobs``: the tokens' log
+        probabilities under the model come with them.
 
         ``feed`` = (previous step's SampledTokens, rows): the step's input tokens are not known
         to the host yet; entry i takes row ``rows[i]`` of what the previous step sampled, on the
@@ -312,8 +324,17 @@ class ModelRunner:
         wanted = sum(len(e.want) for e in entries)
         if len(temperatures) != wanted or len(uniforms) != wanted:
             raise BatchError("one temperature and one uniform number per wanted row")
+        if cuts is not None and (len(cuts) != wanted or not self.draws_under_cuts):
+            raise BatchError("cuts: one entry per wanted row, and a kernel set that draws under them")
+        if logprobs and not self.draws_under_cuts:
+            raise BatchError("logprobs: the kernel set does not score tokens")
+        if cuts is not None and not any(c is not None and t > 0.0 for c, t in zip(cuts, temperatures)):
+            cuts = None
+        if logprobs and self._logprobs is None:
+            r, dev = max(self.max_requests, 1), self.rt.device
+            self._logprobs = (torch.zeros(r, dtype=torch.float32, device=dev), [torch.zeros(r, dtype=torch.float32, pin_memory=self._pin) for _ in range(2)])
         self._reserve(entries)
-        self._run_reserved(entries, temperatures, uniforms, feed, sample=True)
+        self._run_reserved(entries, temperatures, uniforms, feed, sample=True, cuts=cuts, logprobs=logprobs)
         for e in entries:
             self.cache.commit(e.request_id, len(e.tokens))
         self.steps_run += 1
@@ -325,15 +346,17 @@ class ModelRunner:
         dev_part, host_part, sampled_part = self._part(("hist", slot), wanted, dev, host, self.sampled)
         dev_part.copy_(sampled_part)
         host_part.copy_(dev_part, non_blocking=True)
+        if logprobs:
+            self._logprobs[1][slot][:wanted].copy_(self._logprobs[0][:wanted], non_blocking=True)
         event = self._record(("sampled", slot)) if self._pin else None
-        return SampledTokens(dev, host, event, wanted, slot)
+        return SampledTokens(dev, host, event, wanted, slot, self._logprobs[1][slot] if logprobs else None)
 
-    def _run_reserved(self, entries, temperatures, uniforms, feed, sample: bool):
+    def _run_reserved(self, entries, temperatures, uniforms, feed, sample: bool, cuts=None, logprobs=False):
         """``_execute`` for a step whose pages are taken: if it raises, the pages go back, so that a caller
         that goes on after the error (the engine fails the step's requests; a replay ends) finds the
         cache as it was before the step."""
         try:
-            return self._execute(entries, temperatures, uniforms, feed, sample=sample)
+            return self._execute(entries, temperatures, uniforms, feed, sample=sample, cuts=cuts, logprobs=logprobs)
         except BaseException:
             self._table_rows.clear()               # the tables get shorter, and may grow again with other pages
             for held in self._stage_rows:
@@ -355,7 +378,7 @@ class ModelRunner:
             idx = torch.tensor(list(rows), dtype=torch.int64, device=prev.device.device)
             self._dev_small[:n].copy_(prev.device.index_select(0, idx))
 
-    def _forward(self, ctx, sample: bool, greedy: bool):
+    def _forward(self, ctx, sample: bool, greedy: bool, cut: bool = False, logprobs: bool = False):
         logits = self.model.forward(ctx)
         if sample and logits is not None:
             m = logits.shape[0]
@@ -363,9 +386,14 @@ class ModelRunner:
                 self.rt.kernels.sample(logits, None, None, self.sampled[:m])
             else:
                 self.rt.kernels.sample(logits, ctx.temperatures[:m], ctx.uniforms[:m], self.sampled[:m])
+            if cut:      # the rows that have cuts, anew: a row without draws the token that it draws in any other batch
+                k, p, least, temperatures = (x[:m] for x in ctx.cuts)
+                self.rt.kernels.sample_filtered(logits, temperatures, ctx.uniforms[:m], self.sampled[:m], top_k=k, top_p=p, min_p=least)
+            if logprobs:
+                self.rt.kernels.token_logprobs(logits, self.sampled[:m], self._logprobs[0][:m])
         return logits
 
-    def _execute(self, entries, temperatures, uniforms, feed, sample: bool):
+    def _execute(self, entries, temperatures, uniforms, feed, sample: bool, cuts=None, logprobs=False):
         """The step's kernels: launched one by one, or replayed from a CUDA graph.
 
         What a graph fixes is what the launches take from the host: the numbers of tokens, requests
@@ -378,6 +406,9 @@ class ModelRunner:
         recording.  A graph is dropped when a buffer it points at has moved."""
         greedy = sample and all(t == 0.0 for t in temperatures)
         build = dict(temperatures=temperatures, uniforms=uniforms) if sample and not greedy else {}      # nothing reads them then
+        if cuts is not None:
+            build["cuts"] = cuts
+        kind = (greedy, cuts is not None, logprobs)
         # The padding and the length bucket are the same whether graphs are used or not, so that a step launches
         # the same kernels with the same parameters either way (the split of a context over CTAs follows the bucket).
         longest = max(self.cache.num_computed(e.request_id) + len(e.tokens) for e in entries)
@@ -394,13 +425,13 @@ class ModelRunner:
         if not self.use_graphs:
             ctx = self._build_context(entries, pad_to=r_bucket, seq_bucket=seq_bucket, **build)
             self._apply_feed(feed)
-            return self._forward(ctx, sample, greedy)
+            return self._forward(ctx, sample, *kind)
         staged = self._stage_step(entries, pad_to=r_bucket, seq_bucket=seq_bucket, **build)
         if decode_only:
-            key = ("decode", r_bucket, seq_bucket, greedy)
+            key = ("decode", r_bucket, seq_bucket, *kind)
         else:
             key = ("any", staged.num_tokens, staged.num_requests, staged.num_logit_rows, staged.max_q_len, staged.min_q_len,
-                   seq_bucket, sample, greedy)
+                   seq_bucket, sample, *kind)
         self._apply_feed(feed)
         stamp = (self.arena.generation, getattr(self.rt.kernels, "scratch_generation", 0))
         held = self._graphs.get(key)
@@ -414,7 +445,7 @@ class ModelRunner:
         self._shapes_seen[key] = seen
         ctx = self._context(staged)
         # run once as it is (which also makes every allocation) ...
-        logits = self._forward(ctx, sample, greedy)
+        logits = self._forward(ctx, sample, *kind)
         if not decode_only and seen < 2:
             return logits
         # ... then record the same launches for the next time; the recording runs nothing
@@ -430,7 +461,7 @@ class ModelRunner:
         gc.disable()                   # a collection inside the recording could free pinned memory or older graphs, which a
         try:                           # stream that is being recorded does not allow
             with torch.cuda.graph(graph):
-                recorded = self._forward(ctx, sample, greedy)
+                recorded = self._forward(ctx, sample, *kind)
         finally:
             if collecting:
                 gc.enable()
@@ -457,10 +488,10 @@ class ModelRunner:
         return held[2][:n]
 
     # ------------------------------------------------------------------ metadata
-    def _build_context(self, entries, temperatures=None, uniforms=None, pad_to=0, seq_bucket=0) -> StepContext:
-        return self._context(self._stage_step(entries, temperatures, uniforms, pad_to, seq_bucket))
+    def _build_context(self, entries, temperatures=None, uniforms=None, pad_to=0, seq_bucket=0, cuts=None) -> StepContext:
+        return self._context(self._stage_step(entries, temperatures, uniforms, pad_to, seq_bucket, cuts))
 
-    def _stage_step(self, entries, temperatures=None, uniforms=None, pad_to=0, seq_bucket=0) -> _Staged:
+    def _stage_step(self, entries, temperatures=None, uniforms=None, pad_to=0, seq_bucket=0, cuts=None) -> _Staged:
         """Write what the kernels see of a step into a staging set and start its copy to the device.  A replayed step needs no more
         than this: the views that a StepContext is made of cost a third of a small model's step."""
         cache = self.cache
@@ -569,6 +600,13 @@ class ModelRunner:
             if k:
                 hf[o_f:o_f + k] = temperatures
                 hf[o_f + r_max:o_f + r_max + k] = uniforms
+            if cuts is not None:
+                o_c = o_f + 2 * r_max
+                hf[o_c + 3 * r_max:o_c + 4 * r_max] = np.nan
+                for j, (c, t) in enumerate(zip(cuts, temperatures)):
+                    if c is not None and t > 0.0:
+                        h[o_c + j] = c[0]
+                        hf[o_c + r_max + j], hf[o_c + 2 * r_max + j], hf[o_c + 3 * r_max + j] = c[1], c[2], t
         if n_groups == 1:
             end = self._tables_at + R * self.max_pages
             to, source = self._part(("staged", turn), end, self._dev_all, host_all)
@@ -598,6 +636,8 @@ class ModelRunner:
         ctx.max_q_len, ctx.min_q_len, ctx.max_seq_len = staged.max_q_len, staged.min_q_len, staged.max_seq_len
         df = d.view(torch.float32)
         ctx.temperatures, ctx.uniforms = df[o_f:o_f + r_max], df[o_f + r_max:o_f + 2 * r_max]
+        o_c = o_f + 2 * r_max
+        ctx.cuts = (d[o_c:o_c + r_max], *(df[o_c + i * r_max:o_c + (i + 1) * r_max] for i in (1, 2, 3)))
         ctx.num_real_logit_rows = staged.num_real_logit_rows
         ctx.token_ids, ctx.positions = d[:N], d[o_pos:o_pos + N]
         ctx.req_index, ctx.logit_rows = d[o_req:o_req + N], d[o_rows:o_rows + M]

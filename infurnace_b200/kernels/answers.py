@@ -74,7 +74,7 @@ class AnswerKernels:
     def sample_filtered(self, logits, temperature, uniform, out, top_k=None, top_p=None, min_p=None, logprobs=None):
         """A token for each row of ``logits`` (float32 or bfloat16 [rows, vocabulary]; rows may lie apart) from softmax(logits / temperature) cut by
         top-k, then top-p, then min-p, each off where it is None.  All others have one number a row: ``temperature`` (float32; 0: the
-        largest logit), ``uniform`` (float32 in [0, 1)), ``top_k`` (int32; below 1: off), ``top_p`` (float32; from 1 on: off; at least the best
+        largest logit; NaN: the row is not drawn, its outputs stay as they are), ``uniform`` (float32 in [0, 1)), ``top_k`` (int32; below 1: off), ``top_p`` (float32; from 1 on: off; at least the best
         token stays), ``min_p`` (float32; a token stays whose probability is at least this times the best one's), ``out`` (int32) and
         ``logprobs`` (float32: the drawn token's log probability under what the cuts left, 0 at temperature 0).
 

@@ -1,4 +1,4 @@
-"""Sampling: greedy and temperature, on the device, from float32 logits.
+"""Sampling: greedy, temperature, and under top-k, top-p and min-p, on the device, from float32 logits.
 
 The reference samples with ``argmax`` and one device read-back per token
 (src/infurnace/sampler/greedy.py:21-22); its documents ask for a per-request random key and
@@ -10,6 +10,7 @@ or on preemption.
 """
 from __future__ import annotations
 
+import math
 from typing import List, Sequence
 
 import torch
@@ -39,9 +40,9 @@ class Sampler:
         self._pin = torch.device(device).type == "cuda"
 
     def sample(self, logits: torch.Tensor, temperatures: Sequence[float], seeds: Sequence[int],
-               counters: Sequence[int]) -> List[int]:
+               counters: Sequence[int], cuts=None) -> List[int]:
         """One token id per row of ``logits``.  Row m uses temperatures[m] (0: greedy) and the
-        random number of draw counters[m] of seeds[m]."""
+        random number of draw counters[m] of seeds[m], and is drawn under ``cuts[m]`` = (top_k, top_p, min_p) where that is not None."""
         m = logits.shape[0]
         out = torch.empty(m, dtype=torch.int32, device=logits.device)
         if all(t == 0.0 for t in temperatures):
@@ -53,4 +54,11 @@ class Sampler:
                 host = host.pin_memory()
             dev = host.to(logits.device, non_blocking=True)
             self.k.sample(logits, dev[0], dev[1], out)
+            if cuts is not None and any(c is not None for c in cuts):
+                cut = [c is not None and t > 0.0 for c, t in zip(cuts, temperatures)]
+                host = torch.tensor([[t if on else math.nan for t, on in zip(temperatures, cut)],
+                                     [c[1] if on else 1.0 for c, on in zip(cuts, cut)], [c[2] if on else 0.0 for c, on in zip(cuts, cut)]],
+                                    dtype=torch.float32).to(logits.device)
+                k = torch.tensor([c[0] if on else 0 for c, on in zip(cuts, cut)], dtype=torch.int32, device=logits.device)
+                self.k.sample_filtered(logits, host[0], dev[1], out, top_k=k, top_p=host[1], min_p=host[2])
         return out.tolist()
