@@ -108,6 +108,12 @@ __device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp
   const u64 whole = (u64)__double_as_longlong(fma(p, scale, 4503599627370496.0)) & ((1ull << 52) - 1);
   return best ? (u64)UNIT : none ? 0 : whole;
 }
+// What min_p asks of a logit, and a little less.
+__device__ __forceinline__ float least_floor(float m, float least, const RowScale& rs) {
+  const float l = m - (0.01f - log2f(fminf(least, 1.f))) / rs.to_log2;
+  return l - fabsf(l) * 2.4e-7f;
+}
+
 // The place of a number in bins of equal width; BINS or more (NaN included): its weight is 0.
 __device__ __forceinline__ float row_bin(float l, const RowScale& rs) { return l == rs.top ? 0.f : (rs.top - l) * rs.to_bin; }
 
@@ -136,7 +142,7 @@ __device__ __forceinline__ u64 warp_add(u64 v) {
   return v;
 }
 
-struct Row {
+template <int WARPS> struct RowOf {      // (of CTAs of so many warps)
   CutShared* sh;
   int ctas, rank, turn;
   // Every CTA's (a, b) to every CTA; read with got(r) until the call after the next.
@@ -157,7 +163,7 @@ struct Row {
     __syncthreads();
     a = b = 0;
     if (threadIdx.x == 0)
-      for (int w = 0; w < NW; ++w) { a += sh->warp_a[w]; b += sh->warp_b[w]; }
+      for (int w = 0; w < WARPS; ++w) { a += sh->warp_a[w]; b += sh->warp_b[w]; }
     const Exchange* box = tell(a, b);
     a = b = 0;
     for (int r = 0; r < ctas; ++r) { a += box[r].a; b += box[r].b; }
@@ -174,7 +180,7 @@ struct Row {
     if (lane == 0) { sh->warp_a[warp] = a; sh->warp_b[warp] = b; }
     __syncthreads();
     if (threadIdx.x == 0)
-      for (int w = 0; w < NW; ++w) { a = a > sh->warp_a[w] ? a : sh->warp_a[w]; b = b < sh->warp_b[w] ? b : sh->warp_b[w]; }
+      for (int w = 0; w < WARPS; ++w) { a = a > sh->warp_a[w] ? a : sh->warp_a[w]; b = b < sh->warp_b[w] ? b : sh->warp_b[w]; }
     const Exchange* box = tell(a, b);
     a = 0; b = ALL;
     for (int r = 0; r < ctas; ++r) { a = a > box[r].a ? a : box[r].a; b = b < box[r].b ? b : box[r].b; }
@@ -189,13 +195,14 @@ struct Row {
     if (lane == 31) sh->warp_a[warp] = run;
     __syncthreads();
     u64 mine = 0, at = run - v;
-    for (int w = 0; w < NW; ++w) { const u64 x = sh->warp_a[w]; if (w < warp) at += x; mine += x; }
+    for (int w = 0; w < WARPS; ++w) { const u64 x = sh->warp_a[w]; if (w < warp) at += x; mine += x; }
     const Exchange* box = tell(mine, 0);
     total = 0;
     for (int r = 0; r < ctas; ++r) { if (r < rank) at += box[r].a; total += box[r].a; }
     return at;
   }
 };
+using Row = RowOf<NW>;
 
 // The counts and weights of `n` bins over all CTAs of the row, from each CTA's own (weights in two halves): to every CTA.
 __device__ __forceinline__ void merge_bins(const Row& row, int n, const uint32_t* own_count, const uint32_t* own_lo, const uint32_t* own_hi,
@@ -415,6 +422,90 @@ __device__ bool find_cut(Row& row, const CutMemory& mem, const float* vals, int 
   return true;
 }
 
+// Where the cut to the first k lies so high that all tokens of its bin and above fit into a list (`members` of them, bins 0 .. last_bin): both cuts at once from
+// their order, without weights of any other token.
+__device__ void list_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, int last_bin, uint32_t members, uint32_t k,
+                         float p, Cut& cut) {
+  CutShared* sh = row.sh;
+  u64* lw = mem.list_mass;
+  float* ll = mem.list_l;
+  uint32_t* li = mem.list_i;
+  const float f1 = last_bin + 1.f;
+  for (int i0 = threadIdx.x; i0 < n; i0 += 4 * NT) {
+    bool in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) in[j] = i0 + j * NT < n && row_bin(vals[i0 + j * NT], rs) < f1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!in[j]) continue;
+      const int i = i0 + j * NT;
+      const uint32_t at = add_peer(&sh->listed, 0, 1u);
+      if (at >= LIST) continue;      // (never: the members were counted)
+      put_u64(lw + at, 0, row_weight(vals[i], rs, sh->tab));
+      put_u32(reinterpret_cast<uint32_t*>(ll) + at, 0, __float_as_uint(vals[i]));
+      put_u32(li + at, 0, (uint32_t)(base + i));
+    }
+  }
+  row_sync(row.ctas);
+  if (row.rank == 0) {
+    if (threadIdx.x == 0) sh->listed = 0;
+    const int sub = threadIdx.x & 3, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;      // four threads count what comes before a member
+    uint32_t pos[LIST * 4 / NT];
+    u64 before[LIST * 4 / NT], kept_mass = 0;
+#pragma unroll
+    for (int t = 0; t < LIST * 4 / NT; ++t) {
+      const int i = t * (NT / 4) + (int)(threadIdx.x >> 2);
+      if (t * (NT / 4) >= (int)members) break;
+      const bool in = i < (int)members;
+      const float l = in ? ll[i] : INFINITY;
+      const uint32_t idx = in ? li[i] : 0;
+      uint32_t c = 0;
+      u64 w = 0;
+#pragma unroll 4
+      for (int j = sub; j < (int)members; j += 4) {
+        const float other = ll[j];
+        const bool first = other > l || (other == l && li[j] < idx);
+        c += first;
+        w += first ? lw[j] : 0;
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) { c += __shfl_xor_sync(0xffffffffu, c, o); w += __shfl_xor_sync(0xffffffffu, w, o); }
+      pos[t] = in ? c : 0xffffffffu;
+      before[t] = w;
+      if (in && sub == 0 && c < k) kept_mass += lw[i];
+    }
+    kept_mass = warp_add(kept_mass);
+    __syncthreads();
+    if (lane == 0) sh->warp_a[warp] = kept_mass;
+    __syncthreads();
+    kept_mass = 0;
+    for (int v = 0; v < NW; ++v) kept_mass += sh->warp_a[v];
+    u64 goal = ALL;
+    if (p < 1.f) {
+      const double want = ceil((double)p * (double)kept_mass);
+      goal = want >= 1.0 ? (u64)want : 1;
+    }
+    const uint32_t most = members < k ? members : k;
+#pragma unroll
+    for (int t = 0; t < LIST * 4 / NT; ++t) {
+      const int i = t * (NT / 4) + (int)(threadIdx.x >> 2);
+      if (t * (NT / 4) >= (int)members) break;
+      if (sub || pos[t] >= most || before[t] >= goal) continue;
+      if (pos[t] + 1 == most || before[t] + lw[i] >= goal) {      // the last that is kept
+        for (int r = 0; r < row.ctas; ++r) {
+          put_u64(&sh->found[0], r, ((u64)__float_as_uint(ll[i]) << 32) | li[i]);
+          put_u64(&sh->found[1], r, before[t] + lw[i]);
+        }
+      }
+    }
+  }
+  row_sync(row.ctas);
+  cut.l = __uint_as_float((uint32_t)(sh->found[0] >> 32));
+  cut.i = (int)(uint32_t)sh->found[0];
+  cut.mass = sh->found[1];
+  __syncthreads();
+}
+
 template <typename T> struct Vec16;
 template <> struct Vec16<float> {
   static constexpr int N = 4;
@@ -444,6 +535,15 @@ struct CutArgs {
   int* out;
   float* logprobs;
 };
+
+// The drawn token is the first with more than this of the weight up to it.
+__device__ __forceinline__ u64 draw_goal(float u, u64 total) {
+  const u64 goal = u > 0.f ? (u64)((double)u * (double)total) : 0;
+  return goal < total ? goal : total - 1;
+}
+__device__ __forceinline__ float drawn_logprob(float l, float m, float temp, u64 total) {
+  return (float)((l == m ? 0.0 : ((double)l - (double)m) / (double)temp) - log((double)total / UNIT));
+}
 
 template <typename T>
 __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutArgs a) {
@@ -475,18 +575,19 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
 
   const float temp = a.temperature[r], u = a.uniform[r], p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
   const int k = a.top_k ? a.top_k[r] : 0;
-  if (temp != temp) {      // the row is not to be drawn
+  bool by_count = k >= 1 && k < a.vocab;
+  const bool by_mass = p < 1.f, by_least = least > 0.f;
+  if (!(temp > 0.f) || !(by_count || by_mass)) {      // the other kernel's row, or one that is not to be drawn
     if (row.ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
     return;
   }
 
-  // ---- the slice into shared memory, and its best token
+  // ---- the slice into shared memory, and its largest logit
   const T* src = logits + r * a.pitch + base;
   float bv = -INFINITY;
-  int bi = 0x7fffffff;
   auto take = [&](float v, int i) {
     v = v == v ? v + 0.f : -INFINITY;      // -0 becomes 0
-    if (v > bv) { bv = v; bi = i; }
+    bv = fmaxf(bv, v);
     vals[i] = v;
   };
   constexpr int N = Vec16<T>::N;
@@ -502,24 +603,16 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
     }
   }
   for (int i = done + tid; i < n; i += NT) take(to_f32<T>(src[i]), i);
-  bi = bi == 0x7fffffff ? bi : bi + base;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-    if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
-  }
+  for (int o = 16; o > 0; o >>= 1) bv = fmaxf(bv, __shfl_xor_sync(0xffffffffu, bv, o));
   if (row.ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // every peer has begun: its shared memory may be written
-  // (largest first, then lowest index, as one whole number)
-  u64 best = ((u64)ordered(bv) << 32) | (uint32_t)~bi, dummy = ALL;
-  row.extremes(best, dummy);
-  const float m = unordered((uint32_t)(best >> 32));
-  const int first_token = (int)~(uint32_t)best;
-
-  if (!(temp > 0.f) || m == -INFINITY) {
+  u64 best = ordered(bv), unused = ALL;
+  row.extremes(best, unused);
+  const float m = unordered((uint32_t)best);
+  if (m == -INFINITY) {
     if (row.rank == 0 && tid == 0) {
-      a.out[r] = m == -INFINITY ? 0 : first_token;
-      if (a.logprobs) a.logprobs[r] = m == -INFINITY ? __uint_as_float(0x7fc00000u) : 0.f;
+      a.out[r] = 0;
+      if (a.logprobs) a.logprobs[r] = __uint_as_float(0x7fc00000u);
     }
     return;      // (what peers write to one another they have read behind a barrier: nobody need wait)
   }
@@ -528,16 +621,45 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   rs.m = (double)m;
   rs.s = 1.4426950408889634074 / (double)temp;
   rs.to_log2 = (float)fmin(rs.s, 3e38);
-  const bool by_count = k >= 1 && k < a.vocab, by_mass = p < 1.f, by_least = least > 0.f;
 
   // ---- what top-k and top-p keep
   Cut cut = {-INFINITY, 0x7fffffff, 0};
-  if (by_count || by_mass) {
-    bool counted = !by_count, done = false;
-    for (int t = 0; t < TRIES && !done; ++t) {
+  bool found = false, used = false;
+  if (by_count && k <= LIST) {      // by counts alone, if the first k and what shares the last one's bin are a list's worth
+    for (int t = 0; t < TRIES && !found; ++t) {
+      rs.to_bin = (float)fmin(rs.s * (BINS / (double)reach_of(t)), 3e38);
+      if (used) {
+        for (int b = tid; b < BINS; b += NT) mem.count[b] = 0;
+        __syncthreads();
+      }
+      used = true;
+      for (int i0 = tid; i0 < n; i0 += 4 * NT) {
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = i0 + j * NT < n ? row_bin(vals[i0 + j * NT], rs) : INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (f[j] < BINS) atomicAdd(mem.count + (int)f[j], 1u);
+      }
+      merge_bins(row, BINS, mem.count, mem.lo, mem.hi, mem.row_count, mem.row_mass, false);
+      u64 before, unused;
+      const int b = find_bin(sh, BINS, mem.row_count, mem.row_mass, false, (u64)k, before, unused, false);
+      if (b >= BINS) {
+        if (t == TRIES - 1) { by_count = false; found = !by_mass; }      // fewer than k tokens have a weight: top-k keeps them all
+        continue;
+      }
+      const u64 members = before + mem.row_count[b];
+      if (members > LIST) break;
+      list_cut(row, mem, vals, n, base, rs, b, (uint32_t)members, (uint32_t)k, p, cut);
+      found = true;
+    }
+  }
+  if (!found) {
+    bool counted = !by_count;
+    for (int t = 0; t < TRIES && !found; ++t) {
       const bool last_try = t == TRIES - 1;
       rs.to_bin = (float)fmin(rs.s * (BINS / (double)reach_of(t)), 3e38);
-      if (t) {      // (no peer reads these any more)
+      if (t || used) {      // (no peer reads these any more)
         for (int b = tid; b <= BINS; b += NT) mem.count[b] = mem.lo[b] = mem.hi[b] = 0;
         __syncthreads();
       }
@@ -579,10 +701,10 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
       cut.mass = all;
       if (by_count) counted = find_cut(row, mem, vals, n, base, rs, false, (u64)k, by_mass, cut);
       if (!counted && !last_try) continue;      // (with fewer than k tokens in the last try's bins top-k keeps everything)
-      done = true;
+      found = true;
       if (by_mass) {
         const double want = ceil((double)p * (double)cut.mass);
-        done = find_cut(row, mem, vals, n, base, rs, true, want >= 1.0 ? (u64)want : 1, true, cut);
+        found = find_cut(row, mem, vals, n, base, rs, true, want >= 1.0 ? (u64)want : 1, true, cut);
       }
     }
   }
@@ -597,22 +719,13 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   };
   u64 mine = 0, total;
   int i = first;
-  if (!by_count && !by_mass && !by_least) {
-    for (; i + 4 <= last; i += 4)
-      mine += (row_weight(vals[i], rs, sh->tab) + row_weight(vals[i + 1], rs, sh->tab)) + (row_weight(vals[i + 2], rs, sh->tab) + row_weight(vals[i + 3], rs, sh->tab));
-  } else {      // most are not kept
-    float floor = cut.l;
-    if (by_least) {      // what min_p asks, and a little less
-      const float l = m - (0.01f - log2f(fminf(least, 1.f))) / rs.to_log2;
-      floor = fmaxf(floor, l - fabsf(l) * 2.4e-7f);
-    }
-    for (; i + 4 <= last; i += 4)
-      if (fmaxf(fmaxf(vals[i], vals[i + 1]), fmaxf(vals[i + 2], vals[i + 3])) >= floor) mine += (weigh(i) + weigh(i + 1)) + (weigh(i + 2) + weigh(i + 3));
-  }
+  float floor = cut.l;      // most are not kept
+  if (by_least) floor = fmaxf(floor, least_floor(m, least, rs));
+  for (; i + 4 <= last; i += 4)
+    if (fmaxf(fmaxf(vals[i], vals[i + 1]), fmaxf(vals[i + 2], vals[i + 3])) >= floor) mine += (weigh(i) + weigh(i + 1)) + (weigh(i + 2) + weigh(i + 3));
   for (; i < last; ++i) mine += weigh(i);
   const u64 at = row.before(mine, total);
-  u64 goal = u > 0.f ? (u64)((double)u * (double)total) : 0;
-  if (goal >= total) goal = total - 1;
+  const u64 goal = draw_goal(u, total);
   const unsigned owner = __ballot_sync(0xffffffffu, at <= goal && at + mine > goal);
   if (owner) {      // the warp weighs that thread's tokens anew, a lane each
     const int from = __ffs(owner) - 1, i0 = __shfl_sync(0xffffffffu, first, from), i1 = __shfl_sync(0xffffffffu, last, from);
@@ -625,14 +738,151 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
       for (int o = 1; o < 32; o <<= 1) { const u64 y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
       if (run + x > goal && run + x - w <= goal) {
         a.out[r] = base + i;
-        if (a.logprobs) {
-          const float l = vals[i];
-          a.logprobs[r] = (float)((l == m ? 0.0 : ((double)l - (double)m) / (double)temp) - log((double)total / UNIT));
-        }
+        if (a.logprobs) a.logprobs[r] = drawn_logprob(vals[i], m, temp, total);
       }
       run += __shfl_sync(0xffffffffu, x, 31);
     }
   }
+}
+
+// ---------------------------------------------------------------------------------------------------- rows without top-k and top-p
+// Greedy rows, and such as are drawn from all tokens or from those that min_p leaves: nothing has to be looked for, so nothing is kept; a row is read for its
+// largest logit, and a second time, from L2, for its weights.  A CTA needs no shared memory to speak of and four are on an SM, which matters where there are
+// many rows: 256 rows of 151,936 held in shared memory, two CTAs on an SM, took 135 us.  A warp has a stretch of the row, which it
+// takes in blocks of 512; a block's sum is kept, so that the draw goes over 512 tokens anew and no more.
+constexpr int ST_NT = 256, ST_NW = ST_NT / 32, ST_BLOCK = 512, ST_BLOCKS = 16;      // (a CTA has 65,536 logits at most)
+
+// Four numbers from index i on; -inf for NaN and from `end` on.
+template <typename T> __device__ __forceinline__ void stream_read(const T* row, int i, int end, bool aligned, float (&v)[4]) {
+  if (aligned && i + 4 <= end) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(row + i);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(row + i);
+      v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u); v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = i + j < end ? to_f32<T>(row[i + j]) : -INFINITY;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = v[j] == v[j] ? v[j] + 0.f : -INFINITY;
+}
+
+// `beside`: the kernel before this one in the stream has the other rows (attention_shared_narrow.cuh has the argument): this one waits for it at its end.
+template <typename T>
+__global__ void __launch_bounds__(ST_NT, 4) sample_stream_kernel(const T* logits, CutArgs a, int beside) {
+  __shared__ CutShared shared;
+  __shared__ u64 blocks[ST_NW][ST_BLOCKS];
+  CutShared* sh = &shared;
+  RowOf<ST_NW> row = {sh, cluster_size(), cluster_rank(), 0};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long long r = blockIdx.x / row.ctas;
+  sh->tab.t[tid] = exp2(tid / (double)STEPS);
+  static_assert(STEPS == ST_NT, "a thread makes a step of the table");
+  if (row.ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  if (!beside) ifb_pdl_wait();
+  ifb_pdl_trigger();
+  auto draw = [&]() {
+    const float temp = a.temperature[r], u = a.uniform[r], p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
+    const int k = a.top_k ? a.top_k[r] : 0;
+    const bool greedy = !(temp > 0.f), mine = temp == temp && (greedy || !((k >= 1 && k < a.vocab) || p < 1.f));
+    if (row.ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // every peer has begun: its shared memory may be written
+    if (!mine) return;
+    const T* src = logits + r * a.pitch;
+    const bool aligned = (reinterpret_cast<uintptr_t>(src) & (4 * sizeof(T) - 1)) == 0;
+    const int stretch = a.per / ST_NW, from = min((long long)a.vocab, (long long)row.rank * a.per + warp * stretch), end = min(a.vocab, from + stretch);
+    float bv = -INFINITY;
+    int bi = 0x7fffffff;
+    for (int i0 = from; i0 < end; i0 += ST_BLOCK) {
+      float v[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) stream_read<T>(src, i0 + j * 128 + lane * 4, end, aligned, v[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (v[j][e] > bv) { bv = v[j][e]; bi = i0 + j * 128 + lane * 4 + e; }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
+      const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+      if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
+    }
+    // (largest first, then lowest index, as one whole number)
+    u64 best = ((u64)ordered(bv) << 32) | (uint32_t)~bi, unused = ALL;
+    row.extremes(best, unused);
+    const float m = unordered((uint32_t)(best >> 32));
+    if (greedy || m == -INFINITY) {
+      if (row.rank == 0 && tid == 0) {
+        a.out[r] = m == -INFINITY ? 0 : (int)~(uint32_t)best;
+        if (a.logprobs) a.logprobs[r] = m == -INFINITY ? __uint_as_float(0x7fc00000u) : 0.f;
+      }
+      return;
+    }
+    RowScale rs;
+    rs.top = m;
+    rs.m = (double)m;
+    rs.s = 1.4426950408889634074 / (double)temp;
+    rs.to_log2 = (float)fmin(rs.s, 3e38);
+    rs.to_bin = 0.f;
+    const bool by_least = least > 0.f;
+    const float floor = by_least ? least_floor(m, least, rs) : -INFINITY;
+    auto weigh = [&](float l) -> u64 {
+      if (!by_least) return row_weight(l, rs, sh->tab);
+      double w;
+      const u64 whole = row_weight(l, rs, sh->tab, &w);
+      return w >= (double)least * UNIT || l == m ? whole : 0;
+    };
+    u64 all = 0;
+    for (int i0 = from, b = 0; i0 < end; i0 += ST_BLOCK, ++b) {
+      float v[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) stream_read<T>(src, i0 + j * 128 + lane * 4, end, aligned, v[j]);
+      u64 sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!by_least || fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])) >= floor)
+          sum += (weigh(v[j][0]) + weigh(v[j][1])) + (weigh(v[j][2]) + weigh(v[j][3]));
+      sum = warp_add(sum);
+      if (lane == 0) blocks[warp][b] = sum;
+      all += sum;
+    }
+    u64 total, at = row.before(lane == 0 ? all : 0, total);
+    at = __shfl_sync(0xffffffffu, at, 0);
+    const u64 goal = draw_goal(u, total);
+    if (at > goal || at + all <= goal) return;
+    // the warp's block that the draw falls into, and the token of it
+    int b = 0;
+    for (; at + blocks[warp][b] <= goal; ++b) at += blocks[warp][b];
+    for (int j = 0; j < 4; ++j) {
+      const int i = from + b * ST_BLOCK + j * 128 + lane * 4;
+      float v[4];
+      stream_read<T>(src, i, end, aligned, v);
+      u64 w[4], x = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { w[e] = weigh(v[e]); x += w[e]; }
+      u64 run = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const u64 y = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += y; }
+      const u64 sum = __shfl_sync(0xffffffffu, run, 31);
+      if (at + sum <= goal) { at += sum; continue; }
+      u64 c = at + run - x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (c <= goal && c + w[e] > goal) {
+          a.out[r] = i + e;
+          if (a.logprobs) a.logprobs[r] = drawn_logprob(v[e], m, temp, total);
+        }
+        c += w[e];
+      }
+      break;
+    }
+  };
+  draw();
+  if (beside) ifb_pdl_wait();
 }
 
 // How many clusters of `ctas` CTAs with so much shared memory the device holds at a time (remembered by what they fit: two of them on an SM, or one); negative: an
@@ -697,30 +947,46 @@ IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
     ctas *= 2;
   }
   CutArgs a = {call->pitch, vocab, slice(ctas), call->temperature, call->top_k, call->top_p, call->min_p, call->uniform, call->out, call->logprobs};
-  const size_t smem = (size_t)a.per * 4 + CUT_BYTES;
-  auto go = [&](auto kernel, auto typed) -> int {
-    IFB_ALLOW_SMEM(kernel, smem);
+  auto go = [&](auto kernel, int n, int threads, size_t smem, auto... args) -> int {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)rows * ctas);
-    cfg.blockDim = dim3(NT);
+    cfg.gridDim = dim3((unsigned)rows * n);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = call->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.x = n;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ifb_pdl_enabled() ? 2 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, typed, a);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
     return IFB_OK;
   };
-  if (dtype == IFB_F32) return go(sample_cut_kernel<float>, (const float*)call->logits);
-  if (dtype == IFB_BF16) return go(sample_cut_kernel<bf16>, (const bf16*)call->logits);
-  return IFB_ERR_DTYPE;
+  const bool cuts = call->top_k || call->top_p;
+  if (cuts) {
+    const size_t smem = (size_t)a.per * 4 + CUT_BYTES;
+    int st;
+    if (dtype == IFB_F32) {
+      IFB_ALLOW_SMEM(sample_cut_kernel<float>, smem);
+      st = go(sample_cut_kernel<float>, ctas, NT, smem, (const float*)call->logits, a);
+    } else {
+      IFB_ALLOW_SMEM(sample_cut_kernel<bf16>, smem);
+      st = go(sample_cut_kernel<bf16>, ctas, NT, smem, (const bf16*)call->logits, a);
+    }
+    if (st) return st;
+  }
+  // the other rows: as many CTAs of a row as leave no SM idle, each with whole blocks for its warps
+  const int sms = ifb_sm_count();
+  int n = 1;
+  auto stretch = [&](int ctas) { return ((vocab + ctas * ST_NW - 1) / (ctas * ST_NW) + ST_BLOCK - 1) / ST_BLOCK * ST_BLOCK; };
+  while (n < SURE_CLUSTER && (stretch(n) > ST_BLOCKS * ST_BLOCK || ((long long)rows * n * 2 <= 8LL * sms && stretch(n) > 2 * ST_BLOCK))) n *= 2;
+  a.per = stretch(n) * ST_NW;
+  return dtype == IFB_F32 ? go(sample_stream_kernel<float>, n, ST_NT, 0, (const float*)call->logits, a, cuts ? 1 : 0)
+                          : go(sample_stream_kernel<bf16>, n, ST_NT, 0, (const bf16*)call->logits, a, cuts ? 1 : 0);
 }
 
 // ---------------------------------------------------------------------------------------------------- log probabilities
