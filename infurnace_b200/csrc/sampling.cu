@@ -77,7 +77,7 @@ __device__ __forceinline__ void row_sync(int ctas) {
 }
 
 // ---------------------------------------------------------------------------------------------------- weights
-// 2^(j / 256), in shared memory.
+// 2^(44 + j / 256), in shared memory.
 constexpr int STEPS = 256;
 struct Exp2Table { double t[STEPS]; };
 
@@ -87,27 +87,51 @@ struct RowScale {
   float top;        // the largest logit
   float to_bin;     // bins per unit of m - l
   float to_log2;    // s
+  float low;        // a logit whose weight is far below a unit: what lies below it counts as it (a plain row's; see set)
+  bool plain;       // whether that is so: no infinity among the largest, and 500 factors of two are more than a rounding of m
+  __device__ __forceinline__ void set(float largest, float temperature) {
+    top = largest;
+    m = (double)largest;
+    s = 1.4426950408889634074 / (double)temperature;
+    to_log2 = (float)fmin(s, 3e38);
+    to_bin = 0.f;
+    low = largest - 500.f / to_log2;
+    plain = fabsf(largest) * to_log2 < 1e9f && 500.f / to_log2 < 3e38f;      // (false for NaN)
+  }
 };
-// round(2^44 2^y), y = (l - m) s <= 0, as a whole number; `w`, if wanted: before rounding.  y = (n + f) / 256, n whole, |f| <= 1/2: 2^y = 2^(n / 256) e^x,
-// x = f ln 2 / 256, by the first terms of its Taylor series (x^4 / 24 < 2e-13).  Weights below 2^-46 are 0.  Eight operations in 64 bits and a conversion,
-// without a branch, so that a thread has several numbers under way (one after the other they take 250 cycles each, four together 115).
-__device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp2Table& tab, double* w = nullptr) {
-  const bool none = !((rs.top - l) * rs.to_log2 < REACH), best = l == rs.top;      // (infinities too)
+// round(2^44 2^y), y = (l - m) s <= 0: 2^52 as a 64-bit number's bits, with the whole number in its last ones.  y = (n + f) / 256, n whole, |f| <= 1/2:
+// 2^y = 2^(n / 256) e^x, x = f ln 2 / 256, by the first terms of its Taylor series (x^4 / 24 < 2e-13).  Eight operations in 64 bits and a conversion, without a
+// branch, so that a thread has several numbers under way (one after the other they take 250 cycles each, four together 115); NaN counts as `low`.
+constexpr u64 RAW = 0x4330000000000000ull;      // 2^52
+__device__ __forceinline__ double weight_parts(double d, const RowScale& rs, const Exp2Table& tab, double& scale) {
   constexpr double MAGIC = 6755399441055744.0 / STEPS;      // 1.5 2^52 / 256: the sum's last bit is 1/256
   constexpr double LN2 = 0.693147180559945309417;
-  const double d = (double)l - rs.m;
   const double t = fma(d, rs.s, MAGIC);
   const double r = fma(d, rs.s, -(t - MAGIC));
   const int n = __double2loint(t);
   const double step = tab.t[n & (STEPS - 1)];
-  const double scale = __hiloint2double(__double2hiint(step) + (((n >> 8) + 44) << 20), __double2loint(step));
+  scale = __hiloint2double(__double2hiint(step) + (n & ~(STEPS - 1)) * 4096, __double2loint(step));      // n / 256 into the exponent
   double p = fma(r, LN2 * LN2 * LN2 / 6, LN2 * LN2 / 2);
   p = fma(r, p, LN2);
-  p = fma(r, p, 1.0);
+  return fma(r, p, 1.0);
+}
+__device__ __forceinline__ u64 plain_raw(float l, const RowScale& rs, const Exp2Table& tab) {
+  double scale;
+  const double p = weight_parts((double)fmaxf(l, rs.low) - rs.m, rs, tab, scale);
+  return (u64)__double_as_longlong(fma(p, scale, 4503599627370496.0));
+}
+// The whole number of any row; `w`, if wanted: before rounding.  Weights below 2^-46 are 0.
+__device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp2Table& tab, double* w = nullptr) {
+  const bool none = !((rs.top - l) * rs.to_log2 < REACH), best = l == rs.top;      // (infinities too)
+  double scale;
+  const double p = weight_parts((double)l - rs.m, rs, tab, scale);
   if (w) *w = best ? UNIT : none ? 0.0 : p * scale;
   const u64 whole = (u64)__double_as_longlong(fma(p, scale, 4503599627370496.0)) & ((1ull << 52) - 1);
   return best ? (u64)UNIT : none ? 0 : whole;
 }
+// The same as a call, where rows that are not plain go once in a while.
+__device__ __noinline__ u64 called_weight(float l, RowScale rs, const Exp2Table* tab) { return row_weight(l, rs, *tab); }
+
 // What min_p asks of a logit, and a little less.
 __device__ __forceinline__ float least_floor(float m, float least, const RowScale& rs) {
   const float l = m - (0.01f - log2f(fminf(least, 1.f))) / rs.to_log2;
@@ -131,9 +155,7 @@ struct CutShared {
   Exchange swap[2][MAX_CLUSTER];        // what the CTAs of a row tell each other, in turn
   u64 warp_a[NW], warp_b[NW];
   u64 found[4];
-  uint32_t listed, chosen;
-  float best_val;
-  uint32_t best_idx;
+  uint32_t listed;
 };
 
 __device__ __forceinline__ u64 warp_add(u64 v) {
@@ -285,7 +307,7 @@ __device__ __forceinline__ void add_mass(uint32_t* lo, uint32_t* hi, int b, u64 
 }
 
 // The cut through the row's bins after which `goal` tokens (by_mass: at least `goal` of weight) are kept.  False: it does not run through them.
-__device__ bool find_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, bool by_mass, u64 goal, bool weighted,
+__device__ __forceinline__ bool find_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, bool by_mass, u64 goal, bool weighted,
                          Cut& cut) {
   CutShared* sh = row.sh;
   u64 bc, bm;
@@ -424,7 +446,7 @@ __device__ bool find_cut(Row& row, const CutMemory& mem, const float* vals, int 
 
 // Where the cut to the first k lies so high that all tokens of its bin and above fit into a list (`members` of them, bins 0 .. last_bin): both cuts at once from
 // their order, without weights of any other token.
-__device__ void list_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, int last_bin, uint32_t members, uint32_t k,
+__device__ __forceinline__ void list_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, int last_bin, uint32_t members, uint32_t k,
                          float p, Cut& cut) {
   CutShared* sh = row.sh;
   u64* lw = mem.list_mass;
@@ -545,8 +567,16 @@ __device__ __forceinline__ float drawn_logprob(float l, float m, float temp, u64
   return (float)((l == m ? 0.0 : ((double)l - (double)m) / (double)temp) - log((double)total / UNIT));
 }
 
+// Whether a row is drawn, and top-k or top-p may cut something of it.  (What it takes is asked for at once.)
+__device__ __forceinline__ bool has_cuts(const CutArgs& a, long long r) {
+  const float t = a.temperature[r], p = a.top_p ? a.top_p[r] : 1.f;
+  const int k = a.top_k ? a.top_k[r] : 0;
+  return (t > 0.f) & (((k >= 1) & (k < a.vocab)) | (p < 1.f));
+}
+
+// `everything`: rows without top-k and top-p too (of few rows, which all find their SMs at once; a second kernel would cost 2 us).
 template <typename T>
-__global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutArgs a) {
+__global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutArgs a, int everything) {
   extern __shared__ __align__(16) unsigned char cut_smem[];
   __shared__ CutShared shared;
   CutShared* sh = &shared;
@@ -566,21 +596,17 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long r = blockIdx.x / row.ctas;
   const int base = min((long long)a.vocab, (long long)row.rank * a.per), n = min(a.vocab - base, a.per);
-  if (tid < STEPS) sh->tab.t[tid] = exp2(tid / (double)STEPS);
-  if (tid == 0) sh->listed = 0;
-  for (int b = tid; b <= BINS; b += NT) mem.count[b] = mem.lo[b] = mem.hi[b] = 0;
-  if (row.ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
   ifb_pdl_wait();
   ifb_pdl_trigger();
-
   const float temp = a.temperature[r], u = a.uniform[r], p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
   const int k = a.top_k ? a.top_k[r] : 0;
+  if (tid < STEPS) sh->tab.t[tid] = UNIT * exp2(tid / (double)STEPS);
+  if (tid == 0) sh->listed = 0;
+  for (int b = tid; b <= BINS; b += NT) mem.count[b] = mem.lo[b] = mem.hi[b] = 0;
   bool by_count = k >= 1 && k < a.vocab;
-  const bool by_mass = p < 1.f, by_least = least > 0.f;
-  if (!(temp > 0.f) || !(by_count || by_mass)) {      // the other kernel's row, or one that is not to be drawn
-    if (row.ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-    return;
-  }
+  const bool by_mass = p < 1.f, by_least = least > 0.f, cuts = by_count | by_mass;
+  if (everything ? temp != temp : !((temp > 0.f) & cuts)) return;      // the other kernel's row, or one that is not to be drawn
+  if (row.ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
 
   // ---- the slice into shared memory, and its largest logit
   const T* src = logits + r * a.pitch + base;
@@ -614,17 +640,26 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
       a.out[r] = 0;
       if (a.logprobs) a.logprobs[r] = __uint_as_float(0x7fc00000u);
     }
-    return;      // (what peers write to one another they have read behind a barrier: nobody need wait)
+    return;
+  }
+  if (!(temp > 0.f)) {      // the lowest index of the largest
+    u64 where = ALL;
+    unused = 0;
+    for (int i = n - 1 - tid; i >= 0; i -= NT)
+      if (vals[i] == m) where = base + i;
+    row.extremes(unused, where);
+    if (row.rank == 0 && tid == 0) {
+      a.out[r] = (int)where;
+      if (a.logprobs) a.logprobs[r] = 0.f;
+    }
+    return;
   }
   RowScale rs;
-  rs.top = m;
-  rs.m = (double)m;
-  rs.s = 1.4426950408889634074 / (double)temp;
-  rs.to_log2 = (float)fmin(rs.s, 3e38);
+  rs.set(m, temp);
 
   // ---- what top-k and top-p keep
   Cut cut = {-INFINITY, 0x7fffffff, 0};
-  bool found = false, used = false;
+  bool found = !cuts, used = false;
   if (by_count && k <= LIST) {      // by counts alone, if the first k and what shares the last one's bin are a list's worth
     for (int t = 0; t < TRIES && !found; ++t) {
       rs.to_bin = (float)fmin(rs.s * (BINS / (double)reach_of(t)), 3e38);
@@ -655,7 +690,6 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
     }
   }
   if (!found) {
-    bool counted = !by_count;
     for (int t = 0; t < TRIES && !found; ++t) {
       const bool last_try = t == TRIES - 1;
       rs.to_bin = (float)fmin(rs.s * (BINS / (double)reach_of(t)), 3e38);
@@ -665,14 +699,23 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
       }
       u64 beyond = 0;
       for (int i0 = tid; i0 < n; i0 += 4 * NT) {
-        float f[4];
+        float f[4], v[4];
         u64 w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = i0 + j * NT;
           const float l = i < n ? vals[i] : -INFINITY;
+          v[j] = l;
           f[j] = row_bin(l, rs);
-          if (by_mass) w[j] = row_weight(l, rs, sh->tab);
+        }
+        if (by_mass) {
+          if (rs.plain) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = plain_raw(v[j], rs, sh->tab) - RAW;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = called_weight(v[j], rs, &sh->tab);
+          }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -699,12 +742,13 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
         __syncthreads();
       }
       cut.mass = all;
-      if (by_count) counted = find_cut(row, mem, vals, n, base, rs, false, (u64)k, by_mass, cut);
-      if (!counted && !last_try) continue;      // (with fewer than k tokens in the last try's bins top-k keeps everything)
-      found = true;
-      if (by_mass) {
+      // top-k, then top-p in what it left
+      for (int what = by_count ? 0 : 1; what < 2; ++what) {
+        if (what && !by_mass) { found = true; break; }
         const double want = ceil((double)p * (double)cut.mass);
-        found = find_cut(row, mem, vals, n, base, rs, true, want >= 1.0 ? (u64)want : 1, true, cut);
+        const u64 goal = what == 0 ? (u64)k : want >= 1.0 ? (u64)want : 1;
+        found = find_cut(row, mem, vals, n, base, rs, what, goal, by_mass, cut);
+        if (!found && !(what == 0 && last_try)) break;      // (with fewer than k tokens in the last try's bins top-k keeps everything)
       }
     }
   }
@@ -721,6 +765,12 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   int i = first;
   float floor = cut.l;      // most are not kept
   if (by_least) floor = fmaxf(floor, least_floor(m, least, rs));
+  if (!cuts && !by_least && rs.plain) {
+    const int from = i;
+    for (; i + 4 <= last; i += 4)
+      mine += (plain_raw(vals[i], rs, sh->tab) + plain_raw(vals[i + 1], rs, sh->tab)) + (plain_raw(vals[i + 2], rs, sh->tab) + plain_raw(vals[i + 3], rs, sh->tab));
+    mine -= (u64)(i - from) * RAW;
+  }
   for (; i + 4 <= last; i += 4)
     if (fmaxf(fmaxf(vals[i], vals[i + 1]), fmaxf(vals[i + 2], vals[i + 3])) >= floor) mine += (weigh(i) + weigh(i + 1)) + (weigh(i + 2) + weigh(i + 3));
   for (; i < last; ++i) mine += weigh(i);
@@ -752,7 +802,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
 // takes in blocks of 512; a block's sum is kept, so that the draw goes over 512 tokens anew and no more.
 constexpr int ST_NT = 256, ST_NW = ST_NT / 32, ST_BLOCK = 512, ST_BLOCKS = 16;      // (a CTA has 65,536 logits at most)
 
-// Four numbers from index i on; -inf for NaN and from `end` on.
+// Four numbers from index i on; -inf from `end` on.  (NaN passes: a maximum and a comparison take no notice of it, and its weight is 0.)
 template <typename T> __device__ __forceinline__ void stream_read(const T* row, int i, int end, bool aligned, float (&v)[4]) {
   if (aligned && i + 4 <= end) {
     if constexpr (sizeof(T) == 4) {
@@ -766,8 +816,6 @@ template <typename T> __device__ __forceinline__ void stream_read(const T* row, 
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = i + j < end ? to_f32<T>(row[i + j]) : -INFINITY;
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = v[j] == v[j] ? v[j] + 0.f : -INFINITY;
 }
 
 // `beside`: the kernel before this one in the stream has the other rows (attention_shared_narrow.cuh has the argument): this one waits for it at its end.
@@ -779,15 +827,14 @@ __global__ void __launch_bounds__(ST_NT, 4) sample_stream_kernel(const T* logits
   RowOf<ST_NW> row = {sh, cluster_size(), cluster_rank(), 0};
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long r = blockIdx.x / row.ctas;
-  sh->tab.t[tid] = exp2(tid / (double)STEPS);
+  sh->tab.t[tid] = UNIT * exp2(tid / (double)STEPS);
   static_assert(STEPS == ST_NT, "a thread makes a step of the table");
   if (row.ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
   if (!beside) ifb_pdl_wait();
   ifb_pdl_trigger();
   auto draw = [&]() {
-    const float temp = a.temperature[r], u = a.uniform[r], p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
-    const int k = a.top_k ? a.top_k[r] : 0;
-    const bool greedy = !(temp > 0.f), mine = temp == temp && (greedy || !((k >= 1 && k < a.vocab) || p < 1.f));
+    const float temp = a.temperature[r], u = a.uniform[r], least = a.min_p ? a.min_p[r] : 0.f;
+    const bool greedy = !(temp > 0.f), mine = (temp == temp) & !has_cuts(a, r);
     if (row.ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // every peer has begun: its shared memory may be written
     if (!mine) return;
     const T* src = logits + r * a.pitch;
@@ -799,12 +846,18 @@ __global__ void __launch_bounds__(ST_NT, 4) sample_stream_kernel(const T* logits
       float v[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) stream_read<T>(src, i0 + j * 128 + lane * 4, end, aligned, v[j]);
+      if (greedy) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (v[j][e] > bv) { bv = v[j][e]; bi = i0 + j * 128 + lane * 4 + e; }
+          for (int e = 0; e < 4; ++e)
+            if (v[j][e] > bv) { bv = v[j][e]; bi = i0 + j * 128 + lane * 4 + e; }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bv = fmaxf(fmaxf(fmaxf(bv, v[j][0]), fmaxf(v[j][1], v[j][2])), v[j][3]);
+      }
     }
+    bv += 0.f;      // (-0 becomes 0; a largest one is no NaN)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
@@ -823,11 +876,7 @@ __global__ void __launch_bounds__(ST_NT, 4) sample_stream_kernel(const T* logits
       return;
     }
     RowScale rs;
-    rs.top = m;
-    rs.m = (double)m;
-    rs.s = 1.4426950408889634074 / (double)temp;
-    rs.to_log2 = (float)fmin(rs.s, 3e38);
-    rs.to_bin = 0.f;
+    rs.set(m, temp);
     const bool by_least = least > 0.f;
     const float floor = by_least ? least_floor(m, least, rs) : -INFINITY;
     auto weigh = [&](float l) -> u64 {
@@ -842,6 +891,12 @@ __global__ void __launch_bounds__(ST_NT, 4) sample_stream_kernel(const T* logits
 #pragma unroll
       for (int j = 0; j < 4; ++j) stream_read<T>(src, i0 + j * 128 + lane * 4, end, aligned, v[j]);
       u64 sum = 0;
+      if (rs.plain && !by_least) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sum += (plain_raw(v[j][0], rs, sh->tab) + plain_raw(v[j][1], rs, sh->tab)) + (plain_raw(v[j][2], rs, sh->tab) + plain_raw(v[j][3], rs, sh->tab));
+        sum -= 16 * RAW;
+      } else
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (!by_least || fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])) >= floor)
@@ -938,18 +993,22 @@ IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
   const void* kernel = dtype == IFB_F32 ? (const void*)sample_cut_kernel<float> : dtype == IFB_BF16 ? (const void*)sample_cut_kernel<bf16> : nullptr;
   if (!kernel) return IFB_ERR_DTYPE;
   auto slice = [&](int n) { return ((vocab + n - 1) / n + 7) & ~7; };
+  auto room_for = [&](int n) { return cut_clusters(kernel, dtype, n, (size_t)slice(n) * 4 + CUT_BYTES); };
   int ctas = 1;
   while (ctas < SURE_CLUSTER && slice(ctas) > SHARED_SLICE) ctas *= 2;
-  while (ctas < MAX_CLUSTER && vocab / ctas >= 2048) {
-    const int clusters = cut_clusters(kernel, dtype, ctas * 2, (size_t)slice(ctas * 2) * 4 + CUT_BYTES);
-    if (clusters < 0) return clusters;
-    if (rows > clusters) break;
+  int clusters = room_for(ctas);
+  while (ctas < MAX_CLUSTER && vocab / ctas >= 2048 && clusters >= 0) {
+    const int next = room_for(ctas * 2);
+    if (next < rows) break;
     ctas *= 2;
+    clusters = next;
   }
+  if (clusters < 0) return clusters;
+  const bool everything = rows <= clusters, cuts = everything || call->top_k || call->top_p;
   CutArgs a = {call->pitch, vocab, slice(ctas), call->temperature, call->top_k, call->top_p, call->min_p, call->uniform, call->out, call->logprobs};
-  auto go = [&](auto kernel, int n, int threads, size_t smem, auto... args) -> int {
+  auto go = [&](auto kernel, int count, int n, int threads, size_t smem, auto... args) -> int {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)rows * n);
+    cfg.gridDim = dim3((unsigned)count * n);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = call->stream;
@@ -966,18 +1025,17 @@ IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
     if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
     return IFB_OK;
   };
-  const bool cuts = call->top_k || call->top_p;
   if (cuts) {
     const size_t smem = (size_t)a.per * 4 + CUT_BYTES;
     int st;
     if (dtype == IFB_F32) {
       IFB_ALLOW_SMEM(sample_cut_kernel<float>, smem);
-      st = go(sample_cut_kernel<float>, ctas, NT, smem, (const float*)call->logits, a);
+      st = go(sample_cut_kernel<float>, rows, ctas, NT, smem, (const float*)call->logits, a, everything ? 1 : 0);
     } else {
       IFB_ALLOW_SMEM(sample_cut_kernel<bf16>, smem);
-      st = go(sample_cut_kernel<bf16>, ctas, NT, smem, (const bf16*)call->logits, a);
+      st = go(sample_cut_kernel<bf16>, rows, ctas, NT, smem, (const bf16*)call->logits, a, everything ? 1 : 0);
     }
-    if (st) return st;
+    if (st || everything) return st;
   }
   // the other rows: as many CTAs of a row as leave no SM idle, each with whole blocks for its warps
   const int sms = ifb_sm_count();
@@ -985,8 +1043,8 @@ IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
   auto stretch = [&](int ctas) { return ((vocab + ctas * ST_NW - 1) / (ctas * ST_NW) + ST_BLOCK - 1) / ST_BLOCK * ST_BLOCK; };
   while (n < SURE_CLUSTER && (stretch(n) > ST_BLOCKS * ST_BLOCK || ((long long)rows * n * 2 <= 8LL * sms && stretch(n) > 2 * ST_BLOCK))) n *= 2;
   a.per = stretch(n) * ST_NW;
-  return dtype == IFB_F32 ? go(sample_stream_kernel<float>, n, ST_NT, 0, (const float*)call->logits, a, cuts ? 1 : 0)
-                          : go(sample_stream_kernel<bf16>, n, ST_NT, 0, (const bf16*)call->logits, a, cuts ? 1 : 0);
+  return dtype == IFB_F32 ? go(sample_stream_kernel<float>, rows, n, ST_NT, 0, (const float*)call->logits, a, cuts ? 1 : 0)
+                          : go(sample_stream_kernel<bf16>, rows, n, ST_NT, 0, (const bf16*)call->logits, a, cuts ? 1 : 0);
 }
 
 // ---------------------------------------------------------------------------------------------------- log probabilities
