@@ -3,7 +3,7 @@
 
 // Bytes of room for a call's sums.
 IFB_EXPORT long long ifb_attention_shared_room(int n_tokens, int n_req, int n_groups, int kv_heads, int group, int dim) {
-  return parts_bytes(n_tokens) + room_bytes(sh_call(n_tokens, n_req, n_groups, kv_heads, group, EVERY), dim);
+  return parts_bytes(n_tokens) + room_bytes(sh_call(n_tokens, n_req, n_groups, kv_heads, group, dim, EVERY), dim);
 }
 
 // q [n_tokens, heads, dim] with rows `q_row` elements apart; pages [num_pages][2][kv_heads][page_size][dim], pages `page_stride` elements apart; out dense.
@@ -11,7 +11,7 @@ IFB_EXPORT int ifb_attention_shared(const Packed* call) {
   const Packed& a = *call;
   if (a.n_tokens <= 0 || a.n_req <= 0) return IFB_OK;
   if (const int st = check(a, SH_ROWS, 4)) return st;
-  Call c = sh_call(a.n_tokens, a.n_req, a.n_groups, a.kv_heads, a.heads / a.kv_heads, EVERY);
+  Call c = sh_call(a.n_tokens, a.n_req, a.n_groups, a.kv_heads, a.heads / a.kv_heads, a.dim, EVERY);
   fill(c, a);
   room_at(c, a.dim, (char*)a.room + parts_bytes(a.n_tokens));
   const float *q = (const float*)a.q, *pages = (const float*)a.pages;

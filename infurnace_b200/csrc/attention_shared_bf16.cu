@@ -29,7 +29,7 @@ static Call wide_call(bool tc, int n_tokens, int n_req, int n_groups, int kv_hea
 #if HEAD_DIM <= 128
   if (tc) return tc_call(n_tokens, n_req, n_groups, kv_heads, group, page_size);
 #endif
-  return sh_call(n_tokens, n_req, n_groups, kv_heads, group, WIDE);
+  return sh_call(n_tokens, n_req, n_groups, kv_heads, group, D, WIDE);
 }
 
 // Bytes of room for a call's sums at most, whichever kernels it takes.

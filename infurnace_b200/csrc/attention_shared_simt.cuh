@@ -171,13 +171,13 @@ __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_co
   }
 }
 
-static inline Call sh_call(int n_tokens, int n_req, int n_groups, int kv_heads, int group, Class which) {
+static inline Call sh_call(int n_tokens, int n_req, int n_groups, int kv_heads, int group, int dim, Class which) {
   Call c = {};
   c.which = which;
   c.n_tokens = n_tokens; c.n_req = n_req; c.n_groups = n_groups;
   c.kv_heads = kv_heads; c.heads = kv_heads * group;
   c.tokens = SH_ROWS / group; c.rows = SH_ROWS; c.unit_log = 5; c.align_log = 0;
-  c.workers = ifb_sm_count();
+  c.workers = ifb_sm_count() * (which == EVERY && dim <= 128 ? 2 : 1);      // (registers: two CTAs on an SM; beside narrow owners one)
   c.cost = 16;
   c.extra = 1;
   return c;

@@ -1069,10 +1069,22 @@ __device__ __forceinline__ LpSum lp_join(LpSum a, LpSum b) {
   else a.s += b.s;      // (0, or NaN)
   return a;
 }
-template <int N> __device__ __forceinline__ void lp_take(LpSum& t, const float (&v)[N]) {
+// Two numbers per instruction.
+__device__ __forceinline__ u64 lp_pair(float a, float b) { u64 r; asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void lp_unpair(u64 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ u64 lp_add2(u64 a, u64 b) { u64 r; asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ u64 lp_mul2(u64 a, u64 b) { u64 r; asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ float lp_max3(float a, float b, float c) { float y; asm("max.f32 %0, %1, %2, %3;\n" : "=f"(y) : "f"(a), "f"(b), "f"(c)); return y; }
+// N more numbers.  `count`: those of them at or above (AHEAD) or above `lt` are counted, which takes a look at the largest first.
+template <int N, bool AHEAD> __device__ __forceinline__ void lp_take(LpSum& t, const float (&v)[N], float lt, int& count) {
   float top = v[0];
 #pragma unroll
-  for (int j = 1; j < N; ++j) top = fmaxf(top, v[j]);
+  for (int j = 1; j + 1 < N; j += 2) top = lp_max3(top, v[j], v[j + 1]);
+  if (N % 2 == 0) top = fmaxf(top, v[N - 1]);
+  if (top >= lt) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) count += AHEAD ? v[j] >= lt : v[j] > lt;
+  }
   if (top > t.m) {
     t.s = t.m == -INFINITY ? t.s : (1.f + t.s) * lp_exp2((t.m - top) * LOG2E);
     t.m = top;
@@ -1084,12 +1096,23 @@ template <int N> __device__ __forceinline__ void lp_take(LpSum& t, const float (
       t.s += tie ? 0.f : lp_exp2((v[j] - top) * LOG2E);
     }
     t.s += (float)(ties - 1);
+  } else if (N % 4 == 0) {
+    const float m = t.m == -INFINITY ? 0.f : t.m;
+    const u64 minus = lp_pair(-m, -m), log2e = lp_pair(LOG2E, LOG2E);
+    u64 s[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      float a, b;
+      lp_unpair(lp_mul2(lp_add2(lp_pair(v[j], v[j + 1]), minus), log2e), a, b);
+      s[j / 2 & 1] = lp_add2(s[j / 2 & 1], lp_pair(lp_exp2(a), lp_exp2(b)));
+    }
+    float a, b;
+    lp_unpair(lp_add2(s[0], s[1]), a, b);
+    t.s += a + b;
   } else {
     const float m = t.m == -INFINITY ? 0.f : t.m;
-    float s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < N; ++j) s[j & 1] += lp_exp2((v[j] - m) * LOG2E);
-    t.s += s[0] + s[1];
+    for (int j = 0; j < N; ++j) t.s += lp_exp2((v[j] - m) * LOG2E);
   }
 }
 struct LpBox { LpSum sum; int count; int pad; };
@@ -1116,6 +1139,7 @@ __global__ void __launch_bounds__(LP_NT) token_logprob_kernel(const T* logits, l
   const int vecs = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? n / N : 0;
   // whole vectors ahead of the token, then those behind it
   auto run = [&](int from, int to, auto ahead) {
+    constexpr bool AHEAD = decltype(ahead)::value;
     constexpr int U = sizeof(T) == 4 ? 4 : 2;      // vectors at a time: 16 numbers
     int i = from + tid;
     for (; i + (U - 1) * LP_NT < to; i += U * LP_NT) {
@@ -1127,22 +1151,17 @@ __global__ void __launch_bounds__(LP_NT) token_logprob_kernel(const T* logits, l
 #pragma unroll
         for (int j = 0; j < N; ++j) v[u * N + j] = w[j];
       }
-      lp_take(sum, v);
-#pragma unroll
-      for (int j = 0; j < U * N; ++j) count += decltype(ahead)::value ? v[j] >= lt : v[j] > lt;
+      lp_take<U * N, AHEAD>(sum, v, lt, count);
     }
     for (; i < to; i += LP_NT) {
       float v[N];
       Vec16<T>::read(src + (size_t)i * N, v);
-      lp_take(sum, v);
-#pragma unroll
-      for (int j = 0; j < N; ++j) count += decltype(ahead)::value ? v[j] >= lt : v[j] > lt;
+      lp_take<N, AHEAD>(sum, v, lt, count);
     }
   };
   auto one = [&](int i) {
     const float v[1] = {to_f32<T>(src[i])};
-    lp_take(sum, v);
-    count += i < t ? v[0] >= lt : v[0] > lt;
+    if (i < t) lp_take<1, true>(sum, v, lt, count); else lp_take<1, false>(sum, v, lt, count);
   };
   const int split = min(vecs, t / N);
   run(0, split, std::true_type());
