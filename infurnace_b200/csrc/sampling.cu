@@ -1074,45 +1074,50 @@ __device__ __forceinline__ u64 lp_pair(float a, float b) { u64 r; asm("mov.b64 %
 __device__ __forceinline__ void lp_unpair(u64 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); }
 __device__ __forceinline__ u64 lp_add2(u64 a, u64 b) { u64 r; asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ u64 lp_mul2(u64 a, u64 b) { u64 r; asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ float lp_max3(float a, float b, float c) { float y; asm("max.f32 %0, %1, %2, %3;\n" : "=f"(y) : "f"(a), "f"(b), "f"(c)); return y; }
-// N more numbers.  `count`: those of them at or above (AHEAD) or above `lt` are counted, which takes a look at the largest first.
-template <int N, bool AHEAD> __device__ __forceinline__ void lp_take(LpSum& t, const float (&v)[N], float lt, int& count) {
-  float top = v[0];
+__device__ __forceinline__ float lp_min(float a, float b) { float y; asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(y) : "f"(a), "f"(b)); return y; }
+// A thread's running state: its largest number, and the sum of e^(l - ref) over all others.  ref is an earlier largest one, left as it is until the
+// largest is 40 above it: a running maximum that grows is then no branch of its own, which with 32 threads to a warp it was in nearly every step.
+struct LpRun { float m, s, ref; };
+// N more numbers (a power of two).  They are paired off: of two the smaller goes into the sum, the larger on to the next round, so that the sum is over all
+// but one of the largest without a subtraction; NaN goes into the sum.  `count`: those at or above (AHEAD) or above `lt` are counted, which
+// takes a look at the largest first.
+template <int N, bool AHEAD> __device__ __forceinline__ void lp_take(LpRun& t, const float (&v)[N], float lt, int& count) {
+  float up[N], out[N];
 #pragma unroll
-  for (int j = 1; j + 1 < N; j += 2) top = lp_max3(top, v[j], v[j + 1]);
-  if (N % 2 == 0) top = fmaxf(top, v[N - 1]);
-  if (top >= lt) {
+  for (int j = 0; j < N; ++j) up[j] = v[j];
+#pragma unroll
+  for (int n = N, k = 0; n > 1; n /= 2) {
+#pragma unroll
+    for (int j = 0; j < n / 2; ++j, ++k) {
+      out[k] = lp_min(up[2 * j], up[2 * j + 1]);
+      up[j] = fmaxf(up[2 * j], up[2 * j + 1]);
+    }
+  }
+  if (up[0] >= lt) {
 #pragma unroll
     for (int j = 0; j < N; ++j) count += AHEAD ? v[j] >= lt : v[j] > lt;
   }
-  if (top > t.m) {
-    t.s = t.m == -INFINITY ? t.s : (1.f + t.s) * lp_exp2((t.m - top) * LOG2E);
-    t.m = top;
-    int ties = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const bool tie = v[j] == top;
-      ties += tie;
-      t.s += tie ? 0.f : lp_exp2((v[j] - top) * LOG2E);
-    }
-    t.s += (float)(ties - 1);
-  } else if (N % 4 == 0) {
-    const float m = t.m == -INFINITY ? 0.f : t.m;
-    const u64 minus = lp_pair(-m, -m), log2e = lp_pair(LOG2E, LOG2E);
+  out[N - 1] = lp_min(t.m, up[0]);
+  t.m = fmaxf(t.m, up[0]);
+  if (t.m > t.ref + 40.f) {      // (at first, too)
+    t.s *= lp_exp2((t.ref - t.m) * LOG2E);
+    t.ref = t.m;
+  }
+  const float ref = t.ref == -INFINITY ? 0.f : t.ref;
+  if (N > 1) {
+    const u64 minus = lp_pair(-ref, -ref), log2e = lp_pair(LOG2E, LOG2E);
     u64 s[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
       float a, b;
-      lp_unpair(lp_mul2(lp_add2(lp_pair(v[j], v[j + 1]), minus), log2e), a, b);
+      lp_unpair(lp_mul2(lp_add2(lp_pair(out[j], out[(j + 1) % N]), minus), log2e), a, b);
       s[j / 2 & 1] = lp_add2(s[j / 2 & 1], lp_pair(lp_exp2(a), lp_exp2(b)));
     }
     float a, b;
     lp_unpair(lp_add2(s[0], s[1]), a, b);
     t.s += a + b;
   } else {
-    const float m = t.m == -INFINITY ? 0.f : t.m;
-#pragma unroll
-    for (int j = 0; j < N; ++j) t.s += lp_exp2((v[j] - m) * LOG2E);
+    t.s += lp_exp2((out[0] - ref) * LOG2E);
   }
 }
 struct LpBox { LpSum sum; int count; int pad; };
@@ -1134,7 +1139,7 @@ __global__ void __launch_bounds__(LP_NT) token_logprob_kernel(const T* logits, l
   const T* src = row + base;
   const int t = max(0, min(n, token - base));      // numbers of this slice ahead of the token
   constexpr int N = Vec16<T>::N;
-  LpSum sum = {-INFINITY, 0.f};
+  LpRun own = {-INFINITY, 0.f, -INFINITY};
   int count = 0;
   const int vecs = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? n / N : 0;
   // whole vectors ahead of the token, then those behind it
@@ -1151,23 +1156,24 @@ __global__ void __launch_bounds__(LP_NT) token_logprob_kernel(const T* logits, l
 #pragma unroll
         for (int j = 0; j < N; ++j) v[u * N + j] = w[j];
       }
-      lp_take<U * N, AHEAD>(sum, v, lt, count);
+      lp_take<U * N, AHEAD>(own, v, lt, count);
     }
     for (; i < to; i += LP_NT) {
       float v[N];
       Vec16<T>::read(src + (size_t)i * N, v);
-      lp_take<N, AHEAD>(sum, v, lt, count);
+      lp_take<N, AHEAD>(own, v, lt, count);
     }
   };
   auto one = [&](int i) {
     const float v[1] = {to_f32<T>(src[i])};
-    if (i < t) lp_take<1, true>(sum, v, lt, count); else lp_take<1, false>(sum, v, lt, count);
+    if (i < t) lp_take<1, true>(own, v, lt, count); else lp_take<1, false>(own, v, lt, count);
   };
   const int split = min(vecs, t / N);
   run(0, split, std::true_type());
   if (split < vecs && tid < N) one(split * N + tid);      // the vector that the token may be in
   run(split + 1, vecs, std::false_type());
   for (int i = vecs * N + tid; i < n; i += LP_NT) one(i);
+  LpSum sum = {own.m, own.m == -INFINITY ? own.s : own.s * lp_exp2((own.ref - own.m) * LOG2E)};
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const LpSum x = {__shfl_xor_sync(0xffffffffu, sum.m, o), __shfl_xor_sync(0xffffffffu, sum.s, o)};
