@@ -155,7 +155,7 @@ struct CutShared {
   Exchange swap[2][MAX_CLUSTER];        // what the CTAs of a row tell each other, in turn
   u64 warp_a[NW], warp_b[NW];
   u64 found[4];
-  uint32_t listed;
+  uint32_t listed[2], own, own_at;      // members of the row's lists, of this CTA's and where these begin
 };
 
 __device__ __forceinline__ u64 warp_add(u64 v) {
@@ -296,7 +296,7 @@ struct CutMemory {      // of a CTA, behind its slice of the row
   uint32_t* count; uint32_t* lo; uint32_t* hi;             // its own bins [BINS + 1] each
   uint32_t* row_count; u64* row_mass;                      // the row's bins [BINS + 1]
   uint32_t* sub_count; u64* sub_mass;                      // the row's parts of a bin [SUBS]
-  u64* list_mass; float* list_l; uint32_t* list_i;         // the members of a bin [LIST]
+  u64* list;                                               // the members of a bin, for top-k and for top-p [2][LIST]: the logit in order, and behind it the index turned over
 };
 constexpr size_t CUT_BYTES = 16 + (size_t)(BINS + 1) * 24 + (size_t)SUBS * 12 + (size_t)LIST * 16;      // (16: the slice begins up to 3 numbers in)
 
@@ -306,9 +306,90 @@ __device__ __forceinline__ void add_mass(uint32_t* lo, uint32_t* hi, int b, u64 
   if (up) atomicAdd(hi + b, up);
 }
 
+// The members that `in` tells by their bin, at most LIST of them in the row, to every CTA's list `which`, in one order for all.  (A CTA notes its own, in the place
+// of its bins' counts, which are merged, and takes room for all of them at once: an addition over the cluster for each member took longer than all the rest.)
+template <class In>
+__device__ __forceinline__ void gather(const Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, int which, In in) {
+  CutShared* sh = row.sh;
+  uint32_t* own = mem.count;
+  for (int i0 = threadIdx.x; i0 < n; i0 += 4 * NT) {
+    bool is[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) is[j] = i0 + j * NT < n && in(row_bin(vals[i0 + j * NT], rs));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (is[j]) {
+        const uint32_t at = atomicAdd(&sh->own, 1u);
+        if (at < LIST) own[at] = i0 + j * NT;      // (always: they were counted)
+      }
+  }
+  __syncthreads();
+  const int count = min(sh->own, (uint32_t)LIST);
+  if (threadIdx.x == 0 && count) sh->own_at = add_peer(&sh->listed[which], 0, count);
+  __syncthreads();
+  if (threadIdx.x == 0) sh->own = 0;
+  for (int j = threadIdx.x; j < count * row.ctas; j += NT) {
+    const uint32_t i = own[j / row.ctas], at = sh->own_at + j / row.ctas;
+    if (at < LIST) put_u64(mem.list + which * LIST + at, j % row.ctas, ((u64)ordered(vals[i]) << 32) | (uint32_t)~(base + i));
+  }
+  row_sync(row.ctas);
+  // for the next list of this kind, which comes after another barrier of the row (as the next writes to this list do)
+  if (row.rank == 0 && threadIdx.x == 0) sh->listed[which] = 0;
+}
+// A list in order, the best first: the thread's member, and 0 beyond the last.  A bitonic network, within a warp by shuffles, between warps through the list and
+// the place `other` in turn.  (To count for each member what comes before it took 13 us for 512 of them.)
+__device__ __forceinline__ u64 sorted_member(u64* list, u64* other, int members) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  u64 x = tid < members ? list[tid] : 0;
+  const bool some = (tid & ~31) < members;      // (a warp without members has zeros until others' come in)
+  auto step = [&](int j, bool falling) {
+    const u64 y = __shfl_xor_sync(0xffffffffu, x, j);
+    if ((((lane & j) == 0) == falling) == (y > x)) x = y;
+  };
+  if (some) {
+#pragma unroll
+    for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+      for (int j = k / 2; j > 0; j /= 2) step(j, (tid & k) == 0);
+  }
+  for (int k = 64; k / 2 < members; k *= 2) {
+    const bool falling = (tid & k) == 0;
+    for (int j = k / 2; j >= 32; j /= 2) {
+      other[tid] = x;
+      __syncthreads();
+      const u64 y = other[tid ^ j];
+      if ((((tid & j) == 0) == falling) == (y > x)) x = y;
+      u64* t = list; list = other; other = t;
+    }
+#pragma unroll
+    for (int j = 16; j > 0; j /= 2) step(j, falling);
+  }
+  return x;
+}
+// The sum of v over this thread and those of the CTA before it.
+__device__ __forceinline__ u64 running_sum(CutShared* sh, u64 v) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const u64 x = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += x; }
+  __syncthreads();
+  if (lane == 31) sh->warp_a[warp] = v;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) v += sh->warp_a[w];
+  return v;
+}
+// The cut at the member that one thread holds, to all threads of the CTA.
+__device__ __forceinline__ void tell_cut(CutShared* sh, bool last, u64 member, u64 mass, Cut& cut) {
+  if (last) { sh->found[0] = member; sh->found[1] = mass; }
+  __syncthreads();
+  cut.l = unordered((uint32_t)(sh->found[0] >> 32));
+  cut.i = (int)~(uint32_t)sh->found[0];
+  cut.mass = sh->found[1];
+  __syncthreads();
+}
+
 // The cut through the row's bins after which `goal` tokens (by_mass: at least `goal` of weight) are kept.  False: it does not run through them.
 __device__ __forceinline__ bool find_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, bool by_mass, u64 goal, bool weighted,
-                         Cut& cut) {
+                         int key_shift, Cut& cut) {
   CutShared* sh = row.sh;
   u64 bc, bm;
   const int b0 = find_bin(sh, BINS, mem.row_count, mem.row_mass, by_mass, goal, bc, bm, weighted);
@@ -338,70 +419,21 @@ __device__ __forceinline__ bool find_cut(Row& row, const CutMemory& mem, const f
     return f < BINS && (int)f == b0 && (b1 < 0 || (int)((f - b0) * SUBS) == b1);
   };
   if (members <= LIST) {
-    u64* lw = mem.list_mass;
-    float* ll = mem.list_l;
-    uint32_t* li = mem.list_i;
     const float f0 = b1 < 0 ? (float)b0 : b0 + b1 * (1.f / SUBS), f1 = b1 < 0 ? b0 + 1.f : b0 + (b1 + 1) * (1.f / SUBS);      // (exact)
-    for (int i0 = threadIdx.x; i0 < n; i0 += 4 * NT) {
-      bool in[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float f = i0 + j * NT < n ? row_bin(vals[i0 + j * NT], rs) : INFINITY;
-        in[j] = f >= f0 && f < f1;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!in[j]) continue;
-        const int i = i0 + j * NT;
-        const float l = vals[i];
-        const uint32_t at = add_peer(&sh->listed, 0, 1u);      // (0 whenever a list begins: set before the kernel's first barrier and by the one who reads it)
-        if (at >= LIST) continue;      // (never: the members were counted)
-        put_u64(lw + at, 0, weighted ? row_weight(l, rs, sh->tab) : 0);
-        put_u32(reinterpret_cast<uint32_t*>(ll) + at, 0, __float_as_uint(l));
-        put_u32(li + at, 0, (uint32_t)(base + i));
-      }
-    }
-    row_sync(row.ctas);
-    if (row.rank == 0) {
-      if (threadIdx.x == 0) sh->listed = 0;
-      const int sub = threadIdx.x & 3;      // four threads count what comes before a member
-      for (int i0 = 0; i0 < (int)members; i0 += NT / 4) {
-        const int i = i0 + (int)(threadIdx.x >> 2);
-        const bool in = i < (int)members;
-        const float l = in ? ll[i] : INFINITY;
-        const uint32_t idx = in ? li[i] : 0;
-        u64 pos = 0, mass = 0;
-#pragma unroll 4
-        for (int j = sub; j < (int)members; j += 4) {
-          const float other = ll[j];
-          const bool first = other > l || (other == l && li[j] < idx);
-          pos += first;
-          mass += first ? lw[j] : 0;
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) { pos += __shfl_xor_sync(0xffffffffu, pos, o); mass += __shfl_xor_sync(0xffffffffu, mass, o); }
-        pos += bc; mass += bm;
-        if (!in || sub) continue;
-        const u64 at = by_mass ? mass : pos, next = at + (by_mass ? lw[i] : 1);
-        if (at < goal && (next >= goal || pos + 1 == bc + members)) {
-          for (int r = 0; r < row.ctas; ++r) {
-            put_u64(&sh->found[0], r, ((u64)__float_as_uint(l) << 32) | idx);
-            put_u64(&sh->found[1], r, mass + lw[i]);
-          }
-        }
-      }
-    }
-    row_sync(row.ctas);
-    cut.l = __uint_as_float((uint32_t)(sh->found[0] >> 32));
-    cut.i = (int)(uint32_t)sh->found[0];
-    cut.mass = sh->found[1];
-    __syncthreads();
+    gather(row, mem, vals, n, base, rs, by_mass, [&](float f) { return f >= f0 && f < f1; });
+    const int i = threadIdx.x;
+    const u64 member = sorted_member(mem.list + by_mass * LIST, reinterpret_cast<u64*>(mem.count), (int)members);
+    const bool in = i < (int)members;
+    const u64 w = in && weighted ? row_weight(unordered((uint32_t)(member >> 32)), rs, sh->tab) : 0;
+    const u64 mass = bm + (weighted ? running_sum(sh, w) : 0), next = by_mass ? mass : bc + i + 1, at = by_mass ? mass - w : bc + i;
+    tell_cut(sh, in && at < goal && (next >= goal || i + 1 == (int)members), member, mass, cut);
     return true;
   }
   // Many members within a hundred-thousandth of a factor of two: the smallest key above which less than the goal lies, by halving, then its ties in order.
+  // (`key_shift`: of 16-bit logits the upper half says all, and members often have one value or a few: one row of 151,935 52 to 30 us.)
   u64 top = 0, low = ALL;
   for (int i = threadIdx.x; i < n; i += NT)
-    if (member(vals[i])) { const u64 k = ordered(vals[i]); top = top > k ? top : k; low = low < k ? low : k; }
+    if (member(vals[i])) { const u64 k = ordered(vals[i]) >> key_shift; top = top > k ? top : k; low = low < k ? low : k; }
   row.extremes(top, low);
   auto above = [&](u64 key, u64& c, u64& w, u64& ties) {      // what lies above a key among the members, and before them
     c = w = 0;
@@ -409,7 +441,7 @@ __device__ __forceinline__ bool find_cut(Row& row, const CutMemory& mem, const f
     for (int i = threadIdx.x; i < n; i += NT) {
       const float l = vals[i];
       if (!member(l)) continue;
-      const u64 k = ordered(l);
+      const u64 k = ordered(l) >> key_shift;
       if (k > key) { ++c; if (weighted) w += row_weight(l, rs, sh->tab); }
       t += k == key;
     }
@@ -424,7 +456,8 @@ __device__ __forceinline__ bool find_cut(Row& row, const CutMemory& mem, const f
     if ((by_mass ? w : c) < goal) top = mid; else low = mid + 1;
   }
   above(top, c, w, ties);
-  cut.l = unordered((uint32_t)top);
+  const uint32_t whole = (uint32_t)top << key_shift;
+  cut.l = unordered(whole >> 31 ? whole : whole | ((1u << key_shift) - 1));      // (a negative number's bits are turned over)
   const u64 each = weighted ? row_weight(cut.l, rs, sh->tab) : 0;
   u64 take = by_mass ? (each ? (goal - w + each - 1) / each : ties) : goal - c;
   if (take > ties) take = ties;
@@ -449,83 +482,20 @@ __device__ __forceinline__ bool find_cut(Row& row, const CutMemory& mem, const f
 __device__ __forceinline__ void list_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, int last_bin, uint32_t members, uint32_t k,
                          float p, Cut& cut) {
   CutShared* sh = row.sh;
-  u64* lw = mem.list_mass;
-  float* ll = mem.list_l;
-  uint32_t* li = mem.list_i;
   const float f1 = last_bin + 1.f;
-  for (int i0 = threadIdx.x; i0 < n; i0 += 4 * NT) {
-    bool in[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) in[j] = i0 + j * NT < n && row_bin(vals[i0 + j * NT], rs) < f1;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (!in[j]) continue;
-      const int i = i0 + j * NT;
-      const uint32_t at = add_peer(&sh->listed, 0, 1u);
-      if (at >= LIST) continue;      // (never: the members were counted)
-      put_u64(lw + at, 0, row_weight(vals[i], rs, sh->tab));
-      put_u32(reinterpret_cast<uint32_t*>(ll) + at, 0, __float_as_uint(vals[i]));
-      put_u32(li + at, 0, (uint32_t)(base + i));
-    }
-  }
-  row_sync(row.ctas);
-  if (row.rank == 0) {
-    if (threadIdx.x == 0) sh->listed = 0;
-    const int sub = threadIdx.x & 3, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;      // four threads count what comes before a member
-    uint32_t pos[LIST * 4 / NT];
-    u64 before[LIST * 4 / NT], kept_mass = 0;
-#pragma unroll
-    for (int t = 0; t < LIST * 4 / NT; ++t) {
-      const int i = t * (NT / 4) + (int)(threadIdx.x >> 2);
-      if (t * (NT / 4) >= (int)members) break;
-      const bool in = i < (int)members;
-      const float l = in ? ll[i] : INFINITY;
-      const uint32_t idx = in ? li[i] : 0;
-      uint32_t c = 0;
-      u64 w = 0;
-#pragma unroll 4
-      for (int j = sub; j < (int)members; j += 4) {
-        const float other = ll[j];
-        const bool first = other > l || (other == l && li[j] < idx);
-        c += first;
-        w += first ? lw[j] : 0;
-      }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) { c += __shfl_xor_sync(0xffffffffu, c, o); w += __shfl_xor_sync(0xffffffffu, w, o); }
-      pos[t] = in ? c : 0xffffffffu;
-      before[t] = w;
-      if (in && sub == 0 && c < k) kept_mass += lw[i];
-    }
-    kept_mass = warp_add(kept_mass);
+  gather(row, mem, vals, n, base, rs, 0, [&](float f) { return f < f1; });
+  const uint32_t i = threadIdx.x, most = members < k ? members : k;
+  const u64 member = sorted_member(mem.list, reinterpret_cast<u64*>(mem.count), (int)members);
+  const u64 w = i < most ? row_weight(unordered((uint32_t)(member >> 32)), rs, sh->tab) : 0, mass = running_sum(sh, w);
+  u64 goal = ALL;
+  if (p < 1.f) {
     __syncthreads();
-    if (lane == 0) sh->warp_a[warp] = kept_mass;
+    if (i + 1 == most) sh->warp_a[0] = mass;
     __syncthreads();
-    kept_mass = 0;
-    for (int v = 0; v < NW; ++v) kept_mass += sh->warp_a[v];
-    u64 goal = ALL;
-    if (p < 1.f) {
-      const double want = ceil((double)p * (double)kept_mass);
-      goal = want >= 1.0 ? (u64)want : 1;
-    }
-    const uint32_t most = members < k ? members : k;
-#pragma unroll
-    for (int t = 0; t < LIST * 4 / NT; ++t) {
-      const int i = t * (NT / 4) + (int)(threadIdx.x >> 2);
-      if (t * (NT / 4) >= (int)members) break;
-      if (sub || pos[t] >= most || before[t] >= goal) continue;
-      if (pos[t] + 1 == most || before[t] + lw[i] >= goal) {      // the last that is kept
-        for (int r = 0; r < row.ctas; ++r) {
-          put_u64(&sh->found[0], r, ((u64)__float_as_uint(ll[i]) << 32) | li[i]);
-          put_u64(&sh->found[1], r, before[t] + lw[i]);
-        }
-      }
-    }
+    const double want = ceil((double)p * (double)sh->warp_a[0]);
+    goal = want >= 1.0 ? (u64)want : 1;
   }
-  row_sync(row.ctas);
-  cut.l = __uint_as_float((uint32_t)(sh->found[0] >> 32));
-  cut.i = (int)(uint32_t)sh->found[0];
-  cut.mass = sh->found[1];
-  __syncthreads();
+  tell_cut(sh, i < most && mass - w < goal && (i + 1 == most || mass >= goal), member, mass, cut);      // the last that is kept
 }
 
 template <typename T> struct Vec16;
@@ -583,10 +553,8 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   CutMemory mem;
   mem.row_mass = reinterpret_cast<u64*>(cut_smem + 16 + (size_t)((a.per + 3) & ~3) * 4);
   mem.sub_mass = mem.row_mass + BINS + 1;
-  mem.list_mass = mem.sub_mass + SUBS;
-  mem.list_l = reinterpret_cast<float*>(mem.list_mass + LIST);
-  mem.list_i = reinterpret_cast<uint32_t*>(mem.list_l + LIST);
-  mem.count = mem.list_i + LIST;
+  mem.list = mem.sub_mass + SUBS;
+  mem.count = reinterpret_cast<uint32_t*>(mem.list + 2 * LIST);
   mem.lo = mem.count + BINS + 1;
   mem.hi = mem.lo + BINS + 1;
   mem.row_count = mem.hi + BINS + 1;
@@ -600,7 +568,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   const float temp = a.temperature[r], u = a.uniform[r], p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
   const int k = a.top_k ? a.top_k[r] : 0;
   if (tid < STEPS) sh->tab.t[tid] = UNIT * exp2(tid / (double)STEPS);
-  if (tid == 0) sh->listed = 0;
+  if (tid == 0) sh->listed[0] = sh->listed[1] = sh->own = 0;
   for (int b = tid; b <= BINS; b += NT) mem.count[b] = mem.lo[b] = mem.hi[b] = 0;
   bool by_count = k >= 1 && k < a.vocab;
   const bool by_mass = p < 1.f, by_least = least > 0.f, cuts = by_count | by_mass;
@@ -746,7 +714,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
         if (what && !by_mass) { found = true; break; }
         const double want = ceil((double)p * (double)cut.mass);
         const u64 goal = what == 0 ? (u64)k : want >= 1.0 ? (u64)want : 1;
-        found = find_cut(row, mem, vals, n, base, rs, what, goal, by_mass, cut);
+        found = find_cut(row, mem, vals, n, base, rs, what, goal, by_mass, sizeof(T) == 2 ? 16 : 0, cut);
         if (!found && !(what == 0 && last_try)) break;      // (with fewer than k tokens in the last try's bins top-k keeps everything)
       }
     }
