@@ -738,8 +738,16 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
       mine += (plain_raw(vals[i], rs, sh->tab) + plain_raw(vals[i + 1], rs, sh->tab)) + (plain_raw(vals[i + 2], rs, sh->tab) + plain_raw(vals[i + 3], rs, sh->tab));
     mine -= (u64)(i - from) * RAW;
   }
+  const bool quick = !by_least && rs.plain;
   for (; i + 4 <= last; i += 4)
-    if (fmaxf(fmaxf(vals[i], vals[i + 1]), fmaxf(vals[i + 2], vals[i + 3])) >= floor) mine += (weigh(i) + weigh(i + 1)) + (weigh(i + 2) + weigh(i + 3));
+    if (fmaxf(fmaxf(vals[i], vals[i + 1]), fmaxf(vals[i + 2], vals[i + 3])) >= floor) {
+      if (quick) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine += kept(vals[i + j], base + i + j, cut) ? plain_raw(vals[i + j], rs, sh->tab) - RAW : 0;
+      } else {
+        mine += (weigh(i) + weigh(i + 1)) + (weigh(i + 2) + weigh(i + 3));
+      }
+    }
   for (; i < last; ++i) mine += weigh(i);
   const u64 at = row.before(mine, total);
   const u64 goal = draw_goal(u, total);
