@@ -166,6 +166,36 @@ def test_a_row_does_not_depend_on_the_others(K, vocab):
         assert part[0] == [whole[0][i] for i in rows] and part[1] == [whole[1][i] for i in rows]
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_a_high_temperature_puts_many_values_into_a_part_of_a_bin(K, sign, dtype):
+    """Thousands of tokens of some hundred neighbouring values: found by halving, of 16-bit logits by their upper halves."""
+    g = torch.Generator().manual_seed(12)
+    x = (sign * (3.0 + torch.randint(0, 128, (8, 40000), generator=g).float() / 128)).to(dtype)
+    u = torch.rand(8, generator=g).tolist()
+    check(K, x, [1e4, 3e4, 1e5, 1e4] * 2, u, [0, 30001, 0, 777, 39999, 0, 20000, 1], [0.5, 1.0, 0.97, 0.6, 0.3, 0.0, 1.0, 0.2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,offset", [(3, 1), (20001, 0), (20002, 3), (20003, 6)])
+def test_many_rows_without_cuts_that_begin_anywhere(K, vocab, offset, dtype):
+    """More rows than find room at once: the kernel that keeps none of a row, from every place within 16 bytes."""
+    rows = 320
+    wide = torch.full((rows, vocab + 7 + vocab % 2), 50.0).to(dtype)      # an odd pitch; what lies beside a row is larger than all of it
+    wide[:, offset:offset + vocab] = logits_of(rows, vocab, 13, dtype)
+    held = wide.cuda()[:, offset:offset + vocab]
+    u = torch.rand(rows, generator=torch.Generator().manual_seed(14)).tolist()
+    t = [(0.0, 0.8, 1.0, 2.5)[r % 4] for r in range(rows)]
+    tokens, logprobs = draw(K, held, t, u)
+    narrow, least = draw(K, held, t, u, least=[0.05 * (r % 3) for r in range(rows)])
+    f32 = lambda x: float(torch.tensor(x, dtype=torch.float32))
+    for r in range(rows):
+        for got, scores, min_p in ((tokens, logprobs, 0.0), (narrow, least, f32(0.05 * (r % 3)))):
+            want, logprob = sample_row(wide[r, offset:offset + vocab], f32(t[r]), f32(u[r]), 0, 1.0, min_p)
+            assert got[r] == want, r
+            assert abs(scores[r] - logprob) <= 2.0 ** -24 * abs(logprob) + 2.0 ** -45 * vocab
+
+
 def test_no_rows_is_nothing(K):
     assert draw(K, torch.zeros((0, 10)), [], [], [], [], []) == ([], [])
     empty = torch.empty(0, device="cuda")
