@@ -45,6 +45,8 @@ struct Call {
   int heads, kv_heads;
   int table_pages, page_size, window;
   float scale_log2;
+  const void *q, *pages;                 // as they are given: rows `q_row` elements apart
+  long long q_row;
   void* out;                             // [n_tokens, heads, dim]
   int4* parts;                           // [n_tokens]: where a row's pieces are (RowParts)
   int* err;
@@ -311,7 +313,9 @@ struct Walk {
     return make_int2((int)(((a + c.extra + 1) * workers - 1) / total), (int)((b * workers - 1) / total));
   }
 };
-// Whether a piece is all that its rows have (`at`: its item's workers): it is written out where it is worked on.
+// Whether a piece is all that its rows have (`at`: its item's workers): it is written out where it is worked on.  Where something of it is not finite, its item's
+// last worker gets ANEW.
+constexpr int ANEW = 1 << 30;
 __device__ __forceinline__ bool is_sole(const Piece& p, int2 at) { return !p.w.group && p.w.lo == 0 && at.x == at.y; }
 
 // The position of a query row of an owner: of a group's row by its request.
@@ -367,6 +371,90 @@ __device__ inline void write_parts(const Call& wide, const Call& narrow, const P
   }
 }
 
+// ---------------------------------------------------------------------------------------------------- rows worked out anew
+// A token's row of one head, key by key over those that it sees, in two passes (maximum, sums): for rows that come out infinite or NaN.  In a matrix product a
+// value that some rows of a tile see and others do not meets a weight of zero in these, and a weight's second term of zero in those: where the value is
+// infinite or NaN the product is NaN.  All lanes of a warp call it; a lane has a key of 32 for the scores, and the join's columns for the sums.
+template <typename T> __device__ __forceinline__ float dot16(const T* a, const T* b);      // of 16 bytes
+template <> __device__ __forceinline__ float dot16<float>(const float* a, const float* b) {
+  const float4 x = *reinterpret_cast<const float4*>(a), y = *reinterpret_cast<const float4*>(b);
+  return fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, x.w * y.w)));
+}
+template <> __device__ __forceinline__ float dot16<__nv_bfloat16>(const __nv_bfloat16* a, const __nv_bfloat16* b) {
+  const uint4 x = *reinterpret_cast<const uint4*>(a), y = *reinterpret_cast<const uint4*>(b);
+  const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s = fmaf(__uint_as_float(u[i] << 16), __uint_as_float(v[i] << 16), s);
+    s = fmaf(__uint_as_float(u[i] & 0xffff0000u), __uint_as_float(v[i] & 0xffff0000u), s);
+  }
+  return s;
+}
+template <typename T> __device__ __noinline__ void row_anew(const Call& c, int token, int head, int dim) {
+  const int lane = threadIdx.x & 31, N = c.n_groups, R = c.n_req, kv_head = head / (c.heads / c.kv_heads);
+  const int most = (int)min((long long)c.table_pages * c.page_size, 0x7fffff00LL);
+  auto row = [&](int i) { return clamp(c.cu_q[i], 0, c.n_tokens); };
+  auto member = [&](int i) { return clamp(c.cu_groups[i], 0, R); };
+  // as make_plan and write_parts have it: the request, its position, and the keys that it has from its group's first
+  int lo = 0, hi = R;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (max(row(mid), row(mid + 1)) <= token) lo = mid + 1; else hi = mid;
+  }
+  if (lo >= R) return;
+  const int r = lo, len = clamp(c.seq_lens[r], 0, most), pos = len - (max(row(r), row(r + 1)) - token);
+  int first = r, split = 0;
+  if (N > 0 && r >= member(0) && r < member(N)) {
+    int a = 0, b = N - 1;
+    while (a < b) {
+      const int mid = (a + b + 1) >> 1;
+      if (member(mid) <= r) a = mid; else b = mid - 1;
+    }
+    first = member(a);
+    split = clamp(c.shared_lens[a], 0, most);
+  }
+  const int key_lo = c.window > 0 ? max(0, pos - c.window + 1) : 0, key_hi = min(len, pos + 1);
+  const T* q = reinterpret_cast<const T*>(c.q) + token * c.q_row + (long long)head * dim;
+  const T* pages = reinterpret_cast<const T*>(c.pages);
+  const long long values = (long long)c.kv_heads * c.page_size * dim;
+  auto score = [&](int key, long long& at) {      // (what is no page of the pool is zeros)
+    at = page_at(c, key < split ? first : r, key / c.page_size);
+    if (at < 0) return 0.f;
+    at += ((long long)kv_head * c.page_size + key % c.page_size) * dim;
+    float s = 0.f;
+    for (int d = 0; d < dim; d += 16 / (int)sizeof(T)) s += dot16<T>(q + d, pages + at + d);
+    return s * c.scale_log2;
+  };
+  float m = -INFINITY, den = 0.f, sums[8] = {};      // columns 4 lane .. 4 lane + 3, and those 128 on
+  long long at;
+  for (int key = key_lo + lane; key < key_hi; key += 32) m = fmaxf(m, score(key, at));
+  m = warp_max(m);
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int key0 = key_lo; key0 < key_hi && den == den; key0 += 32) {
+    at = -1;
+    const float weight = key0 + lane < key_hi ? exp2f(score(key0 + lane, at) - ref) : 0.f;
+    den += warp_sum(weight);
+    for (int j = 0; j < min(32, key_hi - key0); ++j) {
+      const float g = __shfl_sync(0xffffffffu, weight, j);
+      const long long from = __shfl_sync(0xffffffffu, at, j);
+      if (from < 0) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int col = (i >> 2) * 128 + lane * 4 + (i & 3);
+        if (col < dim) sums[i] = fmaf(g, to_f32<T>(pages[from + values + col]), sums[i]);
+      }
+    }
+  }
+  const float inv = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den;      // (NaN stays)
+  T* dst = reinterpret_cast<T*>(c.out) + ((long long)token * c.heads + head) * dim;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int col = (i >> 2) * 128 + lane * 4 + (i & 3);
+    if (col < dim) dst[col] = from_f32<T>(sums[i] * inv);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------- the join
 // A warp takes a head of a token; a lane has the columns from 4 lane on (WIDTH 2, heads over 128: and from 128 + 4 lane on).  `wide` and `narrow`: the classes' calls (the same one where
 // there is one kernel only).  Lane x first has piece x: its maximum and denominator, from which the factor that its sums get.
@@ -389,7 +477,14 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
     if (item < kv_head) continue;
     const Call& c = how & NARROW_PART ? narrow : wide;
     const int2 workers = c.pieces[item];
-    if (how & SOLE_PART && workers.x == workers.y) return;      // it is written already
+    if (how & SOLE_PART && workers.x == (workers.y & ~ANEW)) {      // it is written already
+      if (workers.y == workers.x) return;
+      const T* row = reinterpret_cast<const T*>(wide.out) + ((long long)token * wide.heads + head) * dim;
+      float finite = 0.f;
+      for (int col = lane; col < dim; col += 32) finite = fmaf(to_f32<T>(row[col]), 0.f, finite);
+      if (__any_sync(0xffffffffu, finite != finite)) row_anew<T>(wide, token, head, dim);
+      return;
+    }
     first[k] = clamp(workers.x, 0, c.workers - 1);
     count[k] = clamp(workers.y, 0, c.workers - 1) - first[k] + 1;
     rows[k] = c.rows;
@@ -447,6 +542,14 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
     }
   }
   const float inv = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den;      // (NaN stays)
+  float finite = 0.f;      // NaN: not all sums are
+#pragma unroll
+  for (int j = 0; j < WIDTH; ++j)
+    if (j * 128 + lane * 4 < dim) finite += acc[j].x * 0.f + acc[j].y * 0.f + (acc[j].z * 0.f + acc[j].w * 0.f);
+  if (__any_sync(0xffffffffu, finite != finite)) {
+    row_anew<T>(wide, token, head, dim);
+    return;
+  }
   T* dst = reinterpret_cast<T*>(wide.out) + ((long long)token * wide.heads + head) * dim;
 #pragma unroll
   for (int j = 0; j < WIDTH; ++j) {
@@ -480,6 +583,7 @@ static inline void fill(Call& c, const Packed& a) {
   c.bt_stride = a.bt_stride; c.num_pages = a.num_pages; c.page_stride = a.page_stride;
   c.table_pages = a.table_pages; c.page_size = a.page_size; c.window = a.window;
   c.scale_log2 = (float)(a.scale * 1.4426950408889634);
+  c.q = a.q; c.pages = a.pages; c.q_row = a.q_row;
   c.out = a.out;
   c.parts = (int4*)a.room;
   c.err = a.err;

@@ -11,7 +11,8 @@
 // times: S^T = K Q^T, O^T += V^T P^T.  (With the rows on the side of 16 a chunk of four rows takes 48 products in place of 24.)  In both a thread
 // has rows 2 (lane mod 4) and the next, so that the factors of a row's maximum need no exchange; weights cross over from accumulator to operand by movmatrix.
 // A row's weights are formed in float32 against its running maximum and enter the second product as two bfloat16 terms (16 bits of a weight); sums
-// are float32.  Values of a chunk that lie outside of the piece's keys are made zeros before they meet weights of zero.
+// are float32.  Values of a chunk that lie outside of the piece's keys are made zeros before they meet weights of zero; rows that come out infinite or NaN by values
+// which only others of the piece see are worked out anew by the join.
 #pragma once
 #include "attention_shared.cuh"
 #include "tc_ops.cuh"
@@ -327,6 +328,7 @@ shared_narrow_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     as.w = p.w;
     const bool sole = is_sole(as, p.workers);
     const long long slot = (long long)(p.item + worker) * c.rows;
+    bool anew = false;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       if (t && rows <= 8) break;
@@ -340,6 +342,10 @@ shared_narrow_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         // columns 16 n + lane / 4 and the one eight on: eight lanes write 32 bytes (16 of bfloat16) together
         if (sole) {
           const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;      // (NaN stays)
+          float finite = 0.f;      // NaN: not all of the thread's numbers are
+#pragma unroll
+          for (int n = 0; n < KB; ++n) finite = fmaf(x.o[t][n][e], 0.f, fmaf(x.o[t][n][2 + e], 0.f, finite));
+          anew |= finite != finite;
           bf16* dst = reinterpret_cast<bf16*>(c.out) + ((long long)(p.row0 + row / G) * c.heads + p.kv_head * G + row % G) * D + (lane >> 2);
 #pragma unroll
           for (int n = 0; n < KB; ++n) {
@@ -354,7 +360,8 @@ shared_narrow_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         }
       }
     }
-    if (lane == 0) c.pieces[p.item] = p.workers;
+    anew = __any_sync(0xffffffffu, anew);
+    if (lane == 0) c.pieces[p.item] = make_int2(p.workers.x, p.workers.y | (anew ? ANEW : 0));
     ++pieces;
   }
   if (TMA && !ok) {                      // a wait gave up: let copies in flight land

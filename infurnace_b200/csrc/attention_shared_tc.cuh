@@ -12,8 +12,8 @@
 // float32 to the room, and maximum and denominator beside them.  A weight is the sum of two bfloat16 numbers (16 of its bits).
 //
 // What no row sees may be anything: keys outside of a piece's are masked as scores; their values, which the product would multiply by a weight of zero, are
-// overwritten with zeros in shared memory by the warp that issues it.  (Within a request's own keys a value that only later queries see is in the product of
-// the earlier ones with weight zero: where it is infinite or NaN they become NaN with them.)
+// overwritten with zeros in shared memory by the warp that issues it.  (A value that some rows of the tile see and others do not is in the product of these with
+// weight zero: rows that come out infinite or NaN are worked out anew by the join.)
 //
 // What bounds it: a half's chain, 2,500 cycles, of which a softmax warp works 1,950 and waits for scores 300 and for the product before 240, two warps to a
 // scheduler; tensor cores are busy 53% of the time and issue slots 48%.  Eight times 230 queries (32 heads of 128) to 6,000 shared keys take 296 us, 630 TFLOP/s not
@@ -370,11 +370,12 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       const int par = ic & 1;
       merge_m[par][x][row] = m_used;
       merge_l[par][x][row] = l;
+      const int2 workers = walk.item_workers(c, p, blockIdx.x);
+      if (threadIdx.x == 128) c.pieces[p.item] = workers;
       tc_fence_before();
       asm volatile("bar.sync 2, 256;\n" ::: "memory");          // the eight softmax warps, on every path
       tc_fence_after();
       const bool go = __all_sync(0xffffffffu, !*abort_flag) != 0;
-      const int2 workers = walk.item_workers(c, p, blockIdx.x);
       if (go && work) {
         const float m0 = merge_m[par][0][row], m1 = merge_m[par][1][row], l0 = merge_l[par][0][row], l1 = merge_l[par][1][row];
         const float m = fmaxf(m0, m1);
@@ -389,6 +390,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         float* dst = c.part_o + (slot - lane) * D;               // of the warp's first row
         const int count = min(32, p.tokens * G - qd * 32);       // its rows that exist
         if (x == 0 && exists && !sole) c.part_ml[slot] = make_float2(m, ml);
+        float finite = 0.f;                                      // NaN: not all of the thread's numbers are
 #pragma unroll 1
         for (int cc = 0; cc < DN / 64; ++cc) {
           const int col0 = x * (DN / 2) + cc * 32;
@@ -403,6 +405,10 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           if (two) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) y[i] = fmaf(__uint_as_float(ob[i]), w1, y[i]);
+          }
+          if (sole && (DN == D || col0 < D)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) finite = fmaf(y[i], 0.f, finite);
           }
           // a row's 128 bytes by eight lanes: through shared memory, a row of it 36 numbers long (no two lanes of a quarter on a bank)
 #pragma unroll
@@ -425,8 +431,8 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           }
           __syncwarp();
         }
+        if (__any_sync(0xffffffffu, exists && finite != finite) && lane == 0) atomicOr(&c.pieces[p.item].y, ANEW);
       }
-      if (threadIdx.x == 128 && go) c.pieces[p.item] = workers;
       tc_fence_before();
       tc_mbar_arrive(&bars.o_free);            // this piece's sums have been read
       if (!go) break;

@@ -115,6 +115,48 @@ def test_requests_that_share_see_what_they_would_alone(K, name, dtype):
     K.check_device_errors()
 
 
+# Keys that some rows of a tile see and others do not: what they hold may be anything for the others.
+PARTLY_SEEN = {
+    "questions": dict(groups=[(300, [(330, 30), (341, 41), (301, 1)])], group=4),
+    "full-tiles": dict(groups=[(208, [(330, 90), (290, 70)])], group=2),
+    "few-queries": dict(groups=[(48, [(55, 4), (60, 2), (49, 1)])], alone=[(20, 7), (3, 3)]),
+    "window": dict(groups=[(300, [(310, 1), (420, 1), (305, 5), (330, 1)] * 5)], window=100, group=4),
+    "few-in-a-window": dict(groups=[(300, [(310, 1), (340, 1), (305, 2)])], window=100),
+    "a-short-one-in-a-group": dict(groups=[(200, [(230, 1), (120, 1), (160, 3), (220, 60)])]),
+}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dim", [64, 128, 80, 144])
+@pytest.mark.parametrize("name", PARTLY_SEEN)
+def test_what_other_rows_see_may_be_anything(K, name, dim, what, dtype):
+    scene = Scene(**PARTLY_SEEN[name], dim=dim, dtype=dtype, seed=31)
+    # the last keys of every request and the shared ones that the windows or lengths of some leave out, in some columns of the values
+    for r, n in enumerate(scene.lens):
+        j = next((j for j in range(len(scene.shared)) if scene.cu_groups[j] <= r < scene.cu_groups[j + 1]), None)
+        for key, columns in ((n - 1, slice(3, 4)), (n - 2, slice(5, 20)), (n - scene.window - 2 if scene.window else n - 3, slice(dim - 1, dim))):
+            if key >= 0:
+                owner = scene.cu_groups[j] if j is not None and key < scene.shared[j] else r
+                scene.pages[int(scene.tables[owner, key // scene.page]), 1, :, key % scene.page, columns] = what
+    out = scene.run(K)
+    want, _ = attention(scene.q[:scene.cu_q[-1]].float(), scene.pages.float(), scene.tables, scene.cu_q, scene.lens, scene.cu_groups, scene.shared, scene.scale,
+                        scene.window)
+    got = out[:scene.cu_q[-1]].double().cpu()
+    assert (want.isfinite()).any() and not want.isfinite().all()
+    assert (got.isfinite() == want.isfinite()).all()
+    assert (got.isnan() == want.isnan()).all() and (got[want == math.inf] == math.inf).all() and (got[want == -math.inf] == -math.inf).all()
+    # the finite ones: those of the same scene with zeros in those places, which none of their rows sees
+    seen = want.isfinite()
+    scene.pages = torch.nan_to_num(scene.pages, nan=0.0, posinf=0.0, neginf=0.0)
+    plain, size = attention(scene.q[:scene.cu_q[-1]].float(), scene.pages.float(), scene.tables, scene.cu_q, scene.lens, scene.cu_groups, scene.shared,
+                            scene.scale, scene.window)
+    norm = scene.q.float().norm(dim=2).max() * scene.pages[:, 0].float().norm(dim=3).max() * scene.scale
+    wide = 2 * dim * 2.0 ** -24 * norm + 2.0 ** -20 + 2 * max(scene.lens) * 2.0 ** -24 + (2.0 ** -16 if dtype == torch.bfloat16 else 0.0)      # as in check
+    bound = float(wide) * size + torch.finfo(dtype).eps / 2 * plain.abs()
+    assert (((got - plain).abs() - bound)[seen] <= 0).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("page", [1, 8, 16, 24, 32, 64, 128])
 def test_pages_of_any_size(K, page, dtype):
