@@ -1,5 +1,7 @@
 // Attention over shared pages in bfloat16, compiled for one head size: -DHEAD_DIM=<multiple of 16, at most 256> (default 128).  Narrow owners by
-// attention_shared_narrow.cuh, wide ones by attention_shared_tc.cuh where heads and pages allow, else by attention_shared_simt.cuh, beside one another.
+// attention_shared_narrow.cuh, wide ones beside them by attention_shared_tc.cuh where heads and pages allow.  Where they do not, all owners by
+// attention_shared_narrow.cuh, in tiles of sixteen rows; groups of more than 16 heads, of which a tile would not hold one token, by
+// attention_shared_simt.cuh, which is several times slower (11 requests of 173 queries and some 300 keys, 40 heads of 256: 2,613 us, and 450 in tiles of sixteen).
 #include <cuda.h>
 
 #ifndef HEAD_DIM
@@ -56,8 +58,13 @@ IFB_EXPORT int ifb_attention_shared_bf16(const Packed* call) {
   char* rest = (char*)a.room + parts_bytes(a.n_tokens);
   room_at(wide, D, rest);
   room_at(few, D, rest + room_bytes(wide, D));
-  const bool any_wide = (long long)a.n_tokens * group > NARROW_ROWS;      // no owner has more rows than all
   const bool any_narrow = group <= NARROW_ROWS;
+  if (any_narrow && !tc) {
+    few.which = EVERY;
+    const int st = narrow::run(by_tma, few, few, q, a.q_row, pages, false, a.stream);
+    return st ? st : join<__nv_bfloat16>(few, few, D, a.stream);
+  }
+  const bool any_wide = (long long)a.n_tokens * group > NARROW_ROWS;      // no owner has more rows than all
   int st = IFB_OK;
   if (any_wide) {
 #if HEAD_DIM <= 128

@@ -226,7 +226,7 @@ class AnswerKernels:
         elif room.dtype is not torch.uint8 or room.dim() != 1 or not room.is_contiguous() or room.numel() < size or room.data_ptr() % 256 \
                 or room.get_device() != index:
             raise KernelError(f"shared_prefix_attention: a room is uint8 [{size} or more], contiguous, on 256 bytes, on the same device")
-        self.launches += 2 if dtype is torch.float32 or group > 16 or n * group <= 16 else 3
+        self.launches += 3 if dtype is not torch.float32 and group <= 16 < n * group and dim <= 128 and page_size in (16, 32, 64) else 2
         self._err_armed = True
         packed = _SHARED_CALL(q.data_ptr(), kv_pages.data_ptr(), block_tables.data_ptr(), cu_q.data_ptr(), seq_lens.data_ptr(), cu_groups.data_ptr(),
                               shared_lens.data_ptr(), out.data_ptr(), room.data_ptr(), self._dev_err_at, _raw_stream(index), q_row, page_stride, pages,
