@@ -15,8 +15,10 @@ IFB_EXPORT int ifb_attention_shared(const Packed* call) {
   fill(c, a);
   room_at(c, a.dim, (char*)a.room + parts_bytes(a.n_tokens));
   const float *q = (const float*)a.q, *pages = (const float*)a.pages;
-  const int st = a.dim <= 64    ? sh_main<float, 8>(c, c, q, a.q_row, pages, a.dim, true, a.stream)
-                 : a.dim <= 128 ? sh_main<float, 16>(c, c, q, a.q_row, pages, a.dim, true, a.stream)
-                                : sh_main<float, 32>(c, c, q, a.q_row, pages, a.dim, true, a.stream);
+  const int st = a.dim <= 64    ? sh_main<float, 2>(c, c, q, a.q_row, pages, a.dim, true, a.stream)
+                 : a.dim <= 96  ? sh_main<float, 3>(c, c, q, a.q_row, pages, a.dim, true, a.stream)
+                 : a.dim <= 128 ? sh_main<float, 4>(c, c, q, a.q_row, pages, a.dim, true, a.stream)
+                 : a.dim <= 192 ? sh_main<float, 6>(c, c, q, a.q_row, pages, a.dim, true, a.stream)
+                                : sh_main<float, 8>(c, c, q, a.q_row, pages, a.dim, true, a.stream);
   return st ? st : join<float>(c, c, a.dim, a.stream);
 }

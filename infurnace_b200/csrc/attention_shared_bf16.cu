@@ -71,7 +71,7 @@ IFB_EXPORT int ifb_attention_shared_bf16(const Packed* call) {
     if (tc) st = tc_main(wide, few, q, a.q_row, pages, !any_narrow, a.stream);
     else
 #endif
-      st = sh_main<__nv_bfloat16, (D <= 64 ? 8 : D <= 128 ? 16 : 32)>(wide, few, q, a.q_row, pages, D, !any_narrow, a.stream);
+      st = sh_main<__nv_bfloat16, (D + 31) / 32>(wide, few, q, a.q_row, pages, D, !any_narrow, a.stream);
     if (st) return st;
   }
   if (any_narrow) {
