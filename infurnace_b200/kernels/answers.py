@@ -111,7 +111,8 @@ class AnswerKernels:
         """The log probability of token ``tokens[r]`` under softmax(logits[r]) into ``out`` (float32), and the number of tokens that come before it by
         falling logit, equal ones by rising index, into ``ranks`` (int32).  ``logits`` float32 or bfloat16 [rows, vocabulary], rows may
         lie apart; ``tokens`` int32, one a row.  A token outside the vocabulary (padding) gives NaN and -1; a row with a NaN
-        or +inf, or with no number above -inf, NaN."""
+        or +inf, or with no number above -inf, NaN.  Sums are float32: a row's last bits may differ with the number of rows and
+        with where in memory it begins."""
         what = "token_logprobs"
         code, rows, vocab, pitch, index = _logit_rows(logits, what)
         args = (_one_per_row(tokens, torch.int32, rows, index, what, "tokens"), _one_per_row(out, torch.float32, rows, index, what, "out"),
@@ -169,7 +170,7 @@ class AnswerKernels:
         a page.)  Requests of no group share nothing.  A row that sees no key becomes zero; rows behind the last request stay as they are.
         ``cu_q``, ``seq_lens``, ``block_tables``, ``cu_groups`` [groups + 1] and ``shared_lens`` [groups] are int32 on the device.  No request has more than
         ``max_q_len`` queries or ``max_seq_len`` keys.  An entry of a table that is read and is no page of the pool counts as zeros and is recorded in the
-        kernels' error word.
+        kernels' error word.  What a row does not see may be anything, infinities and NaN too.
 
         ``room``: None, or a uint8 tensor of at least ``shared_prefix_room`` bytes for the pieces' sums, in place of memory of the allocator's (within
         a recording: of the graph's own pool); calls that share one follow one another."""
