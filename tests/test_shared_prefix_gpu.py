@@ -178,6 +178,23 @@ def test_groups_of_heads(K, kv_heads, group, dtype):
     s.check(s.run(K))
 
 
+@pytest.mark.parametrize("dim,page", [(144, 16), (256, 24), (128, 24), (80, 128)])
+@pytest.mark.parametrize("kv_heads,group", [(3, 1), (1, 5), (2, 7), (1, 16), (1, 17), (1, 64)])
+@pytest.mark.parametrize("name", ["questions", "full-tiles-window", "uneven"])
+def test_groups_of_heads_where_large_tiles_do_not_fit(K, name, kv_heads, group, dim, page):
+    s = Scene(**{**SCENES[name], "kv_heads": kv_heads, "group": group, "dim": dim, "page": page}, seed=21)
+    s.check(s.run(K))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,requests", [(64, 1100), (256, 480)])
+def test_many_requests(K, dim, requests, dtype):
+    """More than the plan of the large tiles' kernel has room for."""
+    groups = [(40 + 16 * j, [(41 + 16 * j + i % 9, 1 + (i % 50 == 0)) for i in range(requests // 4)]) for j in range(3)]
+    s = Scene(groups, alone=[(1 + i % 20, 1) for i in range(requests - 3 * (requests // 4))], kv_heads=1, group=2, dim=dim, dtype=dtype, seed=22)
+    s.check(s.run(K))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scores_of_any_size(K, dtype):
     """Rows with one weight that is all, and scores far beyond the exponents' range."""
