@@ -11,7 +11,7 @@
 // roundings add up to 1e-11).  And sums of whole numbers do not depend on their order: a row's token depends on the row alone, not on how many CTAs or
 // threads share it.  2^44 times the largest vocabulary stays below 2^63.
 //
-// A row is shared by a cluster of C CTAs, which keep its slices in shared memory as float32: it is read from memory once.  A cut is found by counts (top-k)
+// A row is shared by a cluster of C CTAs, which keep its slices in shared memory: it is read from memory once.  A cut is found by counts (top-k)
 // or weights (top-p) in bins of equal width over (l - m) / T.  At first the bins reach 14 factors of two down, where nearly all cuts are and few tokens, so
 // that few take part in the bins' atomics (what lies below is one sum); a cut that is not there is looked for over 24, and then over all 46.  The bin that the cut
 // runs through is divided once more if it has many members; the members left, 512 at most, go to every CTA, which puts them in order and finds the cut
@@ -38,7 +38,7 @@ constexpr int SUBS = 256;                // parts of a bin
 constexpr int LIST = NT;                 // members that are put in order, one a thread
 constexpr int MAX_CLUSTER = 16;          // (beyond 8 a device may refuse: then no such cluster is taken)
 constexpr int SURE_CLUSTER = 8;
-constexpr int SLICE = 46080;             // most logits of a CTA: 180 KB
+constexpr int SLICE = 46080;             // most logits of a CTA: 180 KB (in 32 bits)
 constexpr int SHARED_SLICE = 19072;      // up to here two CTAs fit on an SM
 constexpr double UNIT = 17592186044416.0;      // 2^44
 constexpr u64 ALL = ~0ull;
@@ -297,6 +297,12 @@ __device__ __forceinline__ int find_bin(CutShared* sh, int n, const uint32_t* co
 struct Cut { float l; int i; u64 mass; };
 __device__ __forceinline__ bool kept(float l, int i, const Cut& c) { return l > c.l || (l == c.l && i <= c.i); }
 
+// A CTA's slice of a row, in shared memory in the type that it comes in (of 16 bits twice the rows find room: 203 rows of 97,476 under top-p 154 to 109 us).
+template <typename T> struct Slice {
+  T* at;
+  __device__ __forceinline__ float operator[](int i) const { return to_f32<T>(at[i]); }
+};
+
 struct CutMemory {      // of a CTA, behind its slice of the row
   uint32_t* count; uint32_t* lo; uint32_t* hi;             // its own bins [BINS + 1] each
   uint32_t* row_count; u64* row_mass;                      // the row's bins [BINS + 1]
@@ -313,8 +319,8 @@ __device__ __forceinline__ void add_mass(uint32_t* lo, uint32_t* hi, int b, u64 
 
 // The members that `in` tells by their bin, at most LIST of them in the row, to every CTA's list `which`, in one order for all.  (A CTA notes its own, in the place
 // of its bins' counts, which are merged, and takes room for all of them at once: an addition over the cluster for each member took longer than all the rest.)
-template <class In>
-__device__ __forceinline__ void gather(const Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, int which, In in) {
+template <typename T, class In>
+__device__ __forceinline__ void gather(const Row& row, const CutMemory& mem, Slice<T> vals, int n, int base, const RowScale& rs, int which, In in) {
   CutShared* sh = row.sh;
   uint32_t* own = mem.count;
   for (int i0 = threadIdx.x; i0 < n; i0 += 4 * NT) {
@@ -393,8 +399,10 @@ __device__ __forceinline__ void tell_cut(CutShared* sh, bool last, u64 member, u
 }
 
 // The cut through the row's bins after which `goal` tokens (by_mass: at least `goal` of weight) are kept.  False: it does not run through them.
-__device__ __forceinline__ bool find_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, bool by_mass, u64 goal, bool weighted,
-                         int key_shift, Cut& cut) {
+template <typename T>
+__device__ __forceinline__ bool find_cut(Row& row, const CutMemory& mem, Slice<T> vals, int n, int base, const RowScale& rs, bool by_mass, u64 goal, bool weighted,
+                         Cut& cut) {
+  constexpr int key_shift = sizeof(T) == 2 ? 16 : 0;
   CutShared* sh = row.sh;
   u64 bc, bm;
   const int b0 = find_bin(sh, BINS, mem.row_count, mem.row_mass, by_mass, goal, bc, bm, weighted);
@@ -484,7 +492,8 @@ __device__ __forceinline__ bool find_cut(Row& row, const CutMemory& mem, const f
 
 // Where the cut to the first k lies so high that all tokens of its bin and above fit into a list (`members` of them, bins 0 .. last_bin): both cuts at once from
 // their order, without weights of any other token.
-__device__ __forceinline__ void list_cut(Row& row, const CutMemory& mem, const float* vals, int n, int base, const RowScale& rs, int last_bin, uint32_t members, uint32_t k,
+template <typename T>
+__device__ __forceinline__ void list_cut(Row& row, const CutMemory& mem, Slice<T> vals, int n, int base, const RowScale& rs, int last_bin, uint32_t members, uint32_t k,
                          float p, Cut& cut) {
   CutShared* sh = row.sh;
   const float f1 = last_bin + 1.f;
@@ -509,10 +518,19 @@ template <> struct Vec16<float> {
   static __device__ __forceinline__ void unpack(const uint4& x, float (&v)[4]) {
     v[0] = __uint_as_float(x.x); v[1] = __uint_as_float(x.y); v[2] = __uint_as_float(x.z); v[3] = __uint_as_float(x.w);
   }
+  static __device__ __forceinline__ uint4 pack(const float (&v)[4]) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  }
   static __device__ __forceinline__ void read(const float* p, float (&v)[4]) { unpack(*reinterpret_cast<const uint4*>(p), v); }
 };
 template <> struct Vec16<bf16> {
   static constexpr int N = 8;
+  static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {      // of numbers that have 16 bits
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632);
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
   static __device__ __forceinline__ void read(const bf16* p, float (&v)[8]) { unpack(*reinterpret_cast<const uint4*>(p), v); }
   static __device__ __forceinline__ void unpack(const uint4& x, float (&v)[8]) {
     const uint32_t u[4] = {x.x, x.y, x.z, x.w};
@@ -556,7 +574,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   __shared__ CutShared shared;
   CutShared* sh = &shared;
   CutMemory mem;
-  mem.row_mass = reinterpret_cast<u64*>(cut_smem + 16 + (size_t)((a.per + 3) & ~3) * 4);
+  mem.row_mass = reinterpret_cast<u64*>(cut_smem + 16 + (size_t)a.per * sizeof(T));      // (a slice is a multiple of eight numbers)
   mem.sub_mass = mem.row_mass + BINS + 1;
   mem.list = mem.sub_mass + SUBS;
   mem.count = reinterpret_cast<uint32_t*>(mem.list + 2 * LIST);
@@ -585,22 +603,24 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   constexpr int N = Vec16<T>::N;
   const T* src = logits + r * a.pitch + base;
   const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / (int)sizeof(T)), done = head + (n - head) / N * N;
-  float* vals = reinterpret_cast<float*>(cut_smem) + (-head & 3);
+  const Slice<T> vals = {reinterpret_cast<T*>(cut_smem) + (-head & N - 1)};
   float bv = -INFINITY;
   auto take = [&](float v) {
     v = v == v ? v + 0.f : -INFINITY;      // -0 becomes 0
     bv = fmaxf(bv, v);
     return v;
   };
-  if (tid < head) vals[tid] = take(to_f32<T>(src[tid]));
+  auto put = [&](int i) { vals.at[i] = from_f32<T>(take(to_f32<T>(src[i]))); };      // (exact)
+  if (tid < head) put(tid);
 #pragma unroll 4
   for (int i = head + tid * N; i < done; i += NT * N) {
     float v[N];
     Vec16<T>::read(src + i, v);
 #pragma unroll
-    for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(vals + i + j) = make_float4(take(v[j]), take(v[j + 1]), take(v[j + 2]), take(v[j + 3]));
+    for (int j = 0; j < N; ++j) v[j] = take(v[j]);
+    *reinterpret_cast<uint4*>(vals.at + i) = Vec16<T>::pack(v);
   }
-  for (int i = done + tid; i < n; i += NT) vals[i] = take(to_f32<T>(src[i]));
+  for (int i = done + tid; i < n; i += NT) put(i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) bv = fmaxf(bv, __shfl_xor_sync(0xffffffffu, bv, o));
   if (row.ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // every peer has begun: its shared memory may be written
@@ -719,7 +739,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
         if (what && !by_mass) { found = true; break; }
         const double want = ceil((double)p * (double)cut.mass);
         const u64 goal = what == 0 ? (u64)k : want >= 1.0 ? (u64)want : 1;
-        found = find_cut(row, mem, vals, n, base, rs, what, goal, by_mass, sizeof(T) == 2 ? 16 : 0, cut);
+        found = find_cut(row, mem, vals, n, base, rs, what, goal, by_mass, cut);
         if (!found && !(what == 0 && last_try)) break;      // (with fewer than k tokens in the last try's bins top-k keeps everything)
       }
     }
@@ -972,19 +992,26 @@ IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
   if (rows <= 0) return IFB_OK;
   if (vocab < 1 || vocab > SURE_CLUSTER * SLICE || rows > (1 << 27)) return IFB_ERR_SIZE;
   if (!call->temperature || !call->uniform || !call->out) return IFB_ERR_ARG;
-  // As few CTAs of a row as let two share an SM; more while all rows' clusters find their SMs at once.
+  // As few CTAs of a row as let two share an SM (of 16-bit numbers counted as 32-bit ones, but for half as many where there are rows for several rounds: 36
+  // rows of 95,403 take 40 us in eight CTAs each and 57 in four, 203 of 97,476 154 and 109); more while all rows' clusters find their SMs at once.
   const void* kernel = dtype == IFB_F32 ? (const void*)sample_cut_kernel<float> : dtype == IFB_BF16 ? (const void*)sample_cut_kernel<bf16> : nullptr;
   if (!kernel) return IFB_ERR_DTYPE;
   auto slice = [&](int n) { return ((vocab + n - 1) / n + 7) & ~7; };
-  auto room_for = [&](int n) { return cut_clusters(kernel, dtype, n, (size_t)slice(n) * 4 + CUT_BYTES); };
+  const int width = dtype == IFB_F32 ? 4 : 2;
+  auto room_for = [&](int n) { return cut_clusters(kernel, dtype, n, (size_t)slice(n) * width + CUT_BYTES); };
   int ctas = 1;
   while (ctas < SURE_CLUSTER && slice(ctas) > SHARED_SLICE) ctas *= 2;
   int clusters = room_for(ctas);
-  while (ctas < MAX_CLUSTER && vocab / ctas >= 2048 && clusters >= 0) {
-    const int next = room_for(ctas * 2);
-    if (next < rows) break;
-    ctas *= 2;
-    clusters = next;
+  if (ctas > 1 && slice(ctas / 2) * width <= SHARED_SLICE * 4 && rows > clusters + clusters / 2) {
+    ctas /= 2;
+    clusters = room_for(ctas);
+  } else {
+    while (ctas < MAX_CLUSTER && vocab / ctas >= 2048 && clusters >= 0) {
+      const int next = room_for(ctas * 2);
+      if (next < rows) break;
+      ctas *= 2;
+      clusters = next;
+    }
   }
   if (clusters < 0) return clusters;
   const bool everything = rows <= clusters, cuts = everything || call->top_k || call->top_p;
@@ -1009,7 +1036,7 @@ IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
     return IFB_OK;
   };
   if (cuts) {
-    const size_t smem = (size_t)a.per * 4 + CUT_BYTES;
+    const size_t smem = (size_t)a.per * width + CUT_BYTES;
     int st;
     if (dtype == IFB_F32) {
       IFB_ALLOW_SMEM(sample_cut_kernel<float>, smem);
@@ -1023,7 +1050,7 @@ IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
   // the other rows: as many CTAs of a row as leave no SM idle, each with whole blocks for its warps
   const int sms = ifb_sm_count();
   int n = 1;
-  const int wide = dtype == IFB_F32 ? 4 : 2, early = (call->pitch | (long long)((uintptr_t)call->logits / wide)) & 3 ? 3 : 0;      // (rows may begin up to 3 numbers early)
+  const int early = (call->pitch | (long long)((uintptr_t)call->logits / width)) & 3 ? 3 : 0;      // (rows may begin up to 3 numbers early)
   auto stretch = [&](int ctas) { return ((vocab + early + ctas * ST_NW - 1) / (ctas * ST_NW) + ST_BLOCK - 1) / ST_BLOCK * ST_BLOCK; };
   while (n < SURE_CLUSTER && (stretch(n) > ST_BLOCKS * ST_BLOCK || ((long long)rows * n * 2 <= 8LL * sms && stretch(n) > 2 * ST_BLOCK))) n *= 2;
   a.per = stretch(n) * ST_NW;

@@ -166,6 +166,19 @@ def test_a_row_does_not_depend_on_the_others(K, vocab):
         assert part[0] == [whole[0][i] for i in rows] and part[1] == [whole[1][i] for i in rows]
 
 
+@pytest.mark.parametrize("vocab", [40000, 97477])
+def test_a_row_of_16_bits_does_not_depend_on_the_others(K, vocab):
+    """Many rows have half the CTAs each that few have."""
+    x = logits_of(150, vocab, 15, torch.bfloat16)
+    u = torch.rand(150, generator=torch.Generator().manual_seed(2)).tolist()
+    ps, ks = [0.9, 1.0, 0.95] * 50, [0, 0, 50, 900, 0] * 30
+    whole = draw(K, x, [1.0] * 150, u, ks, ps)
+    for rows in ([7], [4, 5, 6], list(range(100, 130))):
+        part = draw(K, x[rows], [1.0] * len(rows), [u[i] for i in rows], [ks[i] for i in rows], [ps[i] for i in rows])
+        assert part[0] == [whole[0][i] for i in rows] and part[1] == [whole[1][i] for i in rows]
+    check(K, x[:9], [1.0] * 9, u[:9], ks[:9], ps[:9])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("sign", [1.0, -1.0])
 def test_a_high_temperature_puts_many_values_into_a_part_of_a_bin(K, sign, dtype):
