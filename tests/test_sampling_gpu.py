@@ -166,6 +166,27 @@ def test_a_row_does_not_depend_on_the_others(K, vocab):
         assert part[0] == [whole[0][i] for i in rows] and part[1] == [whole[1][i] for i in rows]
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("left", [1, 2, 31, 33, 511, 512, 513, 600])
+@pytest.mark.parametrize("vocab", [700, 50000])
+def test_what_a_grammar_leaves(K, vocab, left, dtype):
+    """Few tokens above -inf, about as many as a list holds, some of them far below the others; among them infinities and the largest numbers."""
+    g = torch.Generator().manual_seed(left)
+    x = torch.full((16, vocab), -math.inf)
+    for r in range(16):
+        at = torch.randperm(vocab, generator=g)[:left]
+        x[r, at] = (1.0, 30.0, 1e4, 0.01)[r % 4] * torch.randn(left, generator=g)
+        if r == 13:
+            x[r, at[:(left + 1) // 2]] = math.inf
+        if r == 14:
+            x[r, at] = torch.where(torch.rand(left, generator=g) < 0.5, 3e38, -3e38)
+        if r == 15:
+            x[r, at] = math.nan if left < 3 else 0.0
+    u = torch.rand(16, generator=g).tolist()
+    ks = [0, 1, 5, left, 0, max(1, left - 1), left + 1, 50] * 2
+    check(K, x.to(dtype), [1.0, 0.2, 5.0, 1.0] * 4, u, ks, [0.9, 1.0, 0.5, 0.99, 0.0, 1.0, 0.7, 1.0] * 2, [0.0, 0.0, 0.1, 0.0] * 4)
+
+
 @pytest.mark.parametrize("vocab", [40000, 97477])
 def test_a_row_of_16_bits_does_not_depend_on_the_others(K, vocab):
     """Many rows have half the CTAs each that few have."""
