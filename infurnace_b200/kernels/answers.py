@@ -162,7 +162,7 @@ class AnswerKernels:
         """``paged_attention`` for requests whose block tables share leading pages, which are then read once for all of them: answers to one
         prompt, questions to one document, conversations behind one system prompt.
 
-        ``q`` and ``out`` are bfloat16 or float32 [tokens, heads, head_dim] (the rows of ``q`` may lie apart, those of ``out`` not), ``kv_pages`` [pages, 2,
+        ``q`` and ``out`` are bfloat16 or float32 [tokens, heads, head_dim] (the rows of ``q`` may lie apart, those of ``out`` not, and share no memory), ``kv_pages`` [pages, 2,
         kv_heads, page_size, head_dim] of the same type.  Request r has the rows cu_q[r] .. cu_q[r + 1] - 1 and ``seq_lens[r]`` keys, these
         queries' own among them, in the pages of ``block_tables[r]``; the query at position p sees positions max(0, p - window + 1) .. p
         (``window`` 0: from 0).  Group g is the requests cu_groups[g] .. cu_groups[g + 1] - 1, the first ``shared_lens[g]`` keys of which are the same: they are
