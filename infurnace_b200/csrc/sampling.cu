@@ -1260,8 +1260,19 @@ __global__ void __launch_bounds__(LP_NT) token_logprob_kernel(const T* logits, l
   }
 }
 
-IFB_EXPORT int ifb_token_logprobs(const void* logits, int dtype, long long pitch, int rows, int vocab, const int* tokens, float* out, int* ranks,
-                                  cudaStream_t stream) {
+struct LpPacked {      // a call as the caller packs it: 8-byte fields first
+  const void* logits;
+  const int* tokens;
+  float* out;
+  int* ranks;
+  cudaStream_t stream;
+  long long pitch;
+  int dtype, rows, vocab, spare;
+};
+IFB_EXPORT int ifb_token_logprobs(const LpPacked* call) {
+  const int dtype = call->dtype, rows = call->rows, vocab = call->vocab;
+  const int* tokens = call->tokens;
+  float* out = call->out;
   if (rows <= 0) return IFB_OK;
   if (vocab < 1 || vocab > (1 << 30) || rows > (1 << 27)) return IFB_ERR_SIZE;
   if (!tokens || !out) return IFB_ERR_ARG;
@@ -1274,7 +1285,7 @@ IFB_EXPORT int ifb_token_logprobs(const void* logits, int dtype, long long pitch
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * ctas);
     cfg.blockDim = dim3(LP_NT);
-    cfg.stream = stream;
+    cfg.stream = call->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = ctas;
@@ -1284,11 +1295,11 @@ IFB_EXPORT int ifb_token_logprobs(const void* logits, int dtype, long long pitch
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ifb_pdl_enabled() ? 2 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, typed, pitch, vocab, per, tokens, out, ranks);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, typed, call->pitch, vocab, per, tokens, out, call->ranks);
     if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
     return IFB_OK;
   };
-  if (dtype == IFB_F32) return go(token_logprob_kernel<float>, (const float*)logits);
-  if (dtype == IFB_BF16) return go(token_logprob_kernel<bf16>, (const bf16*)logits);
+  if (dtype == IFB_F32) return go(token_logprob_kernel<float>, (const float*)call->logits);
+  if (dtype == IFB_BF16) return go(token_logprob_kernel<bf16>, (const bf16*)call->logits);
   return IFB_ERR_DTYPE;
 }

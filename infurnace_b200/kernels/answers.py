@@ -6,7 +6,7 @@ attention is cut into pieces at the head of ``csrc/attention_shared.cuh``.
 """
 from __future__ import annotations
 
-from ctypes import c_char_p, c_int, c_longlong, c_void_p
+from ctypes import c_char_p, c_int, c_longlong
 
 import struct
 
@@ -43,7 +43,7 @@ def _logit_rows(logits, what):
 
 def _one_per_row(t, dtype, rows, index, what, name):
     """The address of a tensor with one number for each row."""
-    if t.dtype is not dtype or t.dim() != 1 or t.numel() != rows or not t.is_contiguous() or t.get_device() != index:
+    if t.dtype is not dtype or t.shape != (rows,) or not t.is_contiguous() or t.get_device() != index:
         raise KernelError(f"{what}: {name} is {dtype} [{rows}], contiguous, on the logits' device; got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
@@ -54,6 +54,7 @@ def _device_of(index):
 
 
 _CUT_CALL = struct.Struct("=10q4i").pack            # csrc/sampling.cu: CutPacked
+_LOGPROB_CALL = struct.Struct("=6q4i").pack         # csrc/sampling.cu: LpPacked
 _SHARED_CALL = struct.Struct("=15qd10i").pack       # csrc/attention_shared.cuh: Packed
 
 
@@ -66,7 +67,7 @@ class AnswerKernels:
         if self._sampling is None:
             lib = load_library("sampling", progress=self._progress)
             lib.ifb_sample_cut.argtypes = [c_char_p]
-            lib.ifb_token_logprobs.argtypes = [c_void_p, c_int, c_longlong, c_int, c_int] + [c_void_p] * 4
+            lib.ifb_token_logprobs.argtypes = [c_char_p]
             self._sampling_max_vocab = int(lib.ifb_sample_cut_max_vocab())
             self._sampling = lib
         return self._sampling
@@ -115,18 +116,19 @@ class AnswerKernels:
         with where in memory it begins."""
         what = "token_logprobs"
         code, rows, vocab, pitch, index = _logit_rows(logits, what)
-        args = (_one_per_row(tokens, torch.int32, rows, index, what, "tokens"), _one_per_row(out, torch.float32, rows, index, what, "out"),
-                0 if ranks is None else _one_per_row(ranks, torch.int32, rows, index, what, "ranks"), _raw_stream(index))
+        args = (logits.data_ptr(), _one_per_row(tokens, torch.int32, rows, index, what, "tokens"), _one_per_row(out, torch.float32, rows, index, what, "out"),
+                0 if ranks is None else _one_per_row(ranks, torch.int32, rows, index, what, "ranks"))
         if rows == 0:
             return out
         self.launches += 1
-        call = (self._sampling or self._sampling_lib()).ifb_token_logprobs
+        lib = self._sampling or self._sampling_lib()
+        call = _LOGPROB_CALL(*args, _raw_stream(index), pitch, code, rows, vocab, 0)
         other = _device_of(index)
         if other is None:
-            status = call(logits.data_ptr(), code, pitch, rows, vocab, *args)
+            status = lib.ifb_token_logprobs(call)
         else:
             with other:
-                status = call(logits.data_ptr(), code, pitch, rows, vocab, *args)
+                status = lib.ifb_token_logprobs(call)
         if status:
             _status(status, what)
         return out
