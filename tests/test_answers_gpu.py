@@ -4,6 +4,7 @@ import math
 import os
 import subprocess
 import sys
+import threading
 
 import pytest
 import torch
@@ -94,6 +95,47 @@ def test_answers_to_one_prompt(K, dtype):
             answers[r].append(token)
             scores[r] += float(logprobs[r])
     assert answers[0] != answers[1] and all(math.isfinite(x) and x < 0 for x in scores)
+
+
+def test_threads_that_call_on_one_stream(K):
+    """Three host threads on one stream, so that the launches of their calls come in any order between one another: what each gets is what it gets alone."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    one = lambda x, t=torch.int32: torch.tensor(x, dtype=t, device="cuda")
+    pages = torch.randn((400, 2, 2, 16, 64), generator=g, device="cuda").to(torch.bfloat16)
+    groups, members = 3, 12
+    tables = torch.stack([torch.cat((torch.arange(20) + 20 * (r // members), 60 + 9 * r + torch.arange(9))) for r in range(groups * members)]).to(torch.int32).cuda()
+    cu_groups, shared = one([members * j for j in range(groups + 1)]), one([320] * groups)
+
+    def attend(seed):
+        tokens = [1 + (r + seed) % 3 if r % 5 else 9 for r in range(groups * members)]
+        cu_q, lens = one([sum(tokens[:r]) for r in range(len(tokens) + 1)]), one([330 + (7 * r + seed) % 130 for r in range(len(tokens))])
+        q = torch.randn((sum(tokens), 8, 64), generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(torch.bfloat16)
+        return lambda: K.shared_prefix_attention(q, pages, tables, cu_q, lens, cu_groups, shared, torch.empty_like(q), 0.125, 0, 9, 464)
+
+    def draw(seed):
+        x = 3 * torch.randn((220, 20011), generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+        u = torch.rand(220, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+        t, p = torch.ones(220, device="cuda"), one([0.9, 1.0] * 110, torch.float32)
+        return lambda: K.sample_filtered(x, t, u, torch.empty(220, dtype=torch.int32, device="cuda"), top_p=p)
+
+    calls = [attend(1), attend(2), draw(3)]
+    alone = [call() for call in calls]
+    torch.cuda.synchronize()
+    results = [[], [], []]
+
+    def work(i):
+        for _ in range(40):
+            results[i].append(calls[i]())
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(3):
+        assert len(results[i]) == 40 and all(torch.equal(x, alone[i]) for x in results[i])
+    K.check_device_errors()
 
 
 def engine(model_dir, name, dtype, **kw):
