@@ -16,7 +16,7 @@
 // weight zero: rows that come out infinite or NaN are worked out anew by the join.)
 //
 // What bounds it: a half's chain, 2,500 cycles, of which a softmax warp works 1,950 and waits for scores 300 and for the product before 240, two warps to a
-// scheduler; tensor cores are busy 53% of the time and issue slots 48%.  Eight times 230 queries (32 heads of 128) to 6,000 shared keys take 296 us, 630 TFLOP/s not
+// scheduler; tensor cores are busy 57% of the time and issue slots 41%.  Eight times 230 queries (32 heads of 128) to 6,000 shared keys take 296 us, 630 TFLOP/s not
 // counting the second terms, or 940 with them, where the power limit lowers clocks to 1.2 to 1.5 GHz.
 #pragma once
 #include "tc_ops.cuh"
