@@ -73,8 +73,8 @@ DEFAULT_VARIANTS += [("attention_tc", {"HEAD_DIM": d, "WEIGHT_TERMS": 2}) for d 
 # attention over 8-bit pages: heads of 128 (bfloat16), the sizes that the tests of the engine run, float32
 DEFAULT_VARIANTS += [(name, {"HEAD_DIM": d}) for name in ("kv8_attention", "kv8_attention_f32") for d in (128, 64, 256, 16)]
 
-# attention over shared pages in bfloat16: heads of 128 and what the tests run most
-DEFAULT_VARIANTS += [("attention_shared_bf16", {"HEAD_DIM": d}) for d in (128, 64, 32)]
+# attention over shared pages in bfloat16: the usual heads and what the tests run most
+DEFAULT_VARIANTS += [("attention_shared_bf16", {"HEAD_DIM": d}) for d in (128, 64, 256, 96, 32)]
 
 def register_library(name: str, sources: Sequence[str], flags: Sequence[str] = (), *, replace: bool = False) -> None:
     """Make a library of CUDA sources from outside the package known to :func:`load_library`, so that a
