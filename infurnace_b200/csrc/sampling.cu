@@ -137,8 +137,9 @@ __device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp
 // The same as a call, where rows that are not plain go once in a while.
 __device__ __noinline__ u64 called_weight(float l, RowScale rs, const Exp2Table* tab) { return row_weight(l, rs, *tab); }
 
-// What min_p asks of a logit, and a little less.
+// What min_p asks of a logit, and a little less (of +inf: +inf, since what else there is has no weight).
 __device__ __forceinline__ float least_floor(float m, float least, const RowScale& rs) {
+  if (m == INFINITY) return m;
   const float l = m - (0.01f - log2f(fminf(least, 1.f))) / rs.to_log2;
   return l - fabsf(l) * 2.4e-7f;
 }
