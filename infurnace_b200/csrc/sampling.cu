@@ -505,13 +505,14 @@ __device__ __forceinline__ bool find_cut(Row& row, const CutMemory& mem, Slice<T
   return true;
 }
 
-// Both cuts at once from the order of a list, without weights of any other token: of all tokens that are above -inf, or of those above the end of a bin (NaN: none),
-// where the cut to the first k lies above it (`members` of them, k at most).
+// Both cuts at once from the order of a list, without weights of any other token: of all tokens that are above -inf (`whole`), or of those that the bins up to `end`
+// counted, where the cut to the first k lies above it (`members` of them, k at most).  (Asked as the bins asked: beside an infinite largest logit a finite one's bin may
+// be NaN, which no bin counts.)
 template <typename T>
-__device__ __forceinline__ void list_cut(Row& row, const CutMemory& mem, Slice<T> vals, int n, int base, const RowScale& rs, float end, uint32_t members, uint32_t k,
-                         float p, Cut& cut) {
+__device__ __forceinline__ void list_cut(Row& row, const CutMemory& mem, Slice<T> vals, int n, int base, const RowScale& rs, bool whole, float end, uint32_t members,
+                         uint32_t k, float p, Cut& cut) {
   CutShared* sh = row.sh;
-  gather(row, mem, vals, n, base, 0, [&](float l) { return l > -INFINITY && !(row_bin(l, rs) >= end); });
+  gather(row, mem, vals, n, base, 0, [&](float l) { return whole ? l > -INFINITY : row_bin(l, rs) < end; });
   const uint32_t i = threadIdx.x, most = members < k ? members : k;
   const u64 member = sorted_member(mem.list, reinterpret_cast<u64*>(mem.count), (int)members);
   const u64 w = i < most ? row_weight(unordered((uint32_t)(member >> 32)), rs, sh->tab) : 0, mass = running_sum(sh, w);
@@ -670,7 +671,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   if (few || (by_count && k <= LIST)) {       // or by counts alone, if the first k and what shares the last one's bin are
     for (int t = 0; t < TRIES && !found; ++t) {
       uint32_t members = live;
-      float end = __uint_as_float(0x7fc00000u);
+      float end = 0.f;
       if (!few) {
         rs.to_bin = (float)fmin(rs.s * (BINS / (double)reach_of(t)), 3e38);
         if (used) {
@@ -697,7 +698,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
         members = (uint32_t)before + mem.row_count[b];
         end = b + 1.f;
       }
-      list_cut(row, mem, vals, n, base, rs, end, members, by_count ? (uint32_t)k : (uint32_t)LIST, p, cut);
+      list_cut(row, mem, vals, n, base, rs, few, end, members, by_count ? (uint32_t)k : (uint32_t)LIST, p, cut);
       found = true;
     }
   }

@@ -47,3 +47,21 @@ def test_infinities_in_many_rows(K, vocab):      # noqa: F811
             got = draw(K, x[part], [t[r] for r in part], [u[r] for r in part], least=[least[r] for r in part])
             assert got[0] == [tokens[r] for r in part]
             assert all(a == b or (math.isnan(a) and math.isnan(b)) for a, b in zip(got[1], (logprobs[r] for r in part)))
+
+
+@pytest.mark.parametrize("infinities", [0, 1, 2, 3])
+@pytest.mark.parametrize("vocab", [700, 5000, 60001])
+def test_infinite_temperatures_under_top_k(K, vocab, infinities):      # noqa: F811
+    """Of finite logits each is as likely as the other, beside an infinite one none has a weight: what the first k's list holds is what was counted."""
+    rows = 24
+    x = logits_of(rows, vocab, 53, torch.float32)
+    at = torch.randperm(vocab, generator=torch.Generator().manual_seed(54))[:infinities]
+    x[:, at] = math.inf
+    x[::4, 1::5] = -math.inf
+    x[1::4, ::7] = math.nan
+    x[:, at] = math.inf
+    u = [(0.0, 0.3, 0.6, 0.95)[r // 6] for r in range(rows)]
+    ks = [(1, 2, 3, 50, 511, 512)[r % 6] for r in range(rows)]
+    for ps in (None, [(1.0, 0.9, 0.4, 0.0)[r % 4] for r in range(rows)]):
+        for t in (math.inf, 3e38, 1e30):
+            check(K, x, [t] * rows, u, ks, ps)
