@@ -91,9 +91,9 @@ struct RowScale {
   double m, s;      // the largest logit, log2(e) / T
   float top;        // the largest logit
   float to_bin;     // bins per unit of m - l
-  float to_log2;    // s
+  float to_log2;    // s, but at most 3e38 (temperatures below the smallest normal number have more): bins and floors by it are wider, no less right
   float low;        // a logit whose weight is far below a unit: what lies below it counts as it (a plain row's; see set)
-  bool plain;       // whether that is so: no infinity among the largest, and 500 factors of two are more than a rounding of m
+  bool plain;       // whether that is so: no infinity among the largest, 500 factors of two are more than a rounding of m, and to_log2 is all of s
   __device__ __forceinline__ void set(float largest, float temperature) {
     top = largest;
     m = (double)largest;
@@ -101,7 +101,7 @@ struct RowScale {
     to_log2 = (float)fmin(s, 3e38);
     to_bin = 0.f;
     low = largest - 500.f / to_log2;
-    plain = fabsf(largest) * to_log2 < 1e9f && 500.f / to_log2 < 3e38f;      // (false for NaN)
+    plain = fabsf(largest) * to_log2 < 1e9f && 500.f / to_log2 < 3e38f && s < 3e38;      // (false for NaN)
   }
 };
 // round(2^44 2^y), y = (l - m) s <= 0: 2^52 as a 64-bit number's bits, with the whole number in its last ones.  y = (n + f) / 256, n whole, |f| <= 1/2:
@@ -127,7 +127,7 @@ __device__ __forceinline__ u64 plain_raw(float l, const RowScale& rs, const Exp2
 }
 // The whole number of any row; `w`, if wanted: before rounding.  Weights below 2^-46 are 0.
 __device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp2Table& tab, double* w = nullptr) {
-  const bool none = !((rs.top - l) * rs.to_log2 < REACH), best = l == rs.top;      // (infinities too)
+  const bool none = !((rs.m - (double)l) * rs.s < (double)REACH), best = l == rs.top;      // (infinities too)
   double scale;
   const double p = weight_parts((double)l - rs.m, rs, tab, scale);
   if (w) *w = best ? UNIT : none ? 0.0 : p * scale;

@@ -65,3 +65,20 @@ def test_infinite_temperatures_under_top_k(K, vocab, infinities):      # noqa: F
     for ps in (None, [(1.0, 0.9, 0.4, 0.0)[r % 4] for r in range(rows)]):
         for t in (math.inf, 3e38, 1e30):
             check(K, x, [t] * rows, u, ks, ps)
+
+
+@pytest.mark.parametrize("rows", [6, 320])
+@pytest.mark.parametrize("vocab", [700, 5000, 60001])
+def test_the_smallest_temperatures(K, vocab, rows):      # noqa: F811
+    """Below the smallest normal number 1 / T passes what 32 bits hold; logits around zero, differences of ordinary size and of the smallest numbers' size."""
+    t = [(1e-45, 1e-43, 1e-41, 1e-40, 3e-39, 1e-38)[r % 6] for r in range(rows)]
+    g = torch.Generator().manual_seed(55)
+    u = torch.rand(rows, generator=g).tolist()
+    x = -torch.rand((rows, vocab), generator=g) - 1e-3
+    x[torch.arange(rows), torch.randint(0, vocab, (rows,), generator=g)] = 0.0
+    y = torch.rand((rows, vocab), generator=g) * torch.tensor(t)[:, None] * 40.0
+    y[::2, ::3] = -1.0
+    for logits in (x, y - 1e-38):
+        check(K, logits, t, u)
+        check(K, logits, t, u, least=[(0.0, 0.1, 1.0, 0.5)[r % 4] for r in range(rows)])
+        check(K, logits, t, u, k=[(50, 0, 600, 3)[r % 4] for r in range(rows)], p=[(0.9, 0.5, 1.0, 0.97, 0.0)[r % 5] for r in range(rows)])
