@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 #include <stdlib.h>
+#include "smem_limit.h"
 
 #define IFB_F32 0
 #define IFB_BF16 1
@@ -63,19 +64,18 @@ static inline bool ifb_pdl_enabled() {
   return on != 0;
 }
 
-// The largest dynamic shared memory a kernel may be launched with is an attribute of (kernel, device), so what has been
-// set is remembered per device, at the call site.  On failure the enclosing function returns the negated CUDA error.
-#define IFB_MAX_DEVICES 64
+// Room for a launch with so many bytes of dynamic shared memory (smem_limit.h), remembered at the call site.  On failure the enclosing function returns the
+// negated CUDA error.
 #define IFB_ALLOW_SMEM(kernel, bytes)                                                                                   \
   do {                                                                                                                  \
-    static size_t ifb_allowed_[IFB_MAX_DEVICES] = {};                                                                   \
+    static IfbSmemLimit ifb_limit_;                                                                                     \
     int ifb_dev_ = 0;                                                                                                   \
     if (cudaGetDevice(&ifb_dev_) != cudaSuccess || ifb_dev_ < 0 || ifb_dev_ >= IFB_MAX_DEVICES) return IFB_ERR_ARG;     \
-    if ((size_t)(bytes) > 48 * 1024 && (size_t)(bytes) > ifb_allowed_[ifb_dev_]) {                                      \
-      cudaError_t ifb_e_ = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes));     \
-      if (ifb_e_ != cudaSuccess) return -(int)ifb_e_;                                                                   \
-      ifb_allowed_[ifb_dev_] = (size_t)(bytes);                                                                         \
-    }                                                                                                                   \
+    const size_t ifb_bytes_ = (size_t)(bytes);                                                                          \
+    const int ifb_e_ = ifb_limit_.raise(ifb_dev_, ifb_bytes_, [&]() {                                                   \
+      return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ifb_bytes_);           \
+    });                                                                                                                 \
+    if (ifb_e_) return -ifb_e_;                                                                                         \
   } while (0)
 
 // SMs of the current device, which the rules that spread work go by (1 where it cannot be asked).

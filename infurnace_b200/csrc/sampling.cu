@@ -964,18 +964,19 @@ __global__ void __launch_bounds__(ST_NT, 4) sample_stream_kernel(const T* logits
   if (beside) ifb_pdl_wait();
 }
 
-// How many clusters of `ctas` CTAs with so much shared memory the device holds at a time (remembered by what they fit: two of them on an SM, or one); negative: an
+constexpr size_t MOST_CUT_SMEM = (size_t)SLICE * 4 + CUT_BYTES;
+// How many clusters of `ctas` CTAs with so much shared memory (MOST_CUT_SMEM is allowed) the device holds at a time (remembered by what they fit: two of them on an SM, or one); negative: an
 // error.
 static int cut_clusters(const void* kernel, int dtype, int ctas, size_t smem) {
-  static int known[IFB_MAX_DEVICES][2][2][MAX_CLUSTER + 1];
+  static std::atomic<int> known[IFB_MAX_DEVICES][2][2][MAX_CLUSTER + 1];      // (host threads ask at once; they find the same)
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= IFB_MAX_DEVICES) return 0;
   const bool pair = smem <= (size_t)SHARED_SLICE * 4 + CUT_BYTES;
-  int& n = known[dev][dtype][pair][ctas];
-  if (n) return n;
-  const size_t size = pair ? (size_t)SHARED_SLICE * 4 + CUT_BYTES : (size_t)SLICE * 4 + CUT_BYTES;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((size_t)SLICE * 4 + CUT_BYTES));
-  if (e == cudaSuccess && ctas > SURE_CLUSTER) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  std::atomic<int>& held = known[dev][dtype][pair][ctas];
+  if (const int n = held.load(std::memory_order_relaxed)) return n;
+  const size_t size = pair ? (size_t)SHARED_SLICE * 4 + CUT_BYTES : MOST_CUT_SMEM;
+  cudaError_t e = cudaSuccess;
+  if (ctas > SURE_CLUSTER) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
@@ -991,7 +992,8 @@ static int cut_clusters(const void* kernel, int dtype, int ctas, size_t smem) {
   int found = 0;
   e = cudaOccupancyMaxActiveClusters(&found, kernel, &cfg);
   if (e != cudaSuccess) { cudaGetLastError(); return -(int)e; }
-  return n = found;
+  held.store(found, std::memory_order_relaxed);
+  return found;
 }
 
 // logits [rows, vocab] with rows `pitch` elements apart (dtype IFB_F32 or IFB_BF16); per row: temperature, uniform number, and top_k, top_p, min_p (each or
@@ -1017,6 +1019,8 @@ IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
   // rows of 95,403 take 40 us in eight CTAs each and 57 in four, 203 of 97,476 154 and 109); more while all rows' clusters find their SMs at once.
   const void* kernel = dtype == IFB_F32 ? (const void*)sample_cut_kernel<float> : dtype == IFB_BF16 ? (const void*)sample_cut_kernel<bf16> : nullptr;
   if (!kernel) return IFB_ERR_DTYPE;
+  if (dtype == IFB_F32) IFB_ALLOW_SMEM(sample_cut_kernel<float>, MOST_CUT_SMEM);
+  else IFB_ALLOW_SMEM(sample_cut_kernel<bf16>, MOST_CUT_SMEM);
   auto slice = [&](int n) { return ((vocab + n - 1) / n + 7) & ~7; };
   const int width = dtype == IFB_F32 ? 4 : 2;
   auto room_for = [&](int n) { return cut_clusters(kernel, dtype, n, (size_t)slice(n) * width + CUT_BYTES); };
@@ -1058,14 +1062,8 @@ IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
   };
   if (cuts) {
     const size_t smem = (size_t)a.per * width + CUT_BYTES;
-    int st;
-    if (dtype == IFB_F32) {
-      IFB_ALLOW_SMEM(sample_cut_kernel<float>, smem);
-      st = go(sample_cut_kernel<float>, rows, ctas, NT, smem, (const float*)call->logits, a, everything ? 1 : 0);
-    } else {
-      IFB_ALLOW_SMEM(sample_cut_kernel<bf16>, smem);
-      st = go(sample_cut_kernel<bf16>, rows, ctas, NT, smem, (const bf16*)call->logits, a, everything ? 1 : 0);
-    }
+    const int st = dtype == IFB_F32 ? go(sample_cut_kernel<float>, rows, ctas, NT, smem, (const float*)call->logits, a, everything ? 1 : 0)
+                                    : go(sample_cut_kernel<bf16>, rows, ctas, NT, smem, (const bf16*)call->logits, a, everything ? 1 : 0);
     if (st || everything) return st;
   }
   // the other rows: as many CTAs of a row as leave no SM idle, each with whole blocks for its warps
