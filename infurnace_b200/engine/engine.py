@@ -59,7 +59,8 @@ class Engine:
                  tokenizer: Optional[Tokenizer] = None, eos_token_ids: Sequence[int] = (), max_prefill_portion=None):
         self.runner = runner
         self.scheduler = scheduler or Scheduler(runner.cache, runner.max_requests, runner.max_tokens,
-                                                runner.max_model_len, max_prefill_portion, cuts=getattr(runner, "draws_under_cuts", False))
+                                                runner.max_model_len, max_prefill_portion, cuts=getattr(runner, "draws_under_cuts", False),
+                                                scores=getattr(runner, "scores_tokens", False))
         self.tokenizer = tokenizer
         self.eos_token_ids = list(eos_token_ids)
         self._detoks: Dict[str, StreamingDetokenizer] = {}

@@ -41,8 +41,9 @@ class SamplingParams:
     above 0 a token is drawn from softmax(logits / temperature), cut by ``top_k`` (the k likeliest; 0: off, 1: greedy whatever
     the temperature), then by ``top_p`` (the likeliest that together have this share; 1.0: off) and by ``min_p`` (those that have
     this share of the likeliest's probability; 0.0: off).  ``top_k`` and ``top_p`` exist in the reference but nothing there
-    reads them.  Cuts other than ``top_k`` 1 need a kernel set that draws under them; without one they are refused at admission, and so
-    is ``logprobs`` (whether the request keeps its tokens' log probabilities under the model, whatever temperature and cuts)."""
+    reads them.  Cuts other than ``top_k`` 1 need a kernel set that draws under them for the model's vocabulary; without one they are refused
+    at admission.  So is ``logprobs`` (whether the request keeps its tokens' log probabilities under the model, whatever temperature and
+    cuts) without a kernel set that scores tokens."""
     temperature: float = 0.0
     top_k: int = 0
     top_p: float = 1.0
@@ -54,8 +55,9 @@ class SamplingParams:
     min_p: float = 0.0
     logprobs: bool = False
 
-    def problem(self, cuts: bool = False) -> Optional[str]:
-        """What is wrong with the options, or None.  ``cuts``: whether tokens can be drawn under cuts, and scored."""
+    def problem(self, cuts: bool = False, scores: Optional[bool] = None) -> Optional[str]:
+        """What is wrong with the options, or None.  ``cuts``: whether tokens can be drawn under cuts; ``scores``: whether they can be scored
+        (None: where cuts can)."""
         if not self.temperature >= 0.0:
             return f"temperature {self.temperature} is negative"
         if self.top_k not in (0, 1) and not (cuts and isinstance(self.top_k, int) and 0 <= self.top_k < 1 << 31):
@@ -64,7 +66,7 @@ class SamplingParams:
             return f"top_p {self.top_p} is not supported (1.0: off" + (", or a share)" if cuts else ")")
         if self.min_p != 0.0 and not (cuts and 0.0 <= self.min_p <= 1.0):
             return f"min_p {self.min_p} is not supported (0.0: off" + (", or a share)" if cuts else ")")
-        if self.logprobs and not cuts:
+        if self.logprobs and not (cuts if scores is None else scores):
             return "logprobs are not supported"
         if self.max_tokens < 0:
             return f"max_tokens {self.max_tokens} is negative"

@@ -27,6 +27,7 @@ Order inside a layer: the step's keys and values are stored before attention rea
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence
 
@@ -204,7 +205,10 @@ class ModelRunner:
         self._hist = [torch.zeros(max(r, 1), dtype=torch.int32, device=dev) for _ in range(2)]
         self._hist_host = [torch.zeros(max(r, 1), dtype=torch.int32, pin_memory=self._pin) for _ in range(2)]
         self._sampled_steps = 0
-        self.draws_under_cuts = hasattr(runtime.kernels, "sample_filtered")      # and scores tokens
+        self.scores_tokens = hasattr(runtime.kernels, "token_logprobs")
+        # (a kernel set may have a largest vocabulary for which it draws under cuts)
+        self.draws_under_cuts = hasattr(runtime.kernels, "sample_filtered") and \
+            getattr(getattr(model, "plan", None), "vocab_size", 0) <= getattr(runtime.kernels, "sample_max_vocab", math.inf)
         self._logprobs = None          # buffers of the tokens' log probabilities, made when they are first asked for
         # decode-only steps are replayed from CUDA graphs, one per (batch bucket, context bucket)
         self.use_graphs = self._pin and bool(getattr(model, "graph_safe", False))
@@ -325,8 +329,8 @@ class ModelRunner:
         if len(temperatures) != wanted or len(uniforms) != wanted:
             raise BatchError("one temperature and one uniform number per wanted row")
         if cuts is not None and (len(cuts) != wanted or not self.draws_under_cuts):
-            raise BatchError("cuts: one entry per wanted row, and a kernel set that draws under them")
-        if logprobs and not self.draws_under_cuts:
+            raise BatchError("cuts: one entry per wanted row, and a kernel set that draws under them for this vocabulary")
+        if logprobs and not self.scores_tokens:
             raise BatchError("logprobs: the kernel set does not score tokens")
         if cuts is not None and not any(c is not None and t > 0.0 for c, t in zip(cuts, temperatures)):
             cuts = None

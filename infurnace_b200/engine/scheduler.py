@@ -55,8 +55,8 @@ class StepPlan:
 
 class Scheduler:
     def __init__(self, cache, max_num_seqs: int, max_num_batched_tokens: int, max_model_len: int,
-                 max_prefill_portion: Optional[int] = None, cuts: bool = False):
-        """``cuts``: tokens can be drawn under top-k, top-p and min-p, and scored."""
+                 max_prefill_portion: Optional[int] = None, cuts: bool = False, scores: Optional[bool] = None):
+        """``cuts``: tokens can be drawn under top-k, top-p and min-p; ``scores``: their log probabilities can be kept (None: where cuts can)."""
         if max_num_seqs < 1:
             raise SchedulerError("max_num_seqs must be >= 1")
         if max_num_batched_tokens < 1:
@@ -70,7 +70,7 @@ class Scheduler:
         self.max_num_batched_tokens = max_num_batched_tokens
         self.max_model_len = max_model_len
         self.max_prefill_portion = max_prefill_portion
-        self.cuts = cuts
+        self.cuts, self.scores = cuts, cuts if scores is None else scores
         self._requests: Dict[str, Request] = {}
         self._waiting: Deque[str] = deque()
         self._running: List[str] = []          # in admission order
@@ -87,7 +87,7 @@ class Scheduler:
         self._requests[req.request_id] = req
         limit = self.max_model_len if req.context_limit is None else min(req.context_limit, self.max_model_len)
         n = len(req.prompt_token_ids)
-        problem = req.sampling_params.problem(self.cuts)
+        problem = req.sampling_params.problem(self.cuts, self.scores)
         if problem is None and n == 0:
             problem = "empty prompt"
         if problem is None and n > limit:

@@ -62,6 +62,7 @@ class AnswerKernels:
     """Mixed into the kernel set, which gives counters and the error word."""
 
     _sampling = None
+    sample_max_vocab = 8 * 46080      # the largest vocabulary that sample_filtered takes (csrc/sampling.cu: SURE_CLUSTER CTAs with SLICE logits each)
 
     def _sampling_lib(self):
         if self._sampling is None:

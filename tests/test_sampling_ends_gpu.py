@@ -82,3 +82,7 @@ def test_the_smallest_temperatures(K, vocab, rows):      # noqa: F811
         check(K, logits, t, u)
         check(K, logits, t, u, least=[(0.0, 0.1, 1.0, 0.5)[r % 4] for r in range(rows)])
         check(K, logits, t, u, k=[(50, 0, 600, 3)[r % 4] for r in range(rows)], p=[(0.9, 0.5, 1.0, 0.97, 0.0)[r % 5] for r in range(rows)])
+
+
+def test_the_largest_vocabulary_is_what_admission_goes_by(K):      # noqa: F811
+    assert K.sample_max_vocab == int(K._sampling_lib().ifb_sample_cut_max_vocab())
