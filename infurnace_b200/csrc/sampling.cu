@@ -108,10 +108,10 @@ struct RowScale {
 // 2^y = 2^(n / 256) e^x, x = f ln 2 / 256, by the first terms of its Taylor series (x^4 / 24 < 2e-13).  Eight operations in 64 bits and a conversion, without a
 // branch, so that a thread has several numbers under way (one after the other they take 250 cycles each, four together 115); NaN counts as `low`.
 constexpr u64 RAW = 0x4330000000000000ull;      // 2^52
-__device__ __forceinline__ double weight_parts(double d, const RowScale& rs, const Exp2Table& tab, double& scale) {
-  constexpr double MAGIC = 6755399441055744.0 / STEPS;      // 1.5 2^52 / 256: the sum's last bit is 1/256
+constexpr double MAGIC = 6755399441055744.0 / STEPS;      // 1.5 2^52 / 256: the sum's last bit is 1/256
+__device__ __forceinline__ double weight_parts(double d, const RowScale& rs, const Exp2Table& tab, double& scale, double& t) {      // (t: MAGIC + y)
   constexpr double LN2 = 0.693147180559945309417;
-  const double t = fma(d, rs.s, MAGIC);
+  t = fma(d, rs.s, MAGIC);
   const double r = fma(d, rs.s, -(t - MAGIC));
   const int n = __double2loint(t);
   const double step = tab.t[n & (STEPS - 1)];
@@ -121,15 +121,15 @@ __device__ __forceinline__ double weight_parts(double d, const RowScale& rs, con
   return fma(r, p, 1.0);
 }
 __device__ __forceinline__ u64 plain_raw(float l, const RowScale& rs, const Exp2Table& tab) {
-  double scale;
-  const double p = weight_parts((double)fmaxf(l, rs.low) - rs.m, rs, tab, scale);
+  double scale, t;
+  const double p = weight_parts((double)fmaxf(l, rs.low) - rs.m, rs, tab, scale, t);
   return (u64)__double_as_longlong(fma(p, scale, 4503599627370496.0));
 }
 // The whole number of any row; `w`, if wanted: before rounding.  Weights below 2^-46 are 0.
 __device__ __forceinline__ u64 row_weight(float l, const RowScale& rs, const Exp2Table& tab, double* w = nullptr) {
-  const bool none = !((rs.m - (double)l) * rs.s < (double)REACH), best = l == rs.top;      // (infinities too)
-  double scale;
-  const double p = weight_parts((double)l - rs.m, rs, tab, scale);
+  double scale, t;
+  const double p = weight_parts((double)l - rs.m, rs, tab, scale, t);
+  const bool none = !(t > MAGIC - REACH), best = l == rs.top;      // (infinities too)
   if (w) *w = best ? UNIT : none ? 0.0 : p * scale;
   const u64 whole = (u64)__double_as_longlong(fma(p, scale, 4503599627370496.0)) & ((1ull << 52) - 1);
   return best ? (u64)UNIT : none ? 0 : whole;
