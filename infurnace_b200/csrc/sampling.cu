@@ -1105,9 +1105,10 @@ __device__ __forceinline__ void lp_unpair(u64 v, float& a, float& b) { asm("mov.
 __device__ __forceinline__ u64 lp_add2(u64 a, u64 b) { u64 r; asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ u64 lp_mul2(u64 a, u64 b) { u64 r; asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ float lp_min(float a, float b) { float y; asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(y) : "f"(a), "f"(b)); return y; }
-// A thread's running state: its largest number, and the sum of e^(l - ref) over all others.  ref is an earlier largest one, left as it is until the
-// largest is 40 above it: a running maximum that grows is then no branch of its own, which with 32 threads to a warp it was in nearly every step.
-struct LpRun { float m, s, ref; };
+// A thread's running state: its largest number, and the sum of e^(l - m) over all others.  The sum is brought to a new largest number without asking whether it is
+// one: a branch would be taken by one of 32 threads in nearly every step, and a reference left behind would round what is added at its distance (left up to 40
+// behind, two near-equal tokens far above what their thread saw first came out 8e-7 off).
+struct LpRun { float m, s; };
 // N more numbers (a power of two).  They are paired off: of two the smaller goes into the sum, the larger on to the next round, so that the sum is over all
 // but one of the largest without a subtraction; NaN goes into the sum.  `count`: those at or above (AHEAD) or above `lt` are counted, which
 // takes a look at the largest first.
@@ -1128,12 +1129,10 @@ template <int N, bool AHEAD> __device__ __forceinline__ void lp_take(LpRun& t, c
     for (int j = 0; j < N; ++j) count += AHEAD ? v[j] >= lt : v[j] > lt;
   }
   out[N - 1] = lp_min(t.m, up[0]);
+  const float before = t.m;
   t.m = fmaxf(t.m, up[0]);
-  if (t.m > t.ref + 40.f) {      // (at first, too)
-    t.s *= lp_exp2((t.ref - t.m) * LOG2E);
-    t.ref = t.m;
-  }
-  const float ref = t.ref == -INFINITY ? 0.f : t.ref;
+  const float ref = t.m == -INFINITY ? 0.f : t.m;
+  t.s *= lp_exp2((before - ref) * LOG2E);      // (1 where it is the same)
   if (N > 1) {
     const u64 minus = lp_pair(-ref, -ref), log2e = lp_pair(LOG2E, LOG2E);
     u64 s[2] = {0, 0};
@@ -1170,7 +1169,7 @@ __global__ void __launch_bounds__(LP_NT) token_logprob_kernel(const T* logits, l
   const T* src = row + base;
   int t = max(0, min(n, token - base));      // numbers of this slice ahead of the token
   constexpr int N = Vec16<T>::N;
-  LpRun own = {-INFINITY, 0.f, -INFINITY};
+  LpRun own = {-INFINITY, 0.f};
   int count = 0;
   auto one = [&](int i) {
     const float v[1] = {to_f32<T>(src[i])};
@@ -1228,7 +1227,7 @@ __global__ void __launch_bounds__(LP_NT) token_logprob_kernel(const T* logits, l
   if (split < vecs && tid < N) one(split * N + tid);      // the vector that the token may be in
   run(split + 1, vecs, std::false_type());
   for (int i = vecs * N + tid; i < n; i += LP_NT) one(i);
-  LpSum sum = {own.m, own.m == -INFINITY ? own.s : own.s * lp_exp2((own.ref - own.m) * LOG2E)};
+  LpSum sum = {own.m, own.s};
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const LpSum x = {__shfl_xor_sync(0xffffffffu, sum.m, o), __shfl_xor_sync(0xffffffffu, sum.s, o)};
