@@ -27,11 +27,12 @@ static bool on_tc(int page_size, int owners, float scale, long long page_stride,
   return false;
 #endif
 }
+// The calls of wide owners' kernels, and of all owners' in groups of more than sixteen heads without tcgen05.
 static Call wide_call(bool tc, int n_tokens, int n_req, int n_groups, int kv_heads, int group, int page_size) {
 #if HEAD_DIM <= 128
   if (tc) return tc_call(n_tokens, n_req, n_groups, kv_heads, group, page_size);
 #endif
-  return sh_call(n_tokens, n_req, n_groups, kv_heads, group, D, WIDE);
+  return sh_call(n_tokens, n_req, n_groups, kv_heads, group, 1);
 }
 
 // Bytes of room for a call's sums at most, whichever kernels it takes.
@@ -59,21 +60,23 @@ IFB_EXPORT int ifb_attention_shared_bf16(const Packed* call) {
   room_at(wide, D, rest);
   room_at(few, D, rest + room_bytes(wide, D));
   const bool any_narrow = group <= NARROW_ROWS;
-  if (any_narrow && !tc) {
-    few.which = EVERY;
-    const int st = narrow::run(by_tma, few, few, q, a.q_row, pages, false, a.stream);
-    return st ? st : join<__nv_bfloat16>(few, few, D, a.stream);
+  int st = IFB_OK;
+  if (!tc) {      // one kernel for all owners
+    if (any_narrow) {
+      few.which = EVERY;
+      st = narrow::run(by_tma, few, few, q, a.q_row, pages, false, a.stream);
+      return st ? st : join<__nv_bfloat16>(few, few, D, a.stream);
+    }
+    st = sh_main<__nv_bfloat16, (D + 31) / 32>(wide, q, a.q_row, pages, D, a.stream);
+    return st ? st : join<__nv_bfloat16>(wide, wide, D, a.stream);
   }
   const bool any_wide = (long long)a.n_tokens * group > NARROW_ROWS;      // no owner has more rows than all
-  int st = IFB_OK;
-  if (any_wide) {
 #if HEAD_DIM <= 128
-    if (tc) st = tc_main(wide, few, q, a.q_row, pages, !any_narrow, a.stream);
-    else
-#endif
-      st = sh_main<__nv_bfloat16, (D + 31) / 32>(wide, few, q, a.q_row, pages, D, !any_narrow, a.stream);
+  if (any_wide) {
+    st = tc_main(wide, few, q, a.q_row, pages, !any_narrow, a.stream);
     if (st) return st;
   }
+#endif
   if (any_narrow) {
     st = narrow::run(by_tma, few, wide, q, a.q_row, pages, any_wide, a.stream);
     if (st) return st;

@@ -39,9 +39,9 @@ __device__ __forceinline__ void sh_store4(__nv_bfloat16* dst, float4 v) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// parts: whether this kernel writes where the rows' pieces are.  NJ: 32 columns each, as many as the head has.
+// NJ: 32 columns each, as many as the head has.
 template <typename T, int NJ>
-__global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_constant__ Call c, const __grid_constant__ Call other, const T* q, long long q_row, const T* pages, int dim, int parts) {
+__global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_constant__ Call c, const T* q, long long q_row, const T* pages, int dim) {
   constexpr int STAGES = sh_stages(NJ);
   extern __shared__ __align__(16) unsigned char sh_smem[];
   __shared__ long long places[2][SH_UNIT];      // of the keys of two units: the first element in the pool, or -1
@@ -52,11 +52,10 @@ __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_co
   float* P = KV + STAGES * 2 * SH_UNIT * pitch;                                         // [64][33]
   ifb_pdl_wait();
   ifb_pdl_trigger();
-  make_plan(c, other, plan);
+  make_plan(c, c, plan);
   Walk walk;
-  const int ctas = c.which == EVERY ? c.workers : wide_sms(c.workers, plan.starts[c.n_groups + c.n_req] * c.cost, plan.sums[63] * other.cost);
-  walk.begin(c, plan, blockIdx.x, ctas);
-  if (parts) write_parts(c, other, plan);
+  walk.begin(c, plan, blockIdx.x, c.workers);
+  write_parts(c, c, plan);
   const int tid = threadIdx.x, x = tid & 7, y = tid >> 3, quads = dim / 4;
   const int group = c.heads / c.kv_heads;
   const long long values = (long long)c.kv_heads * c.page_size * dim;      // from a page's keys to its values
@@ -219,22 +218,21 @@ __global__ void __launch_bounds__(SH_THREADS) shared_simt_kernel(const __grid_co
   }
 }
 
-static inline Call sh_call(int n_tokens, int n_req, int n_groups, int kv_heads, int group, int dim, Class which) {
+static inline Call sh_call(int n_tokens, int n_req, int n_groups, int kv_heads, int group, int ctas) {      // (ctas: of an SM)
   Call c = {};
-  c.which = which;
+  c.which = EVERY;
   c.n_tokens = n_tokens; c.n_req = n_req; c.n_groups = n_groups;
   c.kv_heads = kv_heads; c.heads = kv_heads * group;
   c.tokens = SH_ROWS / group; c.rows = SH_ROWS; c.unit_log = 5; c.align_log = 0;
-  c.workers = ifb_sm_count() * (which == EVERY && dim <= 128 ? 2 : 1);      // (registers: two CTAs on an SM; beside narrow owners one)
-  c.cost = 16;
+  c.workers = ifb_sm_count() * ctas;
   c.extra = 1;
   return c;
 }
 // (one function for each kernel: what IFB_ALLOW_SMEM remembers is a kernel's)
 template <typename T, int NJ>
-static int sh_main(const Call& c, const Call& other, const T* q, long long q_row, const T* pages, int dim, bool parts, cudaStream_t stream) {
+static int sh_main(const Call& c, const T* q, long long q_row, const T* pages, int dim, cudaStream_t stream) {
   const size_t smem = plan_bytes(c.n_req + c.n_groups) + (size_t)((SH_ROWS + sh_stages(NJ) * 2 * SH_UNIT) * (dim + 4) + SH_ROWS * 33) * 4;
   if (smem > MOST_SMEM) return IFB_ERR_SIZE;
   IFB_ALLOW_SMEM((shared_simt_kernel<T, NJ>), smem);
-  return ifb_launch(shared_simt_kernel<T, NJ>, dim3(c.workers), dim3(SH_THREADS), smem, stream, c, other, q, q_row, pages, dim, parts ? 1 : 0);
+  return ifb_launch(shared_simt_kernel<T, NJ>, dim3(c.workers), dim3(SH_THREADS), smem, stream, c, q, q_row, pages, dim);
 }
