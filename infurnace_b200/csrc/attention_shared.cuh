@@ -63,7 +63,10 @@ struct Call {
 };
 
 __host__ __device__ inline int prefix_items(const Call& c) { return (c.n_tokens / c.tokens + c.n_groups + 1) * c.kv_heads; }
-__host__ __device__ inline int all_items(const Call& c) { return prefix_items(c) + (c.n_tokens / c.tokens + c.n_req + 1) * c.kv_heads; }
+// (a narrow owner beside wide ones is one tile, and the items of its class are numbered by owners)
+__host__ __device__ inline int all_items(const Call& c) {
+  return c.which == NARROW ? (c.n_groups + c.n_req) * c.kv_heads : prefix_items(c) + (c.n_tokens / c.tokens + c.n_req + 1) * c.kv_heads;
+}
 __host__ inline long long room_align(long long x) { return (x + 255) & ~255LL; }
 // The room of one class's kernel, in three parts.
 __host__ inline long long room_bytes(const Call& c, int dim) {
@@ -111,6 +114,7 @@ __device__ __forceinline__ Span tile_span(const Call& c, const Owner& w, int til
 __device__ __forceinline__ int span_cost(const Call& c, const Span& s) { return s.units ? s.units + c.extra : 0; }
 __device__ __forceinline__ int owner_tiles(const Call& c, const Owner& w) { return (w.row1 - w.row0 + c.tokens - 1) / c.tokens; }
 __device__ __forceinline__ int owner_item(const Call& c, const Owner& w, int o) {
+  if (c.which == NARROW) return o * c.kv_heads;
   return w.group ? (w.row0 / c.tokens + o) * c.kv_heads : prefix_items(c) + (w.row0 / c.tokens + o - c.n_groups) * c.kv_heads;
 }
 __device__ __forceinline__ bool is_narrow(const Call& c, const Owner& w) { return (w.row1 - w.row0) * (c.heads / c.kv_heads) <= NARROW_ROWS; }

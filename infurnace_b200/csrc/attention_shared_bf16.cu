@@ -27,19 +27,19 @@ static bool on_tc(int page_size, int owners, float scale, long long page_stride,
   return false;
 #endif
 }
-// The calls of wide owners' kernels, and of all owners' in groups of more than sixteen heads without tcgen05.
-static Call wide_call(bool tc, int n_tokens, int n_req, int n_groups, int kv_heads, int group, int page_size) {
-#if HEAD_DIM <= 128
-  if (tc) return tc_call(n_tokens, n_req, n_groups, kv_heads, group, page_size);
-#endif
-  return sh_call(n_tokens, n_req, n_groups, kv_heads, group, 1);
-}
-
 // Bytes of room for a call's sums at most, whichever kernels it takes.
 IFB_EXPORT long long ifb_attention_shared_bf16_room(int n_tokens, int n_req, int n_groups, int kv_heads, int group) {
-  const long long a = room_bytes(wide_call(true, n_tokens, n_req, n_groups, kv_heads, group, 16), D);
-  const long long b = room_bytes(wide_call(false, n_tokens, n_req, n_groups, kv_heads, group, 16), D);
-  return parts_bytes(n_tokens) + (a > b ? a : b) + room_bytes(narrow::call(true, n_tokens, n_req, n_groups, kv_heads, group), D);      // (either has as many workers)
+  const bool any_narrow = group <= NARROW_ROWS;
+  // one kernel for all owners (by TMA or not: with it the narrow one has as many workers or more)
+  long long most = any_narrow ? room_bytes(narrow::call(true, EVERY, n_tokens, n_req, n_groups, kv_heads, group), D)
+                              : room_bytes(sh_call(n_tokens, n_req, n_groups, kv_heads, group, 1), D);
+#if HEAD_DIM <= 128
+  // tcgen05, and narrow owners beside it
+  long long both = room_bytes(tc_call(n_tokens, n_req, n_groups, kv_heads, group, 16), D);
+  if (any_narrow) both += room_bytes(narrow::call(true, NARROW, n_tokens, n_req, n_groups, kv_heads, group), D);
+  if (both > most) most = both;
+#endif
+  return parts_bytes(n_tokens) + most;
 }
 
 // As ifb_attention_shared.
@@ -52,34 +52,35 @@ IFB_EXPORT int ifb_attention_shared_bf16(const Packed* call) {
   const int group = a.heads / a.kv_heads;
   const bool tc = on_tc(a.page_size, a.n_req + a.n_groups, (float)a.scale, a.page_stride, a.num_pages);
   const bool by_tma = narrow::by_tma(a.page_size, a.page_stride, a.num_pages);
-  Call wide = wide_call(tc, a.n_tokens, a.n_req, a.n_groups, a.kv_heads, group, a.page_size);
-  Call few = narrow::call(by_tma, a.n_tokens, a.n_req, a.n_groups, a.kv_heads, group);
-  fill(wide, a);
-  fill(few, a);
-  char* rest = (char*)a.room + parts_bytes(a.n_tokens);
-  room_at(wide, D, rest);
-  room_at(few, D, rest + room_bytes(wide, D));
   const bool any_narrow = group <= NARROW_ROWS;
+  char* rest = (char*)a.room + parts_bytes(a.n_tokens);
   int st = IFB_OK;
   if (!tc) {      // one kernel for all owners
-    if (any_narrow) {
-      few.which = EVERY;
-      st = narrow::run(by_tma, few, few, q, a.q_row, pages, false, a.stream);
-      return st ? st : join<__nv_bfloat16>(few, few, D, a.stream);
-    }
-    st = sh_main<__nv_bfloat16, (D + 31) / 32>(wide, q, a.q_row, pages, D, a.stream);
-    return st ? st : join<__nv_bfloat16>(wide, wide, D, a.stream);
+    Call every = any_narrow ? narrow::call(by_tma, EVERY, a.n_tokens, a.n_req, a.n_groups, a.kv_heads, group)
+                            : sh_call(a.n_tokens, a.n_req, a.n_groups, a.kv_heads, group, 1);
+    fill(every, a);
+    room_at(every, D, rest);
+    st = any_narrow ? narrow::run(by_tma, every, every, q, a.q_row, pages, false, a.stream)
+                    : sh_main<__nv_bfloat16, (D + 31) / 32>(every, q, a.q_row, pages, D, a.stream);
+    return st ? st : join<__nv_bfloat16>(every, every, D, a.stream);
   }
-  const bool any_wide = (long long)a.n_tokens * group > NARROW_ROWS;      // no owner has more rows than all
 #if HEAD_DIM <= 128
+  Call wide = tc_call(a.n_tokens, a.n_req, a.n_groups, a.kv_heads, group, a.page_size);
+  Call few = narrow::call(by_tma, NARROW, a.n_tokens, a.n_req, a.n_groups, a.kv_heads, group);
+  fill(wide, a);
+  fill(few, a);
+  room_at(wide, D, rest);
+  room_at(few, D, rest + room_bytes(wide, D));
+  const bool any_wide = (long long)a.n_tokens * group > NARROW_ROWS;      // no owner has more rows than all
   if (any_wide) {
     st = tc_main(wide, few, q, a.q_row, pages, !any_narrow, a.stream);
     if (st) return st;
   }
-#endif
-  if (any_narrow) {
+  if (any_narrow) {      // (in groups of more heads no owner with rows is)
     st = narrow::run(by_tma, few, wide, q, a.q_row, pages, any_wide, a.stream);
     if (st) return st;
   }
-  return join<__nv_bfloat16>(wide, few, D, a.stream);
+  st = join<__nv_bfloat16>(wide, few, D, a.stream);
+#endif
+  return st;
 }

@@ -376,9 +376,9 @@ shared_narrow_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
 static inline bool by_tma(int page_size, long long page_stride, long long num_pages) {
   return TMA_HEADS && page_size % CHUNK == 0 && page_stride % D == 0 && num_pages * (page_stride / D) < 0x7fffffffLL;
 }
-static inline Call call(bool tma, int n_tokens, int n_req, int n_groups, int kv_heads, int group) {
+static inline Call call(bool tma, Class which, int n_tokens, int n_req, int n_groups, int kv_heads, int group) {
   Call c = {};
-  c.which = NARROW;
+  c.which = which;
   c.n_tokens = n_tokens; c.n_req = n_req; c.n_groups = n_groups;
   c.kv_heads = kv_heads; c.heads = kv_heads * group;
   c.tokens = group <= NARROW_ROWS ? NARROW_ROWS / group : 1; c.rows = NARROW_ROWS; c.unit_log = 5; c.align_log = tma ? 4 : 0;
