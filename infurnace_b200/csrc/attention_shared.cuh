@@ -597,7 +597,7 @@ static inline int check(const Packed& a, int most_group, int least) {
   if (a.kv_heads < 1 || a.heads % a.kv_heads || a.heads / a.kv_heads > most_group || a.dim < 16 || a.dim > 256 || a.dim % 16 || a.n_groups < 0 ||
       a.n_req + a.n_groups > MAX_OWNERS || a.page_size < 1 || a.num_pages < 1)
     return IFB_ERR_SIZE;
-  if ((((uintptr_t)a.q | (uintptr_t)a.pages) & 15) || a.q_row % least || a.page_stride % least || ((uintptr_t)a.room & 255)) return IFB_ERR_ALIGN;
+  if ((((uintptr_t)a.q | (uintptr_t)a.pages | (uintptr_t)a.out) & 15) || a.q_row % least || a.page_stride % least || ((uintptr_t)a.room & 255)) return IFB_ERR_ALIGN;
   if (a.window < 0 || !a.err || !a.room || a.page_stride < 2LL * a.kv_heads * a.page_size * a.dim) return IFB_ERR_ARG;
   return IFB_OK;
 }

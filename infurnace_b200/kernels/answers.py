@@ -165,7 +165,8 @@ class AnswerKernels:
         """``paged_attention`` for requests whose block tables share leading pages, which are then read once for all of them: answers to one
         prompt, questions to one document, conversations behind one system prompt.
 
-        ``q`` and ``out`` are bfloat16 or float32 [tokens, heads, head_dim] (the rows of ``q`` may lie apart, those of ``out`` not, and share no memory), ``kv_pages`` [pages, 2,
+        ``q`` and ``out`` are bfloat16 or float32 [tokens, heads, head_dim] (the rows of ``q`` may lie apart, those of ``out`` not, and share no memory; both begin on 16
+        bytes), ``kv_pages`` [pages, 2,
         kv_heads, page_size, head_dim] of the same type.  Request r has the rows cu_q[r] .. cu_q[r + 1] - 1 and ``seq_lens[r]`` keys, these
         queries' own among them, in the pages of ``block_tables[r]``; the query at position p sees positions max(0, p - window + 1) .. p
         (``window`` 0: from 0).  Group g is the requests cu_groups[g] .. cu_groups[g + 1] - 1, the first ``shared_lens[g]`` keys of which are the same: they are
@@ -208,8 +209,8 @@ class AnswerKernels:
             raise KernelError("shared_prefix_attention: all tensors are on one CUDA device")
         q_row = pitch[0] if n > 1 else heads * dim
         lines = 4 if dtype is torch.float32 else 8          # elements of 16 bytes
-        if q.data_ptr() % 16 or kv_pages.data_ptr() % 16 or q_row % lines or page_stride % lines:
-            raise KernelError("shared_prefix_attention: q's rows and the pages begin on 16 bytes")
+        if q.data_ptr() % 16 or kv_pages.data_ptr() % 16 or out.data_ptr() % 16 or q_row % lines or page_stride % lines:
+            raise KernelError("shared_prefix_attention: q's rows, the pages and out begin on 16 bytes")
         if window < 0 or max_q_len < 1 or max_seq_len < 0:
             raise KernelError("shared_prefix_attention: window and max_seq_len are not negative, max_q_len is positive")
         if table[1] * page_size < max_seq_len:
