@@ -1,7 +1,7 @@
 // Attention over shared pages in bfloat16, compiled for one head size: -DHEAD_DIM=<multiple of 16, at most 256> (default 128).  Narrow owners by
 // attention_shared_narrow.cuh, wide ones beside them by attention_shared_tc.cuh where heads and pages allow.  Where they do not, all owners by
 // attention_shared_narrow.cuh, in tiles of sixteen rows; groups of more than 16 heads, of which a tile would not hold one token, by
-// attention_shared_simt.cuh, which is several times slower (11 requests of 173 queries and some 300 keys, 40 heads of 256: 2,613 us, and 450 in tiles of sixteen).
+// attention_shared_simt.cuh, which is several times slower (11 requests of 173 queries and 189 to 316 keys, 40 on 8 heads of 256: 2,027 us, and 390 in tiles of sixteen).
 #include <cuda.h>
 
 #ifndef HEAD_DIM

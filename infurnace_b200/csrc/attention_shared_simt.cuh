@@ -7,8 +7,8 @@
 // 4 x + 32 j .. + 3.  Rows of keys are padded by four numbers, so that eight lanes that read eight keys 16 bytes at a time meet no bank twice.
 //
 // What bounds it is a chain of units of 2 to 3 us each (a warp's 2,000 multiply-adds and what they read from shared memory, two warps to a scheduler), behind 4 us of
-// plan and first keys; before copies ran ahead and columns came four at a time a unit took 15 to 20 us (nine answers to 1,296 keys 32.9 us, now 19.7; 32
-// requests' tokens at heads of 96 63 to 24; four portions of 121 queries at heads of 256 222 to 91).
+// plan and first keys; before copies ran ahead and columns came four at a time a unit took 15 to 20 us (nine answers to 1,296 keys 32.3 us, now 19.4; 32
+// requests' tokens to 320 shared keys and up to 200 of their own, 12 on 4 heads of 96, 72 to 29; four portions of 121 queries, 8 on 2 heads of 256, 118 to 52).
 #pragma once
 #include "attention_shared.cuh"
 #include <type_traits>

@@ -2,9 +2,8 @@
 // pages of 16, 32 or 64.  attention_shared.cuh says how the work is cut and joined.
 //
 // A tile is 128 score rows (query tokens times the heads of a key head's group: row = token * G + head-in-group), a unit 128 keys.  Decoded tokens
-// of all requests of a group fill a tile together over the keys that they share; over its own keys a request has a tile to itself, most rows of
-// which are empty.  That costs little: what a tile takes from memory is its keys and values, 64 KB a unit, which an SM gets in about 1.5 us when all ask,
-// and the chain of a unit's softmax is shorter than that.
+// of all requests of a group fill tiles together over the keys that they share; over its own keys a request of more than sixteen score rows has tiles to itself
+// (those of fewer are narrow, and are worked on by warps beside this kernel).
 //
 // As in attention_tc.cu a CTA is a pipeline: warp 0 brings queries and keys by TMA, warp 3 values, warps 1 and 2 issue the products of two streams (stream x
 // takes half x of every 128 keys), warps 4-7 and 8-11 do their softmax, a thread a row; scores, weights (over the scores' columns) and the sums stay in
@@ -458,7 +457,9 @@ static inline Call tc_call(int n_tokens, int n_req, int n_groups, int kv_heads, 
   c.kv_heads = kv_heads; c.heads = kv_heads * group;
   c.tokens = ROWS / group; c.rows = ROWS; c.unit_log = 7; c.align_log = page_size == 16 ? 4 : page_size == 32 ? 5 : 6;
   c.workers = ifb_sm_count();
-  c.cost = 6;      // (64 answers to 8,000 keys 42.0 us with 7, 41.2 with 6, 43.1 with 5)
+  // (with 5, 6 and 7: 64 answers to 8,000 keys 43.0, 41.8 and 41.9 us, 32 to 2,000 25.8, 25.5 and 25.3, groups of conversations 82.7, 81.2 and 81.4, others with heads of
+  // 64 28.0, 27.5 and 29.2, with heads of 96 in pages of 64 23.8, 22.9 and 23.1, with eight heads to a key head 30.1, 28.4 and 28.4)
+  c.cost = 6;
   c.extra = 2;
   return c;
 }

@@ -18,9 +18,12 @@
 // for itself.  Where too many are left (ties), a search over the ordered bits of their values finds the last value that is kept, and a count in index order the
 // last of its tokens.
 //
-// What bounds it, by clock stamps in the kernel (one row of 151,936 under top-p, 16 CTAs, 17 us): reading the row 1 us, its maximum 1.4, weights and bins 3, their
-// merging 2.9, the bin and its list 3.5, the weights of what is kept 1, the draw's prefix sums 1.6; each step that tells the cluster something takes about 1.4 us, and
-// there are six.  Many rows are bound by the instructions of the bins and of the weights, and by how many clusters fit on the device (two CTAs to an SM).
+// What bounds it, by clock stamps in the kernel (one row of 151,936 under top-p, 16 CTAs, 17.2 us): its parameters 0.9 us, reading it 0.8, its maximum 1.2, weights
+// and bins 3.2, their merging 2.9 and sum 0.4, the bin and its list in order 4.2, the weights of what is kept 1.3, prefix sums and draw 2.3.  The cluster meets six
+// times: when all have begun, for the maximum, before and after the merging, for the list, for the prefix sums; twice more where the bin is divided, and for every further
+// reach.  Rows with many tokens near the cut take 22 us (the divided bin, and weights of more tokens), rows whose cut the second reach holds 28.  Many rows are
+// bound by the instructions of the bins and of the weights, and by how many clusters fit on the device (two CTAs to an SM): of 64 rows of all kinds
+// those with cuts take 18 to 56 us each, 28 in the mean, the longest ones under top-p in the second reach.
 #include "common.cuh"
 #include <math.h>
 #include <type_traits>
@@ -312,7 +315,8 @@ __device__ __forceinline__ int find_bin(CutShared* sh, int n, const uint32_t* co
 struct Cut { float l; int i; u64 mass; };
 __device__ __forceinline__ bool kept(float l, int i, const Cut& c) { return l > c.l || (l == c.l && i <= c.i); }
 
-// A CTA's slice of a row, in shared memory in the type that it comes in (of 16 bits twice the rows find room: 203 rows of 97,476 under top-p 154 to 109 us).
+// A CTA's slice of a row, in shared memory in the type that it comes in (of 16 bits twice the rows find room: 203 rows of 97,476 under top-p 184 to 145 us, 91 of
+// 84,412 95 to 86).
 template <typename T> struct Slice {
   T* at;
   __device__ __forceinline__ float operator[](int i) const { return to_f32<T>(at[i]); }
@@ -666,7 +670,7 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
   // ---- what top-k and top-p keep
   Cut cut = {-INFINITY, 0x7fffffff, 0};
   bool found = !cuts, used = false;
-  // Tokens of a small vocabulary, or that a grammar leaves: a list's worth (104 rows of 316 18 to 8.6 us, 176 of 2,971 of which 97 in 100 are forbidden 22 to 12).
+  // Tokens of a small vocabulary, or that a grammar leaves: a list's worth (104 rows of 316 21.6 to 7.9 us, 176 of 2,971 of which 97 in 100 are forbidden 29.6 to 11.5).
   const bool few = cuts && live <= LIST;
   if (few || (by_count && k <= LIST)) {       // or by counts alone, if the first k and what shares the last one's bin are
     for (int t = 0; t < TRIES && !found; ++t) {
@@ -819,8 +823,8 @@ __global__ void __launch_bounds__(NT, 2) sample_cut_kernel(const T* logits, CutA
 // ---------------------------------------------------------------------------------------------------- rows without top-k and top-p
 // Greedy rows, and such as are drawn from all tokens or from those that min_p leaves: nothing has to be looked for, so nothing is kept; a row is read for its
 // largest logit, and a second time, from L2, for its weights.  A CTA needs no shared memory to speak of and four are on an SM, which matters where there are
-// many rows: 256 rows of 151,936 held in shared memory, two CTAs on an SM, took 135 us, so they take 85 (a read takes 24: what bounds
-// it is the twenty instructions of a weight).  A warp has a stretch of the row, which it
+// many rows: 256 rows of 151,936 held in shared memory, two CTAs on an SM, took 135 us, so they take 85 (a read takes 24; a weight's twenty instructions fill half
+// of the issue slots, and warps wait for the second pass's loads longer than for anything else).  A warp has a stretch of the row, which it
 // takes in blocks of 512; a block's sum is kept, so that the draw goes over 512 tokens anew and no more.
 constexpr int ST_NT = 256, ST_NW = ST_NT / 32, ST_BLOCK = 512, ST_BLOCKS = 16;      // (a CTA has 65,536 logits at most)
 
@@ -1015,8 +1019,8 @@ IFB_EXPORT int ifb_sample_cut(const CutPacked* call) {
   if (rows <= 0) return IFB_OK;
   if (vocab < 1 || vocab > SURE_CLUSTER * SLICE || rows > (1 << 27)) return IFB_ERR_SIZE;
   if (!call->temperature || !call->uniform || !call->out) return IFB_ERR_ARG;
-  // As few CTAs of a row as let two share an SM (of 16-bit numbers counted as 32-bit ones, but for half as many where there are rows for several rounds: 36
-  // rows of 95,403 take 40 us in eight CTAs each and 57 in four, 203 of 97,476 154 and 109); more while all rows' clusters find their SMs at once.
+  // As few CTAs of a row as let two share an SM (of 16-bit numbers counted as 32-bit ones, but for half as many where there are rows for several rounds: 203
+  // rows of 97,476 under top-p take 191 us in eight CTAs each and 150 in four, 91 of 84,412 101 and 87); more while all rows' clusters find their SMs at once.
   const void* kernel = dtype == IFB_F32 ? (const void*)sample_cut_kernel<float> : dtype == IFB_BF16 ? (const void*)sample_cut_kernel<bf16> : nullptr;
   if (!kernel) return IFB_ERR_DTYPE;
   if (dtype == IFB_F32) IFB_ALLOW_SMEM(sample_cut_kernel<float>, MOST_CUT_SMEM);
